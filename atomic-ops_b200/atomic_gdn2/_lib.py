@@ -22,7 +22,7 @@ PREC = ENUM
 # gdn2_dtype
 F32, BF16 = 0, 1
 # device status bits
-DEV_TIMEOUT, DEV_SPAN, DEV_POSITIVE_GATE = 1, 2, 4
+DEV_TIMEOUT, DEV_SPAN, DEV_POSITIVE_GATE, DEV_BAD_INDEX = 1, 2, 4, 8
 
 
 class Gdn2Desc(ctypes.Structure):
@@ -37,11 +37,39 @@ class Gdn2Desc(ctypes.Structure):
     ]
 
 
+class RecDesc(ctypes.Structure):
+    """struct gdn2_rec_desc."""
+    _fields_ = [
+        ("B", ctypes.c_int32), ("H", ctypes.c_int32), ("L", ctypes.c_int32), ("D", ctypes.c_int32),
+        ("stride", (ctypes.c_int64 * 3) * 6), ("o_stride", ctypes.c_int64 * 3),
+        ("n_states", ctypes.c_int32), ("in_dtype", ctypes.c_int32),
+        ("scale", ctypes.c_float), ("clip", ctypes.c_float),
+    ]
+
+
+class W4Desc(ctypes.Structure):
+    """struct gdn2_w4_desc."""
+    _fields_ = [
+        ("M", ctypes.c_int32), ("K", ctypes.c_int32), ("N", ctypes.c_int32), ("group", ctypes.c_int32),
+        ("dtype", ctypes.c_int32), ("act", ctypes.c_int32),
+        ("x_stride", ctypes.c_int64), ("res_stride", ctypes.c_int64), ("y_stride", ctypes.c_int64),
+    ]
+
+
+class BeamDesc(ctypes.Structure):
+    """struct gdn2_beam_desc."""
+    _fields_ = [
+        ("B", ctypes.c_int32), ("K", ctypes.c_int32), ("V", ctypes.c_int32), ("dtype", ctypes.c_int32),
+        ("stride_b", ctypes.c_int64), ("stride_k", ctypes.c_int64), ("eos", ctypes.c_int32),
+    ]
+
+
 EXPORTS = ("gdn2_residual_bytes", "gdn2_fwd_workspace_bytes", "gdn2_bwd_workspace_bytes", "gdn2_fwd", "gdn2_bwd",
            "gdn2_set_batch_groups", "gdn2_get_batch_groups",
            "gdn2_status_string", "gdn2_selftest_gemm", "gdn2_profile_enable", "gdn2_profile_collect",
            "gdn2_fwd_noalloc", "gdn2_prologue_fwd", "gdn2_prologue_bwd", "gdn2_selftest_engine",
-           "gdn2_selftest_wait_timeout")
+           "gdn2_selftest_wait_timeout", "gdn2_recurrent", "gdn2_w4_linear", "gdn2_beam_select",
+           "gdn2_beam_workspace_bytes")
 # kernel ids of gdn2_profile_collect
 KERNELS = ("fwd_intra", "fwd_scan", "fwd_out", "bwd_pre", "bwd_scan", "bwd_intra")
 
@@ -81,6 +109,14 @@ def _declare(lib):
     lib.gdn2_prologue_fwd.argtypes = [P, I64, I64, I64, I64, ctypes.c_float, ctypes.c_int32] + [P] * 7
     lib.gdn2_prologue_bwd.restype = ctypes.c_int
     lib.gdn2_prologue_bwd.argtypes = [P, I64, I64, I64, I64, ctypes.c_float, ctypes.c_int32] + [P] * 8
+    lib.gdn2_recurrent.restype = ctypes.c_int
+    lib.gdn2_recurrent.argtypes = [P] * 14      # descriptors of the serving operators are passed by address
+    lib.gdn2_w4_linear.restype = ctypes.c_int
+    lib.gdn2_w4_linear.argtypes = [P] * 8
+    lib.gdn2_beam_workspace_bytes.restype = ctypes.c_size_t
+    lib.gdn2_beam_workspace_bytes.argtypes = [P]
+    lib.gdn2_beam_select.restype = ctypes.c_int
+    lib.gdn2_beam_select.argtypes = [P] * 10
     return lib
 
 

@@ -35,6 +35,7 @@ include/gdn2_b200.h.  PyTorch only provides device memory, streams and autograd 
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -97,12 +98,49 @@ def _dev_status(dev: torch.device) -> _DevStatus:
     return st
 
 
+class _HostFlags:
+    """Two words of one device's status in mapped host memory (gdn2_recurrent): kernels set them,
+    the host reads them without a copy."""
+
+    BITS = (_lib.DEV_POSITIVE_GATE, _lib.DEV_BAD_INDEX)
+
+    def __init__(self, dev: torch.device):
+        self.index = dev.index
+        self.tensor = torch.zeros(2, dtype=torch.int32, pin_memory=True)
+        self.ptr = self.tensor.data_ptr()
+        self.words = (ctypes.c_uint32 * 2).from_address(self.ptr)
+
+    def code(self) -> int:
+        return sum(bit for bit, word in zip(self.BITS, self.words) if word)
+
+    def take(self) -> int:
+        code = self.code()
+        self.words[0] = self.words[1] = 0
+        return code
+
+
+_flags = {}
+_NULL = contextlib.nullcontext()
+
+
+def _host_flags(dev: torch.device) -> _HostFlags:
+    fl = _flags.get(dev.index)
+    if fl is None:
+        fl = _flags[dev.index] = _HostFlags(dev)
+    return fl
+
+
 def last_status() -> int:
     """Status bits collected on the current device since they were last raised (synchronises)."""
     if not torch.cuda.is_available():
         return 0
-    st = _status.get(torch.cuda.current_device())
-    return 0 if st is None else int(st.word.item())
+    dev = torch.cuda.current_device()
+    st, fl = _status.get(dev), _flags.get(dev)
+    code = 0 if st is None else int(st.word.item())
+    if fl is not None:
+        torch.cuda.synchronize(dev)
+        code |= fl.code()
+    return code
 
 
 def _status_message(code: int, what: str) -> str:
@@ -111,6 +149,8 @@ def _status_message(code: int, what: str) -> str:
         msgs.append("an on-chip wait timed out (results invalid)")
     if code & _lib.DEV_POSITIVE_GATE:
         msgs.append("g > 0 seen: outside domain I-1 (g <= 0)")
+    if code & _lib.DEV_BAD_INDEX:
+        msgs.append("a state index or a length out of range was seen")
     if not msgs:
         msgs.append(f"device status {code:#x}")
     return f"{what}: " + "; ".join(msgs)

@@ -1,0 +1,159 @@
+"""Products of a few rows with 4-bit weights: y = act(x W + bias) + residual.
+
+W (din, dout) is Q * s: integers Q in [-8, 7] and one bf16 scale per group of 32, 64 or 128 rows of
+a column.  pack_w4 lays a quantised weight out once for the kernel, quantize_w4 quantises one;
+w4_linear multiplies.  x, residual and y are fp32 or bf16; the products are exact for bf16 x and
+carry 24 bits of fp32 x, sums and scales are fp32.  The kernel reads the weight once per 32 rows
+of x, which is what few rows cost; there is no backward.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib, pipeline
+from .recurrent import _raw_stream
+
+GROUPS = (32, 64, 128)
+_ACTS = {None: 0, "gelu": 1}
+
+
+class W4Weight:
+    """A packed 4-bit weight (layout: include/gdn2_b200.h, gdn2_w4_linear).  `packed` and `scales`
+    are its buffers, din x dout its size, `group` the rows per scale."""
+
+    __slots__ = ("packed", "scales", "din", "dout", "group", "device")
+
+    def __init__(self, packed, scales, din, dout, group):
+        self.packed, self.scales, self.din, self.dout, self.group = packed, scales, din, dout, group
+        self.device = packed.device
+
+    def to(self, device):
+        return W4Weight(self.packed.to(device), self.scales.to(device), self.din, self.dout, self.group)
+
+    def integers(self) -> torch.Tensor:
+        """Q (din, dout) int8."""
+        nb, kb = -(-self.dout // 16), -(-self.din // 64)
+        w = self.packed.view(nb, kb, 8, 4, 2, 2, 1)             # column, t, half, step, word
+        sh = torch.arange(0, 32, 4, device=w.device, dtype=torch.int32)
+        n = ((w >> sh) & 15).view(nb, kb, 8, 4, 2, 2, 2, 2, 2)  # ..., e, f, c (nibble c + 2 f + 4 e)
+        n = n.permute(1, 4, 3, 5, 7, 6, 0, 8, 2)                # kb, half, t, step, f, e | nb, c, column
+        return (n.reshape(kb * 64, nb * 16)[:self.din, :self.dout] - 8).to(torch.int8)
+
+    def dequantize(self) -> torch.Tensor:
+        """W (din, dout) fp32."""
+        s = self.scales.permute(1, 0, 2).reshape(self.scales.shape[1], -1)[:, :self.dout].float()
+        return self.integers().float() * s.repeat_interleave(self.group, 0)[:self.din]
+
+
+def pack_w4(q: torch.Tensor, scales: torch.Tensor, group: int = 64) -> W4Weight:
+    """q (din, dout) integers in [-8, 7]; scales (ceil(din / group), dout) bf16.  Lays the weight out
+    on q's device.  Values outside the range are refused."""
+    if q.ndim != 2 or not q.numel() or q.dtype.is_floating_point or q.dtype == torch.bool:
+        raise ValueError("q must be a (din, dout) tensor of integers")
+    if group not in GROUPS:
+        raise ValueError(f"group={group} must be one of {GROUPS}")
+    din, dout = q.shape
+    if scales.shape != (-(-din // group), dout) or scales.dtype != torch.bfloat16:
+        raise ValueError(f"scales must be bfloat16 of shape {(-(-din // group), dout)}")
+    if scales.device != q.device:
+        raise ValueError(f"scales are on {scales.device}, q on {q.device}")
+    lo, hi = torch.stack(torch.aminmax(q)).tolist()
+    if lo < -8 or hi > 7:
+        raise ValueError(f"q has values in [{lo}, {hi}], outside [-8, 7]")
+    nb, kb = -(-dout // 16), -(-din // 64)
+    n = torch.full((kb * 64, nb * 16), 8, dtype=torch.uint8, device=q.device)
+    n[:din, :dout] = (q + 8).to(torch.uint8)
+    # rows 64 kb + 32 half + 8 t + 4 step + 2 f + e, columns 16 nb + 8 c + column
+    n = n.view(kb, 2, 4, 2, 2, 2, nb, 2, 8).permute(6, 0, 8, 2, 1, 3, 5, 4, 7).reshape(nb, kb, 8, 4, 2, 2, 8)
+    by = n[..., 0::2] | (n[..., 1::2] << 4)
+    packed = by.contiguous().view(torch.int32).reshape(nb, kb, 32, 4)
+    s = torch.zeros(scales.shape[0], nb * 16, dtype=torch.bfloat16, device=q.device)
+    s[:, :dout] = scales
+    s = s.view(-1, nb, 16).permute(1, 0, 2).contiguous()
+    return W4Weight(packed, s, din, dout, group)
+
+
+def quantize_w4(weight: torch.Tensor, group: int = 64) -> W4Weight:
+    """Rounds a (din, dout) weight to 4 bits: per group the scale is max |W| / 7 in bf16 (rounded
+    first, so that the integers fit the scale that is used), Q = round(W / s) within [-8, 7]."""
+    if weight.ndim != 2 or not weight.numel() or not weight.dtype.is_floating_point:
+        raise ValueError("weight must be a (din, dout) floating-point tensor")
+    if group not in GROUPS:
+        raise ValueError(f"group={group} must be one of {GROUPS}")
+    w = weight.detach().float()
+    if not bool(torch.isfinite(w).all()):
+        raise ValueError("weight has values that are not finite")
+    din, dout = w.shape
+    n = -(-din // group)
+    p = torch.zeros(n * group, dout, device=w.device)
+    p[:din] = w
+    p = p.view(n, group, dout)
+    s = (p.abs().amax(1) / 7.0).to(torch.bfloat16)
+    q = torch.round(p / torch.where(s > 0, s, torch.ones_like(s)).float()[:, None]).clamp(-8, 7)
+    return pack_w4(q.view(n * group, dout)[:din].to(torch.int8), s, group)
+
+
+_descs = {}
+
+
+def w4_linear(x: torch.Tensor, weight: W4Weight, bias=None, *, act=None, residual=None) -> torch.Tensor:
+    """act(x W + bias) + residual.  x (..., din) fp32 or bf16 CUDA tensor; bias (dout) or None;
+    act None or "gelu" (tanh form); residual (..., dout) of x's type.  Returns (..., dout) of x's
+    type, rounded once."""
+    dt, shape, dev = x.dtype, x.shape, x.device
+    if not x.is_cuda:
+        raise RuntimeError("w4_linear: x must be a CUDA tensor (the product runs only on the B200 kernels)")
+    if dt != torch.float32 and dt != torch.bfloat16:
+        raise ValueError(f"w4_linear: x must be float32 or bfloat16, not {dt}")
+    din, dout = weight.din, weight.dout
+    if not shape or shape[-1] != din:
+        raise ValueError(f"w4_linear: x has shape {tuple(shape)}, the weight {din} rows")
+    if weight.device != dev:
+        raise ValueError(f"w4_linear: x is on {dev}, the weight on {weight.device}")
+    if act not in _ACTS:
+        raise ValueError(f"w4_linear: act={act!r} is not None or 'gelu'")
+    grads = x.requires_grad
+    x2 = x if len(shape) == 2 else x.reshape(-1, din)
+    M = x2.shape[0]
+    if din > 1 and x2.stride(1) != 1:
+        x2 = x2.contiguous()
+    y = torch.empty((*shape[:-1], dout), dtype=dt, device=dev)
+    bp = rp = rs = 0
+    if bias is not None:
+        if bias.shape != (dout,) or bias.device != dev:
+            raise ValueError(f"w4_linear: bias must have shape {(dout,)} on {dev}")
+        grads = grads or bias.requires_grad
+        if bias.dtype != torch.float32 or not bias.is_contiguous():
+            bias = bias.float().contiguous()
+        bp = bias.data_ptr()
+    if residual is not None:
+        if residual.shape != y.shape or residual.dtype != dt or residual.device != dev:
+            raise ValueError(f"w4_linear: residual must be {dt} of shape {tuple(y.shape)} on {dev}")
+        grads = grads or residual.requires_grad
+        r2 = residual if len(shape) == 2 else residual.reshape(-1, dout)
+        if dout > 1 and r2.stride(1) != 1:
+            r2 = r2.contiguous()
+        rp, rs = r2.data_ptr(), r2.stride(0)
+    if grads and torch.is_grad_enabled():
+        raise RuntimeError("w4_linear has no backward: call it under torch.no_grad()")
+    if M == 0:
+        return y
+    key = (M, din, dout, weight.group, dt, act, x2.stride(0), rs)
+    desc = _descs.get(key)
+    if desc is None:
+        d = _lib.W4Desc()
+        d.M, d.K, d.N, d.group = M, din, dout, weight.group
+        d.dtype = _lib.BF16 if dt == torch.bfloat16 else _lib.F32
+        d.act = _ACTS[act]
+        d.x_stride, d.res_stride, d.y_stride = x2.stride(0), rs, dout
+        if len(_descs) > 1024:
+            _descs.clear()
+        desc = _descs[key] = (d, ctypes.addressof(d))
+    with torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else pipeline._NULL:
+        rc = _lib.load().gdn2_w4_linear(desc[1], x2.data_ptr(), weight.packed.data_ptr(), weight.scales.data_ptr(),
+                                        bp, rp, y.data_ptr(), _raw_stream(dev.index))
+    if rc:
+        _lib.check(rc, "gdn2_w4_linear")
+    return y

@@ -60,6 +60,7 @@ typedef enum gdn2_dtype { GDN2_F32 = 0, GDN2_BF16 = 1 } gdn2_dtype;
 #define GDN2_DEV_TIMEOUT 1u        /* a bounded on-chip wait ran out (results invalid) */
 #define GDN2_DEV_SPAN 2u           /* reserved: no longer raised (wide gate spans are computed exactly) */
 #define GDN2_DEV_POSITIVE_GATE 4u  /* g > 0 seen: outside domain I-1 (domain.py:1-6) */
+#define GDN2_DEV_BAD_INDEX 8u      /* a state index or a length out of range was seen (gdn2_recurrent) */
 
 /* Operator descriptor.  Fields mirror BLRConfig (config.py:28-50) where they
  * affect the arithmetic; TPU tiling fields are not part of the ABI. */
@@ -209,6 +210,82 @@ gdn2_status gdn2_prologue_fwd(const float* y, int64_t B, int64_t L, int64_t H, i
 gdn2_status gdn2_prologue_bwd(const float* y, int64_t B, int64_t L, int64_t H, int64_t D, float g_max,
                               int32_t l2norm, const float* dq, const float* dk, const float* dv, const float* dw,
                               const float* db, const float* dg, float* dy, void* stream);
+
+/*
+ * Serving operators (no counterpart in the reference, which has the chunked operator and its
+ * training only).  They run on the caller's stream alone and need no backward.
+ */
+
+/* The recurrent form of the operator (the token recurrence of reference/ref.py:116-130): L >= 0
+ * tokens, one after the other, from a state per sequence.  Per head and token
+ *   a = exp(min(g, 0)), d = w v - (b k)^T (diag(a) S), S <- diag(a) S + k d^T, o = scale q^T S;
+ * o and the final states are sanitized at clip.  It equals gdn2_fwd with wy_eps = 0. */
+typedef struct gdn2_rec_desc {
+  int32_t B, H, L, D;     /* L >= 0, D == 128 */
+  int64_t stride[6][3];   /* element strides of q, k, v, w, b, g over B, H, L: multiples of 16 bytes */
+  int64_t o_stride[3];    /* element strides of o over B, H, L: multiples of 4 */
+  int32_t n_states;       /* rows of h0 */
+  int32_t in_dtype;       /* gdn2_dtype of q..g */
+  float scale, clip;
+} gdn2_rec_desc;
+
+/*   q..g      tensors over (B, H, L, D) with unit stride along D, 16-byte aligned
+ *   h0        (n_states, H, D, D) fp32 contiguous, or NULL for zeros
+ *   h_index   (B) row of h0 that each sequence starts from (negative: zeros), or NULL for row b;
+ *             two sequences may name one row
+ *   lengths   (B) tokens of each sequence, 0..L, or NULL for L; o is zero past them
+ *   o         fp32 over (B, H, L, D) in o_stride, h_out (B, H, D, D) fp32 contiguous.  h_out may
+ *             be h0 itself when h_index is NULL and must not overlap it otherwise
+ *   flags     two uint32 words in device or mapped host memory: a kernel sets [0] to 1 when it
+ *             sees g > 0 (outside domain I-1) and [1] to 1 when it sees an index >= n_states (it
+ *             then starts from zeros) or a length outside 0..L (it then takes the nearer bound) */
+gdn2_status gdn2_recurrent(const gdn2_rec_desc* desc, const void* q, const void* k, const void* v, const void* w,
+                           const void* b, const void* g, const float* h0, const int32_t* h_index,
+                           const int32_t* lengths, float* o, float* h_out, uint32_t* flags, void* stream);
+
+typedef enum gdn2_act { GDN2_ACT_NONE = 0, GDN2_ACT_GELU_TANH = 1 } gdn2_act;
+
+/* y = act(x W + bias) + residual for a 4-bit weight: W[k][n] = scale[k / group][n] * Q[k][n] with Q
+ * in [-8, 7].  Made for few rows (M up to about 32 reads the weight once); any M works. */
+typedef struct gdn2_w4_desc {
+  int32_t M, K, N;
+  int32_t group;          /* rows of W per scale: 32, 64 or 128 */
+  int32_t dtype;          /* gdn2_dtype of x, residual and y */
+  int32_t act;            /* gdn2_act */
+  int64_t x_stride, res_stride, y_stride;  /* element strides between rows */
+} gdn2_w4_desc;
+
+/*   packed    ceil(N / 16) * ceil(K / 64) tiles of 512 bytes, 16-byte aligned: tile (i, j), i the
+ *             slower, holds columns 16 i.. and rows 64 j..; its 32-bit word 4 l + s (lane l in
+ *             0..31, s in 0..3) holds eight nibbles Q + 8: nibble c + 4 e + 2 f is column
+ *             16 i + l / 4 + 8 c, row 64 j + 32 (s / 2) + 8 (l % 4) + 4 (s % 2) + 2 f + e (c, e, f
+ *             in 0..1); 8 where the column or row is past the weight's
+ *   scales    bf16 (ceil(N / 16), ceil(K / group), 16): column 16 i + c, group g at [i][g][c]
+ *   bias      (N) fp32 or NULL;  residual (M, N) or NULL */
+gdn2_status gdn2_w4_linear(const gdn2_w4_desc* desc, const void* x, const void* packed, const void* scales,
+                           const float* bias, const void* residual, void* y, void* stream);
+
+/* One step of beam search: the K best continuations of each of B sequences from the logits of
+ * their K beams (K <= 32).  total = score + (x - max) - log sum exp(x - max).  Order: inside a beam
+ * by logit, the lowest token first among equals; over the beams by total, the lowest beam first
+ * among equals.  A NaN logit or score counts as -inf, +inf as the largest finite value; a beam
+ * whose logits are all -inf offers totals of -inf; a finished beam offers (eos, its score) alone
+ * (further ranks: -inf). */
+typedef struct gdn2_beam_desc {
+  int32_t B, K, V;
+  int32_t dtype;          /* gdn2_dtype of the logits */
+  int64_t stride_b, stride_k;  /* element strides of the logits over B and K; unit along V */
+  int32_t eos;            /* token that finishes a beam, or negative for none */
+} gdn2_beam_desc;
+
+size_t gdn2_beam_workspace_bytes(const gdn2_beam_desc* desc);
+
+/*   scores, out_scores (B, K) fp32;  finished (B, K) bytes or NULL for none;  out_finished (B, K);
+ *   out_row (B, K) b * K + the beam that is continued (a row of the logits and of the states);
+ *   workspace gdn2_beam_workspace_bytes(desc) bytes, 256-byte aligned.  Outputs overlap no input. */
+gdn2_status gdn2_beam_select(const gdn2_beam_desc* desc, const void* logits, const float* scores,
+                             const uint8_t* finished, float* out_scores, int32_t* out_row, int32_t* out_token,
+                             uint8_t* out_finished, void* workspace, void* stream);
 
 /* Profiling hook (no counterpart in the reference).  While enabled, every kernel launch of
  * gdn2_fwd / gdn2_bwd is bracketed by CUDA events recorded on the caller's stream.
