@@ -40,9 +40,10 @@ def _check_flags(fl: pipeline._HostFlags, what: str) -> None:
 
 
 def _rows_ok(t: torch.Tensor) -> bool:
-    """Whether the kernels can read t's rows in place: unit stride, every row on 16 bytes."""
+    """Whether the kernels can read t's rows in place: unit stride, every row on 16 bytes, neighbouring
+    tokens less than 2^27 elements apart."""
     st, n = t.stride(), 16 // t.element_size()
-    return st[3] == 1 and not (st[0] % n or st[1] % n or st[2] % n or t.data_ptr() % 16)
+    return st[3] == 1 and st[2] < 1 << 27 and not (st[0] % n or st[1] % n or st[2] % n or t.data_ptr() % 16)
 
 
 def _int32(t, name, B, dev):
@@ -144,13 +145,16 @@ def make_blr_recurrent(cfg: BLRConfig, scale):
             d.scale, d.clip = scale, clip
             if len(_descs) > 1024:
                 _descs.clear()
-            desc = _descs[key] = (d, ctypes.addressof(d))
+            at = ctypes.addressof(d)
+            desc = _descs[key] = (d, at, _lib.load().gdn2_recurrent_workspace_bytes(at))
+        ws = torch.empty(desc[2], dtype=torch.uint8, device=dev) if desc[2] else None
         fl = pipeline._host_flags(dev)
         with torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else pipeline._NULL:
             rc = _lib.load().gdn2_recurrent(
                 desc[1], xs[0].data_ptr(), xs[1].data_ptr(), xs[2].data_ptr(), xs[3].data_ptr(), xs[4].data_ptr(),
                 xs[5].data_ptr(), 0 if h0 is None else h0.data_ptr(), 0 if h_index is None else h_index.data_ptr(),
-                0 if lengths is None else lengths.data_ptr(), o.data_ptr(), h_out.data_ptr(), fl.ptr,
+                0 if lengths is None else lengths.data_ptr(), o.data_ptr(), h_out.data_ptr(),
+                0 if ws is None else ws.data_ptr(), fl.ptr,
                 _raw_stream(dev.index))
         if rc:
             _lib.check(rc, "gdn2_recurrent")

@@ -12,6 +12,8 @@
 namespace gdn2 {
 namespace {
 
+using u64 = unsigned long long;
+
 struct RecParams {
   const void *q, *k, *v, *w, *b, *g;
   long long sb[6], sh[6], sl[6];  // element strides of q, k, v, w, b, g over B, H, L
@@ -162,138 +164,540 @@ __global__ void __launch_bounds__(kStepThreads) rec_step_kernel(RecParams p) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// Several tokens.  A warp owns kM columns per group of eight lanes and keeps them in registers
-// over all tokens (16 rows each lane), so the token loop reduces inside the warp and waits for
-// no other warp; the tokens' vectors are staged in shared memory for the whole CTA.
+// Several tokens: blocks of 8.  With G_t the gates summed from the block's start through token t,
+//   r_t = (bk_t e^{G_t})^T S,   d_t = w_t v_t - r_t - sum_{s<t} L_ts d_s,
+//   o_t = (scale q_t e^{G_t})^T S + sum_{s<=t} P_ts d_s,
+//   S  <- diag(e^{G_8}) S + sum_t (k_t e^{G_8 - G_t}) d_t^T,
+//   L_ts = sum_d bk_t k_s e^{G_t - G_s},   P_ts = scale sum_d q_t k_s e^{G_t - G_s}
+// is the recurrence with the state read once and written once per block: one reduction over d_k
+// serves eight tokens, and 3 1/8 products per state element and token are left of 4.  Every factor
+// is a product of gates e^g <= 1, so nothing can overflow however far the gates close.
+//
+// rec_prep_kernel writes what does not depend on S, a record per head and block; rec_seq_kernel
+// walks the records with the state in registers.
+//
+// The state's products run on the warp-level tensor instruction (m16n8k8, tf32) with each fp32
+// operand split in two (hi lo, each rounded to nearest: 22 bits) and three products; the lo lo
+// product would be below fp32's own rounding.  A warp holds the transposed state, 16 columns (d_v)
+// x its share of d, in the accumulator layout; the same registers are the next product's first
+// operand, since the sum over d may run in any order.  On the CUDA cores the same work is bound by
+// the shared-memory traffic of the vectors (every lane needs its own copy), measured 2 to 6 times
+// slower.  Sums of the state itself stay outside the tensor instruction, whose additions may
+// truncate: U = sum_t k_t d_t^T there, S <- e S + U in fp32.
 // ---------------------------------------------------------------------------------------------
-constexpr int kSeqWarps = 4;
-constexpr int kSeqTok = 8;  // tokens staged at a time
+constexpr int kSmCount = 148;  // of a B200
+constexpr int kTok = 8;
+// A record, in floats, in the order in which the lanes (g = lane / 4, t = lane % 4) read it:
+constexpr int kRecDot = 0;               // [16 tiles of d][32 lanes]{bk(8j+2t), bk(8j+2t+1), q.., q..} of token g
+constexpr int kRecK = 16 * 128;          // [8 pairs of tiles][32]{k of tokens 2t, 2t+1 at 16i+g, the same at 16i+8+g}
+constexpr int kRecA = kRecK + 8 * 128;   // [8][4 t]{e(16i+2t), e(16i+2t+1), e(16i+8+2t), e(16i+8+2t+1)}
+constexpr int kRecX = kRecA + 128;       // [32]{X(g,2t), X(g,2t+1), P(g,2t), P(g,2t+1)}, X = (I + L)^-1
+constexpr int kRecV = kRecX + 128;       // [8 tiles of columns][32]{wv of tokens 2t, 2t+1 at 16i+g, at 16i+8+g}
+constexpr int kRecFloats = kRecV + 8 * 128;
 
-template <class T, int kM>
-__global__ void __launch_bounds__(kSeqWarps * 32) rec_seq_kernel(RecParams p) {
-  constexpr int kCols = kSeqWarps * 4 * kM;  // columns of a CTA
-  __shared__ float sa[kSeqTok][kD], sk[kSeqTok][kD], sbk[kSeqTok][kD], sq[kSeqTok][kD], swv[kSeqTok][kCols];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int bh = blockIdx.x, b = bh / p.H, h = bh % p.H;
-  const int c0 = blockIdx.y * kCols;
-  const int rg = lane & 7, cg = lane >> 3;
-  const int cw = (warp * 4 + cg) * kM;  // this lane's first column within the CTA
-  const bool first = tid == 0 && h == 0 && blockIdx.y == 0;
-  const int row = state_row(p, b, first);
-  const int n = valid_len(p, b, first);
-  // lane rg holds rows 4 rg + 32 i + j (i, j < 4)
-  float s[16][kM];
-  const size_t at = (size_t)c0 + cw;
+// A warp per head and block of tokens, a quarter of d at a time.  Tokens past the sequence's end
+// become no-ops (gate 1, zeros elsewhere).
+constexpr int kPrepWarps = 4;
+
+template <class T>
+__global__ void __launch_bounds__(kPrepWarps * 32, 4) rec_prep_kernel(RecParams p, float* rec, int tok0, int nblk,
+                                                                   int total) {
+  __shared__ float lps[kPrepWarps][64], xs[kPrepWarps][64];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int unit = blockIdx.x * kPrepWarps + warp;
+  if (unit >= total) return;
+  const int bh = unit / nblk, blk = unit % nblk;
+  const int b = bh / p.H, h = bh % p.H;
+  const int t0 = tok0 + blk * kTok, left = valid_len(p, b, false) - t0;
+  if (left <= 0) return;
+  float* out = rec + (size_t)unit * kRecFloats;
+  // Gram entries: 8 t + s is L_ts (s < t), 8 s + t is P_ts (s <= t)
+  float gram[64];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int r = rg * 4 + (i >> 2) * 32 + (i & 3);
+  for (int i = 0; i < 64; ++i) gram[i] = 0.f;
+  const T* src[6];
+  const void* base[6] = {p.q, p.k, p.v, p.w, p.b, p.g};
+  int sl[6];  // a block's tokens are within 32 bits of one another (checked by the entry)
 #pragma unroll
-    for (int m = 0; m < kM; ++m)
-      s[i][m] = row >= 0 ? p.h0[((size_t)row * p.H + h) * (kD * kD) + (size_t)r * kD + at + m] : 0.f;
+  for (int i = 0; i < 6; ++i) sl[i] = (int)p.sl[i];
+#pragma unroll
+  for (int i = 0; i < 6; ++i)
+    src[i] = static_cast<const T*>(base[i]) + b * p.sb[i] + h * p.sh[i] + t0 * p.sl[i] + lane;
+  bool positive = false;
+#pragma unroll 1
+  for (int d = lane; d < kD; d += 32) {
+    float q[kTok], k[kTok], bk[kTok], a[kTok], v[kTok], wv[kTok];
+#pragma unroll
+    for (int t = 0; t < kTok; ++t) {  // all of the loads first; the last valid token stands in for those past it
+      const int tt = min(t, left - 1);
+      q[t] = ld1(src[0] + tt * sl[0]);
+      k[t] = ld1(src[1] + tt * sl[1]);
+      v[t] = ld1(src[2] + tt * sl[2]);
+      wv[t] = ld1(src[3] + tt * sl[3]);
+      bk[t] = ld1(src[4] + tt * sl[4]);
+      a[t] = ld1(src[5] + tt * sl[5]);
+    }
+#pragma unroll
+    for (int i = 0; i < 6; ++i) src[i] += 32;
+#pragma unroll
+    for (int t = 0; t < kTok; ++t) {
+      const bool on = t < left;
+      positive |= a[t] > 0.f;
+      a[t] = on ? expf(fminf(a[t], 0.f)) : 1.f;
+      q[t] = on ? q[t] * p.scale : 0.f;
+      k[t] = on ? k[t] : 0.f;
+      bk[t] = on ? bk[t] * k[t] : 0.f;
+      wv[t] = on ? wv[t] * v[t] : 0.f;
+    }
+    float kh[kTok];  // k_s e^{G_8 - G_s}
+#pragma unroll
+    for (int s = 0; s < kTok; ++s) {
+      float c = k[s];
+      gram[9 * s] = fmaf(q[s], c, gram[9 * s]);
+#pragma unroll
+      for (int t = s + 1; t < kTok; ++t) {
+        c *= a[t];
+        gram[8 * t + s] = fmaf(bk[t], c, gram[8 * t + s]);
+        gram[8 * s + t] = fmaf(q[t], c, gram[8 * s + t]);
+      }
+      kh[s] = c;
+    }
+    // Two lanes hold the two halves of 16 bytes of the record: each takes every second piece.
+    float e = 1.f;
+    const bool odd = d & 1, high = d & 8;
+#pragma unroll
+    for (int t = 0; t < kTok; t += 2) {
+      e *= a[t];
+      const float b0 = bk[t] * e, q0 = q[t] * e;
+      e *= a[t + 1];
+      const float b1 = bk[t + 1] * e, q1 = q[t + 1] * e;
+      const float bx = __shfl_xor_sync(0xffffffffu, odd ? b0 : b1, 1);
+      const float qx = __shfl_xor_sync(0xffffffffu, odd ? q0 : q1, 1);
+      float4* to = reinterpret_cast<float4*>(out + kRecDot) + (d >> 3) * 32 + (t + odd) * 4 + ((d & 7) >> 1);
+      *to = odd ? make_float4(bx, b1, qx, q1) : make_float4(b0, bx, q0, qx);
+    }
+    out[kRecA + ((d >> 4) * 4 + ((d & 7) >> 1)) * 4 + ((d >> 3) & 1) * 2 + (d & 1)] = e;
+    const int at = (d >> 4) * 32 + (d & 7) * 4 + (high ? 2 : 0);
+#pragma unroll
+    for (int t = 0; t < 4; t += 2) {
+      const float k0 = __shfl_xor_sync(0xffffffffu, high ? kh[t] : kh[t + 4], 8);
+      const float k1 = __shfl_xor_sync(0xffffffffu, high ? kh[t + 1] : kh[t + 5], 8);
+      const float v0 = __shfl_xor_sync(0xffffffffu, high ? wv[t] : wv[t + 4], 8);
+      const float v1 = __shfl_xor_sync(0xffffffffu, high ? wv[t + 1] : wv[t + 5], 8);
+      reinterpret_cast<float4*>(out + kRecK)[at + (t >> 1)] =
+          high ? make_float4(k0, k1, kh[t + 4], kh[t + 5]) : make_float4(kh[t], kh[t + 1], k0, k1);
+      reinterpret_cast<float4*>(out + kRecV)[at + (t >> 1)] =
+          high ? make_float4(v0, v1, wv[t + 4], wv[t + 5]) : make_float4(wv[t], wv[t + 1], v0, v1);
+    }
   }
-  float* op = p.o + b * p.ob + h * p.oh + c0 + cw;
-  for (int t0 = 0; t0 < n; t0 += kSeqTok) {
-    const int tc = min(kSeqTok, n - t0);
-    __syncthreads();
-    for (int i = tid; i < tc * kD; i += kSeqWarps * 32) {
-      const int t = i / kD, d = i % kD;
-      const long long l = t0 + t;
-      const float k = ld1(static_cast<const T*>(p.k) + b * p.sb[1] + h * p.sh[1] + l * p.sl[1] + d);
-      const float be = ld1(static_cast<const T*>(p.b) + b * p.sb[4] + h * p.sh[4] + l * p.sl[4] + d);
-      const float g = ld1(static_cast<const T*>(p.g) + b * p.sb[5] + h * p.sh[5] + l * p.sl[5] + d);
-      if (g > 0.f) p.flags[0] = 1u;
-      sq[t][d] = p.scale * ld1(static_cast<const T*>(p.q) + b * p.sb[0] + h * p.sh[0] + l * p.sl[0] + d);
-      sk[t][d] = k;
-      sbk[t][d] = be * k;
-      sa[t][d] = expf(fminf(g, 0.f));
+  if (positive) p.flags[0] = 1u;
+  // 64 sums over the lanes, halving: lane l ends with entries 2 l and 2 l + 1
+#pragma unroll
+  for (int half = 32; half >= 2; half >>= 1) {
+    const bool up = lane & (half >> 1);
+#pragma unroll
+    for (int i = 0; i < half; ++i) {
+      const float keep = up ? gram[i + half] : gram[i], give = up ? gram[i] : gram[i + half];
+      gram[i] = keep + __shfl_xor_sync(0xffffffffu, give, half >> 1);
     }
-    for (int i = tid; i < tc * kCols; i += kSeqWarps * 32) {
-      const int t = i / kCols, c = i % kCols;
-      const long long l = t0 + t;
-      swv[t][c] = ld1(static_cast<const T*>(p.v) + b * p.sb[2] + h * p.sh[2] + l * p.sl[2] + c0 + c) *
-                  ld1(static_cast<const T*>(p.w) + b * p.sb[3] + h * p.sh[3] + l * p.sl[3] + c0 + c);
+  }
+  float *lp = lps[warp], *x = xs[warp];
+  *reinterpret_cast<float2*>(lp + 2 * lane) = make_float2(gram[0], gram[1]);
+  __syncwarp();
+  if (lane < 8) {  // column `lane` of X = (I + L)^-1 by forward substitution
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      y[i] = i == lane ? 1.f : 0.f;
+#pragma unroll
+      for (int j = 0; j < i; ++j) y[i] = fmaf(-lp[8 * i + j], y[j], y[i]);
+      x[8 * i + lane] = y[i];
     }
-    __syncthreads();
-    for (int t = 0; t < tc; ++t) {
-      float r[kM], o[kM];
+  }
+  __syncwarp();
+  const int g = lane >> 2, s = (lane & 3) * 2;
+  reinterpret_cast<float4*>(out + kRecX)[lane] =
+      make_float4(x[8 * g + s], x[8 * g + s + 1], s <= g ? lp[8 * s + g] : 0.f, s + 1 <= g ? lp[8 * (s + 1) + g] : 0.f);
+}
+
+// x = hi + lo: hi is x in tf32, rounded to nearest, and the tensor instruction drops the 13 low bits
+// of lo, 2^-21 of x at most and either way.  A NaN may lose its bits in hi but stays one in lo.
+struct Split { uint32_t hi, lo; };
+__device__ __forceinline__ Split split(float x) {
+  Split s;
+  s.hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+  s.lo = __float_as_uint(x - __uint_as_float(s.hi));
+  return s;
+}
+struct SplitA { uint32_t hi[4], lo[4]; };
+// An accumulator tile as the next product's first operand (k = t and t + 4 are columns 2t and 2t + 1).
+__device__ __forceinline__ SplitA split_tile(const float c[4]) {
+  SplitA a;
 #pragma unroll
-      for (int m = 0; m < kM; ++m) r[m] = o[m] = 0.f;
+  for (int i = 0; i < 4; ++i) {
+    const Split s = split(c[(i & 1) * 2 + (i >> 1)]);
+    a.hi[i] = s.hi;
+    a.lo[i] = s.lo;
+  }
+  return a;
+}
+__device__ __forceinline__ void mma1688(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// lo hi and hi lo into one accumulator, hi hi into another
+__device__ __forceinline__ void mma3(float big[4], float small[4], const SplitA& a, float b0, float b1) {
+  const Split x = split(b0), y = split(b1);
+  mma1688(small, a.lo, x.hi, y.hi);
+  mma1688(big, a.hi, x.hi, y.hi);
+  mma1688(small, a.hi, x.lo, y.lo);
+}
+
+// What both forms of the kernel share.
+struct SeqSpan {
+  int n, blocks;     // valid tokens of this launch, and their blocks
+  long long state;   // element offset of the head's state, negative for zeros
+  float* o;          // outputs of the launch's first token, at the CTA's first column
+};
+template <int kThreads, int kCols>
+__device__ __forceinline__ SeqSpan seq_span(const RecParams& p, int tok0, int nblk, bool first) {
+  const int bh = blockIdx.x, b = bh / p.H, h = bh % p.H, tid = threadIdx.x;
+  const bool report = first && tid == 0 && h == 0 && blockIdx.y == 0;
+  SeqSpan r;
+  r.n = max(0, min(valid_len(p, b, report) - tok0, nblk * kTok));
+  r.blocks = (r.n + kTok - 1) / kTok;
+  r.o = p.o + b * p.ob + h * p.oh + tok0 * p.ol + blockIdx.y * kCols;
+  const int end = min(p.L - tok0, nblk * kTok);
+  for (int i = r.n * kCols + tid; i < end * kCols; i += kThreads)  // past the sequence's end
+    r.o[(i / kCols) * p.ol + i % kCols] = 0.f;
+  r.state = bh;
+  if (first) {
+    const int row = state_row(p, b, report);
+    r.state = row < 0 ? -1 : (long long)row * p.H + h;
+  }
+  r.state *= kD * kD;
+  return r;
+}
+// Tile j of a warp: columns g (entries 0, 1) and g + 8 (2, 3), rows 8 j + 2 t and 8 j + 2 t + 1.
+template <int kJ>
+__device__ __forceinline__ void seq_load(float s[kJ][4], const float* state, const SeqSpan& r, size_t mine) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float4 a = *reinterpret_cast<const float4*>(&sa[t][rg * 4 + i * 32]);
-        const float4 bk = *reinterpret_cast<const float4*>(&sbk[t][rg * 4 + i * 32]);
-        const float av[4] = {a.x, a.y, a.z, a.w}, bv[4] = {bk.x, bk.y, bk.z, bk.w};
+  for (int j = 0; j < kJ; ++j)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+    for (int c = 0; c < 4; ++c)
+      s[j][c] = r.state >= 0 ? state[r.state + mine + (j * 8 + (c & 1)) * kD + (c >> 1) * 8] : 0.f;
+}
+template <int kJ>
+__device__ __forceinline__ void seq_store(const float s[kJ][4], const RecParams& p, size_t mine, bool last) {
+  float* to = p.h_out + (size_t)blockIdx.x * (kD * kD) + mine;
 #pragma unroll
-          for (int m = 0; m < kM; ++m) {
-            s[i * 4 + j][m] *= av[j];
-            r[m] = fmaf(bv[j], s[i * 4 + j][m], r[m]);
-          }
+  for (int j = 0; j < kJ; ++j)
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      to[(j * 8 + (c & 1)) * kD + (c >> 1) * 8] = last ? sanitize(s[j][c], p.clip) : s[j][c];
+}
+// d = X (wv - r) of the warp's 16 columns
+__device__ __forceinline__ SplitA seq_delta(const float r[4], const float4& wv, const float4& xp) {
+  const float u[4] = {wv.x - r[0], wv.y - r[1], wv.z - r[2], wv.w - r[3]};
+  float big[4] = {}, small[4] = {};
+  mma3(big, small, split_tile(u), xp.x, xp.y);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) big[c] += small[c];
+  return split_tile(big);
+}
+// o + P d, stored for the block's valid tokens
+__device__ __forceinline__ void seq_out(const RecParams& p, const SeqSpan& r, int blk, int col, float o[4],
+                                        const SplitA& d, const float4& xp) {
+  const int t = threadIdx.x & 3;
+  float big[4] = {}, small[4] = {};
+  mma3(big, small, d, xp.z, xp.w);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const int tok = blk * kTok + 2 * t + (c & 1);
+    if (tok < r.n) r.o[tok * p.ol + col + (c >> 1) * 8] = sanitize(o[c] + (big[c] + small[c]), p.clip);
+  }
+}
+template <int kJ>
+__device__ __forceinline__ void seq_update(float s[kJ][4], const SplitA& d, const float* slot, int j0, int lane) {
+#pragma unroll
+  for (int j = 0; j < kJ; j += 2) {
+    const float4 kk = *reinterpret_cast<const float4*>(slot + kRecK + ((j0 + j) * 16 + lane) * 4);
+    const float4 e = *reinterpret_cast<const float4*>(slot + kRecA + ((j0 + j) * 2 + (lane & 3)) * 4);
+    float ub[2][4] = {}, us[2][4] = {};
+    mma3(ub[0], us[0], d, kk.x, kk.y);
+    mma3(ub[1], us[1], d, kk.z, kk.w);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      s[j][c] = fmaf(c & 1 ? e.y : e.x, s[j][c], ub[0][c] + us[0][c]);
+      s[j + 1][c] = fmaf(c & 1 ? e.w : e.z, s[j + 1][c], ub[1][c] + us[1][c]);
+    }
+  }
+}
+__device__ __forceinline__ float4 lds4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kN>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kN) : "memory");
+}
+
+// Many heads: a warp owns 16 columns and all of d, a CTA kCT such tiles.  The records arrive
+// through a ring of asynchronous copies that the whole CTA issues.
+template <int kCT>
+__global__ void __launch_bounds__(kCT * 32) rec_wide_kernel(RecParams p, const float* rec, const float* state,
+                                                          int tok0, int nblk, bool first, bool last) {
+  constexpr int kThreads = kCT * 32, kSlots = 3, kSlot = kRecV + kCT * 128;
+  extern __shared__ float4 smem4[];
+  float* smem = reinterpret_cast<float*>(smem4);
+  const int tid = threadIdx.x, lane = tid & 31, ct = tid >> 5, g = lane >> 2, t = lane & 3;
+  const SeqSpan r = seq_span<kThreads, kCT * 16>(p, tok0, nblk, first);
+  if (r.blocks == 0 && !first && !last) return;
+  const size_t mine = (size_t)(2 * t) * kD + (blockIdx.y * kCT + ct) * 16 + g;
+  float s[16][4];
+  seq_load<16>(s, state, r, mine);
+  const float* src = rec + (size_t)blockIdx.x * nblk * kRecFloats;
+  auto fetch = [&](int blk) {
+    if (blk < r.blocks) {
+      float* dst = smem + (blk % kSlots) * kSlot;
+      const float* from = src + (size_t)blk * kRecFloats;
+      for (int i = tid; i < kRecV / 4; i += kThreads) cp_async16(dst + 4 * i, from + 4 * i);
+      cp_async16(dst + kRecV + 4 * tid, from + kRecV + blockIdx.y * kCT * 128 + 4 * tid);
+    }
+    cp_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kSlots - 1; ++i) fetch(i);
+  for (int blk = 0; blk < r.blocks; ++blk) {
+    cp_wait<kSlots - 2>();
+    __syncthreads();          // block blk is here, and every warp is done with block blk - 1
+    fetch(blk + kSlots - 1);  // into that block's slot
+    const float* slot = smem + (blk % kSlots) * kSlot;
+    float rr[4], o[4];
+    {
+      float rb[2][4] = {}, rs[4] = {}, ob[2][4] = {}, os[4] = {};
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float4 f = lds4(slot + kRecDot + (j * 32 + lane) * 4);
+        const SplitA a = split_tile(s[j]);
+        mma3(rb[j & 1], rs, a, f.x, f.y);
+        mma3(ob[j & 1], os, a, f.z, f.w);
       }
 #pragma unroll
-      for (int x = 1; x < 8; x <<= 1)
-#pragma unroll
-        for (int m = 0; m < kM; ++m) r[m] += __shfl_xor_sync(0xffffffffu, r[m], x);
-#pragma unroll
-      for (int m = 0; m < kM; ++m) r[m] = swv[t][cw + m] - r[m];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float4 kk = *reinterpret_cast<const float4*>(&sk[t][rg * 4 + i * 32]);
-        const float4 q = *reinterpret_cast<const float4*>(&sq[t][rg * 4 + i * 32]);
-        const float kv[4] = {kk.x, kk.y, kk.z, kk.w}, qv[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int m = 0; m < kM; ++m) {
-            s[i * 4 + j][m] = fmaf(kv[j], r[m], s[i * 4 + j][m]);
-            o[m] = fmaf(qv[j], s[i * 4 + j][m], o[m]);
-          }
-      }
-#pragma unroll
-      for (int x = 1; x < 8; x <<= 1)
-#pragma unroll
-        for (int m = 0; m < kM; ++m) o[m] += __shfl_xor_sync(0xffffffffu, o[m], x);
-      if (rg == 0) {
-#pragma unroll
-        for (int m = 0; m < kM; ++m) op[(t0 + t) * p.ol + m] = sanitize(o[m], p.clip);
+      for (int c = 0; c < 4; ++c) {
+        rr[c] = (rb[0][c] + rb[1][c]) + rs[c];
+        o[c] = (ob[0][c] + ob[1][c]) + os[c];
       }
     }
+    const float4 xp = lds4(slot + kRecX + lane * 4);
+    const SplitA d = seq_delta(rr, lds4(slot + kRecV + (ct * 32 + lane) * 4), xp);
+    seq_out(p, r, blk, ct * 16 + g, o, d, xp);
+    seq_update<16>(s, d, slot, 0, lane);
   }
-  for (int i = n * kCols + tid; i < p.L * kCols; i += kSeqWarps * 32)  // past the sequence's end
-    p.o[b * p.ob + h * p.oh + (i / kCols) * p.ol + c0 + i % kCols] = 0.f;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int r = rg * 4 + (i >> 2) * 32 + (i & 3);
-#pragma unroll
-    for (int m = 0; m < kM; ++m)
-      p.h_out[(size_t)bh * (kD * kD) + (size_t)r * kD + at + m] = sanitize(s[i][m], p.clip);
+  seq_store<16>(s, p, mine, last);
+}
+
+// Few heads, where a block's chain of dependent steps is what counts: kW warps share 16 columns and
+// take 16 / kW tiles of d each; one more warp copies the records and one finishes the outputs, a
+// block behind.  One barrier per block: before it the partial sums r of the block are written, after
+// it every warp adds them up.  What is double-buffered by the block's parity:
+//   rpart  written before barrier blk, read until barrier blk + 1
+//   opart, delta  written after barrier blk, read between barriers blk + 1 and blk + 2
+template <int kW>
+__global__ void __launch_bounds__((kW + 2) * 32) rec_deep_kernel(RecParams p, const float* rec, const float* state,
+                                                               int tok0, int nblk, bool first, bool last) {
+  constexpr int kThreads = (kW + 2) * 32, kJ = 16 / kW, kSlots = 6, kSlot = kRecV + 128;
+  extern __shared__ float4 smem4[];
+  float* smem = reinterpret_cast<float*>(smem4);
+  float4* rpart = smem4 + kSlots * kSlot / 4;  // [2][kW][32]
+  float4* opart = rpart + 2 * kW * 32;         // [2][kW][32]
+  float4* delta = opart + 2 * kW * 32;         // [2][32]
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const SeqSpan r = seq_span<kThreads, 16>(p, tok0, nblk, first);
+  if (r.blocks == 0 && !first && !last) return;
+  auto barrier = [] { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); };
+  if (warp == kW) {  // copies
+    const float* src = rec + (size_t)blockIdx.x * nblk * kRecFloats;
+    auto fetch = [&](int blk) {
+      if (blk < r.blocks) {
+        float* dst = smem + (blk % kSlots) * kSlot;
+        const float* from = src + (size_t)blk * kRecFloats;
+#pragma unroll 13
+        for (int i = lane; i < kRecV / 4; i += 32) cp_async16(dst + 4 * i, from + 4 * i);
+        cp_async16(dst + kRecV + 4 * lane, from + kRecV + blockIdx.y * 128 + 4 * lane);
+      }
+      cp_commit();
+    };
+    for (int i = 0; i < kSlots - 2; ++i) fetch(i);
+    cp_wait<kSlots - 3>();
+    barrier();  // block 0 is here
+    for (int blk = 0; blk < r.blocks; ++blk) {
+      cp_wait<kSlots - 4>();
+      barrier();                // block blk + 1 is here, and every warp is done with block blk - 2
+      fetch(blk + kSlots - 2);  // into that block's slot
+    }
+    barrier();
+    return;
   }
+  if (warp == kW + 1) {  // outputs
+    barrier();
+    for (int blk = 0; blk < r.blocks; ++blk) {
+      barrier();  // barrier blk: block blk - 1 is ready
+      if (blk == 0) continue;
+      const int par = (blk - 1) & 1;
+      float o[4] = {};
+#pragma unroll
+      for (int i = 0; i < kW; ++i) {
+        const float4 x = opart[(par * kW + i) * 32 + lane];
+        o[0] += x.x; o[1] += x.y; o[2] += x.z; o[3] += x.w;
+      }
+      const float4 x = delta[par * 32 + lane];
+      const float dl[4] = {x.x, x.y, x.z, x.w};
+      seq_out(p, r, blk - 1, g, o, split_tile(dl), lds4(smem + ((blk - 1) % kSlots) * kSlot + kRecX + lane * 4));
+    }
+    barrier();
+    if (r.blocks) {
+      const int blk = r.blocks - 1, par = blk & 1;
+      float o[4] = {};
+#pragma unroll
+      for (int i = 0; i < kW; ++i) {
+        const float4 x = opart[(par * kW + i) * 32 + lane];
+        o[0] += x.x; o[1] += x.y; o[2] += x.z; o[3] += x.w;
+      }
+      const float4 x = delta[par * 32 + lane];
+      const float dl[4] = {x.x, x.y, x.z, x.w};
+      seq_out(p, r, blk, g, o, split_tile(dl), lds4(smem + (blk % kSlots) * kSlot + kRecX + lane * 4));
+    }
+    return;
+  }
+  const int j0 = warp * kJ;
+  const size_t mine = (size_t)(8 * j0 + 2 * t) * kD + blockIdx.y * 16 + g;
+  float s[kJ][4];
+  seq_load<kJ>(s, state, r, mine);
+  barrier();
+  for (int blk = 0; blk < r.blocks; ++blk) {
+    const float* slot = smem + (blk % kSlots) * kSlot;
+    const int par = blk & 1;
+    SplitA a[kJ];
+    float4 f[kJ];
+    float big[2][4] = {}, small[2][4] = {};
+#pragma unroll
+    for (int j = 0; j < kJ; ++j) {
+      f[j] = lds4(slot + kRecDot + ((j0 + j) * 32 + lane) * 4);
+      a[j] = split_tile(s[j]);
+      mma3(big[j & 1], small[j & 1], a[j], f[j].x, f[j].y);
+    }
+    rpart[(par * kW + warp) * 32 + lane] =
+        make_float4((big[0][0] + big[1][0]) + (small[0][0] + small[1][0]), (big[0][1] + big[1][1]) + (small[0][1] + small[1][1]),
+                    (big[0][2] + big[1][2]) + (small[0][2] + small[1][2]), (big[0][3] + big[1][3]) + (small[0][3] + small[1][3]));
+    barrier();
+    float rr[4] = {};
+#pragma unroll
+    for (int i = 0; i < kW; ++i) {
+      const float4 x = rpart[(par * kW + i) * 32 + lane];
+      rr[0] += x.x; rr[1] += x.y; rr[2] += x.z; rr[3] += x.w;
+    }
+    const float4 xp = lds4(slot + kRecX + lane * 4);
+    const float4 wv = lds4(slot + kRecV + lane * 4);
+    const float u[4] = {wv.x - rr[0], wv.y - rr[1], wv.z - rr[2], wv.w - rr[3]};
+    float dl[4] = {}, ds[4] = {};
+    mma3(dl, ds, split_tile(u), xp.x, xp.y);
+    // the outputs' sums fill the tensor pipe while d is on its way
+    float ob[2][4] = {}, os[2][4] = {};
+#pragma unroll
+    for (int j = 0; j < kJ; ++j) mma3(ob[j & 1], os[j & 1], a[j], f[j].z, f[j].w);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) dl[c] += ds[c];
+    seq_update<kJ>(s, split_tile(dl), slot, j0, lane);
+    opart[(par * kW + warp) * 32 + lane] =
+        make_float4((ob[0][0] + ob[1][0]) + (os[0][0] + os[1][0]), (ob[0][1] + ob[1][1]) + (os[0][1] + os[1][1]),
+                    (ob[0][2] + ob[1][2]) + (os[0][2] + os[1][2]), (ob[0][3] + ob[1][3]) + (os[0][3] + os[1][3]));
+    if (warp == 0) delta[par * 32 + lane] = make_float4(dl[0], dl[1], dl[2], dl[3]);
+  }
+  barrier();
+  seq_store<kJ>(s, p, mine, last);
+}
+
+template <class K>
+cudaError_t launch_seq(K kernel, int cols, int threads, int bytes, const RecParams& p, const float* rec, int BH,
+                       int tok0, int nblk, bool first, bool last, cudaStream_t st) {
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return e;
+  kernel<<<dim3(BH, kD / cols), threads, bytes, st>>>(p, rec, first ? p.h0 : p.h_out, tok0, nblk, first, last);
+  return cudaGetLastError();
+}
+template <int kCT>
+cudaError_t launch_wide(const RecParams& p, const float* rec, int BH, int tok0, int nblk, bool first, bool last,
+                        cudaStream_t st) {
+  return launch_seq(rec_wide_kernel<kCT>, kCT * 16, kCT * 32, 3 * (kRecV + kCT * 128) * 4, p, rec, BH, tok0, nblk,
+                    first, last, st);
+}
+template <int kW>
+cudaError_t launch_deep(const RecParams& p, const float* rec, int BH, int tok0, int nblk, bool first, bool last,
+                        cudaStream_t st) {
+  return launch_seq(rec_deep_kernel<kW>, 16, (kW + 2) * 32, 6 * (kRecV + 128) * 4 + (4 * kW + 2) * 512, p, rec, BH,
+                    tok0, nblk, first, last, st);
+}
+
+// Blocks of tokens that one pair of launches covers: as many as keep the records within 64 MiB
+// (they are read back from L2), but eight at least, so that the state's own traffic stays small.
+int seg_blocks(long long BH, int L) {
+  const long long fit = (64LL << 20) / (BH * kRecFloats * 4), all = ((long long)L + kTok - 1) / kTok;
+  const long long n = fit < 8 ? 8 : fit;
+  return (int)(n < all ? n : all);
 }
 
 template <class T>
-void launch(const RecParams& p, int BH, cudaStream_t st) {
+cudaError_t launch(const RecParams& p, int BH, float* rec, cudaStream_t st) {
   if (p.L <= 1) {
     rec_step_kernel<T, 128><<<dim3(BH, 1), kStepThreads, 0, st>>>(p);
-  } else {
-    rec_seq_kernel<T, 2><<<dim3(BH, kD / (kSeqWarps * 8)), kSeqWarps * 32, 0, st>>>(p);
+    return cudaGetLastError();
   }
+  const int seg = seg_blocks(BH, p.L);
+  // Four warps on a head's 16 columns shorten a block's chain but repeat part of its work; measured
+  // per call (fp32, deep / wide): 6 heads x 4096 tokens 262 / 769 us, 48 x 1024 214 / 254, 96 x 777
+  // 327 / 344, 192 x 256 206 / 187, 384 x 192 330 / 285.  The deep form's 8 CTAs a head fill the GPU
+  // about six times over where the two meet.
+  const bool deep = (long long)BH * 8 <= 6LL * kSmCount;
+  for (int t0 = 0; t0 < p.L; t0 += seg * kTok) {
+    const int nblk = min(seg, (p.L - t0 + kTok - 1) / kTok);
+    const bool first = t0 == 0, last = t0 + seg * kTok >= p.L;
+    rec_prep_kernel<T><<<(BH * nblk + kPrepWarps - 1) / kPrepWarps, kPrepWarps * 32, 0, st>>>(p, rec, t0, nblk, BH * nblk);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    e = deep ? launch_deep<4>(p, rec, BH, t0, nblk, first, last, st)
+             : launch_wide<4>(p, rec, BH, t0, nblk, first, last, st);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Grids count heads x blocks of tokens along x.
+gdn2_status check_rec(const gdn2_rec_desc* d) {
+  if (!d || d->B <= 0 || d->H <= 0 || d->L < 0 || d->D <= 0) return GDN2_ERR_INVALID_ARGUMENT;
+  if (d->in_dtype != GDN2_F32 && d->in_dtype != GDN2_BF16) return GDN2_ERR_INVALID_ARGUMENT;
+  if (!(d->clip > 0.f) || (int64_t)d->B * d->H > (1 << 26)) return GDN2_ERR_INVALID_ARGUMENT;
+  return d->D == kD ? GDN2_OK : GDN2_ERR_UNSUPPORTED;
+}
+
 }  // namespace
 }  // namespace gdn2
+
+extern "C" size_t gdn2_recurrent_workspace_bytes(const gdn2_rec_desc* d) {
+  using namespace gdn2;
+  if (check_rec(d) != GDN2_OK || d->L <= 1) return 0;
+  return (size_t)d->B * d->H * seg_blocks((long long)d->B * d->H, d->L) * kRecFloats * 4;
+}
 
 extern "C" gdn2_status gdn2_recurrent(const gdn2_rec_desc* d, const void* q, const void* k, const void* v,
                                       const void* w, const void* b, const void* g, const float* h0,
                                       const int32_t* h_index, const int32_t* lengths, float* o, float* h_out,
-                                      uint32_t* flags, void* stream) {
+                                      void* workspace, uint32_t* flags, void* stream) {
   using namespace gdn2;
-  if (!d || d->B <= 0 || d->H <= 0 || d->L < 0 || d->D <= 0) return GDN2_ERR_INVALID_ARGUMENT;
-  if (d->in_dtype != GDN2_F32 && d->in_dtype != GDN2_BF16) return GDN2_ERR_INVALID_ARGUMENT;
-  if (!(d->clip > 0.f) || (int64_t)d->B * d->H > 0x7fffffffLL) return GDN2_ERR_INVALID_ARGUMENT;
-  if (d->D != kD) return GDN2_ERR_UNSUPPORTED;
+  const gdn2_status status = check_rec(d);
+  if (status != GDN2_OK) return status;
+  if (d->L > 1 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u))) return GDN2_ERR_INVALID_ARGUMENT;
   const int el = d->in_dtype == GDN2_BF16 ? 2 : 4;
   const void* ins[6] = {q, k, v, w, b, g};
   RecParams p{};
@@ -302,6 +706,8 @@ extern "C" gdn2_status gdn2_recurrent(const gdn2_rec_desc* d, const void* q, con
       if (!ins[i] || !aligned16(ins[i])) return GDN2_ERR_INVALID_ARGUMENT;
       for (int j = 0; j < 3; ++j)
         if (d->stride[i][j] < 0 || (d->stride[i][j] * el) % 16) return GDN2_ERR_INVALID_ARGUMENT;
+    for (int i = 0; i < 6; ++i)
+      if (d->stride[i][2] >= 1 << 27) return GDN2_ERR_INVALID_ARGUMENT;
     }
     if (!o || !aligned16(o)) return GDN2_ERR_INVALID_ARGUMENT;
     for (int j = 0; j < 3; ++j)
@@ -321,7 +727,7 @@ extern "C" gdn2_status gdn2_recurrent(const gdn2_rec_desc* d, const void* q, con
   p.H = d->H; p.L = d->L; p.n_states = d->n_states;
   p.scale = d->scale; p.clip = d->clip;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (el == 2) launch<__nv_bfloat16>(p, d->B * d->H, st);
-  else launch<float>(p, d->B * d->H, st);
-  return cudaGetLastError() == cudaSuccess ? GDN2_OK : GDN2_ERR_CUDA;
+  float* rec = static_cast<float*>(workspace);
+  const cudaError_t e = el == 2 ? launch<__nv_bfloat16>(p, d->B * d->H, rec, st) : launch<float>(p, d->B * d->H, rec, st);
+  return e == cudaSuccess ? GDN2_OK : GDN2_ERR_CUDA;
 }

@@ -222,7 +222,8 @@ gdn2_status gdn2_prologue_bwd(const float* y, int64_t B, int64_t L, int64_t H, i
  * o and the final states are sanitized at clip.  It equals gdn2_fwd with wy_eps = 0. */
 typedef struct gdn2_rec_desc {
   int32_t B, H, L, D;     /* L >= 0, D == 128 */
-  int64_t stride[6][3];   /* element strides of q, k, v, w, b, g over B, H, L: multiples of 16 bytes */
+  int64_t stride[6][3];   /* element strides of q, k, v, w, b, g over B, H, L: multiples of 16 bytes,
+                             those over L below 2^27 */
   int64_t o_stride[3];    /* element strides of o over B, H, L: multiples of 4 */
   int32_t n_states;       /* rows of h0 */
   int32_t in_dtype;       /* gdn2_dtype of q..g */
@@ -236,12 +237,18 @@ typedef struct gdn2_rec_desc {
  *   lengths   (B) tokens of each sequence, 0..L, or NULL for L; o is zero past them
  *   o         fp32 over (B, H, L, D) in o_stride, h_out (B, H, D, D) fp32 contiguous.  h_out may
  *             be h0 itself when h_index is NULL and must not overlap it otherwise
+ *   workspace gdn2_recurrent_workspace_bytes(desc) bytes, 256-byte aligned (not used for L <= 1)
  *   flags     two uint32 words in device or mapped host memory: a kernel sets [0] to 1 when it
  *             sees g > 0 (outside domain I-1) and [1] to 1 when it sees an index >= n_states (it
  *             then starts from zeros) or a length outside 0..L (it then takes the nearer bound) */
 gdn2_status gdn2_recurrent(const gdn2_rec_desc* desc, const void* q, const void* k, const void* v, const void* w,
                            const void* b, const void* g, const float* h0, const int32_t* h_index,
-                           const int32_t* lengths, float* o, float* h_out, uint32_t* flags, void* stream);
+                           const int32_t* lengths, float* o, float* h_out, void* workspace, uint32_t* flags,
+                           void* stream);
+
+/* Bytes of scratch for one call, free once its work has run (0 for L <= 1 and for a descriptor that
+ * gdn2_recurrent rejects). */
+size_t gdn2_recurrent_workspace_bytes(const gdn2_rec_desc* desc);
 
 typedef enum gdn2_act { GDN2_ACT_NONE = 0, GDN2_ACT_GELU_TANH = 1 } gdn2_act;
 

@@ -74,7 +74,7 @@ def test_entry_points_reject_bad_arguments():
     """Everything is refused before a launch, so no GPU is needed; pointers are never followed."""
     lib, inv, uns, at = _lib.load(), _lib.ERR_INVALID_ARGUMENT, _lib.ERR_UNSUPPORTED, 4096
 
-    def rec(ptr=at, h0=at, idx=0, hout=at * 2, flags=at, **kw):
+    def rec(ptr=at, h0=at, idx=0, hout=at * 2, ws=at, flags=at, **kw):
         d = _lib.RecDesc()
         d.B, d.H, d.L, d.D, d.n_states, d.in_dtype, d.scale, d.clip = 2, 1, 3, 128, 2, 0, 1.0, 1e4
         for i in range(6):
@@ -89,11 +89,11 @@ def test_entry_points_reject_bad_arguments():
                 d.o_stride[2] = v
             else:
                 setattr(d, k, v)
-        return lib.gdn2_recurrent(ctypes.addressof(d), at, at, ptr, at, at, at, h0, idx, 0, at, hout, flags, 0)
+        return lib.gdn2_recurrent(ctypes.addressof(d), at, at, ptr, at, at, at, h0, idx, 0, at, hout, ws, flags, 0)
 
-    assert lib.gdn2_recurrent(0, *[at] * 13) == inv
+    assert lib.gdn2_recurrent(0, *[at] * 14) == inv
     for kw in (dict(B=0), dict(H=-1), dict(L=-1), dict(in_dtype=3), dict(clip=0.0), dict(ptr=0), dict(ptr=at + 4),
-               dict(stride=129), dict(stride=-128), dict(o_stride=2), dict(hout=0), dict(hout=at * 2 + 8), dict(flags=0),
+               dict(stride=129), dict(stride=-128), dict(o_stride=2), dict(hout=0), dict(hout=at * 2 + 8), dict(flags=0), dict(ws=0), dict(ws=at + 64),
                dict(n_states=1), dict(n_states=0), dict(h0=at * 2, idx=at), dict(h0=at + 4), dict(D=0)):
         assert rec(**kw) == inv, kw
     assert rec(D=64) == uns
