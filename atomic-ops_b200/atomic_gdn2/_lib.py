@@ -68,7 +68,8 @@ EXPORTS = ("gdn2_residual_bytes", "gdn2_fwd_workspace_bytes", "gdn2_bwd_workspac
            "gdn2_set_batch_groups", "gdn2_get_batch_groups",
            "gdn2_status_string", "gdn2_selftest_gemm", "gdn2_profile_enable", "gdn2_profile_collect",
            "gdn2_fwd_noalloc", "gdn2_prologue_fwd", "gdn2_prologue_bwd", "gdn2_selftest_engine",
-           "gdn2_selftest_wait_timeout", "gdn2_recurrent", "gdn2_recurrent_workspace_bytes", "gdn2_w4_linear", "gdn2_beam_select",
+           "gdn2_selftest_wait_timeout", "gdn2_recurrent", "gdn2_recurrent_workspace_bytes", "gdn2_w4_linear",
+           "gdn2_w4_workspace_bytes", "gdn2_beam_select",
            "gdn2_beam_workspace_bytes")
 # kernel ids of gdn2_profile_collect
 KERNELS = ("fwd_intra", "fwd_scan", "fwd_out", "bwd_pre", "bwd_scan", "bwd_intra")
@@ -114,7 +115,9 @@ def _declare(lib):
     lib.gdn2_recurrent_workspace_bytes.argtypes = [P]
     lib.gdn2_recurrent.argtypes = [P] * 15      # descriptors of the serving operators are passed by address
     lib.gdn2_w4_linear.restype = ctypes.c_int
-    lib.gdn2_w4_linear.argtypes = [P] * 8
+    lib.gdn2_w4_linear.argtypes = [P] * 9
+    lib.gdn2_w4_workspace_bytes.restype = ctypes.c_size_t
+    lib.gdn2_w4_workspace_bytes.argtypes = [P]
     lib.gdn2_beam_workspace_bytes.restype = ctypes.c_size_t
     lib.gdn2_beam_workspace_bytes.argtypes = [P]
     lib.gdn2_beam_select.restype = ctypes.c_int

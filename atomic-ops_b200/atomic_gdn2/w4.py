@@ -34,17 +34,21 @@ class W4Weight:
 
     def integers(self) -> torch.Tensor:
         """Q (din, dout) int8."""
-        nb, kb = -(-self.dout // 16), -(-self.din // 64)
-        w = self.packed.view(nb, kb, 8, 4, 2, 2, 1)             # column, t, half, step, word
+        nb, kb = -(-self.dout // 32), -(-self.din // 128)
+        w = self.packed.view(nb, kb, 2, 2, 8, 4, 2, 2, 1)       # rows' half, columns' half, column, t, quarter, step
         sh = torch.arange(0, 32, 4, device=w.device, dtype=torch.int32)
-        n = ((w >> sh) & 15).view(nb, kb, 8, 4, 2, 2, 2, 2, 2)  # ..., e, f, c (nibble c + 2 f + 4 e)
-        n = n.permute(1, 4, 3, 5, 7, 6, 0, 8, 2)                # kb, half, t, step, f, e | nb, c, column
-        return (n.reshape(kb * 64, nb * 16)[:self.din, :self.dout] - 8).to(torch.int8)
+        n = ((w >> sh) & 15).view(nb, kb, 2, 2, 8, 4, 2, 2, 2, 2, 2)    # ..., e, f, c (nibble c + 2 f + 4 e)
+        n = n.permute(1, 2, 6, 5, 7, 9, 8, 0, 3, 10, 4)         # kb, half, quarter, t, step, f, e | nb, half, c, column
+        return (n.reshape(kb * 128, nb * 32)[:self.din, :self.dout] - 8).to(torch.int8)
 
     def dequantize(self) -> torch.Tensor:
         """W (din, dout) fp32."""
-        s = self.scales.permute(1, 0, 2).reshape(self.scales.shape[1], -1)[:, :self.dout].float()
-        return self.integers().float() * s.repeat_interleave(self.group, 0)[:self.din]
+        return self.integers().float() * self.group_scales().float().repeat_interleave(self.group, 0)[:self.din]
+
+    def group_scales(self) -> torch.Tensor:
+        """s (ceil(din / group), dout) bf16."""
+        s = self.scales.permute(1, 4, 0, 2, 5, 3)               # batch, per | block, half, c, column
+        return s.reshape(s.shape[0] * s.shape[1], -1)[:-(-self.din // self.group), :self.dout]
 
 
 def pack_w4(q: torch.Tensor, scales: torch.Tensor, group: int = 64) -> W4Weight:
@@ -62,16 +66,17 @@ def pack_w4(q: torch.Tensor, scales: torch.Tensor, group: int = 64) -> W4Weight:
     lo, hi = torch.stack(torch.aminmax(q)).tolist()
     if lo < -8 or hi > 7:
         raise ValueError(f"q has values in [{lo}, {hi}], outside [-8, 7]")
-    nb, kb = -(-dout // 16), -(-din // 64)
-    n = torch.full((kb * 64, nb * 16), 8, dtype=torch.uint8, device=q.device)
+    nb, kb = -(-dout // 32), -(-din // 128)
+    n = torch.full((kb * 128, nb * 32), 8, dtype=torch.uint8, device=q.device)
     n[:din, :dout] = (q + 8).to(torch.uint8)
-    # rows 64 kb + 32 half + 8 t + 4 step + 2 f + e, columns 16 nb + 8 c + column
-    n = n.view(kb, 2, 4, 2, 2, 2, nb, 2, 8).permute(6, 0, 8, 2, 1, 3, 5, 4, 7).reshape(nb, kb, 8, 4, 2, 2, 8)
-    by = n[..., 0::2] | (n[..., 1::2] << 4)
-    packed = by.contiguous().view(torch.int32).reshape(nb, kb, 32, 4)
-    s = torch.zeros(scales.shape[0], nb * 16, dtype=torch.bfloat16, device=q.device)
-    s[:, :dout] = scales
-    s = s.view(-1, nb, 16).permute(1, 0, 2).contiguous()
+    # rows 128 kb + 64 half + 32 quarter + 8 t + 4 step + 2 f + e, columns 32 nb + 16 half + 8 c + column
+    n = n.view(kb, 2, 2, 4, 2, 2, 2, nb, 2, 2, 8).permute(7, 0, 1, 8, 10, 3, 2, 4, 6, 5, 9)
+    n = n.reshape(nb, kb, 4, 32, 4, 8)                          # block, batch, tile, lane, step, nibble
+    packed = (n[..., 0::2] | (n[..., 1::2] << 4)).contiguous().view(torch.int32).squeeze(-1)
+    per = 128 // group
+    s = torch.zeros(kb * per, nb * 32, dtype=torch.bfloat16, device=q.device)
+    s[:scales.shape[0], :dout] = scales
+    s = s.view(kb, per, nb, 2, 2, 8).permute(2, 0, 3, 5, 1, 4).contiguous()  # block, batch, half, column, per, c
     return W4Weight(packed, s, din, dout, group)
 
 
@@ -117,8 +122,8 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, bias=None, *, act=None, residua
     grads = x.requires_grad
     x2 = x if len(shape) == 2 else x.reshape(-1, din)
     M = x2.shape[0]
-    if din > 1 and x2.stride(1) != 1:
-        x2 = x2.contiguous()
+    if din > 1 and x2.stride(1) != 1 or x2.data_ptr() % 16:
+        x2 = x2.clone(memory_format=torch.contiguous_format)
     y = torch.empty((*shape[:-1], dout), dtype=dt, device=dev)
     bp = rp = rs = 0
     if bias is not None:
@@ -148,12 +153,15 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, bias=None, *, act=None, residua
         d.dtype = _lib.BF16 if dt == torch.bfloat16 else _lib.F32
         d.act = _ACTS[act]
         d.x_stride, d.res_stride, d.y_stride = x2.stride(0), rs, dout
+        at = ctypes.addressof(d)
         if len(_descs) > 1024:
             _descs.clear()
-        desc = _descs[key] = (d, ctypes.addressof(d))
+        desc = _descs[key] = (d, at, _lib.load().gdn2_w4_workspace_bytes(at))
+    ws = torch.empty(desc[2], dtype=torch.uint8, device=dev) if desc[2] else None
     with torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else pipeline._NULL:
         rc = _lib.load().gdn2_w4_linear(desc[1], x2.data_ptr(), weight.packed.data_ptr(), weight.scales.data_ptr(),
-                                        bp, rp, y.data_ptr(), _raw_stream(dev.index))
+                                        bp, rp, y.data_ptr(), 0 if ws is None else ws.data_ptr(),
+                                        _raw_stream(dev.index))
     if rc:
         _lib.check(rc, "gdn2_w4_linear")
     return y

@@ -262,15 +262,23 @@ typedef struct gdn2_w4_desc {
   int64_t x_stride, res_stride, y_stride;  /* element strides between rows */
 } gdn2_w4_desc;
 
-/*   packed    ceil(N / 16) * ceil(K / 64) tiles of 512 bytes, 16-byte aligned: tile (i, j), i the
- *             slower, holds columns 16 i.. and rows 64 j..; its 32-bit word 4 l + s (lane l in
- *             0..31, s in 0..3) holds eight nibbles Q + 8: nibble c + 4 e + 2 f is column
- *             16 i + l / 4 + 8 c, row 64 j + 32 (s / 2) + 8 (l % 4) + 4 (s % 2) + 2 f + e (c, e, f
- *             in 0..1); 8 where the column or row is past the weight's
- *   scales    bf16 (ceil(N / 16), ceil(K / group), 16): column 16 i + c, group g at [i][g][c]
- *   bias      (N) fp32 or NULL;  residual (M, N) or NULL */
+/*   packed    ceil(N / 32) x ceil(K / 128) blocks of 2048 bytes, 16-byte aligned: block (i, j), i the
+ *             slower, holds columns 32 i.. and rows 128 j.. as [2 halves of the rows][2 halves of the
+ *             columns] tiles of 512 bytes (16 columns x 64 rows); word 4 l + s of a tile (lane l in
+ *             0..31, s in 0..3) holds eight nibbles Q + 8: nibble c + 4 e + 2 f is column l / 4 + 8 c,
+ *             row 32 (s / 2) + 8 (l % 4) + 4 (s % 2) + 2 f + e of the tile (c, e, f in 0..1); 8 where
+ *             the column or row is past the weight's
+ *   scales    bf16, 16-byte aligned: [ceil(N / 32)][ceil(K / 128)][2][8][per][2] with per = 128 /
+ *             group: column 32 i + 16 h + c + 8 e, group per * j + r at [i][j][h][c][r][e]; any finite
+ *             value past the weight's columns and groups
+ *   x         16-byte aligned, rows of any stride;  bias (N) fp32 or NULL;  residual (M, N) or NULL
+ *   workspace gdn2_w4_workspace_bytes(desc) bytes, 16-byte aligned (NULL where that is 0) */
 gdn2_status gdn2_w4_linear(const gdn2_w4_desc* desc, const void* x, const void* packed, const void* scales,
-                           const float* bias, const void* residual, void* y, void* stream);
+                           const float* bias, const void* residual, void* y, void* workspace, void* stream);
+
+/* Bytes of scratch for one call, free once its work has run (0 where x is read in place, and for a
+ * descriptor that gdn2_w4_linear rejects). */
+size_t gdn2_w4_workspace_bytes(const gdn2_w4_desc* desc);
 
 /* One step of beam search: the K best continuations of each of B sequences from the logits of
  * their K beams (K <= 32).  total = score + (x - max) - log sum exp(x - max).  Order: inside a beam

@@ -18,21 +18,26 @@ def test_pack_round_trip(din, dout, group):
     q = torch.randint(-8, 8, (din, dout), generator=gen, dtype=torch.int8)
     s = torch.rand(-(-din // group), dout, generator=gen).to(torch.bfloat16)
     w = pack_w4(q, s, group)
-    assert w.packed.numel() == -(-dout // 16) * -(-din // 64) * 128
-    assert torch.equal(w.integers(), q)
+    assert w.packed.numel() == -(-dout // 32) * -(-din // 128) * 512
+    assert torch.equal(w.integers(), q) and torch.equal(w.group_scales(), s)
     assert torch.equal(w.dequantize(), q.float() * s.float().repeat_interleave(group, 0)[:din])
 
 
 def test_packed_layout_is_the_documented_one():
-    """include/gdn2_b200.h: nibble c + 4 e + 2 f of word 4 l + s of tile (i, j)."""
-    din, dout, group = 192, 40, 64
+    """include/gdn2_b200.h: nibble c + 4 e + 2 f of word 4 l + s of tile (u, v) of block (i, j)."""
+    din, dout, group = 320, 72, 64
     q = torch.randint(-8, 8, (din, dout), generator=torch.Generator().manual_seed(3), dtype=torch.int8)
-    w = pack_w4(q, torch.ones(3, dout, dtype=torch.bfloat16), group).packed.view(-1).tolist()
-    for i, j, l, s, c, e, f in [(0, 0, 0, 0, 0, 0, 0), (1, 2, 31, 3, 1, 1, 1), (2, 1, 13, 2, 0, 1, 0), (2, 0, 9, 1, 1, 0, 1)]:
-        col, row = 16 * i + l // 4 + 8 * c, 64 * j + 32 * (s // 2) + 8 * (l % 4) + 4 * (s % 2) + 2 * f + e
-        word = w[(i * 3 + j) * 128 + 4 * l + s]
-        nib = (word >> (4 * (c + 4 * e + 2 * f))) & 15
-        assert nib == (int(q[row, col]) + 8 if col < dout else 8)
+    sc = torch.rand(5, dout, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16)
+    w = pack_w4(q, sc, group)
+    words, scales = w.packed.view(-1).tolist(), w.scales.float().view(-1).tolist()
+    for i, j, u, v, l, s, c, e, f in [(0, 0, 0, 0, 0, 0, 0, 0, 0), (1, 1, 1, 1, 31, 3, 1, 1, 1), (2, 2, 0, 0, 13, 2, 0, 1, 0),
+                                      (2, 1, 1, 1, 9, 1, 1, 0, 1), (0, 2, 1, 0, 17, 2, 1, 1, 0)]:
+        col = 32 * i + 16 * v + l // 4 + 8 * c
+        row = 128 * j + 64 * u + 32 * (s // 2) + 8 * (l % 4) + 4 * (s % 2) + 2 * f + e
+        nib = (words[((i * 3 + j) * 4 + u * 2 + v) * 128 + 4 * l + s] >> (4 * (c + 4 * e + 2 * f))) & 15
+        assert nib == (int(q[row, col]) + 8 if col < dout and row < din else 8)
+        if col < dout and row < din:  # [i][j][v][column][row half][c]
+            assert scales[((((i * 3 + j) * 2 + v) * 8 + l // 4) * 2 + u) * 2 + c] == float(sc[row // 64, col])
 
 
 def test_quantize_error_is_half_a_step():
@@ -41,7 +46,7 @@ def test_quantize_error_is_half_a_step():
     W = torch.randn(200, 50, generator=torch.Generator().manual_seed(1))
     W[32:64, 3] = 0.0
     w = quantize_w4(W, 32)
-    step = w.scales.permute(1, 0, 2).reshape(7, -1)[:, :50].float().repeat_interleave(32, 0)[:200]
+    step = w.group_scales().float().repeat_interleave(32, 0)[:200]
     assert bool(((w.dequantize() - W).abs() <= step * (0.5 + 7 / 256)).all())
     assert bool((w.dequantize()[32:64, 3] == 0).all())
 
@@ -98,17 +103,18 @@ def test_entry_points_reject_bad_arguments():
         assert rec(**kw) == inv, kw
     assert rec(D=64) == uns
 
-    def w4(x=at, packed=at, scales=at, y=at, **kw):
+    def w4(x=at, packed=at, scales=at, y=at, ws=0, **kw):
         d = _lib.W4Desc()
         d.M, d.K, d.N, d.group, d.x_stride, d.y_stride = 1, 64, 16, 64, 64, 16
         for k, v in kw.items():
             setattr(d, k, v)
-        return lib.gdn2_w4_linear(ctypes.addressof(d), x, packed, scales, 0, 0, y, 0)
+        return lib.gdn2_w4_linear(ctypes.addressof(d), x, packed, scales, 0, 0, y, ws, 0)
 
     for kw in (dict(M=0), dict(K=0), dict(N=-1), dict(dtype=2), dict(act=5), dict(x=0), dict(packed=0), dict(packed=at + 8),
-               dict(scales=0), dict(y=0), dict(x_stride=-1), dict(y_stride=15)):
+               dict(scales=0), dict(scales=at + 2), dict(x=at + 8), dict(y=0), dict(x_stride=65),
+               dict(x_stride=65, ws=at + 8), dict(x_stride=-1), dict(y_stride=15)):
         assert w4(**kw) == inv, kw
-    assert w4(group=48) == uns and lib.gdn2_w4_linear(0, *[at] * 7) == inv
+    assert w4(group=48) == uns and lib.gdn2_w4_linear(0, *[at] * 8) == inv
 
     def beam(logits=at, ws=at, **kw):
         d = _lib.BeamDesc()
