@@ -16,14 +16,13 @@
 // k = 32 (s / 2) + 8 t + 4 (s % 2) + j, nibble r + 4 (j % 2), r = 2 (j / 2) + c, is column g + 8 c.
 // The sum over k may run in any order: this one puts the x values that a lane needs for two k-steps
 // next to one another, so that rows of x on 16 bytes are read as they are.
-#include <cstdlib>
-
 #include "gdn2_common.cuh"
 
 namespace gdn2 {
 namespace {
 
 constexpr int kW4Warps = 8;
+constexpr int kSmCount = 148;  // of a B200
 
 struct W4Params {
   const void* x;
@@ -138,6 +137,10 @@ __device__ __forceinline__ void load_quarter(const W4Params& p, const T* const x
   }
 }
 
+// Two CTAs on an SM where the registers allow.
+template <int kTerms, int kMB>
+constexpr bool kTwoCtas = kMB == 1 || (kTerms == 1 && kMB == 2);
+
 // A warp computes 32 columns for 8 kMB rows over its share of the batches of 128 rows; a CTA has kMB
 // warps side by side (they share x through L1) and 8 / kMB that split the batches, and the CTAs of a
 // cluster split them further.  kPer: scales of a column per batch.
@@ -146,7 +149,7 @@ __device__ __forceinline__ void load_quarter(const W4Params& p, const T* const x
 // of x with -136 in every place, is added to each group's sum.  The cancellation costs five
 // bits of fp32 there, 2^-19 of the result, far below its rounding to bf16.
 template <class T, int kTerms, int kMB, int kPer, bool kPacked>
-__global__ void __launch_bounds__(kW4Warps * 32, kMB == 1 ? 2 : 1) w4_kernel(W4Params p) {
+__global__ void __launch_bounds__(kW4Warps * 32, kTwoCtas<kTerms, kMB> ? 2 : 1) w4_kernel(W4Params p) {
   constexpr int kWN = kMB, kWK = kW4Warps / kWN, kCols = kWN * 32, kRows = kMB * 8 + 1;
   constexpr bool kExact = kTerms > 1 || kMB > 1;
   __shared__ float part[kW4Warps * 32 * kRows];
@@ -323,16 +326,20 @@ int row_blocks(int M) { return M <= 8 ? 1 : M <= 16 ? 2 : 4; }
 bool use_terms(const gdn2_w4_desc* d) {
   const int el = d->dtype == GDN2_BF16 ? 2 : 4;
   if (d->K % 8 || (d->x_stride * el) % 16) return true;
-  const int v = getenv("W4_TERMS") ? atoi(getenv("W4_TERMS")) : 0;
-  if (v) return v == 1;
+  // Measured with and without: fp32 512 x 4608 4.0 / 2.7 us, 4096 x 4096 7.9 / 8.3, 8192 x 8192 19.3 / 24.2
+  // (1 row) and 47 / 79 (32 rows).
   return el == 4 && (long long)d->K * d->N >= (4 << 20);
 }
 
 template <class T, int kTerms, int kMB, int kPer, bool kPacked>
 cudaError_t launch_one(const W4Params& p, cudaStream_t st) {
   const int blocks = ((p.N + 31) / 32 + kMB - 1) / kMB, rows = (p.M + 8 * kMB - 1) / (8 * kMB);
+  // The rows of the weight are split over a cluster while the CTAs stay within one for each SM (two for
+  // 9 to 16 bf16 rows, whose CTAs fit twice) and every warp has a batch: a CTA costs about 2 us besides
+  // its batches.  Measured with 1 / 2 / 8 CTAs: 16384 x 128, 4 rows 12.6 / 8.3 / 4.3 us; 8192 x 8192, 256
+  // CTAs, 12.5 / 15.4 us with 1 / 2.
+  const int most = kSmCount * (kTerms == 1 && kMB == 2 ? 2 : 1);
   int ks = 1;
-  const int most = getenv("W4_KS") ? atoi(getenv("W4_KS")) : 148;
   while (ks < 8 && blocks * rows * ks * 2 <= most && ks * (kW4Warps / kMB) < p.NB) ks *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(blocks, ks, rows);
