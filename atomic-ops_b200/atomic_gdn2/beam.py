@@ -73,10 +73,10 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished=None, *, eo
     rows = torch.empty((B, K), dtype=torch.int32, device=dev)
     tokens = torch.empty((B, K), dtype=torch.int32, device=dev)
     done = torch.empty((B, K), dtype=torch.bool, device=dev)
-    ws = torch.empty(desc[2], dtype=torch.uint8, device=dev)
+    ws = torch.empty(desc[2], dtype=torch.uint8, device=dev) if desc[2] else None
     with torch.cuda.device(dev) if dev.index != torch.cuda.current_device() else pipeline._NULL:
         rc = lib.gdn2_beam_select(desc[1], logits.data_ptr(), scores.data_ptr(), fp, out.data_ptr(), rows.data_ptr(),
-                                  tokens.data_ptr(), done.data_ptr(), ws.data_ptr(), _raw_stream(dev.index))
+                                  tokens.data_ptr(), done.data_ptr(), 0 if ws is None else ws.data_ptr(), _raw_stream(dev.index))
     if rc:
         _lib.check(rc, "gdn2_beam_select")
     return out, rows, tokens, done

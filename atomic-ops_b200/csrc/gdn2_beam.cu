@@ -6,11 +6,15 @@
 // the largest finite value; a beam whose logits are all -inf offers totals of -inf.  A finished
 // beam offers itself alone: (eos, its score).
 //
-// The logits are read once.  A warp keeps the R = min(K, V) best of what it has seen as a sorted
-// list over its lanes (R <= 32), together with the running maximum and sum of the softmax; most
-// values are below the list's last, which one comparison and a vote find out.  Keys join the
-// order-preserving bits of the logit with the inverted index, so that no two are equal and the
-// result does not depend on the order of insertion.
+// The logits are read once, which bounds the call where there are many; the exponentials (a quarter
+// of an SM's lanes a cycle) come next.  A warp takes 256 values at a time, eight to a lane, and a lane
+// keeps the running maximum and sum of its values' softmax.  With R = min(K, V) <= 32, R lanes' maxima
+// bound the R best values from below; only the few lanes whose maximum reaches the bound are looked
+// through again, value by value, into a sorted list over the warp's lanes.  Keys join the order-preserving bits of the logit with the inverted index,
+// so that no two are equal and the result does not depend on the order of insertion.
+//
+// Small vocabularies take one launch (a CTA per sequence); else a first launch reads the logits, a
+// long row's slices spread over CTAs, and a second one, started while the first still runs, joins them.
 #include "gdn2_common.cuh"
 
 namespace gdn2 {
@@ -45,14 +49,39 @@ __device__ __forceinline__ u64 make_key(float x, uint32_t index) {
 }
 __device__ __forceinline__ float key_value(u64 k) { return from_ordered((uint32_t)(k >> 32)); }
 __device__ __forceinline__ uint32_t key_index(u64 k) { return ~(uint32_t)k; }
-__device__ __forceinline__ float clean(float x) {
-  return x != x ? -INFINITY : fminf(x, 3.402823466e38f);
+__device__ __forceinline__ float clean(float x) {  // NaN: -inf; +inf: the largest finite value
+  return fminf(fmaxf(x, -INFINITY), 3.402823466e38f);
+}
+
+// Sorts 32 keys over the lanes, largest first (bitonic).
+__device__ __forceinline__ u64 sort32(u64 k, int lane) {
+#pragma unroll
+  for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+    for (int m = size >> 1; m > 0; m >>= 1) {
+      const u64 other = __shfl_xor_sync(kFull, k, m);
+      const bool down = (lane & size) == 0, low = (lane & m) == 0;
+      k = (down == low) == (k > other) ? k : other;
+    }
+  return k;
 }
 
 // Inserts each lane's key (0: none) that is above the list's R-th into the warp's sorted list.
 __device__ __forceinline__ void insert(u64& list, u64 key, int R, int lane) {
   u64 last = __shfl_sync(kFull, list, R - 1);
   unsigned todo = __ballot_sync(kFull, key > last);
+  if (__popc(todo) > 6) {  // sort them and take the upper half of the two lists' merge
+    const u64 k = sort32(key, lane);
+    const u64 back = __shfl_sync(kFull, k, 31 - lane);
+    u64 m = list > back ? list : back;
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+      const u64 other = __shfl_xor_sync(kFull, m, d);
+      m = ((lane & d) == 0) == (m > other) ? m : other;
+    }
+    list = m;
+    return;
+  }
   while (todo) {
     const int src = __ffs(todo) - 1;
     todo &= todo - 1;
@@ -62,8 +91,17 @@ __device__ __forceinline__ void insert(u64& list, u64 key, int R, int lane) {
     const int pos = __popc(above);
     if (lane == pos) list = k;
     else if (lane > pos) list = up;
-    last = __shfl_sync(kFull, list, R - 1);
-    todo &= __ballot_sync(kFull, key > last);
+  }
+}
+// The best of n keys in memory (0: none), into the warp's list.
+__device__ __forceinline__ void gather(u64& list, const u64* keys, int n, int R, int lane) {
+  for (int i = 0; i < n; i += 128) {
+    u64 k[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) k[j] = i + j * 32 + lane < n ? keys[i + j * 32 + lane] : 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i + j * 32 < n) insert(list, k[j], R, lane);
   }
 }
 
@@ -73,88 +111,212 @@ __device__ __forceinline__ float2 join(float2 a, float2 b) {
   if (m == -INFINITY) return make_float2(m, 0.f);
   return make_float2(m, a.y * expf(a.x - m) + b.y * expf(b.x - m));
 }
+__device__ __forceinline__ float2 join_warp(float2 st) {
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1)
+    st = join(st, make_float2(__shfl_xor_sync(kFull, st.x, m), __shfl_xor_sync(kFull, st.y, m)));
+  return st;
+}
+// e^x for x <= 0, to about 2^-22 of the value
+__device__ __forceinline__ float exp_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+  return y;
+}
+
+// The lane's share of x[v0, v1): the warp takes pieces of 256 values, `first` of `stride`, and a lane
+// every 32nd of a piece.  That needs no alignment of the rows, and which values are summed in which
+// order depends on their place in the row alone.  scan() returns the lane's maximum and sum; the
+// maximum is also the lane's best candidate.
+struct Pieces {
+  int at, hop, count;  // this lane's first value, distance between its pieces, pieces of the warp
+};
+__device__ __forceinline__ Pieces pieces(int v0, int v1, int first, int stride, int lane) {
+  const int start = v0 + first * 256;
+  return {start + lane, stride * 256, start < v1 ? (v1 - start + stride * 256 - 1) / (stride * 256) : 0};
+}
+__device__ __forceinline__ uint32_t bits(const float* p) { return __float_as_uint(__ldg(p)); }
+__device__ __forceinline__ uint32_t bits(const __nv_bfloat16* p) {
+  return (uint32_t)__ldg(reinterpret_cast<const unsigned short*>(p)) << 16;
+}
+template <class T>
+__device__ __forceinline__ float2 scan(const T* x, int v1, const Pieces& pc) {
+  float m = -INFINITY, sum = 0.f;
+  constexpr int kG = 2;  // pieces that are on their way while as many are worked on
+  uint32_t next[kG][8];
+  auto fetch = [&](int i) {
+#pragma unroll
+    for (int g = 0; g < kG; ++g)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int at = pc.at + (i + g) * pc.hop + j * 32;
+        next[g][j] = i + g < pc.count && at < v1 ? bits(x + at) : 0xff800000u;
+      }
+  };
+  fetch(0);
+  for (int i = 0; i < pc.count; i += kG) {
+    float now[kG][8];
+#pragma unroll
+    for (int g = 0; g < kG; ++g)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) now[g][j] = __uint_as_float(next[g][j]);
+    fetch(i + kG);
+#pragma unroll
+    for (int g = 0; g < kG; ++g) {
+      for (int again = 0; again < 2; ++again) {
+        float top = now[g][0];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) top = fmaxf(top, now[g][j]);
+        const float big = fmaxf(m, top);
+        float part = sum;
+        if (big > m) part *= exp_fast(m - big);
+        if (big > -INFINITY) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) part += exp_fast(now[g][j] - big);
+        }
+        if (part == part) {
+          m = big;
+          sum = part;
+          break;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) now[g][j] = clean(now[g][j]);  // a NaN or +inf among the values
+      }
+    }
+  }
+  return make_float2(m, sum);
+}
+// The q-th largest of the lanes' values.
+__device__ __forceinline__ float nth(float v, int q, int lane) {
+  if (q > 4) return key_value(__shfl_sync(kFull, sort32(make_key(v, lane), lane), q - 1));
+  float r = v;
+  for (int i = 0; i < q; ++i) {
+    r = v;
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) r = fmaxf(r, __shfl_xor_sync(kFull, r, m));
+    const unsigned who = __ballot_sync(kFull, v == r);
+    if (lane == __ffs(who) - 1) v = -INFINITY;
+  }
+  return r;
+}
+// The warp's candidates into its list: the values, `least` or more, of the lanes whose maximum is that;
+// the whole warp reads a lane's values again.
+template <class T>
+__device__ __forceinline__ void collect(u64& list, const T* x, int v1, const Pieces& pc, float m, float least, int R,
+                                        int lane) {
+  unsigned who = __ballot_sync(kFull, m >= least);
+  const int own = pc.at - lane;
+  while (who) {
+    const int from = own + __ffs(who) - 1;
+    who &= who - 1;
+    for (int j = lane; j < (pc.count * 8 + 31) / 32 * 32; j += 32) {
+      const int at = from + (j >> 3) * pc.hop + (j & 7) * 32;
+      u64 key = 0;
+      if (j < pc.count * 8 && at < v1) {
+        const float v = clean(ld1(x + at));
+        if (v >= least) key = make_key(v, at);
+      }
+      insert(list, key, R, lane);
+    }
+  }
+}
 
 constexpr int kScanWarps = 8;
 
 // One row's slice: list and softmax statistics into the workspace.
 template <class T>
 __global__ void __launch_bounds__(kScanWarps * 32) beam_scan_kernel(BeamParams p) {
-  __shared__ u64 lists[kScanWarps][32];
+  __shared__ u64 lists[kScanWarps * 32];
   __shared__ float2 stats[kScanWarps];
+  __shared__ float bound[kScanWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.x, split = blockIdx.y;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (p.finished && p.finished[row]) return;
   const T* x = static_cast<const T*>(p.logits) + (row / p.K) * p.sb + (row % p.K) * p.sk;
   const int v0 = split * p.slice, v1 = min(p.V, v0 + p.slice);
-  u64 list = 0;
-  float2 st = make_float2(-INFINITY, 0.f);
-  for (int v = v0 + warp * 32; v < v1; v += kScanWarps * 32) {
-    const int i = v + lane;
-    u64 key = 0;
-    if (i < v1) {
-      const float f = clean(ld1(x + i));
-      key = make_key(f, i);
-      if (f > st.x) {
-        st.y = st.y * expf(st.x - f) + 1.f;
-        st.x = f;
-      } else if (f > -INFINITY) {
-        st.y += expf(f - st.x);
-      }
-    }
-    insert(list, key, p.R, lane);
-  }
-#pragma unroll
-  for (int m = 16; m > 0; m >>= 1)
-    st = join(st, make_float2(__shfl_xor_sync(kFull, st.x, m), __shfl_xor_sync(kFull, st.y, m)));
-  lists[warp][lane] = lane < p.R ? list : 0;
+  const Pieces pc = pieces(v0, v1, warp, kScanWarps, lane);
+  float2 st = scan(x, v1, pc);
+  // R lanes' maxima are at or above the least of the warps' q-th largest, so the slice's R best are too
+  const float top = st.x, mine = nth(top, (p.R + kScanWarps - 1) / kScanWarps, lane);
+  if (lane == 0) bound[warp] = mine;
+  st = join_warp(st);
   if (lane == 0) stats[warp] = st;
   __syncthreads();
+  float least = bound[0];
+#pragma unroll
+  for (int i = 1; i < kScanWarps; ++i) least = fminf(least, bound[i]);
+  u64 list = 0;
+  collect(list, x, v1, pc, top, least, p.R, lane);
+  if (lane < p.R) lists[warp * p.R + lane] = list;
+  __syncthreads();
   if (warp) return;
-#pragma unroll 1
-  for (int i = 1; i < kScanWarps; ++i) {
-    insert(list, lists[i][lane], p.R, lane);
-    st = join(st, stats[i]);
-  }
+  list = 0;
+  gather(list, lists, kScanWarps * p.R, p.R, lane);
+  st = join_warp(lane < kScanWarps ? stats[lane] : make_float2(-INFINITY, 0.f));
   const size_t at = (size_t)row * p.splits + split;
   if (lane < p.R) p.lists[at * p.R + lane] = list;
   if (lane == 0) p.stats[at] = st;
 }
 
-// One sequence: joins its beams' slices (a warp per beam) and selects over them.
-__global__ void __launch_bounds__(1024) beam_pick_kernel(BeamParams p) {
+// One sequence: joins its beams' parts, `per` warps to a beam, and selects over them.  kWhole: reads
+// the logits itself.
+template <class T, bool kWhole>
+__global__ void __launch_bounds__(1024) beam_pick_kernel(BeamParams p, int per) {
+  __shared__ u64 lists[32 * 32];
+  __shared__ float2 stats[32];
   __shared__ float total[32 * 32];
   __shared__ int token[32 * 32];
-  const int tid = threadIdx.x, lane = tid & 31, k = tid >> 5;
-  const int b = blockIdx.x, row = b * p.K + k;
-  const float score0 = p.scores[row];
-  const float score = score0 != score0 ? -INFINITY : score0;
-  if (p.finished && p.finished[row]) {
-    total[k * 32 + lane] = lane == 0 ? score : -INFINITY;
-    token[k * 32 + lane] = p.eos;
-  } else {
-    u64 list = 0;
-    float2 st = make_float2(-INFINITY, 0.f);
-    for (int s = 0; s < p.splits; ++s) {
-      const size_t at = (size_t)row * p.splits + s;
-      insert(list, lane < p.R ? p.lists[at * p.R + lane] : 0, p.R, lane);
-      st = join(st, p.stats[at]);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int k = warp / per, part = warp % per, row = blockIdx.x * p.K + k;
+  const bool done = p.finished && p.finished[row];
+  const float score0 = p.scores[row], score = score0 != score0 ? -INFINITY : score0;
+  if constexpr (!kWhole) asm volatile("griddepcontrol.wait;" ::: "memory");
+  u64 list = 0;
+  float2 st = make_float2(-INFINITY, 0.f);
+  if (!done) {
+    if constexpr (kWhole) {
+      const T* x = static_cast<const T*>(p.logits) + blockIdx.x * p.sb + k * p.sk;
+      const Pieces pc = pieces(0, p.V, part, per, lane);
+      st = scan(x, p.V, pc);
+      // see beam_scan_kernel; here each warp goes by its own lanes
+      collect(list, x, p.V, pc, st.x, nth(st.x, p.R, lane), p.R, lane);
+    } else {
+      const int n = (p.splits + per - 1) / per, s0 = part * n, s1 = min(p.splits, s0 + n);
+      const size_t at = (size_t)row * p.splits;
+      for (int s = s0 + lane; s < s1; s += 32) st = join(st, p.stats[at + s]);
+      if (s0 < s1) gather(list, p.lists + (at + s0) * p.R, (s1 - s0) * p.R, p.R, lane);
     }
+    st = join_warp(st);
+  }
+  if (per > 1) {
+    if (lane < p.R) lists[warp * p.R + lane] = list;
+    if (lane == 0) stats[warp] = st;
+    __syncthreads();
+    if (part == 0) {
+      list = 0;
+      gather(list, lists + warp * p.R, per * p.R, p.R, lane);
+      st = join_warp(lane < per ? stats[warp + lane] : make_float2(-INFINITY, 0.f));
+    }
+  }
+  if (part == 0) {
     float t = -INFINITY;
-    if (lane < p.R && st.x > -INFINITY) {
+    if (done) {
+      t = lane == 0 ? score : t;
+    } else if (lane < p.R && st.x > -INFINITY) {
       t = score + ((key_value(list) - st.x) - logf(st.y));
       if (t != t) t = -INFINITY;
     }
     total[k * 32 + lane] = t;
-    token[k * 32 + lane] = (int)key_index(list);
+    token[k * 32 + lane] = done ? p.eos : (int)key_index(list);
   }
   __syncthreads();
-  if (k) return;
-  u64 best = 0;
-  for (int j = 0; j < p.K; ++j)  // a beam's totals fall with the rank: ranks past R never matter
-    insert(best, lane < p.R ? make_key(total[j * 32 + lane], j * 32 + lane) : 0, p.K, lane);
+  if (warp) return;
+  u64 best = lane < p.R ? make_key(total[lane], lane) : 0;  // a beam's totals fall with the rank
+  for (int j = 1; j < p.K; ++j) insert(best, lane < p.R ? make_key(total[j * 32 + lane], j * 32 + lane) : 0, p.K, lane);
   if (lane < p.K) {
-    const int c = (int)key_index(best), tok = token[c], parent = b * p.K + c / 32;
-    const int at = b * p.K + lane;
+    const int c = (int)key_index(best), tok = token[c], parent = blockIdx.x * p.K + c / 32;
+    const int at = blockIdx.x * p.K + lane;
     p.out_scores[at] = total[c];
     p.out_row[at] = parent;
     p.out_token[at] = tok;
@@ -162,10 +324,14 @@ __global__ void __launch_bounds__(1024) beam_pick_kernel(BeamParams p) {
   }
 }
 
+// Vocabularies up to this are read by the kernel that selects.
+constexpr int kWholeV = 8192;
+
 struct BeamPlan { int R, splits, slice; size_t stats, total; };
 BeamPlan beam_plan(const gdn2_beam_desc* d) {
   BeamPlan pl{};
   pl.R = d->K < d->V ? d->K : d->V;
+  if (d->V <= kWholeV) return pl;
   const long long rows = (long long)d->B * d->K;
   // enough slices to cover the GPU a few times over, none smaller than 4096 values
   long long want = rows >= 592 ? 1 : 592 / rows, most = (d->V + 4095) / 4096;
@@ -174,6 +340,31 @@ BeamPlan beam_plan(const gdn2_beam_desc* d) {
   pl.stats = ((size_t)rows * pl.splits * pl.R * 8 + 255) / 256 * 256;
   pl.total = pl.stats + (size_t)rows * pl.splits * 8;
   return pl;
+}
+template <class T>
+cudaError_t launch(const BeamParams& p, cudaStream_t st) {
+  int per = 32 / p.K;  // warps to a beam
+  if (p.splits == 0) {
+    const int most = p.V / 512;  // values of a warp, where there are warps enough
+    if (per > most) per = most > 1 ? most : 1;
+    beam_pick_kernel<T, true><<<p.B, p.K * per * 32, 0, st>>>(p, per);
+    return cudaGetLastError();
+  }
+  beam_scan_kernel<T><<<dim3(p.B * p.K, p.splits), kScanWarps * 32, 0, st>>>(p);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  const int most = (p.splits * p.R + 31) / 32;
+  if (per > most) per = most;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.B);
+  cfg.blockDim = dim3(p.K * per * 32);
+  cfg.stream = st;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, beam_pick_kernel<T, false>, p, per);
 }
 gdn2_status check_beam(const gdn2_beam_desc* d) {
   if (!d || d->B <= 0 || d->K <= 0 || d->V <= 0) return GDN2_ERR_INVALID_ARGUMENT;
@@ -196,10 +387,11 @@ extern "C" gdn2_status gdn2_beam_select(const gdn2_beam_desc* d, const void* log
   using namespace gdn2;
   const gdn2_status s = check_beam(d);
   if (s != GDN2_OK) return s;
-  if (!logits || !scores || !out_scores || !out_row || !out_token || !out_finished || !workspace ||
-      (reinterpret_cast<uintptr_t>(workspace) & 255u))
-    return GDN2_ERR_INVALID_ARGUMENT;
+  if (!logits || !scores || !out_scores || !out_row || !out_token || !out_finished) return GDN2_ERR_INVALID_ARGUMENT;
   const BeamPlan pl = beam_plan(d);
+  if (pl.total && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u))) return GDN2_ERR_INVALID_ARGUMENT;
+  const size_t el = d->dtype == GDN2_BF16 ? 2 : 4;
+  if (reinterpret_cast<uintptr_t>(logits) % el) return GDN2_ERR_INVALID_ARGUMENT;
   BeamParams p{};
   p.logits = logits; p.sb = d->stride_b; p.sk = d->stride_k;
   p.scores = scores; p.finished = finished;
@@ -208,9 +400,6 @@ extern "C" gdn2_status gdn2_beam_select(const gdn2_beam_desc* d, const void* log
   p.stats = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + pl.stats);
   p.B = d->B; p.K = d->K; p.V = d->V; p.R = pl.R; p.splits = pl.splits; p.slice = pl.slice; p.eos = d->eos;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const dim3 grid(d->B * d->K, pl.splits);
-  if (d->dtype == GDN2_BF16) beam_scan_kernel<__nv_bfloat16><<<grid, kScanWarps * 32, 0, st>>>(p);
-  else beam_scan_kernel<float><<<grid, kScanWarps * 32, 0, st>>>(p);
-  beam_pick_kernel<<<d->B, d->K * 32, 0, st>>>(p);
-  return cudaGetLastError() == cudaSuccess ? GDN2_OK : GDN2_ERR_CUDA;
+  const cudaError_t e = el == 2 ? launch<__nv_bfloat16>(p, st) : launch<float>(p, st);
+  return e == cudaSuccess ? GDN2_OK : GDN2_ERR_CUDA;
 }

@@ -297,7 +297,8 @@ size_t gdn2_beam_workspace_bytes(const gdn2_beam_desc* desc);
 
 /*   scores, out_scores (B, K) fp32;  finished (B, K) bytes or NULL for none;  out_finished (B, K);
  *   out_row (B, K) b * K + the beam that is continued (a row of the logits and of the states);
- *   workspace gdn2_beam_workspace_bytes(desc) bytes, 256-byte aligned.  Outputs overlap no input. */
+ *   workspace gdn2_beam_workspace_bytes(desc) bytes, 256-byte aligned (NULL where that is 0).
+ *   Outputs overlap no input. */
 gdn2_status gdn2_beam_select(const gdn2_beam_desc* desc, const void* logits, const float* scores,
                              const uint8_t* finished, float* out_scores, int32_t* out_row, int32_t* out_token,
                              uint8_t* out_finished, void* workspace, void* stream);

@@ -118,7 +118,7 @@ def test_entry_points_reject_bad_arguments():
 
     def beam(logits=at, ws=at, **kw):
         d = _lib.BeamDesc()
-        d.B, d.K, d.V, d.stride_b, d.stride_k, d.eos = 1, 2, 8, 16, 8, -1
+        d.B, d.K, d.V, d.stride_b, d.stride_k, d.eos = 1, 2, 100000, 200000, 100000, -1
         for k, v in kw.items():
             setattr(d, k, v)
         return (lib.gdn2_beam_select(ctypes.addressof(d), logits, at, 0, at, at, at, at, ws, 0),
@@ -127,5 +127,6 @@ def test_entry_points_reject_bad_arguments():
     for kw in (dict(B=0), dict(K=0), dict(V=0), dict(dtype=9), dict(stride_b=-1)):
         assert beam(**kw) == (inv, 0), kw
     assert beam(K=33) == (uns, 0)
+    assert beam(logits=at + 1)[0] == inv and beam(V=8)[1] == 0
     assert beam(logits=0)[0] == inv and beam(ws=0)[0] == inv and beam(ws=at + 16)[0] == inv
     assert lib.gdn2_beam_select(0, *[at] * 9) == inv
