@@ -1,7 +1,8 @@
 """Build the sm_100a shared library (plain nvcc, no torch extension machinery).
 
 The library is written in-tree to ``atomic_gdn2/_lib/libgdn2_b200.so`` so that it
-travels with the source tree.  Each ``csrc/*.cu`` is compiled to an object in
+travels with the source tree, the serving operators' binding to torch tensors
+(``csrc/gdn2_torch.cpp``, host code) to ``atomic_gdn2/_lib/gdn2_torch.so``.  Each ``csrc/*.cu`` is compiled to an object in
 parallel, then linked with ``-shared``.
 """
 from __future__ import annotations
@@ -19,6 +20,8 @@ INCLUDE = ROOT.parent / "include"
 LIB_DIR = PKG_DIR / "_lib"
 LIB_NAME = "libgdn2_b200.so"
 LIB_PATH = LIB_DIR / LIB_NAME
+EXT_SRC = CSRC / "gdn2_torch.cpp"          # the serving operators' binding to torch tensors
+EXT_PATH = LIB_DIR / "gdn2_torch.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC",
@@ -37,15 +40,45 @@ def sources() -> list[pathlib.Path]:
 
 
 def _stale() -> bool:
-    if not LIB_PATH.exists():
+    if not LIB_PATH.exists() or not EXT_PATH.exists():
         return True
-    t = LIB_PATH.stat().st_mtime
-    deps = list(CSRC.glob("*.cu")) + list(CSRC.glob("*.cuh")) + list(INCLUDE.glob("*.h"))
+    t = min(LIB_PATH.stat().st_mtime, EXT_PATH.stat().st_mtime)
+    deps = [EXT_SRC] + list(CSRC.glob("*.cu")) + list(CSRC.glob("*.cuh")) + list(INCLUDE.glob("*.h"))
     return any(p.stat().st_mtime > t for p in deps)
 
 
+def _ext_object(obj_dir: pathlib.Path) -> pathlib.Path:
+    """Compile the torch binding (host code only)."""
+    import sysconfig
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    obj = obj_dir / (EXT_SRC.stem + ".o")
+    nvcc_include = pathlib.Path(_nvcc()).resolve().parents[1] / "include"
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-c", str(EXT_SRC), "-o", str(obj),
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}", f"-I{nvcc_include}",
+           "-isystem", sysconfig.get_paths()["include"], *[x for p in include_paths() for x in ("-isystem", p)]]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {EXT_SRC.name}:\n{r.stdout}\n{r.stderr}")
+    return obj
+
+
+def _link_ext(obj: pathlib.Path) -> None:
+    import torch
+    lib = pathlib.Path(torch.__file__).resolve().parent / "lib"
+    tmp = EXT_PATH.with_suffix(".so.tmp")
+    cmd = [shutil.which("g++") or "g++", "-shared", "-o", str(tmp), str(obj), f"-L{LIB_DIR}", f"-l:{LIB_NAME}",
+           f"-L{lib}", "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10",
+           "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, EXT_PATH)
+
+
 def build_library(force: bool = False, verbose: bool = False) -> pathlib.Path:
-    """Compile every csrc/*.cu for sm_100a and link libgdn2_b200.so; returns its path."""
+    """Compile every csrc/*.cu for sm_100a and link libgdn2_b200.so, then the torch binding beside it;
+    returns the library's path."""
     if not force and not _stale():
         return LIB_PATH
     nvcc = _nvcc()
@@ -61,7 +94,8 @@ def build_library(force: bool = False, verbose: bool = False) -> pathlib.Path:
             raise RuntimeError(f"nvcc failed for {src.name}:\n{r.stdout}\n{r.stderr}")
         return obj, r.stdout + r.stderr
 
-    with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
+    with cf.ThreadPoolExecutor(max_workers=min(9, (os.cpu_count() or 1) + 1)) as ex:
+        ext = ex.submit(_ext_object, obj_dir)
         results = list(ex.map(compile_one, sources()))
     if verbose:
         for _, log in results:
@@ -72,6 +106,7 @@ def build_library(force: bool = False, verbose: bool = False) -> pathlib.Path:
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB_PATH)
+    _link_ext(ext.result())
     return LIB_PATH
 
 

@@ -14,6 +14,7 @@ from .precision import ENUM
 _LIB_PATH = pathlib.Path(__file__).resolve().parent / "_lib" / "libgdn2_b200.so"
 _lock = threading.Lock()
 _lib = None
+_ext = None
 
 # gdn2_status
 OK, ERR_INVALID_ARGUMENT, ERR_CUDA, ERR_UNSUPPORTED = 0, 1, 2, 3
@@ -165,6 +166,22 @@ def load():
                     "(nvcc, sm_100a). The GDN-2 operator has no fallback implementation.")
             _lib = _declare(ctypes.CDLL(str(_LIB_PATH)))
     return _lib
+
+
+def binding():
+    """The serving operators' short way from torch tensors to the library (csrc/gdn2_torch.cpp), loaded
+    once; raises RuntimeError if it is missing."""
+    global _ext
+    if _ext is None:
+        import importlib.util
+        load()
+        path = _LIB_PATH.with_name("gdn2_torch.so")
+        if not path.exists():
+            raise RuntimeError(f"{path} is missing: build it with `python -c \"import __graft_entry__ as g; g.build()\"`")
+        spec = importlib.util.spec_from_file_location("gdn2_torch", path)
+        _ext = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(_ext)
+    return _ext
 
 
 def status_string(code: int) -> str:

@@ -19,6 +19,7 @@ from .recurrent import _raw_stream
 
 MAX_BEAMS = 32
 _descs = {}
+_fast = None
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished=None, *, eos=None):
@@ -27,7 +28,14 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished=None, *, eo
     Returns, each (B, K), best first: scores fp32; rows int32, b * K + the beam that is continued
     (an index into the (B K) rows of the logits and of the states: make_blr_recurrent's h_index);
     tokens int32; finished bool."""
-    if not logits.is_cuda:
+    global _fast
+    if logits.is_cuda:                                           # the common call; None: it needs more than that
+        if _fast is None:
+            _fast = _lib.binding().beam_select
+        r = _fast(logits, scores, finished, eos)
+        if r is not None:
+            return r
+    else:
         raise RuntimeError("beam_select: logits must be a CUDA tensor (the selection runs only on the B200 kernels)")
     shape, dt, dev = logits.shape, logits.dtype, logits.device
     if len(shape) != 3 or not logits.numel():

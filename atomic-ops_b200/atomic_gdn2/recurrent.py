@@ -39,10 +39,16 @@ def _check_flags(fl: pipeline._HostFlags, what: str) -> None:
         raise RuntimeError(pipeline._status_message(code, what if mode == "sync" else f"{what} (reported at a later call)"))
 
 
+def _strides(t: torch.Tensor):
+    """t's strides, 0 for a dimension of one (never used)."""
+    return [0 if m == 1 else s for m, s in zip(t.shape[:3], t.stride())] + [t.stride(3)]
+
+
 def _rows_ok(t: torch.Tensor) -> bool:
     """Whether the kernels can read t's rows in place: unit stride, every row on 16 bytes, neighbouring
     tokens less than 2^27 elements apart."""
-    st, n = t.stride(), 16 // t.element_size()
+    n = 16 // t.element_size()
+    st = _strides(t)
     return st[3] == 1 and st[2] < 1 << 27 and not (st[0] % n or st[1] % n or st[2] % n or t.data_ptr() % 16)
 
 
@@ -67,6 +73,7 @@ _descs = {}
 def make_blr_recurrent(cfg: BLRConfig, scale):
     """Returns call(q, k, v, w, b, g, h0=None, *, lengths=None, h_index=None, h_out=None) -> (o, h)."""
     scale, clip = float(scale), float(cfg.clip)
+    fast, last = None, (None, None)
 
     def call(q, k, v, w, b, g, h0=None, *, lengths=None, h_index=None, h_out=None):
         """q..g (B, H, L, D) float tensors, D = 128, any strides (rows that are not contiguous or not
@@ -78,6 +85,18 @@ def make_blr_recurrent(cfg: BLRConfig, scale):
           h_out    (B, H, D, D) fp32 contiguous, written and returned as h; it may be h0 itself, or
                    without h_index overlap nothing of it
         Returns o (B, H, L, D) fp32 (token-major in memory where q is) and h (B, H, D, D) fp32."""
+        nonlocal fast, last
+        if isinstance(q, torch.Tensor) and q.is_cuda:           # the common call; None: it needs more than that
+            if fast is None:
+                fast = _lib.binding().recurrent
+            dev, fl = last
+            if dev != q.device:
+                last = dev, fl = q.device, pipeline._host_flags(q.device)
+            r = fast(q, k, v, w, b, g, h0, lengths, h_index, h_out, scale, clip, fl.ptr)
+            if r is not None:
+                if pipeline._check_mode != "async" or fl.words[0] or fl.words[1]:
+                    _check_flags(fl, "gdn2_recurrent")
+                return r
         xs = (q, k, v, w, b, g)
         shape, dt, dev = q.shape, q.dtype, q.device
         if len(shape) != 4:
@@ -137,8 +156,8 @@ def make_blr_recurrent(cfg: BLRConfig, scale):
             d = _lib.RecDesc()
             d.B, d.H, d.L, d.D, d.n_states = B, H, L, D, n_states
             for i, t in enumerate(xs):
-                for j in range(3):
-                    d.stride[i][j] = t.stride(j) if L else 0
+                for j, st in enumerate(_strides(t)[:3]):
+                    d.stride[i][j] = st if L else 0
             for j in range(3):
                 d.o_stride[j] = o.stride(j)
             d.in_dtype = _lib.BF16 if dt == torch.bfloat16 else _lib.F32

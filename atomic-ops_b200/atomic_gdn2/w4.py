@@ -101,12 +101,20 @@ def quantize_w4(weight: torch.Tensor, group: int = 64) -> W4Weight:
 
 
 _descs = {}
+_fast = None
 
 
 def w4_linear(x: torch.Tensor, weight: W4Weight, bias=None, *, act=None, residual=None) -> torch.Tensor:
     """act(x W + bias) + residual.  x (..., din) fp32 or bf16 CUDA tensor; bias (dout) or None;
     act None or "gelu" (tanh form); residual (..., dout) of x's type.  Returns (..., dout) of x's
     type, rounded once."""
+    global _fast
+    if x.is_cuda and act in _ACTS:                               # the common call; None: it needs more than that
+        if _fast is None:
+            _fast = _lib.binding().w4_linear
+        y = _fast(x, weight.packed, weight.scales, bias, residual, weight.din, weight.dout, weight.group, _ACTS[act])
+        if y is not None:
+            return y
     dt, shape, dev = x.dtype, x.shape, x.device
     if not x.is_cuda:
         raise RuntimeError("w4_linear: x must be a CUDA tensor (the product runs only on the B200 kernels)")
@@ -145,14 +153,15 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, bias=None, *, act=None, residua
         raise RuntimeError("w4_linear has no backward: call it under torch.no_grad()")
     if M == 0:
         return y
-    key = (M, din, dout, weight.group, dt, act, x2.stride(0), rs)
+    xs = 0 if M == 1 else x2.stride(0)
+    key = (M, din, dout, weight.group, dt, act, xs, rs)
     desc = _descs.get(key)
     if desc is None:
         d = _lib.W4Desc()
         d.M, d.K, d.N, d.group = M, din, dout, weight.group
         d.dtype = _lib.BF16 if dt == torch.bfloat16 else _lib.F32
         d.act = _ACTS[act]
-        d.x_stride, d.res_stride, d.y_stride = x2.stride(0), rs, dout
+        d.x_stride, d.res_stride, d.y_stride = xs, rs, dout
         at = ctypes.addressof(d)
         if len(_descs) > 1024:
             _descs.clear()

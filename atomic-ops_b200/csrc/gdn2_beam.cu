@@ -112,10 +112,13 @@ __device__ __forceinline__ float2 join(float2 a, float2 b) {
   return make_float2(m, a.y * expf(a.x - m) + b.y * expf(b.x - m));
 }
 __device__ __forceinline__ float2 join_warp(float2 st) {
+  float m = st.x;
 #pragma unroll
-  for (int m = 16; m > 0; m >>= 1)
-    st = join(st, make_float2(__shfl_xor_sync(kFull, st.x, m), __shfl_xor_sync(kFull, st.y, m)));
-  return st;
+  for (int i = 16; i > 0; i >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, i));
+  float s = m > -INFINITY ? st.y * expf(st.x - m) : 0.f;
+#pragma unroll
+  for (int i = 16; i > 0; i >>= 1) s += __shfl_xor_sync(kFull, s, i);
+  return make_float2(m, s);
 }
 // e^x for x <= 0, to about 2^-22 of the value
 __device__ __forceinline__ float exp_fast(float x) {
@@ -209,14 +212,20 @@ __device__ __forceinline__ void collect(u64& list, const T* x, int v1, const Pie
   while (who) {
     const int from = own + __ffs(who) - 1;
     who &= who - 1;
-    for (int j = lane; j < (pc.count * 8 + 31) / 32 * 32; j += 32) {
-      const int at = from + (j >> 3) * pc.hop + (j & 7) * 32;
-      u64 key = 0;
-      if (j < pc.count * 8 && at < v1) {
-        const float v = clean(ld1(x + at));
-        if (v >= least) key = make_key(v, at);
+    for (int j = lane; j < pc.count * 8 + lane; j += 128) {  // four loads at a time
+      uint32_t u[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int n = j + i * 32, at = from + (n >> 3) * pc.hop + (n & 7) * 32;
+        u[i] = n < pc.count * 8 && at < v1 ? bits(x + at) : 0xffffffffu;
       }
-      insert(list, key, R, lane);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int n = j + i * 32, at = from + (n >> 3) * pc.hop + (n & 7) * 32;
+        const float v = clean(__uint_as_float(u[i]));
+        const bool on = n < pc.count * 8 && at < v1 && v >= least;
+        if (__any_sync(kFull, on)) insert(list, on ? make_key(v, at) : 0, R, lane);
+      }
     }
   }
 }
@@ -324,16 +333,19 @@ __global__ void __launch_bounds__(1024) beam_pick_kernel(BeamParams p, int per) 
   }
 }
 
-// Vocabularies up to this are read by the kernel that selects.
-constexpr int kWholeV = 8192;
+// One launch reads and selects where a sequence's logits are few for its CTA.  Measured (one launch / two,
+// us): 8 x 4 x 256 5 / 17, 64 x 8 x 2000 12 / 19, 1 x 5 x 4096 9.5 / 11, 2 x 4 x 8192 10.5 / 10.8,
+// 16 x 16 x 4096 28 / 21, 64 x 16 x 8192 46 / 32.
+bool whole(const gdn2_beam_desc* d) { return d->V <= 8192 && (long long)d->V * d->K <= 32768; }
 
 struct BeamPlan { int R, splits, slice; size_t stats, total; };
 BeamPlan beam_plan(const gdn2_beam_desc* d) {
   BeamPlan pl{};
   pl.R = d->K < d->V ? d->K : d->V;
-  if (d->V <= kWholeV) return pl;
+  if (whole(d)) return pl;
   const long long rows = (long long)d->B * d->K;
-  // enough slices to cover the GPU a few times over, none smaller than 4096 values
+  // enough slices to cover the GPU a few times over, none smaller than 4096 values (twice and four times as
+  // many: 32 x 8 x 50001 27 -> 31 and 41 us, 1 x 5 x 262144 16 -> 18 us)
   long long want = rows >= 592 ? 1 : 592 / rows, most = (d->V + 4095) / 4096;
   pl.splits = (int)(want < most ? want : most);
   pl.slice = (d->V + pl.splits - 1) / pl.splits;
