@@ -99,23 +99,23 @@ def _dev_status(dev: torch.device) -> _DevStatus:
 
 
 class _HostFlags:
-    """Two words of one device's status in mapped host memory (gdn2_recurrent): kernels set them,
+    """Three words of one device's status in mapped host memory (gdn2_recurrent): kernels set them,
     the host reads them without a copy."""
 
-    BITS = (_lib.DEV_POSITIVE_GATE, _lib.DEV_BAD_INDEX)
+    BITS = (_lib.DEV_POSITIVE_GATE, _lib.DEV_BAD_INDEX, _lib.DEV_TIMEOUT)
 
     def __init__(self, dev: torch.device):
         self.index = dev.index
-        self.tensor = torch.zeros(2, dtype=torch.int32, pin_memory=True)
+        self.tensor = torch.zeros(3, dtype=torch.int32, pin_memory=True)
         self.ptr = self.tensor.data_ptr()
-        self.words = (ctypes.c_uint32 * 2).from_address(self.ptr)
+        self.words = (ctypes.c_uint32 * 3).from_address(self.ptr)
 
     def code(self) -> int:
         return sum(bit for bit, word in zip(self.BITS, self.words) if word)
 
     def take(self) -> int:
         code = self.code()
-        self.words[0] = self.words[1] = 0
+        self.words[:] = [0, 0, 0]
         return code
 
 

@@ -32,7 +32,7 @@ def _check_flags(fl: pipeline._HostFlags, what: str) -> None:
         return
     if mode == "sync":
         torch.cuda.current_stream(fl.index).synchronize()
-    if fl.words[0] or fl.words[1]:
+    if any(fl.words):
         if torch.cuda.is_current_stream_capturing():
             return
         code = fl.take()
@@ -94,7 +94,7 @@ def make_blr_recurrent(cfg: BLRConfig, scale):
                 last = dev, fl = q.device, pipeline._host_flags(q.device)
             r = fast(q, k, v, w, b, g, h0, lengths, h_index, h_out, scale, clip, fl.ptr)
             if r is not None:
-                if pipeline._check_mode != "async" or fl.words[0] or fl.words[1]:
+                if pipeline._check_mode != "async" or any(fl.words):
                     _check_flags(fl, "gdn2_recurrent")
                 return r
         xs = (q, k, v, w, b, g)

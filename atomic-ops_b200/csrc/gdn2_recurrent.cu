@@ -23,7 +23,7 @@ struct RecParams {
   const int32_t* lengths;         // (B) valid tokens, or null for L
   float* o;
   float* h_out;                   // (B, H, D, D)
-  uint32_t* flags;                // [0] a positive gate was seen, [1] an index or length out of range was seen
+  uint32_t* flags;                // [0] a positive gate was seen, [1] an index or length out of range, [2] a wait ran out
   int H, L, n_states;
   float scale, clip;
 };
@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(kStepThreads) rec_step_kernel(RecParams p) {
 
 // ---------------------------------------------------------------------------------------------
 // Several tokens: blocks of 8.  With G_t the gates summed from the block's start through token t,
-//   r_t = (bk_t e^{G_t})^T S,   d_t = w_t v_t - r_t - sum_{s<t} L_ts d_s,
+//   d_t = w_t v_t - (bk_t e^{G_t})^T S - sum_{s<t} L_ts d_s,
 //   o_t = (scale q_t e^{G_t})^T S + sum_{s<=t} P_ts d_s,
 //   S  <- diag(e^{G_8}) S + sum_t (k_t e^{G_8 - G_t}) d_t^T,
 //   L_ts = sum_d bk_t k_s e^{G_t - G_s},   P_ts = scale sum_d q_t k_s e^{G_t - G_s}
@@ -173,8 +173,9 @@ __global__ void __launch_bounds__(kStepThreads) rec_step_kernel(RecParams p) {
 // serves eight tokens, and 3 1/8 products per state element and token are left of 4.  Every factor
 // is a product of gates e^g <= 1, so nothing can overflow however far the gates close.
 //
-// rec_prep_kernel writes what does not depend on S, a record per head and block; rec_seq_kernel
-// walks the records with the state in registers.
+// rec_prep_kernel writes what does not depend on S, a record per head and block; rec_wide_kernel or
+// rec_deep_kernel walks the records with the state in registers.  X = (I + L)^-1 does not depend on S
+// either: the record holds B = X (bk e^G) and V = X (w v), and d = V - B S needs no substitution.
 //
 // The state's products run on the warp-level tensor instruction (m16n8k8, tf32) with each fp32
 // operand split in two (hi lo, each rounded to nearest: 22 bits) and three products; the lo lo
@@ -188,45 +189,36 @@ __global__ void __launch_bounds__(kStepThreads) rec_step_kernel(RecParams p) {
 constexpr int kSmCount = 148;  // of a B200
 constexpr int kTok = 8;
 // A record, in floats, in the order in which the lanes (g = lane / 4, t = lane % 4) read it:
-constexpr int kRecDot = 0;               // [16 tiles of d][32 lanes]{bk(8j+2t), bk(8j+2t+1), q.., q..} of token g
+constexpr int kRecDot = 0;               // [16 tiles of d][32 lanes]{B(8j+2t), B(8j+2t+1), q.., q..} of token g
 constexpr int kRecK = 16 * 128;          // [8 pairs of tiles][32]{k of tokens 2t, 2t+1 at 16i+g, the same at 16i+8+g}
 constexpr int kRecA = kRecK + 8 * 128;   // [8][4 t]{e(16i+2t), e(16i+2t+1), e(16i+8+2t), e(16i+8+2t+1)}
-constexpr int kRecX = kRecA + 128;       // [32]{X(g,2t), X(g,2t+1), P(g,2t), P(g,2t+1)}, X = (I + L)^-1
-constexpr int kRecV = kRecX + 128;       // [8 tiles of columns][32]{wv of tokens 2t, 2t+1 at 16i+g, at 16i+8+g}
+constexpr int kRecP = kRecA + 128;       // [32]{P(g,2t), P(g,2t+1)}
+constexpr int kRecV = kRecP + 64;        // [8 tiles of columns][32]{V of tokens 2t, 2t+1 at 16i+g, at 16i+8+g}
 constexpr int kRecFloats = kRecV + 8 * 128;
 
-// A warp per head and block of tokens, a quarter of d at a time.  Tokens past the sequence's end
-// become no-ops (gate 1, zeros elsewhere).
-constexpr int kPrepWarps = 4;
-
+// A CTA per head and block of tokens, a thread per d.  Tokens past the sequence's end become no-ops
+// (gate 1, zeros elsewhere).
 template <class T>
-__global__ void __launch_bounds__(kPrepWarps * 32, 4) rec_prep_kernel(RecParams p, float* rec, int tok0, int nblk,
-                                                                   int total) {
-  __shared__ float lps[kPrepWarps][64], xs[kPrepWarps][64];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int unit = blockIdx.x * kPrepWarps + warp;
-  if (unit >= total) return;
-  const int bh = unit / nblk, blk = unit % nblk;
+__global__ void __launch_bounds__(kD, 4) rec_prep_kernel(RecParams p, float* rec, int tok0, int nblk) {
+  __shared__ float part[kD / 32][64];
+  __shared__ float lp[64];                  // L_ts in 8 t + s (s < t), P_ts in 8 s + t (s <= t)
+  __shared__ __align__(16) float xm[8][8];  // X
+  const int d = threadIdx.x, lane = d & 31, warp = d >> 5;
+  const int bh = blockIdx.x / nblk, blk = blockIdx.x % nblk;
   const int b = bh / p.H, h = bh % p.H;
   const int t0 = tok0 + blk * kTok, left = valid_len(p, b, false) - t0;
   if (left <= 0) return;
-  float* out = rec + (size_t)unit * kRecFloats;
-  // Gram entries: 8 t + s is L_ts (s < t), 8 s + t is P_ts (s <= t)
-  float gram[64];
+  float* out = rec + (size_t)blockIdx.x * kRecFloats;
+  float q[kTok], k[kTok], bk[kTok], a[kTok], v[kTok], wv[kTok];
+  {
+    const void* base[6] = {p.q, p.k, p.v, p.w, p.b, p.g};
+    const T* src[6];
+    int sl[6];  // a block's tokens are within 32 bits of one another (checked by the entry)
 #pragma unroll
-  for (int i = 0; i < 64; ++i) gram[i] = 0.f;
-  const T* src[6];
-  const void* base[6] = {p.q, p.k, p.v, p.w, p.b, p.g};
-  int sl[6];  // a block's tokens are within 32 bits of one another (checked by the entry)
-#pragma unroll
-  for (int i = 0; i < 6; ++i) sl[i] = (int)p.sl[i];
-#pragma unroll
-  for (int i = 0; i < 6; ++i)
-    src[i] = static_cast<const T*>(base[i]) + b * p.sb[i] + h * p.sh[i] + t0 * p.sl[i] + lane;
-  bool positive = false;
-#pragma unroll 1
-  for (int d = lane; d < kD; d += 32) {
-    float q[kTok], k[kTok], bk[kTok], a[kTok], v[kTok], wv[kTok];
+    for (int i = 0; i < 6; ++i) {
+      src[i] = static_cast<const T*>(base[i]) + b * p.sb[i] + h * p.sh[i] + t0 * p.sl[i] + d;
+      sl[i] = (int)p.sl[i];
+    }
 #pragma unroll
     for (int t = 0; t < kTok; ++t) {  // all of the loads first; the last valid token stands in for those past it
       const int tt = min(t, left - 1);
@@ -237,61 +229,33 @@ __global__ void __launch_bounds__(kPrepWarps * 32, 4) rec_prep_kernel(RecParams 
       bk[t] = ld1(src[4] + tt * sl[4]);
       a[t] = ld1(src[5] + tt * sl[5]);
     }
+  }
+  bool positive = false;
 #pragma unroll
-    for (int i = 0; i < 6; ++i) src[i] += 32;
-#pragma unroll
-    for (int t = 0; t < kTok; ++t) {
-      const bool on = t < left;
-      positive |= a[t] > 0.f;
-      a[t] = on ? expf(fminf(a[t], 0.f)) : 1.f;
-      q[t] = on ? q[t] * p.scale : 0.f;
-      k[t] = on ? k[t] : 0.f;
-      bk[t] = on ? bk[t] * k[t] : 0.f;
-      wv[t] = on ? wv[t] * v[t] : 0.f;
-    }
-    float kh[kTok];  // k_s e^{G_8 - G_s}
-#pragma unroll
-    for (int s = 0; s < kTok; ++s) {
-      float c = k[s];
-      gram[9 * s] = fmaf(q[s], c, gram[9 * s]);
-#pragma unroll
-      for (int t = s + 1; t < kTok; ++t) {
-        c *= a[t];
-        gram[8 * t + s] = fmaf(bk[t], c, gram[8 * t + s]);
-        gram[8 * s + t] = fmaf(q[t], c, gram[8 * s + t]);
-      }
-      kh[s] = c;
-    }
-    // Two lanes hold the two halves of 16 bytes of the record: each takes every second piece.
-    float e = 1.f;
-    const bool odd = d & 1, high = d & 8;
-#pragma unroll
-    for (int t = 0; t < kTok; t += 2) {
-      e *= a[t];
-      const float b0 = bk[t] * e, q0 = q[t] * e;
-      e *= a[t + 1];
-      const float b1 = bk[t + 1] * e, q1 = q[t + 1] * e;
-      const float bx = __shfl_xor_sync(0xffffffffu, odd ? b0 : b1, 1);
-      const float qx = __shfl_xor_sync(0xffffffffu, odd ? q0 : q1, 1);
-      float4* to = reinterpret_cast<float4*>(out + kRecDot) + (d >> 3) * 32 + (t + odd) * 4 + ((d & 7) >> 1);
-      *to = odd ? make_float4(bx, b1, qx, q1) : make_float4(b0, bx, q0, qx);
-    }
-    out[kRecA + ((d >> 4) * 4 + ((d & 7) >> 1)) * 4 + ((d >> 3) & 1) * 2 + (d & 1)] = e;
-    const int at = (d >> 4) * 32 + (d & 7) * 4 + (high ? 2 : 0);
-#pragma unroll
-    for (int t = 0; t < 4; t += 2) {
-      const float k0 = __shfl_xor_sync(0xffffffffu, high ? kh[t] : kh[t + 4], 8);
-      const float k1 = __shfl_xor_sync(0xffffffffu, high ? kh[t + 1] : kh[t + 5], 8);
-      const float v0 = __shfl_xor_sync(0xffffffffu, high ? wv[t] : wv[t + 4], 8);
-      const float v1 = __shfl_xor_sync(0xffffffffu, high ? wv[t + 1] : wv[t + 5], 8);
-      reinterpret_cast<float4*>(out + kRecK)[at + (t >> 1)] =
-          high ? make_float4(k0, k1, kh[t + 4], kh[t + 5]) : make_float4(kh[t], kh[t + 1], k0, k1);
-      reinterpret_cast<float4*>(out + kRecV)[at + (t >> 1)] =
-          high ? make_float4(v0, v1, wv[t + 4], wv[t + 5]) : make_float4(wv[t], wv[t + 1], v0, v1);
-    }
+  for (int t = 0; t < kTok; ++t) {
+    const bool on = t < left;
+    positive |= a[t] > 0.f;
+    a[t] = on ? expf(fminf(a[t], 0.f)) : 1.f;
+    q[t] = on ? q[t] * p.scale : 0.f;
+    k[t] = on ? k[t] : 0.f;
+    bk[t] = on ? bk[t] * k[t] : 0.f;
+    wv[t] = on ? wv[t] * v[t] : 0.f;
   }
   if (positive) p.flags[0] = 1u;
-  // 64 sums over the lanes, halving: lane l ends with entries 2 l and 2 l + 1
+  float gram[64], kh[kTok];
+#pragma unroll
+  for (int s = 0; s < kTok; ++s) {
+    float c = k[s];
+    gram[9 * s] = q[s] * c;
+#pragma unroll
+    for (int t = s + 1; t < kTok; ++t) {
+      c *= a[t];
+      gram[8 * t + s] = bk[t] * c;
+      gram[8 * s + t] = q[t] * c;
+    }
+    kh[s] = c;  // k_s e^{G_8 - G_s}
+  }
+  // 64 sums over the warp's lanes, halving: lane l ends with entries 2 l and 2 l + 1
 #pragma unroll
   for (int half = 32; half >= 2; half >>= 1) {
     const bool up = lane & (half >> 1);
@@ -301,23 +265,69 @@ __global__ void __launch_bounds__(kPrepWarps * 32, 4) rec_prep_kernel(RecParams 
       gram[i] = keep + __shfl_xor_sync(0xffffffffu, give, half >> 1);
     }
   }
-  float *lp = lps[warp], *x = xs[warp];
-  *reinterpret_cast<float2*>(lp + 2 * lane) = make_float2(gram[0], gram[1]);
-  __syncwarp();
-  if (lane < 8) {  // column `lane` of X = (I + L)^-1 by forward substitution
+  *reinterpret_cast<float2*>(&part[warp][2 * lane]) = make_float2(gram[0], gram[1]);
+  __syncthreads();
+  if (d < 64) lp[d] = (part[0][d] + part[1][d]) + (part[2][d] + part[3][d]);
+  __syncthreads();
+  if (d < 8) {  // column d of X by forward substitution
     float y[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      y[i] = i == lane ? 1.f : 0.f;
+      y[i] = i == d ? 1.f : 0.f;
 #pragma unroll
       for (int j = 0; j < i; ++j) y[i] = fmaf(-lp[8 * i + j], y[j], y[i]);
-      x[8 * i + lane] = y[i];
+      xm[i][d] = y[i];
     }
   }
-  __syncwarp();
-  const int g = lane >> 2, s = (lane & 3) * 2;
-  reinterpret_cast<float4*>(out + kRecX)[lane] =
-      make_float4(x[8 * g + s], x[8 * g + s + 1], s <= g ? lp[8 * s + g] : 0.f, s + 1 <= g ? lp[8 * (s + 1) + g] : 0.f);
+  // what needs no X, meanwhile.  Two lanes hold the two halves of 16 bytes of the record: each takes every
+  // second piece.
+  const bool odd = d & 1, high = d & 8;
+  float e = 1.f, be[kTok], qe[kTok];
+#pragma unroll
+  for (int t = 0; t < kTok; ++t) {
+    e *= a[t];
+    be[t] = bk[t] * e;
+    qe[t] = q[t] * e;
+  }
+  out[kRecA + ((d >> 4) * 4 + ((d & 7) >> 1)) * 4 + ((d >> 3) & 1) * 2 + (d & 1)] = e;
+  const int at = (d >> 4) * 32 + (d & 7) * 4 + (high ? 2 : 0);
+#pragma unroll
+  for (int t = 0; t < 4; t += 2) {
+    const float k0 = __shfl_xor_sync(0xffffffffu, high ? kh[t] : kh[t + 4], 8);
+    const float k1 = __shfl_xor_sync(0xffffffffu, high ? kh[t + 1] : kh[t + 5], 8);
+    reinterpret_cast<float4*>(out + kRecK)[at + (t >> 1)] =
+        high ? make_float4(k0, k1, kh[t + 4], kh[t + 5]) : make_float4(kh[t], kh[t + 1], k0, k1);
+  }
+  if (d < 64) {
+    const int l = d >> 1, g = l >> 2, s = (l & 3) * 2 + (d & 1);
+    out[kRecP + d] = s <= g ? lp[8 * s + g] : 0.f;
+  }
+  __syncthreads();
+  float bx[kTok], vx[kTok];
+#pragma unroll
+  for (int t = 0; t < kTok; ++t) {
+    bx[t] = be[t];
+    vx[t] = wv[t];
+#pragma unroll
+    for (int s = 0; s < t; ++s) {
+      bx[t] = fmaf(xm[t][s], be[s], bx[t]);
+      vx[t] = fmaf(xm[t][s], wv[s], vx[t]);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < kTok; t += 2) {
+    const float bo = __shfl_xor_sync(0xffffffffu, odd ? bx[t] : bx[t + 1], 1);
+    const float qo = __shfl_xor_sync(0xffffffffu, odd ? qe[t] : qe[t + 1], 1);
+    reinterpret_cast<float4*>(out + kRecDot)[(d >> 3) * 32 + (t + odd) * 4 + ((d & 7) >> 1)] =
+        odd ? make_float4(bo, bx[t + 1], qo, qe[t + 1]) : make_float4(bx[t], bo, qe[t], qo);
+  }
+#pragma unroll
+  for (int t = 0; t < 4; t += 2) {
+    const float v0 = __shfl_xor_sync(0xffffffffu, high ? vx[t] : vx[t + 4], 8);
+    const float v1 = __shfl_xor_sync(0xffffffffu, high ? vx[t + 1] : vx[t + 5], 8);
+    reinterpret_cast<float4*>(out + kRecV)[at + (t >> 1)] =
+        high ? make_float4(v0, v1, vx[t + 4], vx[t + 5]) : make_float4(vx[t], vx[t + 1], v0, v1);
+  }
 }
 
 // x = hi + lo: hi is x in tf32, rounded to nearest, and the tensor instruction drops the 13 low bits
@@ -397,21 +407,12 @@ __device__ __forceinline__ void seq_store(const float s[kJ][4], const RecParams&
     for (int c = 0; c < 4; ++c)
       to[(j * 8 + (c & 1)) * kD + (c >> 1) * 8] = last ? sanitize(s[j][c], p.clip) : s[j][c];
 }
-// d = X (wv - r) of the warp's 16 columns
-__device__ __forceinline__ SplitA seq_delta(const float r[4], const float4& wv, const float4& xp) {
-  const float u[4] = {wv.x - r[0], wv.y - r[1], wv.z - r[2], wv.w - r[3]};
-  float big[4] = {}, small[4] = {};
-  mma3(big, small, split_tile(u), xp.x, xp.y);
-#pragma unroll
-  for (int c = 0; c < 4; ++c) big[c] += small[c];
-  return split_tile(big);
-}
 // o + P d, stored for the block's valid tokens
 __device__ __forceinline__ void seq_out(const RecParams& p, const SeqSpan& r, int blk, int col, float o[4],
-                                        const SplitA& d, const float4& xp) {
+                                        const SplitA& d, const float2& pm) {
   const int t = threadIdx.x & 3;
   float big[4] = {}, small[4] = {};
-  mma3(big, small, d, xp.z, xp.w);
+  mma3(big, small, d, pm.x, pm.y);
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     const int tok = blk * kTok + 2 * t + (c & 1);
@@ -435,19 +436,43 @@ __device__ __forceinline__ void seq_update(float s[kJ][4], const SplitA& d, cons
   }
 }
 __device__ __forceinline__ float4 lds4(const float* p) { return *reinterpret_cast<const float4*>(p); }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int kN>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(kN) : "memory");
-}
+__device__ __forceinline__ float2 lds2(const float* p) { return *reinterpret_cast<const float2*>(p); }
+// The records' way into the ring: bulk copies that one thread issues, a barrier object per slot.  Waits
+// give up after the library's limit, tell the host and do not wait again.
+struct SeqRing {
+  uint64_t* bars;
+  uint32_t* flags;
+  bool gave_up = false;
+  __device__ void init(int slots) {  // one thread
+    for (int i = 0; i < slots; ++i) mbar_init(bars + i, 1);
+    fence_mbar_init();
+  }
+  __device__ void fetch(int slot, float* dst, const float* from, int v_from, int v_floats) {  // one thread
+    mbar_arrive_expect_tx(bars + slot, (kRecV + v_floats) * 4);
+    bulk_g2s(dst, from, kRecV * 4, bars + slot);
+    bulk_g2s(dst + kRecV, from + kRecV + v_from, v_floats * 4, bars + slot);
+  }
+  __device__ void wait(int slot, uint32_t parity) {
+    if (gave_up || mbar_try_wait(bars + slot, parity)) return;
+    const long long t0 = clock64();
+    while (!mbar_try_wait(bars + slot, parity)) {
+      if (clock64() - t0 > kWaitCycles) {
+        gave_up = true;
+        flags[2] = 1u;
+        return;
+      }
+    }
+  }
+};
 
 // Many heads: a warp owns 16 columns and all of d, a CTA kCT such tiles.  The records arrive
-// through a ring of asynchronous copies that the whole CTA issues.
+// through a ring.
 template <int kCT>
 __global__ void __launch_bounds__(kCT * 32) rec_wide_kernel(RecParams p, const float* rec, const float* state,
                                                           int tok0, int nblk, bool first, bool last) {
   constexpr int kThreads = kCT * 32, kSlots = 3, kSlot = kRecV + kCT * 128;
   extern __shared__ float4 smem4[];
+  __shared__ uint64_t bars[kSlots];
   float* smem = reinterpret_cast<float*>(smem4);
   const int tid = threadIdx.x, lane = tid & 31, ct = tid >> 5, g = lane >> 2, t = lane & 3;
   const SeqSpan r = seq_span<kThreads, kCT * 16>(p, tok0, nblk, first);
@@ -456,20 +481,18 @@ __global__ void __launch_bounds__(kCT * 32) rec_wide_kernel(RecParams p, const f
   float s[16][4];
   seq_load<16>(s, state, r, mine);
   const float* src = rec + (size_t)blockIdx.x * nblk * kRecFloats;
+  SeqRing ring{bars, p.flags};
+  if (tid == 0) ring.init(kSlots);
+  __syncthreads();
   auto fetch = [&](int blk) {
-    if (blk < r.blocks) {
-      float* dst = smem + (blk % kSlots) * kSlot;
-      const float* from = src + (size_t)blk * kRecFloats;
-      for (int i = tid; i < kRecV / 4; i += kThreads) cp_async16(dst + 4 * i, from + 4 * i);
-      cp_async16(dst + kRecV + 4 * tid, from + kRecV + blockIdx.y * kCT * 128 + 4 * tid);
-    }
-    cp_commit();
+    if (tid == 0 && blk < r.blocks)
+      ring.fetch(blk % kSlots, smem + (blk % kSlots) * kSlot, src + (size_t)blk * kRecFloats, blockIdx.y * kCT * 128, kCT * 128);
   };
 #pragma unroll
   for (int i = 0; i < kSlots - 1; ++i) fetch(i);
   for (int blk = 0; blk < r.blocks; ++blk) {
-    cp_wait<kSlots - 2>();
-    __syncthreads();          // block blk is here, and every warp is done with block blk - 1
+    ring.wait(blk % kSlots, (blk / kSlots) & 1);
+    __syncthreads();          // every warp is done with block blk - 1
     fetch(blk + kSlots - 1);  // into that block's slot
     const float* slot = smem + (blk % kSlots) * kSlot;
     float rr[4], o[4];
@@ -488,16 +511,17 @@ __global__ void __launch_bounds__(kCT * 32) rec_wide_kernel(RecParams p, const f
         o[c] = (ob[0][c] + ob[1][c]) + os[c];
       }
     }
-    const float4 xp = lds4(slot + kRecX + lane * 4);
-    const SplitA d = seq_delta(rr, lds4(slot + kRecV + (ct * 32 + lane) * 4), xp);
-    seq_out(p, r, blk, ct * 16 + g, o, d, xp);
+    const float4 v = lds4(slot + kRecV + (ct * 32 + lane) * 4);
+    const float dl[4] = {v.x - rr[0], v.y - rr[1], v.z - rr[2], v.w - rr[3]};
+    const SplitA d = split_tile(dl);
+    seq_out(p, r, blk, ct * 16 + g, o, d, lds2(slot + kRecP + lane * 2));
     seq_update<16>(s, d, slot, 0, lane);
   }
   seq_store<16>(s, p, mine, last);
 }
 
 // Few heads, where a block's chain of dependent steps is what counts: kW warps share 16 columns and
-// take 16 / kW tiles of d each; one more warp copies the records and one finishes the outputs, a
+// take 16 / kW tiles of d each; one more warp sees to the records and one finishes the outputs, a
 // block behind.  One barrier per block: before it the partial sums r of the block are written, after
 // it every warp adds them up.  What is double-buffered by the block's parity:
 //   rpart  written before barrier blk, read until barrier blk + 1
@@ -511,27 +535,28 @@ __global__ void __launch_bounds__((kW + 2) * 32) rec_deep_kernel(RecParams p, co
   float4* rpart = smem4 + kSlots * kSlot / 4;  // [2][kW][32]
   float4* opart = rpart + 2 * kW * 32;         // [2][kW][32]
   float4* delta = opart + 2 * kW * 32;         // [2][32]
+  __shared__ uint64_t bars[kSlots];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const SeqSpan r = seq_span<kThreads, 16>(p, tok0, nblk, first);
   if (r.blocks == 0 && !first && !last) return;
   auto barrier = [] { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); };
   if (warp == kW) {  // copies
     const float* src = rec + (size_t)blockIdx.x * nblk * kRecFloats;
+    SeqRing ring{bars, p.flags};
+    if (lane == 0) ring.init(kSlots);
+    __syncwarp();
     auto fetch = [&](int blk) {
-      if (blk < r.blocks) {
-        float* dst = smem + (blk % kSlots) * kSlot;
-        const float* from = src + (size_t)blk * kRecFloats;
-#pragma unroll 13
-        for (int i = lane; i < kRecV / 4; i += 32) cp_async16(dst + 4 * i, from + 4 * i);
-        cp_async16(dst + kRecV + 4 * lane, from + kRecV + blockIdx.y * 128 + 4 * lane);
-      }
-      cp_commit();
+      if (lane == 0 && blk < r.blocks)
+        ring.fetch(blk % kSlots, smem + (blk % kSlots) * kSlot, src + (size_t)blk * kRecFloats, blockIdx.y * 128, 128);
+    };
+    auto landed = [&](int blk) {
+      if (blk < r.blocks) ring.wait(blk % kSlots, (blk / kSlots) & 1);
     };
     for (int i = 0; i < kSlots - 2; ++i) fetch(i);
-    cp_wait<kSlots - 3>();
+    landed(0);
     barrier();  // block 0 is here
     for (int blk = 0; blk < r.blocks; ++blk) {
-      cp_wait<kSlots - 4>();
+      landed(blk + 1);
       barrier();                // block blk + 1 is here, and every warp is done with block blk - 2
       fetch(blk + kSlots - 2);  // into that block's slot
     }
@@ -552,7 +577,7 @@ __global__ void __launch_bounds__((kW + 2) * 32) rec_deep_kernel(RecParams p, co
       }
       const float4 x = delta[par * 32 + lane];
       const float dl[4] = {x.x, x.y, x.z, x.w};
-      seq_out(p, r, blk - 1, g, o, split_tile(dl), lds4(smem + ((blk - 1) % kSlots) * kSlot + kRecX + lane * 4));
+      seq_out(p, r, blk - 1, g, o, split_tile(dl), lds2(smem + ((blk - 1) % kSlots) * kSlot + kRecP + lane * 2));
     }
     barrier();
     if (r.blocks) {
@@ -565,7 +590,7 @@ __global__ void __launch_bounds__((kW + 2) * 32) rec_deep_kernel(RecParams p, co
       }
       const float4 x = delta[par * 32 + lane];
       const float dl[4] = {x.x, x.y, x.z, x.w};
-      seq_out(p, r, blk, g, o, split_tile(dl), lds4(smem + (blk % kSlots) * kSlot + kRecX + lane * 4));
+      seq_out(p, r, blk, g, o, split_tile(dl), lds2(smem + (blk % kSlots) * kSlot + kRecP + lane * 2));
     }
     return;
   }
@@ -590,24 +615,19 @@ __global__ void __launch_bounds__((kW + 2) * 32) rec_deep_kernel(RecParams p, co
         make_float4((big[0][0] + big[1][0]) + (small[0][0] + small[1][0]), (big[0][1] + big[1][1]) + (small[0][1] + small[1][1]),
                     (big[0][2] + big[1][2]) + (small[0][2] + small[1][2]), (big[0][3] + big[1][3]) + (small[0][3] + small[1][3]));
     barrier();
+    const float4 v = lds4(slot + kRecV + lane * 4);
     float rr[4] = {};
 #pragma unroll
     for (int i = 0; i < kW; ++i) {
       const float4 x = rpart[(par * kW + i) * 32 + lane];
       rr[0] += x.x; rr[1] += x.y; rr[2] += x.z; rr[3] += x.w;
     }
-    const float4 xp = lds4(slot + kRecX + lane * 4);
-    const float4 wv = lds4(slot + kRecV + lane * 4);
-    const float u[4] = {wv.x - rr[0], wv.y - rr[1], wv.z - rr[2], wv.w - rr[3]};
-    float dl[4] = {}, ds[4] = {};
-    mma3(dl, ds, split_tile(u), xp.x, xp.y);
-    // the outputs' sums fill the tensor pipe while d is on its way
+    const float dl[4] = {v.x - rr[0], v.y - rr[1], v.z - rr[2], v.w - rr[3]};
+    const SplitA d = split_tile(dl);
     float ob[2][4] = {}, os[2][4] = {};
 #pragma unroll
     for (int j = 0; j < kJ; ++j) mma3(ob[j & 1], os[j & 1], a[j], f[j].z, f[j].w);
-#pragma unroll
-    for (int c = 0; c < 4; ++c) dl[c] += ds[c];
-    seq_update<kJ>(s, split_tile(dl), slot, j0, lane);
+    seq_update<kJ>(s, d, slot, j0, lane);
     opart[(par * kW + warp) * 32 + lane] =
         make_float4((ob[0][0] + ob[1][0]) + (os[0][0] + os[1][0]), (ob[0][1] + ob[1][1]) + (os[0][1] + os[1][1]),
                     (ob[0][2] + ob[1][2]) + (os[0][2] + os[1][2]), (ob[0][3] + ob[1][3]) + (os[0][3] + os[1][3]));
@@ -661,7 +681,7 @@ cudaError_t launch(const RecParams& p, int BH, float* rec, cudaStream_t st) {
   for (int t0 = 0; t0 < p.L; t0 += seg * kTok) {
     const int nblk = min(seg, (p.L - t0 + kTok - 1) / kTok);
     const bool first = t0 == 0, last = t0 + seg * kTok >= p.L;
-    rec_prep_kernel<T><<<(BH * nblk + kPrepWarps - 1) / kPrepWarps, kPrepWarps * 32, 0, st>>>(p, rec, t0, nblk, BH * nblk);
+    rec_prep_kernel<T><<<BH * nblk, kD, 0, st>>>(p, rec, t0, nblk);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     e = deep ? launch_deep<4>(p, rec, BH, t0, nblk, first, last, st)

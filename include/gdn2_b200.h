@@ -238,9 +238,10 @@ typedef struct gdn2_rec_desc {
  *   o         fp32 over (B, H, L, D) in o_stride, h_out (B, H, D, D) fp32 contiguous.  h_out may
  *             be h0 itself when h_index is NULL and must not overlap it otherwise
  *   workspace gdn2_recurrent_workspace_bytes(desc) bytes, 256-byte aligned (not used for L <= 1)
- *   flags     two uint32 words in device or mapped host memory: a kernel sets [0] to 1 when it
+ *   flags     three uint32 words in device or mapped host memory: a kernel sets [0] to 1 when it
  *             sees g > 0 (outside domain I-1) and [1] to 1 when it sees an index >= n_states (it
- *             then starts from zeros) or a length outside 0..L (it then takes the nearer bound) */
+ *             then starts from zeros) or a length outside 0..L (it then takes the nearer bound),
+ *             [2] to 1 when an on-chip wait ran out (the results are invalid) */
 gdn2_status gdn2_recurrent(const gdn2_rec_desc* desc, const void* q, const void* k, const void* v, const void* w,
                            const void* b, const void* g, const float* h0, const int32_t* h_index,
                            const int32_t* lengths, float* o, float* h_out, void* workspace, uint32_t* flags,
