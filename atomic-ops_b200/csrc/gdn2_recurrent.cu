@@ -614,6 +614,9 @@ __global__ void __launch_bounds__((kW + 2) * 32) rec_deep_kernel(RecParams p, co
     rpart[(par * kW + warp) * 32 + lane] =
         make_float4((big[0][0] + big[1][0]) + (small[0][0] + small[1][0]), (big[0][1] + big[1][1]) + (small[0][1] + small[1][1]),
                     (big[0][2] + big[1][2]) + (small[0][2] + small[1][2]), (big[0][3] + big[1][3]) + (small[0][3] + small[1][3]));
+    float ob[2][4] = {}, os[2][4] = {};
+#pragma unroll
+    for (int j = 0; j < kJ; ++j) mma3(ob[j & 1], os[j & 1], a[j], f[j].z, f[j].w);
     barrier();
     const float4 v = lds4(slot + kRecV + lane * 4);
     float rr[4] = {};
@@ -624,9 +627,6 @@ __global__ void __launch_bounds__((kW + 2) * 32) rec_deep_kernel(RecParams p, co
     }
     const float dl[4] = {v.x - rr[0], v.y - rr[1], v.z - rr[2], v.w - rr[3]};
     const SplitA d = split_tile(dl);
-    float ob[2][4] = {}, os[2][4] = {};
-#pragma unroll
-    for (int j = 0; j < kJ; ++j) mma3(ob[j & 1], os[j & 1], a[j], f[j].z, f[j].w);
     seq_update<kJ>(s, d, slot, j0, lane);
     opart[(par * kW + warp) * 32 + lane] =
         make_float4((ob[0][0] + ob[1][0]) + (os[0][0] + os[1][0]), (ob[0][1] + ob[1][1]) + (os[0][1] + os[1][1]),
