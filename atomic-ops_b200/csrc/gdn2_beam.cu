@@ -53,8 +53,9 @@ __device__ __forceinline__ float clean(float x) {  // NaN: -inf; +inf: the large
   return fminf(fmaxf(x, -INFINITY), 3.402823466e38f);
 }
 
-// Sorts 32 keys over the lanes, largest first (bitonic).
-__device__ __forceinline__ u64 sort32(u64 k, int lane) {
+// Sorts 32 keys over the lanes, largest first (bitonic).  Like insert() a function of its own: inlined
+// wherever they are used they are most of the kernels' code, and fetching that costs more than calls do.
+__device__ __noinline__ u64 sort32(u64 k, int lane) {
 #pragma unroll
   for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
@@ -66,8 +67,8 @@ __device__ __forceinline__ u64 sort32(u64 k, int lane) {
   return k;
 }
 
-// Inserts each lane's key (0: none) that is above the list's R-th into the warp's sorted list.
-__device__ __forceinline__ void insert(u64& list, u64 key, int R, int lane) {
+// The warp's sorted list with each lane's key (0: none) that is above its R-th inserted.
+__device__ __noinline__ u64 inserted(u64 list, u64 key, int R, int lane) {
   u64 last = __shfl_sync(kFull, list, R - 1);
   unsigned todo = __ballot_sync(kFull, key > last);
   if (__popc(todo) > 6) {  // sort them and take the upper half of the two lists' merge
@@ -79,8 +80,7 @@ __device__ __forceinline__ void insert(u64& list, u64 key, int R, int lane) {
       const u64 other = __shfl_xor_sync(kFull, m, d);
       m = ((lane & d) == 0) == (m > other) ? m : other;
     }
-    list = m;
-    return;
+    return m;
   }
   while (todo) {
     const int src = __ffs(todo) - 1;
@@ -92,7 +92,9 @@ __device__ __forceinline__ void insert(u64& list, u64 key, int R, int lane) {
     if (lane == pos) list = k;
     else if (lane > pos) list = up;
   }
+  return list;
 }
+__device__ __forceinline__ void insert(u64& list, u64 key, int R, int lane) { list = inserted(list, key, R, lane); }
 // The best of n keys in memory (0: none), into the warp's list.
 __device__ __forceinline__ void gather(u64& list, const u64* keys, int n, int R, int lane) {
   for (int i = 0; i < n; i += 128) {
@@ -202,30 +204,52 @@ __device__ __forceinline__ float nth(float v, int q, int lane) {
   }
   return r;
 }
-// The warp's candidates into its list: the values, `least` or more, of the lanes whose maximum is that;
-// the whole warp reads a lane's values again.
+// Four candidates a lane, x[at] where at < v1, into the warp's list.
+template <class T>
+__device__ __forceinline__ void offer(u64& list, const T* x, int v1, const int at[4], float least, int R, int lane) {
+  uint32_t u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) u[i] = at[i] < v1 ? bits(x + at[i]) : 0u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float v = clean(__uint_as_float(u[i]));
+    const bool on = at[i] < v1 && v >= least;
+    if (__any_sync(kFull, on)) insert(list, on ? make_key(v, at[i]) : 0, R, lane);
+  }
+}
+// The warp's candidates into its list: the values, `least` or more, of the lanes whose maximum is that.
+// Those lanes' values are read again by the whole warp: one lane's after the other's, or, where a lane has
+// fewer than 32, several lanes' at a time.
 template <class T>
 __device__ __forceinline__ void collect(u64& list, const T* x, int v1, const Pieces& pc, float m, float least, int R,
-                                        int lane) {
+                                        int lane, uint8_t lanes[32]) {
   unsigned who = __ballot_sync(kFull, m >= least);
-  const int own = pc.at - lane;
-  while (who) {
-    const int from = own + __ffs(who) - 1;
-    who &= who - 1;
-    for (int j = lane; j < pc.count * 8 + lane; j += 128) {  // four loads at a time
-      uint32_t u[4];
+  const int own = pc.at - lane, each = pc.count * 8;
+  int at[4];
+  if (each >= 32) {
+    while (who) {
+      const int from = own + __ffs(who) - 1;
+      who &= who - 1;
+      for (int c = lane; c < each + lane; c += 128) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int n = c + i * 32;
+          at[i] = n < each ? from + (n >> 3) * pc.hop + (n & 7) * 32 : v1;
+        }
+        offer(list, x, v1, at, least, R, lane);
+      }
+    }
+  } else {
+    if (m >= least) lanes[__popc(who & ((1u << lane) - 1))] = (uint8_t)lane;
+    __syncwarp();
+    const int total = __popc(who) * each;
+    for (int c = lane; c < total + lane; c += 128) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int n = j + i * 32, at = from + (n >> 3) * pc.hop + (n & 7) * 32;
-        u[i] = n < pc.count * 8 && at < v1 ? bits(x + at) : 0xffffffffu;
+        const int n = c + i * 32;
+        at[i] = n < total ? own + lanes[n / each] + (n % each >> 3) * pc.hop + (n & 7) * 32 : v1;
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int n = j + i * 32, at = from + (n >> 3) * pc.hop + (n & 7) * 32;
-        const float v = clean(__uint_as_float(u[i]));
-        const bool on = n < pc.count * 8 && at < v1 && v >= least;
-        if (__any_sync(kFull, on)) insert(list, on ? make_key(v, at) : 0, R, lane);
-      }
+      offer(list, x, v1, at, least, R, lane);
     }
   }
 }
@@ -238,6 +262,7 @@ __global__ void __launch_bounds__(kScanWarps * 32) beam_scan_kernel(BeamParams p
   __shared__ u64 lists[kScanWarps * 32];
   __shared__ float2 stats[kScanWarps];
   __shared__ float bound[kScanWarps];
+  __shared__ uint8_t lanes[kScanWarps][32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int row = blockIdx.x, split = blockIdx.y;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -256,7 +281,7 @@ __global__ void __launch_bounds__(kScanWarps * 32) beam_scan_kernel(BeamParams p
 #pragma unroll
   for (int i = 1; i < kScanWarps; ++i) least = fminf(least, bound[i]);
   u64 list = 0;
-  collect(list, x, v1, pc, top, least, p.R, lane);
+  collect(list, x, v1, pc, top, least, p.R, lane, lanes[warp]);
   if (lane < p.R) lists[warp * p.R + lane] = list;
   __syncthreads();
   if (warp) return;
@@ -276,6 +301,7 @@ __global__ void __launch_bounds__(1024) beam_pick_kernel(BeamParams p, int per) 
   __shared__ float2 stats[32];
   __shared__ float total[32 * 32];
   __shared__ int token[32 * 32];
+  __shared__ uint8_t lanes[32][32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int k = warp / per, part = warp % per, row = blockIdx.x * p.K + k;
   const bool done = p.finished && p.finished[row];
@@ -289,7 +315,7 @@ __global__ void __launch_bounds__(1024) beam_pick_kernel(BeamParams p, int per) 
       const Pieces pc = pieces(0, p.V, part, per, lane);
       st = scan(x, p.V, pc);
       // see beam_scan_kernel; here each warp goes by its own lanes
-      collect(list, x, p.V, pc, st.x, nth(st.x, p.R, lane), p.R, lane);
+      collect(list, x, p.V, pc, st.x, nth(st.x, p.R, lane), p.R, lane, lanes[warp]);
     } else {
       const int n = (p.splits + per - 1) / per, s0 = part * n, s1 = min(p.splits, s0 + n);
       const size_t at = (size_t)row * p.splits;
