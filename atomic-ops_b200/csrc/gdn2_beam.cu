@@ -147,46 +147,42 @@ __device__ __forceinline__ uint32_t bits(const __nv_bfloat16* p) {
 template <class T>
 __device__ __forceinline__ float2 scan(const T* x, int v1, const Pieces& pc) {
   float m = -INFINITY, sum = 0.f;
-  constexpr int kG = 2;  // pieces that are on their way while as many are worked on
-  uint32_t next[kG][8];
+  float next[8];  // a piece is on its way while one is worked on (two or four: no faster, more code to fetch)
   auto fetch = [&](int i) {
+    const int from = pc.at + i * pc.hop;
+    const T* src = x + from;
+    if (i < pc.count && from + 7 * 32 < v1) {
 #pragma unroll
-    for (int g = 0; g < kG; ++g)
+      for (int j = 0; j < 8; ++j) next[j] = __uint_as_float(bits(src + j * 32));
+    } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int at = pc.at + (i + g) * pc.hop + j * 32;
-        next[g][j] = i + g < pc.count && at < v1 ? bits(x + at) : 0xff800000u;
-      }
+      for (int j = 0; j < 8; ++j) next[j] = i < pc.count && from + j * 32 < v1 ? __uint_as_float(bits(src + j * 32)) : -INFINITY;
+    }
   };
   fetch(0);
-  for (int i = 0; i < pc.count; i += kG) {
-    float now[kG][8];
+  for (int i = 0; i < pc.count; ++i) {
+    float c[8];
 #pragma unroll
-    for (int g = 0; g < kG; ++g)
+    for (int j = 0; j < 8; ++j) c[j] = next[j];
+    fetch(i + 1);
+    for (int again = 0; again < 2; ++again) {
+      float top = c[0];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) now[g][j] = __uint_as_float(next[g][j]);
-    fetch(i + kG);
+      for (int j = 1; j < 8; ++j) top = fmaxf(top, c[j]);
+      const float big = fmaxf(m, top);
+      float part = sum;
+      if (big > m) part *= exp_fast(m - big);
+      if (big > -INFINITY) {
 #pragma unroll
-    for (int g = 0; g < kG; ++g) {
-      for (int again = 0; again < 2; ++again) {
-        float top = now[g][0];
-#pragma unroll
-        for (int j = 1; j < 8; ++j) top = fmaxf(top, now[g][j]);
-        const float big = fmaxf(m, top);
-        float part = sum;
-        if (big > m) part *= exp_fast(m - big);
-        if (big > -INFINITY) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) part += exp_fast(now[g][j] - big);
-        }
-        if (part == part) {
-          m = big;
-          sum = part;
-          break;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) now[g][j] = clean(now[g][j]);  // a NaN or +inf among the values
+        for (int j = 0; j < 8; ++j) part += exp_fast(c[j] - big);
       }
+      if (part == part) {
+        m = big;
+        sum = part;
+        break;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) c[j] = clean(c[j]);  // a NaN or +inf among the values
     }
   }
   return make_float2(m, sum);
