@@ -11,7 +11,10 @@ Device status: the kernels report a positive gate (outside domain I-1) and an in
 out of range by writing to mapped host memory, which the host reads without a copy or a wait.  As
 with the chunked operator the default raises at a later call, set_checks(True) synchronises and
 raises at once, set_checks(False) leaves it to last_status(); nothing is checked while a stream is
-being captured.
+being captured (make a device's first call outside a capture: it sets that memory up).
+
+A value that is not finite counts from its token on: in q for that token's o, in v or w for its
+column, in k, b or g for the head; what it reaches is sanitized to 0 (a NaN) or to the bound.
 """
 from __future__ import annotations
 

@@ -404,7 +404,7 @@ gdn2_status check_beam(const gdn2_beam_desc* d) {
   if (!d || d->B <= 0 || d->K <= 0 || d->V <= 0) return GDN2_ERR_INVALID_ARGUMENT;
   if (d->dtype != GDN2_F32 && d->dtype != GDN2_BF16) return GDN2_ERR_INVALID_ARGUMENT;
   if (d->stride_b < 0 || d->stride_k < 0) return GDN2_ERR_INVALID_ARGUMENT;
-  if (d->K > 32 || (int64_t)d->B * d->K > (1 << 30)) return GDN2_ERR_UNSUPPORTED;
+  if (d->K > 32 || d->V > (1 << 30) || (int64_t)d->B * d->K > (1 << 30)) return GDN2_ERR_UNSUPPORTED;
   return GDN2_OK;
 }
 

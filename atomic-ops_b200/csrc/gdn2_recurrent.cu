@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kStepThreads) rec_step_kernel(RecParams p) {
     const float be = ld1(static_cast<const T*>(p.b) + b * p.sb[4] + h * p.sh[4] + tid);
     const float g = ld1(static_cast<const T*>(p.g) + b * p.sb[5] + h * p.sh[5] + tid);
     if (g > 0.f) p.flags[0] = 1u;
-    const float a = expf(fminf(g, 0.f));
+    const float a = expf(g > 0.f ? 0.f : g);  // a NaN stays one
     vec[tid] = make_float4(a, k, be * k * a, q * a);
     float qk = q * k;
 #pragma unroll
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(kD, 4) rec_prep_kernel(RecParams p, float* rec
   for (int t = 0; t < kTok; ++t) {
     const bool on = t < left;
     positive |= a[t] > 0.f;
-    a[t] = on ? expf(fminf(a[t], 0.f)) : 1.f;
+    a[t] = on ? expf(a[t] > 0.f ? 0.f : a[t]) : 1.f;  // a NaN stays one
     q[t] = on ? q[t] * p.scale : 0.f;
     k[t] = on ? k[t] : 0.f;
     bk[t] = on ? bk[t] * k[t] : 0.f;
@@ -407,16 +407,41 @@ __device__ __forceinline__ void seq_store(const float s[kJ][4], const RecParams&
     for (int c = 0; c < 4; ++c)
       to[(j * 8 + (c & 1)) * kD + (c >> 1) * 8] = last ? sanitize(s[j][c], p.clip) : s[j][c];
 }
-// o + P d, stored for the block's valid tokens
-__device__ __forceinline__ void seq_out(const RecParams& p, const SeqSpan& r, int blk, int col, float o[4],
-                                        const SplitA& d, const float2& pm) {
-  const int t = threadIdx.x & 3;
-  float big[4] = {}, small[4] = {};
-  mma3(big, small, d, pm.x, pm.y);
+// o + P d, stored for the block's valid tokens.  `pm`: the record's P.  The product's zeros above P's
+// diagonal would carry a d that is not finite into the tokens before it: then it is done token by token.
+__device__ __noinline__ void seq_out_careful(float o[4], const float dl[4], const float* pm) {
+  const int lane = threadIdx.x & 31, t = lane & 3;
+#pragma unroll 1
+  for (int s = 0; s < kTok; ++s) {
+    const int from = (lane & ~3) | (s >> 1);
+    const float lo0 = __shfl_sync(0xffffffffu, dl[0], from), lo1 = __shfl_sync(0xffffffffu, dl[1], from);
+    const float hi0 = __shfl_sync(0xffffffffu, dl[2], from), hi1 = __shfl_sync(0xffffffffu, dl[3], from);
+    const float d0 = s & 1 ? lo1 : lo0, d1 = s & 1 ? hi1 : hi0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int tok = 2 * t + (c & 1);
+      if (s <= tok) o[c] = fmaf(pm[tok * kTok + s], c & 2 ? d1 : d0, o[c]);
+    }
+  }
+}
+__device__ __forceinline__ void seq_out(const RecParams& p, const SeqSpan& r, int blk, int col, const float in[4],
+                                        const float dl[4], const SplitA& d, const float* pm) {
+  const int lane = threadIdx.x & 31, t = lane & 3;
+  float o[4] = {in[0], in[1], in[2], in[3]};
+  const float probe = (dl[0] - dl[0]) + (dl[1] - dl[1]) + (dl[2] - dl[2]) + (dl[3] - dl[3]);  // 0, or NaN
+  if (__any_sync(0xffffffffu, probe != 0.f)) {
+    seq_out_careful(o, dl, pm);
+  } else {
+    const float2 f = *reinterpret_cast<const float2*>(pm + lane * 2);
+    float big[4] = {}, small[4] = {};
+    mma3(big, small, d, f.x, f.y);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[c] += big[c] + small[c];
+  }
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     const int tok = blk * kTok + 2 * t + (c & 1);
-    if (tok < r.n) r.o[tok * p.ol + col + (c >> 1) * 8] = sanitize(o[c] + (big[c] + small[c]), p.clip);
+    if (tok < r.n) r.o[tok * p.ol + col + (c >> 1) * 8] = sanitize(o[c], p.clip);
   }
 }
 template <int kJ>
@@ -436,7 +461,6 @@ __device__ __forceinline__ void seq_update(float s[kJ][4], const SplitA& d, cons
   }
 }
 __device__ __forceinline__ float4 lds4(const float* p) { return *reinterpret_cast<const float4*>(p); }
-__device__ __forceinline__ float2 lds2(const float* p) { return *reinterpret_cast<const float2*>(p); }
 // The records' way into the ring: bulk copies that one thread issues, a barrier object per slot.  Waits
 // give up after the library's limit, tell the host and do not wait again.
 struct SeqRing {
@@ -514,7 +538,7 @@ __global__ void __launch_bounds__(kCT * 32) rec_wide_kernel(RecParams p, const f
     const float4 v = lds4(slot + kRecV + (ct * 32 + lane) * 4);
     const float dl[4] = {v.x - rr[0], v.y - rr[1], v.z - rr[2], v.w - rr[3]};
     const SplitA d = split_tile(dl);
-    seq_out(p, r, blk, ct * 16 + g, o, d, lds2(slot + kRecP + lane * 2));
+    seq_out(p, r, blk, ct * 16 + g, o, dl, d, slot + kRecP);
     seq_update<16>(s, d, slot, 0, lane);
   }
   seq_store<16>(s, p, mine, last);
@@ -577,7 +601,7 @@ __global__ void __launch_bounds__((kW + 2) * 32) rec_deep_kernel(RecParams p, co
       }
       const float4 x = delta[par * 32 + lane];
       const float dl[4] = {x.x, x.y, x.z, x.w};
-      seq_out(p, r, blk - 1, g, o, split_tile(dl), lds2(smem + ((blk - 1) % kSlots) * kSlot + kRecP + lane * 2));
+      seq_out(p, r, blk - 1, g, o, dl, split_tile(dl), smem + ((blk - 1) % kSlots) * kSlot + kRecP);
     }
     barrier();
     if (r.blocks) {
@@ -590,7 +614,7 @@ __global__ void __launch_bounds__((kW + 2) * 32) rec_deep_kernel(RecParams p, co
       }
       const float4 x = delta[par * 32 + lane];
       const float dl[4] = {x.x, x.y, x.z, x.w};
-      seq_out(p, r, blk, g, o, split_tile(dl), lds2(smem + (blk % kSlots) * kSlot + kRecP + lane * 2));
+      seq_out(p, r, blk, g, o, dl, split_tile(dl), smem + (blk % kSlots) * kSlot + kRecP);
     }
     return;
   }

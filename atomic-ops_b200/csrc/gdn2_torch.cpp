@@ -91,8 +91,20 @@ PyObject* recurrent(PyObject*, PyObject* const* a, Py_ssize_t n) {
       Py_RETURN_NONE;
     ints[i] = static_cast<const int32_t*>(t->data_ptr());
   }
-  if ((ints[1] && !h0) || a[9] != Py_None) Py_RETURN_NONE;
-  at::Tensor h = fresh(state, at::kFloat, dev);
+  if (ints[1] && !h0) Py_RETURN_NONE;
+  at::Tensor h;
+  if (a[9] != Py_None) {
+    const at::Tensor* t = plain(a[9]);
+    if (!t || t->device() != dev || t->scalar_type() != at::kFloat || t->sizes() != c10::IntArrayRef(state) ||
+        !t->is_contiguous() || !on16(*t))
+      Py_RETURN_NONE;
+    // h0 itself without an index, or no overlap
+    const float *lo = static_cast<const float*>(t->data_ptr()), *hi = lo + t->numel();
+    if (h0 && lo < h0 + (int64_t)d.n_states * H * D * D && h0 < hi && (ints[1] || lo != h0)) Py_RETURN_NONE;
+    h = *t;
+  } else {
+    h = fresh(state, at::kFloat, dev);
+  }
   at::Tensor o;
   if (q.stride(1) < q.stride(2)) {  // token-major: so is o
     const int64_t size[4] = {B, H, L, D}, st[4] = {L * H * D, D, H * D, 1};

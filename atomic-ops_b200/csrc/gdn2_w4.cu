@@ -141,13 +141,36 @@ __device__ __forceinline__ void load_quarter(const W4Params& p, const T* const x
 template <int kTerms, int kMB>
 constexpr bool kTwoCtas = kMB == 1 || (kTerms == 1 && kMB == 2);
 
+// One output's sum over k, value by value.
+template <class T, int kPer>
+__device__ __noinline__ float w4_careful(const W4Params& p, int row, int col) {
+  const int cb = col >> 5, v = (col >> 4) & 1, c = (col >> 3) & 1, l = col & 7;
+  const T* x = static_cast<const T*>(p.x) + (long long)row * p.xs;
+  float y = 0.f, part = 0.f;
+  for (int k = 0; k < p.K; ++k) {
+    const size_t block = (size_t)cb * p.NB + (k >> 7);
+    const int u = (k >> 6) & 1, s = ((k >> 5) & 1) * 2 + ((k >> 2) & 1), t = (k >> 3) & 3;
+    const uint32_t word = reinterpret_cast<const uint32_t*>(p.w)[((block * 4 + u * 2 + v) * 32 + l * 4 + t) * 4 + s];
+    const int q = (int)((word >> (4 * (c + (k & 2) + 4 * (k & 1)))) & 15) - 8;
+    part = fmaf((float)q, ld1(x + k), part);
+    if (k + 1 == p.K || (k + 1) % (128 / kPer) == 0) {
+      const uint16_t* sc = reinterpret_cast<const uint16_t*>(p.scales);
+      const uint32_t bits = sc[(((block * 2 + v) * 8 + l) * kPer + (k & 127) / (128 / kPer)) * 2 + c];
+      y = fmaf(__uint_as_float(bits << 16), part, y);
+      part = 0.f;
+    }
+  }
+  return y;
+}
+
 // A warp computes 32 columns for 8 kMB rows over its share of the batches of 128 rows; a CTA has kMB
 // warps side by side (they share x through L1) and 8 / kMB that split the batches, and the CTAs of a
 // cluster split them further.  kPer: scales of a column per batch.
 //
 // With one block of bf16 rows the slots count most: the 136 of widen() stays in, and one more product,
 // of x with -136 in every place, is added to each group's sum.  The cancellation costs five
-// bits of fp32 there, 2^-19 of the result, far below its rounding to bf16.
+// bits of fp32 there, 2^-19 of the result, far below its rounding to bf16.  Where it leaves no finite
+// value (x beyond 2^121, infinities, NaN) the sum is done again without it.
 template <class T, int kTerms, int kMB, int kPer, bool kPacked>
 __global__ void __launch_bounds__(kW4Warps * 32, kTwoCtas<kTerms, kMB> ? 2 : 1) w4_kernel(W4Params p) {
   constexpr int kWN = kMB, kWK = kW4Warps / kWN, kCols = kWN * 32, kRows = kMB * 8 + 1;
@@ -309,6 +332,9 @@ __global__ void __launch_bounds__(kW4Warps * 32, kTwoCtas<kTerms, kMB> ? 2 : 1) 
     } else {
 #pragma unroll
       for (int i = 0; i < kWK; ++i) y += *local(i * kCols + n, m);
+    }
+    if constexpr (!kExact) {
+      if (!isfinite(y)) y = w4_careful<T, kPer>(p, row, col);
     }
     if (p.bias) y += p.bias[col];
     if (p.gelu) y = gelu_tanh(y);

@@ -156,6 +156,34 @@ def test_recurrent_sanitizes(L):
     assert float(h.abs().max()) <= 2.0 and _rel(h, h_r) < REC_TOL and _rel(o, o_r) < REC_TOL
 
 
+@pytest.mark.parametrize("B", [1, 40])
+@pytest.mark.parametrize("which,col", [(0, None), (1, None), (2, 7), (3, 90), (4, None), (5, None)])
+def test_recurrent_nan_counts_from_its_token_on(which, col, B):
+    """A NaN in one token of one head: the tokens before it, the other heads and (v, w) the other columns keep
+    their values; o of q's token, the column, or everything after it, becomes 0."""
+    H, L, at = 3, 21, 12
+    xs, dev, h0 = _inputs(B, H, L, 31)
+    fn = make_blr_recurrent(make_cfg(), SCALE)
+    o_w, h_w = fn(*dev, h0.cuda())
+    bad = [t.clone() for t in dev]
+    bad[which][0, 1, at, col if col is not None else 5] = float("nan")
+    o, h = fn(*bad, h0.cuda())
+    assert torch.equal(o[1:], o_w[1:]) and torch.equal(o[0, 0], o_w[0, 0]) and torch.equal(o[0, 2], o_w[0, 2])
+    assert _rel(o[0, 1, :at], o_w[0, 1, :at].double().cpu()) < REC_TOL
+    if which == 0:
+        assert bool((o[0, 1, at] == 0).all())
+        assert _rel(o[0, 1, at + 1:], o_w[0, 1, at + 1:].double().cpu()) < REC_TOL
+        assert _rel(h, h_w.double().cpu()) < REC_TOL
+    elif col is not None:
+        keep = [c for c in range(D) if c != col]
+        assert bool((o[0, 1, at:, col] == 0).all()) and bool((h[0, 1, :, col] == 0).all())
+        assert _rel(o[0, 1, at:][:, keep], o_w[0, 1, at:][:, keep].double().cpu()) < REC_TOL
+        assert _rel(h[0, 1][:, keep], h_w[0, 1][:, keep].double().cpu()) < REC_TOL
+    else:
+        assert bool((o[0, 1, at + 1:] == 0).all())
+        assert bool((h[0, 1, 5] == 0).all()) if which in (1, 5) else True
+
+
 def test_recurrent_equals_the_chunked_operator():
     """wy_eps = 0: both evaluate the same function (the chunked one to its fp32-class tolerance, 1e-4)."""
     xs, dev, h0 = _inputs(2, 2, 256, 6)
@@ -294,6 +322,24 @@ def test_w4_fp32_range():
     w = pack_w4(q.cuda(), s.cuda(), 32)
     for f in (1e30, 1e-25):
         _w4_check(w4_linear((x * f).cuda(), w) , *w4_ref(x * f, q, s, 32), 96, torch.float32)
+
+
+@pytest.mark.parametrize("M,din", [(3, 200), (3, 131), (12, 200)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_w4_huge_and_infinite_values(M, din, dtype):
+    """Values near the type's end, an infinity (the sign of each weight; NaN where one is 0) and a NaN."""
+    for group in (32, 64, 128):
+        q, s, x, _, _ = _w4_inputs(M, din, 50, group, dtype, 8)
+        w = pack_w4(q.cuda(), s.cuda(), group)
+        big = (x.float() * 1e36).to(dtype)
+        _w4_check(w4_linear(big.cuda(), w), *w4_ref(big, q, s, group), din, dtype)
+        x[1, 77], x[2, 9] = -math.inf, float("nan")
+        y = w4_linear(x.cuda(), w).float().cpu()
+        want = x[1:2].double() @ (q.double() * s.double().repeat_interleave(group, 0)[:din])
+        assert torch.equal(torch.isnan(y[1]), torch.isnan(want[0])) and bool(torch.isnan(y[2]).all())
+        assert torch.equal(torch.nan_to_num(y[1], nan=0.0, posinf=1.0, neginf=-1.0).double(),
+                           torch.nan_to_num(want[0], nan=0.0, posinf=1.0, neginf=-1.0))
+        _w4_check(w4_linear(x[:1].cuda(), w), *w4_ref(x[:1], q, s, group), din, dtype)
 
 
 def test_w4_refusals():
@@ -436,5 +482,30 @@ def test_other_stream_and_graph_capture():
         t.mul_(0.5)
     lg.copy_(lg.flip(0))
     graph.replay()
+    want = run()
+    assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_dependent_launches_in_a_graph():
+    """The paths of two launches (x laid out first, slices joined after, blocks of tokens) captured and
+    replayed on new values, on another stream than the one they were captured on."""
+    xs, dev, h0 = _inputs(2, 2, 20, 9)
+    q, s, x, bias, res = _w4_inputs(3, 131, 64, 64, torch.bfloat16, 6)
+    lg, sc, _ = _beam_inputs(1, 3, 20000, torch.float32, 6)
+    fn, w = make_blr_recurrent(make_cfg(), SCALE), pack_w4(q.cuda(), s.cuda(), 64)
+    h0, x, lg, sc = h0.cuda(), x.cuda(), lg.cuda(), sc.cuda()
+    run = lambda: (*fn(*dev, h0), w4_linear(x, w), *beam_select(lg, sc, eos=1))
+    run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for t in (h0, x):
+        t.mul_(0.5)
+    lg.copy_(lg.flip(-1))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        graph.replay()
+    torch.cuda.current_stream().wait_stream(side)
     want = run()
     assert all(torch.equal(a, b) for a, b in zip(out, want))
