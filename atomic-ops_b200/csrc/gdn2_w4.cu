@@ -167,6 +167,9 @@ __device__ __noinline__ float w4_careful(const W4Params& p, int row, int col) {
 // warps side by side (they share x through L1) and 8 / kMB that split the batches, and the CTAs of a
 // cluster split them further.  kPer: scales of a column per batch.
 //
+// Measured (bf16): 4 x 8192 x 8192 12.2 us (2.8 TB/s of weight; 9.7 us without any load, so the slots that
+// widening takes bound it), 16 x 8192 x 8192 17.4 us, 32 x 5000 x 12345 36 us, 8 x 2048 x 512 4.5 us.
+//
 // With one block of bf16 rows the slots count most: the 136 of widen() stays in, and one more product,
 // of x with -136 in every place, is added to each group's sum.  The cancellation costs five
 // bits of fp32 there, 2^-19 of the result, far below its rounding to bf16.  Where it leaves no finite
