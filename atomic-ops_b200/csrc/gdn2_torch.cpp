@@ -10,6 +10,7 @@
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "gdn2_b200.h"
@@ -38,18 +39,12 @@ gdn2_dtype dtype_of(at::ScalarType t) { return t == at::kBFloat16 ? GDN2_BF16 : 
 // Whether `dev` is the current device: the launch and its workspace go there.
 bool current(c10::Device dev) { return dev.index() == c10::cuda::current_device(); }
 
-// A status other than OK leaves the call to the Python path, whose own call reports it.
-#define GDN2_BEGIN try {
-#define GDN2_END                                        \
-  }                                                     \
-  catch (const std::exception& e) {                     \
-    PyErr_SetString(PyExc_RuntimeError, e.what());      \
-    return nullptr;                                     \
-  }
+// A status other than OK leaves the call to the Python path, whose own call reports it.  torch's exceptions
+// (out of memory) become their Python ones.
 
 // recurrent(q, k, v, w, b, g, h0, lengths, h_index, h_out, scale, clip, flags)
 PyObject* recurrent(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  GDN2_BEGIN
+  HANDLE_TH_ERRORS
   if (n != 13) Py_RETURN_NONE;
   gdn2_rec_desc d{};
   const at::Tensor* x[6];
@@ -132,12 +127,12 @@ PyObject* recurrent(PyObject*, PyObject* const* a, Py_ssize_t n) {
       c10::cuda::getCurrentCUDAStream(dev.index()).stream());
   if (s != GDN2_OK) Py_RETURN_NONE;
   return pair(std::move(o), std::move(h));
-  GDN2_END
+  END_HANDLE_TH_ERRORS
 }
 
 // w4_linear(x, packed, scales, bias, residual, din, dout, group, act)
 PyObject* w4_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  GDN2_BEGIN
+  HANDLE_TH_ERRORS
   if (n != 9) Py_RETURN_NONE;
   const at::Tensor *x = plain(a[0]), *w = plain(a[1]), *sc = plain(a[2]);
   if (!x || !w || !sc) Py_RETURN_NONE;
@@ -183,12 +178,12 @@ PyObject* w4_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                        c10::cuda::getCurrentCUDAStream(dev.index()).stream());
   if (s != GDN2_OK) Py_RETURN_NONE;
   return THPVariable_Wrap(std::move(y));
-  GDN2_END
+  END_HANDLE_TH_ERRORS
 }
 
 // beam_select(logits, scores, finished, eos)
 PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  GDN2_BEGIN
+  HANDLE_TH_ERRORS
   if (n != 4) Py_RETURN_NONE;
   const at::Tensor *x = plain(a[0]), *sc = plain(a[1]);
   if (!x || !sc || x->dim() != 3 || sc->dim() != 2) Py_RETURN_NONE;
@@ -241,7 +236,7 @@ PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n) {
   PyTuple_SET_ITEM(r, 2, THPVariable_Wrap(std::move(tokens)));
   PyTuple_SET_ITEM(r, 3, THPVariable_Wrap(std::move(done)));
   return r;
-  GDN2_END
+  END_HANDLE_TH_ERRORS
 }
 
 PyMethodDef methods[] = {
