@@ -50,8 +50,8 @@ __device__ __forceinline__ int valid_len(const RecParams& p, int b, bool report)
 }
 
 // ---------------------------------------------------------------------------------------------
-// One token (or none).  The call moves the states once through the SMs: one CTA holds CW columns
-// of a head's state in registers (a thread has four neighbouring columns of CW / 8 rows).  Both
+// One token (or none).  The call moves the states once through the SMs: one CTA holds a head's
+// state in registers (a thread has four neighbouring columns of 16 rows, a warp whole rows).  Both
 // products read the undecayed state, r = (bk a)^T S and p = (q a)^T S, so one reduction serves
 // them: d = w v - r, o = scale (p + (q . k) d).  Bound by HBM, 128 KB a head: a CTA's 64 KB of loads are
 // in flight before anything is computed.  Measured: 6144 heads 122 us (6.77 TB/s, as fast as a copy), 1536
@@ -59,24 +59,23 @@ __device__ __forceinline__ int valid_len(const RecParams& p, int b, bool report)
 // ---------------------------------------------------------------------------------------------
 constexpr int kStepThreads = 256;
 
-template <class T, int CW>
+template <class T>
 __global__ void __launch_bounds__(kStepThreads) rec_step_kernel(RecParams p) {
-  constexpr int kCols4 = CW / 4;                    // threads along a row
+  constexpr int kCols4 = kD / 4;                    // threads along a row: a warp
   constexpr int kRowsPass = kStepThreads / kCols4;  // rows per pass
   constexpr int kR = kD / kRowsPass;                // rows per thread
   constexpr int kWarps = kStepThreads / 32;
   __shared__ float4 vec[kD];  // a, k, b k a, q a scale
-  __shared__ float wv[CW];
+  __shared__ float wv[kD];
   __shared__ float qk_part[kD / 32];
   __shared__ float4 red[kWarps][2][kCols4];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int bh = blockIdx.x, b = bh / p.H, h = bh % p.H;
-  const int c0 = blockIdx.y * CW;
   const int cx = tid % kCols4, ry = tid / kCols4;
-  const bool first = tid == 0 && h == 0 && blockIdx.y == 0;
+  const bool first = tid == 0 && h == 0;
   const int row = state_row(p, b, first);
   const int n = valid_len(p, b, first);
-  const size_t tile = (size_t)ry * kD + c0 + cx * 4;
+  const size_t tile = (size_t)ry * kD + cx * 4;
   float4 s[kR];
   if (row >= 0) {
     const float* src = p.h0 + ((size_t)row * p.H + h) * (kD * kD) + tile;
@@ -94,7 +93,7 @@ __global__ void __launch_bounds__(kStepThreads) rec_step_kernel(RecParams p) {
       *reinterpret_cast<float4*>(dst + (size_t)i * kRowsPass * kD) =
           make_float4(sanitize(x.x, p.clip), sanitize(x.y, p.clip), sanitize(x.z, p.clip), sanitize(x.w, p.clip));
     }
-    if (p.L > 0 && tid < CW) p.o[b * p.ob + h * p.oh + c0 + tid] = 0.f;
+    if (p.L > 0 && tid < kD) p.o[b * p.ob + h * p.oh + tid] = 0.f;
     return;
   }
   if (tid < kD) {
@@ -109,9 +108,9 @@ __global__ void __launch_bounds__(kStepThreads) rec_step_kernel(RecParams p) {
 #pragma unroll
     for (int m = 16; m > 0; m >>= 1) qk += __shfl_xor_sync(0xffffffffu, qk, m);
     if (lane == 0) qk_part[warp] = qk;
-  } else if (tid - kD < CW) {
-    const int c = c0 + tid - kD;
-    wv[tid - kD] = ld1(static_cast<const T*>(p.v) + b * p.sb[2] + h * p.sh[2] + c) *
+  } else {
+    const int c = tid - kD;
+    wv[c] = ld1(static_cast<const T*>(p.v) + b * p.sb[2] + h * p.sh[2] + c) *
                    ld1(static_cast<const T*>(p.w) + b * p.sb[3] + h * p.sh[3] + c);
   }
   __syncthreads();
@@ -124,18 +123,8 @@ __global__ void __launch_bounds__(kStepThreads) rec_step_kernel(RecParams p) {
     o.x = fmaf(f.w, s[i].x, o.x); o.y = fmaf(f.w, s[i].y, o.y);
     o.z = fmaf(f.w, s[i].z, o.z); o.w = fmaf(f.w, s[i].w, o.w);
   }
-  // threads of a warp that share columns (kCols4 < 32), then the warps
-#pragma unroll
-  for (int m = 16; m >= kCols4; m >>= 1) {
-    r.x += __shfl_xor_sync(0xffffffffu, r.x, m); r.y += __shfl_xor_sync(0xffffffffu, r.y, m);
-    r.z += __shfl_xor_sync(0xffffffffu, r.z, m); r.w += __shfl_xor_sync(0xffffffffu, r.w, m);
-    o.x += __shfl_xor_sync(0xffffffffu, o.x, m); o.y += __shfl_xor_sync(0xffffffffu, o.y, m);
-    o.z += __shfl_xor_sync(0xffffffffu, o.z, m); o.w += __shfl_xor_sync(0xffffffffu, o.w, m);
-  }
-  if (lane < kCols4) {
-    red[warp][0][cx] = r;
-    red[warp][1][cx] = o;
-  }
+  red[warp][0][cx] = r;
+  red[warp][1][cx] = o;
   __syncthreads();
   r = make_float4(0.f, 0.f, 0.f, 0.f);
   o = r;
@@ -159,7 +148,7 @@ __global__ void __launch_bounds__(kStepThreads) rec_step_kernel(RecParams p) {
   }
   if (ry == 0) {
     const float qk = qk_part[0] + qk_part[1] + qk_part[2] + qk_part[3];
-    *reinterpret_cast<float4*>(p.o + b * p.ob + h * p.oh + c0 + cx * 4) =
+    *reinterpret_cast<float4*>(p.o + b * p.ob + h * p.oh + cx * 4) =
         make_float4(sanitize(fmaf(qk, d.x, o.x), p.clip), sanitize(fmaf(qk, d.y, o.y), p.clip),
                     sanitize(fmaf(qk, d.z, o.z), p.clip), sanitize(fmaf(qk, d.w, o.w), p.clip));
   }
@@ -700,7 +689,7 @@ int seg_blocks(long long BH, int L) {
 template <class T>
 cudaError_t launch(const RecParams& p, int BH, float* rec, cudaStream_t st) {
   if (p.L <= 1) {
-    rec_step_kernel<T, 128><<<dim3(BH, 1), kStepThreads, 0, st>>>(p);
+    rec_step_kernel<T><<<BH, kStepThreads, 0, st>>>(p);
     return cudaGetLastError();
   }
   const int seg = seg_blocks(BH, p.L);
