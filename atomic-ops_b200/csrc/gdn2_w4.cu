@@ -43,18 +43,14 @@ __device__ __forceinline__ void mma16816(float c[4], const uint32_t a[4], uint32
 }
 
 // Eight nibbles -> four bf16 pairs.  0x4300 is 128, whose last mantissa bit is worth 1: 136 + Q by an
-// OR; subtracting 136 is exact.  Without kExact the 136 stays in, see w4_kernel.
-template <bool kExact>
+// OR; subtracting 136 is exact.
 __device__ __forceinline__ void widen(uint32_t w, uint32_t a[4]) {
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     uint32_t v = ((w >> (4 * r)) & 0x000f000fu) | 0x43004300u;
-    if constexpr (kExact) {
-      const uint32_t off = 0x43084308u;
-      __nv_bfloat162 d = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&off));
-      v = *reinterpret_cast<uint32_t*>(&d);
-    }
-    a[r] = v;
+    const uint32_t off = 0x43084308u;
+    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&v), *reinterpret_cast<const __nv_bfloat162*>(&off));
+    a[r] = *reinterpret_cast<const uint32_t*>(&d);
   }
 }
 
@@ -141,43 +137,17 @@ __device__ __forceinline__ void load_quarter(const W4Params& p, const T* const x
 template <int kTerms, int kMB>
 constexpr bool kTwoCtas = kMB == 1 || (kTerms == 1 && kMB == 2);
 
-// One output's sum over k, value by value.
-template <class T, int kPer>
-__device__ __noinline__ float w4_careful(const W4Params& p, int row, int col) {
-  const int cb = col >> 5, v = (col >> 4) & 1, c = (col >> 3) & 1, l = col & 7;
-  const T* x = static_cast<const T*>(p.x) + (long long)row * p.xs;
-  float y = 0.f, part = 0.f;
-  for (int k = 0; k < p.K; ++k) {
-    const size_t block = (size_t)cb * p.NB + (k >> 7);
-    const int u = (k >> 6) & 1, s = ((k >> 5) & 1) * 2 + ((k >> 2) & 1), t = (k >> 3) & 3;
-    const uint32_t word = reinterpret_cast<const uint32_t*>(p.w)[((block * 4 + u * 2 + v) * 32 + l * 4 + t) * 4 + s];
-    const int q = (int)((word >> (4 * (c + (k & 2) + 4 * (k & 1)))) & 15) - 8;
-    part = fmaf((float)q, ld1(x + k), part);
-    if (k + 1 == p.K || (k + 1) % (128 / kPer) == 0) {
-      const uint16_t* sc = reinterpret_cast<const uint16_t*>(p.scales);
-      const uint32_t bits = sc[(((block * 2 + v) * 8 + l) * kPer + (k & 127) / (128 / kPer)) * 2 + c];
-      y = fmaf(__uint_as_float(bits << 16), part, y);
-      part = 0.f;
-    }
-  }
-  return y;
-}
-
 // A warp computes 32 columns for 8 kMB rows over its share of the batches of 128 rows; a CTA has kMB
 // warps side by side (they share x through L1) and 8 / kMB that split the batches, and the CTAs of a
 // cluster split them further.  kPer: scales of a column per batch.
 //
-// Measured (bf16): 4 x 8192 x 8192 12.2 us (2.8 TB/s of weight; 9.7 us without any load, so the slots that
-// widening takes bound it), 16 x 8192 x 8192 17.4 us, 32 x 5000 x 12345 36 us, 8 x 2048 x 512 4.5 us.
-//
-// With one block of bf16 rows the slots count most: the 136 of widen() stays in, and one more product,
-// of x with -136 in every place, is added to each group's sum.  The cancellation costs five
-// bits of fp32 there, 2^-19 of the result, far below its rounding to bf16.  Where it leaves no finite
-// value (x beyond 2^121, infinities, NaN) the sum is done again without it.
+// Measured (bf16): 4 x 8192 x 8192 11.8 us (2.9 TB/s of weight), 16 x 8192 x 8192 16.1 us, 32 x 5000 x 12345
+// 35.4 us, 8 x 2048 x 512 3.7 us.  Widening takes 136 out of every value before the product: leaving it in and
+// taking 136 sum x out of the group's sum costs the bits of every x that is far below the group's largest,
+// and was no faster (12.2 us).
 template <class T, int kTerms, int kMB, int kPer, bool kPacked>
 __global__ void __launch_bounds__(kW4Warps * 32, kTwoCtas<kTerms, kMB> ? 2 : 1) w4_kernel(W4Params p) {
   constexpr int kWN = kMB, kWK = kW4Warps / kWN, kCols = kWN * 32, kRows = kMB * 8 + 1;
-  constexpr bool kExact = kTerms > 1 || kMB > 1;
   __shared__ float part[kW4Warps * 32 * kRows];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int wk = warp / kWN, wn = warp % kWN;
@@ -236,7 +206,7 @@ __global__ void __launch_bounds__(kW4Warps * 32, kTwoCtas<kTerms, kMB> ? 2 : 1) 
     for (int i = 0; i < 4; ++i) cur[i] = w[i];
     cs[0] = sc[0]; cs[1] = sc[1];
     if (nb + step < p.NB) fetch();
-    float acc[2][kMB][4], base[4];
+    float acc[2][kMB][4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       uint32_t f[kMB][kTerms][4];
@@ -255,18 +225,12 @@ __global__ void __launch_bounds__(kW4Warps * 32, kTwoCtas<kTerms, kMB> ? 2 : 1) 
 #pragma unroll
           for (int j = 0; j < kMB; ++j) acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.f;
       }
-      if constexpr (!kExact) {
-        const uint32_t off[4] = {0xc308c308u, 0xc308c308u, 0xc308c308u, 0xc308c308u};
-        if (start) base[0] = base[1] = base[2] = base[3] = 0.f;
-        mma16816(base, off, f[0][0][0], f[0][0][1]);
-        mma16816(base, off, f[0][0][2], f[0][0][3]);
-      }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const uint4 v = cur[(q >> 1) * 2 + i];
         uint32_t a0[4], a1[4];
-        widen<kExact>(q & 1 ? v.z : v.x, a0);
-        widen<kExact>(q & 1 ? v.w : v.y, a1);
+        widen(q & 1 ? v.z : v.x, a0);
+        widen(q & 1 ? v.w : v.y, a1);
 #pragma unroll
         for (int j = 0; j < kMB; ++j)
 #pragma unroll
@@ -277,10 +241,6 @@ __global__ void __launch_bounds__(kW4Warps * 32, kTwoCtas<kTerms, kMB> ? 2 : 1) 
         if (end) {
           const uint32_t u = cs[i].v[q / (4 / kPer)];
           const float s0 = __uint_as_float(u << 16), s1 = __uint_as_float(u & 0xffff0000u);
-          if constexpr (!kExact) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) acc[i][0][c] += base[c];
-          }
 #pragma unroll
           for (int j = 0; j < kMB; ++j) {
             sum[i][j][0] = fmaf(s0, acc[i][j][0], sum[i][j][0]);
@@ -335,9 +295,6 @@ __global__ void __launch_bounds__(kW4Warps * 32, kTwoCtas<kTerms, kMB> ? 2 : 1) 
     } else {
 #pragma unroll
       for (int i = 0; i < kWK; ++i) y += *local(i * kCols + n, m);
-    }
-    if constexpr (!kExact) {
-      if (!isfinite(y)) y = w4_careful<T, kPer>(p, row, col);
     }
     if (p.bias) y += p.bias[col];
     if (p.gelu) y = gelu_tanh(y);

@@ -342,6 +342,21 @@ def test_w4_huge_and_infinite_values(M, din, dtype):
         _w4_check(w4_linear(x[:1].cuda(), w), *w4_ref(x[:1], q, s, group), din, dtype)
 
 
+@pytest.mark.parametrize("M", [1, 8, 9])
+@pytest.mark.parametrize("far", [1e3, 1e5, 1e6, 2.0 ** 30])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_w4_one_value_far_above_the_rest(M, far, dtype):
+    """A value of x that a zero weight leaves out of half the columns (and the smallest weights let into the
+    others) must not cost those columns their bits."""
+    for group in (32, 64, 128):
+        q, s, x, _, _ = _w4_inputs(M, 512, 64, group, dtype, 17)
+        for k in (5, 77, 300):
+            x[:, k] = far
+            q[k, :32], q[k, 32:] = 0, torch.tensor([1, -1], dtype=torch.int8).repeat(16)
+        w = pack_w4(q.cuda(), s.cuda(), group)
+        _w4_check(w4_linear(x.cuda(), w), *w4_ref(x, q, s, group), 512, dtype)
+
+
 def test_w4_refusals():
     q, s, x, bias, res = (t.cuda() for t in _w4_inputs(2, 64, 16, 64, torch.float32, 5))
     w = pack_w4(q, s, 64)
