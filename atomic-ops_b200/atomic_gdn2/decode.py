@@ -24,25 +24,31 @@ from .recurrent import make_blr_recurrent
 from .w4 import quantize_w4, w4_linear
 
 
+def _own(p):
+    """A parameter's values in memory of their own."""
+    return p.detach().clone(memory_format=torch.contiguous_format)
+
+
 class _Layer:
     def __init__(self, layer, group):
-        pack = lambda w, b: (quantize_w4(w, group), b.detach().float().contiguous())
+        pack = lambda w, b: (quantize_w4(w, group), _own(b).float())
         self.proj, self.o = pack(layer.proj_w, layer.proj_b), pack(layer.o_w, layer.o_b)
         self.up, self.down = pack(layer.up_w, layer.up_b), pack(layer.down_w, layer.down_b)
 
 
 class BeamDecoder:
     """A GDN2LM (on a CUDA device, fp32) with its weights packed to 4 bits, `group` rows per scale.  The
-    model itself is not changed and not needed afterwards."""
+    model itself is not changed and not needed afterwards: biases and embedding are copies, so a model that
+    is trained further leaves the decoder as it was made."""
 
     def __init__(self, model, group: int = 64):
         lay = model.layers[0]
         self.n_heads, self.d_head, self.l2norm_k, self.cfg = lay.n_heads, lay.d_head, model.l2norm_k, model.cfg
-        self.embed = model.embed.detach()
+        self.embed = _own(model.embed)
         if not self.embed.is_cuda:
             raise RuntimeError("BeamDecoder: the model must be on a CUDA device (the operators run only on the B200 kernels)")
         self.layers = [_Layer(x, group) for x in model.layers]
-        self.head = quantize_w4(model.head_w, group), model.head_b.detach().float().contiguous()
+        self.head = quantize_w4(model.head_w, group), _own(model.head_b).float()
         self.blr = make_blr_recurrent(model.cfg, 1.0 / math.sqrt(self.d_head))
 
     def _layers(self, x, states, lengths, rows):

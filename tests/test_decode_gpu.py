@@ -100,6 +100,21 @@ def test_search_scores_are_the_models(eos):
     assert last_status() == 0
 
 
+def test_decoder_keeps_its_own_weights():
+    """Training the model further changes nothing of a decoder that was made before."""
+    m = _model()
+    dec = BeamDecoder(m)
+    toks = torch.randint(0, V, (2, 6), generator=torch.Generator().manual_seed(8)).cuda()
+    want, _ = dec.prefill(toks)
+    best = dec.search(toks, beams=2, steps=3, eos=1)
+    with torch.no_grad():
+        for p in m.parameters():
+            p.mul_(-0.5).add_(0.25)
+    got, _ = dec.prefill(toks)
+    assert torch.equal(got, want)
+    assert all(torch.equal(a, b) for a, b in zip(dec.search(toks, beams=2, steps=3, eos=1), best))
+
+
 def test_decoder_refusals():
     m = _model(1)
     with pytest.raises(RuntimeError):
