@@ -27,6 +27,8 @@ struct RecParams {
   int H, L, n_states;
   float scale, clip;
 };
+// 0, or NaN if x is not finite; summed up it tells whether any value was not.
+__device__ __forceinline__ float not_finite(float x) { return x * 0.f; }
 
 // The state row of sequence b in h0, or -1 for zeros.
 __device__ __forceinline__ int state_row(const RecParams& p, int b, bool report) {
@@ -146,12 +148,35 @@ __global__ void __launch_bounds__(kStepThreads) rec_step_kernel(RecParams p) {
     x.w = sanitize(fmaf(f.y, d.w, f.x * x.w), p.clip);
     *reinterpret_cast<float4*>(dst + (size_t)i * kRowsPass * kD) = x;
   }
-  if (ry == 0) {
-    const float qk = qk_part[0] + qk_part[1] + qk_part[2] + qk_part[3];
-    *reinterpret_cast<float4*>(p.o + b * p.ob + h * p.oh + cx * 4) =
-        make_float4(sanitize(fmaf(qk, d.x, o.x), p.clip), sanitize(fmaf(qk, d.y, o.y), p.clip),
-                    sanitize(fmaf(qk, d.z, o.z), p.clip), sanitize(fmaf(qk, d.w, o.w), p.clip));
+  const float qk = qk_part[0] + qk_part[1] + qk_part[2] + qk_part[3];
+  o = make_float4(fmaf(qk, d.x, o.x), fmaf(qk, d.y, o.y), fmaf(qk, d.z, o.z), fmaf(qk, d.w, o.w));
+  // With an infinity about, p + (q . k) d is not q^T S (k_j d and S_j may cancel to a NaN): o is summed from the
+  // new state then.  Every warp has all columns, so the warps of the CTA agree.
+  const float probe = not_finite(o.x) + not_finite(o.y) + not_finite(o.z) + not_finite(o.w);
+  if (__any_sync(0xffffffffu, probe != 0.f)) {
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < kR; ++i) {
+      const float4 f = vec[ry + i * kRowsPass];
+      const float q = ld1(static_cast<const T*>(p.q) + b * p.sb[0] + h * p.sh[0] + ry + i * kRowsPass);
+      o.x = fmaf(q, fmaf(f.y, d.x, f.x * s[i].x), o.x);
+      o.y = fmaf(q, fmaf(f.y, d.y, f.x * s[i].y), o.y);
+      o.z = fmaf(q, fmaf(f.y, d.z, f.x * s[i].z), o.z);
+      o.w = fmaf(q, fmaf(f.y, d.w, f.x * s[i].w), o.w);
+    }
+    __syncthreads();  // red is read no more
+    red[warp][0][cx] = o;
+    __syncthreads();
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i < kWarps; ++i) {
+      const float4 x = red[i][0][cx];
+      o.x = fmaf(p.scale, x.x, o.x); o.y = fmaf(p.scale, x.y, o.y);
+      o.z = fmaf(p.scale, x.z, o.z); o.w = fmaf(p.scale, x.w, o.w);
+    }
   }
+  if (ry == 0)
+    *reinterpret_cast<float4*>(p.o + b * p.ob + h * p.oh + cx * 4) =
+        make_float4(sanitize(o.x, p.clip), sanitize(o.y, p.clip), sanitize(o.z, p.clip), sanitize(o.w, p.clip));
 }
 
 // ---------------------------------------------------------------------------------------------

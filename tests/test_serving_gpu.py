@@ -184,6 +184,35 @@ def test_recurrent_nan_counts_from_its_token_on(which, col, B):
         assert bool((h[0, 1, 5] == 0).all()) if which in (1, 5) else True
 
 
+def _same_with_infinities(got, ref, clip=1e4):
+    """What an infinity or a NaN reaches is 0 or at the bound, exactly as in 64 bits; the rest as ever."""
+    got, at = got.detach().double().cpu(), (ref == 0) | (ref.abs() == clip)
+    assert torch.equal(got[at], ref[at])
+    assert bool(at.all()) or float((got[~at] - ref[~at]).norm() / ref[~at].norm()) < REC_TOL
+
+
+@pytest.mark.parametrize("B", [1, 40])
+@pytest.mark.parametrize("L,at", [(1, 0)])
+@pytest.mark.parametrize("which,value", [(0, math.inf), (1, math.inf), (2, math.inf), (3, -math.inf), (4, math.inf),
+                                         (5, -math.inf), ("h0", math.inf), ("h0", math.nan)])
+def test_recurrent_infinities(which, value, L, at, B):
+    """An infinity in one token of one head, or in its state: in the token's o and in the state what the
+    recurrence makes of it, the bound where it stays an infinity and 0 where it becomes a NaN."""
+    xs, dev, h0 = _inputs(B, 3, L, 23)
+    for t in xs[:2] + dev[:2]:
+        t[0, 2] = t[0, 2].abs()                # one head whose sums of infinities keep their sign
+    for head in (1, 2):
+        if which == "h0":
+            h0[0, head, 50, 7] = value
+        else:
+            for t in (xs, dev):
+                t[which][0, head, at, 7] = value
+    o, h = make_blr_recurrent(make_cfg(), SCALE)(*dev, h0.cuda())
+    o_r, h_r = recurrent_ref(*xs, SCALE, h0)
+    _same_with_infinities(o, o_r)
+    _same_with_infinities(h, h_r)
+
+
 def test_recurrent_equals_the_chunked_operator():
     """wy_eps = 0: both evaluate the same function (the chunked one to its fp32-class tolerance, 1e-4)."""
     xs, dev, h0 = _inputs(2, 2, 256, 6)
