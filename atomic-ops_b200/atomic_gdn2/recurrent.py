@@ -14,7 +14,8 @@ raises at once, set_checks(False) leaves it to last_status(); nothing is checked
 being captured (make a device's first call outside a capture: it sets that memory up).
 
 A value that is not finite counts from its token on: in q for that token's o, in v or w for its
-column, in k, b or g for the head; what it reaches is sanitized to 0 (a NaN) or to the bound.
+column, in k, b or g for the head.  What it reaches is what the recurrence makes of it, a NaN sanitized
+to 0 and an infinity to the bound; where there are several tokens such columns take about 0.6 us each.
 """
 from __future__ import annotations
 

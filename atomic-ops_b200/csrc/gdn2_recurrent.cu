@@ -26,6 +26,7 @@ struct RecParams {
   uint32_t* flags;                // [0] a positive gate was seen, [1] an index or length out of range, [2] a wait ran out
   int H, L, n_states;
   float scale, clip;
+  int bf16;                       // the type of q..g, for code that is not compiled for one
 };
 // 0, or NaN if x is not finite; summed up it tells whether any value was not.
 __device__ __forceinline__ float not_finite(float x) { return x * 0.f; }
@@ -201,6 +202,10 @@ __global__ void __launch_bounds__(kStepThreads) rec_step_kernel(RecParams p) {
 // the shared-memory traffic of the vectors (every lane needs its own copy), measured 2 to 6 times
 // slower.  Sums of the state itself stay outside the tensor instruction, whose additions may
 // truncate: U = sum_t k_t d_t^T there, S <- e S + U in fp32.
+//
+// A value that is not finite reaches every token of its block in these products, and an infinity has no lo.
+// It always shows in a d or an o: a CTA that has met one does its columns again from the launch's first
+// token on, by the definition, token by token (seq_literal).
 // ---------------------------------------------------------------------------------------------
 constexpr int kSmCount = 148;  // of a B200
 constexpr int kTok = 8;
@@ -425,41 +430,97 @@ __device__ __forceinline__ void seq_store(const float s[kJ][4], const RecParams&
     for (int c = 0; c < 4; ++c)
       to[(j * 8 + (c & 1)) * kD + (c >> 1) * 8] = last ? sanitize(s[j][c], p.clip) : s[j][c];
 }
-// o + P d, stored for the block's valid tokens.  `pm`: the record's P.  The product's zeros above P's
-// diagonal would carry a d that is not finite into the tokens before it: then it is done token by token.
-__device__ __noinline__ void seq_out_careful(float o[4], const float dl[4], const float* pm) {
-  const int lane = threadIdx.x & 31, t = lane & 3;
-#pragma unroll 1
-  for (int s = 0; s < kTok; ++s) {
-    const int from = (lane & ~3) | (s >> 1);
-    const float lo0 = __shfl_sync(0xffffffffu, dl[0], from), lo1 = __shfl_sync(0xffffffffu, dl[1], from);
-    const float hi0 = __shfl_sync(0xffffffffu, dl[2], from), hi1 = __shfl_sync(0xffffffffu, dl[3], from);
-    const float d0 = s & 1 ? lo1 : lo0, d1 = s & 1 ? hi1 : hi0;
+// The launch's tokens by the definition, for 16 columns from `col` on (the CTA's column `mine`), by the CTA's first
+// four warps: a thread has 16 rows of a column.  The state has not been written back yet, and the records are done with: 19 KB
+// of their place are used.  Measured: 0.6 us a token (the latency of its loads and barriers).
+constexpr int kLitThreads = 128;
+template <class T>
+__device__ __noinline__ void seq_literal(const RecParams& p, const SeqSpan& r, const float* state, int tok0, int col,
+                                         int mine, bool last) {
+  extern __shared__ float4 smem4[];
+  float* mem = reinterpret_cast<float*>(smem4);
+  const int tid = threadIdx.x, c = tid & 15, d0 = (tid >> 4) * 16, warp = tid >> 5, row = tid >> 4;
+  const long long b = blockIdx.x / p.H, h = blockIdx.x % p.H;
+  float (*vec)[4][kD] = reinterpret_cast<float (*)[4][kD]>(mem);                                    // a, k, b k, q of a token
+  float (*wv)[16] = reinterpret_cast<float (*)[16]>(mem + kTok * 4 * kD);
+  float (*part)[4][16] = reinterpret_cast<float (*)[4][16]>(mem + kTok * (4 * kD + 16));            // by a token's parity
+  float (*outs)[4][16] = reinterpret_cast<float (*)[4][16]>(mem + kTok * (4 * kD + 16) + 2 * 64);   // by token
+  auto barrier = [] { asm volatile("bar.sync 2, %0;" ::"n"(kLitThreads) : "memory"); };
+  auto in = [&](const void* x, int i, int t, int d) {
+    return ld1(static_cast<const T*>(x) + b * p.sb[i] + h * p.sh[i] + (tok0 + t) * p.sl[i] + d);
+  };
+  const size_t at = (size_t)d0 * kD + col + c;
+  float s[16];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int tok = 2 * t + (c & 1);
-      if (s <= tok) o[c] = fmaf(pm[tok * kTok + s], c & 2 ? d1 : d0, o[c]);
+  for (int i = 0; i < 16; ++i) s[i] = r.state >= 0 ? state[r.state + at + i * kD] : 0.f;
+  for (int t0 = 0; t0 < r.n; t0 += kTok) {
+    const int n = min(kTok, r.n - t0);
+    float x[kTok][4];
+#pragma unroll
+    for (int t = 0; t < kTok; ++t) {  // all of the loads first; the last token stands in for those past it
+      const int tt = t0 + min(t, n - 1);
+      x[t][0] = in(p.g, 5, tt, tid);
+      x[t][1] = in(p.k, 1, tt, tid);
+      x[t][2] = in(p.b, 4, tt, tid);
+      x[t][3] = in(p.q, 0, tt, tid);
     }
-  }
-}
-__device__ __forceinline__ void seq_out(const RecParams& p, const SeqSpan& r, int blk, int col, const float in[4],
-                                        const float dl[4], const SplitA& d, const float* pm) {
-  const int lane = threadIdx.x & 31, t = lane & 3;
-  float o[4] = {in[0], in[1], in[2], in[3]};
-  const float probe = (dl[0] - dl[0]) + (dl[1] - dl[1]) + (dl[2] - dl[2]) + (dl[3] - dl[3]);  // 0, or NaN
-  if (__any_sync(0xffffffffu, probe != 0.f)) {
-    seq_out_careful(o, dl, pm);
-  } else {
-    const float2 f = *reinterpret_cast<const float2*>(pm + lane * 2);
-    float big[4] = {}, small[4] = {};
-    mma3(big, small, d, f.x, f.y);
+    barrier();  // the tokens before are done with
 #pragma unroll
-    for (int c = 0; c < 4; ++c) o[c] += big[c] + small[c];
+    for (int t = 0; t < kTok; ++t) {
+      vec[t][0][tid] = expf(x[t][0] > 0.f ? 0.f : x[t][0]);
+      vec[t][1][tid] = x[t][1];
+      vec[t][2][tid] = x[t][2] * x[t][1];
+      vec[t][3][tid] = x[t][3];
+    }
+    if (row < n) wv[row][c] = in(p.w, 3, t0 + row, col + c) * in(p.v, 2, t0 + row, col + c);
+    barrier();
+    for (int t = 0; t < n; ++t) {
+      float sum = 0.f, out = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[i] *= vec[t][0][d0 + i];
+        sum = fmaf(vec[t][2][d0 + i], s[i], sum);
+      }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+      if ((tid & 16) == 0) part[t & 1][warp][c] = sum;
+      barrier();
+      const float d = wv[t][c] - ((part[t & 1][0][c] + part[t & 1][1][c]) + (part[t & 1][2][c] + part[t & 1][3][c]));
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[i] = fmaf(vec[t][1][d0 + i], d, s[i]);
+        out = fmaf(vec[t][3][d0 + i], s[i], out);
+      }
+      out += __shfl_xor_sync(0xffffffffu, out, 16);
+      if ((tid & 16) == 0) outs[t][warp][c] = out;
+    }
+    barrier();
+    if (row < n)
+      r.o[(t0 + row) * p.ol + mine + c] =
+          sanitize(p.scale * ((outs[row][0][c] + outs[row][1][c]) + (outs[row][2][c] + outs[row][3][c])), p.clip);
   }
+  float* to = p.h_out + (size_t)blockIdx.x * (kD * kD) + at;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) to[i * kD] = last ? sanitize(s[i], p.clip) : s[i];
+}
+__device__ __forceinline__ void seq_again(const RecParams& p, const SeqSpan& r, const float* state, int tok0, int col,
+                                          int mine, bool last) {
+  if (p.bf16) seq_literal<__nv_bfloat16>(p, r, state, tok0, col, mine, last);
+  else seq_literal<float>(p, r, state, tok0, col, mine, last);
+}
+__device__ __forceinline__ float not_finite4(const float x[4]) {
+  return (not_finite(x[0]) + not_finite(x[1])) + (not_finite(x[2]) + not_finite(x[3]));
+}
+// o + P d, stored for the block's valid tokens.  `pm`: the record's P.
+__device__ __forceinline__ void seq_out(const RecParams& p, const SeqSpan& r, int blk, int col, const float o[4],
+                                        const SplitA& d, const float* pm) {
+  const int lane = threadIdx.x & 31, t = lane & 3;
+  const float2 f = *reinterpret_cast<const float2*>(pm + lane * 2);
+  float big[4] = {}, small[4] = {};
+  mma3(big, small, d, f.x, f.y);
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     const int tok = blk * kTok + 2 * t + (c & 1);
-    if (tok < r.n) r.o[tok * p.ol + col + (c >> 1) * 8] = sanitize(o[c], p.clip);
+    if (tok < r.n) r.o[tok * p.ol + col + (c >> 1) * 8] = sanitize(o[c] + (big[c] + small[c]), p.clip);
   }
 }
 template <int kJ>
@@ -509,11 +570,11 @@ struct SeqRing {
 
 // Many heads: a warp owns 16 columns and all of d, a CTA kCT such tiles.  Bound by the tensor pipe (144
 // products of 8 cycles a warp and block, half busy) and the splits' integer slots.  Measured: 384 heads x 80
-// tokens 80 us, 11 us of it the floor of its bytes.  The records arrive
-// through a ring.
+// tokens 71 us, 11 us of it the floor of its bytes.  The records arrive through a ring.  The bound of
+// three CTAs an SM gives a thread 168 registers; without it the compiler takes 128 and spills (75 us).
 template <int kCT>
-__global__ void __launch_bounds__(kCT * 32) rec_wide_kernel(RecParams p, const float* rec, const float* state,
-                                                          int tok0, int nblk, bool first, bool last) {
+__global__ void __launch_bounds__(kCT * 32, 3) rec_wide_kernel(const __grid_constant__ RecParams p, const float* rec,
+                                                             const float* state, int tok0, int nblk, bool first, bool last) {
   constexpr int kThreads = kCT * 32, kSlots = 3, kSlot = kRecV + kCT * 128;
   extern __shared__ float4 smem4[];
   __shared__ uint64_t bars[kSlots];
@@ -534,6 +595,7 @@ __global__ void __launch_bounds__(kCT * 32) rec_wide_kernel(RecParams p, const f
   };
 #pragma unroll
   for (int i = 0; i < kSlots - 1; ++i) fetch(i);
+  float probe = 0.f;
   for (int blk = 0; blk < r.blocks; ++blk) {
     ring.wait(blk % kSlots, (blk / kSlots) & 1);
     __syncthreads();          // every warp is done with block blk - 1
@@ -558,22 +620,28 @@ __global__ void __launch_bounds__(kCT * 32) rec_wide_kernel(RecParams p, const f
     const float4 v = lds4(slot + kRecV + (ct * 32 + lane) * 4);
     const float dl[4] = {v.x - rr[0], v.y - rr[1], v.z - rr[2], v.w - rr[3]};
     const SplitA d = split_tile(dl);
-    seq_out(p, r, blk, ct * 16 + g, o, dl, d, slot + kRecP);
+    probe += not_finite4(dl) + not_finite4(o);
+    seq_out(p, r, blk, ct * 16 + g, o, d, slot + kRecP);
     seq_update<16>(s, d, slot, 0, lane);
   }
-  seq_store<16>(s, p, mine, last);
+  static_assert(kThreads == kLitThreads);
+  if (!__syncthreads_or(probe != 0.f)) {
+    seq_store<16>(s, p, mine, last);
+  } else {
+    for (int i = 0; i < kCT; ++i) seq_again(p, r, state, tok0, (blockIdx.y * kCT + i) * 16, i * 16, last);
+  }
 }
 
-// Few heads, where a block's chain of dependent steps is what counts (measured: 420 ns for 8 tokens, 6 heads
-// x 4096 tokens 215 us): kW warps share 16 columns and
-// take 16 / kW tiles of d each; one more warp sees to the records and one finishes the outputs, a
-// block behind.  One barrier per block: before it the partial sums r of the block are written, after
+// Few heads, where a block's chain of dependent steps is what counts (measured: 425 ns for 8 tokens, 6 heads
+// x 4096 tokens 218 us): kW warps share 16 columns and take 16 / kW tiles of d each; one more warp sees to the
+// records and one finishes the outputs, a block behind.  Two CTAs fit on an SM by shared memory; the bound
+// of three is for registers (96 a thread; without it the compiler takes 80, and 265 us).  One barrier per block: before it the partial sums r of the block are written, after
 // it every warp adds them up.  What is double-buffered by the block's parity:
 //   rpart  written before barrier blk, read until barrier blk + 1
 //   opart, delta  written after barrier blk, read between barriers blk + 1 and blk + 2
 template <int kW>
-__global__ void __launch_bounds__((kW + 2) * 32) rec_deep_kernel(RecParams p, const float* rec, const float* state,
-                                                               int tok0, int nblk, bool first, bool last) {
+__global__ void __launch_bounds__((kW + 2) * 32, 3) rec_deep_kernel(const __grid_constant__ RecParams p, const float* rec,
+                                                                  const float* state, int tok0, int nblk, bool first, bool last) {
   constexpr int kThreads = (kW + 2) * 32, kJ = 16 / kW, kSlots = 6, kSlot = kRecV + 128;
   extern __shared__ float4 smem4[];
   float* smem = reinterpret_cast<float*>(smem4);
@@ -581,6 +649,7 @@ __global__ void __launch_bounds__((kW + 2) * 32) rec_deep_kernel(RecParams p, co
   float4* opart = rpart + 2 * kW * 32;         // [2][kW][32]
   float4* delta = opart + 2 * kW * 32;         // [2][32]
   __shared__ uint64_t bars[kSlots];
+  __shared__ int bad;  // set before the last barrier, where a warp has met a value that is not finite
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const SeqSpan r = seq_span<kThreads, 16>(p, tok0, nblk, first);
   if (r.blocks == 0 && !first && !last) return;
@@ -588,7 +657,10 @@ __global__ void __launch_bounds__((kW + 2) * 32) rec_deep_kernel(RecParams p, co
   if (warp == kW) {  // copies
     const float* src = rec + (size_t)blockIdx.x * nblk * kRecFloats;
     SeqRing ring{bars, p.flags};
-    if (lane == 0) ring.init(kSlots);
+    if (lane == 0) {
+      ring.init(kSlots);
+      bad = 0;
+    }
     __syncwarp();
     auto fetch = [&](int blk) {
       if (lane == 0 && blk < r.blocks)
@@ -622,10 +694,10 @@ __global__ void __launch_bounds__((kW + 2) * 32) rec_deep_kernel(RecParams p, co
       }
       const float4 x = delta[par * 32 + lane];
       const float dl[4] = {x.x, x.y, x.z, x.w};
-      seq_out(p, r, blk - 1, g, o, dl, split_tile(dl), smem + ((blk - 1) % kSlots) * kSlot + kRecP);
+      seq_out(p, r, blk - 1, g, o, split_tile(dl), smem + ((blk - 1) % kSlots) * kSlot + kRecP);
     }
     barrier();
-    if (r.blocks) {
+    if (r.blocks && !bad) {
       const int blk = r.blocks - 1, par = blk & 1;
       float o[4] = {};
 #pragma unroll
@@ -635,7 +707,7 @@ __global__ void __launch_bounds__((kW + 2) * 32) rec_deep_kernel(RecParams p, co
       }
       const float4 x = delta[par * 32 + lane];
       const float dl[4] = {x.x, x.y, x.z, x.w};
-      seq_out(p, r, blk, g, o, dl, split_tile(dl), smem + (blk % kSlots) * kSlot + kRecP);
+      seq_out(p, r, blk, g, o, split_tile(dl), smem + (blk % kSlots) * kSlot + kRecP);
     }
     return;
   }
@@ -643,6 +715,7 @@ __global__ void __launch_bounds__((kW + 2) * 32) rec_deep_kernel(RecParams p, co
   const size_t mine = (size_t)(8 * j0 + 2 * t) * kD + blockIdx.y * 16 + g;
   float s[kJ][4];
   seq_load<kJ>(s, state, r, mine);
+  float probe = 0.f;
   barrier();
   for (int blk = 0; blk < r.blocks; ++blk) {
     const float* slot = smem + (blk % kSlots) * kSlot;
@@ -673,13 +746,17 @@ __global__ void __launch_bounds__((kW + 2) * 32) rec_deep_kernel(RecParams p, co
     const float dl[4] = {v.x - rr[0], v.y - rr[1], v.z - rr[2], v.w - rr[3]};
     const SplitA d = split_tile(dl);
     seq_update<kJ>(s, d, slot, j0, lane);
-    opart[(par * kW + warp) * 32 + lane] =
-        make_float4((ob[0][0] + ob[1][0]) + (os[0][0] + os[1][0]), (ob[0][1] + ob[1][1]) + (os[0][1] + os[1][1]),
-                    (ob[0][2] + ob[1][2]) + (os[0][2] + os[1][2]), (ob[0][3] + ob[1][3]) + (os[0][3] + os[1][3]));
+    const float o[4] = {(ob[0][0] + ob[1][0]) + (os[0][0] + os[1][0]), (ob[0][1] + ob[1][1]) + (os[0][1] + os[1][1]),
+                        (ob[0][2] + ob[1][2]) + (os[0][2] + os[1][2]), (ob[0][3] + ob[1][3]) + (os[0][3] + os[1][3])};
+    opart[(par * kW + warp) * 32 + lane] = make_float4(o[0], o[1], o[2], o[3]);
+    probe += not_finite4(dl) + not_finite4(o);
     if (warp == 0) delta[par * 32 + lane] = make_float4(dl[0], dl[1], dl[2], dl[3]);
   }
+  if (probe != 0.f) bad = 1;
   barrier();
-  seq_store<kJ>(s, p, mine, last);
+  static_assert(kW * 32 == kLitThreads);
+  if (!bad) seq_store<kJ>(s, p, mine, last);
+  else seq_again(p, r, state, tok0, blockIdx.y * 16, 0, last);
 }
 
 template <class K>
@@ -790,6 +867,7 @@ extern "C" gdn2_status gdn2_recurrent(const gdn2_rec_desc* d, const void* q, con
   p.ob = d->o_stride[0]; p.oh = d->o_stride[1]; p.ol = d->o_stride[2];
   p.h0 = h0; p.h_index = h_index; p.lengths = lengths; p.o = o; p.h_out = h_out; p.flags = flags;
   p.H = d->H; p.L = d->L; p.n_states = d->n_states;
+  p.bf16 = el == 2;
   p.scale = d->scale; p.clip = d->clip;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   float* rec = static_cast<float*>(workspace);

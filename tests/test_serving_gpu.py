@@ -192,7 +192,7 @@ def _same_with_infinities(got, ref, clip=1e4):
 
 
 @pytest.mark.parametrize("B", [1, 40])
-@pytest.mark.parametrize("L,at", [(1, 0)])
+@pytest.mark.parametrize("L,at", [(1, 0), (2, 1), (9, 8), (16, 15), (21, 6), (21, 20)])
 @pytest.mark.parametrize("which,value", [(0, math.inf), (1, math.inf), (2, math.inf), (3, -math.inf), (4, math.inf),
                                          (5, -math.inf), ("h0", math.inf), ("h0", math.nan)])
 def test_recurrent_infinities(which, value, L, at, B):
@@ -209,6 +209,22 @@ def test_recurrent_infinities(which, value, L, at, B):
                 t[which][0, head, at, 7] = value
     o, h = make_blr_recurrent(make_cfg(), SCALE)(*dev, h0.cuda())
     o_r, h_r = recurrent_ref(*xs, SCALE, h0)
+    _same_with_infinities(o, o_r)
+    _same_with_infinities(h, h_r)
+
+
+@pytest.mark.parametrize("B", [2, 60])
+def test_recurrent_infinite_state_of_short_sequences(B):
+    """One token from a state with infinities in a batch of longer ones, and infinities past a sequence's end."""
+    xs, dev, h0 = _inputs(B, 2, 20, 29, torch.bfloat16)
+    h0[0, 1, 3, 5], h0[0, 1, 90, 100], h0[1, 0, 7, 7] = math.inf, -math.inf, math.nan
+    lengths = torch.tensor([1, 0] + [17] * (B - 2), dtype=torch.int32)
+    for t in xs + dev:
+        t[0, :, 1:] = math.inf
+        if B > 2:
+            t[2, :, 17:] = math.nan
+    o, h = make_blr_recurrent(make_cfg(), SCALE)(*dev, h0.cuda(), lengths=lengths.cuda())
+    o_r, h_r = recurrent_ref(*xs, SCALE, h0, lengths)
     _same_with_infinities(o, o_r)
     _same_with_infinities(h, h_r)
 
