@@ -100,6 +100,29 @@ def test_search_scores_are_the_models(eos):
     assert last_status() == 0
 
 
+def test_one_beam_goes_greedily():
+    """Each token is the reference's best one, and the score the sum of their log-probabilities; the first of 32
+    beams over two tokens is the best pair of all (the 32 best first tokens hold it)."""
+    m = _model()
+    dec = BeamDecoder(m)
+    pre = torch.randint(0, V, (4,), generator=torch.Generator().manual_seed(6))
+    out, scores, n = dec.search(pre[None].cuda(), beams=1, steps=5)
+    seq, want = pre, 0.0
+    for tok in out[0, 0].tolist():
+        lp = torch.log_softmax(_ref_logits(m, seq)[-1], -1)
+        assert tok == int(torch.argmax(lp))
+        want += float(lp[tok])
+        seq = torch.cat([seq, torch.tensor([tok])])
+    assert int(n[0, 0]) == 5 and abs(float(scores[0, 0]) - want) < 5 * TOL * max(1.0, abs(want))
+    out, scores, _ = dec.search(pre[None].cuda(), beams=32, steps=2)
+    first = torch.log_softmax(_ref_logits(m, pre)[-1], -1)
+    second = torch.stack([torch.log_softmax(_ref_logits(m, torch.cat([pre, torch.tensor([t])]))[-1], -1) for t in range(V)])
+    total = (first[:, None] + second).flatten()
+    assert float(first.topk(33)[0][-1]) < float(total.max())
+    assert out[0, 0].tolist() == [int(total.argmax()) // V, int(total.argmax()) % V]
+    assert abs(float(scores[0, 0]) - float(total.max())) < 2 * TOL * max(1.0, abs(float(total.max())))
+
+
 def test_decoder_keeps_its_own_weights():
     """Training the model further changes nothing of a decoder that was made before."""
     m = _model()

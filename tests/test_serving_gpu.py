@@ -93,6 +93,36 @@ def test_recurrent_lengths_and_index(L):
         assert torch.equal(keep.cpu(), pool)
 
 
+@pytest.mark.parametrize("B,H,L", [(56, 2, 53), (19, 6, 100)])
+def test_recurrent_many_heads_many_blocks(B, H, L):
+    """112 and 114 heads: the state walks on from block to block, through every slot of the records' ring."""
+    xs, dev, h0 = _inputs(B, H, L, L)
+    o, h = make_blr_recurrent(make_cfg(), SCALE)(*dev, h0.cuda())
+    o_r, h_r = recurrent_ref(*xs, SCALE, h0)
+    assert _rel(o, o_r) < REC_TOL and _rel(h, h_r) < REC_TOL
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("B,H,L,layout", [(120, 3, 173, "bhld"), (32, 3, 345, "blhd")])
+def test_recurrent_records_in_several_segments(B, H, L, layout, in_place):
+    """More records than are kept at a time (64 MiB: 80 tokens of 360 heads, 320 of 96): sequences that are
+    empty, end inside a segment, on its border or in the last one, their states in place or through an index."""
+    xs, dev, h0 = _inputs(B, H, L, 41, layout=layout)
+    gen = torch.Generator().manual_seed(42)
+    lengths = torch.randint(0, L + 1, (B,), generator=gen, dtype=torch.int32)
+    edge = 80 if B * H == 360 else 320
+    lengths[:8] = torch.tensor([L, 0, edge, edge + 1, edge - 1, 1, min(2 * edge, L), L - 1])
+    index = None if in_place else torch.randint(-1, B, (B,), generator=gen, dtype=torch.int32)
+    state = h0.cuda()
+    o, h = make_blr_recurrent(make_cfg(), SCALE)(*dev, state, lengths=lengths.cuda(),
+                                                 **(dict(h_out=state) if in_place else dict(h_index=index.cuda())))
+    o_r, h_r = recurrent_ref(*xs, SCALE, h0, lengths, index)
+    assert (h is state) == in_place and (in_place or torch.equal(state.cpu(), h0))
+    assert _rel(o, o_r) < REC_TOL and _rel(h, h_r) < REC_TOL
+    for i, n in enumerate(lengths.tolist()):
+        assert bool((o[i, :, n:] == 0).all())
+
+
 def test_recurrent_no_tokens():
     h0 = torch.randn(2, 3, D, D, generator=torch.Generator().manual_seed(1)).cuda()
     x = [torch.empty(2, 3, 0, D, device="cuda") for _ in range(6)]
@@ -209,6 +239,36 @@ def test_recurrent_infinities(which, value, L, at, B):
                 t[which][0, head, at, 7] = value
     o, h = make_blr_recurrent(make_cfg(), SCALE)(*dev, h0.cuda())
     o_r, h_r = recurrent_ref(*xs, SCALE, h0)
+    _same_with_infinities(o, o_r)
+    _same_with_infinities(h, h_r)
+
+
+@pytest.mark.parametrize("B", [1, 40])
+@pytest.mark.parametrize("L,at", [(1, 0), (8, 7), (19, 3)])
+@pytest.mark.parametrize("which", range(6))
+def test_recurrent_nan_is_the_recurrences(which, L, at, B):
+    """The state and the outputs after a NaN in one token, value by value."""
+    xs, dev, h0 = _inputs(B, 2, L, 37)
+    for t in (xs, dev):
+        t[which][0, 1, at, 99] = math.nan
+    o, h = make_blr_recurrent(make_cfg(), SCALE)(*dev, h0.cuda())
+    o_r, h_r = recurrent_ref(*xs, SCALE, h0)
+    _same_with_infinities(o, o_r)
+    _same_with_infinities(h, h_r)
+
+
+def test_recurrent_infinities_in_several_segments():
+    """The second of two segments starts from a state with an infinity, and from one that is NaN."""
+    B, H, L = 120, 3, 90
+    xs, dev, h0 = _inputs(B, H, L, 43, torch.bfloat16)
+    for t in (xs, dev):
+        t[2][3, 1, 79, 20] = math.inf
+        t[2][4, 0, 50, 21] = -math.inf
+        t[0][5, 2, 85, 22] = math.inf
+    lengths = torch.full((B,), L, dtype=torch.int32)
+    lengths[3], lengths[6] = 81, 80
+    o, h = make_blr_recurrent(make_cfg(), SCALE)(*dev, h0.cuda(), lengths=lengths.cuda())
+    o_r, h_r = recurrent_ref(*xs, SCALE, h0, lengths)
     _same_with_infinities(o, o_r)
     _same_with_infinities(h, h_r)
 
