@@ -55,8 +55,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished=None, *, eo
         raise ValueError(f"beam_select: eos={eos} is not a token of 0..{V - 1}")
     if finished is not None and (finished.shape != (B, K) or finished.dtype != torch.bool or finished.device != dev):
         raise ValueError(f"beam_select: finished must be bool of shape {(B, K)} on {dev}")
-    if torch.is_grad_enabled() and (logits.requires_grad or scores.requires_grad):
-        raise RuntimeError("beam_select has no backward: call it under torch.no_grad()")
+    pipeline._refuse_gradients("beam_select", (logits, scores))
     if V > 1 and logits.stride(2) != 1:
         logits = logits.contiguous()
     scores = scores.contiguous()

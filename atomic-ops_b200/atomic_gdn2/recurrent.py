@@ -119,8 +119,7 @@ def make_blr_recurrent(cfg: BLRConfig, scale):
             raise NotImplementedError(f"gdn2: head size {D}; the B200 kernels implement {_D}")
         if B == 0 or H == 0:
             raise ValueError(f"gdn2: empty batch or no heads: {tuple(shape)}")
-        if torch.is_grad_enabled() and (any(t.requires_grad for t in xs) or (h0 is not None and h0.requires_grad)):
-            raise RuntimeError("make_blr_recurrent has no backward: use make_blr_trainable, or torch.no_grad()")
+        pipeline._refuse_gradients("make_blr_recurrent", (*xs, h0))
         if not same or dt not in (torch.float32, torch.bfloat16):
             dt = torch.float32
             xs = tuple(t.to(dt) for t in xs)

@@ -127,7 +127,7 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, bias=None, *, act=None, residua
         raise ValueError(f"w4_linear: x is on {dev}, the weight on {weight.device}")
     if act not in _ACTS:
         raise ValueError(f"w4_linear: act={act!r} is not None or 'gelu'")
-    grads = x.requires_grad
+    pipeline._refuse_gradients("w4_linear", (x, bias, residual))
     x2 = x if len(shape) == 2 else x.reshape(-1, din)
     M = x2.shape[0]
     if din > 1 and x2.stride(1) != 1 or x2.data_ptr() % 16:
@@ -137,20 +137,16 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, bias=None, *, act=None, residua
     if bias is not None:
         if bias.shape != (dout,) or bias.device != dev:
             raise ValueError(f"w4_linear: bias must have shape {(dout,)} on {dev}")
-        grads = grads or bias.requires_grad
         if bias.dtype != torch.float32 or not bias.is_contiguous():
             bias = bias.float().contiguous()
         bp = bias.data_ptr()
     if residual is not None:
         if residual.shape != y.shape or residual.dtype != dt or residual.device != dev:
             raise ValueError(f"w4_linear: residual must be {dt} of shape {tuple(y.shape)} on {dev}")
-        grads = grads or residual.requires_grad
         r2 = residual if len(shape) == 2 else residual.reshape(-1, dout)
         if dout > 1 and r2.stride(1) != 1:
             r2 = r2.contiguous()
         rp, rs = r2.data_ptr(), r2.stride(0)
-    if grads and torch.is_grad_enabled():
-        raise RuntimeError("w4_linear has no backward: call it under torch.no_grad()")
     if M == 0:
         return y
     xs = 0 if M == 1 else x2.stride(0)

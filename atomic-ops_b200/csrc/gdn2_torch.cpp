@@ -17,11 +17,12 @@
 
 namespace {
 
-// A plain tensor argument that needs no gradient, or null.
+// A plain tensor argument that needs no gradient of either mode, or null.
 const at::Tensor* plain(PyObject* o) {
   if (!THPVariable_CheckExact(o)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(o);
   if (!t.is_cuda() || t.layout() != at::kStrided || (t.requires_grad() && c10::GradMode::is_enabled())) return nullptr;
+  if (t._fw_grad(0).defined()) return nullptr;
   return &t;
 }
 bool on16(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }

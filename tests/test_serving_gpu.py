@@ -579,6 +579,29 @@ def test_beam_refusals():
         beam_select(x.requires_grad_(True), sc)
 
 
+# ---- gradients --------------------------------------------------------------------------------------
+def test_forward_mode_is_refused():
+    """A dual tensor's tangent would be lost: every operator refuses it, in each of its arguments."""
+    fw = torch.autograd.forward_ad
+    _, dev, h0 = _inputs(2, 1, 3, 1)
+    q, s, x, bias, res = (t.cuda() for t in _w4_inputs(2, 64, 16, 64, torch.float32, 5))
+    lg, sc, _ = (t.cuda() for t in _beam_inputs(2, 3, 20, torch.float32, 4))
+    fn, w, h0 = make_blr_recurrent(make_cfg(), SCALE), pack_w4(q, s, 64), h0.cuda()
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))
+        for i in range(6):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                fn(*dev[:i], dual(dev[i]), *dev[i + 1:], h0)
+        for bad in (lambda: fn(*dev, dual(h0)), lambda: w4_linear(dual(x), w), lambda: w4_linear(x, w, dual(bias)),
+                    lambda: w4_linear(x, w, residual=dual(res)), lambda: beam_select(dual(lg), sc),
+                    lambda: beam_select(lg, dual(sc))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                bad()
+            with pytest.raises(RuntimeError, match="forward-mode"), torch.no_grad():
+                bad()
+        fn(*dev, h0), w4_linear(x, w, bias, residual=res), beam_select(lg, sc)
+
+
 # ---- streams and graphs --------------------------------------------------------------------------
 def test_other_stream_and_graph_capture():
     """On a side stream, and captured into a CUDA graph and replayed on new values."""
