@@ -86,8 +86,8 @@ def make_blr_recurrent(cfg: BLRConfig, scale):
           h_index  (B) the row of h0 that each sequence starts from, negative for zeros: the rows
                    that beam_select returns read each beam's parent without a copy of the states
           lengths  (B) tokens of each sequence, 0..L; past them o is zero and the state stands still
-          h_out    (B, H, D, D) fp32 contiguous, written and returned as h; it may be h0 itself, or
-                   without h_index overlap nothing of it
+          h_out    (B, H, D, D) fp32 contiguous, written and returned as h (an in-place change to
+                   autograd); it may be h0 itself, or without h_index overlap nothing of it
         Returns o (B, H, L, D) fp32 (token-major in memory where q is) and h (B, H, D, D) fp32."""
         nonlocal fast, last
         if isinstance(q, torch.Tensor) and q.is_cuda:           # the common call; None: it needs more than that
@@ -119,13 +119,13 @@ def make_blr_recurrent(cfg: BLRConfig, scale):
             raise NotImplementedError(f"gdn2: head size {D}; the B200 kernels implement {_D}")
         if B == 0 or H == 0:
             raise ValueError(f"gdn2: empty batch or no heads: {tuple(shape)}")
-        pipeline._refuse_gradients("make_blr_recurrent", (*xs, h0))
+        pipeline._refuse_gradients("make_blr_recurrent", (*xs, h0, h_out))
         if not same or dt not in (torch.float32, torch.bfloat16):
             dt = torch.float32
             xs = tuple(t.to(dt) for t in xs)
         if L and not all([_rows_ok(t) for t in xs]):
             xs = tuple(t if _rows_ok(t) else t.clone(memory_format=torch.contiguous_format) for t in xs)
-        n_states = 0
+        n_states, given = 0, h_out is not None
         if h0 is not None:
             if h0.ndim != 4 or h0.shape[1:] != (H, D, D) or (h_index is None and h0.shape[0] != B) or not h0.shape[0]:
                 raise ValueError(f"h0 must have shape {(B if h_index is None else 'n', H, D, D)}")
@@ -180,6 +180,8 @@ def make_blr_recurrent(cfg: BLRConfig, scale):
                 _raw_stream(dev.index))
         if rc:
             _lib.check(rc, "gdn2_recurrent")
+        if given and not h_out.is_inference():                 # autograd may have saved it
+            torch.autograd.graph.increment_version(h_out)
         _check_flags(fl, "gdn2_recurrent")
         return o, h_out
 

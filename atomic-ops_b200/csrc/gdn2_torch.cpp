@@ -127,6 +127,7 @@ PyObject* recurrent(PyObject*, PyObject* const* a, Py_ssize_t n) {
       ws.defined() ? ws.data_ptr() : nullptr, static_cast<uint32_t*>(flags),
       c10::cuda::getCurrentCUDAStream(dev.index()).stream());
   if (s != GDN2_OK) Py_RETURN_NONE;
+  if (a[9] != Py_None && !h.is_inference()) h.unsafeGetTensorImpl()->bump_version();  // autograd may have saved it
   return pair(std::move(o), std::move(h));
   END_HANDLE_TH_ERRORS
 }

@@ -602,6 +602,28 @@ def test_forward_mode_is_refused():
         fn(*dev, h0), w4_linear(x, w, bias, residual=res), beam_select(lg, sc)
 
 
+def test_h_out_is_an_in_place_change():
+    """A tensor that autograd has saved and h_out overwrites makes its backward raise; one that needs a gradient
+    is refused."""
+    _, dev, h0 = _inputs(2, 1, 3, 1)
+    h0, fn = h0.cuda(), make_blr_recurrent(make_cfg(), SCALE)
+    for xs in (dev, [t.double() for t in dev], [t[:, :, :0] for t in dev]):
+        buf, p = torch.zeros_like(h0), torch.ones_like(h0).requires_grad_(True)
+        y = (p * buf).sum()
+        before = buf._version
+        fn(*xs, h0, h_out=buf)
+        assert buf._version > before
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+        with pytest.raises(RuntimeError, match="no backward"):
+            fn(*xs, h0, h_out=p)
+        with torch.no_grad():
+            fn(*xs, h0, h_out=p)
+        with torch.inference_mode():
+            fn(*xs, h0, h_out=torch.empty_like(h0))
+        assert fn(*xs, h0)[1]._version == 0
+
+
 # ---- streams and graphs --------------------------------------------------------------------------
 def test_other_stream_and_graph_capture():
     """On a side stream, and captured into a CUDA graph and replayed on new values."""
