@@ -117,7 +117,7 @@ __device__ __forceinline__ void load_quarter(const W4Params& p, const T* const x
     if constexpr (kPacked) {
 #pragma unroll
       for (int e = 0; e < kTerms; ++e) {
-        const uint4 v = __ldg(xp + (j * kTerms + e) * 32);
+        const uint4 v = xp[(j * kTerms + e) * 32];  // not __ldg: the grid before may still write it when this one starts
         f[j][e][0] = v.x; f[j][e][1] = v.y; f[j][e][2] = v.z; f[j][e][3] = v.w;
       }
     } else if constexpr (sizeof(T) == 2) {
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(kW4Warps * 32, kTwoCtas<kTerms, kMB> ? 2 : 1) 
     ssrc += (size_t)step * 16 * (kPer * 4);
   };
   if (nb < p.NB) fetch();
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the terms; nothing else of the stream is waited for less
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // for the terms; everything before them is done
   float sum[2][kMB][4];
 #pragma unroll
   for (int i = 0; i < 2; ++i)

@@ -421,6 +421,21 @@ def test_w4_rows_do_not_touch_one_another():
     assert not bool(torch.isfinite(y[2]).any()) and bool(torch.isnan(y[4]).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_w4_calls_one_after_the_other(dtype):
+    """Calls whose rows are laid out first, back to back in the same workspace: each sees its own x."""
+    q, s, x, _, _ = _w4_inputs(8, 1131, 300, 32, dtype, 9)
+    w, x = pack_w4(q.cuda(), s.cuda(), 32), x.cuda()
+    xs = [(x * f).contiguous() for f in (1.0, -2.0, 0.5, 4.0)]
+    want = []
+    for t in xs:
+        want.append(w4_linear(t, w))
+        torch.cuda.synchronize()
+    got = [w4_linear(xs[i % 4], w) for i in range(200)]
+    assert all(torch.equal(y, want[i % 4]) for i, y in enumerate(got))
+    _w4_check(want[0], *w4_ref(x.cpu(), q, s, 32), 1131, dtype)
+
+
 def test_w4_fp32_range():
     """Very large and very small fp32 values keep their 24 bits."""
     q, s, x, _, _ = _w4_inputs(4, 96, 40, 32, torch.float32, 4)
