@@ -20,14 +20,29 @@ _ACTS = {None: 0, "gelu": 1}
 
 
 class W4Weight:
-    """A packed 4-bit weight (layout: include/gdn2_b200.h, gdn2_w4_linear).  `packed` and `scales`
-    are its buffers, din x dout its size, `group` the rows per scale."""
+    """A packed 4-bit weight (layout: include/gdn2_b200.h, gdn2_w4_linear).  `packed` (int32) and
+    `scales` (bf16) are its buffers, din x dout its size, `group` the rows per scale.  Buffers that
+    do not have that size are refused, here and by w4_linear: the kernel trusts them."""
 
     __slots__ = ("packed", "scales", "din", "dout", "group", "device")
 
     def __init__(self, packed, scales, din, dout, group):
         self.packed, self.scales, self.din, self.dout, self.group = packed, scales, din, dout, group
+        self.check()
         self.device = packed.device
+
+    def check(self) -> None:
+        """Raises ValueError where the buffers are not those of a din x dout weight."""
+        if self.group not in GROUPS:
+            raise ValueError(f"group={self.group} must be one of {GROUPS}")
+        if self.din < 1 or self.dout < 1:
+            raise ValueError(f"a weight cannot be {self.din} x {self.dout}")
+        blocks = -(-self.dout // 32) * -(-self.din // 128)
+        for name, t, dtype, n in (("packed", self.packed, torch.int32, blocks * 512),
+                                  ("scales", self.scales, torch.bfloat16, blocks * 32 * (128 // self.group))):
+            if t.dtype != dtype or t.numel() != n or not t.is_contiguous() or t.device != self.packed.device:
+                raise ValueError(f"{name} of a {self.din} x {self.dout} weight must be {n} contiguous {dtype} on one "
+                                 f"device; got {tuple(t.shape)} {t.dtype} on {t.device}")
 
     def to(self, device):
         return W4Weight(self.packed.to(device), self.scales.to(device), self.din, self.dout, self.group)
@@ -123,8 +138,9 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, bias=None, *, act=None, residua
     din, dout = weight.din, weight.dout
     if not shape or shape[-1] != din:
         raise ValueError(f"w4_linear: x has shape {tuple(shape)}, the weight {din} rows")
-    if weight.device != dev:
-        raise ValueError(f"w4_linear: x is on {dev}, the weight on {weight.device}")
+    weight.check()
+    if weight.packed.device != dev:
+        raise ValueError(f"w4_linear: x is on {dev}, the weight on {weight.packed.device}")
     if act not in _ACTS:
         raise ValueError(f"w4_linear: act={act!r} is not None or 'gelu'")
     pipeline._refuse_gradients("w4_linear", (x, bias, residual))

@@ -145,6 +145,11 @@ PyObject* w4_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (PyErr_Occurred()) return nullptr;
   if ((type != at::kFloat && type != at::kBFloat16) || !current(dev) || w->device() != dev || sc->device() != dev)
     Py_RETURN_NONE;
+  if (din < 1 || dout < 1 || (group != 32 && group != 64 && group != 128)) Py_RETURN_NONE;
+  const int64_t blocks = (dout + 31) / 32 * ((din + 127) / 128);  // the kernel trusts the buffers' sizes
+  if (w->scalar_type() != at::kInt || w->numel() != blocks * 512 || !w->is_contiguous() ||
+      sc->scalar_type() != at::kBFloat16 || sc->numel() != blocks * 32 * (128 / group) || !sc->is_contiguous())
+    Py_RETURN_NONE;
   if (x->dim() != 2 || x->size(1) != din || x->size(0) < 1 || x->size(0) >= (1 << 30) || x->stride(1) != 1 || !on16(*x))
     Py_RETURN_NONE;
   gdn2_w4_desc d{};

@@ -491,6 +491,16 @@ def test_w4_refusals():
             bad()
 
 
+def test_w4_refuses_a_weight_of_another_size():
+    """A weight whose size was changed after it was packed: nothing is launched."""
+    q, s, x, _, _ = (t.cuda() for t in _w4_inputs(2, 128, 32, 64, torch.float32, 5))
+    for name, value in (("dout", 64), ("din", 256), ("group", 32), ("group", 0), ("scales", s[:1])):
+        w = pack_w4(q, s, 64)
+        setattr(w, name, value)
+        with pytest.raises(ValueError):
+            w4_linear(torch.zeros(2, w.din, device="cuda"), w)
+
+
 # ---- beam ----------------------------------------------------------------------------------------
 def _beam_inputs(B, K, V, dtype, seed, masked=0.0):
     """Inputs whose totals are apart (module docstring): the first seed from `seed` on that gives them."""

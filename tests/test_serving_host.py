@@ -64,6 +64,20 @@ def test_pack_refusals():
         quantize_w4(torch.zeros(4, 4), group=16)
 
 
+def test_weight_buffers_have_their_size():
+    """The kernel reads din x dout: buffers of another size, type or order are refused when they are put together."""
+    from atomic_gdn2 import W4Weight
+    w = pack_w4(torch.zeros(130, 40, dtype=torch.int8), torch.ones(3, 40, dtype=torch.bfloat16), 64)
+    assert torch.equal(W4Weight(w.packed, w.scales, 130, 40, 64).integers(), w.integers())
+    for packed, scales, din, dout, group in (
+            (w.packed[:1], w.scales, 130, 40, 64), (w.packed, w.scales[:, :1], 130, 40, 64), (w.packed, w.scales, 257, 40, 64),
+            (w.packed, w.scales, 130, 65, 64), (w.packed, w.scales, 130, 40, 32), (w.packed, w.scales, 130, 40, 48),
+            (w.packed.long(), w.scales, 130, 40, 64), (w.packed, w.scales.float(), 130, 40, 64), (w.packed, w.scales, 0, 40, 64),
+            (w.packed.transpose(0, 1), w.scales, 130, 40, 64)):
+        with pytest.raises(ValueError):
+            W4Weight(packed, scales, din, dout, group)
+
+
 def test_operators_have_no_cpu_path():
     x = [torch.zeros(1, 1, 1, 128)] * 6
     with pytest.raises(RuntimeError):
