@@ -2,8 +2,9 @@
 
 The library is written in-tree to ``atomic_gdn2/_lib/libgdn2_b200.so`` so that it
 travels with the source tree, the serving operators' binding to torch tensors
-(``csrc/gdn2_torch.cpp``, host code) to ``atomic_gdn2/_lib/gdn2_torch.so``.  Each ``csrc/*.cu`` is compiled to an object in
-parallel, then linked with ``-shared``.
+(``csrc/gdn2_torch.cpp``, host code) to ``atomic_gdn2/_lib/gdn2_torch-<torch>-<python>.so``: it fits
+the torch that it was built against and no other, so its name says which.  Each ``csrc/*.cu`` is
+compiled to an object in parallel, then linked with ``-shared``.
 """
 from __future__ import annotations
 
@@ -12,6 +13,7 @@ import os
 import pathlib
 import shutil
 import subprocess
+import sys
 
 PKG_DIR = pathlib.Path(__file__).resolve().parent
 ROOT = PKG_DIR.parent                      # atomic-ops_b200/
@@ -21,7 +23,6 @@ LIB_DIR = PKG_DIR / "_lib"
 LIB_NAME = "libgdn2_b200.so"
 LIB_PATH = LIB_DIR / LIB_NAME
 EXT_SRC = CSRC / "gdn2_torch.cpp"          # the serving operators' binding to torch tensors
-EXT_PATH = LIB_DIR / "gdn2_torch.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC",
@@ -35,14 +36,21 @@ def _nvcc() -> str:
     raise RuntimeError("nvcc not found: the GDN-2 B200 library cannot be built")
 
 
+def ext_path() -> pathlib.Path:
+    """The torch binding for the running torch and Python."""
+    import torch
+    return LIB_DIR / f"gdn2_torch-{torch.__version__}-cp{sys.version_info[0]}{sys.version_info[1]}.so"
+
+
 def sources() -> list[pathlib.Path]:
     return sorted(CSRC.glob("*.cu"))
 
 
 def _stale() -> bool:
-    if not LIB_PATH.exists() or not EXT_PATH.exists():
+    ext = ext_path()
+    if not LIB_PATH.exists() or not ext.exists():
         return True
-    t = min(LIB_PATH.stat().st_mtime, EXT_PATH.stat().st_mtime)
+    t = min(LIB_PATH.stat().st_mtime, ext.stat().st_mtime)
     deps = [EXT_SRC] + list(CSRC.glob("*.cu")) + list(CSRC.glob("*.cuh")) + list(INCLUDE.glob("*.h"))
     return any(p.stat().st_mtime > t for p in deps)
 
@@ -66,14 +74,15 @@ def _ext_object(obj_dir: pathlib.Path) -> pathlib.Path:
 def _link_ext(obj: pathlib.Path) -> None:
     import torch
     lib = pathlib.Path(torch.__file__).resolve().parent / "lib"
-    tmp = EXT_PATH.with_suffix(".so.tmp")
+    path = ext_path()
+    tmp = path.with_name(path.name + ".tmp")
     cmd = [shutil.which("g++") or "g++", "-shared", "-o", str(tmp), str(obj), f"-L{LIB_DIR}", f"-l:{LIB_NAME}",
            f"-L{lib}", "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10",
            "-Wl,-rpath,$ORIGIN"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
-    os.replace(tmp, EXT_PATH)
+    os.replace(tmp, path)
 
 
 def build_library(force: bool = False, verbose: bool = False) -> pathlib.Path:
@@ -111,5 +120,4 @@ def build_library(force: bool = False, verbose: bool = False) -> pathlib.Path:
 
 
 if __name__ == "__main__":
-    import sys
     print(build_library(force="--force" in sys.argv, verbose="-v" in sys.argv))

@@ -170,17 +170,23 @@ def load():
 
 def binding():
     """The serving operators' short way from torch tensors to the library (csrc/gdn2_torch.cpp), loaded
-    once; raises RuntimeError if it is missing."""
+    once; raises RuntimeError if there is none for the running torch."""
     global _ext
     if _ext is None:
         import importlib.util
+        from . import _build
         load()
-        path = _LIB_PATH.with_name("gdn2_torch.so")
+        path = _build.ext_path()
+        how = "build it with `python -c \"import __graft_entry__ as g; g.build()\"`"
         if not path.exists():
-            raise RuntimeError(f"{path} is missing: build it with `python -c \"import __graft_entry__ as g; g.build()\"`")
+            raise RuntimeError(f"{path} is missing: {how}")
         spec = importlib.util.spec_from_file_location("gdn2_torch", path)
-        _ext = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(_ext)
+        try:
+            ext = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(ext)
+        except ImportError as e:
+            raise RuntimeError(f"{path} does not load ({e}): {how}") from e
+        _ext = ext
     return _ext
 
 

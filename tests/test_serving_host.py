@@ -78,6 +78,27 @@ def test_weight_buffers_have_their_size():
             W4Weight(packed, scales, din, dout, group)
 
 
+def test_binding_is_the_running_torchs(monkeypatch):
+    """A binding built against another torch is neither taken for current nor loaded."""
+    from atomic_gdn2 import _build
+    assert _build.ext_path().exists() and hasattr(_lib.binding(), "recurrent")
+    monkeypatch.setattr(torch, "__version__", "9.9.9+other")
+    monkeypatch.setattr(_lib, "_ext", None)
+    assert _build._stale()
+    with pytest.raises(RuntimeError, match="build it with"):
+        _lib.binding()
+
+
+def test_binding_that_does_not_load(monkeypatch, tmp_path):
+    from atomic_gdn2 import _build
+    bad = tmp_path / "gdn2_torch.so"
+    bad.write_bytes(b"not a library")
+    monkeypatch.setattr(_build, "ext_path", lambda: bad)
+    monkeypatch.setattr(_lib, "_ext", None)
+    with pytest.raises(RuntimeError, match="does not load"):
+        _lib.binding()
+
+
 def test_operators_have_no_cpu_path():
     x = [torch.zeros(1, 1, 1, 128)] * 6
     with pytest.raises(RuntimeError):
