@@ -45,6 +45,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished=None, *, eo
     B, K, V = shape
     if K > MAX_BEAMS:
         raise NotImplementedError(f"beam_select: {K} beams; the B200 kernels implement up to {MAX_BEAMS}")
+    if B >= 1 << 31:
+        raise NotImplementedError(f"beam_select: {B} sequences")
     if scores.shape != (B, K) or scores.dtype != torch.float32 or scores.device != dev:
         raise ValueError(f"beam_select: scores must be float32 of shape {(B, K)} on {dev}")
     if eos is None:

@@ -146,6 +146,8 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, bias=None, *, act=None, residua
     pipeline._refuse_gradients("w4_linear", (x, bias, residual))
     x2 = x if len(shape) == 2 else x.reshape(-1, din)
     M = x2.shape[0]
+    if M >= 1 << 31:
+        raise NotImplementedError(f"w4_linear: {M} rows of x")
     if din > 1 and x2.stride(1) != 1 or x2.data_ptr() % 16:
         x2 = x2.clone(memory_format=torch.contiguous_format)
     y = torch.empty((*shape[:-1], dout), dtype=dt, device=dev)

@@ -820,7 +820,7 @@ gdn2_status check_rec(const gdn2_rec_desc* d) {
   if (!d || d->B <= 0 || d->H <= 0 || d->L < 0 || d->D <= 0) return GDN2_ERR_INVALID_ARGUMENT;
   if (d->in_dtype != GDN2_F32 && d->in_dtype != GDN2_BF16) return GDN2_ERR_INVALID_ARGUMENT;
   if (!(d->clip > 0.f) || (int64_t)d->B * d->H > (1 << 26)) return GDN2_ERR_INVALID_ARGUMENT;
-  return d->D == kD ? GDN2_OK : GDN2_ERR_UNSUPPORTED;
+  return d->D == kD && d->L <= (1 << 30) ? GDN2_OK : GDN2_ERR_UNSUPPORTED;
 }
 
 }  // namespace

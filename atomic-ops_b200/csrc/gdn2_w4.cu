@@ -380,7 +380,7 @@ gdn2_status check_w4(const gdn2_w4_desc* d) {
   if (d->act != GDN2_ACT_NONE && d->act != GDN2_ACT_GELU_TANH) return GDN2_ERR_INVALID_ARGUMENT;
   if (d->x_stride < 0 || d->y_stride < d->N || d->res_stride < 0) return GDN2_ERR_INVALID_ARGUMENT;
   if (d->group != 32 && d->group != 64 && d->group != 128) return GDN2_ERR_UNSUPPORTED;
-  if (d->M > 65535 * 32 || d->K > (1 << 30)) return GDN2_ERR_UNSUPPORTED;  // rows: the grid's limit
+  if (d->M > 65535 * 32 || d->K > (1 << 30) || d->N > (1 << 30)) return GDN2_ERR_UNSUPPORTED;  // rows: the grid's limit
   return GDN2_OK;
 }
 

@@ -221,7 +221,7 @@ gdn2_status gdn2_prologue_bwd(const float* y, int64_t B, int64_t L, int64_t H, i
  *   a = exp(min(g, 0)), d = w v - (b k)^T (diag(a) S), S <- diag(a) S + k d^T, o = scale q^T S;
  * o and the final states are sanitized at clip.  It equals gdn2_fwd with wy_eps = 0. */
 typedef struct gdn2_rec_desc {
-  int32_t B, H, L, D;     /* L >= 0, D == 128 */
+  int32_t B, H, L, D;     /* 0 <= L <= 2^30, D == 128 */
   int64_t stride[6][3];   /* element strides of q, k, v, w, b, g over B, H, L: multiples of 16 bytes,
                              those over L below 2^27 */
   int64_t o_stride[3];    /* element strides of o over B, H, L: multiples of 4 */
@@ -256,7 +256,7 @@ typedef enum gdn2_act { GDN2_ACT_NONE = 0, GDN2_ACT_GELU_TANH = 1 } gdn2_act;
 /* y = act(x W + bias) + residual for a 4-bit weight: W[k][n] = scale[k / group][n] * Q[k][n] with Q
  * in [-8, 7].  Made for few rows (M up to about 32 reads the weight once); any M works. */
 typedef struct gdn2_w4_desc {
-  int32_t M, K, N;
+  int32_t M, K, N;        /* M up to 32 * 65535, K and N up to 2^30 */
   int32_t group;          /* rows of W per scale: 32, 64 or 128 */
   int32_t dtype;          /* gdn2_dtype of x, residual and y */
   int32_t act;            /* gdn2_act */

@@ -501,6 +501,16 @@ def test_w4_refuses_a_weight_of_another_size():
             w4_linear(torch.zeros(2, w.din, device="cuda"), w)
 
 
+def test_row_counts_past_32_bits_are_refused():
+    """They would have been cut to their low 32 bits on the way to the kernels."""
+    q, s, x, _, _ = (t.cuda() for t in _w4_inputs(1, 64, 1, 64, torch.bfloat16, 5))
+    with pytest.raises(NotImplementedError):
+        w4_linear(x.expand(2 ** 32 + 1, 64), pack_w4(q, s, 64))
+    with pytest.raises(NotImplementedError):
+        beam_select(torch.zeros(1, 1, 8, device="cuda").expand(2 ** 32 + 1, 1, 8),
+                    torch.zeros(1, 1, device="cuda").expand(2 ** 32 + 1, 1))
+
+
 # ---- beam ----------------------------------------------------------------------------------------
 def _beam_inputs(B, K, V, dtype, seed, masked=0.0):
     """Inputs whose totals are apart (module docstring): the first seed from `seed` on that gives them."""

@@ -64,6 +64,17 @@ def test_pack_refusals():
         quantize_w4(torch.zeros(4, 4), group=16)
 
 
+def test_sizes_past_the_kernels_counters_are_refused():
+    """Sizes near 2^31, where tokens and columns would be counted past the type's end."""
+    lib, at, d = _lib.load(), 4096, _lib.RecDesc()
+    d.B, d.H, d.L, d.D, d.n_states, d.in_dtype, d.scale, d.clip = 1, 1, 2 ** 31 - 4, 128, 1, 0, 1.0, 1e4
+    assert lib.gdn2_recurrent(ctypes.addressof(d), *[at] * 6, 0, 0, 0, at, at, at, at, 0) == _lib.ERR_UNSUPPORTED
+    assert lib.gdn2_recurrent_workspace_bytes(ctypes.addressof(d)) == 0
+    d = _lib.W4Desc()
+    d.M, d.K, d.N, d.group, d.x_stride, d.y_stride = 1, 64, 2 ** 31 - 1, 64, 64, 2 ** 31
+    assert lib.gdn2_w4_linear(ctypes.addressof(d), at, at, at, 0, 0, at, 0, 0) == _lib.ERR_UNSUPPORTED
+
+
 def test_weight_buffers_have_their_size():
     """The kernel reads din x dout: buffers of another size, type or order are refused when they are put together."""
     from atomic_gdn2 import W4Weight
