@@ -67,8 +67,9 @@ class BeamDecoder:
 
     @torch.no_grad()
     def prefill(self, tokens: torch.Tensor, lengths=None):
-        """Prompts (B, L) padded on the right, `lengths` (B) tokens of each (1..L; None: all L).  Returns the
-        logits after each prompt's last token (B, vocab) and the layers' states."""
+        """Prompts (B, L) padded on the right with anything, `lengths` (B) tokens of each (1..L; None: all L).
+        Returns the logits after each prompt's last token (B, vocab) and the layers' states.  Tokens that no row
+        of the embedding belongs to are refused (nothing looks at them while a stream is being captured)."""
         if tokens.ndim != 2 or not tokens.numel():
             raise ValueError(f"prompts must be (B, L) and not empty; got shape {tuple(tokens.shape)}")
         B, L = tokens.shape
@@ -76,7 +77,14 @@ class BeamDecoder:
             lo, hi = torch.stack(torch.aminmax(lengths)).tolist()
             if lengths.shape != (B,) or lo < 1 or hi > L:
                 raise ValueError(f"lengths must be (B,) with values in 1..{L}")
+            past = torch.arange(L, device=tokens.device) >= lengths.to(tokens.device)[:, None]
+            tokens = tokens.masked_fill(past, 0)
             lengths = lengths.to(self.embed.device, torch.int32)
+        V = self.embed.shape[0]
+        if not torch.cuda.is_current_stream_capturing():
+            lo, hi = torch.stack(torch.aminmax(tokens)).tolist()
+            if lo < -V or hi >= V:
+                raise ValueError(f"prompts have tokens in {lo}..{hi}, the embedding {V} rows")
         x, states = self._layers(self.embed[tokens], None, lengths, None)
         last = x[:, -1] if lengths is None else x[torch.arange(B, device=x.device), lengths.long() - 1]
         return w4_linear(lnorm(last), *self.head), states
@@ -84,7 +92,8 @@ class BeamDecoder:
     @torch.no_grad()
     def step(self, tokens: torch.Tensor, states, rows=None):
         """One more token (N) for each of N sequences; sequence i goes on from row rows[i] of `states` (None:
-        row i).  Returns logits (N, vocab) and the new states."""
+        row i).  Returns logits (N, vocab) and the new states.  Tokens have to be of the vocabulary, as those of
+        beam_select are: nothing looks at them here."""
         x, states = self._layers(self.embed[tokens][:, None], states, None, rows)
         return w4_linear(lnorm(x[:, 0]), *self.head), states
 

@@ -123,6 +123,23 @@ def test_one_beam_goes_greedily():
     assert abs(float(scores[0, 0]) - float(total.max())) < 2 * TOL * max(1.0, abs(float(total.max())))
 
 
+def test_prompts_of_another_vocabulary_are_refused():
+    """On the host, before anything is gathered with them; what a prompt is padded with does not matter."""
+    dec = BeamDecoder(_model(1))
+    toks = torch.randint(0, V, (2, 4), generator=torch.Generator().manual_seed(3)).cuda()
+    lengths = torch.tensor([4, 2])
+    want = dec.prefill(toks, lengths)[0]
+    for bad in (V, -V - 1, 2 ** 31 - 1):
+        for t in (toks, toks.cpu(), toks.int()):
+            t = t.clone()
+            t[1, 2] = bad
+            assert torch.equal(dec.prefill(t, lengths)[0], want)
+            with pytest.raises(ValueError, match="embedding"):
+                dec.prefill(t)
+            with pytest.raises(ValueError, match="embedding"):
+                dec.search(t, torch.tensor([4, 3]))
+
+
 def test_decoder_keeps_its_own_weights():
     """Training the model further changes nothing of a decoder that was made before."""
     m = _model()
