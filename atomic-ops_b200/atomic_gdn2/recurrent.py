@@ -15,7 +15,8 @@ being captured (make a device's first call outside a capture: it sets that memor
 
 A value that is not finite counts from its token on: in q for that token's o, in v or w for its
 column, in k, b or g for the head.  What it reaches is what the recurrence makes of it, a NaN sanitized
-to 0 and an infinity to the bound; where there are several tokens such columns take about 0.6 us each.
+to 0 and an infinity to the bound.  Where there are several tokens, each of such a head takes about
+0.6 us.
 """
 from __future__ import annotations
 

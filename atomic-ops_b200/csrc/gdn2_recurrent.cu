@@ -195,8 +195,9 @@ __global__ void __launch_bounds__(kStepThreads) rec_step_kernel(RecParams p) {
 // either: the record holds B = X (bk e^G) and V = X (w v), and d = V - B S needs no substitution.
 //
 // The state's products run on the warp-level tensor instruction (m16n8k8, tf32) with each fp32
-// operand split in two (hi lo, each rounded to nearest: 22 bits) and three products; the lo lo
-// product would be below fp32's own rounding.  A warp holds the transposed state, 16 columns (d_v)
+// operand split in two (hi lo: 22 bits) and three products; the lo lo product is left out.  That is
+// 2^-21 of a product or less, four times fp32's own rounding: errors come out 15 to 20 % above those of a
+// plain fp32 form, whose sums they share.  A warp holds the transposed state, 16 columns (d_v)
 // x its share of d, in the accumulator layout; the same registers are the next product's first
 // operand, since the sum over d may run in any order.  On the CUDA cores the same work is bound by
 // the shared-memory traffic of the vectors (every lane needs its own copy), measured 2 to 6 times
@@ -795,10 +796,10 @@ cudaError_t launch(const RecParams& p, int BH, float* rec, cudaStream_t st) {
     return cudaGetLastError();
   }
   const int seg = seg_blocks(BH, p.L);
-  // Four warps on a head's 16 columns shorten a block's chain but repeat part of its work; measured
-  // per call (fp32, deep / wide): 6 heads x 4096 tokens 262 / 769 us, 48 x 1024 214 / 254, 96 x 777
-  // 327 / 344, 192 x 256 206 / 187, 384 x 192 330 / 285.  The deep form's 8 CTAs a head fill the GPU
-  // about six times over where the two meet.
+  // Four warps on a head's 16 columns shorten a block's chain but repeat part of its work; measured on
+  // the device (fp32, deep / wide): 6 heads x 4096 tokens 250 / 663 us, 48 x 1024 205 / 226, 96 x 777
+  // 308 / 314, 108 x 400 169 / 170, 120 x 400 192 / 177, 192 x 256 198 / 176, 384 x 192 310 / 264.  Where
+  // the two meet the deep form's 8 CTAs a head, two to an SM, take three turns.
   const bool deep = (long long)BH * 8 <= 6LL * kSmCount;
   for (int t0 = 0; t0 < p.L; t0 += seg * kTok) {
     const int nblk = min(seg, (p.L - t0 + kTok - 1) / kTok);

@@ -141,7 +141,8 @@ constexpr bool kTwoCtas = kMB == 1 || (kTerms == 1 && kMB == 2);
 // warps side by side (they share x through L1) and 8 / kMB that split the batches, and the CTAs of a
 // cluster split them further.  kPer: scales of a column per batch.
 //
-// Measured (bf16): 4 x 8192 x 8192 11.8 us (2.9 TB/s of weight), 16 x 8192 x 8192 16.1 us, 32 x 5000 x 12345
+// Bound, where there are many columns, by the waits for its loads (a batch ahead; it issues in half of the
+// cycles), then by the slots that widening takes.  Measured (bf16): 4 x 8192 x 8192 11.8 us (2.9 TB/s of weight), 16 x 8192 x 8192 16.1 us, 32 x 5000 x 12345
 // 35.4 us, 8 x 2048 x 512 3.7 us.  Widening takes 136 out of every value before the product: leaving it in and
 // taking 136 sum x out of the group's sum costs the bits of every x that is far below the group's largest,
 // and was no faster (12.2 us).
@@ -312,8 +313,8 @@ int row_blocks(int M) { return M <= 8 ? 1 : M <= 16 ? 2 : 4; }
 bool use_terms(const gdn2_w4_desc* d) {
   const int el = d->dtype == GDN2_BF16 ? 2 : 4;
   if (d->K % 8 || (d->x_stride * el) % 16) return true;
-  // Measured with and without: fp32 512 x 4608 4.0 / 2.7 us, 4096 x 4096 7.9 / 8.3, 8192 x 8192 19.3 / 24.2
-  // (1 row) and 47 / 79 (32 rows).
+  // Measured with and without: fp32 512 x 4608 3.8 / 2.5 us, 2048 x 2048 4.9 / 3.9, 4096 x 4096 7.3 / 7.7,
+  // 8192 x 8192 17.4 / 24.6 (1 row) and 48 / 78 (32 rows).
   return el == 4 && (long long)d->K * d->N >= (4 << 20);
 }
 
@@ -322,8 +323,8 @@ cudaError_t launch_one(const W4Params& p, cudaStream_t st) {
   const int blocks = ((p.N + 31) / 32 + kMB - 1) / kMB, rows = (p.M + 8 * kMB - 1) / (8 * kMB);
   // The rows of the weight are split over a cluster while the CTAs stay within one for each SM (two for
   // 9 to 16 bf16 rows, whose CTAs fit twice) and every warp has a batch: a CTA costs about 2 us besides
-  // its batches.  Measured with 1 / 2 / 8 CTAs: 16384 x 128, 4 rows 12.6 / 8.3 / 4.3 us; 8192 x 8192, 256
-  // CTAs, 12.5 / 15.4 us with 1 / 2.
+  // its batches.  Measured with 1 / 2 / 8 CTAs: 16384 x 128, 4 rows 11.4 / 7.8 / 4.2 us; 8192 x 8192, 256
+  // CTAs, 11.8 / 14.7 us with 1 / 2.
   const int most = kSmCount * (kTerms == 1 && kMB == 2 ? 2 : 1);
   int ks = 1;
   while (ks < 8 && blocks * rows * ks * 2 <= most && ks * (kW4Warps / kMB) < p.NB) ks *= 2;
