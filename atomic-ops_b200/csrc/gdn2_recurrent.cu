@@ -542,30 +542,42 @@ __device__ __forceinline__ void seq_update(float s[kJ][4], const SplitA& d, cons
 }
 __device__ __forceinline__ float4 lds4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 // The records' way into the ring: bulk copies that one thread issues, a barrier object per slot.  Waits
-// give up after the library's limit, tell the host and do not wait again.
+// give up after the library's limit, tell the host and do not wait again; the thread that issued the copies
+// issues no more then, and gives those on their way one more limit each before the CTA ends (drain).
+template <int kSlots>
 struct SeqRing {
   uint64_t* bars;
   uint32_t* flags;
-  bool gave_up = false;
-  __device__ void init(int slots) {  // one thread
-    for (int i = 0; i < slots; ++i) mbar_init(bars + i, 1);
+  int gave_up = -1;  // at the wait for this block
+  __device__ void init() {  // one thread
+    for (int i = 0; i < kSlots; ++i) mbar_init(bars + i, 1);
     fence_mbar_init();
   }
-  __device__ void fetch(int slot, float* dst, const float* from, int v_from, int v_floats) {  // one thread
+  __device__ void fetch(int blk, float* dst, const float* from, int v_from, int v_floats) {  // one thread
+    if (gave_up >= 0) return;
+    const int slot = blk % kSlots;
     mbar_arrive_expect_tx(bars + slot, (kRecV + v_floats) * 4);
     bulk_g2s(dst, from, kRecV * 4, bars + slot);
     bulk_g2s(dst + kRecV, from + kRecV + v_from, v_floats * 4, bars + slot);
   }
-  __device__ void wait(int slot, uint32_t parity) {
-    if (gave_up || mbar_try_wait(bars + slot, parity)) return;
+  __device__ bool landed(int blk) {
+    uint64_t* bar = bars + blk % kSlots;
+    const uint32_t parity = (blk / kSlots) & 1;
+    if (mbar_try_wait(bar, parity)) return true;
     const long long t0 = clock64();
-    while (!mbar_try_wait(bars + slot, parity)) {
-      if (clock64() - t0 > kWaitCycles) {
-        gave_up = true;
-        flags[2] = 1u;
-        return;
-      }
-    }
+    while (!mbar_try_wait(bar, parity))
+      if (clock64() - t0 > kWaitCycles) return false;
+    return true;
+  }
+  __device__ void wait(int blk) {
+    if (gave_up >= 0 || landed(blk)) return;
+    gave_up = blk;
+    flags[2] = 1u;
+  }
+  // The thread that fetches; `ahead`: blocks issued, from the one waited for on, at a wait.
+  __device__ void drain(int ahead, int blocks) {
+    if (gave_up < 0) return;
+    for (int blk = gave_up; blk < min(gave_up + ahead, blocks); ++blk) landed(blk);
   }
 };
 
@@ -587,18 +599,18 @@ __global__ void __launch_bounds__(kCT * 32, 3) rec_wide_kernel(const __grid_cons
   float s[16][4];
   seq_load<16>(s, state, r, mine);
   const float* src = rec + (size_t)blockIdx.x * nblk * kRecFloats;
-  SeqRing ring{bars, p.flags};
-  if (tid == 0) ring.init(kSlots);
+  SeqRing<kSlots> ring{bars, p.flags};
+  if (tid == 0) ring.init();
   __syncthreads();
   auto fetch = [&](int blk) {
     if (tid == 0 && blk < r.blocks)
-      ring.fetch(blk % kSlots, smem + (blk % kSlots) * kSlot, src + (size_t)blk * kRecFloats, blockIdx.y * kCT * 128, kCT * 128);
+      ring.fetch(blk, smem + (blk % kSlots) * kSlot, src + (size_t)blk * kRecFloats, blockIdx.y * kCT * 128, kCT * 128);
   };
 #pragma unroll
   for (int i = 0; i < kSlots - 1; ++i) fetch(i);
   float probe = 0.f;
   for (int blk = 0; blk < r.blocks; ++blk) {
-    ring.wait(blk % kSlots, (blk / kSlots) & 1);
+    ring.wait(blk);
     __syncthreads();          // every warp is done with block blk - 1
     fetch(blk + kSlots - 1);  // into that block's slot
     const float* slot = smem + (blk % kSlots) * kSlot;
@@ -625,6 +637,7 @@ __global__ void __launch_bounds__(kCT * 32, 3) rec_wide_kernel(const __grid_cons
     seq_out(p, r, blk, ct * 16 + g, o, d, slot + kRecP);
     seq_update<16>(s, d, slot, 0, lane);
   }
+  if (tid == 0) ring.drain(kSlots - 1, r.blocks);
   static_assert(kThreads == kLitThreads);
   if (!__syncthreads_or(probe != 0.f)) {
     seq_store<16>(s, p, mine, last);
@@ -657,18 +670,18 @@ __global__ void __launch_bounds__((kW + 2) * 32, 3) rec_deep_kernel(const __grid
   auto barrier = [] { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); };
   if (warp == kW) {  // copies
     const float* src = rec + (size_t)blockIdx.x * nblk * kRecFloats;
-    SeqRing ring{bars, p.flags};
+    SeqRing<kSlots> ring{bars, p.flags};
     if (lane == 0) {
-      ring.init(kSlots);
+      ring.init();
       bad = 0;
     }
     __syncwarp();
     auto fetch = [&](int blk) {
       if (lane == 0 && blk < r.blocks)
-        ring.fetch(blk % kSlots, smem + (blk % kSlots) * kSlot, src + (size_t)blk * kRecFloats, blockIdx.y * 128, 128);
+        ring.fetch(blk, smem + (blk % kSlots) * kSlot, src + (size_t)blk * kRecFloats, blockIdx.y * 128, 128);
     };
     auto landed = [&](int blk) {
-      if (blk < r.blocks) ring.wait(blk % kSlots, (blk / kSlots) & 1);
+      if (blk < r.blocks) ring.wait(blk);
     };
     for (int i = 0; i < kSlots - 2; ++i) fetch(i);
     landed(0);
@@ -678,6 +691,7 @@ __global__ void __launch_bounds__((kW + 2) * 32, 3) rec_deep_kernel(const __grid
       barrier();                // block blk + 1 is here, and every warp is done with block blk - 2
       fetch(blk + kSlots - 2);  // into that block's slot
     }
+    if (lane == 0) ring.drain(kSlots - 2, r.blocks);
     barrier();
     return;
   }
