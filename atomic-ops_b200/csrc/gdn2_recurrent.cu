@@ -432,8 +432,8 @@ __device__ __forceinline__ void seq_store(const float s[kJ][4], const RecParams&
       to[(j * 8 + (c & 1)) * kD + (c >> 1) * 8] = last ? sanitize(s[j][c], p.clip) : s[j][c];
 }
 // The launch's tokens by the definition, for 16 columns from `col` on (the CTA's column `mine`), by the CTA's first
-// four warps: a thread has 16 rows of a column.  The state has not been written back yet, and the records are done with: 19 KB
-// of their place are used.  Measured: 0.6 us a token (the latency of its loads and barriers).
+// four warps: a thread has 16 rows of a column.  The state has not been written back yet, and the records are done
+// with: 19 KB of their place are used.  Measured: 0.6 us a token (the latency of its loads and barriers).
 constexpr int kLitThreads = 128;
 template <class T>
 __device__ __noinline__ void seq_literal(const RecParams& p, const SeqSpan& r, const float* state, int tok0, int col,
@@ -442,10 +442,10 @@ __device__ __noinline__ void seq_literal(const RecParams& p, const SeqSpan& r, c
   float* mem = reinterpret_cast<float*>(smem4);
   const int tid = threadIdx.x, c = tid & 15, d0 = (tid >> 4) * 16, warp = tid >> 5, row = tid >> 4;
   const long long b = blockIdx.x / p.H, h = blockIdx.x % p.H;
-  float (*vec)[4][kD] = reinterpret_cast<float (*)[4][kD]>(mem);                                    // a, k, b k, q of a token
+  float (*vec)[4][kD] = reinterpret_cast<float (*)[4][kD]>(mem);  // a, k, b k, q of a token
   float (*wv)[16] = reinterpret_cast<float (*)[16]>(mem + kTok * 4 * kD);
-  float (*part)[4][16] = reinterpret_cast<float (*)[4][16]>(mem + kTok * (4 * kD + 16));            // by a token's parity
-  float (*outs)[4][16] = reinterpret_cast<float (*)[4][16]>(mem + kTok * (4 * kD + 16) + 2 * 64);   // by token
+  float (*part)[4][16] = reinterpret_cast<float (*)[4][16]>(mem + kTok * (4 * kD + 16));  // by a token's parity
+  float (*outs)[4][16] = part + 2;                                                        // by token
   auto barrier = [] { asm volatile("bar.sync 2, %0;" ::"n"(kLitThreads) : "memory"); };
   auto in = [&](const void* x, int i, int t, int d) {
     return ld1(static_cast<const T*>(x) + b * p.sb[i] + h * p.sh[i] + (tok0 + t) * p.sl[i] + d);
@@ -548,49 +548,53 @@ template <int kSlots>
 struct SeqRing {
   uint64_t* bars;
   uint32_t* flags;
-  int gave_up = -1;  // at the wait for this block
+  int* last;  // in shared memory: blocks that had been issued when the thread that issues them gave up
+  bool gave_up = false;
   __device__ void init() {  // one thread
     for (int i = 0; i < kSlots; ++i) mbar_init(bars + i, 1);
     fence_mbar_init();
   }
   __device__ void fetch(int blk, float* dst, const float* from, int v_from, int v_floats) {  // one thread
-    if (gave_up >= 0) return;
     const int slot = blk % kSlots;
     mbar_arrive_expect_tx(bars + slot, (kRecV + v_floats) * 4);
     bulk_g2s(dst, from, kRecV * 4, bars + slot);
     bulk_g2s(dst + kRecV, from + kRecV + v_from, v_floats * 4, bars + slot);
   }
-  __device__ bool landed(int blk) {
-    uint64_t* bar = bars + blk % kSlots;
-    const uint32_t parity = (blk / kSlots) & 1;
-    if (mbar_try_wait(bar, parity)) return true;
+  __device__ void wait(int slot, uint32_t parity, int issued) {  // `issued`: blocks by now, 0 by other threads
+    if (gave_up || mbar_try_wait(bars + slot, parity)) return;
     const long long t0 = clock64();
-    while (!mbar_try_wait(bar, parity))
-      if (clock64() - t0 > kWaitCycles) return false;
-    return true;
+    while (!mbar_try_wait(bars + slot, parity)) {
+      if (clock64() - t0 > kWaitCycles) {
+        gave_up = true;
+        flags[2] = 1u;
+        if (issued) *last = issued;
+        return;
+      }
+    }
   }
-  __device__ void wait(int blk) {
-    if (gave_up >= 0 || landed(blk)) return;
-    gave_up = blk;
-    flags[2] = 1u;
-  }
-  // The thread that fetches; `ahead`: blocks issued, from the one waited for on, at a wait.
-  __device__ void drain(int ahead, int blocks) {
-    if (gave_up < 0) return;
-    for (int blk = gave_up; blk < min(gave_up + ahead, blocks); ++blk) landed(blk);
+  __device__ void drain(int blocks) {  // the thread that fetches
+    if (!gave_up) return;
+    const int end = min(*last, blocks);
+    for (int blk = max(0, end - kSlots); blk < end; ++blk) {
+      const long long t0 = clock64();
+      while (!mbar_try_wait(bars + blk % kSlots, (blk / kSlots) & 1) && clock64() - t0 <= kWaitCycles) {
+      }
+    }
   }
 };
 
 // Many heads: a warp owns 16 columns and all of d, a CTA kCT such tiles.  Bound by the tensor pipe (144
 // products of 8 cycles a warp and block, half busy) and the splits' integer slots.  Measured: 384 heads x 80
-// tokens 71 us, 11 us of it the floor of its bytes.  The records arrive through a ring.  The bound of
+// tokens 72 us, 11 us of it the floor of its bytes.  The records arrive through a ring.  The bound of
 // three CTAs an SM gives a thread 168 registers; without it the compiler takes 128 and spills (75 us).
 template <int kCT>
 __global__ void __launch_bounds__(kCT * 32, 3) rec_wide_kernel(const __grid_constant__ RecParams p, const float* rec,
-                                                             const float* state, int tok0, int nblk, bool first, bool last) {
+                                                               const float* state, int tok0, int nblk, bool first,
+                                                               bool last) {
   constexpr int kThreads = kCT * 32, kSlots = 3, kSlot = kRecV + kCT * 128;
   extern __shared__ float4 smem4[];
   __shared__ uint64_t bars[kSlots];
+  __shared__ int issued;
   float* smem = reinterpret_cast<float*>(smem4);
   const int tid = threadIdx.x, lane = tid & 31, ct = tid >> 5, g = lane >> 2, t = lane & 3;
   const SeqSpan r = seq_span<kThreads, kCT * 16>(p, tok0, nblk, first);
@@ -599,18 +603,18 @@ __global__ void __launch_bounds__(kCT * 32, 3) rec_wide_kernel(const __grid_cons
   float s[16][4];
   seq_load<16>(s, state, r, mine);
   const float* src = rec + (size_t)blockIdx.x * nblk * kRecFloats;
-  SeqRing<kSlots> ring{bars, p.flags};
+  SeqRing<kSlots> ring{bars, p.flags, &issued};
   if (tid == 0) ring.init();
   __syncthreads();
   auto fetch = [&](int blk) {
-    if (tid == 0 && blk < r.blocks)
+    if (tid == 0 && blk < r.blocks && !ring.gave_up)
       ring.fetch(blk, smem + (blk % kSlots) * kSlot, src + (size_t)blk * kRecFloats, blockIdx.y * kCT * 128, kCT * 128);
   };
 #pragma unroll
   for (int i = 0; i < kSlots - 1; ++i) fetch(i);
   float probe = 0.f;
   for (int blk = 0; blk < r.blocks; ++blk) {
-    ring.wait(blk);
+    ring.wait(blk % kSlots, (blk / kSlots) & 1, tid == 0 ? blk + kSlots - 1 : 0);
     __syncthreads();          // every warp is done with block blk - 1
     fetch(blk + kSlots - 1);  // into that block's slot
     const float* slot = smem + (blk % kSlots) * kSlot;
@@ -637,7 +641,7 @@ __global__ void __launch_bounds__(kCT * 32, 3) rec_wide_kernel(const __grid_cons
     seq_out(p, r, blk, ct * 16 + g, o, d, slot + kRecP);
     seq_update<16>(s, d, slot, 0, lane);
   }
-  if (tid == 0) ring.drain(kSlots - 1, r.blocks);
+  if (tid == 0) ring.drain(r.blocks);
   static_assert(kThreads == kLitThreads);
   if (!__syncthreads_or(probe != 0.f)) {
     seq_store<16>(s, p, mine, last);
@@ -646,16 +650,18 @@ __global__ void __launch_bounds__(kCT * 32, 3) rec_wide_kernel(const __grid_cons
   }
 }
 
-// Few heads, where a block's chain of dependent steps is what counts (measured: 425 ns for 8 tokens, 6 heads
-// x 4096 tokens 218 us): kW warps share 16 columns and take 16 / kW tiles of d each; one more warp sees to the
+// Few heads, where a block's chain of dependent steps is what counts (measured: 422 ns for 8 tokens, 6 heads
+// x 4096 tokens 216 us): kW warps share 16 columns and take 16 / kW tiles of d each; one more warp sees to the
 // records and one finishes the outputs, a block behind.  Two CTAs fit on an SM by shared memory; the bound
-// of three is for registers (96 a thread; without it the compiler takes 80, and 265 us).  One barrier per block: before it the partial sums r of the block are written, after
-// it every warp adds them up.  What is double-buffered by the block's parity:
+// of three is for registers (96 a thread; without it the compiler takes 80, and 265 us).  One barrier per
+// block: before it the partial sums r of the block are written, after it every warp adds them up.  What is
+// double-buffered by the block's parity:
 //   rpart  written before barrier blk, read until barrier blk + 1
 //   opart, delta  written after barrier blk, read between barriers blk + 1 and blk + 2
 template <int kW>
-__global__ void __launch_bounds__((kW + 2) * 32, 3) rec_deep_kernel(const __grid_constant__ RecParams p, const float* rec,
-                                                                  const float* state, int tok0, int nblk, bool first, bool last) {
+__global__ void __launch_bounds__((kW + 2) * 32, 3) rec_deep_kernel(const __grid_constant__ RecParams p,
+                                                                    const float* rec, const float* state, int tok0,
+                                                                    int nblk, bool first, bool last) {
   constexpr int kThreads = (kW + 2) * 32, kJ = 16 / kW, kSlots = 6, kSlot = kRecV + 128;
   extern __shared__ float4 smem4[];
   float* smem = reinterpret_cast<float*>(smem4);
@@ -663,6 +669,7 @@ __global__ void __launch_bounds__((kW + 2) * 32, 3) rec_deep_kernel(const __grid
   float4* opart = rpart + 2 * kW * 32;         // [2][kW][32]
   float4* delta = opart + 2 * kW * 32;         // [2][32]
   __shared__ uint64_t bars[kSlots];
+  __shared__ int issued;
   __shared__ int bad;  // set before the last barrier, where a warp has met a value that is not finite
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const SeqSpan r = seq_span<kThreads, 16>(p, tok0, nblk, first);
@@ -670,18 +677,18 @@ __global__ void __launch_bounds__((kW + 2) * 32, 3) rec_deep_kernel(const __grid
   auto barrier = [] { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); };
   if (warp == kW) {  // copies
     const float* src = rec + (size_t)blockIdx.x * nblk * kRecFloats;
-    SeqRing<kSlots> ring{bars, p.flags};
+    SeqRing<kSlots> ring{bars, p.flags, &issued};
     if (lane == 0) {
       ring.init();
       bad = 0;
     }
     __syncwarp();
     auto fetch = [&](int blk) {
-      if (lane == 0 && blk < r.blocks)
+      if (lane == 0 && blk < r.blocks && !ring.gave_up)
         ring.fetch(blk, smem + (blk % kSlots) * kSlot, src + (size_t)blk * kRecFloats, blockIdx.y * 128, 128);
     };
     auto landed = [&](int blk) {
-      if (blk < r.blocks) ring.wait(blk);
+      if (blk < r.blocks) ring.wait(blk % kSlots, (blk / kSlots) & 1, lane ? 0 : blk ? blk + kSlots - 3 : kSlots - 2);
     };
     for (int i = 0; i < kSlots - 2; ++i) fetch(i);
     landed(0);
@@ -691,7 +698,7 @@ __global__ void __launch_bounds__((kW + 2) * 32, 3) rec_deep_kernel(const __grid
       barrier();                // block blk + 1 is here, and every warp is done with block blk - 2
       fetch(blk + kSlots - 2);  // into that block's slot
     }
-    if (lane == 0) ring.drain(kSlots - 2, r.blocks);
+    if (lane == 0) ring.drain(r.blocks);
     barrier();
     return;
   }
