@@ -128,8 +128,7 @@ def _refuse_gradients(what: str, tensors) -> None:
     tensors = [t for t in tensors if isinstance(t, torch.Tensor)]
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise RuntimeError(f"{what} has no backward: call it under torch.no_grad()")
-    forward = torch.autograd.forward_ad
-    if forward._current_level >= 0 and any(forward.unpack_dual(t).tangent is not None for t in tensors):
+    if any(torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise RuntimeError(f"{what} has no forward-mode derivative: its inputs must not be dual tensors")
 
 

@@ -7,11 +7,12 @@
 // beam offers itself alone: (eos, its score).
 //
 // The logits are read once (a few lanes' of them twice), and the waits for them bound the call where there are
-// many; the exponentials (a quarter of an SM's lanes a cycle) come next.  A warp takes 256 values at a time, eight to a lane, and a lane
-// keeps the running maximum and sum of its values' softmax.  With R = min(K, V) <= 32, R lanes' maxima
-// bound the R best values from below; only the few lanes whose maximum reaches the bound are looked
-// through again, value by value, into a sorted list over the warp's lanes.  Keys join the order-preserving bits of the logit with the inverted index,
-// so that no two are equal and the result does not depend on the order of insertion.
+// many; the exponentials (a quarter of an SM's lanes a cycle) come next.  A warp takes 256 values at a time,
+// eight to a lane, and a lane keeps the running maximum and sum of its values' softmax.  With R = min(K, V) <= 32,
+// R lanes' maxima bound the R best values from below; only the few lanes whose maximum reaches the bound are
+// looked through again, value by value, into a sorted list over the warp's lanes.  Keys join the order-preserving
+// bits of the logit with the inverted index, so that no two are equal and the result does not depend on the order
+// of insertion.
 //
 // Small vocabularies take one launch (a CTA per sequence); else a first launch reads the logits, a
 // long row's slices spread over CTAs, and a second one, started while the first still runs, joins them.

@@ -142,10 +142,10 @@ constexpr bool kTwoCtas = kMB == 1 || (kTerms == 1 && kMB == 2);
 // cluster split them further.  kPer: scales of a column per batch.
 //
 // Bound, where there are many columns, by the waits for its loads (a batch ahead; it issues in half of the
-// cycles), then by the slots that widening takes.  Measured (bf16): 4 x 8192 x 8192 11.8 us (2.9 TB/s of weight), 16 x 8192 x 8192 16.1 us, 32 x 5000 x 12345
-// 35.4 us, 8 x 2048 x 512 3.7 us.  Widening takes 136 out of every value before the product: leaving it in and
-// taking 136 sum x out of the group's sum costs the bits of every x that is far below the group's largest,
-// and was no faster (12.2 us).
+// cycles), then by the slots that widening takes.  Measured (bf16): 4 x 8192 x 8192 11.8 us (2.9 TB/s of
+// weight), 16 x 8192 x 8192 16.1 us, 32 x 5000 x 12345 35.4 us, 8 x 2048 x 512 3.7 us.  Widening takes 136 out
+// of every value before the product: leaving it in and taking 136 sum x out of the group's sum costs the bits
+// of every x that is far below the group's largest, and was no faster (12.2 us).
 template <class T, int kTerms, int kMB, int kPer, bool kPacked>
 __global__ void __launch_bounds__(kW4Warps * 32, kTwoCtas<kTerms, kMB> ? 2 : 1) w4_kernel(W4Params p) {
   constexpr int kWN = kMB, kWK = kW4Warps / kWN, kCols = kWN * 32, kRows = kMB * 8 + 1;
