@@ -65,13 +65,22 @@ class BeamDesc(ctypes.Structure):
     ]
 
 
+class GatedDesc(ctypes.Structure):
+    """struct gdn2_gated_desc."""
+    _fields_ = [
+        ("B", ctypes.c_int32), ("L", ctypes.c_int32), ("C", ctypes.c_int32), ("dtype", ctypes.c_int32),
+        ("n_states", ctypes.c_int32), ("reserved", ctypes.c_int32),
+        ("x_stride", ctypes.c_int64 * 2), ("g_stride", ctypes.c_int64 * 2),
+    ]
+
+
 EXPORTS = ("gdn2_residual_bytes", "gdn2_fwd_workspace_bytes", "gdn2_bwd_workspace_bytes", "gdn2_fwd", "gdn2_bwd",
            "gdn2_set_batch_groups", "gdn2_get_batch_groups",
            "gdn2_status_string", "gdn2_selftest_gemm", "gdn2_profile_enable", "gdn2_profile_collect",
            "gdn2_fwd_noalloc", "gdn2_prologue_fwd", "gdn2_prologue_bwd", "gdn2_selftest_engine",
            "gdn2_selftest_wait_timeout", "gdn2_recurrent", "gdn2_recurrent_workspace_bytes", "gdn2_w4_linear",
            "gdn2_w4_workspace_bytes", "gdn2_beam_select",
-           "gdn2_beam_workspace_bytes")
+           "gdn2_beam_workspace_bytes", "gdn2_gated_fwd", "gdn2_gated_bwd", "gdn2_gated_marks_bytes")
 # kernel ids of gdn2_profile_collect
 KERNELS = ("fwd_intra", "fwd_scan", "fwd_out", "bwd_pre", "bwd_scan", "bwd_intra")
 
@@ -123,6 +132,12 @@ def _declare(lib):
     lib.gdn2_beam_workspace_bytes.argtypes = [P]
     lib.gdn2_beam_select.restype = ctypes.c_int
     lib.gdn2_beam_select.argtypes = [P] * 10
+    lib.gdn2_gated_fwd.restype = ctypes.c_int
+    lib.gdn2_gated_fwd.argtypes = [P] * 12
+    lib.gdn2_gated_bwd.restype = ctypes.c_int
+    lib.gdn2_gated_bwd.argtypes = [P] * 12
+    lib.gdn2_gated_marks_bytes.restype = ctypes.c_size_t
+    lib.gdn2_gated_marks_bytes.argtypes = [P]
     return lib
 
 

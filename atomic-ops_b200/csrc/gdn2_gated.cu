@@ -1,0 +1,532 @@
+// The diagonal gated linear recurrence over (B, L, C), forward and backward (sm_100a).
+//   h_t = a_t h_{t-1} + x_t,  a_t = exp(min(g_t, 0));   a reset drops the state before its token: h_t = x_t
+//   backward, from the last token to the first:  d_t = dy_t + e_t,  e_{t-1} = a_t d_t (0 at a reset),
+//   dx_t = d_t,  dg_t = d_t a_t h_{t-1},  dh0 = e_{-1};  e_{L-1} is the final state's gradient.
+// Past a sequence's length the state stands still and outputs and gradients are zero.
+//
+// The bytes bound it: x and g are read and h is written once, backward x, g and dy are read and dx and dg
+// written once.  A thread walks S tokens of V channels in registers: once from zero, for what the segment
+// does to a state (h -> A h + q), and, when the state that enters is known, once more as the recurrence
+// itself, so that an output carries the rounding of its own steps and of the few joined segments before.
+// Segments are joined over a CTA's threads in shared memory and over the CTAs of a cluster, which take
+// neighbouring stretches of one sequence, in distributed shared memory: one launch, no waiting on memory
+// flags, no workspace, and the same order of additions every time.  A cluster walks its sequence in rounds.
+// The backward pass starts its segments from the states that the forward pass left at their borders (4 / S
+// bytes a value) and computes h again from x: reading the rounded h instead would cost as many bytes and,
+// for bf16, half a step of h in dg.
+#include <cooperative_groups.h>
+
+#include "gdn2_common.cuh"
+
+namespace gdn2 {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr float kReset = -1.f;        // a segment's factor when a reset is in it: what entered is dropped
+constexpr float kTiny = 1.17549435e-38f;
+constexpr int kMaxWarps = 8;
+
+struct GatedParams {
+  const void *x, *g, *dy;
+  long long xb, xl, gb, gl;           // element strides over B and L
+  const float* h0;                    // (n_states, C) or null
+  const int32_t* index;               // (B) or null
+  const int32_t* lengths;             // (B) or null
+  const uint8_t* reset;               // (B, L) or null
+  void* h;                            // (B, L, C)
+  float* last;                        // (B, C)
+  float* marks;                       // (B, ceil(L / S), C): the state before each segment, or null
+  const float* dlast;                 // (B, C) or null
+  void *dx, *dg;                      // (B, L, C)
+  float* dh0;                         // (B, C) or null
+  uint32_t* flags;
+  int B, L, C, n_states;
+  int cols, clusters, lanes_log2;     // column blocks, CTAs of a cluster, lanes along C
+};
+
+// ---- values of V neighbouring channels ----------------------------------------------------------
+template <class T, int V>
+struct Lane;
+template <>
+struct Lane<float, 1> {
+  using raw = float;
+  static __device__ __forceinline__ void get(raw r, float* v) { v[0] = r; }
+  static __device__ __forceinline__ raw put(const float* v) { return v[0]; }
+};
+template <>
+struct Lane<__nv_bfloat16, 1> {
+  using raw = __nv_bfloat16;
+  static __device__ __forceinline__ void get(raw r, float* v) { v[0] = __bfloat162float(r); }
+  static __device__ __forceinline__ raw put(const float* v) { return __float2bfloat16_rn(v[0]); }
+};
+template <>
+struct Lane<__nv_bfloat16, 2> {
+  using raw = __nv_bfloat162;
+  static __device__ __forceinline__ void get(raw r, float* v) {
+    const float2 f = __bfloat1622float2(r);
+    v[0] = f.x;
+    v[1] = f.y;
+  }
+  static __device__ __forceinline__ raw put(const float* v) { return __floats2bfloat162_rn(v[0], v[1]); }
+};
+
+// What a stretch of tokens does to the state that enters it: h -> A h + q, or q where A is kReset.  A is
+// held at the smallest normal number or above as long as no gate in the stretch is zero: an infinite state
+// stays infinite through any number of them, as it does token by token.
+struct Seg {
+  float A, q;
+};
+__device__ __forceinline__ float step(Seg s, float h) { return s.A < 0.f ? s.q : fmaf(s.A, h, s.q); }
+__device__ __forceinline__ Seg join(Seg a, Seg b) {  // a first
+  Seg r;
+  r.q = step(b, a.q);
+  r.A = (a.A < 0.f || b.A < 0.f) ? kReset : (a.A == 0.f || b.A == 0.f) ? 0.f : fmaxf(a.A * b.A, kTiny);
+  return r;
+}
+
+__device__ __forceinline__ int length_of(const GatedParams& p, int b) {
+  if (!p.lengths) return p.L;
+  int n = p.lengths[b];
+  if (n < 0 || n > p.L) {
+    if (p.flags) p.flags[1] = 1;
+    n = n < 0 ? 0 : p.L;
+  }
+  return n;
+}
+__device__ __forceinline__ long long state_row(const GatedParams& p, int b) {  // -1: zeros
+  if (!p.h0) return -1;
+  if (!p.index) return b;
+  const int i = p.index[b];
+  if (i >= p.n_states) {
+    if (p.flags) p.flags[1] = 1;
+    return -1;
+  }
+  return i < 0 ? -1 : i;
+}
+
+// Bit i: token t0 + i drops the state before it.
+template <int S>
+__device__ __forceinline__ uint32_t resets_of(const GatedParams& p, int b, long long t0, int live) {
+  if (!p.reset) return 0;
+  const uint8_t* r = p.reset + b * (long long)p.L + t0;
+  uint32_t bits = 0;
+#pragma unroll
+  for (int i = 0; i < S; ++i)
+    if (i < live && r[i]) bits |= 1u << i;
+  return bits;
+}
+
+struct Shared {  // [buffer][segment of the CTA][channel of a row of lanes]: at most 8 x 32 / lanes x lanes x V
+  Seg part[kMaxWarps * 32 * 2];
+  Seg whole[2][32 * 2];
+};
+
+// Joins the segments of all threads: `mine` of this thread's V channels comes at place `place` of `places`
+// in the CTA and the CTA at place `rank` of `n` in its cluster.  enter[] is the state that the cluster's
+// first segment enters with; on return `mine_in` is what this thread's enters with, and enter[] what the
+// next round's first one does.
+template <int V>
+__device__ __forceinline__ void exchange(Shared& sm, int buf, const Seg mine[V], int place, int places, int lane,
+                                         int lanes, int rank, int n, float enter[V], float mine_in[V]) {
+  const int w = lanes * V;
+#pragma unroll
+  for (int v = 0; v < V; ++v) sm.part[place * w + lane * V + v] = mine[v];
+  __syncthreads();
+  Seg before[V];  // of this CTA's segments before this thread's
+#pragma unroll
+  for (int v = 0; v < V; ++v) before[v] = {1.f, 0.f};
+  for (int i = 0; i < place; ++i)
+#pragma unroll
+    for (int v = 0; v < V; ++v) before[v] = join(before[v], sm.part[i * w + lane * V + v]);
+  if (place == places - 1) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) sm.whole[buf][lane * V + v] = join(before[v], mine[v]);
+  }
+  if (n > 1) {
+    cg::cluster_group cl = cg::this_cluster();
+    cl.sync();
+    for (int r = 0; r < n; ++r) {
+      const Seg* other = cl.map_shared_rank(&sm.whole[buf][0], r);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if (r == rank) mine_in[v] = step(before[v], enter[v]);
+        enter[v] = step(other[lane * V + v], enter[v]);
+      }
+    }
+  } else {
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      mine_in[v] = step(before[v], enter[v]);
+      enter[v] = step(sm.whole[buf][lane * V + v], enter[v]);
+    }
+  }
+}
+
+template <class T, int V>
+__global__ void __launch_bounds__(32 * kMaxWarps) gated_fwd_kernel(const __grid_constant__ GatedParams p) {
+  using L = Lane<T, V>;
+  using raw = typename L::raw;
+  constexpr int S = 32 / V;
+  __shared__ Shared sm;
+  const int lanes = 1 << p.lanes_log2, lane = threadIdx.x & (lanes - 1);
+  const int place = threadIdx.x >> p.lanes_log2, places = blockDim.x >> p.lanes_log2;
+  const int rank = blockIdx.x % p.clusters, block = blockIdx.x / p.clusters;
+  const int b = block / p.cols, c = ((block % p.cols) * lanes + lane) * V;
+  const bool on = c < p.C;
+  const int len = length_of(p, b);
+  const long long row = state_row(p, b);
+  float enter[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) enter[v] = on && row >= 0 ? p.h0[row * p.C + c + v] : 0.f;
+  const raw* x = reinterpret_cast<const raw*>(static_cast<const T*>(p.x) + b * p.xb + c);
+  const raw* g = reinterpret_cast<const raw*>(static_cast<const T*>(p.g) + b * p.gb + c);
+  raw* h = reinterpret_cast<raw*>(static_cast<T*>(p.h) + (long long)b * p.L * p.C + c);
+  const int segs = (p.L + S - 1) / S, per_round = places * p.clusters;
+  bool positive = false;
+  for (int round = 0, buf = 0; round * (long long)per_round < segs; ++round, buf ^= 1) {
+    const long long seg = (long long)round * per_round + rank * places + place;
+    const long long t0 = seg * S;
+    const int live = on ? (int)max(0ll, min((long long)S, len - t0)) : 0;
+    float a[S][V], q[S][V];
+    const uint32_t resets = resets_of<S>(p, b, t0, live);
+    {
+      raw rx[S], rg[S];
+      const raw* px = x + t0 * (p.xl / V);
+      const raw* pg = g + t0 * (p.gl / V);
+#pragma unroll
+      for (int i = 0; i < S; ++i)
+        if (i < live) {
+          rx[i] = px[i * (p.xl / V)];
+          rg[i] = pg[i * (p.gl / V)];
+        }
+#pragma unroll
+      for (int i = 0; i < S; ++i) {
+        L::get(rx[i], q[i]);
+        L::get(rg[i], a[i]);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          if (i < live) {
+            positive |= a[i][v] > 0.f;
+            a[i][v] = expf(a[i][v] > 0.f ? 0.f : a[i][v]);  // a NaN stays one
+          } else {
+            a[i][v] = 1.f;
+            q[i][v] = 0.f;
+          }
+        }
+      }
+    }
+    Seg mine[V];
+    float mine_in[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float A = 1.f, s = 0.f;
+      bool zero = false;
+#pragma unroll
+      for (int i = 0; i < S; ++i) {
+        const bool r = (resets >> i) & 1u;
+        s = r ? q[i][v] : fmaf(a[i][v], s, q[i][v]);
+        zero |= a[i][v] == 0.f;
+        A *= a[i][v];
+      }
+      mine[v] = {resets ? kReset : zero ? 0.f : fmaxf(A, kTiny), s};
+    }
+    exchange<V>(sm, buf, mine, place, places, lane, lanes, rank, p.clusters, enter, mine_in);
+    if (on && t0 < p.L) {
+      if (p.marks) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) p.marks[((long long)b * segs + seg) * p.C + c + v] = mine_in[v];
+      }
+      raw* ph = h + t0 * (p.C / V);
+#pragma unroll
+      for (int i = 0; i < S; ++i) {
+        float y[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          mine_in[v] = ((resets >> i) & 1u) ? q[i][v] : fmaf(a[i][v], mine_in[v], q[i][v]);
+          y[v] = i < live ? mine_in[v] : 0.f;
+        }
+        if (t0 + i < p.L) ph[i * (long long)(p.C / V)] = L::put(y);
+      }
+    }
+  }
+  if (on && rank == 0 && place == 0) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) p.last[(long long)b * p.C + c + v] = enter[v];
+  }
+  if (positive && p.flags) p.flags[0] = 1;
+  if (p.clusters > 1) cg::this_cluster().sync();  // a CTA's shared memory is read until here
+}
+
+template <class T, int V>
+__global__ void __launch_bounds__(32 * kMaxWarps) gated_bwd_kernel(const __grid_constant__ GatedParams p) {
+  using L = Lane<T, V>;
+  using raw = typename L::raw;
+  constexpr int S = 32 / V;
+  __shared__ Shared sm;
+  const int lanes = 1 << p.lanes_log2, lane = threadIdx.x & (lanes - 1);
+  const int place = threadIdx.x >> p.lanes_log2, places = blockDim.x >> p.lanes_log2;
+  const int rank = blockIdx.x % p.clusters, block = blockIdx.x / p.clusters;
+  const int b = block / p.cols, c = ((block % p.cols) * lanes + lane) * V;
+  const bool on = c < p.C;
+  const int len = length_of(p, b);
+  float enter[V];  // e after the last token of a round, the sequence's last round first
+#pragma unroll
+  for (int v = 0; v < V; ++v) enter[v] = on && p.dlast ? p.dlast[(long long)b * p.C + c + v] : 0.f;
+  const raw* x = reinterpret_cast<const raw*>(static_cast<const T*>(p.x) + b * p.xb + c);
+  const raw* g = reinterpret_cast<const raw*>(static_cast<const T*>(p.g) + b * p.gb + c);
+  const long long at = (long long)b * p.L * p.C + c, row = p.C / V;
+  const raw* dy = reinterpret_cast<const raw*>(static_cast<const T*>(p.dy) + at);
+  raw* dx = reinterpret_cast<raw*>(static_cast<T*>(p.dx) + at);
+  raw* dg = reinterpret_cast<raw*>(static_cast<T*>(p.dg) + at);
+  const int segs = (p.L + S - 1) / S, per_round = places * p.clusters;
+  for (int round = 0, buf = 0; round * (long long)per_round < segs; ++round, buf ^= 1) {
+    const long long seg = segs - 1 - ((long long)round * per_round + rank * places + place);  // below 0: none
+    const long long t0 = seg * S;
+    const int live = on && seg >= 0 ? (int)max(0ll, min((long long)S, len - t0)) : 0;
+    const uint32_t resets = resets_of<S>(p, b, t0, live);
+    float a[S][V], h[S][V], d[S][V];
+    uint32_t open[V] = {};  // bit i: the gate is not above zero
+    {
+      raw rx[S], rg[S], ry[S];
+      const raw* px = x + t0 * (p.xl / V);
+      const raw* pg = g + t0 * (p.gl / V);
+      const raw* py = dy + t0 * row;
+#pragma unroll
+      for (int i = 0; i < S; ++i)
+        if (i < live) {
+          rx[i] = px[i * (p.xl / V)];
+          rg[i] = pg[i * (p.gl / V)];
+          ry[i] = py[i * row];
+        }
+      float s[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) s[v] = live ? p.marks[((long long)b * segs + seg) * p.C + c + v] : 0.f;
+#pragma unroll
+      for (int i = 0; i < S; ++i) {
+        float q[V];
+        L::get(rx[i], q);
+        L::get(rg[i], a[i]);
+        L::get(ry[i], d[i]);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          h[i][v] = s[v];  // the state before the token
+          if (i < live) {
+            open[v] |= (a[i][v] > 0.f ? 0u : 1u) << i;
+            a[i][v] = expf(a[i][v] > 0.f ? 0.f : a[i][v]);
+            s[v] = ((resets >> i) & 1u) ? q[v] : fmaf(a[i][v], s[v], q[v]);
+          } else {
+            a[i][v] = 1.f;
+            d[i][v] = 0.f;
+          }
+        }
+      }
+    }
+    Seg mine[V];
+    float e[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float A = 1.f, s = 0.f;
+      bool zero = false;
+#pragma unroll
+      for (int i = S - 1; i >= 0; --i) {
+        s = ((resets >> i) & 1u) ? 0.f : a[i][v] * (d[i][v] + s);
+        zero |= a[i][v] == 0.f;
+        A *= a[i][v];
+      }
+      mine[v] = {resets ? kReset : zero ? 0.f : fmaxf(A, kTiny), s};
+    }
+    exchange<V>(sm, buf, mine, place, places, lane, lanes, rank, p.clusters, enter, e);
+    if (on && seg >= 0) {
+      raw* qx = dx + t0 * row;
+      raw* qg = dg + t0 * row;
+#pragma unroll
+      for (int i = S - 1; i >= 0; --i) {
+        float ox[V], og[V];
+        const bool r = (resets >> i) & 1u;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          ox[v] = og[v] = 0.f;
+          if (i < live) {
+            ox[v] = d[i][v] + e[v];
+            e[v] = r ? 0.f : a[i][v] * ox[v];
+            og[v] = r || !((open[v] >> i) & 1u) ? 0.f : e[v] * h[i][v];
+          }
+        }
+        if (t0 + i < p.L) {
+          qx[i * row] = L::put(ox);
+          qg[i * row] = L::put(og);
+        }
+      }
+    }
+  }
+  if (p.dh0 && on && rank == 0 && place == 0) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) p.dh0[(long long)b * p.C + c + v] = enter[v];
+  }
+  if (p.clusters > 1) cg::this_cluster().sync();  // a CTA's shared memory is read until here
+}
+
+// A few tokens while a model answers: a thread walks them for V channels of a sequence.
+template <class T, int V>
+__global__ void __launch_bounds__(128) gated_step_kernel(const __grid_constant__ GatedParams p) {
+  using L = Lane<T, V>;
+  using raw = typename L::raw;
+  const long long per = (p.C + V - 1) / V, i = blockIdx.x * 128ll + threadIdx.x;
+  if (i >= p.B * per) return;
+  const int b = (int)(i / per), c = (int)(i % per) * V;
+  const int len = length_of(p, b);
+  const long long row = state_row(p, b);
+  float s[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) s[v] = row >= 0 ? p.h0[row * p.C + c + v] : 0.f;
+  bool positive = false;
+  for (int t = 0; t < p.L; ++t) {
+    float a[V], q[V], y[V];
+    const bool live = t < len;
+    if (live) {
+      L::get(reinterpret_cast<const raw*>(static_cast<const T*>(p.x) + b * p.xb + t * p.xl + c)[0], q);
+      L::get(reinterpret_cast<const raw*>(static_cast<const T*>(p.g) + b * p.gb + t * p.gl + c)[0], a);
+      const bool r = p.reset && p.reset[b * (long long)p.L + t];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        positive |= a[v] > 0.f;
+        s[v] = r ? q[v] : fmaf(expf(a[v] > 0.f ? 0.f : a[v]), s[v], q[v]);
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) y[v] = live ? s[v] : 0.f;
+    reinterpret_cast<raw*>(static_cast<T*>(p.h) + ((long long)b * p.L + t) * p.C + c)[0] = L::put(y);
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) p.last[(long long)b * p.C + c + v] = s[v];
+  if (positive && p.flags) p.flags[0] = 1;
+}
+
+// ---- host ---------------------------------------------------------------------------------------
+constexpr int kStepTokens = 4;
+
+// Two channels to a lane where bf16 rows allow 4-byte accesses.
+bool pairs(const gdn2_gated_desc* d) {
+  return d->dtype == GDN2_BF16 && d->C % 2 == 0 && d->x_stride[0] % 2 == 0 && d->x_stride[1] % 2 == 0 &&
+         d->g_stride[0] % 2 == 0 && d->g_stride[1] % 2 == 0;
+}
+
+gdn2_status check_gated(const gdn2_gated_desc* d) {
+  if (!d || d->B < 1 || d->L < 0 || d->C < 1 || d->n_states < 0) return GDN2_ERR_INVALID_ARGUMENT;
+  if (d->dtype != GDN2_F32 && d->dtype != GDN2_BF16) return GDN2_ERR_INVALID_ARGUMENT;
+  for (int i = 0; i < 2; ++i)
+    if (d->x_stride[i] < 0 || d->g_stride[i] < 0) return GDN2_ERR_INVALID_ARGUMENT;
+  if (d->L > 1 << 30 || d->C > 1 << 30) return GDN2_ERR_UNSUPPORTED;
+  if ((long long)d->B * ((d->C + 7) / 8) > (1ll << 27)) return GDN2_ERR_UNSUPPORTED;  // CTAs of a grid
+  return GDN2_OK;
+}
+
+struct GatedPlan {
+  int warps, lanes_log2, clusters, cols;
+};
+
+template <class K>
+cudaError_t launch_gated(K kernel, GatedParams& p, int V, cudaStream_t st) {
+  const int S = 32 / V, segs = (p.L + S - 1) / S;
+  const GatedPlan pl = [&] {
+    GatedPlan r{};
+    r.lanes_log2 = 5;
+    auto cols = [&] { return (p.C + (V << r.lanes_log2) - 1) / (V << r.lanes_log2); };
+    r.warps = segs < kMaxWarps ? (segs < 1 ? 1 : segs) : kMaxWarps;
+    r.clusters = 1;
+    while (r.clusters < 8 && (long long)p.B * cols() * r.clusters < 296 && r.clusters * r.warps < segs) r.clusters *= 2;
+    r.cols = cols();
+    return r;
+  }();
+  p.cols = pl.cols;
+  p.clusters = pl.clusters;
+  p.lanes_log2 = pl.lanes_log2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.B * pl.cols * pl.clusters));
+  cfg.blockDim = dim3(32u * pl.warps);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)pl.clusters;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+GatedParams params_of(const gdn2_gated_desc* d) {
+  GatedParams p{};
+  p.B = d->B; p.L = d->L; p.C = d->C; p.n_states = d->n_states;
+  p.xb = d->x_stride[0]; p.xl = d->x_stride[1];
+  p.gb = d->g_stride[0]; p.gl = d->g_stride[1];
+  return p;
+}
+bool off(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n != 0; }
+size_t access(const gdn2_gated_desc* d) { return d->dtype == GDN2_F32 || pairs(d) ? 4 : 2; }
+
+}  // namespace
+}  // namespace gdn2
+
+extern "C" size_t gdn2_gated_marks_bytes(const gdn2_gated_desc* d) {
+  using namespace gdn2;
+  if (check_gated(d) != GDN2_OK) return 0;
+  const long long S = pairs(d) ? 16 : 32;
+  return (size_t)d->B * (size_t)((d->L + S - 1) / S) * (size_t)d->C * sizeof(float);
+}
+
+extern "C" gdn2_status gdn2_gated_fwd(const gdn2_gated_desc* d, const void* x, const void* g, const float* h0,
+                                      const int32_t* h_index, const int32_t* lengths, const uint8_t* reset, void* h,
+                                      float* last, float* marks, uint32_t* flags, void* stream) {
+  using namespace gdn2;
+  const gdn2_status s = check_gated(d);
+  if (s != GDN2_OK) return s;
+  if (!last || !flags || (d->L && (!x || !g || !h))) return GDN2_ERR_INVALID_ARGUMENT;
+  if (h_index ? !h0 || d->n_states < 1 : h0 && d->n_states != d->B) return GDN2_ERR_INVALID_ARGUMENT;
+  const size_t n = access(d);
+  if (off(x, n) || off(g, n) || off(h, n) || off(h0, 4) || off(last, 4) || off(marks, 4) || off(flags, 4) ||
+      off(lengths, 4) || off(h_index, 4))
+    return GDN2_ERR_INVALID_ARGUMENT;
+  GatedParams p = params_of(d);
+  p.x = x; p.g = g; p.h0 = h0; p.index = h_index; p.lengths = lengths; p.reset = reset;
+  p.h = h; p.last = last; p.marks = marks; p.flags = flags;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (d->L <= kStepTokens && !marks) {
+    const int V = pairs(d) ? 2 : 1;
+    const unsigned grid = (unsigned)(((long long)d->B * ((d->C + V - 1) / V) + 127) / 128);
+    if (d->dtype == GDN2_F32) gated_step_kernel<float, 1><<<grid, 128, 0, st>>>(p);
+    else if (V == 2) gated_step_kernel<__nv_bfloat16, 2><<<grid, 128, 0, st>>>(p);
+    else gated_step_kernel<__nv_bfloat16, 1><<<grid, 128, 0, st>>>(p);
+    e = cudaGetLastError();
+  } else if (d->dtype == GDN2_F32) {
+    e = launch_gated(gated_fwd_kernel<float, 1>, p, 1, st);
+  } else if (pairs(d)) {
+    e = launch_gated(gated_fwd_kernel<__nv_bfloat16, 2>, p, 2, st);
+  } else {
+    e = launch_gated(gated_fwd_kernel<__nv_bfloat16, 1>, p, 1, st);
+  }
+  return e == cudaSuccess ? GDN2_OK : GDN2_ERR_CUDA;
+}
+
+extern "C" gdn2_status gdn2_gated_bwd(const gdn2_gated_desc* d, const void* x, const void* g, const int32_t* lengths,
+                                      const uint8_t* reset, const float* marks, const void* dh, const float* dlast,
+                                      void* dx, void* dg, float* dh0, void* stream) {
+  using namespace gdn2;
+  const gdn2_status s = check_gated(d);
+  if (s != GDN2_OK) return s;
+  if (d->L < 1 || !x || !g || !marks || !dh || !dx || !dg) return GDN2_ERR_INVALID_ARGUMENT;
+  const size_t n = access(d);
+  if (off(x, n) || off(g, n) || off(dh, n) || off(dx, n) || off(dg, n) || off(marks, 4) || off(dlast, 4) ||
+      off(dh0, 4) || off(lengths, 4))
+    return GDN2_ERR_INVALID_ARGUMENT;
+  GatedParams p = params_of(d);
+  p.x = x; p.g = g; p.lengths = lengths; p.reset = reset; p.marks = const_cast<float*>(marks);
+  p.dy = dh; p.dlast = dlast; p.dx = dx; p.dg = dg; p.dh0 = dh0;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = d->dtype == GDN2_F32 ? launch_gated(gated_bwd_kernel<float, 1>, p, 1, st)
+                        : pairs(d)           ? launch_gated(gated_bwd_kernel<__nv_bfloat16, 2>, p, 2, st)
+                                             : launch_gated(gated_bwd_kernel<__nv_bfloat16, 1>, p, 1, st);
+  return e == cudaSuccess ? GDN2_OK : GDN2_ERR_CUDA;
+}

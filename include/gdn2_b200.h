@@ -304,6 +304,42 @@ gdn2_status gdn2_beam_select(const gdn2_beam_desc* desc, const void* logits, con
                              const uint8_t* finished, float* out_scores, int32_t* out_row, int32_t* out_token,
                              uint8_t* out_finished, void* workspace, void* stream);
 
+/*
+ * Training operators beside the chunked one (no counterpart in the reference, whose layers and optimizer are XLA's).
+ */
+
+/* The diagonal gated linear recurrence over (B, L, C) and its backward:
+ *   h_t = exp(min(g_t, 0)) h_{t-1} + x_t,  and h_t = x_t at a token whose reset byte is not zero. */
+typedef struct gdn2_gated_desc {
+  int32_t B, L, C;        /* 0 <= L <= 2^30, 1 <= C <= 2^30 */
+  int32_t dtype;          /* gdn2_dtype of x, g, h and of their gradients */
+  int32_t n_states;       /* rows of h0 */
+  int32_t reserved;
+  int64_t x_stride[2], g_stride[2];  /* element strides over B and L, >= 0; unit along C */
+} gdn2_gated_desc;
+
+/*   x, g      aligned to their type; bf16 whose C and strides are even: to 4 bytes (so h, dh, dx and dg)
+ *   h0        (n_states, C) fp32 or NULL for zeros;  h_index (B) its row for each sequence (negative: zeros)
+ *             or NULL for row b (n_states == B)
+ *   lengths   (B) tokens of each sequence, 0..L, or NULL for L: past them the state stands still and h is zero
+ *   reset     (B, L) bytes or NULL
+ *   h         (B, L, C) contiguous;  last (B, C) fp32, which may be h0 itself when h_index is NULL and overlaps
+ *             no input otherwise
+ *   marks     gdn2_gated_marks_bytes(desc) bytes for the backward (states inside the sequences), or NULL
+ *   flags     two uint32 words in device or mapped host memory: [0] becomes 1 when g > 0 is seen, [1] when an
+ *             index >= n_states (zeros are taken) or a length outside 0..L (the nearer bound is taken) is */
+gdn2_status gdn2_gated_fwd(const gdn2_gated_desc* desc, const void* x, const void* g, const float* h0,
+                           const int32_t* h_index, const int32_t* lengths, const uint8_t* reset, void* h,
+                           float* last, float* marks, uint32_t* flags, void* stream);
+
+size_t gdn2_gated_marks_bytes(const gdn2_gated_desc* desc);
+
+/* Gradients from dh (B, L, C) contiguous and dlast (B, C) fp32 or NULL for zeros: dx, dg (B, L, C) contiguous, dh0
+ * (B, C) fp32 or NULL.  dg is zero where g > 0.  desc, x, g, lengths, reset and marks are the forward's; L >= 1. */
+gdn2_status gdn2_gated_bwd(const gdn2_gated_desc* desc, const void* x, const void* g, const int32_t* lengths,
+                           const uint8_t* reset, const float* marks, const void* dh, const float* dlast, void* dx,
+                           void* dg, float* dh0, void* stream);
+
 /* Profiling hook (no counterpart in the reference).  While enabled, every kernel launch of
  * gdn2_fwd / gdn2_bwd is bracketed by CUDA events recorded on the caller's stream.
  * gdn2_profile_collect synchronises on those events, writes per-kernel summed milliseconds and
