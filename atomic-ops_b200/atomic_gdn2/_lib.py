@@ -74,13 +74,33 @@ class GatedDesc(ctypes.Structure):
     ]
 
 
+class AdamwDesc(ctypes.Structure):
+    """struct gdn2_adamw_desc."""
+    _fields_ = [
+        ("state_bits", ctypes.c_int32), ("reserved", ctypes.c_int32),
+        ("beta1", ctypes.c_double), ("beta2", ctypes.c_double), ("eps", ctypes.c_double),
+        ("clip", ctypes.c_double), ("spike", ctypes.c_double),
+    ]
+
+
+class AdamwTensor(ctypes.Structure):
+    """struct gdn2_adamw_tensor."""
+    _fields_ = [
+        ("p", ctypes.c_void_p), ("m", ctypes.c_void_p), ("v", ctypes.c_void_p), ("g", ctypes.c_void_p),
+        ("m_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p), ("step", ctypes.c_void_p), ("lr_at", ctypes.c_void_p),
+        ("lr", ctypes.c_double), ("weight_decay", ctypes.c_double), ("n", ctypes.c_int64),
+        ("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32),
+    ]
+
+
 EXPORTS = ("gdn2_residual_bytes", "gdn2_fwd_workspace_bytes", "gdn2_bwd_workspace_bytes", "gdn2_fwd", "gdn2_bwd",
            "gdn2_set_batch_groups", "gdn2_get_batch_groups",
            "gdn2_status_string", "gdn2_selftest_gemm", "gdn2_profile_enable", "gdn2_profile_collect",
            "gdn2_fwd_noalloc", "gdn2_prologue_fwd", "gdn2_prologue_bwd", "gdn2_selftest_engine",
            "gdn2_selftest_wait_timeout", "gdn2_recurrent", "gdn2_recurrent_workspace_bytes", "gdn2_w4_linear",
            "gdn2_w4_workspace_bytes", "gdn2_beam_select",
-           "gdn2_beam_workspace_bytes", "gdn2_gated_fwd", "gdn2_gated_bwd", "gdn2_gated_marks_bytes")
+           "gdn2_beam_workspace_bytes", "gdn2_gated_fwd", "gdn2_gated_bwd", "gdn2_gated_marks_bytes",
+           "gdn2_adamw_step", "gdn2_adamw_workspace_bytes", "gdn2_adamw_moments")
 # kernel ids of gdn2_profile_collect
 KERNELS = ("fwd_intra", "fwd_scan", "fwd_out", "bwd_pre", "bwd_scan", "bwd_intra")
 
@@ -138,6 +158,12 @@ def _declare(lib):
     lib.gdn2_gated_bwd.argtypes = [P] * 12
     lib.gdn2_gated_marks_bytes.restype = ctypes.c_size_t
     lib.gdn2_gated_marks_bytes.argtypes = [P]
+    lib.gdn2_adamw_step.restype = ctypes.c_int
+    lib.gdn2_adamw_step.argtypes = [P, P, ctypes.c_int32, P, P, P, P]
+    lib.gdn2_adamw_workspace_bytes.restype = ctypes.c_size_t
+    lib.gdn2_adamw_workspace_bytes.argtypes = [P, P, ctypes.c_int32]
+    lib.gdn2_adamw_moments.restype = ctypes.c_int
+    lib.gdn2_adamw_moments.argtypes = [P, ctypes.c_int32, P]
     return lib
 
 

@@ -1,0 +1,197 @@
+"""AdamW over all of a model's tensors at once, on hand-written kernels.
+
+    opt = AdamW(model.parameters(), lr=3e-4, clip=1.0, state_bits=8)
+    loss.backward(); opt.step(loss=loss); opt.zero_grad()
+
+One step is two launches, whatever the number of tensors: the gradients' global norm, then the update.
+
+    n = |g|,  g' = g clip / max(n, clip)
+    m = b1 m + (1 - b1) g',   v = b2 v + (1 - b2) g'^2
+    p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+
+`clip` bounds the gradients' global norm (as optax.clip_by_global_norm), `spike_factor` skips steps whose norm is
+not below that many times the running mean of the norms of the steps that were made (0.98 / 0.02; as the
+reference's training step, training/train.py:47-53).  With either of them a step whose norm, or whose `loss` where
+it is given, is not finite is skipped as well: weights, moments and step counts stay as they are.  Nothing of
+that comes to the host: grad_norm and step_made are device values.
+
+Moments take 8 bytes a parameter, or 2 with state_bits=8: 256 values that follow one another in memory share a
+scale; the first moment is e4m3, the second is held as its root with four bits of exponent and four of mantissa
+(half a step is 1/32 of it), and a root above zero never becomes zero.  The update itself uses the moments before
+they are rounded.  Arithmetic is fp32, the norm's squares are summed in fp64 in a fixed order: the same inputs
+give the same bits.  bf16 parameters are rounded to nearest; there is no fp32 copy of them.
+
+state_dict() has torch.optim.AdamW's keys (and the scales); with state_bits=32 either loads the other's.
+A step may be captured into a CUDA graph after one that was not (the first one makes the moments); give lr as a
+tensor of one fp32 value on the device where it changes between replays.
+"""
+from __future__ import annotations
+
+import torch
+
+from .. import _lib
+
+BLOCK = 256
+
+
+class AdamW(torch.optim.Optimizer):
+    """`params`: as for torch.optim.AdamW, fp32 or bf16 tensors on one CUDA device.  Groups may differ in lr and
+    weight_decay.  clip and spike_factor: None for none.  state_bits: 32 or 8."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.95), eps=1e-8, weight_decay=0.1, *, clip=None, spike_factor=None,
+                 state_bits: int = 32):
+        if state_bits not in (32, 8):
+            raise ValueError(f"AdamW: state_bits={state_bits} must be 32 or 8")
+        self.clip, self.spike_factor, self.state_bits = clip, spike_factor, state_bits
+        self._control = None
+        self._check_guard()
+        defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay)
+        self._check_group(defaults)
+        super().__init__(params, defaults)
+        for group in self.param_groups:
+            self._check_group(group)
+
+    @staticmethod
+    def _check_group(g):
+        if not all(0.0 <= b < 1.0 for b in g["betas"]) or len(g["betas"]) != 2:
+            raise ValueError(f"AdamW: betas={g['betas']} must be two values in [0, 1)")
+        if not g["eps"] >= 0.0:
+            raise ValueError(f"AdamW: eps={g['eps']} must not be negative")
+        if not isinstance(g["lr"], torch.Tensor) and not g["lr"] >= 0.0:
+            raise ValueError(f"AdamW: lr={g['lr']} must not be negative")
+        if not g["weight_decay"] >= 0.0:
+            raise ValueError(f"AdamW: weight_decay={g['weight_decay']} must not be negative")
+
+    def _check_guard(self):
+        for name in ("clip", "spike_factor"):
+            x = getattr(self, name)
+            if x is not None and not x > 0.0:
+                raise ValueError(f"AdamW: {name}={x} must be above zero, or None for none")
+
+    def _ready(self, p):
+        """The parameter's state, made at its first step."""
+        st = self.state[p]
+        if not st or self._control is None:
+            if p.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW: make a first step outside the capture: it makes the moments")
+            if not p.is_cuda:
+                raise RuntimeError("AdamW: the parameters must be on a CUDA device (the step runs only on the B200 kernels)")
+            if self._control is None:
+                self._control = torch.zeros(5, device=p.device)
+        if not st:
+            eight = self.state_bits == 8
+            st["step"] = torch.zeros((), device=p.device)
+            for name in ("exp_avg", "exp_avg_sq"):
+                st[name] = torch.zeros_like(p, dtype=torch.uint8 if eight else torch.float32, requires_grad=False)
+                if eight:
+                    st[name + "_scale"] = torch.zeros(-(-p.numel() // BLOCK), device=p.device)
+        return st
+
+    @torch.no_grad()
+    def step(self, closure=None, *, loss=None):
+        """One step; returns closure's loss, or None.  Parameters without a gradient are passed over."""
+        result = None
+        if closure is not None:
+            with torch.enable_grad():
+                result = closure()
+            if loss is None and isinstance(result, torch.Tensor):
+                loss = result
+        self._check_guard()
+        first = self.param_groups[0]
+        lists = [[] for _ in range(9)]
+        for group in self.param_groups:
+            if group["betas"] != first["betas"] or group["eps"] != first["eps"]:
+                raise ValueError("AdamW: betas and eps must be the same in all groups")
+            lr, wd = group["lr"], float(group["weight_decay"])
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise RuntimeError("AdamW: sparse gradients are not supported")
+                st = self._ready(p)
+                row = (p, p.grad, st["exp_avg"], st["exp_avg_sq"], st.get("exp_avg_scale"), st.get("exp_avg_sq_scale"),
+                       st["step"], lr, wd)
+                for to, x in zip(lists, row):
+                    to.append(x)
+        if not lists[0]:
+            return result
+        if self.state_bits != 8:
+            lists[4], lists[5] = [], []
+        rc = _lib.binding().adamw_step(*lists, float(first["betas"][0]), float(first["betas"][1]), float(first["eps"]),
+                                       float(self.clip or 0.0), float(self.spike_factor or 0.0), self.state_bits, loss,
+                                       self._control)
+        if rc:
+            _lib.check(rc, "gdn2_adamw_step")
+        return result
+
+    def _word(self, i):
+        if self._control is None:
+            raise RuntimeError("AdamW: no step was made yet")
+        return self._control[i].clone()
+
+    @property
+    def grad_norm(self) -> torch.Tensor:
+        """The last step's global gradient norm before clipping (with clip or spike_factor)."""
+        return self._word(1)
+
+    @property
+    def step_made(self) -> torch.Tensor:
+        """Whether the last step was made (bool, on the device)."""
+        return self._word(2) != 0
+
+    @property
+    def norm_mean(self) -> torch.Tensor:
+        """The running mean of the norms that spike_factor goes by; 0 before the first step."""
+        return torch.zeros(()) if self._control is None else self._word(0)
+
+    @norm_mean.setter
+    def norm_mean(self, value):
+        if self._control is None:
+            self._control = torch.zeros(5, device=self.param_groups[0]["params"][0].device)
+        self._control[0] = value
+
+    @torch.no_grad()
+    def moments(self, params=None, out=None):
+        """What the moments of `params` (all that have been stepped, if None) stand for: a list of (m, v), fp32 in
+        the parameters' shape and order.  `out`: such a list to write into."""
+        if params is None:
+            params = [p for group in self.param_groups for p in group["params"] if self.state.get(p)]
+        states = [self.state[p] for p in params]
+        if any(not st for st in states):
+            raise ValueError("AdamW: a parameter has not been stepped")
+        if out is None:
+            out = [tuple(torch.empty_like(p, dtype=torch.float32, requires_grad=False) for _ in range(2)) for p in params]
+        if len(out) != len(params):
+            raise ValueError("AdamW: params and out have different lengths")
+        if self.state_bits == 32:
+            for st, (m, v) in zip(states, out):
+                m.copy_(st["exp_avg"])
+                v.copy_(st["exp_avg_sq"])
+            return out
+        cols = [[st[n] for st in states] for n in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")]
+        rc = _lib.binding().adamw_moments(*cols, [m for m, _ in out], [v for _, v in out])
+        if rc:
+            _lib.check(rc, "gdn2_adamw_moments")
+        return out
+
+    def load_state_dict(self, state_dict):
+        """torch casts a state to its parameter's type: codes, scales and steps are put back as they were saved."""
+        super().load_state_dict(state_dict)
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        mine = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(saved, mine):
+            st = state_dict["state"].get(i)
+            if not st:
+                continue
+            have = "exp_avg_scale" in st
+            if have != (self.state_bits == 8):
+                raise ValueError(f"AdamW: the saved moments have {8 if have else 32} bits, this optimizer {self.state_bits}")
+            new = self.state[p]
+            for name, x in st.items():
+                if not isinstance(x, torch.Tensor):
+                    x = torch.tensor(float(x))
+                if name in ("exp_avg", "exp_avg_sq"):
+                    new[name] = torch.empty_like(p, dtype=torch.uint8 if have else torch.float32, requires_grad=False)
+                    new[name].copy_(x)
+                else:
+                    new[name] = x.detach().to(p.device, torch.float32).clone()

@@ -12,6 +12,9 @@ Per step, as the reference's jitted `step`:
 Everything stays on the device: `ok` gates the fused AdamW kernel through its found_inf input,
 so a skipped step leaves parameters, moments and the step count untouched (the reference keeps
 the old params and optimizer state) without a host synchronisation.
+
+With the optimizer of .optim (make_optimizer(..., state_bits=32 or 8)) norm, clipping, guard and AdamW are two
+launches of its kernels instead of some seventy of torch's.
 """
 from __future__ import annotations
 
@@ -19,6 +22,8 @@ import math
 
 import torch
 import torch.nn.functional as F
+
+from .optim import AdamW
 
 
 def decay_mask(model: torch.nn.Module):
@@ -38,9 +43,13 @@ def warmup_cosine(step: int, lr: float, warmup: int, total: int, end_frac: float
     return end + (lr - end) * 0.5 * (1.0 + math.cos(math.pi * t))
 
 
-def make_optimizer(model: torch.nn.Module, lr: float, wd: float = 0.1):
-    """train.py:16-19 (the AdamW part; the clip is in TrainStep)."""
+def make_optimizer(model: torch.nn.Module, lr: float, wd: float = 0.1, state_bits=None):
+    """train.py:16-19 (the AdamW part; the clip is in TrainStep).  state_bits 32 or 8: the AdamW of .optim with
+    moments of that size; None: torch's."""
     decay, no_decay = decay_mask(model)
+    if state_bits is not None:
+        return AdamW([{"params": decay, "weight_decay": wd}, {"params": no_decay, "weight_decay": 0.0}],
+                     lr=lr, betas=(0.9, 0.95), eps=1e-8, state_bits=state_bits)
     fused = all(p.is_cuda for p in model.parameters()) or not any(p.is_cuda for p in model.parameters())
     return torch.optim.AdamW([{"params": decay, "weight_decay": wd}, {"params": no_decay, "weight_decay": 0.0}],
                              lr=lr, betas=(0.9, 0.95), eps=1e-8, fused=fused)
@@ -55,8 +64,24 @@ class TrainStep:
         self.lr, self.warmup, self.total, self.clip, self.spike = lr, warmup, total, clip, spike_factor
         dev = next(model.parameters()).device
         self.params = [p for p in model.parameters()]
-        self.gn_ema = torch.zeros((), device=dev)
+        self.own = isinstance(opt, AdamW)     # clips and guards by itself
+        if self.own:
+            opt.clip, opt.spike_factor = clip, spike_factor
+        else:
+            self.gn_ema = torch.zeros((), device=dev)
         self.i = 0
+
+    @property
+    def gn_ema(self) -> torch.Tensor:
+        """The running mean of the gradient norms of the steps that were made."""
+        return self.opt.norm_mean if self.own else self._gn_ema
+
+    @gn_ema.setter
+    def gn_ema(self, value):
+        if self.own:
+            self.opt.norm_mean = value
+        else:
+            self._gn_ema = value
 
     def loss(self, ids: torch.Tensor) -> torch.Tensor:
         lg = self.model(ids)[:, :-1]
@@ -66,6 +91,13 @@ class TrainStep:
         self.i += 1
         loss = self.loss(ids)
         loss.backward()
+        if self.own:
+            lr = warmup_cosine(self.i, self.lr, self.warmup, self.total)
+            for grp in self.opt.param_groups:
+                grp["lr"] = lr
+            self.opt.step(loss=loss)
+            self.opt.zero_grad(set_to_none=False)
+            return loss.detach(), self.opt.grad_norm, self.opt.step_made
         grads = [p.grad for p in self.params]
         gn = torch.linalg.vector_norm(torch.stack(torch._foreach_norm(grads)))
         ok = torch.isfinite(loss) & torch.isfinite(gn) & ((self.gn_ema <= 0) | (gn < self.spike * self.gn_ema))

@@ -1,0 +1,559 @@
+// One AdamW step over all tensors of a model (sm_100a), with the gradients' global norm, clipping by it and a
+// guard that skips steps whose loss or norm is not finite or whose norm jumps.
+//   n = |g|,  g' = g clip / max(n, clip)
+//   m = b1 m + (1 - b1) g',   v = b2 v + (1 - b2) g'^2
+//   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+// Each operation is rounded to fp32 by itself, in this order: the moments that are stored in 8 bits are codes
+// that depend on every bit, and so do not depend on how a compiler joins products and sums.  The squares of the
+// norm are summed in fp64 in a fixed order.
+//
+// Moments in 8 bits: 256 neighbouring values share a scale.  m is e4m3 of m / scale, scale = max |m| / 448.  Of v
+// the root r is stored, unsigned with four bits of exponent and four of mantissa (c 2^-18 below code 16, else
+// (16 + c % 16) 2^(c / 16 - 19)), scale = max r / 1.9375: half a step is 1/32 of r.  A root above zero is never
+// stored as zero, or a later step would divide by eps alone.
+//
+// Bytes bound it: the gradients are read once for their norm and once for the update, p, m and v are read and
+// written once.  Two launches: the norm's, whose last CTA also counts the steps and prepares the tensors'
+// factors, and the update's.  The tensors' table travels in the kernels' parameters: nothing is copied to the
+// device, and a captured graph keeps what it needs.
+#include <cuda_fp8.h>
+
+#include "gdn2_common.cuh"
+
+namespace gdn2 {
+namespace {
+
+constexpr int kChunk = 8192;          // values of a tensor that a CTA takes at a time
+constexpr int kBlock = 256;           // values that share a scale
+constexpr int kAdamThreads = 256;
+constexpr float kNormal = 1.17549435e-38f;
+
+struct AdamEntry {
+  void *p, *m, *v;
+  const void* g;
+  float *ms, *vs, *step;
+  const float* lr_at;
+  double lr, wd;
+  long long n;
+  int first;                          // the tensor's first chunk
+  short bf16, vec;                    // types of p and g; whether all of it may be read 4 values at a time
+};
+template <int N>
+struct AdamTable {
+  AdamEntry e[N];
+  int count, chunks;
+};
+struct Factors {                      // of a tensor
+  float size, root, decay;
+};
+struct AdamControl {                  // the caller's control words
+  float ema, norm, ok, coef;
+  unsigned ticket;
+};
+struct AdamParams {
+  AdamControl* ctl;
+  double* parts;                      // workspace: a chunk's sum of squares
+  Factors* factors;                   // workspace: a tensor's factors
+  const float* loss;
+  double b1, b2, log2_b1, log2_b2;
+  float fb1, gb1, fb2, gb2, eps, clip, spike;
+  int norm, chunk0, all_chunks, tensor0, last, alone;
+};
+
+template <int N>
+__device__ __forceinline__ int find(const AdamTable<N>& t, int chunk) {
+  int lo = 0, hi = t.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (t.e[mid].first <= chunk) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// The tensors' step counts and factors, after the guard has decided.
+template <int N>
+__device__ __forceinline__ void prepare(const AdamTable<N>& t, const AdamParams& a, bool ok) {
+  if (!ok) return;
+  for (int i = threadIdx.x; i < t.count; i += blockDim.x) {
+    const AdamEntry& e = t.e[i];
+    const float n = *e.step + 1.f;
+    *e.step = n;
+    const double lr = e.lr_at ? (double)*e.lr_at : e.lr;
+    a.factors[a.tensor0 + i] = {(float)(lr / (1.0 - exp2((double)n * a.log2_b1))),
+                                (float)sqrt(1.0 - exp2((double)n * a.log2_b2)), (float)(1.0 - lr * e.wd)};
+  }
+}
+
+__device__ __forceinline__ double block_sum(double s, double* sm) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = s;
+  __syncthreads();
+  s = 0.0;
+#pragma unroll
+  for (int i = 0; i < kAdamThreads / 32; ++i) s += sm[i];
+  __syncthreads();
+  return s;
+}
+
+// Sums of the gradients' squares, a CTA to a chunk; the last CTA adds them up and decides.
+template <int N>
+__global__ void __launch_bounds__(kAdamThreads) adamw_norm_kernel(const __grid_constant__ AdamTable<N> t,
+                                                                  const __grid_constant__ AdamParams a) {
+  __shared__ double sm[kAdamThreads / 32];
+  __shared__ bool final, go;
+  pdl_enter();
+  double total = 0.0;
+  if (a.norm) {
+    const AdamEntry& e = t.e[find(t, blockIdx.x)];
+    const long long at = (long long)(blockIdx.x - e.first) * kChunk;
+    const int n = (int)min((long long)kChunk, e.n - at);
+    double s = 0.0;
+    auto add = [&](float x) { s = fma((double)x, (double)x, s); };
+    if (e.bf16) {
+      const __nv_bfloat16* g = static_cast<const __nv_bfloat16*>(e.g) + at;
+      if (e.vec && n == kChunk) {
+#pragma unroll
+        for (int i = 0; i < kChunk / 4 / kAdamThreads; ++i) {
+          float v[4];
+          ld4(g + 4 * (i * kAdamThreads + threadIdx.x), v);
+          for (int j = 0; j < 4; ++j) add(v[j]);
+        }
+      } else {
+        for (int i = threadIdx.x; i < n; i += kAdamThreads) add(ld1(g + i));
+      }
+    } else {
+      const float* g = static_cast<const float*>(e.g) + at;
+      if (e.vec && n == kChunk) {
+#pragma unroll
+        for (int i = 0; i < kChunk / 4 / kAdamThreads; ++i) {
+          float v[4];
+          ld4(g + 4 * (i * kAdamThreads + threadIdx.x), v);
+          for (int j = 0; j < 4; ++j) add(v[j]);
+        }
+      } else {
+        for (int i = threadIdx.x; i < n; i += kAdamThreads) add(ld1(g + i));
+      }
+    }
+    s = block_sum(s, sm);
+    if (threadIdx.x == 0) {
+      a.parts[a.chunk0 + blockIdx.x] = s;
+      __threadfence();
+      final = atomicAdd(&a.ctl->ticket, 1u) == (unsigned)a.all_chunks - 1u;
+    }
+    __syncthreads();
+    if (!final) return;
+    __threadfence();
+    s = 0.0;
+    for (int i = threadIdx.x; i < a.all_chunks; i += kAdamThreads) s += __ldcg(a.parts + i);
+    total = block_sum(s, sm);
+  }
+  // the last CTA, or the only one
+  if (threadIdx.x == 0) {
+    AdamControl& c = *a.ctl;
+    bool ok = !a.loss || isfinite(*a.loss);
+    float coef = 1.f;
+    if (a.norm) {
+      const float n = (float)sqrt(total), ema = c.ema;
+      ok = ok && isfinite(n) && (a.spike <= 0.f || ema <= 0.f || n < a.spike * ema);
+      if (a.clip > 0.f) coef = __fdiv_rn(a.clip, fmaxf(n, a.clip));
+      if (ok) c.ema = ema > 0.f ? __fadd_rn(__fmul_rn(0.98f, ema), __fmul_rn(0.02f, n)) : n;
+      c.norm = n;
+      c.ticket = 0;
+    }
+    c.ok = ok ? 1.f : 0.f;
+    c.coef = coef;
+    go = ok;
+  }
+  __syncthreads();
+  if (a.alone) prepare(t, a, go);
+}
+
+// The factors of one of several tables.
+template <int N>
+__global__ void __launch_bounds__(kAdamThreads) adamw_prepare_kernel(const __grid_constant__ AdamTable<N> t,
+                                                                     const __grid_constant__ AdamParams a) {
+  pdl_enter();
+  prepare(t, a, a.ctl->ok != 0.f);
+}
+
+// One value's step, every operation rounded by itself.
+__device__ __forceinline__ float update(float p, float g, float& m, float& v, const Factors& f, const AdamParams& a) {
+  m = __fadd_rn(__fmul_rn(a.fb1, m), __fmul_rn(a.gb1, g));
+  v = __fadd_rn(__fmul_rn(a.fb2, v), __fmul_rn(a.gb2, __fmul_rn(g, g)));
+  const float d = __fadd_rn(__fdiv_rn(__fsqrt_rn(v), f.root), a.eps);
+  return __fsub_rn(__fmul_rn(p, f.decay), __fmul_rn(f.size, __fdiv_rn(m, d)));
+}
+
+// Loads of memory that the kernel also writes.
+__device__ __forceinline__ void own4(const float* p, float v[4]) {
+  const float4 x = *reinterpret_cast<const float4*>(p);
+  v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+}
+__device__ __forceinline__ void own4(const __nv_bfloat16* p, float v[4]) {
+  const uint2 x = *reinterpret_cast<const uint2*>(p);
+  v[0] = __uint_as_float(x.x << 16); v[1] = __uint_as_float(x.x & 0xffff0000u);
+  v[2] = __uint_as_float(x.y << 16); v[3] = __uint_as_float(x.y & 0xffff0000u);
+}
+__device__ __forceinline__ float own1(const float* p) { return *p; }
+__device__ __forceinline__ float own1(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+template <class T>
+__device__ __forceinline__ void load4(const T* p, float v[4], bool vec, int n) {
+  if (vec) {
+    own4(p, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = j < n ? own1(p + j) : 0.f;
+  }
+}
+__device__ __forceinline__ void store1(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store1(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+template <class T>
+__device__ __forceinline__ void store4(T* p, const float v[4], bool vec, int n) {
+  if (vec) {
+    st4(p, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < n) store1(p + j, v[j]);
+  }
+}
+__device__ __forceinline__ uint32_t codes4(const uint8_t* p, bool vec, int n) {
+  if (vec) return *reinterpret_cast<const uint32_t*>(p);
+  uint32_t c = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (j < n) c |= (uint32_t)p[j] << (8 * j);
+  return c;
+}
+__device__ __forceinline__ void codes4(uint8_t* p, uint32_t c, bool vec, int n) {
+  if (vec) {
+    *reinterpret_cast<uint32_t*>(p) = c;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < n) p[j] = (uint8_t)(c >> (8 * j));
+  }
+}
+
+__device__ __forceinline__ void decode_m(uint32_t c, float scale, float v[4]) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(c >> (16 * j)), __NV_E4M3);
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    v[2 * j] = __fmul_rn(f.x, scale);
+    v[2 * j + 1] = __fmul_rn(f.y, scale);
+  }
+}
+__device__ __forceinline__ void decode_v(uint32_t c, float scale, float v[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    // the code's bits are a float's exponent and mantissa, 2^112 too small
+    const float r = __fmul_rn(__uint_as_float(((c >> (8 * j)) & 255u) << 19) * 0x1p112f, scale);
+    v[j] = __fmul_rn(r, r);
+  }
+}
+__device__ __forceinline__ float bounded(float x, float most) { return x < -most ? -most : x > most ? most : x; }
+// The scale of a warp's block from its lanes' largest magnitude, and what values are multiplied by (0: all are stored
+// as zero).  Compared as bits, so that a NaN is the largest.
+__device__ __forceinline__ float scale_of(float largest, float inverse_top, float& up) {
+  const float s = __fmul_rn(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(largest))), inverse_top);
+  up = s >= kNormal ? __frcp_rn(s) : 0.f;
+  return s;
+}
+__device__ __forceinline__ uint32_t encode_m(const float v[4], float up) {
+  uint32_t c = 0;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const float2 f = make_float2(bounded(__fmul_rn(v[2 * j], up), 448.f), bounded(__fmul_rn(v[2 * j + 1], up), 448.f));
+    c |= (uint32_t)__nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3) << (16 * j);
+  }
+  return c;
+}
+__device__ __forceinline__ uint32_t encode_r(const float r[4], float up) {
+  uint32_t c = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float x = bounded(__fmul_rn(r[j], up), 1.9375f);
+    const uint32_t u = __float_as_uint(x);
+    uint32_t k = x >= 0x1p-14f ? ((u + 0x3ffffu + ((u >> 19) & 1u)) >> 19) - (112u << 4) : (uint32_t)__float2int_rn(x * 0x1p18f);
+    if (r[j] > 0.f && k == 0) k = 1;
+    c |= (k & 255u) << (8 * j);
+  }
+  return c;
+}
+__device__ __forceinline__ float magnitude(float a, float b) {  // the larger magnitude; a NaN is the largest
+  return __uint_as_float(max(__float_as_uint(a) & 0x7fffffffu, __float_as_uint(b) & 0x7fffffffu));
+}
+
+// 4 values of a thread, 8 bits: 8 of a lane, a warp to a block.
+template <class T, bool EIGHT>
+__device__ __forceinline__ void chunk_update(const AdamEntry& e, const AdamParams& a, const Factors& f, float coef,
+                                             long long at, int n) {
+  T* p = static_cast<T*>(e.p) + at;
+  const T* g = static_cast<const T*>(e.g) + at;
+  if constexpr (!EIGHT) {
+    float* m = static_cast<float*>(e.m) + at;
+    float* v = static_cast<float*>(e.v) + at;
+#pragma unroll 2
+    for (int i = threadIdx.x * 4; i < n; i += kAdamThreads * 4) {
+      const bool vec = e.vec && i + 4 <= n;
+      float x[4], y[4], mm[4], vv[4];
+      load4(p + i, x, vec, n - i);
+      load4(g + i, y, vec, n - i);
+      load4(m + i, mm, vec, n - i);
+      load4(v + i, vv, vec, n - i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = update(x[j], __fmul_rn(y[j], coef), mm[j], vv[j], f, a);
+      store4(p + i, x, vec, n - i);
+      store4(m + i, mm, vec, n - i);
+      store4(v + i, vv, vec, n - i);
+    }
+  } else {
+    uint8_t* m = static_cast<uint8_t*>(e.m) + at;
+    uint8_t* v = static_cast<uint8_t*>(e.v) + at;
+    const int lane = threadIdx.x & 31;
+    for (int blk = threadIdx.x >> 5; blk * kBlock < n; blk += kAdamThreads / 32) {
+      const long long s = at / kBlock + blk;
+      const float ms = e.ms[s], vs = e.vs[s];
+      float x[2][4], y[2][4], mm[2][4], vv[2][4], r[2][4], top_m = 0.f, top_r = 0.f;
+      int left[2];
+      bool vec[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int i = blk * kBlock + h * 128 + lane * 4;
+        left[h] = n - i;
+        vec[h] = e.vec && left[h] >= 4;
+        load4(p + i, x[h], vec[h], left[h]);
+        load4(g + i, y[h], vec[h], left[h]);
+        decode_m(codes4(m + i, vec[h], left[h]), ms, mm[h]);
+        decode_v(codes4(v + i, vec[h], left[h]), vs, vv[h]);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          x[h][j] = update(x[h][j], __fmul_rn(y[h][j], coef), mm[h][j], vv[h][j], f, a);
+          if (j >= left[h]) mm[h][j] = vv[h][j] = 0.f;  // past the tensor's end
+          r[h][j] = __fsqrt_rn(vv[h][j]);
+          top_m = magnitude(top_m, mm[h][j]);
+          top_r = magnitude(top_r, r[h][j]);
+        }
+      float up_m, up_r;
+      const float new_ms = scale_of(top_m, 1.f / 448.f, up_m), new_vs = scale_of(top_r, 1.f / 1.9375f, up_r);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int i = blk * kBlock + h * 128 + lane * 4;
+        store4(p + i, x[h], vec[h], left[h]);
+        codes4(m + i, encode_m(mm[h], up_m), vec[h], left[h]);
+        codes4(v + i, encode_r(r[h], up_r), vec[h], left[h]);
+      }
+      if (lane == 0) {
+        e.ms[s] = new_ms;
+        e.vs[s] = new_vs;
+      }
+    }
+  }
+}
+
+template <int N, bool EIGHT>
+__global__ void __launch_bounds__(kAdamThreads) adamw_update_kernel(const __grid_constant__ AdamTable<N> t,
+                                                                    const __grid_constant__ AdamParams a) {
+  pdl_enter();
+  if (__ldcg(&a.ctl->ok) == 0.f) return;
+  const float coef = __ldcg(&a.ctl->coef);
+  for (int chunk = blockIdx.x; chunk < t.chunks; chunk += gridDim.x) {
+    const int i = find(t, chunk);
+    const AdamEntry& e = t.e[i];
+    const Factors& from = a.factors[a.tensor0 + i];
+    const Factors f = {__ldcg(&from.size), __ldcg(&from.root), __ldcg(&from.decay)};
+    const long long at = (long long)(chunk - e.first) * kChunk;
+    const int n = (int)min((long long)kChunk, e.n - at);
+    if (e.bf16) chunk_update<__nv_bfloat16, EIGHT>(e, a, f, coef, at, n);
+    else chunk_update<float, EIGHT>(e, a, f, coef, at, n);
+  }
+}
+
+// What 8-bit moments stand for: m and v in fp32, to where the entry's p and g point.
+template <int N>
+__global__ void __launch_bounds__(kAdamThreads) adamw_moments_kernel(const __grid_constant__ AdamTable<N> t) {
+  for (int chunk = blockIdx.x; chunk < t.chunks; chunk += gridDim.x) {
+    const AdamEntry& e = t.e[find(t, chunk)];
+    const long long at = (long long)(chunk - e.first) * kChunk;
+    const int n = (int)min((long long)kChunk, e.n - at);
+    const uint8_t* m = static_cast<const uint8_t*>(e.m) + at;
+    const uint8_t* v = static_cast<const uint8_t*>(e.v) + at;
+    float* om = static_cast<float*>(e.p) + at;
+    float* ov = static_cast<float*>(const_cast<void*>(e.g)) + at;
+#pragma unroll 2
+    for (int i = threadIdx.x * 4; i < n; i += kAdamThreads * 4) {
+      const bool vec = e.vec && i + 4 <= n;
+      float x[4];
+      decode_m(codes4(m + i, vec, n - i), e.ms[(at + i) / kBlock], x);
+      store4(om + i, x, vec, n - i);
+      decode_v(codes4(v + i, vec, n - i), e.vs[(at + i) / kBlock], x);
+      store4(ov + i, x, vec, n - i);
+    }
+  }
+}
+
+// ---- host ---------------------------------------------------------------------------------------
+constexpr int kFew = 32, kMany = 320;  // tensors of a table: 3 and 31 KB of parameters
+
+bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+gdn2_status check_adamw(const gdn2_adamw_desc* d, const gdn2_adamw_tensor* ts, int32_t n) {
+  if (!d || n < 0 || (n && !ts) || (d->state_bits != 32 && d->state_bits != 8)) return GDN2_ERR_INVALID_ARGUMENT;
+  if (!(d->beta1 >= 0 && d->beta1 < 1 && d->beta2 >= 0 && d->beta2 < 1 && d->eps >= 0 && d->clip >= 0 && d->spike >= 0))
+    return GDN2_ERR_INVALID_ARGUMENT;
+  long long chunks = 0;
+  for (int i = 0; i < n; ++i) {
+    const gdn2_adamw_tensor& t = ts[i];
+    if (t.n < 0 || (t.dtype != GDN2_F32 && t.dtype != GDN2_BF16)) return GDN2_ERR_INVALID_ARGUMENT;
+    if (t.n > 1ll << 42) return GDN2_ERR_UNSUPPORTED;
+    if (!t.n) continue;
+    const size_t el = t.dtype == GDN2_BF16 ? 2 : 4, st = d->state_bits == 8 ? 1 : 4;
+    if (!t.p || !t.g || !t.m || !t.v || !aligned(t.p, el) || !aligned(t.g, el) || !aligned(t.m, st) || !aligned(t.v, st))
+      return GDN2_ERR_INVALID_ARGUMENT;
+    if (st == 1 && (!t.m_scale || !t.v_scale || !aligned(t.m_scale, 4) || !aligned(t.v_scale, 4)))
+      return GDN2_ERR_INVALID_ARGUMENT;
+    chunks += (t.n + kChunk - 1) / kChunk;
+  }
+  return chunks < 1ll << 30 ? GDN2_OK : GDN2_ERR_UNSUPPORTED;
+}
+
+// Fills a table from ts[i..) and returns the next index.
+template <int N>
+int fill(AdamTable<N>& t, const gdn2_adamw_desc* d, const gdn2_adamw_tensor* ts, int i, int n) {
+  t.count = t.chunks = 0;
+  const size_t st = d->state_bits == 8 ? 4 : 16;
+  for (; i < n && t.count < N; ++i) {
+    const gdn2_adamw_tensor& s = ts[i];
+    if (!s.n) continue;
+    const size_t el = s.dtype == GDN2_BF16 ? 8 : 16;
+    AdamEntry& e = t.e[t.count++];
+    e.p = s.p; e.g = s.g; e.m = s.m; e.v = s.v; e.ms = s.m_scale; e.vs = s.v_scale;
+    e.step = s.step; e.lr_at = s.lr_at; e.lr = s.lr; e.wd = s.weight_decay; e.n = s.n;
+    e.first = t.chunks;
+    e.bf16 = s.dtype == GDN2_BF16;
+    e.vec = aligned(s.p, el) && aligned(s.g, el) && aligned(s.m, st) && aligned(s.v, st);
+    t.chunks += (int)((s.n + kChunk - 1) / kChunk);
+  }
+  return i;
+}
+
+struct AdamTotal {
+  int tensors, chunks;
+};
+AdamTotal totals(const gdn2_adamw_tensor* ts, int n) {
+  AdamTotal r{0, 0};
+  for (int i = 0; i < n; ++i)
+    if (ts[i].n) {
+      ++r.tensors;
+      r.chunks += (int)((ts[i].n + kChunk - 1) / kChunk);
+    }
+  return r;
+}
+size_t parts_bytes(int chunks) { return ((size_t)chunks * sizeof(double) + 255) / 256 * 256; }
+
+template <int N>
+cudaError_t run_adamw(const gdn2_adamw_desc* d, const gdn2_adamw_tensor* ts, int n, AdamParams a, cudaStream_t st) {
+  static thread_local AdamTable<N> t;  // 31 KB: not on the stack
+  cudaError_t e = cudaSuccess;
+  const AdamTotal all = totals(ts, n);
+  a.alone = all.tensors <= N;
+  a.all_chunks = all.chunks;
+  a.chunk0 = a.tensor0 = 0;
+  if (a.norm || a.alone) {
+    for (int i = 0, done = 0; i < n && e == cudaSuccess;) {
+      i = fill(t, d, ts, i, n);
+      if (!t.count) break;
+      e = launch_pdl(adamw_norm_kernel<N>, a.norm ? t.chunks : 1, kAdamThreads, 0, st, t, a);
+      a.chunk0 += t.chunks;
+      done += t.count;
+    }
+  }
+  if (!a.alone) {
+    if (!a.norm && e == cudaSuccess) {  // the guard alone, over no tensors
+      t.count = t.chunks = 0;
+      e = launch_pdl(adamw_norm_kernel<N>, 1, kAdamThreads, 0, st, t, a);
+    }
+    for (int i = 0; i < n && e == cudaSuccess;) {
+      i = fill(t, d, ts, i, n);
+      if (!t.count) break;
+      e = launch_pdl(adamw_prepare_kernel<N>, 1, kAdamThreads, 0, st, t, a);
+      a.tensor0 += t.count;
+    }
+    a.tensor0 = 0;
+  }
+  for (int i = 0; i < n && e == cudaSuccess;) {
+    i = fill(t, d, ts, i, n);
+    if (!t.count) break;
+    const unsigned grid = t.chunks < 148 * 8 ? t.chunks : 148 * 8;
+    e = d->state_bits == 8 ? launch_pdl(adamw_update_kernel<N, true>, grid, kAdamThreads, 0, st, t, a)
+                           : launch_pdl(adamw_update_kernel<N, false>, grid, kAdamThreads, 0, st, t, a);
+    a.tensor0 += t.count;
+  }
+  return e;
+}
+
+template <int N>
+cudaError_t run_moments(const gdn2_adamw_desc* d, const gdn2_adamw_tensor* ts, int n, cudaStream_t st) {
+  static thread_local AdamTable<N> t;
+  for (int i = 0; i < n;) {
+    i = fill(t, d, ts, i, n);
+    if (!t.count) break;
+    adamw_moments_kernel<N><<<t.chunks < 148 * 8 ? t.chunks : 148 * 8, kAdamThreads, 0, st>>>(t);
+  }
+  return cudaGetLastError();
+}
+
+}  // namespace
+}  // namespace gdn2
+
+extern "C" size_t gdn2_adamw_workspace_bytes(const gdn2_adamw_desc* d, const gdn2_adamw_tensor* tensors, int32_t n) {
+  using namespace gdn2;
+  if (check_adamw(d, tensors, n) != GDN2_OK) return 0;
+  const AdamTotal all = totals(tensors, n);
+  return all.tensors ? parts_bytes(all.chunks) + all.tensors * sizeof(Factors) : 0;
+}
+
+extern "C" gdn2_status gdn2_adamw_step(const gdn2_adamw_desc* d, const gdn2_adamw_tensor* tensors, int32_t n,
+                                       const float* loss, void* control, void* workspace, void* stream) {
+  using namespace gdn2;
+  const gdn2_status s = check_adamw(d, tensors, n);
+  if (s != GDN2_OK) return s;
+  const AdamTotal all = totals(tensors, n);
+  if (!all.tensors) return GDN2_OK;
+  for (int i = 0; i < n; ++i)
+    if (tensors[i].n && (!tensors[i].step || !aligned(tensors[i].step, 4))) return GDN2_ERR_INVALID_ARGUMENT;
+  if (!control || !aligned(control, 4) || !workspace || !aligned(workspace, 256)) return GDN2_ERR_INVALID_ARGUMENT;
+  AdamParams a{};
+  a.ctl = static_cast<AdamControl*>(control);
+  a.parts = static_cast<double*>(workspace);
+  a.factors = reinterpret_cast<Factors*>(static_cast<uint8_t*>(workspace) + parts_bytes(all.chunks));
+  a.loss = loss;
+  a.log2_b1 = log2(d->beta1); a.log2_b2 = log2(d->beta2);
+  a.fb1 = (float)d->beta1; a.gb1 = (float)(1.0 - d->beta1);
+  a.fb2 = (float)d->beta2; a.gb2 = (float)(1.0 - d->beta2);
+  a.eps = (float)d->eps; a.clip = (float)d->clip; a.spike = (float)d->spike;
+  a.norm = d->clip > 0 || d->spike > 0;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = all.tensors <= kFew ? run_adamw<kFew>(d, tensors, n, a, st) : run_adamw<kMany>(d, tensors, n, a, st);
+  return e == cudaSuccess ? GDN2_OK : GDN2_ERR_CUDA;
+}
+
+extern "C" gdn2_status gdn2_adamw_moments(const gdn2_adamw_tensor* tensors, int32_t n, void* stream) {
+  using namespace gdn2;
+  gdn2_adamw_desc d{};
+  d.state_bits = 8;
+  const gdn2_status s = check_adamw(&d, tensors, n);
+  if (s != GDN2_OK) return s;
+  for (int i = 0; i < n; ++i)
+    if (tensors[i].dtype != GDN2_F32) return GDN2_ERR_INVALID_ARGUMENT;
+  const AdamTotal all = totals(tensors, n);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = all.tensors <= kFew ? run_moments<kFew>(&d, tensors, n, st) : run_moments<kMany>(&d, tensors, n, st);
+  return e == cudaSuccess ? GDN2_OK : GDN2_ERR_CUDA;
+}

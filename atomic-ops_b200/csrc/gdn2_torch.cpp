@@ -1,4 +1,5 @@
-// The short way from a Python call of a serving operator to its launch, as a CPython extension.
+// The short way from a Python call of a serving operator to its launch, and the optimizer's step, as a CPython
+// extension.
 //
 // A decode step's kernels take a few microseconds, less than the interpreter needs to look at the
 // tensors, allocate the outputs and pass the pointers on.  These functions do that for calls that need
@@ -7,8 +8,10 @@
 // The checks here are a subset of that path's, so nothing is accepted that it would refuse.
 #include <ATen/cuda/EmptyTensor.h>
 #include <ATen/core/Tensor.h>
+#include <ATen/ops/empty_like.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -246,10 +249,170 @@ PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- the optimizer ----------------------------------------------------------------------------------
+// Its step is one call over lists of tensors, so these are the whole host path, with errors of their own.
+
+std::vector<at::Tensor> tensors(PyObject* list, const char* what) {
+  TORCH_CHECK_TYPE(PyList_CheckExact(list), what, " must be a list");
+  std::vector<at::Tensor> r;
+  r.reserve(PyList_GET_SIZE(list));
+  for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) {
+    PyObject* o = PyList_GET_ITEM(list, i);
+    TORCH_CHECK_TYPE(THPVariable_Check(o), what, " must hold tensors");
+    r.push_back(THPVariable_Unpack(o));
+  }
+  return r;
+}
+void changed(const at::Tensor& t) {  // in place: autograd may have saved it
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+float* floats(const at::Tensor& t) { return static_cast<float*>(t.data_ptr()); }
+// The codes or values of a moment: p's shape and order.
+void check_moment(const at::Tensor& t, const at::Tensor& p, at::ScalarType type, const char* what) {
+  TORCH_CHECK_VALUE(t.device() == p.device() && t.scalar_type() == type && t.sizes() == p.sizes() &&
+                        (t.strides() == p.strides() || (t.is_contiguous() && p.is_contiguous())),
+                    "AdamW: ", what, " of a ", p.sizes(), " parameter must be ", type, " of its shape and order on ",
+                    p.device(), "; got ", t.sizes(), " ", t.scalar_type(), " on ", t.device());
+}
+void check_scale(const at::Tensor& t, const at::Tensor& p, const char* what) {
+  TORCH_CHECK_VALUE(t.device() == p.device() && t.scalar_type() == at::kFloat && t.is_contiguous() &&
+                        t.numel() == (p.numel() + 255) / 256,
+                    "AdamW: ", what, " of a ", p.sizes(), " parameter must be ", (p.numel() + 255) / 256,
+                    " contiguous float32 on ", p.device());
+}
+
+// adamw_step(params, grads, m, v, m_scales, v_scales, steps, lrs, decays, beta1, beta2, eps, clip, spike, bits, loss, control)
+PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 17, "adamw_step takes 17 arguments");
+  auto p = tensors(a[0], "params"), g = tensors(a[1], "grads"), m = tensors(a[2], "exp_avg"), v = tensors(a[3], "exp_avg_sq");
+  auto ms = tensors(a[4], "scales"), vs = tensors(a[5], "scales"), steps = tensors(a[6], "steps");
+  gdn2_adamw_desc d{};
+  d.beta1 = PyFloat_AsDouble(a[9]);
+  d.beta2 = PyFloat_AsDouble(a[10]);
+  d.eps = PyFloat_AsDouble(a[11]);
+  d.clip = PyFloat_AsDouble(a[12]);
+  d.spike = PyFloat_AsDouble(a[13]);
+  d.state_bits = (int32_t)PyLong_AsLong(a[14]);
+  if (PyErr_Occurred()) return nullptr;
+  const size_t k = p.size();
+  const bool eight = d.state_bits == 8;
+  TORCH_CHECK_VALUE(g.size() == k && m.size() == k && v.size() == k && steps.size() == k &&
+                        (!eight || (ms.size() == k && vs.size() == k)) && PyList_CheckExact(a[7]) &&
+                        (size_t)PyList_GET_SIZE(a[7]) == k && PyList_CheckExact(a[8]) && (size_t)PyList_GET_SIZE(a[8]) == k,
+                    "AdamW: lists of different lengths");
+  if (!k) Py_RETURN_NONE;
+  const auto dev = p[0].device();
+  TORCH_CHECK(dev.is_cuda(), "AdamW: the parameters must be on a CUDA device (the step runs only on the B200 kernels)");
+  std::vector<gdn2_adamw_tensor> table(k);
+  const c10::cuda::CUDAGuard guard(dev);
+  for (size_t i = 0; i < k; ++i) {
+    gdn2_adamw_tensor& t = table[i];
+    const at::Tensor& q = p[i];
+    const auto type = q.scalar_type();
+    TORCH_CHECK_VALUE(q.device() == dev, "AdamW: parameters on ", q.device(), " and on ", dev, ": one optimizer steps one device's");
+    TORCH_CHECK_VALUE(type == at::kFloat || type == at::kBFloat16, "AdamW: parameters must be float32 or bfloat16, not ", type);
+    TORCH_CHECK_VALUE(q.layout() == at::kStrided && q.is_non_overlapping_and_dense(),
+                      "AdamW: a parameter's values must fill their memory, each at one place");
+    TORCH_CHECK_VALUE(g[i].layout() == at::kStrided && g[i].device() == dev && g[i].sizes() == q.sizes() && !g[i].is_complex(),
+                      "AdamW: a gradient must be dense, of its parameter's shape and device");
+    if (g[i].scalar_type() != type || (g[i].strides() != q.strides() && !(g[i].is_contiguous() && q.is_contiguous()))) {
+      at::Tensor c = at::empty_like(q);
+      c.copy_(g[i]);
+      g[i] = std::move(c);
+    }
+    check_moment(m[i], q, eight ? at::kByte : at::kFloat, "exp_avg");
+    check_moment(v[i], q, eight ? at::kByte : at::kFloat, "exp_avg_sq");
+    if (eight) {
+      check_scale(ms[i], q, "exp_avg_scale");
+      check_scale(vs[i], q, "exp_avg_sq_scale");
+      t.m_scale = floats(ms[i]);
+      t.v_scale = floats(vs[i]);
+    }
+    TORCH_CHECK_VALUE(steps[i].device() == dev && steps[i].scalar_type() == at::kFloat && steps[i].numel() == 1,
+                      "AdamW: step must be one float32 value on ", dev);
+    t.p = q.data_ptr(); t.g = g[i].data_ptr(); t.m = m[i].data_ptr(); t.v = v[i].data_ptr();
+    t.step = floats(steps[i]);
+    PyObject* lr = PyList_GET_ITEM(a[7], i);
+    if (THPVariable_Check(lr)) {
+      const at::Tensor& r = THPVariable_Unpack(lr);
+      TORCH_CHECK_VALUE(r.device() == dev && r.scalar_type() == at::kFloat && r.numel() == 1,
+                        "AdamW: a tensor for lr must be one float32 value on ", dev);
+      t.lr_at = floats(r);
+    } else {
+      t.lr = PyFloat_AsDouble(lr);
+    }
+    t.weight_decay = PyFloat_AsDouble(PyList_GET_ITEM(a[8], i));
+    if (PyErr_Occurred()) return nullptr;
+    t.n = q.numel();
+    t.dtype = dtype_of(type);
+  }
+  const float* loss = nullptr;
+  at::Tensor loss32;
+  if (a[15] != Py_None) {
+    TORCH_CHECK_TYPE(THPVariable_Check(a[15]), "AdamW: loss must be a tensor");
+    loss32 = THPVariable_Unpack(a[15]);
+    TORCH_CHECK_VALUE(loss32.device() == dev && loss32.numel() == 1, "AdamW: loss must be one value on ", dev);
+    loss32 = loss32.detach().to(at::kFloat);
+    loss = floats(loss32);
+  }
+  TORCH_CHECK_TYPE(THPVariable_Check(a[16]), "AdamW: control must be a tensor");
+  const at::Tensor& control = THPVariable_Unpack(a[16]);
+  TORCH_CHECK_VALUE(control.device() == dev && control.scalar_type() == at::kFloat && control.numel() == 5 && control.is_contiguous(),
+                    "AdamW: control must be five float32 words on ", dev);
+  const int64_t size[1] = {(int64_t)gdn2_adamw_workspace_bytes(&d, table.data(), (int32_t)k)};
+  at::Tensor ws = fresh(size, at::kByte, dev);
+  const gdn2_status s = gdn2_adamw_step(&d, table.data(), (int32_t)k, loss, control.data_ptr(), ws.data_ptr(),
+                                        c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+  if (s == GDN2_OK)
+    for (size_t i = 0; i < k; ++i) {
+      changed(p[i]); changed(m[i]); changed(v[i]); changed(steps[i]);
+      if (eight) { changed(ms[i]); changed(vs[i]); }
+    }
+  return PyLong_FromLong(s);
+  END_HANDLE_TH_ERRORS
+}
+
+// adamw_moments(m, v, m_scales, v_scales, out_m, out_v)
+PyObject* adamw_moments(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 6, "adamw_moments takes 6 arguments");
+  auto m = tensors(a[0], "exp_avg"), v = tensors(a[1], "exp_avg_sq"), ms = tensors(a[2], "scales"), vs = tensors(a[3], "scales");
+  auto om = tensors(a[4], "out"), ov = tensors(a[5], "out");
+  const size_t k = m.size();
+  TORCH_CHECK_VALUE(v.size() == k && ms.size() == k && vs.size() == k && om.size() == k && ov.size() == k,
+                    "AdamW: lists of different lengths");
+  if (!k) return PyLong_FromLong(GDN2_OK);
+  const auto dev = m[0].device();
+  TORCH_CHECK(dev.is_cuda(), "AdamW: the moments must be on a CUDA device");
+  const c10::cuda::CUDAGuard guard(dev);
+  std::vector<gdn2_adamw_tensor> table(k);
+  for (size_t i = 0; i < k; ++i) {
+    gdn2_adamw_tensor& t = table[i];
+    TORCH_CHECK_VALUE(m[i].device() == dev && m[i].is_non_overlapping_and_dense(), "AdamW: moments on several devices");
+    check_moment(m[i], m[i], at::kByte, "exp_avg");
+    check_moment(v[i], m[i], at::kByte, "exp_avg_sq");
+    check_scale(ms[i], m[i], "exp_avg_scale");
+    check_scale(vs[i], m[i], "exp_avg_sq_scale");
+    check_moment(om[i], m[i], at::kFloat, "out");
+    check_moment(ov[i], m[i], at::kFloat, "out");
+    t.m = m[i].data_ptr(); t.v = v[i].data_ptr(); t.m_scale = floats(ms[i]); t.v_scale = floats(vs[i]);
+    t.p = om[i].data_ptr(); t.g = ov[i].data_ptr();
+    t.n = m[i].numel();
+    t.dtype = GDN2_F32;
+  }
+  const gdn2_status s = gdn2_adamw_moments(table.data(), (int32_t)k, c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+  for (size_t i = 0; i < k; ++i) { changed(om[i]); changed(ov[i]); }
+  return PyLong_FromLong(s);
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"recurrent", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(recurrent)), METH_FASTCALL, nullptr},
     {"w4_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(w4_linear)), METH_FASTCALL, nullptr},
     {"beam_select", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(beam_select)), METH_FASTCALL, nullptr},
+    {"adamw_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(adamw_step)), METH_FASTCALL, nullptr},
+    {"adamw_moments", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(adamw_moments)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "gdn2_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

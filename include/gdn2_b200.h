@@ -340,6 +340,43 @@ gdn2_status gdn2_gated_bwd(const gdn2_gated_desc* desc, const void* x, const voi
                            const uint8_t* reset, const float* marks, const void* dh, const float* dlast, void* dx,
                            void* dg, float* dh0, void* stream);
 
+/* One AdamW step over many tensors, with their gradients' global norm n, clipping and a guard:
+ *   g' = g clip / max(n, clip),  m = b1 m + (1 - b1) g',  v = b2 v + (1 - b2) g'^2,
+ *   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps).
+ * With clip or spike > 0 the norm is taken, and a step whose loss or norm is not finite, or whose norm is not below
+ * spike times the mean of earlier norms (ema > 0), changes nothing but the control's norm and ok. */
+typedef struct gdn2_adamw_desc {
+  int32_t state_bits;     /* 32: m and v are fp32.  8: codes with a scale per 256 values */
+  int32_t reserved;
+  double beta1, beta2, eps;
+  double clip, spike;     /* 0: none */
+} gdn2_adamw_desc;
+
+typedef struct gdn2_adamw_tensor {
+  void *p, *m, *v;        /* n values each, in one order, aligned to their types */
+  const void* g;
+  float *m_scale, *v_scale; /* ceil(n / 256) fp32 each (state_bits 8): m = e4m3(code) m_scale; v = (r v_scale)^2 with
+                               r = c 2^-18 for codes c < 16, (16 + c % 16) 2^(c / 16 - 19) from there on */
+  float* step;            /* the tensor's step count, in device memory */
+  const float* lr_at;     /* the rate in device memory, or NULL for lr */
+  double lr, weight_decay;
+  int64_t n;              /* 0: the tensor is passed over */
+  int32_t dtype;          /* gdn2_dtype of p and g */
+  int32_t reserved;
+} gdn2_adamw_tensor;
+
+/*   loss      one fp32 value in device memory, or NULL
+ *   control   five 32-bit words in device memory, zero before the first step and kept between steps: the mean of
+ *             earlier norms (fp32), the norm, whether the step was made (0 or 1), the clipping factor, a counter
+ *   workspace gdn2_adamw_workspace_bytes bytes, 256-byte aligned */
+gdn2_status gdn2_adamw_step(const gdn2_adamw_desc* desc, const gdn2_adamw_tensor* tensors, int32_t n,
+                            const float* loss, void* control, void* workspace, void* stream);
+size_t gdn2_adamw_workspace_bytes(const gdn2_adamw_desc* desc, const gdn2_adamw_tensor* tensors, int32_t n);
+
+/* What 8-bit moments stand for: m and v in fp32 to where p and g of the entries point (dtype GDN2_F32; step, lr and
+ * weight_decay are not read). */
+gdn2_status gdn2_adamw_moments(const gdn2_adamw_tensor* tensors, int32_t n, void* stream);
+
 /* Profiling hook (no counterpart in the reference).  While enabled, every kernel launch of
  * gdn2_fwd / gdn2_bwd is bracketed by CUDA events recorded on the caller's stream.
  * gdn2_profile_collect synchronises on those events, writes per-kernel summed milliseconds and
