@@ -74,6 +74,15 @@ class GatedDesc(ctypes.Structure):
     ]
 
 
+class LinearDesc(ctypes.Structure):
+    """struct gdn2_linear_desc."""
+    _fields_ = [
+        ("M", ctypes.c_int32), ("K", ctypes.c_int32), ("N", ctypes.c_int32), ("dtype", ctypes.c_int32),
+        ("bias_dtype", ctypes.c_int32), ("act", ctypes.c_int32),
+        ("x_stride", ctypes.c_int64), ("w_stride", ctypes.c_int64), ("res_stride", ctypes.c_int64),
+    ]
+
+
 class AdamwDesc(ctypes.Structure):
     """struct gdn2_adamw_desc."""
     _fields_ = [
@@ -100,6 +109,7 @@ EXPORTS = ("gdn2_residual_bytes", "gdn2_fwd_workspace_bytes", "gdn2_bwd_workspac
            "gdn2_selftest_wait_timeout", "gdn2_recurrent", "gdn2_recurrent_workspace_bytes", "gdn2_w4_linear",
            "gdn2_w4_workspace_bytes", "gdn2_beam_select",
            "gdn2_beam_workspace_bytes", "gdn2_gated_fwd", "gdn2_gated_bwd", "gdn2_gated_marks_bytes",
+           "gdn2_linear_fwd", "gdn2_linear_fwd_workspace_bytes", "gdn2_linear_bwd", "gdn2_linear_bwd_workspace_bytes",
            "gdn2_adamw_step", "gdn2_adamw_workspace_bytes", "gdn2_adamw_moments")
 # kernel ids of gdn2_profile_collect
 KERNELS = ("fwd_intra", "fwd_scan", "fwd_out", "bwd_pre", "bwd_scan", "bwd_intra")
@@ -158,6 +168,14 @@ def _declare(lib):
     lib.gdn2_gated_bwd.argtypes = [P] * 12
     lib.gdn2_gated_marks_bytes.restype = ctypes.c_size_t
     lib.gdn2_gated_marks_bytes.argtypes = [P]
+    lib.gdn2_linear_fwd.restype = ctypes.c_int
+    lib.gdn2_linear_fwd.argtypes = [P] * 10
+    lib.gdn2_linear_fwd_workspace_bytes.restype = ctypes.c_size_t
+    lib.gdn2_linear_fwd_workspace_bytes.argtypes = [P]
+    lib.gdn2_linear_bwd.restype = ctypes.c_int
+    lib.gdn2_linear_bwd.argtypes = [P] * 11
+    lib.gdn2_linear_bwd_workspace_bytes.restype = ctypes.c_size_t
+    lib.gdn2_linear_bwd_workspace_bytes.argtypes = [P, ctypes.c_int32]
     lib.gdn2_adamw_step.restype = ctypes.c_int
     lib.gdn2_adamw_step.argtypes = [P, P, ctypes.c_int32, P, P, P, P]
     lib.gdn2_adamw_workspace_bytes.restype = ctypes.c_size_t

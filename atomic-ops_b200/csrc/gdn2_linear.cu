@@ -1,0 +1,946 @@
+// The linear product with its epilogue, and its backward (sm_100a).
+//   z = x W + b,  y = act(z) + r;    dz = dy act'(z),  db = sum over rows of dz,  dx = dz W^T,  dW = x^T dz
+// x (M, K), W (K, N), y, z, r (M, N) are bf16 or fp32; sums are fp32.
+//
+// All three products run on the 5th-generation tensor cores from bf16 operands: D (rows, cols) = A B with A and B
+// read in place by tiled copies, either of them contiguous along the summed dimension or across it (W in the
+// forward, x and dz for dW), so that nothing is transposed in memory.  An fp32 operand is first cut into three
+// bf16 terms of 8 bits each (x = t0 + t1 + t2 to 2^-27 of x), and the six products t_i u_j with i + j <= 2 are
+// summed, the small ones first: what is left out is below 2^-26 of a product.  fp32's whole range of exponents
+// is kept, which two fp16 terms with a scale (half the products) would not.
+// The tensor cores' additions may truncate, so fp32 sums leave them every 64 values of the summed dimension and
+// go on in registers with rounded additions.
+// An infinite or huge fp32 value makes infinities of opposite signs in its terms: a result that is NaN is summed
+// again by itself from the fp32 operands, and so is what the plain sum makes of them.
+//
+// One CTA a SM (or a pair of CTAs on two SMs, whose tile of 256 x 256 shares the operands between them) walks
+// output tiles; a warp issues the copies, one thread the products into one of two accumulators in tensor
+// memory, eight warps empty the other one through the epilogue.  Few tiles with a long sum are split along it,
+// and a second launch adds the parts in a fixed order.
+#include <cooperative_groups.h>
+#include <cuda.h>
+
+#include "gdn2_common.cuh"
+
+namespace gdn2 {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int kBK = 64;                 // values of the summed dimension in a stage: 128 bytes of bf16
+constexpr int kEpiWarps = 8;
+constexpr int kGemmThreads = 32 * (kEpiWarps + 2);
+constexpr int kStageRow = 128;          // bytes
+constexpr size_t kStagingBytes = kEpiWarps * 32 * 33 * sizeof(float);
+
+// How a result element leaves: y = act(v + bias) + residual, with v + bias kept in z.
+struct Epilogue {
+  void* y;
+  void* z;                              // null: not kept
+  const void* bias;                     // null: none
+  const void* residual;                 // null: none
+  long long ldr;
+  long long ldy;                        // y and z
+  int y_bf16, bias_bf16, act;
+  float* parts;                         // not null: sums go here, (splits, rows, cols) fp32
+  // the operands in fp32, for sums that are NaN; null: bf16 operands, whose sums are as they are
+  const float *a, *b;
+  long long a_row, a_k, b_col, b_k;     // element strides
+};
+
+struct GemmParams {
+  Epilogue ep;
+  int rows, cols, k;
+  int tiles_m, tiles_n, splits, kblocks, per_split;   // per_split: k blocks of a split
+  int a_mn, b_mn;                       // contiguous across the summed dimension
+  uint32_t* flags;
+};
+
+// ---- activation ---------------------------------------------------------------------------------
+constexpr float kGeluC = 0.7978845608028654f, kGeluA = 0.044715f;
+__device__ __forceinline__ float gelu(float z) {
+  const float t = tanhf(kGeluC * (z + kGeluA * z * z * z));
+  return 0.5f * z * (1.f + t);
+}
+__device__ __forceinline__ float gelu_slope(float z) {
+  const float t = tanhf(kGeluC * (z + kGeluA * z * z * z));
+  return 0.5f * (1.f + t) + 0.5f * z * (1.f - t * t) * kGeluC * (1.f + 3.f * kGeluA * z * z);
+}
+
+__device__ __forceinline__ float load_f(const void* p, long long i, int bf16) {
+  return bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]) : static_cast<const float*>(p)[i];
+}
+__device__ __forceinline__ void store_f(void* p, long long i, int bf16, float v) {
+  if (bf16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  else static_cast<float*>(p)[i] = v;
+}
+
+// A sum that is NaN, again from the operands themselves.
+__device__ __noinline__ float plain_sum(const Epilogue& e, long long row, long long col, int k) {
+  float s = 0.f;
+  for (int i = 0; i < k; ++i) s = fmaf(e.a[row * e.a_row + i * e.a_k], e.b[col * e.b_col + i * e.b_k], s);
+  return s;
+}
+
+__device__ __forceinline__ void finish(const Epilogue& e, long long row, long long col, float v, int k, float bias) {
+  if (e.a && v != v) v = plain_sum(e, row, col, k);
+  v += bias;
+  const long long at = row * e.ldy + col;
+  if (e.z) store_f(e.z, at, e.y_bf16, v);
+  if (e.act == GDN2_ACT_GELU_TANH) v = gelu(v);
+  if (e.residual) v += load_f(e.residual, row * e.ldr + col, e.y_bf16);
+  store_f(e.y, at, e.y_bf16, v);
+}
+
+// ---- the product --------------------------------------------------------------------------------
+template <int CG, int P>
+struct Gemm {
+  static constexpr int kTileM = 128 * CG, kTileN = 128 * CG;        // of the CTA or the pair
+  static constexpr int kOperand = 128 * kStageRow;                  // a CTA's part of one term of A or of B
+  static constexpr int kStage = 2 * P * kOperand;
+  static constexpr int kStages = P == 1 ? 6 : 2;
+  static constexpr int kTmem = 2 * kTileN;                          // two accumulators' columns
+  static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + kStagingBytes + 256;
+};
+
+// A wait that ends: after kWaitCycles, or once another of this CTA's waits has run out.
+__device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t parity, volatile int* dead, uint32_t* flags) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  for (uint32_t it = 0;; ++it) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (*dead) return false;
+    if ((it & 255u) == 255u && clock64() - t0 > kWaitCycles) {
+      *dead = 1;
+      if (flags) flags[2] = 1;
+      return false;
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t leader_addr(const void* p) {    // the same place in the cluster's CTA 0
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
+  return r;
+}
+template <int CG>
+__device__ __forceinline__ void tile_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
+        "%4}], [%5];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(0), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
+            "r"(dst), "l"(map), "r"(x), "r"(y), "r"(0), "r"(bar)
+        : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void mma_bf16(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(accumulate)
+        : "memory");
+  else
+    mma_t<kBF16>(d, a, b, id, accumulate);
+}
+// Arrives at the barrier of every CTA of the pair once the products issued so far are done.
+template <int CG>
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+  else
+    mma_commit(bar);
+}
+// Operand descriptors, 128-byte swizzle.  Contiguous along the sum: rows of 128 bytes, eight rows (1024 bytes) an
+// atom, 16 values further 32 bytes on.  Contiguous across it: blocks of 64 across x 64 along, `group` bytes apart;
+// eight values along the sum are 1024 bytes, 16 are 2048.
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr, bool mn, uint32_t group) {
+  return sdesc(addr, mn ? group : 16u, 1024u) | ((uint64_t)2u << 61);
+}
+
+struct Work {
+  int tm, tn, kb0, kb1, split;
+};
+__device__ __forceinline__ Work work_of(const GemmParams& p, int i) {
+  Work w;
+  const int tiles = p.tiles_m * p.tiles_n;
+  w.split = i / tiles;
+  const int t = i - w.split * tiles;
+  // bands of 16 tiles down the rows: the CTAs at work at a time share both operands in L2
+  const int band = t / (16 * p.tiles_n), first = band * 16, high = min(16, p.tiles_m - first);
+  const int in = t - band * 16 * p.tiles_n;
+  w.tm = first + in % high;
+  w.tn = in / high;
+  w.kb0 = w.split * p.per_split;
+  w.kb1 = min(p.kblocks, w.kb0 + p.per_split);
+  return w;
+}
+
+template <int CG, int P>
+__global__ void __launch_bounds__(kGemmThreads) linear_gemm_kernel(const __grid_constant__ CUtensorMap map_a,
+                                                                   const __grid_constant__ CUtensorMap map_b,
+                                                                   const __grid_constant__ GemmParams p) {
+  using G = Gemm<CG, P>;
+  extern __shared__ uint8_t raw[];
+  uint8_t* stages = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+  float* staging = reinterpret_cast<float*>(stages + (size_t)G::kStages * G::kStage);
+  uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(staging) + kStagingBytes);
+  uint64_t* empty = full + G::kStages;
+  uint64_t* acc_full = empty + G::kStages;
+  uint64_t* acc_empty = acc_full + 2;
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  volatile int* dead = reinterpret_cast<volatile int*>(tmem_at + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = CG == 2 ? blockIdx.x & 1 : 0;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < G::kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], kEpiWarps * CG);
+    }
+    *dead = 0;
+    fence_mbar_init();
+  }
+  if (warp == kEpiWarps + 1) {
+    if constexpr (CG == 2) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_at)),
+                   "r"(G::kTmem) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      tmem_alloc(tmem_at, G::kTmem);
+      tmem_relinquish();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) cg::this_cluster().sync();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_at;
+  const int items = p.tiles_m * p.tiles_n * p.splits, stride = gridDim.x / CG;
+  const uint32_t group = P * 8192;      // 64 values across the sum of all terms, contiguous across
+
+  if (warp == kEpiWarps) {
+    if (lane == 0) {  // copies
+      uint32_t stage = 0, phase = 0;
+      bool fine = true;
+      for (int it = blockIdx.x / CG; it < items && fine; it += stride) {
+        const Work w = work_of(p, it);
+        const int m0 = w.tm * G::kTileM + rank * 128, n0 = w.tn * G::kTileN + rank * 128;
+        for (int kb = w.kb0; kb < w.kb1; ++kb) {
+          if (!(fine = bounded_wait(&empty[stage], phase ^ 1u, dead, p.flags))) break;
+          const uint32_t bar = CG == 2 ? leader_addr(&full[stage]) : smem_u32(&full[stage]);
+          if (rank == 0) mbar_arrive_expect_tx(&full[stage], G::kStage * CG);
+          const uint32_t a = smem_u32(stages + (size_t)stage * G::kStage), b = a + P * G::kOperand;
+          const int k0 = kb * kBK;
+          if (p.a_mn) {
+            tile_load<CG>(a, &map_a, m0, k0, bar);
+            tile_load<CG>(a + group, &map_a, m0 + 64, k0, bar);
+          } else {
+            tile_load<CG>(a, &map_a, k0, m0, bar);
+          }
+          if (p.b_mn) {
+            tile_load<CG>(b, &map_b, n0, k0, bar);
+            tile_load<CG>(b + group, &map_b, n0 + 64, k0, bar);
+          } else {
+            tile_load<CG>(b, &map_b, k0, n0, bar);
+          }
+          if (++stage == G::kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      // No copy is in flight when the CTA ends: every stage was consumed, or a wait ran out, and then what was
+      // issued is given its time.
+      for (int i = 0; i < G::kStages && fine; ++i) {
+        fine = bounded_wait(&empty[stage], phase ^ 1u, dead, p.flags);
+        if (++stage == G::kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (!fine) {
+        const long long t0 = clock64();
+        while (clock64() - t0 < 20 * 1000 * 1000) __nanosleep(1000);
+      }
+    }
+  } else if (warp == kEpiWarps + 1) {
+    if (lane == 0 && rank == 0) {  // products
+      const uint32_t id = (idesc(kBF16, G::kTileN, p.a_mn, p.b_mn, false) & ~(31u << 24)) | (uint32_t)(G::kTileM >> 4) << 24;
+      const uint32_t step_a = (p.a_mn ? 2048u : 32u) >> 4, step_b = (p.b_mn ? 2048u : 32u) >> 4;
+      const uint32_t term_a = (p.a_mn ? 8192u : (uint32_t)G::kOperand) >> 4, term_b = (p.b_mn ? 8192u : (uint32_t)G::kOperand) >> 4;
+      uint32_t stage = 0, phase = 0, acc = 0, acc_phase = 0;
+      bool fine = true;
+      for (int it = blockIdx.x / CG; it < items && fine; it += stride) {
+        const Work w = work_of(p, it);
+        for (int kb = w.kb0; kb < w.kb1 && fine; ++kb) {
+          const bool first = P == 3 || kb == w.kb0;      // of an accumulator's turn
+          if (first && !(fine = bounded_wait(&acc_empty[acc], acc_phase ^ 1u, dead, p.flags))) break;
+          if (!(fine = bounded_wait(&full[stage], phase, dead, p.flags))) break;
+          tc_fence_after();
+          const uint32_t d = tmem + acc * G::kTileN;
+          const uint32_t sa = smem_u32(stages + (size_t)stage * G::kStage);
+          const uint64_t a = operand_desc(sa, p.a_mn, group), b = operand_desc(sa + P * G::kOperand, p.b_mn, group);
+          uint32_t add = first ? 0u : 1u;
+          if constexpr (P == 3) {
+            constexpr int kA[6] = {2, 1, 0, 1, 0, 0}, kB[6] = {0, 1, 2, 0, 1, 0};  // terms, small products first
+#pragma unroll
+            for (int c = 0; c < 6; ++c)
+#pragma unroll
+              for (int s = 0; s < kBK / 16; ++s) {
+                mma_bf16<CG>(d, a + kA[c] * term_a + s * step_a, b + kB[c] * term_b + s * step_b, id, add);
+                add = 1u;
+              }
+          } else {
+#pragma unroll
+            for (int s = 0; s < kBK / 16; ++s) {
+              mma_bf16<CG>(d, a + s * step_a, b + s * step_b, id, add);
+              add = 1u;
+            }
+          }
+          commit<CG>(&empty[stage]);
+          if (++stage == G::kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+          if (P == 3 || kb == w.kb1 - 1) {
+            commit<CG>(&acc_full[acc]);
+            acc ^= 1u;
+            if (!acc) acc_phase ^= 1u;
+          }
+        }
+      }
+    }
+  } else {  // epilogue: warp w has rows 32 (w % 4).. and half w / 4 of the columns
+    constexpr int kHalf = G::kTileN / 2;
+    float* mine = staging + warp * 32 * 33;
+    const uint32_t col0 = (warp >> 2) * kHalf;
+    uint32_t acc = 0, acc_phase = 0;
+    auto release = [&] {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (CG == 2)
+          asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_addr(&acc_empty[acc]))
+                       : "memory");
+        else
+          asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&acc_empty[acc])) : "memory");
+      }
+      acc ^= 1u;
+      if (!acc) acc_phase ^= 1u;
+    };
+    for (int it = blockIdx.x / CG; it < items; it += stride) {
+      const Work w = work_of(p, it);
+      const long long row0 = (long long)w.tm * G::kTileM + rank * 128 + (warp & 3) * 32;
+      const long long out0 = (long long)w.tn * G::kTileN + col0;
+      // 32 rows x 32 columns at a time: from rows to lanes through shared memory, so that a warp reads and
+      // writes 32 neighbouring columns of a row
+      auto put = [&](const float* v, int c) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) mine[lane * 33 + j] = v[j];
+        __syncwarp();
+        const long long col = out0 + c + lane;
+        if (col < p.cols) {
+          const int n = (int)max(0ll, min(32ll, p.rows - row0));
+          if (p.ep.parts) {
+            float* q = p.ep.parts + ((long long)w.split * p.rows + row0) * p.cols + col;
+            for (int i = 0; i < n; ++i) q[(long long)i * p.cols] = mine[i * 33 + lane];
+          } else {
+            const float bias = p.ep.bias ? load_f(p.ep.bias, col, p.ep.bias_bf16) : 0.f;
+            for (int i = 0; i < n; ++i) finish(p.ep, row0 + i, col, mine[i * 33 + lane], p.k, bias);
+          }
+        }
+        __syncwarp();
+      };
+      if constexpr (P == 3) {
+        float sum[kHalf];
+#pragma unroll
+        for (int j = 0; j < kHalf; ++j) sum[j] = 0.f;
+        for (int kb = w.kb0; kb < w.kb1; ++kb) {
+          bounded_wait(&acc_full[acc], acc_phase, dead, p.flags);
+          __syncwarp();
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < kHalf; c += 32) {
+            float v[32];
+            tmem_ld32(tmem + acc * G::kTileN, col0 + c, v);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) sum[c + j] += v[j];
+          }
+          release();
+        }
+#pragma unroll
+        for (int c = 0; c < kHalf; c += 32) put(sum + c, c);
+      } else {
+        bounded_wait(&acc_full[acc], acc_phase, dead, p.flags);
+        __syncwarp();
+        tc_fence_after();
+        for (int c = 0; c < kHalf; c += 32) {
+          float v[32];
+          tmem_ld32(tmem + acc * G::kTileN, col0 + c, v);
+          if (c + 32 == kHalf) release();
+          put(v, c);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) cg::this_cluster().sync();  // the pair's products and arrivals are over
+  tc_fence_after();
+  if (warp == kEpiWarps + 1) {
+    if constexpr (CG == 2)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(G::kTmem) : "memory");
+    else
+      tmem_dealloc(tmem, G::kTmem);
+  }
+}
+
+// Adds the parts of a split sum in their order and finishes.
+__global__ void __launch_bounds__(256) linear_join_kernel(const float* parts, int splits, int rows, int cols, int k,
+                                                          const __grid_constant__ Epilogue e) {
+  const long long n = (long long)rows * cols;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+    float v = parts[i];
+    for (int s = 1; s < splits; ++s) v += parts[s * n + i];
+    const long long row = i / cols, col = i - row * cols;
+    finish(e, row, col, v, k, e.bias ? load_f(e.bias, col, e.bias_bf16) : 0.f);
+  }
+}
+
+// ---- operands in the form that the copies need --------------------------------------------------
+// rows x cols of T with rows `ld` apart -> terms of bf16, rows `ldt` apart, terms rows * ldt apart: an fp32 matrix
+// in three terms, or a bf16 matrix whose rows are not on 16 bytes as it is.
+template <class T>
+__global__ void __launch_bounds__(256) linear_terms_kernel(const T* x, long long ld, int rows, int cols,
+                                                           __nv_bfloat16* out, long long ldt) {
+  const int per = (int)(ldt / 2);
+  const long long n = (long long)rows * per, term = rows * ldt;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+    const long long r = i / per;
+    const int c = (int)(i - r * per) * 2;
+    float v[2];
+    for (int j = 0; j < 2; ++j) v[j] = c + j < cols ? to_f<T>(x[r * ld + c + j]) : 0.f;
+    __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(out + r * ldt + c);
+    if constexpr (sizeof(T) == 2) {
+      *o = __floats2bfloat162_rn(v[0], v[1]);
+    } else {
+#pragma unroll
+      for (int t = 0; t < 3; ++t) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[0], v[1]);
+        o[t * (term / 2)] = h;
+        v[0] -= __low2float(h);
+        v[1] -= __high2float(h);
+      }
+    }
+  }
+}
+
+// dz = dy act'(z) (or dy) in the same form, and db's parts: a CTA takes 64 columns of `band` rows.
+template <class T, bool ACT>
+__global__ void __launch_bounds__(256) linear_dz_kernel(const T* dy, long long ld, const T* z, int rows, int cols, int band,
+                                                        int col_blocks, __nv_bfloat16* out, long long ldt, float* out32,
+                                                        float* parts) {
+  __shared__ float sums[8][64];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int in_band = blockIdx.x / col_blocks, c0 = (blockIdx.x - in_band * col_blocks) * 64, c = c0 + lane * 2;
+  const long long r0 = (long long)in_band * band, r1 = min((long long)rows, r0 + band), term = rows * ldt;
+  float s[2] = {0.f, 0.f};
+  for (long long r = r0 + warp; r < r1; r += 8) {
+    float v[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      v[j] = 0.f;
+      if (c + j < cols) {
+        v[j] = to_f<T>(dy[r * ld + c + j]);
+        if constexpr (ACT) v[j] *= gelu_slope(to_f<T>(z[r * cols + c + j]));
+        s[j] += v[j];
+        if (out32) out32[r * cols + c + j] = v[j];
+      }
+    }
+    if (out && c < ldt) {
+      __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(out + r * ldt + c);
+#pragma unroll
+      for (int t = 0; t < (sizeof(T) == 2 ? 1 : 3); ++t) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[0], v[1]);
+        o[t * (term / 2)] = h;
+        v[0] -= __low2float(h);
+        v[1] -= __high2float(h);
+      }
+    }
+  }
+  if (!parts) return;
+  sums[warp][lane * 2] = s[0];
+  sums[warp][lane * 2 + 1] = s[1];
+  __syncthreads();
+  if (threadIdx.x < 64 && c0 + (int)threadIdx.x < cols) {
+    float t = 0.f;
+    for (int i = 0; i < 8; ++i) t += sums[i][threadIdx.x];
+    parts[(long long)in_band * cols + c0 + threadIdx.x] = t;
+  }
+}
+__global__ void __launch_bounds__(256) linear_db_kernel(const float* parts, int bands, int cols, void* db, int bf16) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= cols) return;
+  float s = 0.f;
+  for (int i = 0; i < bands; ++i) s += parts[(long long)i * cols + c];
+  store_f(db, c, bf16, s);
+}
+
+// ---- few rows -----------------------------------------------------------------------------------
+// Up to 16 rows of x: W is read once, straight into fp32 products.  A CTA takes 32 V columns and a stretch of
+// the sum, its eight warps and the CTAs of a cluster shares of it; their parts meet in shared memory.
+constexpr int kFewRows = 16, kFewStretch = 512;
+
+struct FewParams {
+  Epilogue ep;
+  const void *x, *w;
+  long long ldx, ldw;
+  int rows, cols, k, clusters;
+};
+template <class T, int V>
+__device__ __forceinline__ void load_w(const T* p, float v[V], bool whole, int left) {
+  if (whole) {
+    if constexpr (V == 4) {
+      ld4(p, v);
+    } else if constexpr (V == 2 && sizeof(T) == 4) {
+      const float2 f = __ldg(reinterpret_cast<const float2*>(p));
+      v[0] = f.x; v[1] = f.y;
+    } else if constexpr (V == 2) {
+      const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p));
+      v[0] = f.x; v[1] = f.y;
+    } else {
+      v[0] = ld1(p);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = j < left ? ld1(p + j) : 0.f;
+  }
+}
+template <class T, int V, int R>
+__global__ void __launch_bounds__(256) linear_few_kernel(const __grid_constant__ FewParams p) {
+  __shared__ float xs[R][kFewStretch];
+  __shared__ float part[8][R][32 * V];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rank = blockIdx.x % p.clusters, c = (blockIdx.x / p.clusters * 32 + lane) * V;
+  const int share = (p.k + p.clusters - 1) / p.clusters, k0 = rank * share, k1 = min(p.k, k0 + share);
+  const T* w = static_cast<const T*>(p.w) + c;
+  const T* x = static_cast<const T*>(p.x);
+  const int left = p.cols - c;
+  const bool whole = left >= V && (V == 1 || (p.ldw % V == 0 && (reinterpret_cast<uintptr_t>(p.w) % (V * sizeof(T))) == 0));
+  float acc[R][V];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int j = 0; j < V; ++j) acc[r][j] = 0.f;
+  for (int s = k0; s < k1; s += kFewStretch) {
+    const int n = min(kFewStretch, k1 - s);
+    __syncthreads();
+    for (int i = threadIdx.x; i < R * n; i += 256) {
+      const int r = i / n, j = i - r * n;
+      xs[r][j] = r < p.rows ? to_f<T>(x[r * p.ldx + s + j]) : 0.f;
+    }
+    __syncthreads();
+    if (left > 0) {
+#pragma unroll 8
+      for (int j = warp; j < n; j += 8) {
+        float v[V];
+        load_w<T, V>(w + (long long)(s + j) * p.ldw, v, whole, left);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int i = 0; i < V; ++i) acc[r][i] = fmaf(xs[r][j], v[i], acc[r][i]);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int i = 0; i < V; ++i) part[warp][r][lane * V + i] = acc[r][i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < R * 32 * V; i += 256) {
+    const int r = i / (32 * V), j = i % (32 * V);
+    float s = 0.f;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) s += part[u][r][j];
+    part[0][r][j] = s;
+  }
+  if (p.clusters > 1) cg::this_cluster().sync();
+  else __syncthreads();
+  for (int i = threadIdx.x + rank * 256; i < p.rows * 32 * V; i += 256 * p.clusters) {
+    const int r = i / (32 * V), j = i % (32 * V), col = blockIdx.x / p.clusters * 32 * V + j;
+    if (col >= p.cols) continue;
+    float s = part[0][r][j];
+    if (p.clusters > 1) {
+      s = 0.f;
+      for (int u = 0; u < p.clusters; ++u) s += cg::this_cluster().map_shared_rank(&part[0][r][j], u)[0];
+    }
+    finish(p.ep, r, col, s, p.k, p.ep.bias ? load_f(p.ep.bias, col, p.ep.bias_bf16) : 0.f);
+  }
+  if (p.clusters > 1) cg::this_cluster().sync();  // a CTA's parts are read until here
+}
+
+// ---- host ---------------------------------------------------------------------------------------
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encoder() {
+  static const EncodeFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &r) != cudaSuccess ||
+        r != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<EncodeFn>(f);
+  }();
+  return fn;
+}
+
+// A bf16 matrix (terms of it `term` elements apart), outer x inner, rows `ld` elements apart.
+struct Operand {
+  const void* p;
+  long long outer, inner, ld, term;
+  bool mn;                              // the summed dimension is the outer one
+};
+bool make_map(CUtensorMap* m, const Operand& o, int terms) {
+  const EncodeFn fn = encoder();
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)o.inner, (cuuint64_t)o.outer, (cuuint64_t)terms};
+  const cuuint64_t strides[2] = {(cuuint64_t)o.ld * 2, (cuuint64_t)(terms > 1 ? o.term : o.ld * o.outer) * 2};
+  const cuuint32_t box[3] = {64, o.mn ? 64u : 128u, (cuuint32_t)terms}, unit[3] = {1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(o.p), dims, strides, box, unit,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+constexpr int kSMs = 148;
+struct GemmPlan {
+  int cg, tiles_m, tiles_n, kblocks, splits, per_split;
+};
+GemmPlan plan_gemm(long long rows, long long cols, long long k) {
+  GemmPlan g{};
+  g.kblocks = (int)((k + kBK - 1) / kBK);
+  auto tiles = [&](int t) { return ((rows + t - 1) / t) * ((cols + t - 1) / t); };
+  g.cg = tiles(256) >= 37 ? 2 : 1;
+  const int t = 128 * g.cg, workers = kSMs / g.cg;
+  g.tiles_m = (int)((rows + t - 1) / t);
+  g.tiles_n = (int)((cols + t - 1) / t);
+  const long long n = (long long)g.tiles_m * g.tiles_n;
+  g.splits = 1;
+  if (2 * n <= workers) {
+    long long s = workers / n;
+    if (s > g.kblocks / 4) s = g.kblocks / 4;
+    if (s > 16) s = 16;
+    if (s > 1) g.splits = (int)s;
+  }
+  g.per_split = (g.kblocks + g.splits - 1) / g.splits;
+  g.splits = (g.kblocks + g.per_split - 1) / g.per_split;
+  return g;
+}
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+size_t parts_of(const GemmPlan& g, long long rows, long long cols) {
+  return g.splits > 1 ? round256((size_t)g.splits * rows * cols * sizeof(float)) : 0;
+}
+
+template <int CG, int P>
+cudaError_t launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p, cudaStream_t st) {
+  using G = Gemm<CG, P>;
+  static unsigned long long done = 0;
+  cudaError_t e = smem_attr_once(linear_gemm_kernel<CG, P>, (int)G::kSmem, done);
+  if (e != cudaSuccess) return e;
+  const int items = p.tiles_m * p.tiles_n * p.splits, workers = kSMs / CG;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((items < workers ? items : workers) * CG));
+  cfg.blockDim = dim3(kGemmThreads);
+  cfg.dynamicSmemBytes = G::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = CG;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, linear_gemm_kernel<CG, P>, a, b, p);
+}
+
+// One product; `parts` has parts_of() bytes.
+cudaError_t gemm(const Operand& a, const Operand& b, int terms, Epilogue ep, long long rows, long long cols, long long k,
+                 float* parts, uint32_t* flags, cudaStream_t st) {
+  const GemmPlan g = plan_gemm(rows, cols, k);
+  CUtensorMap ma, mb;
+  if (!make_map(&ma, a, terms) || !make_map(&mb, b, terms)) return cudaErrorInvalidValue;
+  GemmParams p{};
+  p.ep = ep;
+  p.rows = (int)rows; p.cols = (int)cols; p.k = (int)k;
+  p.tiles_m = g.tiles_m; p.tiles_n = g.tiles_n; p.splits = g.splits; p.kblocks = g.kblocks; p.per_split = g.per_split;
+  p.a_mn = a.mn; p.b_mn = b.mn;
+  p.flags = flags;
+  p.ep.parts = g.splits > 1 ? parts : nullptr;
+  cudaError_t e = g.cg == 2 ? (terms == 3 ? launch_gemm<2, 3>(ma, mb, p, st) : launch_gemm<2, 1>(ma, mb, p, st))
+                            : (terms == 3 ? launch_gemm<1, 3>(ma, mb, p, st) : launch_gemm<1, 1>(ma, mb, p, st));
+  if (e != cudaSuccess || g.splits == 1) return e;
+  const long long n = rows * cols, want = (n + 255) / 256;
+  linear_join_kernel<<<(unsigned)(want < kSMs * 16 ? want : kSMs * 16), 256, 0, st>>>(parts, g.splits, p.rows, p.cols, p.k, ep);
+  return cudaGetLastError();
+}
+
+// Where an operand's terms go, and whether it needs them at all.
+bool direct(const gdn2_linear_desc* d, const void* p, long long ld) {
+  return d->dtype == GDN2_BF16 && ld % 8 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+}
+long long padded(long long n) { return (n + 7) / 8 * 8; }
+size_t terms_bytes(const gdn2_linear_desc* d, long long rows, long long cols) {
+  return round256((size_t)rows * padded(cols) * 2 * (d->dtype == GDN2_F32 ? 3 : 1));
+}
+cudaError_t make_terms(const gdn2_linear_desc* d, const void* p, long long ld, long long rows, long long cols, void* to,
+                       cudaStream_t st) {
+  const long long ldt = padded(cols), want = (rows * (ldt / 2) + 255) / 256;
+  const unsigned grid = (unsigned)(want < kSMs * 16 ? want : kSMs * 16);
+  __nv_bfloat16* o = static_cast<__nv_bfloat16*>(to);
+  if (d->dtype == GDN2_F32) linear_terms_kernel<float><<<grid, 256, 0, st>>>(static_cast<const float*>(p), ld, (int)rows, (int)cols, o, ldt);
+  else linear_terms_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(p), ld, (int)rows, (int)cols, o, ldt);
+  return cudaGetLastError();
+}
+
+gdn2_status check_linear(const gdn2_linear_desc* d) {
+  if (!d || d->M < 0 || d->K < 1 || d->N < 1) return GDN2_ERR_INVALID_ARGUMENT;
+  if ((d->dtype != GDN2_F32 && d->dtype != GDN2_BF16) || (d->bias_dtype != GDN2_F32 && d->bias_dtype != GDN2_BF16))
+    return GDN2_ERR_INVALID_ARGUMENT;
+  if (d->act != GDN2_ACT_NONE && d->act != GDN2_ACT_GELU_TANH) return GDN2_ERR_INVALID_ARGUMENT;
+  if (d->x_stride < d->K || d->w_stride < d->N || d->res_stride < 0) return GDN2_ERR_INVALID_ARGUMENT;
+  if (d->M > 1 << 28 || d->K > 1 << 28 || d->N > 1 << 28) return GDN2_ERR_UNSUPPORTED;
+  const long long most = 1ll << 36;     // strides and terms of a tensor map stay below 2^40 bytes
+  if (d->x_stride > 1ll << 28 || d->w_stride > 1ll << 28 || (long long)d->M * d->N > most ||
+      (long long)d->M * d->x_stride > most || (long long)d->K * d->w_stride > most)
+    return GDN2_ERR_UNSUPPORTED;
+  return GDN2_OK;
+}
+bool off(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n != 0; }
+size_t element(const gdn2_linear_desc* d) { return d->dtype == GDN2_BF16 ? 2 : 4; }
+
+struct FwdPlan {
+  bool few, x_terms, w_terms;
+  size_t x_at, w_at, parts_at, total;
+};
+FwdPlan plan_fwd(const gdn2_linear_desc* d, bool x_direct, bool w_direct) {
+  FwdPlan f{};
+  f.few = d->M <= kFewRows;
+  if (f.few) return f;
+  f.x_terms = !x_direct;
+  f.w_terms = !w_direct;
+  f.w_at = f.x_terms ? terms_bytes(d, d->M, d->K) : 0;
+  f.parts_at = f.w_at + (f.w_terms ? terms_bytes(d, d->K, d->N) : 0);
+  f.total = f.parts_at + parts_of(plan_gemm(d->M, d->N, d->K), d->M, d->N);
+  return f;
+}
+
+constexpr int kBand = 256;              // rows of a CTA of the dz kernel
+struct BwdPlan {
+  bool dz, x_terms, w_terms;            // dz: its own buffer (an activation, fp32, or rows not on 16 bytes)
+  size_t dz_at, dz32_at, w_at, x_at, db_at, parts_at, total;
+};
+BwdPlan plan_bwd(const gdn2_linear_desc* d, bool dx, bool dw, bool db, bool x_direct, bool w_direct, bool dy_direct) {
+  BwdPlan b{};
+  size_t at = 0;
+  auto take = [&](size_t n) { const size_t r = at; at += round256(n); return r; };
+  b.dz = (dx || dw) && (!dy_direct || d->act != GDN2_ACT_NONE);
+  if (b.dz) b.dz_at = take(terms_bytes(d, d->M, d->N));
+  // dz itself, for sums that are NaN
+  if (b.dz && d->dtype == GDN2_F32 && d->act != GDN2_ACT_NONE) b.dz32_at = take((size_t)d->M * d->N * 4);
+  b.w_terms = dx && !w_direct;
+  b.x_terms = dw && !x_direct;
+  if (b.w_terms) b.w_at = take(terms_bytes(d, d->K, d->N));
+  if (b.x_terms) b.x_at = take(terms_bytes(d, d->M, d->K));
+  if (db) b.db_at = take((size_t)((d->M + kBand - 1) / kBand) * d->N * 4);
+  b.parts_at = at;
+  size_t parts = 0;
+  if (dx) parts = parts_of(plan_gemm(d->M, d->K, d->N), d->M, d->K);
+  if (dw) {
+    const size_t q = parts_of(plan_gemm(d->K, d->N, d->M), d->K, d->N);
+    if (q > parts) parts = q;
+  }
+  b.total = at + parts;
+  return b;
+}
+
+template <class T, int V>
+cudaError_t launch_few(FewParams p, cudaStream_t st) {
+  const long long blocks = (p.cols + 32 * V - 1) / (32 * V);
+  p.clusters = 1;
+  while (p.clusters < 8 && blocks * p.clusters < 2 * kSMs && p.k / p.clusters >= 128) p.clusters *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(blocks * p.clusters));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)p.clusters;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  if (p.rows == 1) return cudaLaunchKernelEx(&cfg, linear_few_kernel<T, V, 1>, p);
+  if (p.rows <= 4) return cudaLaunchKernelEx(&cfg, linear_few_kernel<T, V, 4>, p);
+  return cudaLaunchKernelEx(&cfg, linear_few_kernel<T, V, 8>, p);
+}
+cudaError_t run_few(const gdn2_linear_desc* d, const FewParams& all, cudaStream_t st) {
+  for (int r = 0; r < d->M; r += 8) {   // eight rows a launch
+    FewParams p = all;
+    const size_t el = element(d);
+    p.rows = d->M - r < 8 ? d->M - r : 8;
+    p.x = static_cast<const uint8_t*>(p.x) + (size_t)r * p.ldx * el;
+    p.ep.y = static_cast<uint8_t*>(p.ep.y) + (size_t)r * p.ep.ldy * el;
+    if (p.ep.z) p.ep.z = static_cast<uint8_t*>(p.ep.z) + (size_t)r * p.ep.ldy * el;
+    if (p.ep.residual) p.ep.residual = static_cast<const uint8_t*>(p.ep.residual) + (size_t)r * p.ep.ldr * el;
+    const cudaError_t e = d->dtype == GDN2_F32 ? launch_few<float, 1>(p, st) : launch_few<__nv_bfloat16, 2>(p, st);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
+}  // namespace
+}  // namespace gdn2
+
+extern "C" size_t gdn2_linear_fwd_workspace_bytes(const gdn2_linear_desc* d) {
+  using namespace gdn2;
+  if (check_linear(d) != GDN2_OK || !d->M) return 0;
+  const bool bf16 = d->dtype == GDN2_BF16;
+  return plan_fwd(d, bf16 && d->x_stride % 8 == 0, bf16 && d->w_stride % 8 == 0).total;
+}
+
+extern "C" gdn2_status gdn2_linear_fwd(const gdn2_linear_desc* d, const void* x, const void* w, const void* bias,
+                                       const void* residual, void* y, void* z, void* workspace, uint32_t* flags,
+                                       void* stream) {
+  using namespace gdn2;
+  const gdn2_status s = check_linear(d);
+  if (s != GDN2_OK) return s;
+  if (!d->M) return GDN2_OK;
+  const size_t el = element(d);
+  if (!x || !w || !y || !flags || off(x, 16) || off(w, 16) || off(y, el) || off(z, el) || off(residual, el) ||
+      off(bias, d->bias_dtype == GDN2_BF16 ? 2 : 4))
+    return GDN2_ERR_INVALID_ARGUMENT;
+  const FwdPlan f = plan_fwd(d, direct(d, x, d->x_stride), direct(d, w, d->w_stride));
+  if (f.total && (!workspace || off(workspace, 256))) return GDN2_ERR_INVALID_ARGUMENT;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  Epilogue ep{};
+  ep.y = y; ep.z = z; ep.bias = bias; ep.residual = residual;
+  ep.ldr = d->res_stride; ep.ldy = d->N;
+  ep.y_bf16 = d->dtype == GDN2_BF16; ep.bias_bf16 = d->bias_dtype == GDN2_BF16; ep.act = d->act;
+  cudaError_t e = cudaSuccess;
+  if (f.few) {
+    FewParams p{};
+    p.ep = ep;
+    p.x = x; p.w = w; p.ldx = d->x_stride; p.ldw = d->w_stride; p.cols = d->N; p.k = d->K;
+    e = run_few(d, p, st);
+  } else {
+    const int terms = d->dtype == GDN2_F32 ? 3 : 1;
+    if (terms == 3) {
+      ep.a = static_cast<const float*>(x); ep.a_row = d->x_stride; ep.a_k = 1;
+      ep.b = static_cast<const float*>(w); ep.b_col = 1; ep.b_k = d->w_stride;
+    }
+    Operand a{x, d->M, d->K, d->x_stride, 0, false}, b{w, d->K, d->N, d->w_stride, 0, true};
+    if (f.x_terms) {
+      e = make_terms(d, x, d->x_stride, d->M, d->K, ws + f.x_at, st);
+      a.p = ws + f.x_at; a.ld = padded(d->K); a.term = d->M * a.ld;
+    }
+    if (f.w_terms && e == cudaSuccess) {
+      e = make_terms(d, w, d->w_stride, d->K, d->N, ws + f.w_at, st);
+      b.p = ws + f.w_at; b.ld = padded(d->N); b.term = d->K * b.ld;
+    }
+    if (e == cudaSuccess)
+      e = gemm(a, b, terms, ep, d->M, d->N, d->K, reinterpret_cast<float*>(ws + f.parts_at), flags, st);
+  }
+  return e == cudaSuccess ? GDN2_OK : GDN2_ERR_CUDA;
+}
+
+extern "C" size_t gdn2_linear_bwd_workspace_bytes(const gdn2_linear_desc* d, int32_t want) {
+  using namespace gdn2;
+  if (check_linear(d) != GDN2_OK || !d->M) return 0;
+  const bool bf16 = d->dtype == GDN2_BF16;
+  return plan_bwd(d, want & 1, want & 2, want & 4, bf16 && d->x_stride % 8 == 0, bf16 && d->w_stride % 8 == 0,
+                  bf16 && d->N % 8 == 0).total;
+}
+
+extern "C" gdn2_status gdn2_linear_bwd(const gdn2_linear_desc* d, const void* x, const void* w, const void* z,
+                                       const void* dy, void* dx, void* dw, void* db, void* workspace, uint32_t* flags,
+                                       void* stream) {
+  using namespace gdn2;
+  const gdn2_status s = check_linear(d);
+  if (s != GDN2_OK) return s;
+  const size_t el = element(d);
+  if (d->M < 1 || !dy || !flags || (dx && !w) || (dw && !x) || (d->act != GDN2_ACT_NONE && !z) || off(x, 16) || off(w, 16) ||
+      off(dy, 16) || off(z, el) || off(dx, el) || off(dw, el) || off(db, d->bias_dtype == GDN2_BF16 ? 2 : 4))
+    return GDN2_ERR_INVALID_ARGUMENT;
+  if (!dx && !dw && !db) return GDN2_OK;
+  const BwdPlan b = plan_bwd(d, dx, dw, db, direct(d, x, d->x_stride), direct(d, w, d->w_stride), direct(d, dy, d->N));
+  if (b.total && (!workspace || off(workspace, 256))) return GDN2_ERR_INVALID_ARGUMENT;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool act = d->act != GDN2_ACT_NONE, bf16 = d->dtype == GDN2_BF16;
+  const int terms = bf16 ? 1 : 3, bands = (d->M + kBand - 1) / kBand;
+  const long long ldz = padded(d->N);
+  float* dz32 = b.dz && !bf16 && act ? reinterpret_cast<float*>(ws + b.dz32_at) : nullptr;
+  cudaError_t e = cudaSuccess;
+  if (b.dz || db) {
+    const int col_blocks = (d->N + 63) / 64;
+    const unsigned grid = (unsigned)(col_blocks * (long long)bands);
+    __nv_bfloat16* out = b.dz ? reinterpret_cast<__nv_bfloat16*>(ws + b.dz_at) : nullptr;
+    float* parts = db ? reinterpret_cast<float*>(ws + b.db_at) : nullptr;
+    auto go = [&](auto kernel, auto t) {
+      using T = decltype(t);
+      kernel<<<grid, 256, 0, st>>>(static_cast<const T*>(dy), (long long)d->N, static_cast<const T*>(z), d->M, d->N, kBand,
+                                   col_blocks, out, ldz, dz32, parts);
+    };
+    if (bf16) act ? go(linear_dz_kernel<__nv_bfloat16, true>, __nv_bfloat16()) : go(linear_dz_kernel<__nv_bfloat16, false>, __nv_bfloat16());
+    else act ? go(linear_dz_kernel<float, true>, 0.f) : go(linear_dz_kernel<float, false>, 0.f);
+    e = cudaGetLastError();
+    if (db && e == cudaSuccess) {
+      linear_db_kernel<<<(d->N + 255) / 256, 256, 0, st>>>(parts, bands, d->N, db, d->bias_dtype == GDN2_BF16);
+      e = cudaGetLastError();
+    }
+  }
+  const void* pz = b.dz ? static_cast<const void*>(ws + b.dz_at) : dy;
+  const long long ldp = b.dz ? ldz : d->N, term_z = d->M * ldz;
+  const float* dz_plain = bf16 ? nullptr : act ? dz32 : static_cast<const float*>(dy);
+  float* parts = reinterpret_cast<float*>(ws + b.parts_at);
+  if (dx && e == cudaSuccess) {
+    Operand bo{w, d->K, d->N, d->w_stride, 0, false};
+    if (b.w_terms) {
+      e = make_terms(d, w, d->w_stride, d->K, d->N, ws + b.w_at, st);
+      bo.p = ws + b.w_at; bo.ld = padded(d->N); bo.term = d->K * bo.ld;
+    }
+    Epilogue ep{};
+    ep.y = dx; ep.ldy = d->K; ep.y_bf16 = bf16;
+    if (!bf16) {
+      ep.a = dz_plain; ep.a_row = d->N; ep.a_k = 1;
+      ep.b = static_cast<const float*>(w); ep.b_col = d->w_stride; ep.b_k = 1;
+    }
+    if (e == cudaSuccess) e = gemm({pz, d->M, d->N, ldp, term_z, false}, bo, terms, ep, d->M, d->K, d->N, parts, flags, st);
+  }
+  if (dw && e == cudaSuccess) {
+    Operand a{x, d->M, d->K, d->x_stride, 0, true};
+    if (b.x_terms) {
+      e = make_terms(d, x, d->x_stride, d->M, d->K, ws + b.x_at, st);
+      a.p = ws + b.x_at; a.ld = padded(d->K); a.term = d->M * a.ld;
+    }
+    Epilogue ep{};
+    ep.y = dw; ep.ldy = d->N; ep.y_bf16 = bf16;
+    if (!bf16) {
+      ep.a = static_cast<const float*>(x); ep.a_row = 1; ep.a_k = d->x_stride;
+      ep.b = dz_plain; ep.b_col = 1; ep.b_k = d->N;
+    }
+    if (e == cudaSuccess) e = gemm(a, {pz, d->M, d->N, ldp, term_z, true}, terms, ep, d->K, d->N, d->M, parts, flags, st);
+  }
+  return e == cudaSuccess ? GDN2_OK : GDN2_ERR_CUDA;
+}

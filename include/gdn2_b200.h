@@ -340,6 +340,31 @@ gdn2_status gdn2_gated_bwd(const gdn2_gated_desc* desc, const void* x, const voi
                            const uint8_t* reset, const float* marks, const void* dh, const float* dlast, void* dx,
                            void* dg, float* dh0, void* stream);
 
+/* The linear product with its epilogue, z = x W + b, y = act(z) + r, and its backward dz = dy act'(z),
+ * db = sum over rows of dz, dx = dz W^T, dW = x^T dz.  x (M, K), W (K, N), r, y, z, dy (M, N). */
+typedef struct gdn2_linear_desc {
+  int32_t M, K, N;        /* M >= 0, K and N >= 1 */
+  int32_t dtype;          /* gdn2_dtype of x, W, r, y, z and of their gradients */
+  int32_t bias_dtype;     /* gdn2_dtype of b and db */
+  int32_t act;            /* gdn2_act */
+  int64_t x_stride, w_stride, res_stride;  /* element strides between rows; y, z, dy, dx and dW are contiguous */
+} gdn2_linear_desc;
+
+/*   x, W      16-byte aligned, rows of any stride (those of bf16 that are a multiple of 8 are read in place)
+ *   bias (N), residual: NULL for none;  z: where x W + b is kept for the backward, or NULL
+ *   workspace gdn2_linear_fwd_workspace_bytes bytes, 256-byte aligned
+ *   flags     three uint32 words in device or mapped host memory: [2] becomes 1 when an on-chip wait ran out (the
+ *             results are invalid) */
+gdn2_status gdn2_linear_fwd(const gdn2_linear_desc* desc, const void* x, const void* w, const void* bias,
+                            const void* residual, void* y, void* z, void* workspace, uint32_t* flags, void* stream);
+size_t gdn2_linear_fwd_workspace_bytes(const gdn2_linear_desc* desc);
+
+/* dx, dw and db: NULL where they are not wanted (x, w need not be given then).  z is read where act is not none.
+ * x, w, dy 16-byte aligned; M >= 1.  `want`: 1 for dx + 2 for dw + 4 for db. */
+gdn2_status gdn2_linear_bwd(const gdn2_linear_desc* desc, const void* x, const void* w, const void* z, const void* dy,
+                            void* dx, void* dw, void* db, void* workspace, uint32_t* flags, void* stream);
+size_t gdn2_linear_bwd_workspace_bytes(const gdn2_linear_desc* desc, int32_t want);
+
 /* One AdamW step over many tensors, with their gradients' global norm n, clipping and a guard:
  *   g' = g clip / max(n, clip),  m = b1 m + (1 - b1) g',  v = b2 v + (1 - b2) g'^2,
  *   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps).

@@ -77,3 +77,13 @@ def adamw_ref(p, g, m, v, t, lr, wd, b1, b2, eps, coef):
     size, r = f(lr / (1 - b1 ** t)), f((1 - b2 ** t) ** 0.5)
     p = p * f(1 - lr * wd) - size * (m / (np.sqrt(v) / r + f(eps)))
     return torch.from_numpy(p), torch.from_numpy(m), torch.from_numpy(v)
+
+
+def linear_ref(x, w, b=None, act=None, residual=None):
+    """act(x W + b) + residual in 64 bits; differentiable."""
+    y = x @ w
+    if b is not None:
+        y = y + b
+    if act == "gelu":
+        y = torch.nn.functional.gelu(y, approximate="tanh")
+    return y if residual is None else y + residual
