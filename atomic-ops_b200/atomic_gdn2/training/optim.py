@@ -98,28 +98,18 @@ class AdamW(torch.optim.Optimizer):
                 loss = result
         self._check_guard()
         first = self.param_groups[0]
-        lists = [[] for _ in range(9)]
-        for group in self.param_groups:
+        for group in self.param_groups[1:]:
             if group["betas"] != first["betas"] or group["eps"] != first["eps"]:
                 raise ValueError("AdamW: betas and eps must be the same in all groups")
-            lr, wd = group["lr"], float(group["weight_decay"])
-            for p in group["params"]:
-                if p.grad is None:
-                    continue
-                if p.grad.is_sparse:
-                    raise RuntimeError("AdamW: sparse gradients are not supported")
-                st = self._ready(p)
-                row = (p, p.grad, st["exp_avg"], st["exp_avg_sq"], st.get("exp_avg_scale"), st.get("exp_avg_sq_scale"),
-                       st["step"], lr, wd)
-                for to, x in zip(lists, row):
-                    to.append(x)
-        if not lists[0]:
-            return result
-        if self.state_bits != 8:
-            lists[4], lists[5] = [], []
-        rc = _lib.binding().adamw_step(*lists, float(first["betas"][0]), float(first["betas"][1]), float(first["eps"]),
-                                       float(self.clip or 0.0), float(self.spike_factor or 0.0), self.state_bits, loss,
-                                       self._control)
+        args = (float(first["betas"][0]), float(first["betas"][1]), float(first["eps"]), float(self.clip or 0.0),
+                float(self.spike_factor or 0.0), self.state_bits, loss)
+        rc = _lib.binding().adamw_step(self.param_groups, self.state, *args, self._control)
+        if rc is None:                                       # a parameter's first step
+            for group in self.param_groups:
+                for p in group["params"]:
+                    if p.grad is not None:
+                        self._ready(p)
+            rc = _lib.binding().adamw_step(self.param_groups, self.state, *args, self._control)
         if rc:
             _lib.check(rc, "gdn2_adamw_step")
         return result

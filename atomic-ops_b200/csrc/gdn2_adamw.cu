@@ -3,9 +3,9 @@
 //   n = |g|,  g' = g clip / max(n, clip)
 //   m = b1 m + (1 - b1) g',   v = b2 v + (1 - b2) g'^2
 //   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
-// Each operation is rounded to fp32 by itself, in this order: the moments that are stored in 8 bits are codes
-// that depend on every bit, and so do not depend on how a compiler joins products and sums.  The squares of the
-// norm are summed in fp64 in a fixed order.
+// In the moments each operation is rounded to fp32 by itself, in this order, and so is the root that is stored in
+// 8 bits: codes depend on every bit, and these do not depend on how a compiler joins products and sums.  The
+// squares of the norm are summed in fp64 in a fixed order.
 //
 // Moments in 8 bits: 256 neighbouring values share a scale.  m is e4m3 of m / scale, scale = max |m| / 448.  Of v
 // the root r is stored, unsigned with four bits of exponent and four of mantissa (c 2^-18 below code 16, else
@@ -44,7 +44,7 @@ struct AdamTable {
   int count, chunks;
 };
 struct Factors {                      // of a tensor
-  float size, root, decay;
+  float size, root, decay;            // lr / (1 - b1^t), 1 / sqrt(1 - b2^t), 1 - lr wd
 };
 struct AdamControl {                  // the caller's control words
   float ema, norm, ok, coef;
@@ -52,12 +52,12 @@ struct AdamControl {                  // the caller's control words
 };
 struct AdamParams {
   AdamControl* ctl;
-  double* parts;                      // workspace: a chunk's sum of squares
+  double* parts;                      // workspace: a CTA's sum of squares
   Factors* factors;                   // workspace: a tensor's factors
   const float* loss;
   double b1, b2, log2_b1, log2_b2;
   float fb1, gb1, fb2, gb2, eps, clip, spike;
-  int norm, chunk0, all_chunks, tensor0, last, alone;
+  int norm, part0, all_parts, tensor0, alone;
 };
 
 template <int N>
@@ -71,18 +71,19 @@ __device__ __forceinline__ int find(const AdamTable<N>& t, int chunk) {
   return lo;
 }
 
-// The tensors' step counts and factors, after the guard has decided.
+// The factors of the tensors' next step, and once the guard has decided for it the step counts.
 template <int N>
-__device__ __forceinline__ void prepare(const AdamTable<N>& t, const AdamParams& a, bool ok) {
-  if (!ok) return;
+__device__ __forceinline__ void factors(const AdamTable<N>& t, const AdamParams& a) {
   for (int i = threadIdx.x; i < t.count; i += blockDim.x) {
     const AdamEntry& e = t.e[i];
-    const float n = *e.step + 1.f;
-    *e.step = n;
-    const double lr = e.lr_at ? (double)*e.lr_at : e.lr;
-    a.factors[a.tensor0 + i] = {(float)(lr / (1.0 - exp2((double)n * a.log2_b1))),
-                                (float)sqrt(1.0 - exp2((double)n * a.log2_b2)), (float)(1.0 - lr * e.wd)};
+    const double n = *e.step + 1.f, lr = e.lr_at ? (double)*e.lr_at : e.lr;
+    a.factors[a.tensor0 + i] = {(float)(lr / (1.0 - exp2(n * a.log2_b1))), (float)rsqrt(1.0 - exp2(n * a.log2_b2)),
+                                (float)(1.0 - lr * e.wd)};
   }
+}
+template <int N>
+__device__ __forceinline__ void count_up(const AdamTable<N>& t) {
+  for (int i = threadIdx.x; i < t.count; i += blockDim.x) *t.e[i].step += 1.f;
 }
 
 __device__ __forceinline__ double block_sum(double s, double* sm) {
@@ -97,7 +98,39 @@ __device__ __forceinline__ double block_sum(double s, double* sm) {
   return s;
 }
 
-// Sums of the gradients' squares, a CTA to a chunk; the last CTA adds them up and decides.
+// |x| in fp64, put together from x's bits: the conversion instruction runs at a fraction of the rate.  The bits
+// stand for |x| 2^-896 for every finite x; an infinity or a NaN becomes 2^128 or more, and the norm infinite.
+__device__ __forceinline__ double wide(float x) {
+  const uint32_t u = __float_as_uint(x) & 0x7fffffffu;
+  return __hiloint2double((int)(u >> 3), (int)(u << 29)) * 0x1p896;
+}
+template <class T>
+__device__ __forceinline__ void squares(const T* g, int n, bool vec, double q[4]) {
+  int done = 0;
+  if (vec) {
+    float v[kChunk / 4 / kAdamThreads][4];
+#pragma unroll
+    for (int i = 0; i < kChunk / 4 / kAdamThreads; ++i) {
+      const int at = 4 * (i * kAdamThreads + (int)threadIdx.x);
+      if (at + 4 <= n) ld4(g + at, v[i]);
+      else v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kChunk / 4 / kAdamThreads; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const double w = wide(v[i][j]);
+        q[j] = fma(w, w, q[j]);
+      }
+    done = n & ~3;
+  }
+  for (int i = done + threadIdx.x; i < n; i += kAdamThreads) {
+    const double v = wide(ld1(g + i));
+    q[0] = fma(v, v, q[0]);
+  }
+}
+
+// Sums of the gradients' squares; the last CTA adds the CTAs' up and decides.
 template <int N>
 __global__ void __launch_bounds__(kAdamThreads) adamw_norm_kernel(const __grid_constant__ AdamTable<N> t,
                                                                   const __grid_constant__ AdamParams a) {
@@ -105,48 +138,28 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_norm_kernel(const __grid_c
   __shared__ bool final, go;
   pdl_enter();
   double total = 0.0;
+  if (a.alone && blockIdx.x == gridDim.x - 1) factors(t, a);  // the last CTA to start has the least to add up
   if (a.norm) {
-    const AdamEntry& e = t.e[find(t, blockIdx.x)];
-    const long long at = (long long)(blockIdx.x - e.first) * kChunk;
-    const int n = (int)min((long long)kChunk, e.n - at);
-    double s = 0.0;
-    auto add = [&](float x) { s = fma((double)x, (double)x, s); };
-    if (e.bf16) {
-      const __nv_bfloat16* g = static_cast<const __nv_bfloat16*>(e.g) + at;
-      if (e.vec && n == kChunk) {
-#pragma unroll
-        for (int i = 0; i < kChunk / 4 / kAdamThreads; ++i) {
-          float v[4];
-          ld4(g + 4 * (i * kAdamThreads + threadIdx.x), v);
-          for (int j = 0; j < 4; ++j) add(v[j]);
-        }
-      } else {
-        for (int i = threadIdx.x; i < n; i += kAdamThreads) add(ld1(g + i));
-      }
-    } else {
-      const float* g = static_cast<const float*>(e.g) + at;
-      if (e.vec && n == kChunk) {
-#pragma unroll
-        for (int i = 0; i < kChunk / 4 / kAdamThreads; ++i) {
-          float v[4];
-          ld4(g + 4 * (i * kAdamThreads + threadIdx.x), v);
-          for (int j = 0; j < 4; ++j) add(v[j]);
-        }
-      } else {
-        for (int i = threadIdx.x; i < n; i += kAdamThreads) add(ld1(g + i));
-      }
+    double q[4] = {};                  // four sums: an addition waits for the one before
+    for (int chunk = blockIdx.x; chunk < t.chunks; chunk += gridDim.x) {
+      const AdamEntry& e = t.e[find(t, chunk)];
+      const long long at = (long long)(chunk - e.first) * kChunk;
+      const int n = (int)min((long long)kChunk, e.n - at);
+      if (e.bf16) squares(static_cast<const __nv_bfloat16*>(e.g) + at, n, e.vec, q);
+      else squares(static_cast<const float*>(e.g) + at, n, e.vec, q);
     }
+    double s = (q[0] + q[1]) + (q[2] + q[3]);
     s = block_sum(s, sm);
     if (threadIdx.x == 0) {
-      a.parts[a.chunk0 + blockIdx.x] = s;
+      a.parts[a.part0 + blockIdx.x] = s;
       __threadfence();
-      final = atomicAdd(&a.ctl->ticket, 1u) == (unsigned)a.all_chunks - 1u;
+      final = atomicAdd(&a.ctl->ticket, 1u) == (unsigned)a.all_parts - 1u;
     }
     __syncthreads();
     if (!final) return;
     __threadfence();
     s = 0.0;
-    for (int i = threadIdx.x; i < a.all_chunks; i += kAdamThreads) s += __ldcg(a.parts + i);
+    for (int i = threadIdx.x; i < a.all_parts; i += kAdamThreads) s += __ldcg(a.parts + i);
     total = block_sum(s, sm);
   }
   // the last CTA, or the only one
@@ -167,7 +180,7 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_norm_kernel(const __grid_c
     go = ok;
   }
   __syncthreads();
-  if (a.alone) prepare(t, a, go);
+  if (a.alone && go) count_up(t);
 }
 
 // The factors of one of several tables.
@@ -175,15 +188,26 @@ template <int N>
 __global__ void __launch_bounds__(kAdamThreads) adamw_prepare_kernel(const __grid_constant__ AdamTable<N> t,
                                                                      const __grid_constant__ AdamParams a) {
   pdl_enter();
-  prepare(t, a, a.ctl->ok != 0.f);
+  if (a.ctl->ok == 0.f) return;
+  factors(t, a);
+  __syncthreads();
+  count_up(t);
 }
 
-// One value's step, every operation rounded by itself.
-__device__ __forceinline__ float update(float p, float g, float& m, float& v, const Factors& f, const AdamParams& a) {
+// One value's moments, every operation rounded by itself.
+__device__ __forceinline__ void moments(float g, float& m, float& v, const AdamParams& a) {
   m = __fadd_rn(__fmul_rn(a.fb1, m), __fmul_rn(a.gb1, g));
   v = __fadd_rn(__fmul_rn(a.fb2, v), __fmul_rn(a.gb2, __fmul_rn(g, g)));
-  const float d = __fadd_rn(__fdiv_rn(__fsqrt_rn(v), f.root), a.eps);
-  return __fsub_rn(__fmul_rn(p, f.decay), __fmul_rn(f.size, __fdiv_rn(m, d)));
+}
+// Its step from m and the root of v.  The quotient is within 3 ulp: that is 2^-22 of a step, which is itself
+// some 2^-6 of p or less.
+__device__ __forceinline__ float stepped(float p, float m, float r, const Factors& f, const AdamParams& a) {
+  return fmaf(p, f.decay, -f.size * __fdividef(m, fmaf(r, f.root, a.eps)));
+}
+__device__ __forceinline__ float root_near(float v) {  // within an ulp
+  float r;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
 }
 
 // Loads of memory that the kernel also writes.
@@ -254,7 +278,6 @@ __device__ __forceinline__ void decode_v(uint32_t c, float scale, float v[4]) {
     v[j] = __fmul_rn(r, r);
   }
 }
-__device__ __forceinline__ float bounded(float x, float most) { return x < -most ? -most : x > most ? most : x; }
 // The scale of a warp's block from its lanes' largest magnitude, and what values are multiplied by (0: all are stored
 // as zero).  Compared as bits, so that a NaN is the largest.
 __device__ __forceinline__ float scale_of(float largest, float inverse_top, float& up) {
@@ -266,7 +289,7 @@ __device__ __forceinline__ uint32_t encode_m(const float v[4], float up) {
   uint32_t c = 0;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    const float2 f = make_float2(bounded(__fmul_rn(v[2 * j], up), 448.f), bounded(__fmul_rn(v[2 * j + 1], up), 448.f));
+    const float2 f = make_float2(__fmul_rn(v[2 * j], up), __fmul_rn(v[2 * j + 1], up));  // at most 448 and an ulp
     c |= (uint32_t)__nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3) << (16 * j);
   }
   return c;
@@ -275,7 +298,7 @@ __device__ __forceinline__ uint32_t encode_r(const float r[4], float up) {
   uint32_t c = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float x = bounded(__fmul_rn(r[j], up), 1.9375f);
+    const float x = __fmul_rn(r[j], up);  // at most 1.9375 and an ulp
     const uint32_t u = __float_as_uint(x);
     uint32_t k = x >= 0x1p-14f ? ((u + 0x3ffffu + ((u >> 19) & 1u)) >> 19) - (112u << 4) : (uint32_t)__float2int_rn(x * 0x1p18f);
     if (r[j] > 0.f && k == 0) k = 1;
@@ -287,8 +310,8 @@ __device__ __forceinline__ float magnitude(float a, float b) {  // the larger ma
   return __uint_as_float(max(__float_as_uint(a) & 0x7fffffffu, __float_as_uint(b) & 0x7fffffffu));
 }
 
-// 4 values of a thread, 8 bits: 8 of a lane, a warp to a block.
-template <class T, bool EIGHT>
+// 4 values of a thread, 8 bits: 8 of a lane, a warp to a block.  WHOLE: a full chunk, read 4 values at a time.
+template <class T, bool EIGHT, bool WHOLE>
 __device__ __forceinline__ void chunk_update(const AdamEntry& e, const AdamParams& a, const Factors& f, float coef,
                                              long long at, int n) {
   T* p = static_cast<T*>(e.p) + at;
@@ -296,19 +319,30 @@ __device__ __forceinline__ void chunk_update(const AdamEntry& e, const AdamParam
   if constexpr (!EIGHT) {
     float* m = static_cast<float*>(e.m) + at;
     float* v = static_cast<float*>(e.v) + at;
-#pragma unroll 2
-    for (int i = threadIdx.x * 4; i < n; i += kAdamThreads * 4) {
-      const bool vec = e.vec && i + 4 <= n;
-      float x[4], y[4], mm[4], vv[4];
-      load4(p + i, x, vec, n - i);
-      load4(g + i, y, vec, n - i);
-      load4(m + i, mm, vec, n - i);
-      load4(v + i, vv, vec, n - i);
+    for (int i0 = threadIdx.x * 4; i0 < n; i0 += kAdamThreads * 8) {  // two at a time: their loads come first
+      float x[2][4], y[2][4], mm[2][4], vv[2][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = update(x[j], __fmul_rn(y[j], coef), mm[j], vv[j], f, a);
-      store4(p + i, x, vec, n - i);
-      store4(m + i, mm, vec, n - i);
-      store4(v + i, vv, vec, n - i);
+      for (int h = 0; h < 2; ++h) {
+        const int i = i0 + h * kAdamThreads * 4;
+        const bool vec = WHOLE || (e.vec && i + 4 <= n);
+        load4(p + i, x[h], vec, n - i);
+        load4(g + i, y[h], vec, n - i);
+        load4(m + i, mm[h], vec, n - i);
+        load4(v + i, vv[h], vec, n - i);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int i = i0 + h * kAdamThreads * 4;
+        const bool vec = WHOLE || (e.vec && i + 4 <= n);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          moments(__fmul_rn(y[h][j], coef), mm[h][j], vv[h][j], a);
+          x[h][j] = stepped(x[h][j], mm[h][j], root_near(vv[h][j]), f, a);
+        }
+        store4(p + i, x[h], vec, n - i);
+        store4(m + i, mm[h], vec, n - i);
+        store4(v + i, vv[h], vec, n - i);
+      }
     }
   } else {
     uint8_t* m = static_cast<uint8_t*>(e.m) + at;
@@ -318,36 +352,40 @@ __device__ __forceinline__ void chunk_update(const AdamEntry& e, const AdamParam
       const long long s = at / kBlock + blk;
       const float ms = e.ms[s], vs = e.vs[s];
       float x[2][4], y[2][4], mm[2][4], vv[2][4], r[2][4], top_m = 0.f, top_r = 0.f;
-      int left[2];
-      bool vec[2];
+      uint32_t cm[2], cv[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int i = blk * kBlock + h * 128 + lane * 4;
-        left[h] = n - i;
-        vec[h] = e.vec && left[h] >= 4;
-        load4(p + i, x[h], vec[h], left[h]);
-        load4(g + i, y[h], vec[h], left[h]);
-        decode_m(codes4(m + i, vec[h], left[h]), ms, mm[h]);
-        decode_v(codes4(v + i, vec[h], left[h]), vs, vv[h]);
+        const bool vec = WHOLE || (e.vec && n - i >= 4);
+        load4(p + i, x[h], vec, n - i);
+        load4(g + i, y[h], vec, n - i);
+        cm[h] = codes4(m + i, vec, n - i);
+        cv[h] = codes4(v + i, vec, n - i);
       }
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h) {
+        const int left = n - (blk * kBlock + h * 128 + lane * 4);
+        decode_m(cm[h], ms, mm[h]);
+        decode_v(cv[h], vs, vv[h]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          x[h][j] = update(x[h][j], __fmul_rn(y[h][j], coef), mm[h][j], vv[h][j], f, a);
-          if (j >= left[h]) mm[h][j] = vv[h][j] = 0.f;  // past the tensor's end
+          moments(__fmul_rn(y[h][j], coef), mm[h][j], vv[h][j], a);
+          if (!WHOLE && j >= left) mm[h][j] = vv[h][j] = 0.f;  // past the tensor's end
           r[h][j] = __fsqrt_rn(vv[h][j]);
+          x[h][j] = stepped(x[h][j], mm[h][j], r[h][j], f, a);
           top_m = magnitude(top_m, mm[h][j]);
           top_r = magnitude(top_r, r[h][j]);
         }
+      }
       float up_m, up_r;
       const float new_ms = scale_of(top_m, 1.f / 448.f, up_m), new_vs = scale_of(top_r, 1.f / 1.9375f, up_r);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int i = blk * kBlock + h * 128 + lane * 4;
-        store4(p + i, x[h], vec[h], left[h]);
-        codes4(m + i, encode_m(mm[h], up_m), vec[h], left[h]);
-        codes4(v + i, encode_r(r[h], up_r), vec[h], left[h]);
+        const bool vec = WHOLE || (e.vec && n - i >= 4);
+        store4(p + i, x[h], vec, n - i);
+        codes4(m + i, encode_m(mm[h], up_m), vec, n - i);
+        codes4(v + i, encode_r(r[h], up_r), vec, n - i);
       }
       if (lane == 0) {
         e.ms[s] = new_ms;
@@ -358,7 +396,7 @@ __device__ __forceinline__ void chunk_update(const AdamEntry& e, const AdamParam
 }
 
 template <int N, bool EIGHT>
-__global__ void __launch_bounds__(kAdamThreads) adamw_update_kernel(const __grid_constant__ AdamTable<N> t,
+__global__ void __launch_bounds__(kAdamThreads, 4) adamw_update_kernel(const __grid_constant__ AdamTable<N> t,
                                                                     const __grid_constant__ AdamParams a) {
   pdl_enter();
   if (__ldcg(&a.ctl->ok) == 0.f) return;
@@ -370,8 +408,12 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_update_kernel(const __grid
     const Factors f = {__ldcg(&from.size), __ldcg(&from.root), __ldcg(&from.decay)};
     const long long at = (long long)(chunk - e.first) * kChunk;
     const int n = (int)min((long long)kChunk, e.n - at);
-    if (e.bf16) chunk_update<__nv_bfloat16, EIGHT>(e, a, f, coef, at, n);
-    else chunk_update<float, EIGHT>(e, a, f, coef, at, n);
+    const bool whole = e.vec && n == kChunk;
+    if (e.bf16)
+      whole ? chunk_update<__nv_bfloat16, EIGHT, true>(e, a, f, coef, at, kChunk)
+            : chunk_update<__nv_bfloat16, EIGHT, false>(e, a, f, coef, at, n);
+    else
+      whole ? chunk_update<float, EIGHT, true>(e, a, f, coef, at, kChunk) : chunk_update<float, EIGHT, false>(e, a, f, coef, at, n);
   }
 }
 
@@ -386,14 +428,26 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_moments_kernel(const __gri
     const uint8_t* v = static_cast<const uint8_t*>(e.v) + at;
     float* om = static_cast<float*>(e.p) + at;
     float* ov = static_cast<float*>(const_cast<void*>(e.g)) + at;
+    const int lane = threadIdx.x & 31;
 #pragma unroll 2
-    for (int i = threadIdx.x * 4; i < n; i += kAdamThreads * 4) {
-      const bool vec = e.vec && i + 4 <= n;
-      float x[4];
-      decode_m(codes4(m + i, vec, n - i), e.ms[(at + i) / kBlock], x);
-      store4(om + i, x, vec, n - i);
-      decode_v(codes4(v + i, vec, n - i), e.vs[(at + i) / kBlock], x);
-      store4(ov + i, x, vec, n - i);
+    for (int blk = threadIdx.x >> 5; blk * kBlock < n; blk += kAdamThreads / 32) {
+      const float ms = e.ms[at / kBlock + blk], vs = e.vs[at / kBlock + blk];
+      uint32_t cm[2], cv[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int i = blk * kBlock + h * 128 + lane * 4;
+        cm[h] = codes4(m + i, e.vec && n - i >= 4, n - i);
+        cv[h] = codes4(v + i, e.vec && n - i >= 4, n - i);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int i = blk * kBlock + h * 128 + lane * 4;
+        float x[4];
+        decode_m(cm[h], ms, x);
+        store4(om + i, x, e.vec && n - i >= 4, n - i);
+        decode_v(cv[h], vs, x);
+        store4(ov + i, x, e.vec && n - i >= 4, n - i);
+      }
     }
   }
 }
@@ -443,35 +497,45 @@ int fill(AdamTable<N>& t, const gdn2_adamw_desc* d, const gdn2_adamw_tensor* ts,
   return i;
 }
 
+constexpr int kMostCtas = 148 * 5;          // as many as are at work at a time
+int norm_grid(int chunks) { return chunks < kMostCtas ? chunks : kMostCtas; }
 struct AdamTotal {
-  int tensors, chunks;
+  int tensors, parts;                   // parts: CTAs of the norm's launches
 };
-AdamTotal totals(const gdn2_adamw_tensor* ts, int n) {
+// Tables have `most` tensors.
+AdamTotal totals(const gdn2_adamw_tensor* ts, int n, int most) {
   AdamTotal r{0, 0};
-  for (int i = 0; i < n; ++i)
-    if (ts[i].n) {
-      ++r.tensors;
-      r.chunks += (int)((ts[i].n + kChunk - 1) / kChunk);
+  int chunks = 0, in = 0;
+  for (int i = 0; i < n; ++i) {
+    if (!ts[i].n) continue;
+    if (in == most) {
+      r.parts += norm_grid(chunks);
+      chunks = in = 0;
     }
+    ++in;
+    ++r.tensors;
+    chunks += (int)((ts[i].n + kChunk - 1) / kChunk);
+  }
+  r.parts += norm_grid(chunks);
   return r;
 }
-size_t parts_bytes(int chunks) { return ((size_t)chunks * sizeof(double) + 255) / 256 * 256; }
+size_t parts_bytes(int parts) { return ((size_t)parts * sizeof(double) + 255) / 256 * 256; }
 
 template <int N>
 cudaError_t run_adamw(const gdn2_adamw_desc* d, const gdn2_adamw_tensor* ts, int n, AdamParams a, cudaStream_t st) {
   static thread_local AdamTable<N> t;  // 31 KB: not on the stack
   cudaError_t e = cudaSuccess;
-  const AdamTotal all = totals(ts, n);
+  const AdamTotal all = totals(ts, n, N);
   a.alone = all.tensors <= N;
-  a.all_chunks = all.chunks;
-  a.chunk0 = a.tensor0 = 0;
+  a.all_parts = all.parts;
+  a.part0 = a.tensor0 = 0;
   if (a.norm || a.alone) {
-    for (int i = 0, done = 0; i < n && e == cudaSuccess;) {
+    for (int i = 0; i < n && e == cudaSuccess;) {
       i = fill(t, d, ts, i, n);
       if (!t.count) break;
-      e = launch_pdl(adamw_norm_kernel<N>, a.norm ? t.chunks : 1, kAdamThreads, 0, st, t, a);
-      a.chunk0 += t.chunks;
-      done += t.count;
+      const int grid = a.norm ? norm_grid(t.chunks) : 1;
+      e = launch_pdl(adamw_norm_kernel<N>, grid, kAdamThreads, 0, st, t, a);
+      a.part0 += grid;
     }
   }
   if (!a.alone) {
@@ -490,7 +554,9 @@ cudaError_t run_adamw(const gdn2_adamw_desc* d, const gdn2_adamw_tensor* ts, int
   for (int i = 0; i < n && e == cudaSuccess;) {
     i = fill(t, d, ts, i, n);
     if (!t.count) break;
-    const unsigned grid = t.chunks < 148 * 8 ? t.chunks : 148 * 8;
+    // codes: a CTA walks several chunks (8 bits, 348 M bf16 weights: 945 us; a CTA for each chunk 1235); 32 bits
+    // move more bytes than they compute and are better off with the scheduler's order (39 M weights: 161, not 174 us)
+    const unsigned grid = (unsigned)(d->state_bits == 8 && t.chunks > 148 * 8 ? 148 * 8 : t.chunks);
     e = d->state_bits == 8 ? launch_pdl(adamw_update_kernel<N, true>, grid, kAdamThreads, 0, st, t, a)
                            : launch_pdl(adamw_update_kernel<N, false>, grid, kAdamThreads, 0, st, t, a);
     a.tensor0 += t.count;
@@ -504,7 +570,7 @@ cudaError_t run_moments(const gdn2_adamw_desc* d, const gdn2_adamw_tensor* ts, i
   for (int i = 0; i < n;) {
     i = fill(t, d, ts, i, n);
     if (!t.count) break;
-    adamw_moments_kernel<N><<<t.chunks < 148 * 8 ? t.chunks : 148 * 8, kAdamThreads, 0, st>>>(t);
+    adamw_moments_kernel<N><<<(unsigned)t.chunks, kAdamThreads, 0, st>>>(t);
   }
   return cudaGetLastError();
 }
@@ -515,8 +581,8 @@ cudaError_t run_moments(const gdn2_adamw_desc* d, const gdn2_adamw_tensor* ts, i
 extern "C" size_t gdn2_adamw_workspace_bytes(const gdn2_adamw_desc* d, const gdn2_adamw_tensor* tensors, int32_t n) {
   using namespace gdn2;
   if (check_adamw(d, tensors, n) != GDN2_OK) return 0;
-  const AdamTotal all = totals(tensors, n);
-  return all.tensors ? parts_bytes(all.chunks) + all.tensors * sizeof(Factors) : 0;
+  const AdamTotal all = totals(tensors, n, kMany);
+  return all.tensors ? parts_bytes(all.parts) + all.tensors * sizeof(Factors) : 0;
 }
 
 extern "C" gdn2_status gdn2_adamw_step(const gdn2_adamw_desc* d, const gdn2_adamw_tensor* tensors, int32_t n,
@@ -524,7 +590,7 @@ extern "C" gdn2_status gdn2_adamw_step(const gdn2_adamw_desc* d, const gdn2_adam
   using namespace gdn2;
   const gdn2_status s = check_adamw(d, tensors, n);
   if (s != GDN2_OK) return s;
-  const AdamTotal all = totals(tensors, n);
+  const AdamTotal all = totals(tensors, n, kMany);
   if (!all.tensors) return GDN2_OK;
   for (int i = 0; i < n; ++i)
     if (tensors[i].n && (!tensors[i].step || !aligned(tensors[i].step, 4))) return GDN2_ERR_INVALID_ARGUMENT;
@@ -532,7 +598,7 @@ extern "C" gdn2_status gdn2_adamw_step(const gdn2_adamw_desc* d, const gdn2_adam
   AdamParams a{};
   a.ctl = static_cast<AdamControl*>(control);
   a.parts = static_cast<double*>(workspace);
-  a.factors = reinterpret_cast<Factors*>(static_cast<uint8_t*>(workspace) + parts_bytes(all.chunks));
+  a.factors = reinterpret_cast<Factors*>(static_cast<uint8_t*>(workspace) + parts_bytes(all.parts));
   a.loss = loss;
   a.log2_b1 = log2(d->beta1); a.log2_b2 = log2(d->beta2);
   a.fb1 = (float)d->beta1; a.gb1 = (float)(1.0 - d->beta1);
@@ -552,7 +618,7 @@ extern "C" gdn2_status gdn2_adamw_moments(const gdn2_adamw_tensor* tensors, int3
   if (s != GDN2_OK) return s;
   for (int i = 0; i < n; ++i)
     if (tensors[i].dtype != GDN2_F32) return GDN2_ERR_INVALID_ARGUMENT;
-  const AdamTotal all = totals(tensors, n);
+  const AdamTotal all = totals(tensors, n, kMany);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = all.tensors <= kFew ? run_moments<kFew>(&d, tensors, n, st) : run_moments<kMany>(&d, tensors, n, st);
   return e == cudaSuccess ? GDN2_OK : GDN2_ERR_CUDA;

@@ -281,94 +281,137 @@ void check_scale(const at::Tensor& t, const at::Tensor& p, const char* what) {
                     " contiguous float32 on ", p.device());
 }
 
-// adamw_step(params, grads, m, v, m_scales, v_scales, steps, lrs, decays, beta1, beta2, eps, clip, spike, bits, loss, control)
+// A new reference's value in a dict, borrowed, or null without an error.
+PyObject* item(PyObject* dict, PyObject* key) { return PyDict_GetItemWithError(dict, key); }
+at::Tensor tensor_of(PyObject* dict, PyObject* key, const char* what) {
+  PyObject* o = item(dict, key);
+  if (!o && PyErr_Occurred()) throw python_error();
+  TORCH_CHECK_VALUE(o && THPVariable_Check(o), "AdamW: the state of a parameter has no tensor ", what);
+  return THPVariable_Unpack(o);
+}
+struct Names {
+  PyObject *params = PyUnicode_InternFromString("params"), *lr = PyUnicode_InternFromString("lr"),
+           *wd = PyUnicode_InternFromString("weight_decay"), *step = PyUnicode_InternFromString("step"),
+           *m = PyUnicode_InternFromString("exp_avg"), *v = PyUnicode_InternFromString("exp_avg_sq"),
+           *ms = PyUnicode_InternFromString("exp_avg_scale"), *vs = PyUnicode_InternFromString("exp_avg_sq_scale");
+};
+
+// adamw_step(param_groups, state, beta1, beta2, eps, clip, spike, bits, loss, control) -> status, or None where a
+// parameter with a gradient has no state yet (or control is None).
 PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  TORCH_CHECK_TYPE(n == 17, "adamw_step takes 17 arguments");
-  auto p = tensors(a[0], "params"), g = tensors(a[1], "grads"), m = tensors(a[2], "exp_avg"), v = tensors(a[3], "exp_avg_sq");
-  auto ms = tensors(a[4], "scales"), vs = tensors(a[5], "scales"), steps = tensors(a[6], "steps");
+  static const Names names;
+  TORCH_CHECK_TYPE(n == 10 && PyList_Check(a[0]) && PyDict_Check(a[1]), "adamw_step takes a list, a dict and 8 values");
   gdn2_adamw_desc d{};
-  d.beta1 = PyFloat_AsDouble(a[9]);
-  d.beta2 = PyFloat_AsDouble(a[10]);
-  d.eps = PyFloat_AsDouble(a[11]);
-  d.clip = PyFloat_AsDouble(a[12]);
-  d.spike = PyFloat_AsDouble(a[13]);
-  d.state_bits = (int32_t)PyLong_AsLong(a[14]);
+  d.beta1 = PyFloat_AsDouble(a[2]);
+  d.beta2 = PyFloat_AsDouble(a[3]);
+  d.eps = PyFloat_AsDouble(a[4]);
+  d.clip = PyFloat_AsDouble(a[5]);
+  d.spike = PyFloat_AsDouble(a[6]);
+  d.state_bits = (int32_t)PyLong_AsLong(a[7]);
   if (PyErr_Occurred()) return nullptr;
-  const size_t k = p.size();
   const bool eight = d.state_bits == 8;
-  TORCH_CHECK_VALUE(g.size() == k && m.size() == k && v.size() == k && steps.size() == k &&
-                        (!eight || (ms.size() == k && vs.size() == k)) && PyList_CheckExact(a[7]) &&
-                        (size_t)PyList_GET_SIZE(a[7]) == k && PyList_CheckExact(a[8]) && (size_t)PyList_GET_SIZE(a[8]) == k,
-                    "AdamW: lists of different lengths");
-  if (!k) Py_RETURN_NONE;
-  const auto dev = p[0].device();
-  TORCH_CHECK(dev.is_cuda(), "AdamW: the parameters must be on a CUDA device (the step runs only on the B200 kernels)");
-  std::vector<gdn2_adamw_tensor> table(k);
-  const c10::cuda::CUDAGuard guard(dev);
-  for (size_t i = 0; i < k; ++i) {
-    gdn2_adamw_tensor& t = table[i];
-    const at::Tensor& q = p[i];
-    const auto type = q.scalar_type();
-    TORCH_CHECK_VALUE(q.device() == dev, "AdamW: parameters on ", q.device(), " and on ", dev, ": one optimizer steps one device's");
-    TORCH_CHECK_VALUE(type == at::kFloat || type == at::kBFloat16, "AdamW: parameters must be float32 or bfloat16, not ", type);
-    TORCH_CHECK_VALUE(q.layout() == at::kStrided && q.is_non_overlapping_and_dense(),
-                      "AdamW: a parameter's values must fill their memory, each at one place");
-    TORCH_CHECK_VALUE(g[i].layout() == at::kStrided && g[i].device() == dev && g[i].sizes() == q.sizes() && !g[i].is_complex(),
-                      "AdamW: a gradient must be dense, of its parameter's shape and device");
-    if (g[i].scalar_type() != type || (g[i].strides() != q.strides() && !(g[i].is_contiguous() && q.is_contiguous()))) {
-      at::Tensor c = at::empty_like(q);
-      c.copy_(g[i]);
-      g[i] = std::move(c);
-    }
-    check_moment(m[i], q, eight ? at::kByte : at::kFloat, "exp_avg");
-    check_moment(v[i], q, eight ? at::kByte : at::kFloat, "exp_avg_sq");
-    if (eight) {
-      check_scale(ms[i], q, "exp_avg_scale");
-      check_scale(vs[i], q, "exp_avg_sq_scale");
-      t.m_scale = floats(ms[i]);
-      t.v_scale = floats(vs[i]);
-    }
-    TORCH_CHECK_VALUE(steps[i].device() == dev && steps[i].scalar_type() == at::kFloat && steps[i].numel() == 1,
-                      "AdamW: step must be one float32 value on ", dev);
-    t.p = q.data_ptr(); t.g = g[i].data_ptr(); t.m = m[i].data_ptr(); t.v = v[i].data_ptr();
-    t.step = floats(steps[i]);
-    PyObject* lr = PyList_GET_ITEM(a[7], i);
-    if (THPVariable_Check(lr)) {
-      const at::Tensor& r = THPVariable_Unpack(lr);
-      TORCH_CHECK_VALUE(r.device() == dev && r.scalar_type() == at::kFloat && r.numel() == 1,
-                        "AdamW: a tensor for lr must be one float32 value on ", dev);
-      t.lr_at = floats(r);
-    } else {
-      t.lr = PyFloat_AsDouble(lr);
-    }
-    t.weight_decay = PyFloat_AsDouble(PyList_GET_ITEM(a[8], i));
+  const auto moment_type = eight ? at::kByte : at::kFloat;
+  std::vector<at::Tensor> kept;          // what the call has to hold, and what it changes
+  std::vector<at::Tensor> written;
+  std::vector<gdn2_adamw_tensor> table;
+  c10::Device dev(c10::kCPU);
+  for (Py_ssize_t gi = 0; gi < PyList_GET_SIZE(a[0]); ++gi) {
+    PyObject* group = PyList_GET_ITEM(a[0], gi);
+    TORCH_CHECK_TYPE(PyDict_Check(group), "AdamW: a parameter group must be a dict");
+    PyObject *params = item(group, names.params), *lr = item(group, names.lr), *wd = item(group, names.wd);
+    TORCH_CHECK_VALUE(params && PyList_Check(params) && lr && wd, "AdamW: a parameter group needs params, lr and weight_decay");
+    double rate = 0.0;
+    at::Tensor rate_at;
+    if (THPVariable_Check(lr)) rate_at = THPVariable_Unpack(lr);
+    else rate = PyFloat_AsDouble(lr);
+    const double decay = PyFloat_AsDouble(wd);
     if (PyErr_Occurred()) return nullptr;
-    t.n = q.numel();
-    t.dtype = dtype_of(type);
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(params); ++i) {
+      PyObject* key = PyList_GET_ITEM(params, i);
+      TORCH_CHECK_TYPE(THPVariable_Check(key), "AdamW: params must hold tensors");
+      const at::Tensor& q = THPVariable_Unpack(key);
+      at::Tensor g = q.grad();
+      if (!g.defined()) continue;
+      PyObject* st = item(a[1], key);
+      if (!st) {
+        if (PyErr_Occurred()) return nullptr;
+        Py_RETURN_NONE;
+      }
+      TORCH_CHECK_TYPE(PyDict_Check(st), "AdamW: the state of a parameter must be a dict");
+      if (!PyDict_GET_SIZE(st) || a[9] == Py_None) Py_RETURN_NONE;
+      gdn2_adamw_tensor t{};
+      const auto type = q.scalar_type();
+      if (table.empty()) dev = q.device();
+      TORCH_CHECK(q.is_cuda(), "AdamW: the parameters must be on a CUDA device (the step runs only on the B200 kernels)");
+      TORCH_CHECK_VALUE(q.device() == dev, "AdamW: parameters on ", q.device(), " and on ", dev, ": one optimizer steps one device's");
+      TORCH_CHECK_VALUE(type == at::kFloat || type == at::kBFloat16, "AdamW: parameters must be float32 or bfloat16, not ", type);
+      TORCH_CHECK_VALUE(q.layout() == at::kStrided && q.is_non_overlapping_and_dense(),
+                        "AdamW: a parameter's values must fill their memory, each at one place");
+      TORCH_CHECK_VALUE(g.layout() == at::kStrided && g.device() == dev && g.sizes() == q.sizes() && !g.is_complex(),
+                        "AdamW: a gradient must be dense, of its parameter's shape and device");
+      if (g.scalar_type() != type || (g.strides() != q.strides() && !(g.is_contiguous() && q.is_contiguous()))) {
+        const c10::cuda::CUDAGuard guard(dev);
+        at::Tensor c = at::empty_like(q);
+        c.copy_(g);
+        g = std::move(c);
+      }
+      at::Tensor m = tensor_of(st, names.m, "exp_avg"), v = tensor_of(st, names.v, "exp_avg_sq"),
+                 step = tensor_of(st, names.step, "step");
+      check_moment(m, q, moment_type, "exp_avg");
+      check_moment(v, q, moment_type, "exp_avg_sq");
+      TORCH_CHECK_VALUE(step.device() == dev && step.scalar_type() == at::kFloat && step.numel() == 1,
+                        "AdamW: step must be one float32 value on ", dev);
+      t.p = q.data_ptr(); t.g = g.data_ptr(); t.m = m.data_ptr(); t.v = v.data_ptr();
+      t.step = floats(step);
+      if (eight) {
+        at::Tensor ms = tensor_of(st, names.ms, "exp_avg_scale"), vs = tensor_of(st, names.vs, "exp_avg_sq_scale");
+        check_scale(ms, q, "exp_avg_scale");
+        check_scale(vs, q, "exp_avg_sq_scale");
+        t.m_scale = floats(ms);
+        t.v_scale = floats(vs);
+        written.push_back(std::move(ms));
+        written.push_back(std::move(vs));
+      }
+      if (rate_at.defined()) {
+        TORCH_CHECK_VALUE(rate_at.device() == dev && rate_at.scalar_type() == at::kFloat && rate_at.numel() == 1,
+                          "AdamW: a tensor for lr must be one float32 value on ", dev);
+        t.lr_at = floats(rate_at);
+      }
+      t.lr = rate;
+      t.weight_decay = decay;
+      t.n = q.numel();
+      t.dtype = dtype_of(type);
+      table.push_back(t);
+      written.push_back(q);
+      written.push_back(std::move(m));
+      written.push_back(std::move(v));
+      written.push_back(std::move(step));
+      kept.push_back(std::move(g));
+    }
   }
+  if (table.empty()) return PyLong_FromLong(GDN2_OK);
+  const int32_t k = (int32_t)table.size();
+  const c10::cuda::CUDAGuard guard(dev);
   const float* loss = nullptr;
   at::Tensor loss32;
-  if (a[15] != Py_None) {
-    TORCH_CHECK_TYPE(THPVariable_Check(a[15]), "AdamW: loss must be a tensor");
-    loss32 = THPVariable_Unpack(a[15]);
+  if (a[8] != Py_None) {
+    TORCH_CHECK_TYPE(THPVariable_Check(a[8]), "AdamW: loss must be a tensor");
+    loss32 = THPVariable_Unpack(a[8]);
     TORCH_CHECK_VALUE(loss32.device() == dev && loss32.numel() == 1, "AdamW: loss must be one value on ", dev);
     loss32 = loss32.detach().to(at::kFloat);
     loss = floats(loss32);
   }
-  TORCH_CHECK_TYPE(THPVariable_Check(a[16]), "AdamW: control must be a tensor");
-  const at::Tensor& control = THPVariable_Unpack(a[16]);
+  TORCH_CHECK_TYPE(THPVariable_Check(a[9]), "AdamW: control must be a tensor");
+  const at::Tensor& control = THPVariable_Unpack(a[9]);
   TORCH_CHECK_VALUE(control.device() == dev && control.scalar_type() == at::kFloat && control.numel() == 5 && control.is_contiguous(),
                     "AdamW: control must be five float32 words on ", dev);
-  const int64_t size[1] = {(int64_t)gdn2_adamw_workspace_bytes(&d, table.data(), (int32_t)k)};
+  const int64_t size[1] = {(int64_t)gdn2_adamw_workspace_bytes(&d, table.data(), k)};
   at::Tensor ws = fresh(size, at::kByte, dev);
-  const gdn2_status s = gdn2_adamw_step(&d, table.data(), (int32_t)k, loss, control.data_ptr(), ws.data_ptr(),
+  const gdn2_status s = gdn2_adamw_step(&d, table.data(), k, loss, control.data_ptr(), ws.data_ptr(),
                                         c10::cuda::getCurrentCUDAStream(dev.index()).stream());
   if (s == GDN2_OK)
-    for (size_t i = 0; i < k; ++i) {
-      changed(p[i]); changed(m[i]); changed(v[i]); changed(steps[i]);
-      if (eight) { changed(ms[i]); changed(vs[i]); }
-    }
+    for (const at::Tensor& t : written) changed(t);
   return PyLong_FromLong(s);
   END_HANDLE_TH_ERRORS
 }
