@@ -165,7 +165,7 @@ def _declare(lib):
     lib.gdn2_gated_fwd.restype = ctypes.c_int
     lib.gdn2_gated_fwd.argtypes = [P] * 12
     lib.gdn2_gated_bwd.restype = ctypes.c_int
-    lib.gdn2_gated_bwd.argtypes = [P] * 12
+    lib.gdn2_gated_bwd.argtypes = [P] * 13
     lib.gdn2_gated_marks_bytes.restype = ctypes.c_size_t
     lib.gdn2_gated_marks_bytes.argtypes = [P]
     lib.gdn2_linear_fwd.restype = ctypes.c_int

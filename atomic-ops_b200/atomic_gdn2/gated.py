@@ -112,10 +112,13 @@ class _Gated(torch.autograd.Function):
         dx, dg = torch.empty_like(dh), torch.empty_like(dh)
         d0 = torch.empty((B, C), dtype=torch.float32, device=dev) if th is not None and ctx.needs_input_grad[2] else None
         d, at, _ = _desc(x, g, 0)
+        fl = pipeline._host_flags(dev)
         with _guard(dev):
             rc = _lib.load().gdn2_gated_bwd(at, _ptr(x), _ptr(g), _ptr(lengths), _ptr(reset), _ptr(marks), _ptr(dh),
-                                            _ptr(dlast), _ptr(dx), _ptr(dg), _ptr(d0), _raw_stream(dev.index))
+                                            _ptr(dlast), _ptr(dx), _ptr(dg), _ptr(d0), fl.ptr,
+                                            _raw_stream(dev.index))
         _lib.check(rc, "gdn2_gated_bwd")
+        _check_flags(fl, "gdn2_gated_bwd")
         return dx.to(tx), dg.to(tg), None if d0 is None else d0.to(th), None, None
 
 

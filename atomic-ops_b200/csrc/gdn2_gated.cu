@@ -8,9 +8,10 @@
 // written once.  A thread walks S tokens of V channels in registers: once from zero, for what the segment
 // does to a state (h -> A h + q), and, when the state that enters is known, once more as the recurrence
 // itself, so that an output carries the rounding of its own steps and of the few joined segments before.
-// Segments are joined over a CTA's threads in shared memory and over the CTAs of a cluster, which take
-// neighbouring stretches of one sequence, in distributed shared memory: one launch, no waiting on memory
-// flags, no workspace, and the same order of additions every time.  A cluster walks its sequence in rounds.
+// Segments are joined over a warp's lanes by shuffles, over a CTA's warps in shared memory and over the CTAs of
+// a cluster, which take neighbouring stretches of one sequence, through each other's shared memory: one launch,
+// no flags in global memory, no workspace, and the same order of additions every time.  A cluster walks its
+// sequence in rounds.
 // The backward pass starts its segments from the states that the forward pass left at their borders (4 / S
 // bytes a value) and computes h again from x: reading the rounded h instead would cost as many bytes and,
 // for bf16, half a step of h in dg.
@@ -25,7 +26,8 @@ namespace cg = cooperative_groups;
 
 constexpr float kReset = -1.f;        // a segment's factor when a reset is in it: what entered is dropped
 constexpr float kTiny = 1.17549435e-38f;
-constexpr int kMaxWarps = 8;
+constexpr int kMaxWarps = 8, kMaxCluster = 8;
+constexpr int kValues = 16;           // of a thread's segment: S tokens of V channels
 
 struct GatedParams {
   const void *x, *g, *dy;
@@ -117,58 +119,175 @@ __device__ __forceinline__ uint32_t resets_of(const GatedParams& p, int b, long 
   return bits;
 }
 
-struct Shared {  // [buffer][segment of the CTA][channel of a row of lanes]: at most 8 x 32 / lanes x lanes x V
-  Seg part[kMaxWarps * 32 * 2];
-  Seg whole[2][32 * 2];
+// The first `live` of S rows: all at once where there are S.
+template <int S, class raw>
+__device__ __forceinline__ void rows_of(raw r[S], const raw* p, long long ld, int live) {
+  if (live == S) {
+#pragma unroll
+    for (int i = 0; i < S; ++i) r[i] = __ldg(p + i * ld);
+  } else {
+    for (int i = 0; i < S; ++i) r[i] = raw{};
+#pragma unroll
+    for (int i = 0; i < S; ++i)
+      if (i < live) r[i] = __ldg(p + i * ld);
+  }
+}
+
+struct Shared {
+  Seg part[2][kMaxWarps][32 * 2];       // a warp's segments together, by channel of a row of lanes, for two rounds
+  Seg inbox[2][kMaxCluster][32 * 2];    // the CTAs' of the cluster, for two rounds
+  uint64_t bar[2];                      // that they are there
+  volatile int dead;                    // a wait ran out
 };
 
-// Joins the segments of all threads: `mine` of this thread's V channels comes at place `place` of `places`
-// in the CTA and the CTA at place `rank` of `n` in its cluster.  enter[] is the state that the cluster's
-// first segment enters with; on return `mine_in` is what this thread's enters with, and enter[] what the
-// next round's first one does.
-template <int V>
-__device__ __forceinline__ void exchange(Shared& sm, int buf, const Seg mine[V], int place, int places, int lane,
-                                         int lanes, int rank, int n, float enter[V], float mine_in[V]) {
-  const int w = lanes * V;
-#pragma unroll
-  for (int v = 0; v < V; ++v) sm.part[place * w + lane * V + v] = mine[v];
-  __syncthreads();
-  Seg before[V];  // of this CTA's segments before this thread's
-#pragma unroll
-  for (int v = 0; v < V; ++v) before[v] = {1.f, 0.f};
-  for (int i = 0; i < place; ++i)
-#pragma unroll
-    for (int v = 0; v < V; ++v) before[v] = join(before[v], sm.part[i * w + lane * V + v]);
-  if (place == places - 1) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) sm.whole[buf][lane * V + v] = join(before[v], mine[v]);
+// The CTAs of a cluster write what their segments come to into each other's inbox, and each write is counted at the
+// receiver's barrier.  (A barrier over the cluster would order all of the CTA's memory accesses, the outputs' of the
+// round before among them: 5.0 us a round of 8 CTAs.)  A CTA sends round r + 2 after it has seen every CTA's
+// round r + 1, which these send after they have read round r: two boxes are enough.
+__device__ __forceinline__ void send(Shared& sm, int box, int from, int to, int at, Seg s) {
+  uint32_t dst, bar;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(dst) : "r"(smem_u32(&sm.inbox[box][from][at])), "r"(to));
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_u32(&sm.bar[box])), "r"(to));
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b32 [%0], {%1, %2}, [%3];" ::"r"(dst),
+               "r"(__float_as_uint(s.A)), "r"(__float_as_uint(s.q)), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ bool cluster_wait(uint64_t* bar, uint32_t parity) {
+  const long long t0 = clock64();
+  for (uint32_t it = 0;; ++it) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if ((it & 255u) == 255u && clock64() - t0 > kWaitCycles) return false;
   }
-  if (n > 1) {
-    cg::cluster_group cl = cg::this_cluster();
-    cl.sync();
-    for (int r = 0; r < n; ++r) {
-      const Seg* other = cl.map_shared_rank(&sm.whole[buf][0], r);
+}
+
+__device__ __forceinline__ void begin(Shared& sm, int n) {
+  if (n == 1) return;
+  if (threadIdx.x == 0) {
+    mbar_init(&sm.bar[0], 1);
+    mbar_init(&sm.bar[1], 1);
+    sm.dead = 0;
+    fence_mbar_init();
+  }
+  cg::this_cluster().sync();
+}
+
+// join() and step() where no reset and no gate of zero is about (plain), or with them.
+template <bool PLAIN>
+__device__ __forceinline__ Seg join_as(Seg a, Seg b) {
+  if constexpr (PLAIN) return {fmaxf(a.A * b.A, kTiny), fmaf(b.A, a.q, b.q)};
+  else return join(a, b);
+}
+template <bool PLAIN>
+__device__ __forceinline__ float step_as(Seg s, float h) {
+  if constexpr (PLAIN) return fmaf(s.A, h, s.q);
+  else return step(s, h);
+}
+template <bool PLAIN, int V>
+__device__ __forceinline__ void join_warp(Seg (*part)[32 * 2], const Seg mine[V], int lanes, Seg before[V]) {
+  const int at = threadIdx.x & 31, lane = at & (lanes - 1), warp = threadIdx.x >> 5;
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        if (r == rank) mine_in[v] = step(before[v], enter[v]);
-        enter[v] = step(other[lane * V + v], enter[v]);
-      }
+  for (int v = 0; v < V; ++v) {
+    Seg all = mine[v];
+    for (int d = lanes; d < 32; d <<= 1) {
+      const Seg left = {__shfl_up_sync(0xffffffffu, all.A, d), __shfl_up_sync(0xffffffffu, all.q, d)};
+      if (at >= d) all = join_as<PLAIN>(left, all);
     }
-  } else {
-    __syncthreads();
+    if (at >= 32 - lanes) part[warp][lane * V + v] = all;
+    before[v] = {1.f, 0.f};
+    if (lanes < 32) {
+      before[v] = {__shfl_up_sync(0xffffffffu, all.A, lanes), __shfl_up_sync(0xffffffffu, all.q, lanes)};
+      if (at < lanes) before[v] = {1.f, 0.f};
+    }
+  }
+}
+template <bool PLAIN, int V>
+__device__ __forceinline__ void join_cta(Shared& sm, int round, int lanes, int rank, int n, Seg before[V], float enter[V], float mine_in[V]) {
+  const int at = threadIdx.x & 31, lane = at & (lanes - 1), warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      mine_in[v] = step(before[v], enter[v]);
-      enter[v] = step(sm.whole[buf][lane * V + v], enter[v]);
+  for (int v = 0; v < V; ++v) {
+    if (n > 1) {
+      Seg pre = {1.f, 0.f};
+      for (int i = 0; i < warp; ++i) pre = join_as<PLAIN>(pre, sm.part[round & 1][i][lane * V + v]);
+      if (warp == warps - 1 && at < lanes) {
+        const Seg all = join_as<PLAIN>(pre, sm.part[round & 1][warp][lane * V + v]);
+        for (int r = 0; r < n; ++r) send(sm, round & 1, rank, r, lane * V + v, all);
+      }
+      before[v] = join_as<PLAIN>(pre, before[v]);
+    } else {                            // the state itself goes from warp to warp
+      float h = enter[v], in = h;
+      for (int i = 0; i < warps; ++i) {
+        if (i == warp) in = h;
+        h = step_as<PLAIN>(sm.part[round & 1][i][lane * V + v], h);
+      }
+      mine_in[v] = step_as<PLAIN>(before[v], in);
+      enter[v] = h;
     }
   }
 }
 
+// Joins the segments of all threads.  The lanes of a warp hold 32 / lanes neighbouring segments of the same
+// channels, the warps of a CTA and the CTAs of a cluster follow one another.  enter[] is the state that the
+// cluster's first segment enters with; on return mine_in[] is what this thread's enters with, and enter[] what the
+// next round's first one does.  `plain`: no reset and no gate of zero in this thread's segment.
+template <int V>
+__device__ __forceinline__ void exchange(Shared& sm, int round, const Seg mine[V], bool plain, int lanes, int rank, int n,
+                                         float enter[V], float mine_in[V], uint32_t* flags) {
+  const int lane = threadIdx.x & (lanes - 1);
+  Seg before[V];                        // of this warp's segments before this thread's
+  if (__all_sync(0xffffffffu, plain)) join_warp<true, V>(sm.part[round & 1], mine, lanes, before);
+  else join_warp<false, V>(sm.part[round & 1], mine, lanes, before);
+  if (__syncthreads_and(plain)) join_cta<true, V>(sm, round, lanes, rank, n, before, enter, mine_in);
+  else join_cta<false, V>(sm, round, lanes, rank, n, before, enter, mine_in);
+  if (n > 1) {
+    Seg(*inbox)[32 * 2] = sm.inbox[round & 1];
+    if (threadIdx.x == 0) mbar_arrive_expect_tx(&sm.bar[round & 1], (uint32_t)(n * lanes * V * sizeof(Seg)));
+    if (!sm.dead && !cluster_wait(&sm.bar[round & 1], (round >> 1) & 1)) {
+      sm.dead = 1;
+      if (flags) flags[2] = 1;
+    }
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r)
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (r < n) {
+          if (r == rank) mine_in[v] = step(before[v], enter[v]);
+          enter[v] = step(inbox[r][lane * V + v], enter[v]);
+        }
+  }
+}
+
+__device__ __forceinline__ float at_most_zero(float g) {  // a NaN stays one
+  float r;
+  asm("min.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(g));
+  return r;
+}
+// What S tokens do to a state, from the product of their gates and the state that they make of zero.
+template <int S, int V>
+__device__ __forceinline__ Seg segment(const float (*a)[V], int v, float A, float q, uint32_t resets, bool& plain) {
+  if (resets) A = kReset;
+  else if (!(A >= kTiny)) {             // underflow, or a gate that is zero (or a NaN)
+    bool zero = false;
+#pragma unroll
+    for (int i = 0; i < S; ++i) zero |= a[i][v] == 0.f;
+    A = A != A ? A : zero ? 0.f : kTiny;
+  }
+  plain = plain && A > 0.f;
+  return {A, q};
+}
+
 template <class T, int V>
-__global__ void __launch_bounds__(32 * kMaxWarps) gated_fwd_kernel(const __grid_constant__ GatedParams p) {
+__global__ void __launch_bounds__(32 * kMaxWarps, 3) gated_fwd_kernel(const __grid_constant__ GatedParams p) {
   using L = Lane<T, V>;
   using raw = typename L::raw;
-  constexpr int S = 32 / V;
+  constexpr int S = kValues / V;
   __shared__ Shared sm;
   const int lanes = 1 << p.lanes_log2, lane = threadIdx.x & (lanes - 1);
   const int place = threadIdx.x >> p.lanes_log2, places = blockDim.x >> p.lanes_log2;
@@ -177,77 +296,81 @@ __global__ void __launch_bounds__(32 * kMaxWarps) gated_fwd_kernel(const __grid_
   const bool on = c < p.C;
   const int len = length_of(p, b);
   const long long row = state_row(p, b);
+  begin(sm, p.clusters);
   float enter[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) enter[v] = on && row >= 0 ? p.h0[row * p.C + c + v] : 0.f;
   const raw* x = reinterpret_cast<const raw*>(static_cast<const T*>(p.x) + b * p.xb + c);
   const raw* g = reinterpret_cast<const raw*>(static_cast<const T*>(p.g) + b * p.gb + c);
   raw* h = reinterpret_cast<raw*>(static_cast<T*>(p.h) + (long long)b * p.L * p.C + c);
+  const long long xl = p.xl / V, gl = p.gl / V, hl = p.C / V;
   const int segs = (p.L + S - 1) / S, per_round = places * p.clusters;
-  bool positive = false;
-  for (int round = 0, buf = 0; round * (long long)per_round < segs; ++round, buf ^= 1) {
+  float top = -1.f;                     // the largest gate
+  for (int round = 0; round * (long long)per_round < segs; ++round) {
     const long long seg = (long long)round * per_round + rank * places + place;
     const long long t0 = seg * S;
     const int live = on ? (int)max(0ll, min((long long)S, len - t0)) : 0;
     float a[S][V], q[S][V];
-    const uint32_t resets = resets_of<S>(p, b, t0, live);
     {
       raw rx[S], rg[S];
-      const raw* px = x + t0 * (p.xl / V);
-      const raw* pg = g + t0 * (p.gl / V);
-#pragma unroll
-      for (int i = 0; i < S; ++i)
-        if (i < live) {
-          rx[i] = px[i * (p.xl / V)];
-          rg[i] = pg[i * (p.gl / V)];
-        }
+      rows_of<S>(rx, x + t0 * xl, xl, live);   // past the end zeros: gates of one
+      rows_of<S>(rg, g + t0 * gl, gl, live);
 #pragma unroll
       for (int i = 0; i < S; ++i) {
         L::get(rx[i], q[i]);
         L::get(rg[i], a[i]);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          if (i < live) {
-            positive |= a[i][v] > 0.f;
-            a[i][v] = expf(a[i][v] > 0.f ? 0.f : a[i][v]);  // a NaN stays one
-          } else {
-            a[i][v] = 1.f;
-            q[i][v] = 0.f;
-          }
+          top = fmaxf(top, a[i][v]);
+          a[i][v] = expf(at_most_zero(a[i][v]));
         }
       }
     }
+    const uint32_t resets = resets_of<S>(p, b, t0, live);
     Seg mine[V];
     float mine_in[V];
+    bool plain = true;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       float A = 1.f, s = 0.f;
-      bool zero = false;
+      if (!resets) {
 #pragma unroll
-      for (int i = 0; i < S; ++i) {
-        const bool r = (resets >> i) & 1u;
-        s = r ? q[i][v] : fmaf(a[i][v], s, q[i][v]);
-        zero |= a[i][v] == 0.f;
-        A *= a[i][v];
+        for (int i = 0; i < S; ++i) {
+          s = fmaf(a[i][v], s, q[i][v]);
+          A *= a[i][v];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < S; ++i) s = ((resets >> i) & 1u) ? q[i][v] : fmaf(a[i][v], s, q[i][v]);
       }
-      mine[v] = {resets ? kReset : zero ? 0.f : fmaxf(A, kTiny), s};
+      mine[v] = segment<S, V>(a, v, A, s, resets, plain);
     }
-    exchange<V>(sm, buf, mine, place, places, lane, lanes, rank, p.clusters, enter, mine_in);
+    exchange<V>(sm, round, mine, plain, lanes, rank, p.clusters, enter, mine_in, p.flags);
     if (on && t0 < p.L) {
       if (p.marks) {
 #pragma unroll
         for (int v = 0; v < V; ++v) p.marks[((long long)b * segs + seg) * p.C + c + v] = mine_in[v];
       }
-      raw* ph = h + t0 * (p.C / V);
+      raw* ph = h + t0 * hl;
+      if (live == S && !resets) {
 #pragma unroll
-      for (int i = 0; i < S; ++i) {
-        float y[V];
+        for (int i = 0; i < S; ++i) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          mine_in[v] = ((resets >> i) & 1u) ? q[i][v] : fmaf(a[i][v], mine_in[v], q[i][v]);
-          y[v] = i < live ? mine_in[v] : 0.f;
+          for (int v = 0; v < V; ++v) mine_in[v] = fmaf(a[i][v], mine_in[v], q[i][v]);
+          ph[i * hl] = L::put(mine_in);
         }
-        if (t0 + i < p.L) ph[i * (long long)(p.C / V)] = L::put(y);
+      } else {
+        const int rows = (int)min((long long)S, p.L - t0);
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+          float y[V];
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            mine_in[v] = ((resets >> i) & 1u) ? q[i][v] : fmaf(a[i][v], mine_in[v], q[i][v]);
+            y[v] = i < live ? mine_in[v] : 0.f;
+          }
+          if (i < rows) ph[i * hl] = L::put(y);
+        }
       }
     }
   }
@@ -255,15 +378,15 @@ __global__ void __launch_bounds__(32 * kMaxWarps) gated_fwd_kernel(const __grid_
 #pragma unroll
     for (int v = 0; v < V; ++v) p.last[(long long)b * p.C + c + v] = enter[v];
   }
-  if (positive && p.flags) p.flags[0] = 1;
-  if (p.clusters > 1) cg::this_cluster().sync();  // a CTA's shared memory is read until here
+  if (top > 0.f) p.flags[0] = 1;
+  if (p.clusters > 1) cg::this_cluster().sync();  // a CTA's shared memory is written until here
 }
 
 template <class T, int V>
-__global__ void __launch_bounds__(32 * kMaxWarps) gated_bwd_kernel(const __grid_constant__ GatedParams p) {
+__global__ void __launch_bounds__(32 * kMaxWarps, 2) gated_bwd_kernel(const __grid_constant__ GatedParams p) {
   using L = Lane<T, V>;
   using raw = typename L::raw;
-  constexpr int S = 32 / V;
+  constexpr int S = kValues / V;
   __shared__ Shared sm;
   const int lanes = 1 << p.lanes_log2, lane = threadIdx.x & (lanes - 1);
   const int place = threadIdx.x >> p.lanes_log2, places = blockDim.x >> p.lanes_log2;
@@ -271,6 +394,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps) gated_bwd_kernel(const __grid_
   const int b = block / p.cols, c = ((block % p.cols) * lanes + lane) * V;
   const bool on = c < p.C;
   const int len = length_of(p, b);
+  begin(sm, p.clusters);
   float enter[V];  // e after the last token of a round, the sequence's last round first
 #pragma unroll
   for (int v = 0; v < V; ++v) enter[v] = on && p.dlast ? p.dlast[(long long)b * p.C + c + v] : 0.f;
@@ -280,26 +404,19 @@ __global__ void __launch_bounds__(32 * kMaxWarps) gated_bwd_kernel(const __grid_
   const raw* dy = reinterpret_cast<const raw*>(static_cast<const T*>(p.dy) + at);
   raw* dx = reinterpret_cast<raw*>(static_cast<T*>(p.dx) + at);
   raw* dg = reinterpret_cast<raw*>(static_cast<T*>(p.dg) + at);
+  const long long xl = p.xl / V, gl = p.gl / V;
   const int segs = (p.L + S - 1) / S, per_round = places * p.clusters;
-  for (int round = 0, buf = 0; round * (long long)per_round < segs; ++round, buf ^= 1) {
+  for (int round = 0; round * (long long)per_round < segs; ++round) {
     const long long seg = segs - 1 - ((long long)round * per_round + rank * places + place);  // below 0: none
     const long long t0 = seg * S;
     const int live = on && seg >= 0 ? (int)max(0ll, min((long long)S, len - t0)) : 0;
+    float a[S][V], h[S][V], d[S][V], top = -1.f;
     const uint32_t resets = resets_of<S>(p, b, t0, live);
-    float a[S][V], h[S][V], d[S][V];
-    uint32_t open[V] = {};  // bit i: the gate is not above zero
     {
       raw rx[S], rg[S], ry[S];
-      const raw* px = x + t0 * (p.xl / V);
-      const raw* pg = g + t0 * (p.gl / V);
-      const raw* py = dy + t0 * row;
-#pragma unroll
-      for (int i = 0; i < S; ++i)
-        if (i < live) {
-          rx[i] = px[i * (p.xl / V)];
-          rg[i] = pg[i * (p.gl / V)];
-          ry[i] = py[i * row];
-        }
+      rows_of<S>(rx, x + t0 * xl, xl, live);   // past the end zeros: gates of one, nothing added
+      rows_of<S>(rg, g + t0 * gl, gl, live);
+      rows_of<S>(ry, dy + t0 * row, row, live);
       float s[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) s[v] = live ? p.marks[((long long)b * segs + seg) * p.C + c + v] : 0.f;
@@ -311,52 +428,69 @@ __global__ void __launch_bounds__(32 * kMaxWarps) gated_bwd_kernel(const __grid_
         L::get(ry[i], d[i]);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
+          top = fmaxf(top, a[i][v]);
+          a[i][v] = expf(at_most_zero(a[i][v]));
           h[i][v] = s[v];  // the state before the token
-          if (i < live) {
-            open[v] |= (a[i][v] > 0.f ? 0u : 1u) << i;
-            a[i][v] = expf(a[i][v] > 0.f ? 0.f : a[i][v]);
-            s[v] = ((resets >> i) & 1u) ? q[v] : fmaf(a[i][v], s[v], q[v]);
-          } else {
-            a[i][v] = 1.f;
-            d[i][v] = 0.f;
-          }
+          const float next = fmaf(a[i][v], s[v], q[v]);
+          s[v] = resets && ((resets >> i) & 1u) ? q[v] : next;
         }
       }
     }
     Seg mine[V];
     float e[V];
+    bool plain = true;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       float A = 1.f, s = 0.f;
-      bool zero = false;
+      if (!resets) {
 #pragma unroll
-      for (int i = S - 1; i >= 0; --i) {
-        s = ((resets >> i) & 1u) ? 0.f : a[i][v] * (d[i][v] + s);
-        zero |= a[i][v] == 0.f;
-        A *= a[i][v];
+        for (int i = S - 1; i >= 0; --i) {
+          s = a[i][v] * (d[i][v] + s);
+          A *= a[i][v];
+        }
+      } else {
+#pragma unroll
+        for (int i = S - 1; i >= 0; --i) s = ((resets >> i) & 1u) ? 0.f : a[i][v] * (d[i][v] + s);
       }
-      mine[v] = {resets ? kReset : zero ? 0.f : fmaxf(A, kTiny), s};
+      mine[v] = segment<S, V>(a, v, A, s, resets, plain);
     }
-    exchange<V>(sm, buf, mine, place, places, lane, lanes, rank, p.clusters, enter, e);
+    exchange<V>(sm, round, mine, plain, lanes, rank, p.clusters, enter, e, p.flags);
     if (on && seg >= 0) {
       raw* qx = dx + t0 * row;
       raw* qg = dg + t0 * row;
+      if (live == S && !resets && !(top > 0.f)) {
 #pragma unroll
-      for (int i = S - 1; i >= 0; --i) {
-        float ox[V], og[V];
-        const bool r = (resets >> i) & 1u;
+        for (int i = S - 1; i >= 0; --i) {
+          float ox[V], og[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          ox[v] = og[v] = 0.f;
-          if (i < live) {
+          for (int v = 0; v < V; ++v) {
             ox[v] = d[i][v] + e[v];
-            e[v] = r ? 0.f : a[i][v] * ox[v];
-            og[v] = r || !((open[v] >> i) & 1u) ? 0.f : e[v] * h[i][v];
+            e[v] = a[i][v] * ox[v];
+            og[v] = e[v] * h[i][v];
           }
-        }
-        if (t0 + i < p.L) {
           qx[i * row] = L::put(ox);
           qg[i * row] = L::put(og);
+        }
+      } else {
+        const int rows = (int)min((long long)S, p.L - t0);
+#pragma unroll
+        for (int i = S - 1; i >= 0; --i) {
+          float ox[V] = {}, og[V] = {};
+          if (i < live) {
+            const bool r = (resets >> i) & 1u;
+            float gate[V];
+            L::get(g[(t0 + i) * gl], gate);
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+              ox[v] = d[i][v] + e[v];
+              e[v] = r ? 0.f : a[i][v] * ox[v];
+              og[v] = r || gate[v] > 0.f ? 0.f : e[v] * h[i][v];
+            }
+          }
+          if (i < rows) {
+            qx[i * row] = L::put(ox);
+            qg[i * row] = L::put(og);
+          }
         }
       }
     }
@@ -365,7 +499,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps) gated_bwd_kernel(const __grid_
 #pragma unroll
     for (int v = 0; v < V; ++v) p.dh0[(long long)b * p.C + c + v] = enter[v];
   }
-  if (p.clusters > 1) cg::this_cluster().sync();  // a CTA's shared memory is read until here
+  if (p.clusters > 1) cg::this_cluster().sync();  // a CTA's shared memory is written until here
 }
 
 // A few tokens while a model answers: a thread walks them for V channels of a sequence.
@@ -429,15 +563,21 @@ struct GatedPlan {
 
 template <class K>
 cudaError_t launch_gated(K kernel, GatedParams& p, int V, cudaStream_t st) {
-  const int S = 32 / V, segs = (p.L + S - 1) / S;
+  const int S = kValues / V, segs = (p.L + S - 1) / S;
+  // Enough CTAs for two on every SM: narrower ones first (32-byte rows of 8 channels; their lanes take more
+  // segments), then clusters.  8 x 2048 x 768 fp32, forward + backward: 110 us with 192 CTAs of 32 channels, 92 with
+  // 384 of 16, 99 with 768 of 8, 136 with 384 of 32 in pairs; 1 x 131072 x 256: 794 us with 64 CTAs of 32 channels
+  // in clusters of 8, 459 with 128 of 16, 300 with 256 of 8.
   const GatedPlan pl = [&] {
-    GatedPlan r{};
-    r.lanes_log2 = 5;
-    auto cols = [&] { return (p.C + (V << r.lanes_log2) - 1) / (V << r.lanes_log2); };
-    r.warps = segs < kMaxWarps ? (segs < 1 ? 1 : segs) : kMaxWarps;
-    r.clusters = 1;
-    while (r.clusters < 8 && (long long)p.B * cols() * r.clusters < 296 && r.clusters * r.warps < segs) r.clusters *= 2;
+    GatedPlan r{0, 5, 1, 0};
+    auto cols = [&] { return (int)((p.C + (long long)(V << r.lanes_log2) - 1) / (V << r.lanes_log2)); };
+    auto groups = [&] { return 32 >> r.lanes_log2; };
+    while (r.lanes_log2 > 3 && (long long)p.B * cols() < 296 && 2 * groups() <= segs) --r.lanes_log2;
     r.cols = cols();
+    r.warps = (segs + groups() - 1) / groups();
+    r.warps = r.warps < 1 ? 1 : r.warps > kMaxWarps ? kMaxWarps : r.warps;
+    const int places = r.warps * groups();
+    while (r.clusters < kMaxCluster && (long long)p.B * r.cols * r.clusters * 2 <= 296 && r.clusters * places < segs) r.clusters *= 2;
     return r;
   }();
   p.cols = pl.cols;
@@ -472,7 +612,7 @@ size_t access(const gdn2_gated_desc* d) { return d->dtype == GDN2_F32 || pairs(d
 extern "C" size_t gdn2_gated_marks_bytes(const gdn2_gated_desc* d) {
   using namespace gdn2;
   if (check_gated(d) != GDN2_OK) return 0;
-  const long long S = pairs(d) ? 16 : 32;
+  const long long S = kValues / (pairs(d) ? 2 : 1);
   return (size_t)d->B * (size_t)((d->L + S - 1) / S) * (size_t)d->C * sizeof(float);
 }
 
@@ -512,18 +652,18 @@ extern "C" gdn2_status gdn2_gated_fwd(const gdn2_gated_desc* d, const void* x, c
 
 extern "C" gdn2_status gdn2_gated_bwd(const gdn2_gated_desc* d, const void* x, const void* g, const int32_t* lengths,
                                       const uint8_t* reset, const float* marks, const void* dh, const float* dlast,
-                                      void* dx, void* dg, float* dh0, void* stream) {
+                                      void* dx, void* dg, float* dh0, uint32_t* flags, void* stream) {
   using namespace gdn2;
   const gdn2_status s = check_gated(d);
   if (s != GDN2_OK) return s;
-  if (d->L < 1 || !x || !g || !marks || !dh || !dx || !dg) return GDN2_ERR_INVALID_ARGUMENT;
+  if (d->L < 1 || !x || !g || !marks || !dh || !dx || !dg || !flags) return GDN2_ERR_INVALID_ARGUMENT;
   const size_t n = access(d);
   if (off(x, n) || off(g, n) || off(dh, n) || off(dx, n) || off(dg, n) || off(marks, 4) || off(dlast, 4) ||
-      off(dh0, 4) || off(lengths, 4))
+      off(dh0, 4) || off(lengths, 4) || off(flags, 4))
     return GDN2_ERR_INVALID_ARGUMENT;
   GatedParams p = params_of(d);
   p.x = x; p.g = g; p.lengths = lengths; p.reset = reset; p.marks = const_cast<float*>(marks);
-  p.dy = dh; p.dlast = dlast; p.dx = dx; p.dg = dg; p.dh0 = dh0;
+  p.dy = dh; p.dlast = dlast; p.dx = dx; p.dg = dg; p.dh0 = dh0; p.flags = flags;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = d->dtype == GDN2_F32 ? launch_gated(gated_bwd_kernel<float, 1>, p, 1, st)
                         : pairs(d)           ? launch_gated(gated_bwd_kernel<__nv_bfloat16, 2>, p, 2, st)

@@ -326,8 +326,9 @@ typedef struct gdn2_gated_desc {
  *   h         (B, L, C) contiguous;  last (B, C) fp32, which may be h0 itself when h_index is NULL and overlaps
  *             no input otherwise
  *   marks     gdn2_gated_marks_bytes(desc) bytes for the backward (states inside the sequences), or NULL
- *   flags     two uint32 words in device or mapped host memory: [0] becomes 1 when g > 0 is seen, [1] when an
- *             index >= n_states (zeros are taken) or a length outside 0..L (the nearer bound is taken) is */
+ *   flags     three uint32 words in device or mapped host memory: [0] becomes 1 when g > 0 is seen, [1] when an
+ *             index >= n_states (zeros are taken) or a length outside 0..L (the nearer bound is taken) is, [2] when
+ *             an on-chip wait ran out (the results are invalid) */
 gdn2_status gdn2_gated_fwd(const gdn2_gated_desc* desc, const void* x, const void* g, const float* h0,
                            const int32_t* h_index, const int32_t* lengths, const uint8_t* reset, void* h,
                            float* last, float* marks, uint32_t* flags, void* stream);
@@ -338,7 +339,7 @@ size_t gdn2_gated_marks_bytes(const gdn2_gated_desc* desc);
  * (B, C) fp32 or NULL.  dg is zero where g > 0.  desc, x, g, lengths, reset and marks are the forward's; L >= 1. */
 gdn2_status gdn2_gated_bwd(const gdn2_gated_desc* desc, const void* x, const void* g, const int32_t* lengths,
                            const uint8_t* reset, const float* marks, const void* dh, const float* dlast, void* dx,
-                           void* dg, float* dh0, void* stream);
+                           void* dg, float* dh0, uint32_t* flags, void* stream);
 
 /* The linear product with its epilogue, z = x W + b, y = act(z) + r, and its backward dz = dy act'(z),
  * db = sum over rows of dz, dx = dz W^T, dW = x^T dz.  x (M, K), W (K, N), r, y, z, dy (M, N). */
