@@ -15,10 +15,12 @@
 //
 // One CTA a SM (or a pair of CTAs on two SMs, whose tile of 256 x 256 shares the operands between them) walks
 // output tiles; a warp issues the copies, one thread the products into one of two accumulators in tensor
-// memory, eight warps empty the other one through the epilogue.  Few tiles with a long sum are split along it,
+// memory, sixteen warps empty the other one through the epilogue.  Few tiles with a long sum are split along it,
 // and a second launch adds the parts in a fixed order.
 #include <cooperative_groups.h>
 #include <cuda.h>
+
+#include <type_traits>
 
 #include "gdn2_common.cuh"
 
@@ -28,10 +30,10 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kBK = 64;                 // values of the summed dimension in a stage: 128 bytes of bf16
-constexpr int kEpiWarps = 8;
+constexpr int kEpiWarps = 16;
 constexpr int kGemmThreads = 32 * (kEpiWarps + 2);
 constexpr int kStageRow = 128;          // bytes
-constexpr size_t kStagingBytes = kEpiWarps * 32 * 33 * sizeof(float);
+constexpr size_t kStagingBytes = kEpiWarps * 32 * 16 * sizeof(float);
 
 // How a result element leaves: y = act(v + bias) + residual, with v + bias kept in z.
 struct Epilogue {
@@ -45,6 +47,7 @@ struct Epilogue {
   float* parts;                         // not null: sums go here, (splits, rows, cols) fp32
   // the operands in fp32, for sums that are NaN; null: bf16 operands, whose sums are as they are
   const float *a, *b;
+  const float *az, *bz;                 // not null: that operand is times the slope of GELU at these
   long long a_row, a_k, b_col, b_k;     // element strides
 };
 
@@ -58,13 +61,12 @@ struct GemmParams {
 
 // ---- activation ---------------------------------------------------------------------------------
 constexpr float kGeluC = 0.7978845608028654f, kGeluA = 0.044715f;
-__device__ __forceinline__ float gelu(float z) {
-  const float t = tanhf(kGeluC * (z + kGeluA * z * z * z));
-  return 0.5f * z * (1.f + t);
-}
+// 0.5 z (1 + tanh u) = z / (1 + exp(-2 u)),  u = C (z + A z^3)
+__device__ __forceinline__ float gelu_gate(float z) { return __fdividef(1.f, 1.f + expf(-2.f * kGeluC * (z + kGeluA * z * z * z))); }
+__device__ __forceinline__ float gelu(float z) { return z * gelu_gate(z); }
 __device__ __forceinline__ float gelu_slope(float z) {
-  const float t = tanhf(kGeluC * (z + kGeluA * z * z * z));
-  return 0.5f * (1.f + t) + 0.5f * z * (1.f - t * t) * kGeluC * (1.f + 3.f * kGeluA * z * z);
+  const float s = gelu_gate(z);
+  return s + z * s * (1.f - s) * (2.f * kGeluC) * (1.f + 3.f * kGeluA * z * z);
 }
 
 __device__ __forceinline__ float load_f(const void* p, long long i, int bf16) {
@@ -78,7 +80,13 @@ __device__ __forceinline__ void store_f(void* p, long long i, int bf16, float v)
 // A sum that is NaN, again from the operands themselves.
 __device__ __noinline__ float plain_sum(const Epilogue& e, long long row, long long col, int k) {
   float s = 0.f;
-  for (int i = 0; i < k; ++i) s = fmaf(e.a[row * e.a_row + i * e.a_k], e.b[col * e.b_col + i * e.b_k], s);
+  for (int i = 0; i < k; ++i) {
+    const long long at = row * e.a_row + i * e.a_k, bt = col * e.b_col + i * e.b_k;
+    float x = e.a[at], y = e.b[bt];
+    if (e.az) x *= gelu_slope(e.az[at]);
+    if (e.bz) y *= gelu_slope(e.bz[bt]);
+    s = fmaf(x, y, s);
+  }
   return s;
 }
 
@@ -90,6 +98,50 @@ __device__ __forceinline__ void finish(const Epilogue& e, long long row, long lo
   if (e.act == GDN2_ACT_GELU_TANH) v = gelu(v);
   if (e.residual) v += load_f(e.residual, row * e.ldr + col, e.y_bf16);
   store_f(e.y, at, e.y_bf16, v);
+}
+
+// The same for eight rows, two apart, of a column; those from `rows` on are not there.  Loads come first.
+template <bool BF16>
+__device__ __forceinline__ void finish8(const Epilogue& e, float v[8], long long row, long long col, long long rows, int k,
+                                        float bias) {
+  using T = std::conditional_t<BF16, __nv_bfloat16, float>;
+  bool in[8];
+  float r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) in[i] = row + 2 * i < rows;
+  if (e.residual) {
+    const T* p = static_cast<const T*>(e.residual) + row * e.ldr + col;
+#pragma unroll
+    for (int i = 0; i < 8; ++i, p += 2 * e.ldr) r[i] = in[i] ? to_f<T>(*p) : 0.f;
+  }
+  if constexpr (!BF16) {
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) nan |= v[i] != v[i];
+    if (nan && e.a)
+      for (int i = 0; i < 8; ++i)
+        if (in[i] && v[i] != v[i]) v[i] = plain_sum(e, row + 2 * i, col, k);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] += bias;
+  if (e.z) {
+    T* p = static_cast<T*>(e.z) + row * e.ldy + col;
+#pragma unroll
+    for (int i = 0; i < 8; ++i, p += 2 * e.ldy)
+      if (in[i]) *p = static_cast<T>(v[i]);
+  }
+  if (e.act == GDN2_ACT_GELU_TANH) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = gelu(v[i]);
+  }
+  if (e.residual) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += r[i];
+  }
+  T* p = static_cast<T*>(e.y) + row * e.ldy + col;
+#pragma unroll
+  for (int i = 0; i < 8; ++i, p += 2 * e.ldy)
+    if (in[i]) *p = static_cast<T>(v[i]);
 }
 
 // ---- the product --------------------------------------------------------------------------------
@@ -322,10 +374,11 @@ __global__ void __launch_bounds__(kGemmThreads) linear_gemm_kernel(const __grid_
         }
       }
     }
-  } else {  // epilogue: warp w has rows 32 (w % 4).. and half w / 4 of the columns
-    constexpr int kHalf = G::kTileN / 2;
-    float* mine = staging + warp * 32 * 33;
-    const uint32_t col0 = (warp >> 2) * kHalf;
+  } else {  // epilogue: warp w has rows 32 (w % 4).. and quarter w / 4 of the columns
+    constexpr int kQuarter = G::kTileN / 4;
+    float* mine = staging + warp * 32 * 16;
+    const uint32_t col0 = (warp >> 2) * kQuarter;
+    const int half = lane >> 4, in = lane & 15;
     uint32_t acc = 0, acc_phase = 0;
     auto release = [&] {
       tc_fence_before();
@@ -344,53 +397,68 @@ __global__ void __launch_bounds__(kGemmThreads) linear_gemm_kernel(const __grid_
       const Work w = work_of(p, it);
       const long long row0 = (long long)w.tm * G::kTileM + rank * 128 + (warp & 3) * 32;
       const long long out0 = (long long)w.tn * G::kTileN + col0;
-      // 32 rows x 32 columns at a time: from rows to lanes through shared memory, so that a warp reads and
-      // writes 32 neighbouring columns of a row
+      if (p.ep.residual && row0 + lane < p.rows && out0 < p.cols) {  // on its way to L2 while the products run
+        const size_t el = P == 1 ? 2 : 4;
+        const char* r = static_cast<const char*>(p.ep.residual) + ((row0 + lane) * p.ep.ldr + out0) * el;
+        const int bytes = (int)(min((long long)kQuarter, p.cols - out0) * el);
+        for (int i = 0; i < bytes; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(r + i));
+      }
+      // 32 rows x 16 columns at a time: from rows to lanes through shared memory, so that a warp reads and writes 16
+      // neighbouring columns of two rows (columns permuted by the row there: no two lanes meet in a bank)
       auto put = [&](const float* v, int c) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) mine[lane * 33 + j] = v[j];
+        for (int j = 0; j < 16; ++j) mine[lane * 16 + (j ^ (lane >> 1))] = v[j];
         __syncwarp();
-        const long long col = out0 + c + lane;
+        const long long col = out0 + c + in;
         if (col < p.cols) {
-          const int n = (int)max(0ll, min(32ll, p.rows - row0));
-          if (p.ep.parts) {
-            float* q = p.ep.parts + ((long long)w.split * p.rows + row0) * p.cols + col;
-            for (int i = 0; i < n; ++i) q[(long long)i * p.cols] = mine[i * 33 + lane];
-          } else {
-            const float bias = p.ep.bias ? load_f(p.ep.bias, col, p.ep.bias_bf16) : 0.f;
-            for (int i = 0; i < n; ++i) finish(p.ep, row0 + i, col, mine[i * 33 + lane], p.k, bias);
+          const float bias = p.ep.bias && !p.ep.parts ? load_f(p.ep.bias, col, p.ep.bias_bf16) : 0.f;
+#pragma unroll
+          for (int i0 = half; i0 < 32; i0 += 16) {
+            float u[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) u[i] = mine[(i0 + 2 * i) * 16 + (in ^ ((i0 >> 1) + i))];
+            if (p.ep.parts) {
+              float* q = p.ep.parts + ((long long)w.split * p.rows + row0 + i0) * p.cols + col;
+#pragma unroll
+              for (int i = 0; i < 8; ++i, q += 2 * (long long)p.cols)
+                if (row0 + i0 + 2 * i < p.rows) *q = u[i];
+            } else {
+              finish8<P == 1>(p.ep, u, row0 + i0, col, p.rows, p.k, bias);
+            }
           }
         }
         __syncwarp();
       };
       if constexpr (P == 3) {
-        float sum[kHalf];
+        float sum[kQuarter];
 #pragma unroll
-        for (int j = 0; j < kHalf; ++j) sum[j] = 0.f;
+        for (int j = 0; j < kQuarter; ++j) sum[j] = 0.f;
         for (int kb = w.kb0; kb < w.kb1; ++kb) {
           bounded_wait(&acc_full[acc], acc_phase, dead, p.flags);
           __syncwarp();
           tc_fence_after();
 #pragma unroll
-          for (int c = 0; c < kHalf; c += 32) {
-            float v[32];
-            tmem_ld32(tmem + acc * G::kTileN, col0 + c, v);
+          for (int c = 0; c < kQuarter; c += 16) {
+            float v[16];
+            tmem_ld16(tmem + acc * G::kTileN, col0 + c, v);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) sum[c + j] += v[j];
+            for (int j = 0; j < 16; ++j) sum[c + j] += v[j];
           }
           release();
         }
 #pragma unroll
-        for (int c = 0; c < kHalf; c += 32) put(sum + c, c);
+        for (int c = 0; c < kQuarter; c += 16) put(sum + c, c);
       } else {
         bounded_wait(&acc_full[acc], acc_phase, dead, p.flags);
         __syncwarp();
         tc_fence_after();
-        for (int c = 0; c < kHalf; c += 32) {
+#pragma unroll
+        for (int c = 0; c < kQuarter; c += 32) {
           float v[32];
           tmem_ld32(tmem + acc * G::kTileN, col0 + c, v);
-          if (c + 32 == kHalf) release();
+          if (c + 32 == kQuarter) release();
           put(v, c);
+          put(v + 16, c + 16);
         }
       }
     }
@@ -450,8 +518,7 @@ __global__ void __launch_bounds__(256) linear_terms_kernel(const T* x, long long
 // dz = dy act'(z) (or dy) in the same form, and db's parts: a CTA takes 64 columns of `band` rows.
 template <class T, bool ACT>
 __global__ void __launch_bounds__(256) linear_dz_kernel(const T* dy, long long ld, const T* z, int rows, int cols, int band,
-                                                        int col_blocks, __nv_bfloat16* out, long long ldt, float* out32,
-                                                        float* parts) {
+                                                        int col_blocks, __nv_bfloat16* out, long long ldt, float* parts) {
   __shared__ float sums[8][64];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int in_band = blockIdx.x / col_blocks, c0 = (blockIdx.x - in_band * col_blocks) * 64, c = c0 + lane * 2;
@@ -466,7 +533,6 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const T* dy, long long l
         v[j] = to_f<T>(dy[r * ld + c + j]);
         if constexpr (ACT) v[j] *= gelu_slope(to_f<T>(z[r * cols + c + j]));
         s[j] += v[j];
-        if (out32) out32[r * cols + c + j] = v[j];
       }
     }
     if (out && c < ldt) {
@@ -748,7 +814,7 @@ FwdPlan plan_fwd(const gdn2_linear_desc* d, bool x_direct, bool w_direct) {
 constexpr int kBand = 256;              // rows of a CTA of the dz kernel
 struct BwdPlan {
   bool dz, x_terms, w_terms;            // dz: its own buffer (an activation, fp32, or rows not on 16 bytes)
-  size_t dz_at, dz32_at, w_at, x_at, db_at, parts_at, total;
+  size_t dz_at, w_at, x_at, db_at, parts_at, total;
 };
 BwdPlan plan_bwd(const gdn2_linear_desc* d, bool dx, bool dw, bool db, bool x_direct, bool w_direct, bool dy_direct) {
   BwdPlan b{};
@@ -756,8 +822,6 @@ BwdPlan plan_bwd(const gdn2_linear_desc* d, bool dx, bool dw, bool db, bool x_di
   auto take = [&](size_t n) { const size_t r = at; at += round256(n); return r; };
   b.dz = (dx || dw) && (!dy_direct || d->act != GDN2_ACT_NONE);
   if (b.dz) b.dz_at = take(terms_bytes(d, d->M, d->N));
-  // dz itself, for sums that are NaN
-  if (b.dz && d->dtype == GDN2_F32 && d->act != GDN2_ACT_NONE) b.dz32_at = take((size_t)d->M * d->N * 4);
   b.w_terms = dx && !w_direct;
   b.x_terms = dw && !x_direct;
   if (b.w_terms) b.w_at = take(terms_bytes(d, d->K, d->N));
@@ -890,7 +954,6 @@ extern "C" gdn2_status gdn2_linear_bwd(const gdn2_linear_desc* d, const void* x,
   const bool act = d->act != GDN2_ACT_NONE, bf16 = d->dtype == GDN2_BF16;
   const int terms = bf16 ? 1 : 3, bands = (d->M + kBand - 1) / kBand;
   const long long ldz = padded(d->N);
-  float* dz32 = b.dz && !bf16 && act ? reinterpret_cast<float*>(ws + b.dz32_at) : nullptr;
   cudaError_t e = cudaSuccess;
   if (b.dz || db) {
     const int col_blocks = (d->N + 63) / 64;
@@ -900,7 +963,7 @@ extern "C" gdn2_status gdn2_linear_bwd(const gdn2_linear_desc* d, const void* x,
     auto go = [&](auto kernel, auto t) {
       using T = decltype(t);
       kernel<<<grid, 256, 0, st>>>(static_cast<const T*>(dy), (long long)d->N, static_cast<const T*>(z), d->M, d->N, kBand,
-                                   col_blocks, out, ldz, dz32, parts);
+                                   col_blocks, out, ldz, parts);
     };
     if (bf16) act ? go(linear_dz_kernel<__nv_bfloat16, true>, __nv_bfloat16()) : go(linear_dz_kernel<__nv_bfloat16, false>, __nv_bfloat16());
     else act ? go(linear_dz_kernel<float, true>, 0.f) : go(linear_dz_kernel<float, false>, 0.f);
@@ -912,7 +975,8 @@ extern "C" gdn2_status gdn2_linear_bwd(const gdn2_linear_desc* d, const void* x,
   }
   const void* pz = b.dz ? static_cast<const void*>(ws + b.dz_at) : dy;
   const long long ldp = b.dz ? ldz : d->N, term_z = d->M * ldz;
-  const float* dz_plain = bf16 ? nullptr : act ? dz32 : static_cast<const float*>(dy);
+  const float* dz_plain = bf16 ? nullptr : static_cast<const float*>(dy);
+  const float* z_plain = bf16 || !act ? nullptr : static_cast<const float*>(z);
   float* parts = reinterpret_cast<float*>(ws + b.parts_at);
   if (dx && e == cudaSuccess) {
     Operand bo{w, d->K, d->N, d->w_stride, 0, false};
@@ -923,7 +987,7 @@ extern "C" gdn2_status gdn2_linear_bwd(const gdn2_linear_desc* d, const void* x,
     Epilogue ep{};
     ep.y = dx; ep.ldy = d->K; ep.y_bf16 = bf16;
     if (!bf16) {
-      ep.a = dz_plain; ep.a_row = d->N; ep.a_k = 1;
+      ep.a = dz_plain; ep.az = z_plain; ep.a_row = d->N; ep.a_k = 1;
       ep.b = static_cast<const float*>(w); ep.b_col = d->w_stride; ep.b_k = 1;
     }
     if (e == cudaSuccess) e = gemm({pz, d->M, d->N, ldp, term_z, false}, bo, terms, ep, d->M, d->K, d->N, parts, flags, st);
@@ -938,7 +1002,7 @@ extern "C" gdn2_status gdn2_linear_bwd(const gdn2_linear_desc* d, const void* x,
     ep.y = dw; ep.ldy = d->N; ep.y_bf16 = bf16;
     if (!bf16) {
       ep.a = static_cast<const float*>(x); ep.a_row = 1; ep.a_k = d->x_stride;
-      ep.b = dz_plain; ep.b_col = 1; ep.b_k = d->N;
+      ep.b = dz_plain; ep.bz = z_plain; ep.b_col = 1; ep.b_k = d->N;
     }
     if (e == cudaSuccess) e = gemm(a, {pz, d->M, d->N, ldp, term_z, true}, terms, ep, d->K, d->N, d->M, parts, flags, st);
   }
