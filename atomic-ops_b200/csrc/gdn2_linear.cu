@@ -61,8 +61,15 @@ struct GemmParams {
 
 // ---- activation ---------------------------------------------------------------------------------
 constexpr float kGeluC = 0.7978845608028654f, kGeluA = 0.044715f;
-// 0.5 z (1 + tanh u) = z / (1 + exp(-2 u)),  u = C (z + A z^3)
-__device__ __forceinline__ float gelu_gate(float z) { return __fdividef(1.f, 1.f + expf(-2.f * kGeluC * (z + kGeluA * z * z * z))); }
+// 0.5 z (1 + tanh u) = z / (1 + exp(-2 u)),  u = C (z + A z^3); the approximate exponential and reciprocal leave
+// about 2^-22 of the gate
+__device__ __forceinline__ float gelu_gate(float z) {
+  constexpr float kA = -2.f * kGeluC * 1.4426950408889634f, kB = kA * kGeluA;
+  float e, r;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(z * fmaf(kB * z, z, kA)));
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return r;
+}
 __device__ __forceinline__ float gelu(float z) { return z * gelu_gate(z); }
 __device__ __forceinline__ float gelu_slope(float z) {
   const float s = gelu_gate(z);
@@ -488,71 +495,103 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const float* parts, in
 }
 
 // ---- operands in the form that the copies need --------------------------------------------------
-// rows x cols of T with rows `ld` apart -> terms of bf16, rows `ldt` apart, terms rows * ldt apart: an fp32 matrix
-// in three terms, or a bf16 matrix whose rows are not on 16 bytes as it is.
+// Eight neighbouring values of a row, zeros past its end; `whole`: eight that may be read 16 bytes at a time.
 template <class T>
-__global__ void __launch_bounds__(256) linear_terms_kernel(const T* x, long long ld, int rows, int cols,
-                                                           __nv_bfloat16* out, long long ldt) {
-  const int per = (int)(ldt / 2);
-  const long long n = (long long)rows * per, term = rows * ldt;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
-    const long long r = i / per;
-    const int c = (int)(i - r * per) * 2;
-    float v[2];
-    for (int j = 0; j < 2; ++j) v[j] = c + j < cols ? to_f<T>(x[r * ld + c + j]) : 0.f;
-    __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(out + r * ldt + c);
-    if constexpr (sizeof(T) == 2) {
-      *o = __floats2bfloat162_rn(v[0], v[1]);
+__device__ __forceinline__ void load8(const T* p, float v[8], bool whole, int left) {
+  if (whole) {
+    if constexpr (sizeof(T) == 4) {
+      ld4(p, v);
+      ld4(p + 4, v + 4);
     } else {
+      const uint4 x = __ldg(reinterpret_cast<const uint4*>(p));
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-      for (int t = 0; t < 3; ++t) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(v[0], v[1]);
-        o[t * (term / 2)] = h;
-        v[0] -= __low2float(h);
-        v[1] -= __high2float(h);
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
       }
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < left ? ld1(p + i) : 0.f;
+  }
+}
+// Their terms: three of an fp32 value, `term` elements apart, or the bf16 value itself.
+template <class T>
+__device__ __forceinline__ void store_terms(__nv_bfloat16* o, long long term, float v[8]) {
+#pragma unroll
+  for (int t = 0; t < (sizeof(T) == 2 ? 1 : 3); ++t) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+      v[2 * i] -= __uint_as_float(w[i] << 16);
+      v[2 * i + 1] -= __uint_as_float(w[i] & 0xffff0000u);
+    }
+    *reinterpret_cast<uint4*>(o + t * term) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+template <class T>
+__device__ __forceinline__ bool by16(const T* p, long long ld) {
+  return ld % (16 / (int)sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+}
+
+// rows x cols of T with rows `ld` apart -> terms of bf16, rows `ldt` apart, terms rows * ldt apart: an fp32 matrix
+// in three terms, or a bf16 matrix whose rows are not on 16 bytes as it is.  Two matrices a launch.
+struct TermsJob {
+  const void* x;
+  __nv_bfloat16* out;
+  long long ld, ldt, items;             // items: groups of eight columns of all rows
+  int rows, cols;
+};
+template <class T>
+__global__ void __launch_bounds__(256) linear_terms_kernel(const __grid_constant__ TermsJob j0,
+                                                           const __grid_constant__ TermsJob j1) {
+  const long long all = j0.items + j1.items;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < all; i += gridDim.x * 256ll) {
+    const bool second = i >= j0.items;
+    const TermsJob& j = second ? j1 : j0;
+    const long long at = second ? i - j0.items : i, per = j.ldt / 8, r = at / per;
+    const int c = (int)(at - r * per) * 8;
+    const T* x = static_cast<const T*>(j.x) + r * j.ld + c;
+    float v[8];
+    load8<T>(x, v, c + 8 <= j.cols && by16(static_cast<const T*>(j.x), j.ld), j.cols - c);
+    store_terms<T>(j.out + r * j.ldt + c, (long long)j.rows * j.ldt, v);
   }
 }
 
-// dz = dy act'(z) (or dy) in the same form, and db's parts: a CTA takes 64 columns of `band` rows.
+// dz = dy act'(z) (or dy) in the same form, and db's parts: a CTA takes 64 columns of `band` rows, 8 threads beside
+// one another a row's.
 template <class T, bool ACT>
-__global__ void __launch_bounds__(256) linear_dz_kernel(const T* dy, long long ld, const T* z, int rows, int cols, int band,
-                                                        int col_blocks, __nv_bfloat16* out, long long ldt, float* parts) {
-  __shared__ float sums[8][64];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int in_band = blockIdx.x / col_blocks, c0 = (blockIdx.x - in_band * col_blocks) * 64, c = c0 + lane * 2;
+__global__ void __launch_bounds__(256) linear_dz_kernel(const T* dy, const T* z, int rows, int cols, int band, int col_blocks,
+                                                        __nv_bfloat16* out, long long ldt, float* parts) {
+  __shared__ float sums[32][64 + 4];
+  const int in_band = blockIdx.x / col_blocks, c0 = (blockIdx.x - in_band * col_blocks) * 64;
+  const int tc = (threadIdx.x & 7) * 8, tr = threadIdx.x >> 3, c = c0 + tc;
   const long long r0 = (long long)in_band * band, r1 = min((long long)rows, r0 + band), term = rows * ldt;
-  float s[2] = {0.f, 0.f};
-  for (long long r = r0 + warp; r < r1; r += 8) {
-    float v[2];
+  const bool whole = c + 8 <= cols && by16(dy, cols) && (!ACT || by16(z, cols));
+  float s[8] = {};
+#pragma unroll 2
+  for (long long r = r0 + tr; r < r1; r += 32) {
+    float v[8], u[8];
+    load8<T>(dy + r * cols + c, v, whole, cols - c);
+    if constexpr (ACT) {
+      load8<T>(z + r * cols + c, u, whole, cols - c);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      v[j] = 0.f;
-      if (c + j < cols) {
-        v[j] = to_f<T>(dy[r * ld + c + j]);
-        if constexpr (ACT) v[j] *= gelu_slope(to_f<T>(z[r * cols + c + j]));
-        s[j] += v[j];
-      }
+      for (int i = 0; i < 8; ++i) v[i] *= gelu_slope(u[i]);
     }
-    if (out && c < ldt) {
-      __nv_bfloat162* o = reinterpret_cast<__nv_bfloat162*>(out + r * ldt + c);
 #pragma unroll
-      for (int t = 0; t < (sizeof(T) == 2 ? 1 : 3); ++t) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(v[0], v[1]);
-        o[t * (term / 2)] = h;
-        v[0] -= __low2float(h);
-        v[1] -= __high2float(h);
-      }
-    }
+    for (int i = 0; i < 8; ++i) s[i] += v[i];
+    if (out && c < ldt) store_terms<T>(out + r * ldt + c, term, v);
   }
   if (!parts) return;
-  sums[warp][lane * 2] = s[0];
-  sums[warp][lane * 2 + 1] = s[1];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sums[tr][tc + i] = s[i];
   __syncthreads();
   if (threadIdx.x < 64 && c0 + (int)threadIdx.x < cols) {
     float t = 0.f;
-    for (int i = 0; i < 8; ++i) t += sums[i][threadIdx.x];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) t += sums[i][threadIdx.x];
     parts[(long long)in_band * cols + c0 + threadIdx.x] = t;
   }
 }
@@ -694,21 +733,33 @@ constexpr int kSMs = 148;
 struct GemmPlan {
   int cg, tiles_m, tiles_n, kblocks, splits, per_split;
 };
-GemmPlan plan_gemm(long long rows, long long cols, long long k) {
+GemmPlan plan_gemm(long long rows, long long cols, long long k, int terms) {
+  const int terms_cost = terms == 3 ? 6 : 1;
   GemmPlan g{};
   g.kblocks = (int)((k + kBK - 1) / kBK);
-  auto tiles = [&](int t) { return ((rows + t - 1) / t) * ((cols + t - 1) / t); };
-  g.cg = tiles(256) >= 37 ? 2 : 1;
-  const int t = 128 * g.cg, workers = kSMs / g.cg;
-  g.tiles_m = (int)((rows + t - 1) / t);
-  g.tiles_n = (int)((cols + t - 1) / t);
-  const long long n = (long long)g.tiles_m * g.tiles_n;
-  g.splits = 1;
-  if (2 * n <= workers) {
-    long long s = workers / n;
-    if (s > g.kblocks / 4) s = g.kblocks / 4;
-    if (s > 16) s = 16;
-    if (s > 1) g.splits = (int)s;
+  // Single CTAs or pairs, by what the busiest SM has to do: a block of the sum takes a pair 512 cycles and a
+  // single CTA, which reads its operands from shared memory twice as often, about 320; an epilogue of 128 columns
+  // about 3000.  (bf16, 777 x 1001 x 2503: 22.5 us as 40 pairs, XX as 140 CTAs.)
+  long long best = 0;
+  for (int cg = 1; cg <= 2; ++cg) {
+    const int t = 128 * cg, workers = kSMs / cg;
+    const long long tm = (rows + t - 1) / t, tn = (cols + t - 1) / t, n = tm * tn;
+    long long s = 1;
+    if (2 * n <= workers) {
+      s = workers / n;
+      if (s > g.kblocks / 4) s = g.kblocks / 4;
+      if (s > 16) s = 16;
+      if (s < 1) s = 1;
+    }
+    const long long waves = (n * s + workers - 1) / workers, blocks = (g.kblocks + s - 1) / s;
+    const long long cost = waves * (blocks * (cg == 2 ? 512 : 320) * terms_cost + 3000 * cg);
+    if (cg == 1 || cost < best) {
+      best = cost;
+      g.cg = cg;
+      g.tiles_m = (int)tm;
+      g.tiles_n = (int)tn;
+      g.splits = (int)s;
+    }
   }
   g.per_split = (g.kblocks + g.splits - 1) / g.splits;
   g.splits = (g.kblocks + g.per_split - 1) / g.per_split;
@@ -743,7 +794,7 @@ cudaError_t launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmPa
 // One product; `parts` has parts_of() bytes.
 cudaError_t gemm(const Operand& a, const Operand& b, int terms, Epilogue ep, long long rows, long long cols, long long k,
                  float* parts, uint32_t* flags, cudaStream_t st) {
-  const GemmPlan g = plan_gemm(rows, cols, k);
+  const GemmPlan g = plan_gemm(rows, cols, k, terms);
   CUtensorMap ma, mb;
   if (!make_map(&ma, a, terms) || !make_map(&mb, b, terms)) return cudaErrorInvalidValue;
   GemmParams p{};
@@ -769,13 +820,16 @@ long long padded(long long n) { return (n + 7) / 8 * 8; }
 size_t terms_bytes(const gdn2_linear_desc* d, long long rows, long long cols) {
   return round256((size_t)rows * padded(cols) * 2 * (d->dtype == GDN2_F32 ? 3 : 1));
 }
-cudaError_t make_terms(const gdn2_linear_desc* d, const void* p, long long ld, long long rows, long long cols, void* to,
-                       cudaStream_t st) {
-  const long long ldt = padded(cols), want = (rows * (ldt / 2) + 255) / 256;
-  const unsigned grid = (unsigned)(want < kSMs * 16 ? want : kSMs * 16);
-  __nv_bfloat16* o = static_cast<__nv_bfloat16*>(to);
-  if (d->dtype == GDN2_F32) linear_terms_kernel<float><<<grid, 256, 0, st>>>(static_cast<const float*>(p), ld, (int)rows, (int)cols, o, ldt);
-  else linear_terms_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(p), ld, (int)rows, (int)cols, o, ldt);
+TermsJob terms_job(const void* p, long long ld, long long rows, long long cols, void* to) {
+  const long long ldt = padded(cols);
+  return {p, static_cast<__nv_bfloat16*>(to), ld, ldt, rows * (ldt / 8), (int)rows, (int)cols};
+}
+cudaError_t make_terms(const gdn2_linear_desc* d, const TermsJob& a, const TermsJob& b, cudaStream_t st) {
+  const long long want = (a.items + b.items + 255) / 256;
+  if (!want) return cudaSuccess;
+  const unsigned grid = (unsigned)(want < kSMs * 32 ? want : kSMs * 32);
+  if (d->dtype == GDN2_F32) linear_terms_kernel<float><<<grid, 256, 0, st>>>(a, b);
+  else linear_terms_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a, b);
   return cudaGetLastError();
 }
 
@@ -807,7 +861,7 @@ FwdPlan plan_fwd(const gdn2_linear_desc* d, bool x_direct, bool w_direct) {
   f.w_terms = !w_direct;
   f.w_at = f.x_terms ? terms_bytes(d, d->M, d->K) : 0;
   f.parts_at = f.w_at + (f.w_terms ? terms_bytes(d, d->K, d->N) : 0);
-  f.total = f.parts_at + parts_of(plan_gemm(d->M, d->N, d->K), d->M, d->N);
+  f.total = f.parts_at + parts_of(plan_gemm(d->M, d->N, d->K, d->dtype == GDN2_F32 ? 3 : 1), d->M, d->N);
   return f;
 }
 
@@ -829,9 +883,10 @@ BwdPlan plan_bwd(const gdn2_linear_desc* d, bool dx, bool dw, bool db, bool x_di
   if (db) b.db_at = take((size_t)((d->M + kBand - 1) / kBand) * d->N * 4);
   b.parts_at = at;
   size_t parts = 0;
-  if (dx) parts = parts_of(plan_gemm(d->M, d->K, d->N), d->M, d->K);
+  const int terms = d->dtype == GDN2_F32 ? 3 : 1;
+  if (dx) parts = parts_of(plan_gemm(d->M, d->K, d->N, terms), d->M, d->K);
   if (dw) {
-    const size_t q = parts_of(plan_gemm(d->K, d->N, d->M), d->K, d->N);
+    const size_t q = parts_of(plan_gemm(d->K, d->N, d->M, terms), d->K, d->N);
     if (q > parts) parts = q;
   }
   b.total = at + parts;
@@ -914,14 +969,16 @@ extern "C" gdn2_status gdn2_linear_fwd(const gdn2_linear_desc* d, const void* x,
       ep.b = static_cast<const float*>(w); ep.b_col = 1; ep.b_k = d->w_stride;
     }
     Operand a{x, d->M, d->K, d->x_stride, 0, false}, b{w, d->K, d->N, d->w_stride, 0, true};
+    TermsJob jx{}, jw{};
     if (f.x_terms) {
-      e = make_terms(d, x, d->x_stride, d->M, d->K, ws + f.x_at, st);
+      jx = terms_job(x, d->x_stride, d->M, d->K, ws + f.x_at);
       a.p = ws + f.x_at; a.ld = padded(d->K); a.term = d->M * a.ld;
     }
-    if (f.w_terms && e == cudaSuccess) {
-      e = make_terms(d, w, d->w_stride, d->K, d->N, ws + f.w_at, st);
+    if (f.w_terms) {
+      jw = terms_job(w, d->w_stride, d->K, d->N, ws + f.w_at);
       b.p = ws + f.w_at; b.ld = padded(d->N); b.term = d->K * b.ld;
     }
+    e = make_terms(d, jx, jw, st);
     if (e == cudaSuccess)
       e = gemm(a, b, terms, ep, d->M, d->N, d->K, reinterpret_cast<float*>(ws + f.parts_at), flags, st);
   }
@@ -962,8 +1019,8 @@ extern "C" gdn2_status gdn2_linear_bwd(const gdn2_linear_desc* d, const void* x,
     float* parts = db ? reinterpret_cast<float*>(ws + b.db_at) : nullptr;
     auto go = [&](auto kernel, auto t) {
       using T = decltype(t);
-      kernel<<<grid, 256, 0, st>>>(static_cast<const T*>(dy), (long long)d->N, static_cast<const T*>(z), d->M, d->N, kBand,
-                                   col_blocks, out, ldz, parts);
+      kernel<<<grid, 256, 0, st>>>(static_cast<const T*>(dy), static_cast<const T*>(z), d->M, d->N, kBand, col_blocks, out, ldz,
+                                   parts);
     };
     if (bf16) act ? go(linear_dz_kernel<__nv_bfloat16, true>, __nv_bfloat16()) : go(linear_dz_kernel<__nv_bfloat16, false>, __nv_bfloat16());
     else act ? go(linear_dz_kernel<float, true>, 0.f) : go(linear_dz_kernel<float, false>, 0.f);
@@ -978,10 +1035,12 @@ extern "C" gdn2_status gdn2_linear_bwd(const gdn2_linear_desc* d, const void* x,
   const float* dz_plain = bf16 ? nullptr : static_cast<const float*>(dy);
   const float* z_plain = bf16 || !act ? nullptr : static_cast<const float*>(z);
   float* parts = reinterpret_cast<float*>(ws + b.parts_at);
+  if (e == cudaSuccess)
+    e = make_terms(d, b.x_terms ? terms_job(x, d->x_stride, d->M, d->K, ws + b.x_at) : TermsJob{},
+                   b.w_terms ? terms_job(w, d->w_stride, d->K, d->N, ws + b.w_at) : TermsJob{}, st);
   if (dx && e == cudaSuccess) {
     Operand bo{w, d->K, d->N, d->w_stride, 0, false};
     if (b.w_terms) {
-      e = make_terms(d, w, d->w_stride, d->K, d->N, ws + b.w_at, st);
       bo.p = ws + b.w_at; bo.ld = padded(d->N); bo.term = d->K * bo.ld;
     }
     Epilogue ep{};
@@ -995,7 +1054,6 @@ extern "C" gdn2_status gdn2_linear_bwd(const gdn2_linear_desc* d, const void* x,
   if (dw && e == cudaSuccess) {
     Operand a{x, d->M, d->K, d->x_stride, 0, true};
     if (b.x_terms) {
-      e = make_terms(d, x, d->x_stride, d->M, d->K, ws + b.x_at, st);
       a.p = ws + b.x_at; a.ld = padded(d->K); a.term = d->M * a.ld;
     }
     Epilogue ep{};
