@@ -107,19 +107,19 @@ __device__ __forceinline__ void finish(const Epilogue& e, long long row, long lo
   store_f(e.y, at, e.y_bf16, v);
 }
 
-// The same for eight rows, two apart, of a column; those from `rows` on are not there.  Loads come first.
-template <bool BF16>
+// The same for eight rows, STEP apart, of a column; those from `rows` on are not there.  Loads come first.
+template <bool BF16, int STEP>
 __device__ __forceinline__ void finish8(const Epilogue& e, float v[8], long long row, long long col, long long rows, int k,
                                         float bias) {
   using T = std::conditional_t<BF16, __nv_bfloat16, float>;
   bool in[8];
   float r[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) in[i] = row + 2 * i < rows;
+  for (int i = 0; i < 8; ++i) in[i] = row + STEP * i < rows;
   if (e.residual) {
     const T* p = static_cast<const T*>(e.residual) + row * e.ldr + col;
 #pragma unroll
-    for (int i = 0; i < 8; ++i, p += 2 * e.ldr) r[i] = in[i] ? to_f<T>(*p) : 0.f;
+    for (int i = 0; i < 8; ++i, p += STEP * e.ldr) r[i] = in[i] ? to_f<T>(*p) : 0.f;
   }
   if constexpr (!BF16) {
     bool nan = false;
@@ -127,14 +127,14 @@ __device__ __forceinline__ void finish8(const Epilogue& e, float v[8], long long
     for (int i = 0; i < 8; ++i) nan |= v[i] != v[i];
     if (nan && e.a)
       for (int i = 0; i < 8; ++i)
-        if (in[i] && v[i] != v[i]) v[i] = plain_sum(e, row + 2 * i, col, k);
+        if (in[i] && v[i] != v[i]) v[i] = plain_sum(e, row + STEP * i, col, k);
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] += bias;
   if (e.z) {
     T* p = static_cast<T*>(e.z) + row * e.ldy + col;
 #pragma unroll
-    for (int i = 0; i < 8; ++i, p += 2 * e.ldy)
+    for (int i = 0; i < 8; ++i, p += STEP * e.ldy)
       if (in[i]) *p = static_cast<T>(v[i]);
   }
   if (e.act == GDN2_ACT_GELU_TANH) {
@@ -147,7 +147,7 @@ __device__ __forceinline__ void finish8(const Epilogue& e, float v[8], long long
   }
   T* p = static_cast<T*>(e.y) + row * e.ldy + col;
 #pragma unroll
-  for (int i = 0; i < 8; ++i, p += 2 * e.ldy)
+  for (int i = 0; i < 8; ++i, p += STEP * e.ldy)
     if (in[i]) *p = static_cast<T>(v[i]);
 }
 
@@ -260,6 +260,8 @@ __global__ void __launch_bounds__(kGemmThreads) linear_gemm_kernel(const __grid_
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = CG == 2 ? blockIdx.x & 1 : 0;
   if (threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_a) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_b) : "memory");
     for (int i = 0; i < G::kStages; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
@@ -285,6 +287,7 @@ __global__ void __launch_bounds__(kGemmThreads) linear_gemm_kernel(const __grid_
   __syncthreads();
   if constexpr (CG == 2) cg::this_cluster().sync();
   tc_fence_after();
+  pdl_enter();                          // from here on what the kernel before wrote is read
   const uint32_t tmem = *tmem_at;
   const int items = p.tiles_m * p.tiles_n * p.splits, stride = gridDim.x / CG;
   const uint32_t group = P * 8192;      // 64 values across the sum of all terms, contiguous across
@@ -430,7 +433,7 @@ __global__ void __launch_bounds__(kGemmThreads) linear_gemm_kernel(const __grid_
               for (int i = 0; i < 8; ++i, q += 2 * (long long)p.cols)
                 if (row0 + i0 + 2 * i < p.rows) *q = u[i];
             } else {
-              finish8<P == 1>(p.ep, u, row0 + i0, col, p.rows, p.k, bias);
+              finish8<P == 1, 2>(p.ep, u, row0 + i0, col, p.rows, p.k, bias);
             }
           }
         }
@@ -482,16 +485,25 @@ __global__ void __launch_bounds__(kGemmThreads) linear_gemm_kernel(const __grid_
   }
 }
 
-// Adds the parts of a split sum in their order and finishes.
+// Adds the parts of a split sum in their order and finishes: 32 neighbouring columns to a warp, four rows to a thread.
+template <bool BF16>
 __global__ void __launch_bounds__(256) linear_join_kernel(const float* parts, int splits, int rows, int cols, int k,
-                                                          const __grid_constant__ Epilogue e) {
+                                                          int col_blocks, const __grid_constant__ Epilogue e) {
+  pdl_enter();
   const long long n = (long long)rows * cols;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
-    float v = parts[i];
-    for (int s = 1; s < splits; ++s) v += parts[s * n + i];
-    const long long row = i / cols, col = i - row * cols;
-    finish(e, row, col, v, k, e.bias ? load_f(e.bias, col, e.bias_bf16) : 0.f);
+  const int block = blockIdx.x / col_blocks;
+  const long long row = block * 64ll + (threadIdx.x >> 5), col = (blockIdx.x - block * col_blocks) * 32ll + (threadIdx.x & 31);
+  if (col >= cols) return;
+  const float* q = parts + row * cols + col;
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = row + 8 * i < rows ? q[8ll * i * cols] : 0.f;
+  for (int s = 1; s < splits; ++s) {
+    q += n;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += row + 8 * i < rows ? q[8ll * i * cols] : 0.f;
   }
+  finish8<BF16, 8>(e, v, row, col, rows, k, e.bias ? load_f(e.bias, col, e.bias_bf16) : 0.f);
 }
 
 // ---- operands in the form that the copies need --------------------------------------------------
@@ -571,7 +583,7 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const T* dy, const T* z,
   const long long r0 = (long long)in_band * band, r1 = min((long long)rows, r0 + band), term = rows * ldt;
   const bool whole = c + 8 <= cols && by16(dy, cols) && (!ACT || by16(z, cols));
   float s[8] = {};
-#pragma unroll 2
+#pragma unroll(ACT ? 2 : 4)
   for (long long r = r0 + tr; r < r1; r += 32) {
     float v[8], u[8];
     load8<T>(dy + r * cols + c, v, whole, cols - c);
@@ -595,11 +607,20 @@ __global__ void __launch_bounds__(256) linear_dz_kernel(const T* dy, const T* z,
     parts[(long long)in_band * cols + c0 + threadIdx.x] = t;
   }
 }
+// The bands' sums of a column: 32 columns to a CTA, eight threads to a column.
 __global__ void __launch_bounds__(256) linear_db_kernel(const float* parts, int bands, int cols, void* db, int bf16) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= cols) return;
+  __shared__ float sums[8][32];
+  pdl_enter();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   float s = 0.f;
-  for (int i = 0; i < bands; ++i) s += parts[(long long)i * cols + c];
+  if (c < cols)
+#pragma unroll 4
+    for (int i = warp; i < bands; i += 8) s += parts[(long long)i * cols + c];
+  sums[warp][lane] = s;
+  __syncthreads();
+  if (warp || c >= cols) return;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) s += sums[i][lane];
   store_f(db, c, bf16, s);
 }
 
@@ -782,12 +803,14 @@ cudaError_t launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmPa
   cfg.blockDim = dim3(kGemmThreads);
   cfg.dynamicSmemBytes = G::kSmem;
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = CG;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, linear_gemm_kernel<CG, P>, a, b, p);
 }
 
@@ -807,9 +830,12 @@ cudaError_t gemm(const Operand& a, const Operand& b, int terms, Epilogue ep, lon
   cudaError_t e = g.cg == 2 ? (terms == 3 ? launch_gemm<2, 3>(ma, mb, p, st) : launch_gemm<2, 1>(ma, mb, p, st))
                             : (terms == 3 ? launch_gemm<1, 3>(ma, mb, p, st) : launch_gemm<1, 1>(ma, mb, p, st));
   if (e != cudaSuccess || g.splits == 1) return e;
-  const long long n = rows * cols, want = (n + 255) / 256;
-  linear_join_kernel<<<(unsigned)(want < kSMs * 16 ? want : kSMs * 16), 256, 0, st>>>(parts, g.splits, p.rows, p.cols, p.k, ep);
-  return cudaGetLastError();
+  const int col_blocks = (int)((cols + 31) / 32);
+  const unsigned grid = (unsigned)(col_blocks * ((rows + 63) / 64));
+  return terms == 1 ? launch_pdl(linear_join_kernel<true>, grid, 256, 0, st, static_cast<const float*>(parts), g.splits, p.rows,
+                                 p.cols, p.k, col_blocks, ep)
+                    : launch_pdl(linear_join_kernel<false>, grid, 256, 0, st, static_cast<const float*>(parts), g.splits, p.rows,
+                                 p.cols, p.k, col_blocks, ep);
 }
 
 // Where an operand's terms go, and whether it needs them at all.
@@ -1026,8 +1052,8 @@ extern "C" gdn2_status gdn2_linear_bwd(const gdn2_linear_desc* d, const void* x,
     else act ? go(linear_dz_kernel<float, true>, 0.f) : go(linear_dz_kernel<float, false>, 0.f);
     e = cudaGetLastError();
     if (db && e == cudaSuccess) {
-      linear_db_kernel<<<(d->N + 255) / 256, 256, 0, st>>>(parts, bands, d->N, db, d->bias_dtype == GDN2_BF16);
-      e = cudaGetLastError();
+      e = launch_pdl(linear_db_kernel, (unsigned)((d->N + 31) / 32), 256, 0, st, static_cast<const float*>(parts), bands, d->N, db,
+                     (int)(d->bias_dtype == GDN2_BF16));
     }
   }
   const void* pz = b.dz ? static_cast<const void*>(ws + b.dz_at) : dy;
