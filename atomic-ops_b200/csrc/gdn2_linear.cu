@@ -33,7 +33,6 @@ constexpr int kBK = 64;                 // values of the summed dimension in a s
 constexpr int kEpiWarps = 16;
 constexpr int kGemmThreads = 32 * (kEpiWarps + 2);
 constexpr int kStageRow = 128;          // bytes
-constexpr size_t kStagingBytes = kEpiWarps * 32 * 16 * sizeof(float);
 
 // How a result element leaves: y = act(v + bias) + residual, with v + bias kept in z.
 struct Epilogue {
@@ -56,6 +55,7 @@ struct GemmParams {
   int rows, cols, k;
   int tiles_m, tiles_n, splits, kblocks, per_split;   // per_split: k blocks of a split
   int a_mn, b_mn;                       // contiguous across the summed dimension
+  int pairs;                            // y, z and the residual may be read and written two bf16 values at a time
   uint32_t* flags;
 };
 
@@ -85,7 +85,7 @@ __device__ __forceinline__ void store_f(void* p, long long i, int bf16, float v)
 }
 
 // A sum that is NaN, again from the operands themselves.
-__device__ __noinline__ float plain_sum(const Epilogue& e, long long row, long long col, int k) {
+__device__ __forceinline__ float plain_sum(const Epilogue& e, long long row, long long col, int k) {
   float s = 0.f;
   for (int i = 0; i < k; ++i) {
     const long long at = row * e.a_row + i * e.a_k, bt = col * e.b_col + i * e.b_k;
@@ -106,49 +106,74 @@ __device__ __forceinline__ void finish(const Epilogue& e, long long row, long lo
   if (e.residual) v += load_f(e.residual, row * e.ldr + col, e.y_bf16);
   store_f(e.y, at, e.y_bf16, v);
 }
+// The rows of a column whose bit is set, `step` apart, whose sums are NaN.
+__device__ __noinline__ void again(const Epilogue& e, long long row, int step, long long col, uint32_t rows, int k, float bias) {
+  for (int i = 0; i < 8; ++i)
+    if ((rows >> i) & 1u) finish(e, row + i * step, col, __int_as_float(0x7fc00000), k, bias);
+}
 
-// The same for eight rows, STEP apart, of a column; those from `rows` on are not there.  Loads come first.
-template <bool BF16, int STEP>
-__device__ __forceinline__ void finish8(const Epilogue& e, float v[8], long long row, long long col, long long rows, int k,
-                                        float bias) {
-  using T = std::conditional_t<BF16, __nv_bfloat16, float>;
-  bool in[8];
-  float r[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) in[i] = row + STEP * i < rows;
+// W neighbouring values (1 or 2) of T.
+template <class T, int W>
+struct Values {
+  T x[W];
+};
+template <>
+struct alignas(4) Values<__nv_bfloat16, 2> {
+  __nv_bfloat16 x[2];
+};
+template <class T>
+__device__ __forceinline__ T narrow(float v) {
+  if constexpr (sizeof(T) == 2) return __float2bfloat16_rn(v);
+  else return v;
+}
+// The same for eight rows, STEP apart, of W columns; rows from `rows` on are not there (ALL: they all are).  Loads
+// come first.
+template <class T, int W, int STEP, bool ALL>
+__device__ __forceinline__ void finish8(const Epilogue& e, float (&v)[8][W], long long row, long long col, long long rows, int k,
+                                        const float (&bias)[W]) {
+  using Vec = Values<T, W>;
+  const int left = ALL ? 8 : (int)max(0ll, min(8ll, (rows - row + STEP - 1) / STEP));
+  Vec r[8];
   if (e.residual) {
     const T* p = static_cast<const T*>(e.residual) + row * e.ldr + col;
 #pragma unroll
-    for (int i = 0; i < 8; ++i, p += STEP * e.ldr) r[i] = in[i] ? to_f<T>(*p) : 0.f;
+    for (int i = 0; i < 8; ++i, p += STEP * e.ldr)
+      if (ALL || i < left) r[i] = *reinterpret_cast<const Vec*>(p);
   }
-  if constexpr (!BF16) {
-    bool nan = false;
+  uint32_t nan = 0;
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) nan |= v[i] != v[i];
-    if (nan && e.a)
-      for (int i = 0; i < 8; ++i)
-        if (in[i] && v[i] != v[i]) v[i] = plain_sum(e, row + STEP * i, col, k);
+    for (int i = 0; i < 8; ++i) nan |= (v[i][0] != v[i][0] && (ALL || i < left) ? 1u : 0u) << i;
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] += bias;
-  if (e.z) {
-    T* p = static_cast<T*>(e.z) + row * e.ldy + col;
+  for (int i = 0; i < 8; ++i)
 #pragma unroll
-    for (int i = 0; i < 8; ++i, p += STEP * e.ldy)
-      if (in[i]) *p = static_cast<T>(v[i]);
-  }
+    for (int j = 0; j < W; ++j) v[i][j] += bias[j];
+  auto put = [&](void* to) {
+    T* p = static_cast<T*>(to) + row * e.ldy + col;
+#pragma unroll
+    for (int i = 0; i < 8; ++i, p += STEP * e.ldy) {
+      Vec o;
+#pragma unroll
+      for (int j = 0; j < W; ++j) o.x[j] = narrow<T>(v[i][j]);
+      if (ALL || i < left) *reinterpret_cast<Vec*>(p) = o;
+    }
+  };
+  if (e.z) put(e.z);
   if (e.act == GDN2_ACT_GELU_TANH) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = gelu(v[i]);
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < W; ++j) v[i][j] = gelu(v[i][j]);
   }
   if (e.residual) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += r[i];
-  }
-  T* p = static_cast<T*>(e.y) + row * e.ldy + col;
+    for (int i = 0; i < 8; ++i)
 #pragma unroll
-  for (int i = 0; i < 8; ++i, p += STEP * e.ldy)
-    if (in[i]) *p = static_cast<T>(v[i]);
+      for (int j = 0; j < W; ++j) v[i][j] += to_f<T>(r[i].x[j]);
+  }
+  put(e.y);
+  if (nan && e.a) again(e, row, STEP, col, nan, k, bias[0]);
 }
 
 // ---- the product --------------------------------------------------------------------------------
@@ -157,9 +182,11 @@ struct Gemm {
   static constexpr int kTileM = 128 * CG, kTileN = 128 * CG;        // of the CTA or the pair
   static constexpr int kOperand = 128 * kStageRow;                  // a CTA's part of one term of A or of B
   static constexpr int kStage = 2 * P * kOperand;
-  static constexpr int kStages = P == 1 ? 6 : 2;
+  static constexpr int kStages = P == 1 ? 5 : 2;
   static constexpr int kTmem = 2 * kTileN;                          // two accumulators' columns
-  static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + kStagingBytes + 256;
+  static constexpr int kCols = P == 1 ? 32 : 16;                    // columns that a warp turns around at a time
+  static constexpr size_t kStaging = kEpiWarps * 32 * kCols * sizeof(float);
+  static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + kStaging + 256;
 };
 
 // A wait that ends: after kWaitCycles, or once another of this CTA's waits has run out.
@@ -250,7 +277,7 @@ __global__ void __launch_bounds__(kGemmThreads) linear_gemm_kernel(const __grid_
   extern __shared__ uint8_t raw[];
   uint8_t* stages = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
   float* staging = reinterpret_cast<float*>(stages + (size_t)G::kStages * G::kStage);
-  uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(staging) + kStagingBytes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(staging) + G::kStaging);
   uint64_t* empty = full + G::kStages;
   uint64_t* acc_full = empty + G::kStages;
   uint64_t* acc_empty = acc_full + 2;
@@ -386,7 +413,7 @@ __global__ void __launch_bounds__(kGemmThreads) linear_gemm_kernel(const __grid_
     }
   } else {  // epilogue: warp w has rows 32 (w % 4).. and quarter w / 4 of the columns
     constexpr int kQuarter = G::kTileN / 4;
-    float* mine = staging + warp * 32 * 16;
+    float* mine = staging + warp * 32 * G::kCols;
     const uint32_t col0 = (warp >> 2) * kQuarter;
     const int half = lane >> 4, in = lane & 15;
     uint32_t acc = 0, acc_phase = 0;
@@ -413,27 +440,59 @@ __global__ void __launch_bounds__(kGemmThreads) linear_gemm_kernel(const __grid_
         const int bytes = (int)(min((long long)kQuarter, p.cols - out0) * el);
         for (int i = 0; i < bytes; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(r + i));
       }
-      // 32 rows x 16 columns at a time: from rows to lanes through shared memory, so that a warp reads and writes 16
-      // neighbouring columns of two rows (columns permuted by the row there: no two lanes meet in a bank)
-      auto put = [&](const float* v, int c) {
+      // 32 rows x 16 or 32 columns at a time: from rows to lanes through shared memory, so that half a warp reads and
+      // writes 16 neighbouring columns (bf16: 16 pairs) of a row; permuted there by the row, so that no two lanes
+      // meet in a bank
+      const bool all_rows = row0 + 32 <= p.rows;
+      auto put = [&](const float* v, int c) __attribute__((always_inline)) {
+        using T = std::conditional_t<P == 1, __nv_bfloat16, float>;
+        constexpr int W = P == 1 ? 2 : 1, kRow = 16 * W;
+        using Pair = Values<float, W>;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) mine[lane * 16 + (j ^ (lane >> 1))] = v[j];
+        for (int j = 0; j < 16; ++j) {
+          Pair q;
+#pragma unroll
+          for (int u = 0; u < W; ++u) q.x[u] = v[W * j + u];
+          *reinterpret_cast<Pair*>(mine + lane * kRow + W * (j ^ (P == 1 ? lane & 15 : lane >> 1))) = q;
+        }
         __syncwarp();
-        const long long col = out0 + c + in;
+        const long long col = out0 + c + W * in;
         if (col < p.cols) {
-          const float bias = p.ep.bias && !p.ep.parts ? load_f(p.ep.bias, col, p.ep.bias_bf16) : 0.f;
+          float bias[W];
+#pragma unroll
+          for (int u = 0; u < W; ++u)
+            bias[u] = p.ep.bias && !p.ep.parts && col + u < p.cols ? load_f(p.ep.bias, col + u, p.ep.bias_bf16) : 0.f;
 #pragma unroll
           for (int i0 = half; i0 < 32; i0 += 16) {
-            float u[8];
+            float u[8][W];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) u[i] = mine[(i0 + 2 * i) * 16 + (in ^ ((i0 >> 1) + i))];
+            for (int i = 0; i < 8; ++i) {
+              const int r = i0 + 2 * i;
+              const Pair q = *reinterpret_cast<const Pair*>(mine + r * kRow + W * (in ^ (P == 1 ? r & 15 : r >> 1)));
+#pragma unroll
+              for (int x = 0; x < W; ++x) u[i][x] = q.x[x];
+            }
             if (p.ep.parts) {
               float* q = p.ep.parts + ((long long)w.split * p.rows + row0 + i0) * p.cols + col;
 #pragma unroll
               for (int i = 0; i < 8; ++i, q += 2 * (long long)p.cols)
-                if (row0 + i0 + 2 * i < p.rows) *q = u[i];
-            } else {
-              finish8<P == 1, 2>(p.ep, u, row0 + i0, col, p.rows, p.k, bias);
+                if (row0 + i0 + 2 * i < p.rows) {
+#pragma unroll
+                  for (int x = 0; x < W; ++x)
+                    if (col + x < p.cols) q[x] = u[i][x];
+                }
+            } else if (W == 1 || p.pairs) {
+              if (all_rows) finish8<T, W, 2, true>(p.ep, u, row0 + i0, col, p.rows, p.k, bias);
+              else finish8<T, W, 2, false>(p.ep, u, row0 + i0, col, p.rows, p.k, bias);
+            } else {  // rows that start on odd places: one column after the other
+#pragma unroll
+              for (int x = 0; x < W; ++x) {
+                float one[8][1];
+                const float b1[1] = {bias[x]};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) one[i][0] = u[i][x];
+                if (col + x < p.cols) finish8<T, 1, 2, false>(p.ep, one, row0 + i0, col + x, p.rows, p.k, b1);
+              }
             }
           }
         }
@@ -443,7 +502,7 @@ __global__ void __launch_bounds__(kGemmThreads) linear_gemm_kernel(const __grid_
         float sum[kQuarter];
 #pragma unroll
         for (int j = 0; j < kQuarter; ++j) sum[j] = 0.f;
-        for (int kb = w.kb0; kb < w.kb1; ++kb) {
+        for (int kb = w.kb0;; ++kb) {
           bounded_wait(&acc_full[acc], acc_phase, dead, p.flags);
           __syncwarp();
           tc_fence_after();
@@ -454,10 +513,19 @@ __global__ void __launch_bounds__(kGemmThreads) linear_gemm_kernel(const __grid_
 #pragma unroll
             for (int j = 0; j < 16; ++j) sum[c + j] += v[j];
           }
+          if (kb + 1 >= w.kb1) break;
           release();
         }
+        // the sums go back to the accumulator that they came from last: the epilogue needs the registers
 #pragma unroll
-        for (int c = 0; c < kQuarter; c += 16) put(sum + c, c);
+        for (int c = 0; c < kQuarter; c += 16) tmem_st16(tmem + acc * G::kTileN, col0 + c, sum + c);
+#pragma unroll 1
+        for (int c = 0; c < kQuarter; c += 16) {
+          float v[16];
+          tmem_ld16(tmem + acc * G::kTileN, col0 + c, v);
+          if (c + 16 == kQuarter) release();
+          put(v, c);
+        }
       } else {
         bounded_wait(&acc_full[acc], acc_phase, dead, p.flags);
         __syncwarp();
@@ -468,7 +536,6 @@ __global__ void __launch_bounds__(kGemmThreads) linear_gemm_kernel(const __grid_
           tmem_ld32(tmem + acc * G::kTileN, col0 + c, v);
           if (c + 32 == kQuarter) release();
           put(v, c);
-          put(v + 16, c + 16);
         }
       }
     }
@@ -495,15 +562,16 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const float* parts, in
   const long long row = block * 64ll + (threadIdx.x >> 5), col = (blockIdx.x - block * col_blocks) * 32ll + (threadIdx.x & 31);
   if (col >= cols) return;
   const float* q = parts + row * cols + col;
-  float v[8];
+  float v[8][1];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = row + 8 * i < rows ? q[8ll * i * cols] : 0.f;
+  for (int i = 0; i < 8; ++i) v[i][0] = row + 8 * i < rows ? q[8ll * i * cols] : 0.f;
   for (int s = 1; s < splits; ++s) {
     q += n;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += row + 8 * i < rows ? q[8ll * i * cols] : 0.f;
+    for (int i = 0; i < 8; ++i) v[i][0] += row + 8 * i < rows ? q[8ll * i * cols] : 0.f;
   }
-  finish8<BF16, 8>(e, v, row, col, rows, k, e.bias ? load_f(e.bias, col, e.bias_bf16) : 0.f);
+  const float bias[1] = {e.bias ? load_f(e.bias, col, e.bias_bf16) : 0.f};
+  finish8<std::conditional_t<BF16, __nv_bfloat16, float>, 1, 8, false>(e, v, row, col, rows, k, bias);
 }
 
 // ---- operands in the form that the copies need --------------------------------------------------
@@ -825,6 +893,8 @@ cudaError_t gemm(const Operand& a, const Operand& b, int terms, Epilogue ep, lon
   p.rows = (int)rows; p.cols = (int)cols; p.k = (int)k;
   p.tiles_m = g.tiles_m; p.tiles_n = g.tiles_n; p.splits = g.splits; p.kblocks = g.kblocks; p.per_split = g.per_split;
   p.a_mn = a.mn; p.b_mn = b.mn;
+  auto even = [](const void* q, long long ld) { return !q || (ld % 2 == 0 && reinterpret_cast<uintptr_t>(q) % 4 == 0); };
+  p.pairs = cols % 2 == 0 && even(ep.y, ep.ldy) && even(ep.z, ep.ldy) && even(ep.residual, ep.ldr);
   p.flags = flags;
   p.ep.parts = g.splits > 1 ? parts : nullptr;
   cudaError_t e = g.cg == 2 ? (terms == 3 ? launch_gemm<2, 3>(ma, mb, p, st) : launch_gemm<2, 1>(ma, mb, p, st))
