@@ -26,6 +26,7 @@ from . import _lib, pipeline
 from .recurrent import _check_flags, _int32, _overlap, _raw_stream
 
 _descs = {}
+_fast, _last = None, (None, None)
 
 
 def _readable(t: torch.Tensor) -> torch.Tensor:
@@ -132,6 +133,18 @@ def gated_scan(x: torch.Tensor, g: torch.Tensor, h0=None, *, lengths=None, reset
                be h0 itself, or without h_index overlap nothing of it
     Returns h (B, L, C) of x's type and last (B, C) fp32, the state after each sequence's last token.
     Differentiable in x, g and h0, but not with h_index or h_out: those are for answering."""
+    global _fast, _last
+    if isinstance(x, torch.Tensor) and x.is_cuda and pipeline._check_mode != "sync":
+        if _fast is None:                                        # the common call; None: it needs more than that
+            _fast = _lib.binding().gated_scan
+        dev, fl = _last
+        if dev != x.device:
+            _last = dev, fl = x.device, pipeline._host_flags(x.device)
+        r = _fast(x, g, h0, lengths, reset, h_index, h_out, fl.ptr)
+        if r is not None:
+            if any(fl.words):
+                _check_flags(fl, "gdn2_gated_fwd")
+            return r
     if not isinstance(x, torch.Tensor) or x.ndim != 3:
         raise ValueError("gated_scan: x must be a (B, L, C) tensor")
     if not isinstance(g, torch.Tensor) or g.shape != x.shape:

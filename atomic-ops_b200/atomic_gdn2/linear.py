@@ -24,6 +24,7 @@ from .recurrent import _check_flags, _raw_stream
 
 _ACTS = {None: 0, "gelu": 1}
 _descs = {}
+_fast, _last = None, (None, None)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -127,6 +128,18 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias=None, *, act=None, residu
     """act(x W + bias) + residual.  x (..., din) and weight (din, dout), both fp32 or both bf16, on one CUDA device,
     any strides; bias (dout) fp32 or bf16, or None; act None or "gelu" (tanh form); residual (..., dout) of x's
     type, or None.  Returns (..., dout) of x's type.  Differentiable (once) in all four."""
+    global _fast, _last
+    if isinstance(x, torch.Tensor) and x.is_cuda and act in _ACTS and pipeline._check_mode != "sync":
+        if _fast is None:                                        # the common call; None: it needs more than that
+            _fast = _lib.binding().linear
+        dev, fl = _last
+        if dev != x.device:
+            _last = dev, fl = x.device, pipeline._host_flags(x.device)
+        y = _fast(x, weight, bias, residual, _ACTS[act], fl.ptr)
+        if y is not None:
+            if any(fl.words):
+                _check_flags(fl, "gdn2_linear_fwd")
+            return y
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise RuntimeError("linear: x must be a CUDA tensor (the product runs only on the B200 kernels)")
     dt, shape, dev = x.dtype, x.shape, x.device

@@ -1,5 +1,5 @@
-// The short way from a Python call of a serving operator to its launch, and the optimizer's step, as a CPython
-// extension.
+// The short way from a Python call of an operator to its launch, with the backward of those that have one, and the
+// optimizer's step, as a CPython extension.
 //
 // A decode step's kernels take a few microseconds, less than the interpreter needs to look at the
 // tensors, allocate the outputs and pass the pointers on.  These functions do that for calls that need
@@ -9,11 +9,14 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty_like.h>
+#include <ATen/ops/zeros_like.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "gdn2_b200.h"
@@ -39,6 +42,7 @@ PyObject* pair(at::Tensor a, at::Tensor b) {
   PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(std::move(b)));
   return r;
 }
+float* floats(const at::Tensor& t) { return static_cast<float*>(t.data_ptr()); }
 gdn2_dtype dtype_of(at::ScalarType t) { return t == at::kBFloat16 ? GDN2_BF16 : GDN2_F32; }
 // Whether `dev` is the current device: the launch and its workspace go there.
 bool current(c10::Device dev) { return dev.index() == c10::cuda::current_device(); }
@@ -249,6 +253,266 @@ PyObject* beam_select(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- differentiable operators -----------------------------------------------------------------------
+// The common call of linear and gated_scan, their backward with it.  What the Python path does besides (other types,
+// copies, checks at once) it does; the results are the same.
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// Like plain(), for a tensor that may need a gradient; `grad` becomes true where it does.
+const at::Tensor* input(PyObject* o, bool& grad) {
+  if (!THPVariable_CheckExact(o)) return nullptr;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_cuda() || t.layout() != at::kStrided || t._fw_grad(0).defined()) return nullptr;
+  grad = grad || (t.requires_grad() && c10::GradMode::is_enabled());
+  return &t;
+}
+at::Tensor workspace(size_t bytes, c10::Device dev) {
+  if (!bytes) return {};
+  const int64_t size[1] = {(int64_t)bytes};
+  return fresh(size, at::kByte, dev);
+}
+const void* ptr(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+void* ptr(at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+cudaStream_t stream_of(c10::Device dev) { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
+// Gradients of a backward under create_graph: a second derivative raises.
+variable_list once(variable_list grads, const char* what) {
+  if (!c10::GradMode::is_enabled()) return grads;
+  for (auto& g : grads)
+    if (g.defined()) g = g.detach().requires_grad_(true);
+  auto node = std::make_shared<torch::autograd::DelayedError>(
+      std::string("trying to differentiate twice through ") + what + ", which has no second derivative", (int64_t)grads.size());
+  return (*node)(std::move(grads));
+}
+
+struct LinearCall {
+  gdn2_linear_desc d;
+  std::vector<int64_t> out;            // y's shape
+};
+at::Tensor linear_forward(const LinearCall& c, const at::Tensor& x, const at::Tensor& w, const at::Tensor& bias,
+                          const at::Tensor& res, at::Tensor* z, uint32_t* flags, gdn2_status& s) {
+  at::Tensor y = fresh(c.out, x.scalar_type(), x.device());
+  if (z) *z = fresh(c.out, x.scalar_type(), x.device());
+  at::Tensor ws = workspace(gdn2_linear_fwd_workspace_bytes(&c.d), x.device());
+  s = gdn2_linear_fwd(&c.d, x.data_ptr(), w.data_ptr(), ptr(bias), ptr(res), y.data_ptr(), z ? z->data_ptr() : nullptr, ptr(ws),
+                      flags, stream_of(x.device()));
+  return y;
+}
+struct LinearFn : torch::autograd::Function<LinearFn> {
+  // Of the inputs that may be missing only those that are there have an edge.
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const std::optional<at::Tensor>& bias,
+                            const std::optional<at::Tensor>& res, const LinearCall* c, uint32_t* flags) {
+    at::Tensor z;
+    gdn2_status s;
+    at::Tensor y = linear_forward(*c, x, w, bias.value_or(at::Tensor()), res.value_or(at::Tensor()), c->d.act ? &z : nullptr,
+                                  flags, s);
+    TORCH_CHECK(s == GDN2_OK, "gdn2_linear_fwd: ", gdn2_status_string(s));
+    ctx->save_for_backward({x, w, z});
+    auto& data = ctx->saved_data;
+    const gdn2_linear_desc& d = c->d;
+    data["desc"] = std::vector<int64_t>{d.M, d.K, d.N, d.dtype, d.bias_dtype, d.act, d.x_stride, d.w_stride,
+                                        bias.has_value(), res.has_value()};
+    data["flags"] = (int64_t) reinterpret_cast<intptr_t>(flags);
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &x = saved[0], &w = saved[1], &z = saved[2];
+    const auto v = ctx->saved_data["desc"].toIntVector();
+    gdn2_linear_desc d{(int32_t)v[0], (int32_t)v[1], (int32_t)v[2], (int32_t)v[3], (int32_t)v[4], (int32_t)v[5], v[6], v[7], 0};
+    const auto dev = x.device();
+    const c10::cuda::CUDAGuard guard(dev);
+    at::Tensor dy = grads[0].contiguous(), dx, dw, db;
+    if (!on16(dy)) dy = dy.clone();
+    if (ctx->needs_input_grad(0)) dx = fresh(x.sizes(), x.scalar_type(), dev);
+    if (ctx->needs_input_grad(1)) dw = fresh(w.sizes(), w.scalar_type(), dev);
+    const int64_t n[1] = {d.N};
+    const bool has_b = v[8], has_r = v[9];
+    if (has_b && ctx->needs_input_grad(2)) db = fresh(n, d.bias_dtype == GDN2_BF16 ? at::kBFloat16 : at::kFloat, dev);
+    const int32_t want = (dx.defined() ? 1 : 0) + (dw.defined() ? 2 : 0) + (db.defined() ? 4 : 0);
+    if (want) {
+      at::Tensor ws = workspace(gdn2_linear_bwd_workspace_bytes(&d, want), dev);
+      const gdn2_status s = gdn2_linear_bwd(&d, x.data_ptr(), w.data_ptr(), ptr(z), dy.data_ptr(), ptr(dx), ptr(dw), ptr(db),
+                                            ptr(ws), reinterpret_cast<uint32_t*>((intptr_t)ctx->saved_data["flags"].toInt()),
+                                            stream_of(dev));
+      TORCH_CHECK(s == GDN2_OK, "gdn2_linear_bwd: ", gdn2_status_string(s));
+    }
+    variable_list r{dx, dw, db, has_r && ctx->needs_input_grad(2 + has_b) ? grads[0] : at::Tensor(), at::Tensor(), at::Tensor()};
+    return once(std::move(r), "linear");
+  }
+};
+
+// linear(x, weight, bias, residual, act, flags)
+PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6) Py_RETURN_NONE;
+  bool grad = false;
+  const at::Tensor *x = input(a[0], grad), *w = input(a[1], grad);
+  if (!x || !w || w->dim() != 2 || x->dim() < 2) Py_RETURN_NONE;
+  const auto type = x->scalar_type();
+  const auto dev = x->device();
+  if ((type != at::kFloat && type != at::kBFloat16) || w->scalar_type() != type || !current(dev) || w->device() != dev ||
+      !on16(*x) || !on16(*w) || !(x->dim() == 2 || x->is_contiguous()))
+    Py_RETURN_NONE;
+  const int64_t K = w->size(0), N = w->size(1), last = x->dim() - 1;
+  if (x->size(last) != K || K < 1 || N < 1 || x->numel() < 1 || w->stride(1) != 1 || x->stride(last) != 1) Py_RETURN_NONE;
+  const int64_t M = x->numel() / K;
+  if (M >= (1 << 28) || K >= (1 << 28) || N >= (1 << 28)) Py_RETURN_NONE;
+  LinearCall c{};
+  c.d.M = (int32_t)M; c.d.K = (int32_t)K; c.d.N = (int32_t)N;
+  c.d.dtype = dtype_of(type);
+  c.d.act = (int32_t)PyLong_AsLong(a[4]);
+  c.d.x_stride = M > 1 && x->dim() == 2 ? x->stride(0) : K;
+  c.d.w_stride = K > 1 ? w->stride(0) : N;
+  if (c.d.x_stride < K || c.d.w_stride < N) Py_RETURN_NONE;
+  c.out = x->sizes().vec();
+  c.out[last] = N;
+  std::optional<at::Tensor> bias, res;
+  if (a[2] != Py_None) {
+    const at::Tensor* t = input(a[2], grad);
+    if (!t || t->device() != dev || t->dim() != 1 || t->size(0) != N || !t->is_contiguous() ||
+        (t->scalar_type() != at::kFloat && t->scalar_type() != at::kBFloat16))
+      Py_RETURN_NONE;
+    bias = *t;
+    c.d.bias_dtype = dtype_of(t->scalar_type());
+  }
+  if (a[3] != Py_None) {
+    const at::Tensor* t = input(a[3], grad);
+    if (!t || t->device() != dev || t->scalar_type() != type || t->sizes() != c10::IntArrayRef(c.out) || !t->is_contiguous())
+      Py_RETURN_NONE;
+    res = *t;
+    c.d.res_stride = N;
+  }
+  uint32_t* flags = static_cast<uint32_t*>(PyLong_AsVoidPtr(a[5]));
+  if (PyErr_Occurred()) return nullptr;
+  if (grad) return THPVariable_Wrap(LinearFn::apply(*x, *w, bias, res, &c, flags));
+  gdn2_status s;
+  at::Tensor y = linear_forward(c, *x, *w, bias.value_or(at::Tensor()), res.value_or(at::Tensor()), nullptr, flags, s);
+  if (s != GDN2_OK) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+gdn2_gated_desc gated_desc(const at::Tensor& x, const at::Tensor& g) {
+  gdn2_gated_desc d{};
+  d.B = (int32_t)x.size(0); d.L = (int32_t)x.size(1); d.C = (int32_t)x.size(2);
+  d.dtype = dtype_of(x.scalar_type());
+  for (int i = 0; i < 2; ++i) {
+    d.x_stride[i] = x.size(i) > 1 ? x.stride(i) : 0;
+    d.g_stride[i] = g.size(i) > 1 ? g.stride(i) : 0;
+  }
+  return d;
+}
+struct GatedMasks {
+  at::Tensor lengths, reset;
+};
+struct GatedFn : torch::autograd::Function<GatedFn> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& g, const std::optional<at::Tensor>& first,
+                               const GatedMasks* masks, uint32_t* flags) {
+    const auto dev = x.device();
+    const at::Tensor h0 = first.value_or(at::Tensor()), &lengths = masks->lengths, &reset = masks->reset;
+    gdn2_gated_desc d = gated_desc(x, g);
+    d.n_states = h0.defined() ? d.B : 0;
+    const int64_t state[2] = {d.B, d.C};
+    at::Tensor h = fresh(x.sizes(), x.scalar_type(), dev), last = fresh(state, at::kFloat, dev),
+               marks = workspace(gdn2_gated_marks_bytes(&d), dev);
+    const gdn2_status s = gdn2_gated_fwd(&d, x.data_ptr(), g.data_ptr(), static_cast<const float*>(ptr(h0)), nullptr,
+                                         static_cast<const int32_t*>(ptr(lengths)), static_cast<const uint8_t*>(ptr(reset)),
+                                         h.data_ptr(), floats(last), floats(marks), flags, stream_of(dev));
+    TORCH_CHECK(s == GDN2_OK, "gdn2_gated_fwd: ", gdn2_status_string(s));
+    ctx->save_for_backward({x, g, marks, lengths, reset});
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["h0"] = h0.defined();
+    ctx->saved_data["flags"] = (int64_t) reinterpret_cast<intptr_t>(flags);
+    return {h, last};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &x = saved[0], &g = saved[1], &marks = saved[2], &lengths = saved[3], &reset = saved[4];
+    const auto dev = x.device();
+    const c10::cuda::CUDAGuard guard(dev);
+    gdn2_gated_desc d = gated_desc(x, g);
+    at::Tensor dh = grads[0], dlast = grads[1], dx = fresh(x.sizes(), x.scalar_type(), dev), dg = fresh(x.sizes(), x.scalar_type(), dev), d0;
+    if (dh.defined()) {
+      dh = dh.contiguous();
+      if (reinterpret_cast<uintptr_t>(dh.data_ptr()) % 4) dh = dh.clone();
+    } else {
+      dh = at::zeros_like(dx);
+    }
+    if (dlast.defined()) dlast = dlast.contiguous();
+    const int64_t state[2] = {d.B, d.C};
+    if (ctx->saved_data["h0"].toBool() && ctx->needs_input_grad(2)) d0 = fresh(state, at::kFloat, dev);
+    const gdn2_status s = gdn2_gated_bwd(&d, x.data_ptr(), g.data_ptr(), static_cast<const int32_t*>(ptr(lengths)),
+                                         static_cast<const uint8_t*>(ptr(reset)), static_cast<const float*>(marks.data_ptr()),
+                                         dh.data_ptr(), static_cast<const float*>(ptr(dlast)), dx.data_ptr(), dg.data_ptr(),
+                                         static_cast<float*>(ptr(d0)),
+                                         reinterpret_cast<uint32_t*>((intptr_t)ctx->saved_data["flags"].toInt()), stream_of(dev));
+    TORCH_CHECK(s == GDN2_OK, "gdn2_gated_bwd: ", gdn2_status_string(s));
+    variable_list r{dx, dg, d0, at::Tensor(), at::Tensor()};
+    return once(std::move(r), "gated_scan");
+  }
+};
+
+// gated_scan(x, g, h0, lengths, reset, h_index, h_out, flags)
+PyObject* gated_scan(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8) Py_RETURN_NONE;
+  bool grad = false;
+  const at::Tensor *x = input(a[0], grad), *g = input(a[1], grad);
+  if (!x || !g || x->dim() != 3 || g->sizes() != x->sizes()) Py_RETURN_NONE;
+  const auto type = x->scalar_type();
+  const auto dev = x->device();
+  const int64_t B = x->size(0), L = x->size(1), C = x->size(2);
+  if ((type != at::kFloat && type != at::kBFloat16) || g->scalar_type() != type || g->device() != dev || !current(dev) || B < 1 ||
+      L < 1 || C < 1 || B >= (1 << 28) || L >= (1 << 30) || C >= (1 << 30))
+    Py_RETURN_NONE;
+  for (const at::Tensor* t : {x, g})
+    if ((C > 1 && t->stride(2) != 1) || reinterpret_cast<uintptr_t>(t->data_ptr()) % 4) Py_RETURN_NONE;
+  at::Tensor h0, ints[2], reset;       // ints: lengths, h_index
+  if (a[2] != Py_None) {
+    const at::Tensor* t = input(a[2], grad);
+    if (!t || t->device() != dev || t->scalar_type() != at::kFloat || t->dim() != 2 || !t->is_contiguous() || t->size(1) != C ||
+        t->size(0) < 1 || t->size(0) >= (1 << 30) || (a[5] == Py_None && t->size(0) != B))
+      Py_RETURN_NONE;
+    h0 = *t;
+  }
+  for (int i = 0; i < 2; ++i) {
+    PyObject* o = a[i ? 5 : 3];
+    if (o == Py_None) continue;
+    const at::Tensor* t = plain(o);
+    if (!t || t->device() != dev || t->scalar_type() != at::kInt || t->dim() != 1 || t->size(0) != B || !t->is_contiguous())
+      Py_RETURN_NONE;
+    ints[i] = *t;
+  }
+  if (a[4] != Py_None) {
+    const at::Tensor* t = plain(a[4]);
+    if (!t || t->device() != dev || t->scalar_type() != at::kBool || t->dim() != 2 || t->size(0) != B || t->size(1) != L ||
+        !t->is_contiguous())
+      Py_RETURN_NONE;
+    reset = *t;
+  }
+  uint32_t* flags = static_cast<uint32_t*>(PyLong_AsVoidPtr(a[7]));
+  if (PyErr_Occurred()) return nullptr;
+  if (a[6] != Py_None || (ints[1].defined() && (grad || !h0.defined()))) Py_RETURN_NONE;
+  if (grad) {
+    const GatedMasks masks{ints[0], reset};
+    auto r = GatedFn::apply(*x, *g, h0.defined() ? std::optional<at::Tensor>(h0) : std::nullopt, &masks, flags);
+    return pair(std::move(r[0]), std::move(r[1]));
+  }
+  gdn2_gated_desc d = gated_desc(*x, *g);
+  d.n_states = h0.defined() ? (int32_t)h0.size(0) : 0;
+  const int64_t state[2] = {B, C};
+  at::Tensor h = fresh(x->sizes(), type, dev), last = fresh(state, at::kFloat, dev);
+  const gdn2_status s =
+      gdn2_gated_fwd(&d, x->data_ptr(), g->data_ptr(), static_cast<const float*>(ptr(h0)), static_cast<const int32_t*>(ptr(ints[1])),
+                     static_cast<const int32_t*>(ptr(ints[0])), static_cast<const uint8_t*>(ptr(reset)), h.data_ptr(), floats(last),
+                     nullptr, flags, stream_of(dev));
+  if (s != GDN2_OK) Py_RETURN_NONE;
+  return pair(std::move(h), std::move(last));
+  END_HANDLE_TH_ERRORS
+}
+
 // ---- the optimizer ----------------------------------------------------------------------------------
 // Its step is one call over lists of tensors, so these are the whole host path, with errors of their own.
 
@@ -266,7 +530,6 @@ std::vector<at::Tensor> tensors(PyObject* list, const char* what) {
 void changed(const at::Tensor& t) {  // in place: autograd may have saved it
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
-float* floats(const at::Tensor& t) { return static_cast<float*>(t.data_ptr()); }
 // The codes or values of a moment: p's shape and order.
 void check_moment(const at::Tensor& t, const at::Tensor& p, at::ScalarType type, const char* what) {
   TORCH_CHECK_VALUE(t.device() == p.device() && t.scalar_type() == type && t.sizes() == p.sizes() &&
@@ -454,6 +717,8 @@ PyMethodDef methods[] = {
     {"recurrent", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(recurrent)), METH_FASTCALL, nullptr},
     {"w4_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(w4_linear)), METH_FASTCALL, nullptr},
     {"beam_select", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(beam_select)), METH_FASTCALL, nullptr},
+    {"linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(linear)), METH_FASTCALL, nullptr},
+    {"gated_scan", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(gated_scan)), METH_FASTCALL, nullptr},
     {"adamw_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(adamw_step)), METH_FASTCALL, nullptr},
     {"adamw_moments", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(adamw_moments)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};

@@ -17,18 +17,20 @@ import torch
 
 sys.path.insert(0, str(pathlib.Path(__file__).resolve().parent))
 import atomic_gdn2  # noqa: E402
-from atomic_gdn2 import linear  # noqa: E402
+from atomic_gdn2 import last_status, linear  # noqa: E402
 from training_ref import linear_ref  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
 
 
-@pytest.fixture(autouse=True)
-def _sync_checks():
-    atomic_gdn2.set_checks(True)
+@pytest.fixture(autouse=True, params=["binding", "python"])
+def _path(request):
+    """The common call through the compiled binding; with checks at once everything goes the Python way."""
+    atomic_gdn2.set_checks("async" if request.param == "binding" else "sync")
     yield
     atomic_gdn2.set_checks("async")
+    assert last_status() == 0
 
 
 def _close(y, ref, size, k, dtype, extra=0.0):
