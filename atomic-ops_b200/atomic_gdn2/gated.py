@@ -20,7 +20,6 @@ from __future__ import annotations
 import ctypes
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib, pipeline
 from .recurrent import _check_flags, _int32, _overlap, _raw_stream
@@ -94,7 +93,6 @@ class _Gated(torch.autograd.Function):
         return h, last
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dh, dlast):
         x, g, marks, lengths, reset = ctx.saved_tensors
         B, L, C = x.shape
@@ -106,7 +104,8 @@ class _Gated(torch.autograd.Function):
             d0 = None
             if th is not None:
                 d0 = (torch.zeros(B, C, device=dev) if dlast is None else dlast).to(th)
-            return torch.empty(B, L, C, dtype=tx, device=dev), torch.empty(B, L, C, dtype=tg, device=dev), d0, None, None
+            empty = [torch.empty(B, L, C, dtype=t, device=dev) for t in (tx, tg)]
+            return *pipeline._once("gated_scan", (*empty, d0)), None, None
         dh = torch.zeros(x.shape, dtype=x.dtype, device=dev) if dh is None else dh.to(x.dtype).contiguous()
         if dh.data_ptr() % 4:
             dh = dh.clone()
@@ -120,7 +119,7 @@ class _Gated(torch.autograd.Function):
                                             _raw_stream(dev.index))
         _lib.check(rc, "gdn2_gated_bwd")
         _check_flags(fl, "gdn2_gated_bwd")
-        return dx.to(tx), dg.to(tg), None if d0 is None else d0.to(th), None, None
+        return *pipeline._once("gated_scan", (dx.to(tx), dg.to(tg), None if d0 is None else d0.to(th))), None, None
 
 
 def gated_scan(x: torch.Tensor, g: torch.Tensor, h0=None, *, lengths=None, reset=None, h_index=None, h_out=None):

@@ -10,6 +10,8 @@ B200 layout choices (the arithmetic is the reference's):
 * the layer prologue (head split, L2 norms, sigmoid, softplus clamp, relayout to the operator's
   (B, H, L, D)) is one fused CUDA kernel over the projection output, and one for its backward
   (`prologue`, csrc/gdn2_prologue.cu);
+* with `linear_fn` (atomic_gdn2.linear) the four products run on the framework's own kernels, GELU and the
+  residuals in their epilogues; without it they are torch.addmm;
 * the operator is whatever `blr_fn` the caller passes (the CUDA operator from
   `make_blr_trainable` in production), exactly like the reference's `layer_fwd(x, p, blr_fn, ...)`.
 """
@@ -82,10 +84,11 @@ class GDN2Layer(torch.nn.Module):
     proj_w / proj_b = the q, k, v, w, b, g dense layers side by side; o_*, up_*, down_*."""
 
     def __init__(self, d_model: int, n_heads: int, d_head: int, expansion: int = 4, g_init: float = 0.05,
-                 generator=None, prologue_fn=None):
+                 generator=None, prologue_fn=None, linear_fn=None):
         super().__init__()
         self.n_heads, self.d_head = n_heads, d_head
         self.prologue_fn = prologue_fn or prologue
+        self.linear_fn = linear_fn
         dh = n_heads * d_head
         ws, bs = [], []
         for name in QKVWBG:
@@ -107,13 +110,21 @@ class GDN2Layer(torch.nn.Module):
         B, L, _ = x.shape
         H, D = self.n_heads, self.d_head
         h = lnorm(x)
-        y = torch.addmm(self.proj_b, h.reshape(B * L, -1), self.proj_w).view(B, L, -1)
+        if self.linear_fn is None:
+            y = torch.addmm(self.proj_b, h.reshape(B * L, -1), self.proj_w).view(B, L, -1)
+        else:
+            y = self.linear_fn(h, self.proj_w, self.proj_b)
         q, k, v, w, b, g = self.prologue_fn(y, H, D, cfg.g_max, l2norm_k)
         o, _ = blr_fn(q, k, v, w, b, g)
         o = o.to(x.dtype).permute(0, 2, 1, 3).reshape(B * L, H * D)
-        x = x + torch.addmm(self.o_b, o, self.o_w).view(B, L, -1)
-        h2 = F.gelu(torch.addmm(self.up_b, lnorm(x).reshape(B * L, -1), self.up_w), approximate="tanh")
-        x = x + torch.addmm(self.down_b, h2, self.down_w).view(B, L, -1)
+        if self.linear_fn is None:
+            x = x + torch.addmm(self.o_b, o, self.o_w).view(B, L, -1)
+            h2 = F.gelu(torch.addmm(self.up_b, lnorm(x).reshape(B * L, -1), self.up_w), approximate="tanh")
+            x = x + torch.addmm(self.down_b, h2, self.down_w).view(B, L, -1)
+        else:  # GELU and the residuals in the products' epilogues
+            x = self.linear_fn(o.view(B, L, -1), self.o_w, self.o_b, residual=x)
+            h2 = self.linear_fn(lnorm(x), self.up_w, self.up_b, act="gelu")
+            x = self.linear_fn(h2, self.down_w, self.down_b, residual=x)
         if not stats:
             return x
         from .domain import bk2_stat, half_span_from_g

@@ -17,7 +17,6 @@ from __future__ import annotations
 import ctypes
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib, pipeline
 from .recurrent import _check_flags, _raw_stream
@@ -97,7 +96,6 @@ class _Linear(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
         x, w, z = ctx.saved_tensors
         M, K, N, dev = x.shape[0], x.shape[1], w.shape[1], x.device
@@ -121,7 +119,7 @@ class _Linear(torch.autograd.Function):
             if rc:
                 _lib.check(rc, "gdn2_linear_bwd")
             _check_flags(fl, "gdn2_linear_bwd")
-        return dx, dw, db, dr, None
+        return *pipeline._once("linear", (dx, dw, db, dr)), None
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias=None, *, act=None, residual=None) -> torch.Tensor:

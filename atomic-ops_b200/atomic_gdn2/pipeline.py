@@ -132,6 +132,15 @@ def _refuse_gradients(what: str, tensors) -> None:
         raise RuntimeError(f"{what} has no forward-mode derivative: its inputs must not be dual tensors")
 
 
+def _once(what: str, grads: tuple) -> tuple:
+    """A backward's gradients; under create_graph a second derivative through them raises."""
+    if not torch.is_grad_enabled():
+        return grads
+    error = torch._C._functions.DelayedError(
+        f"trying to differentiate twice through {what}, which has no second derivative".encode(), len(grads))
+    return error(*[None if g is None else g.detach().requires_grad_(True) for g in grads])
+
+
 def _host_flags(dev: torch.device) -> _HostFlags:
     fl = _flags.get(dev.index)
     if fl is None:

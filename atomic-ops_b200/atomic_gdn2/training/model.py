@@ -21,16 +21,19 @@ def lm_config():
 class GDN2LM(torch.nn.Module):
     """init_model + model_fwd.  `blr_fn` defaults to the CUDA operator
     make_blr_trainable(cfg, 1/sqrt(d_head)) (model.py:13) and `prologue_fn` to the fused CUDA
-    prologue; CPU tests pass restatements of both."""
+    prologue; CPU tests pass restatements of both.  `linear_fn`: what multiplies (atomic_gdn2.linear), or
+    None for torch.addmm."""
 
     def __init__(self, cfg, d_model, n_heads, d_head, n_layers, vocab=256, expansion=4, g_init=0.05, seed=0,
-                 blr_fn=None, l2norm_k=True, prologue_fn=None):
+                 blr_fn=None, l2norm_k=True, prologue_fn=None, linear_fn=None):
         super().__init__()
+        self.linear_fn = linear_fn
         gen = torch.Generator().manual_seed(seed)
         self.cfg, self.l2norm_k = cfg, l2norm_k
         self.embed = torch.nn.Parameter(torch.randn(vocab, d_model, generator=gen) * 0.02)
         self.layers = torch.nn.ModuleList(
-            GDN2Layer(d_model, n_heads, d_head, expansion, g_init, generator=gen, prologue_fn=prologue_fn)
+            GDN2Layer(d_model, n_heads, d_head, expansion, g_init, generator=gen, prologue_fn=prologue_fn,
+                      linear_fn=linear_fn)
             for _ in range(n_layers))
         w, b = dense_init(d_model, vocab, generator=gen)
         self.head_w, self.head_b = torch.nn.Parameter(w), torch.nn.Parameter(b)
@@ -44,7 +47,10 @@ class GDN2LM(torch.nn.Module):
             x, s = r if stats else (r, None)
             st.append(s)
         B, L, d = x.shape
-        logits = torch.addmm(self.head_b, lnorm(x).reshape(B * L, d), self.head_w).view(B, L, -1)
+        if self.linear_fn is None:
+            logits = torch.addmm(self.head_b, lnorm(x).reshape(B * L, d), self.head_w).view(B, L, -1)
+        else:
+            logits = self.linear_fn(lnorm(x), self.head_w, self.head_b)
         return (logits, st) if stats else logits
 
 

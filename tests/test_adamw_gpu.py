@@ -112,3 +112,241 @@ def test_steps_equal_the_definition(dtypes, bits, clip, spike):
             if not p.numel():
                 opt.state[p]["step"].zero_()
         _same(opt, params, ref)
+
+
+def _train(opt, params, gen, n=3, scale=1.0):
+    for _ in range(n):
+        for p in params:
+            p.grad = (torch.randn(p.shape, generator=gen) * scale).to(p.dtype).cuda()
+        opt.step()
+
+
+def test_against_torch():
+    """The same weights as torch's AdamW after some steps (its order of operations differs: 2^-20 of a step each), and
+    either's state_dict loads into the other."""
+    a, gen = _model([torch.float32], 3)
+    b = [torch.nn.Parameter(p.detach().clone()) for p in a]
+    kw = dict(lr=1e-2, betas=(0.9, 0.99), eps=1e-8, weight_decay=0.05)
+    mine, theirs = AdamW(a, **kw), torch.optim.AdamW(b, **kw)
+    for k in range(6):
+        for p, q in zip(a, b):
+            p.grad = torch.randn(p.shape, generator=gen).cuda()
+            q.grad = p.grad.clone()
+        mine.step()
+        theirs.step()
+        for p, q in zip(a, b):
+            if p.numel():
+                assert float((p.detach() - q.detach()).abs().max()) < 7 * (2.0 ** -20 * 0.1 + 4 * U)
+        if k == 2:
+            s = copy.deepcopy(mine.state_dict())
+            mine.load_state_dict(theirs.state_dict())
+            theirs.load_state_dict(s)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_dict(bits):
+    params, gen = _model([torch.float32, torch.bfloat16], 4)
+    opt = AdamW(params, lr=1e-2, clip=1.0, state_bits=bits)
+    _train(opt, params, gen)
+    saved = copy.deepcopy(opt.state_dict())
+    twin = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    other = AdamW(twin, lr=1.0, clip=1.0, state_bits=bits)
+    other.load_state_dict(saved)
+    state = gen.get_state()
+    _train(opt, params, gen)
+    gen.set_state(state)
+    _train(other, twin, gen)
+    for p, q in zip(params, twin):
+        assert torch.equal(p, q)
+        for k, v in opt.state[p].items():
+            assert torch.equal(v, other.state[q][k]) and v.dtype == other.state[q][k].dtype
+    with pytest.raises(ValueError):
+        AdamW(twin, state_bits=40 - bits).load_state_dict(saved)
+
+
+def test_moments():
+    for bits in (8, 32):
+        params, gen = _model([torch.float32], 5)
+        params = [p for p in params if p.numel()]
+        opt = AdamW(params, state_bits=bits)
+        _train(opt, params, gen)
+        got = opt.moments()
+        for p, (m, v) in zip(params, got):
+            st = opt.state[p]
+            if bits == 8:
+                a, b = decode(st["exp_avg"].cpu(), st["exp_avg_scale"].cpu(), st["exp_avg_sq"].cpu(), st["exp_avg_sq_scale"].cpu())
+            else:
+                a, b = st["exp_avg"].cpu().flatten(), st["exp_avg_sq"].cpu().flatten()
+            assert m.shape == v.shape == p.shape and torch.equal(m.cpu().flatten(), a) and torch.equal(v.cpu().flatten(), b)
+        out = [(torch.zeros_like(p), torch.zeros_like(p)) for p in params[:2]]
+        assert opt.moments(params[:2], out=out) is out and torch.equal(out[1][0], got[1][0])
+        with pytest.raises(ValueError):
+            opt.moments(params, out=out)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_many_tensors(bits):
+    """More tensors than a table holds, with and without a norm."""
+    gen = torch.Generator().manual_seed(6)
+    sizes = [1 + (i * 37) % 700 for i in range(700)] + [20000]
+    for clip in (None, 1.0):
+        params = [torch.nn.Parameter(torch.randn(n, generator=gen).cuda()) for n in sizes]
+        opt = AdamW(params, lr=1e-2, clip=clip, state_bits=bits, weight_decay=0.1)
+        ref = Ref(params, bits, [0.1] * len(params), clip=clip)
+        for _ in range(2):
+            grads = [torch.randn(n, generator=gen) for n in sizes]
+            for p, g in zip(params, grads):
+                p.grad = g.cuda()
+            opt.step()
+            ref.step(grads)
+            if clip:
+                assert float(opt.grad_norm) == float(ref.norm)
+        _same(opt, params, ref)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_views_and_orders(bits, dtype):
+    """Weights that start anywhere, weights and gradients in other orders than each other's: every value takes its own step."""
+    gen = torch.Generator().manual_seed(7)
+    pool = torch.zeros(40000, dtype=dtype, device="cuda")
+    shapes, at, params = [(17, 31), (3000,), (90, 100), (4, 6, 10)], 1, []
+    for s in shapes:
+        n = math.prod(s)
+        params.append(torch.nn.Parameter(pool[at:at + n].view(s)))
+        at += n + 3
+    params[2] = torch.nn.Parameter(pool[at:at + 9000].view(100, 90).t())
+    opt = AdamW(params, lr=1e-2, clip=1.0, state_bits=bits)
+    order = lambda t: t.t() if t.shape == (90, 100) else t            # its memory's order
+    twins = [torch.nn.Parameter(order(p.detach()).contiguous().clone()) for p in params]
+    ref = Ref(twins, bits, [0.1] * 4, clip=1.0)
+    for _ in range(3):
+        grads = [torch.randn(s, generator=gen).to(dtype) for s in shapes]
+        for i, (p, g) in enumerate(zip(params, grads)):
+            g = g.cuda()
+            p.grad = g if i else g.t().contiguous().t()               # a gradient in another order
+        opt.step()
+        ref.step([order(g) for g in grads])
+    for i, p in enumerate(params):
+        far = ref.t[i] * (8 * U * 0.2 + 64 * U * 0.1 + (2.0 ** -7 * 0.2 if dtype == torch.bfloat16 else 0))
+        assert float((order(p.detach()).cpu().double() - ref.p[i].double()).abs().max()) <= far
+    assert bool((pool[0] == 0).all()) and bool((pool[at + 9000:] == 0).all())
+
+
+def test_guard():
+    """Steps that are not made: the weights, moments, counts and the mean stay; the norm is told."""
+    for bits in (32, 8):
+        for bad in ("nan", "inf", "loss", "spike"):
+            params, gen = _model([torch.float32], 8)
+            opt = AdamW(params, lr=1e-2, clip=1.0, spike_factor=4.0, state_bits=bits)
+            _train(opt, params, gen, 2)
+            before = [p.detach().clone() for p in params], copy.deepcopy(opt.state_dict()["state"]), opt.norm_mean
+            for p in params:
+                p.grad = torch.randn(p.shape, generator=gen).cuda() * (100.0 if bad == "spike" else 1.0)
+            if bad in ("nan", "inf"):
+                params[5].grad[77] = float(bad)
+            opt.step(loss=torch.tensor(float("nan") if bad == "loss" else 1.0, device="cuda"))
+            assert not bool(opt.step_made) and float(opt.norm_mean) == float(before[2])
+            assert math.isfinite(float(opt.grad_norm)) == (bad in ("loss", "spike"))
+            assert all(torch.equal(a, p) for a, p in zip(before[0], params))
+            for i, st in opt.state_dict()["state"].items():
+                assert all(torch.equal(v, before[1][i][k]) for k, v in st.items())
+            _train(opt, params, gen, 1)
+            assert bool(opt.step_made)
+    params, gen = _model([torch.float32], 9)                          # without clip or spike_factor only the loss counts
+    opt = AdamW(params, lr=1e-2)
+    _train(opt, params, gen, 1)
+    was = params[0].detach().clone()
+    opt.step(loss=torch.tensor(float("inf"), device="cuda"))
+    assert torch.equal(params[0], was) and not bool(opt.step_made)
+    params[0].grad.zero_()
+    params[4].grad.fill_(float("nan"))
+    opt.step()
+    assert bool(torch.isnan(params[4]).all()) and bool(torch.isfinite(params[0]).all())
+
+
+def test_zero_and_extreme_gradients():
+    """A gradient of zeros has norm zero; gradients whose squares fp32 cannot hold are clipped like others."""
+    for bits in (32, 8):
+        params, gen = _model([torch.float32], 10)
+        for scale in (0.0, 1e-30, 1e25):
+            opt = AdamW(params, lr=1e-3, clip=1.0, state_bits=bits, weight_decay=0.0)
+            grads = [torch.randn(p.shape, generator=gen) * scale for p in params]
+            for p, g in zip(params, grads):
+                p.grad = g.cuda()
+            was = [p.detach().clone() for p in params]
+            opt.step()
+            want = math.sqrt(sum(float((g.double() ** 2).sum()) for g in grads))
+            assert float(opt.grad_norm) == pytest.approx(want, rel=1e-6, abs=0.0) and bool(opt.step_made)
+            # a first step moves every weight by lr g / (|g| + eps): at most lr
+            assert all(float((p - a).abs().max()) <= 1.001e-3 + 4 * U for p, a in zip(params, was) if p.numel())
+            if scale == 0.0:
+                assert all(torch.equal(p, a) for p, a in zip(params, was))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_graph_and_streams(bits):
+    """A captured step, its rate in device memory, replays like eager steps; steps go to the current stream."""
+    params, gen = _model([torch.float32], 11)
+    twin = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    rate = torch.full((), 1e-2, device="cuda")
+    a, b = AdamW(params, lr=rate, clip=1.0, state_bits=bits), AdamW(twin, lr=1e-2, clip=1.0, state_bits=bits)
+    for p, q in zip(params, twin):
+        p.grad = torch.randn(p.shape, generator=gen).cuda()
+        q.grad = p.grad.clone()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="outside the capture"):
+        with torch.cuda.graph(graph):
+            a.step()
+    a.step()
+    b.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.step()
+    for k in range(3):
+        lr = 1e-2 / (k + 1)
+        rate.fill_(lr)
+        b.param_groups[0]["lr"] = float(torch.tensor(lr))             # what fp32 holds of it
+        for p, q in zip(params, twin):
+            q.grad.normal_(generator=torch.Generator(device="cuda").manual_seed(k))
+            p.grad.copy_(q.grad)
+        graph.replay()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(5_000_000)
+            b.step()
+        torch.cuda.current_stream().wait_stream(side)
+        assert all(torch.equal(p, q) for p, q in zip(params, twin))
+        assert float(a.grad_norm) == float(b.grad_norm) and float(a.state[params[0]]["step"]) == k + 2
+
+
+def test_refusals():
+    cuda = lambda *s, dtype=torch.float32: torch.nn.Parameter(torch.zeros(*s, device="cuda", dtype=dtype))
+    for p in (cuda(4, dtype=torch.float16), cuda(4, dtype=torch.float64), torch.nn.Parameter(torch.zeros(1, device="cuda").expand(5)),
+              torch.nn.Parameter(torch.zeros(8, device="cuda")[::2])):
+        p.grad = torch.zeros_like(p)
+        with pytest.raises(ValueError):
+            AdamW([p]).step()
+    p = cuda(6, 2)
+    p.grad = torch.zeros(6, 2, device="cuda").to_sparse()
+    with pytest.raises(ValueError):
+        AdamW([p]).step()
+    p.grad = torch.zeros(6, 2, device="cuda")
+    opt = AdamW([p], state_bits=8)
+    opt.step()
+    for name, bad in (("exp_avg", torch.zeros(6, 2, device="cuda")), ("exp_avg_scale", torch.zeros(2, device="cuda")),
+                      ("step", torch.zeros(())), ("exp_avg_sq", torch.zeros(3, 2, dtype=torch.uint8, device="cuda"))):
+        good = opt.state[p][name]
+        opt.state[p][name] = bad
+        with pytest.raises(ValueError):
+            opt.step()
+        opt.state[p][name] = good
+    with pytest.raises(ValueError):
+        opt.step(loss=torch.zeros(2, device="cuda"))
+    with pytest.raises(ValueError):
+        AdamW([p], lr=torch.zeros(2, device="cuda")).step()
+    version = p._version
+    opt.step()
+    assert p._version > version                                       # a change in place to autograd
+    assert float(opt.step(lambda: (p * 2).sum().detach() + 1.0)) == 1.0

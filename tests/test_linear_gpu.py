@@ -81,3 +81,191 @@ def test_gradients(M, K, N, act, dtype):
         _norm_close(a, g, (48 + k / 64 + 64) * U if dtype == torch.float32 else 3 * 2.0 ** -8)
     with torch.no_grad():
         assert torch.equal(linear(*leaves[:3], act=act, residual=leaves[3]), y)
+
+
+def _data(M, K, N, dtype=torch.float32, seed=0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    n = lambda *s: torch.randn(*s, generator=gen, device="cuda")
+    return [t.to(dtype) for t in (n(M, K), n(K, N) / math.sqrt(K), n(N), n(M, N), n(M, N))]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M", [3, 150])
+def test_strides_and_shapes(M, dtype):
+    """Views that the kernels read in place, views that they cannot, batches of rows, broadcast inputs, other bias types."""
+    K, N = 96, 72
+    x, w, b, r, dy = _data(M, K, N, dtype, M)
+    y_r = linear_ref(x.double(), w.double(), b.double(), "gelu", r.double())
+    wide = torch.zeros(M, K + 40, dtype=dtype, device="cuda")
+    wide[:, 8:8 + K] = x
+    odd = torch.zeros(M, K + 3, dtype=dtype, device="cuda")
+    odd[:, 1:1 + K] = x
+    size = x.double().abs() @ w.double().abs()
+    extra = 8 * U + 4 * U * (b.double().abs() + r.double().abs())
+    for x2 in (wide[:, 8:8 + K], odd[:, 1:1 + K], x.t().contiguous().t(), torch.stack([x, x], 2)[..., 0]):
+        for w2 in (w, w.t().contiguous().t(), torch.cat([w, w], 1)[:, :N], torch.cat([w, w[:, :3]], 1)[:, :N]):
+            for r2 in (r, torch.cat([r, r], 1)[:, N:], r.t().contiguous().t()):
+                leaves = [t.detach().requires_grad_(True) for t in (x2, w2, r2)]
+                y = linear(leaves[0], leaves[1], b, act="gelu", residual=leaves[2])
+                _close(y, y_r, size, K, dtype, extra)
+        g = torch.autograd.grad(y, leaves, dy.t().contiguous().t())
+        ref = [t.double().requires_grad_(True) for t in (x, w, r)]
+        g_r = torch.autograd.grad(linear_ref(ref[0], ref[1], b.double(), "gelu", ref[2]), ref, dy.double())
+        for a, c in zip(g, g_r):
+            _norm_close(a, c, (48 + 66) * U if dtype == torch.float32 else 3 * 2.0 ** -8)
+    for bias in (b.float(), b.bfloat16(), torch.stack([b, b], 1)[:, 0]):
+        _close(linear(x, w, bias), linear_ref(x.double(), w.double(), bias.double()), size, K, dtype, extra)
+    if M % 3 == 0:
+        for shape in ((3, M // 3), (1, 3, M // 3), (M, 1)):
+            x3, r3 = x.view(*shape, K), r.view(*shape, N)
+            y = linear(x3, w, b, act="gelu", residual=r3)
+            assert y.shape == (*shape, N) and torch.equal(y.view(M, N), linear(x, w, b, act="gelu", residual=r))
+            leaf = x3.clone().requires_grad_(True)
+            d = torch.autograd.grad(linear(leaf, w, b, act="gelu", residual=r3), leaf, dy.view(*shape, N))[0]
+            flat = x.clone().requires_grad_(True)
+            assert torch.equal(d.view(M, K), torch.autograd.grad(linear(flat, w, b, act="gelu", residual=r), flat, dy)[0])
+    _close(linear(x[0], w), x[0].double() @ w.double(), size[0], K, dtype)
+    one = x[:1].clone().requires_grad_(True)                          # a broadcast row and a broadcast residual
+    row = r[:1].clone().requires_grad_(True)
+    y = linear(one.expand(M, K), w, residual=row.expand(M, N))
+    _close(y, (one.double() @ w.double() + row.double()).expand(M, N), size[:1].expand(M, N), K, dtype, extra)
+    d1, d2 = torch.autograd.grad(y, (one, row), dy)
+    _norm_close(d2, dy.double().sum(0, keepdim=True), 2 * U * M if dtype == torch.float32 else 2.0 ** -7)
+    _norm_close(d1, dy.double().sum(0, keepdim=True) @ w.double().t(), 300 * U if dtype == torch.float32 else 3 * 2.0 ** -7)
+
+
+@pytest.mark.parametrize("M,K,N", [(1, 40, 24), (20, 70, 50), (300, 130, 200), (2560, 64, 1920), (40, 4096, 40)])
+def test_values_that_are_not_finite(M, K, N):
+    """What the plain fp32 sums make of infinities, NaN and values next to overflow (in one launch, in parts, few rows)."""
+    for dtype in (torch.float32, torch.bfloat16):
+        x, w, b, r, dy = _data(M, K, N, dtype, 2)
+        x[0, 3], w[5, 7 % N] = float("inf"), float("-inf")
+        if M > 1:
+            x[1, 2] = float("nan")
+            x[M - 1, 9] = 3.39e38                                     # rounds to infinity in eight bits
+        w[11, 3] = 0.0
+        w[:, 4] = 0.0                                                 # infinity times zero
+        w[:, 5] = w[:, 5].abs() * 1e-3 + 1e-3
+        y, y_r = linear(x, w), (x.double() @ w.double()).to(dtype)
+        assert torch.equal(torch.isnan(y), torch.isnan(y_r))
+        assert torch.equal(torch.isinf(y), torch.isinf(y_r)) and torch.equal(y[torch.isinf(y)], y_r[torch.isinf(y_r)])
+        fine = torch.isfinite(y_r)
+        assert bool(((y.double() - y_r.double()).abs()[fine] <= 1e-2 * (y_r.double().abs()[fine] + 1)).all())
+        ts = [t.clone().requires_grad_(True) for t in (x, w)]
+        d = torch.autograd.grad(linear(*ts), ts, dy)
+        for a, c in zip(d, (dy.double() @ w.double().t(), x.double().t() @ dy.double())):
+            c = c.to(dtype)
+            assert torch.equal(torch.isnan(a), torch.isnan(c)) and torch.equal(a[torch.isinf(a)], c[torch.isinf(c)])
+
+
+def test_range_of_fp32():
+    """Rows and columns of very different sizes keep their own precision."""
+    x, w, _, _, _ = _data(200, 300, 100, seed=4)
+    x *= torch.logspace(-25, 12, 200, device="cuda")[:, None]
+    w *= torch.logspace(-12, 20, 100, device="cuda")
+    y = linear(x, w).double()
+    ref, size = x.double() @ w.double(), x.double().abs() @ w.double().abs()
+    assert float(((y - ref).abs() / size).max()) < 60 * U
+
+
+def test_refusals():
+    x, w, b, r, _ = _data(4, 8, 6)
+    for kw in (dict(x=x.double()), dict(x=x.half()), dict(w=w.bfloat16()), dict(w=w.cpu()), dict(w=w[0]), dict(w=w[:, :0]), dict(x=x[:, :5]),
+               dict(b=b[:3]), dict(b=b.double()), dict(b=b.cpu()), dict(act="relu"), dict(residual=r[:2]), dict(residual=r.bfloat16()),
+               dict(residual=r[:1]), dict(x=x.sum())):
+        a = dict(x=x, w=w, b=b)
+        a.update(kw)
+        with pytest.raises(ValueError):
+            linear(a.pop("x"), a.pop("w"), a.pop("b"), **a)
+    with pytest.raises(RuntimeError):
+        linear(x.cpu(), w)
+    with torch.autograd.forward_ad.dual_level(), torch.no_grad():
+        with pytest.raises(RuntimeError):
+            linear(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)), w)
+    ts = [t.clone().requires_grad_(True) for t in (x, w)]
+    (d,) = torch.autograd.grad(linear(*ts).sum(), ts[0], create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        d.sum().backward()
+    y = linear(*ts)
+    with torch.no_grad():
+        ts[1].add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
+
+
+def test_no_rows_and_some_gradients_only():
+    x, w, b, r, dy = _data(40, 33, 21, seed=6)
+    e = [t.clone().requires_grad_(True) for t in (x[:0], w, b, r[:0])]
+    y = linear(*e[:3], act="gelu", residual=e[3])
+    assert y.shape == (0, 21)
+    for t, g in zip(e, torch.autograd.grad(y.sum(), e)):
+        assert g.shape == t.shape and bool((g == 0).all())
+    ref = [t.double().requires_grad_(True) for t in (x, w, b, r)]
+    g_r = torch.autograd.grad(linear_ref(*ref[:3], "gelu", ref[3]), ref, dy.double())
+    for want in range(1, 16):
+        ts = [t.clone().requires_grad_(bool(want >> i & 1)) for i, t in enumerate((x, w, b, r))]
+        got = torch.autograd.grad(linear(*ts[:3], act="gelu", residual=ts[3]), [t for t in ts if t.requires_grad], dy)
+        for a, c in zip(got, [g for i, g in enumerate(g_r) if want >> i & 1]):
+            _norm_close(a, c, 120 * U)
+
+
+def test_gradients_against_differences():
+    """Along each gradient, with a step of 2^-7: t^2 of GELU's third derivative and fp32's rounding of f, some 1e-4."""
+    x, w, b, r, dy = _data(30, 50, 40, seed=7)
+    ts = [t.clone().requires_grad_(True) for t in (x, w, b, r)]
+    f = lambda *a: (linear(a[0], a[1], a[2], act="gelu", residual=a[3]).double() * dy.double()).sum()
+    grads = torch.autograd.grad(f(*ts), ts)
+    for i in range(4):
+        d, t = grads[i] / grads[i].norm(), 2.0 ** -7
+        with torch.no_grad():
+            up, down = ([u + s * t * d if j == i else u for j, u in enumerate(ts)] for s in (1, -1))
+            slope = float(f(*up) - f(*down)) / (2 * t)
+        assert abs(slope / float(grads[i].norm()) - 1) < 2e-3
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_other_stream_and_graph(dtype):
+    """The current stream; captured forward and backward replay on new inputs; two graphs in turn; the same bits."""
+    atomic_gdn2.set_checks("async")
+    x, w, b, r, dy = _data(300, 515, 260, dtype, 9)
+    ts = [t.clone().requires_grad_(True) for t in (x, w, b, r)]
+    call = lambda: (lambda y: (y, *torch.autograd.grad(y, ts, dy)))(linear(*ts[:3], act="gelu", residual=ts[3]))
+    want = call()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        got = call()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, c) for a, c in zip(want, got))
+    del want, got         # torch captures no backward while an eager graph of the same leaves lives
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+            with torch.no_grad():
+                few = linear(ts[0][:2], ts[1])
+        graphs.append((graph, out, few))
+    with torch.no_grad():
+        ts[0].mul_(-0.5)
+        ts[1].add_(0.01)
+    for graph, *_ in graphs * 2:
+        graph.replay()
+    want = call()
+    with torch.no_grad():
+        want_few = linear(ts[0][:2], ts[1])
+    for _, out, few in graphs:
+        assert all(torch.equal(a, c) for a, c in zip(want, out)) and torch.equal(few, want_few)
+
+
+def test_large_offsets():
+    """Outputs of more than 2^31 values."""
+    M, K, N = 70000, 16, 32768
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(M, K, generator=gen, device="cuda").bfloat16()
+    w = torch.randn(K, N, generator=gen, device="cuda").bfloat16()
+    with torch.no_grad():
+        y = linear(x, w)
+    rows = [0, 1, 32767, 65535, 65536, 69887, 69999]
+    _close(y[rows], x[rows].double() @ w.double(), x[rows].double().abs() @ w.double().abs(), K, torch.bfloat16)

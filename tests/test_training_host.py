@@ -1,0 +1,150 @@
+"""Host side of the training operators: refusals that need no GPU, and the 8-bit moments' formats."""
+import ctypes
+import pathlib
+import sys
+
+import pytest
+import torch
+
+sys.path.insert(0, str(pathlib.Path(__file__).resolve().parent))
+from atomic_gdn2 import _lib, gated_scan, linear, make_cfg  # noqa: E402
+from atomic_gdn2.training import GDN2LM, AdamW, TrainStep, make_optimizer  # noqa: E402
+from training_ref import code_m, code_r, decode, encode, root  # noqa: E402
+
+
+def test_operators_have_no_cpu_path():
+    with pytest.raises(RuntimeError):
+        linear(torch.zeros(2, 3), torch.zeros(3, 4))
+    with pytest.raises(RuntimeError):
+        gated_scan(torch.zeros(1, 2, 3), torch.zeros(1, 2, 3))
+    p = torch.nn.Parameter(torch.zeros(3))
+    p.grad = torch.zeros(3)
+    with pytest.raises(RuntimeError):
+        AdamW([p]).step()
+    with pytest.raises(ValueError):
+        gated_scan(torch.zeros(2, 3), torch.zeros(2, 3))
+
+
+def test_adamw_refusals():
+    p = [torch.nn.Parameter(torch.zeros(3))]
+    for kw in (dict(state_bits=16), dict(betas=(1.0, 0.9)), dict(betas=(0.9, -0.1)), dict(eps=-1.0), dict(lr=-1.0),
+               dict(weight_decay=-1.0), dict(clip=0.0), dict(clip=-1.0), dict(spike_factor=0.0), dict(lr=float("nan"))):
+        with pytest.raises(ValueError):
+            AdamW(p, **kw)
+    opt = AdamW(p)
+    assert opt.step() is None                      # nothing has a gradient
+    with pytest.raises(RuntimeError):
+        opt.grad_norm
+    with pytest.raises(ValueError):
+        opt.moments(p)
+    opt = AdamW([dict(params=p, lr=0.1), dict(params=[torch.nn.Parameter(torch.zeros(1))], eps=1e-3)])
+    p[0].grad = torch.zeros(3)
+    with pytest.raises(ValueError):
+        opt.step()
+
+
+def test_model_and_step_take_the_operators():
+    """The options reach where they are used; without them everything is as it was."""
+    m = GDN2LM(make_cfg(), d_model=32, n_heads=1, d_head=16, n_layers=1, blr_fn=lambda *a: None, linear_fn=linear)
+    assert m.layers[0].linear_fn is linear and m.linear_fn is linear
+    opt = make_optimizer(m, 1e-3, state_bits=8)
+    assert isinstance(opt, AdamW) and opt.state_bits == 8 and [g["weight_decay"] for g in opt.param_groups] == [0.1, 0.0]
+    step = TrainStep(m, opt, clip=0.7, spike_factor=3.0)
+    assert opt.clip == 0.7 and opt.spike_factor == 3.0 and float(step.gn_ema) == 0.0
+    plain = GDN2LM(make_cfg(), d_model=32, n_heads=1, d_head=16, n_layers=1, blr_fn=lambda *a: None)
+    assert plain.linear_fn is None and isinstance(make_optimizer(plain, 1e-3), torch.optim.AdamW)
+
+
+def test_moment_codes():
+    """Half a step: 1/16 of an e4m3 value, 1/32 of a root, each next to the smallest normal numbers of the format;
+    zeros stay zeros, and roots above zero stay above zero."""
+    gen = torch.Generator().manual_seed(1)
+    x = torch.randn(1000, generator=gen) * torch.exp(torch.randn(1000, generator=gen) * 3)
+    x[:10] = 0.0
+    v = (torch.randn(1000, generator=gen) * torch.exp(torch.randn(1000, generator=gen) * 3)) ** 2
+    v[256:300] = 0.0
+    v[512] = 1e30                                    # a block of one large value and many that are next to nothing
+    (m8, ms), (v8, vs) = encode(x, 448.0, code_m), encode(root(v), 1.9375, code_r)
+    m, v2 = decode(m8, ms, v8, vs)
+    steps = ms.repeat_interleave(256)[:1000]
+    assert bool(((m - x).abs() <= (x.abs() / 16 + steps * 2.0 ** -10) * 1.0001).all())
+    r, r2 = v.sqrt(), v2.sqrt()
+    scale = vs.repeat_interleave(256)[:1000]
+    assert bool(((r2 - r).abs() <= (r / 32 + scale * 2.0 ** -18) * 1.0001).all())
+    assert bool(((v2 > 0) == (v > 0)).all()) and bool((m[:10] == 0).all())
+    codes = torch.arange(256, dtype=torch.uint8)
+    again, s = encode(decode(codes * 0, torch.ones(1), codes, torch.ones(1))[1].sqrt(), 1.9375, code_r)
+    assert torch.equal(again, codes) and float(s) == 1.0
+
+
+def test_entry_points_reject_bad_arguments():
+    """Everything is refused before a launch, so no GPU is needed; pointers are never followed."""
+    lib, inv, uns, at = _lib.load(), _lib.ERR_INVALID_ARGUMENT, _lib.ERR_UNSUPPORTED, 4096
+
+    def lin(x=at, w=at, y=at, ws=at, flags=at, bias=0, **kw):
+        d = _lib.LinearDesc()
+        d.M, d.K, d.N, d.x_stride, d.w_stride = 32, 64, 16, 64, 16
+        for k, v in kw.items():
+            setattr(d, k, v)
+        a = ctypes.addressof(d)
+        return (lib.gdn2_linear_fwd(a, x, w, bias, 0, y, 0, ws, flags, 0), lib.gdn2_linear_fwd_workspace_bytes(a),
+                lib.gdn2_linear_bwd(a, x, w, 0, y, at, at, at, ws, flags, 0), lib.gdn2_linear_bwd_workspace_bytes(a, 7))
+
+    for kw in (dict(M=-1), dict(K=0), dict(N=0), dict(dtype=2), dict(bias_dtype=7), dict(act=3), dict(x_stride=63), dict(w_stride=15)):
+        assert lin(**kw) == (inv, 0, inv, 0), kw
+    for kw in (dict(M=2 ** 29), dict(K=2 ** 30, x_stride=2 ** 30), dict(x_stride=2 ** 31), dict(M=2 ** 27, N=2 ** 27, w_stride=2 ** 27)):
+        assert lin(**kw)[0] == uns and lin(**kw)[1] == 0, kw
+    for kw in (dict(x=0), dict(w=0), dict(y=0), dict(flags=0), dict(x=at + 8), dict(w=at + 4), dict(y=at + 2), dict(bias=at + 2),
+               dict(ws=0), dict(ws=at + 64)):
+        assert lin(**kw)[0] == inv, kw
+    for kw in (dict(x=at + 8), dict(flags=0), dict(act=1), dict(ws=0), dict(y=at + 4)):
+        assert lin(**kw)[2] == inv, kw
+    assert lib.gdn2_linear_fwd(0, *[at] * 9) == inv and lib.gdn2_linear_bwd(0, *[at] * 10) == inv
+    assert lin(M=0)[0] == _lib.OK and lin(M=0)[2] == inv
+
+    def gated(x=at, g=at, h0=0, idx=0, last=at, flags=at, marks=at, **kw):
+        d = _lib.GatedDesc()
+        d.B, d.L, d.C = 2, 8, 16
+        for i in range(2):
+            d.x_stride[i] = d.g_stride[i] = 16
+        for k, v in kw.items():
+            if k == "stride":
+                d.x_stride[1] = v
+            else:
+                setattr(d, k, v)
+        a = ctypes.addressof(d)
+        return (lib.gdn2_gated_fwd(a, x, g, h0, idx, 0, 0, at, last, 0, flags, 0), lib.gdn2_gated_marks_bytes(a),
+                lib.gdn2_gated_bwd(a, x, g, 0, 0, marks, at, 0, at, at, 0, flags, 0))
+
+    for kw in (dict(B=0), dict(L=-1), dict(C=0), dict(dtype=5), dict(n_states=-1), dict(stride=-16)):
+        assert gated(**kw) == (inv, 0, inv), kw
+    assert gated(B=2 ** 27, C=2 ** 20)[0] == uns
+    for kw in (dict(x=0), dict(g=0), dict(x=at + 2), dict(last=0), dict(flags=0), dict(idx=at), dict(h0=at), dict(h0=at, n_states=1),
+               dict(h0=at, idx=at), dict(h0=at + 2, n_states=2), dict(dtype=1, x=at + 2)):
+        assert gated(**kw)[0] == inv, kw
+    for kw in (dict(x=0), dict(marks=0), dict(marks=at + 2), dict(flags=0), dict(L=0)):
+        assert gated(**kw)[2] == inv, kw
+    assert lib.gdn2_gated_fwd(0, *[at] * 11) == inv and lib.gdn2_gated_bwd(0, *[at] * 12) == inv
+
+    def adamw(n=1, control=at, ws=at, desc=None, **kw):
+        d, t = _lib.AdamwDesc(), (_lib.AdamwTensor * 2)()
+        d.state_bits, d.beta1, d.beta2, d.eps = 32, 0.9, 0.95, 1e-8
+        for k, v in (desc or {}).items():
+            setattr(d, k, v)
+        t[0].p = t[0].g = t[0].m = t[0].v = t[0].step = at
+        t[0].n = 100
+        for k, v in kw.items():
+            setattr(t[0], k, v)
+        a, b = ctypes.addressof(d), ctypes.addressof(t)
+        return lib.gdn2_adamw_step(a, b, n, 0, control, ws, 0), lib.gdn2_adamw_workspace_bytes(a, b, n)
+
+    for kw in (dict(n=-1), dict(desc=dict(state_bits=4)), dict(desc=dict(beta1=1.0)), dict(desc=dict(beta2=-0.5)),
+               dict(desc=dict(eps=-1.0)), dict(desc=dict(clip=-1.0)), dict(desc=dict(spike=float("nan"))), dict(p=0), dict(g=at + 2),
+               dict(m=0), dict(v=at + 1), dict(dtype=4), dict(desc=dict(state_bits=8))):
+        assert adamw(**kw) == (inv, 0), kw
+    for kw in (dict(step=0), dict(control=0), dict(control=at + 2), dict(ws=0), dict(ws=at + 128)):
+        assert adamw(**kw)[0] == inv, kw
+    assert adamw(n=0) == (_lib.OK, 0) and adamw(**{"n": 1, "p": 0, "g": 0}) == (inv, 0)
+    t = (_lib.AdamwTensor * 1)()
+    t[0].n = 5
+    assert lib.gdn2_adamw_moments(ctypes.addressof(t), 1, 0) == inv and lib.gdn2_adamw_step(0, 0, 0, 0, at, at, 0) == inv
