@@ -16,6 +16,9 @@
 // bytes a value) and computes h again from x: reading the rounded h instead would cost as many bytes and,
 // for bf16, half a step of h in dg.
 #include <cooperative_groups.h>
+#include <cuda.h>
+
+#include <cstring>
 
 #include "gdn2_common.cuh"
 
@@ -27,7 +30,12 @@ namespace cg = cooperative_groups;
 constexpr float kReset = -1.f;        // a segment's factor when a reset is in it: what entered is dropped
 constexpr float kTiny = 1.17549435e-38f;
 constexpr int kMaxWarps = 8, kMaxCluster = 8;
-constexpr int kValues = 16;           // of a thread's segment: S tokens of V channels
+constexpr int kTileStages = 2;
+// Tokens of a thread's segment of V channels.  Odd: where the lanes of a warp hold several segments, their rows in a
+// tile in shared memory start in different banks.  Three CTAs of the backward pass fit an SM with 11 (5 of pairs), two
+// with 15 (7): where there are many sequences and channels the former count (8 x 2048 x 768: 60 -> 45 us), where few
+// long ones are walked in clusters the fewer rounds (1 x 131072 x 256: 174 -> 141 us).
+constexpr int tokens(int V, bool many) { return V == 1 ? (many ? 11 : 15) : many ? 5 : 7; }
 
 struct GatedParams {
   const void *x, *g, *dy;
@@ -107,15 +115,17 @@ __device__ __forceinline__ long long state_row(const GatedParams& p, int b) {  /
   return i < 0 ? -1 : i;
 }
 
-// Bit i: token t0 + i drops the state before it.
+// Bit i: token t0 + i of `live` drops the state before it.  The lanes of a segment look at a token each.
 template <int S>
-__device__ __forceinline__ uint32_t resets_of(const GatedParams& p, int b, long long t0, int live) {
+__device__ __forceinline__ uint32_t resets_of(const GatedParams& p, int b, long long t0, int live, int lane, int lanes) {
   if (!p.reset) return 0;
   const uint8_t* r = p.reset + b * (long long)p.L + t0;
+  const int first = (threadIdx.x & 31) & ~(lanes - 1);
   uint32_t bits = 0;
-#pragma unroll
-  for (int i = 0; i < S; ++i)
-    if (i < live && r[i]) bits |= 1u << i;
+  for (int i0 = 0; i0 < S; i0 += lanes) {
+    const uint32_t all = __ballot_sync(0xffffffffu, i0 + lane < live && r[i0 + lane]);
+    bits |= ((all >> first) & (lanes == 32 ? 0xffffffffu : (1u << lanes) - 1u)) << i0;
+  }
   return bits;
 }
 
@@ -133,10 +143,12 @@ __device__ __forceinline__ void rows_of(raw r[S], const raw* p, long long ld, in
   }
 }
 
+template <int V>
 struct Shared {
-  Seg part[2][kMaxWarps][32 * 2];       // a warp's segments together, by channel of a row of lanes, for two rounds
-  Seg inbox[2][kMaxCluster][32 * 2];    // the CTAs' of the cluster, for two rounds
+  Seg part[2][kMaxWarps][32 * V];       // a warp's segments together, by channel of a row of lanes, for two rounds
+  Seg inbox[2][kMaxCluster][32 * V];    // the CTAs' of the cluster, for two rounds
   uint64_t bar[2];                      // that they are there
+  uint64_t full[kTileStages];           // that a stage's tiles are
   volatile int dead;                    // a wait ran out
 };
 
@@ -144,7 +156,8 @@ struct Shared {
 // receiver's barrier.  (A barrier over the cluster would order all of the CTA's memory accesses, the outputs' of the
 // round before among them: 5.0 us a round of 8 CTAs.)  A CTA sends round r + 2 after it has seen every CTA's
 // round r + 1, which these send after they have read round r: two boxes are enough.
-__device__ __forceinline__ void send(Shared& sm, int box, int from, int to, int at, Seg s) {
+template <int V>
+__device__ __forceinline__ void send(Shared<V>& sm, int box, int from, int to, int at, Seg s) {
   uint32_t dst, bar;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(dst) : "r"(smem_u32(&sm.inbox[box][from][at])), "r"(to));
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_u32(&sm.bar[box])), "r"(to));
@@ -168,15 +181,33 @@ __device__ __forceinline__ bool cluster_wait(uint64_t* bar, uint32_t parity) {
   }
 }
 
-__device__ __forceinline__ void begin(Shared& sm, int n) {
-  if (n == 1) return;
+template <int V>
+__device__ __forceinline__ void begin(Shared<V>& sm, int n, bool tiles) {
+  if (n == 1 && !tiles) return;
   if (threadIdx.x == 0) {
     mbar_init(&sm.bar[0], 1);
     mbar_init(&sm.bar[1], 1);
+    for (int i = 0; i < kTileStages; ++i) mbar_init(&sm.full[i], 1);
     sm.dead = 0;
     fence_mbar_init();
   }
-  cg::this_cluster().sync();
+  if (n > 1) cg::this_cluster().sync();
+  else __syncthreads();
+}
+template <int V>
+__device__ __forceinline__ void tile_wait(Shared<V>& sm, int stage, uint32_t parity, uint32_t* flags) {
+  if (sm.dead || cluster_wait(&sm.full[stage], parity)) return;
+  sm.dead = 1;
+  if (flags) flags[2] = 1;
+}
+// Before the CTA ends: its copies out of shared memory are over, and had a wait run out, those into it are given time.
+template <int V>
+__device__ __forceinline__ void tiles_done(const Shared<V>& sm) {
+  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  if (sm.dead) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 20 * 1000 * 1000) __nanosleep(1000);
+  }
 }
 
 // join() and step() where no reset and no gate of zero is about (plain), or with them.
@@ -191,7 +222,7 @@ __device__ __forceinline__ float step_as(Seg s, float h) {
   else return step(s, h);
 }
 template <bool PLAIN, int V>
-__device__ __forceinline__ void join_warp(Seg (*part)[32 * 2], const Seg mine[V], int lanes, Seg before[V]) {
+__device__ __forceinline__ void join_warp(Seg (*part)[32 * V], const Seg mine[V], int lanes, Seg before[V]) {
   const int at = threadIdx.x & 31, lane = at & (lanes - 1), warp = threadIdx.x >> 5;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
@@ -209,7 +240,7 @@ __device__ __forceinline__ void join_warp(Seg (*part)[32 * 2], const Seg mine[V]
   }
 }
 template <bool PLAIN, int V>
-__device__ __forceinline__ void join_cta(Shared& sm, int round, int lanes, int rank, int n, Seg before[V], float enter[V], float mine_in[V]) {
+__device__ __forceinline__ void join_cta(Shared<V>& sm, int round, int lanes, int rank, int n, Seg before[V], float enter[V], float mine_in[V]) {
   const int at = threadIdx.x & 31, lane = at & (lanes - 1), warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
@@ -238,7 +269,7 @@ __device__ __forceinline__ void join_cta(Shared& sm, int round, int lanes, int r
 // cluster's first segment enters with; on return mine_in[] is what this thread's enters with, and enter[] what the
 // next round's first one does.  `plain`: no reset and no gate of zero in this thread's segment.
 template <int V>
-__device__ __forceinline__ void exchange(Shared& sm, int round, const Seg mine[V], bool plain, int lanes, int rank, int n,
+__device__ __forceinline__ void exchange(Shared<V>& sm, int round, const Seg mine[V], bool plain, int lanes, int rank, int n,
                                          float enter[V], float mine_in[V], uint32_t* flags) {
   const int lane = threadIdx.x & (lanes - 1);
   Seg before[V];                        // of this warp's segments before this thread's
@@ -247,7 +278,7 @@ __device__ __forceinline__ void exchange(Shared& sm, int round, const Seg mine[V
   if (__syncthreads_and(plain)) join_cta<true, V>(sm, round, lanes, rank, n, before, enter, mine_in);
   else join_cta<false, V>(sm, round, lanes, rank, n, before, enter, mine_in);
   if (n > 1) {
-    Seg(*inbox)[32 * 2] = sm.inbox[round & 1];
+    Seg(*inbox)[32 * V] = sm.inbox[round & 1];
     if (threadIdx.x == 0) mbar_arrive_expect_tx(&sm.bar[round & 1], (uint32_t)(n * lanes * V * sizeof(Seg)));
     if (!sm.dead && !cluster_wait(&sm.bar[round & 1], (round >> 1) & 1)) {
       sm.dead = 1;
@@ -283,50 +314,127 @@ __device__ __forceinline__ Seg segment(const float (*a)[V], int v, float A, floa
   return {A, q};
 }
 
-template <class T, int V>
-__global__ void __launch_bounds__(32 * kMaxWarps, 3) gated_fwd_kernel(const __grid_constant__ GatedParams p) {
+// A tile in shared memory: `tokens` rows of the lanes' 4-byte words, brought and taken away by tiled copies.  Rows past
+// the sequences' end arrive as zeros (gates of one, nothing added) and are not taken away.
+struct Tiles {
+  CUtensorMap x, g, dy, o0, o1;         // o0: h or dx, o1: dg
+  int boxes;                            // copies of a tile: their boxes have up to 256 rows
+};
+struct Ring {
+  uint64_t* bar;
+  uint8_t* base;
+  uint32_t tile;                        // bytes
+  int arrays;                           // tiles of a stage
+  __device__ __forceinline__ uint32_t at(int stage, int array) const { return smem_u32(base) + (stage * arrays + array) * tile; }
+};
+__device__ __forceinline__ void tile_in(uint32_t dst, const CUtensorMap* m, int c, int t, int b, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(m), "r"(c), "r"(t), "r"(b), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tile_out(const CUtensorMap* m, uint32_t src, int c, int t, int b) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(m), "r"(c), "r"(t), "r"(b),
+               "r"(src)
+               : "memory");
+}
+__device__ __forceinline__ void tiles_read() {  // what was sent away has been read from shared memory
+  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+__device__ __forceinline__ void stage_in(const Ring& r, const Tiles& m, int stage, int c, int t, int b, int rows) {
+  mbar_arrive_expect_tx(&r.bar[stage], r.tile * r.arrays);
+  const uint32_t bar = smem_u32(&r.bar[stage]), part = r.tile / m.boxes;
+  for (int i = 0; i < m.boxes; ++i) {
+    tile_in(r.at(stage, 0) + i * part, &m.x, c, t + i * rows, b, bar);
+    tile_in(r.at(stage, 1) + i * part, &m.g, c, t + i * rows, b, bar);
+    if (r.arrays == 3) tile_in(r.at(stage, 2) + i * part, &m.dy, c, t + i * rows, b, bar);
+  }
+}
+template <class raw>
+__device__ __forceinline__ raw word(uint32_t at) {
+  uint32_t u;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(u) : "r"(at));
+  raw r;
+  memcpy(&r, &u, sizeof(raw));
+  return r;
+}
+template <class raw>
+__device__ __forceinline__ void put_word(uint32_t at, raw r) {
+  uint32_t u = 0;
+  memcpy(&u, &r, sizeof(raw));
+  asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(u) : "memory");
+}
+
+// TILE: the rows come and go by tiled copies, a stage ahead of the work; else each thread reads and writes its own.
+template <class T, int V, int S, bool TILE>
+__global__ void __launch_bounds__(32 * kMaxWarps, 3) gated_fwd_kernel(const __grid_constant__ GatedParams p,
+                                                                      const __grid_constant__ Tiles m) {
   using L = Lane<T, V>;
   using raw = typename L::raw;
-  constexpr int S = kValues / V;
-  __shared__ Shared sm;
+  extern __shared__ __align__(128) uint8_t tiles[];
+  __shared__ Shared<V> sm;
   const int lanes = 1 << p.lanes_log2, lane = threadIdx.x & (lanes - 1);
   const int place = threadIdx.x >> p.lanes_log2, places = blockDim.x >> p.lanes_log2;
   const int rank = blockIdx.x % p.clusters, block = blockIdx.x / p.clusters;
-  const int b = block / p.cols, c = ((block % p.cols) * lanes + lane) * V;
+  const int b = block / p.cols, c0 = (block % p.cols) * lanes * V, c = c0 + lane * V;
   const bool on = c < p.C;
   const int len = length_of(p, b);
   const long long row = state_row(p, b);
-  begin(sm, p.clusters);
+  const int segs = (p.L + S - 1) / S, count = (segs + places - 1) / places, TT = places * S;  // tiles of TT tokens
+  const Ring ring{sm.full, tiles, (uint32_t)(TT * lanes * 4), 2};
+  begin(sm, p.clusters, TILE);
+  if (TILE && threadIdx.x == 0)
+    for (int s = 0; s < kTileStages && s * p.clusters + rank < count; ++s)
+      stage_in(ring, m, s, c0, (s * p.clusters + rank) * TT, b, TT / m.boxes);
   float enter[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) enter[v] = on && row >= 0 ? p.h0[row * p.C + c + v] : 0.f;
-  const raw* x = reinterpret_cast<const raw*>(static_cast<const T*>(p.x) + b * p.xb + c);
-  const raw* g = reinterpret_cast<const raw*>(static_cast<const T*>(p.g) + b * p.gb + c);
-  raw* h = reinterpret_cast<raw*>(static_cast<T*>(p.h) + (long long)b * p.L * p.C + c);
   const long long xl = p.xl / V, gl = p.gl / V, hl = p.C / V;
-  const int segs = (p.L + S - 1) / S, per_round = places * p.clusters;
   float top = -1.f;                     // the largest gate
-  for (int round = 0; round * (long long)per_round < segs; ++round) {
-    const long long seg = (long long)round * per_round + rank * places + place;
-    const long long t0 = seg * S;
-    const int live = on ? (int)max(0ll, min((long long)S, len - t0)) : 0;
+  for (int round = 0; round * p.clusters < count; ++round) {
+    const int tile = round * p.clusters + rank, seg = tile * places + place, slot = round % kTileStages;
+    const long long t0 = (long long)seg * S;
+    const int alive = max(0, min(S, (int)min((long long)S, len - t0))), live = on ? alive : 0;
+    const uint32_t words = ring.at(slot, 0) + (place * S * lanes + lane) * 4;
     float a[S][V], q[S][V];
-    {
+    if constexpr (TILE) {
+      if (threadIdx.x == 0 && round > 0) {  // the stage of the round before takes the next one
+        tiles_read();
+        const int next = tile + (kTileStages - 1) * p.clusters;
+        if (next < count) stage_in(ring, m, (round - 1) % kTileStages, c0, next * TT, b, TT / m.boxes);
+      }
+      if (tile < count) tile_wait(sm, slot, (round / kTileStages) & 1, p.flags);
+#pragma unroll
+      for (int i = 0; i < S; ++i) {
+        L::get(word<raw>(words + i * lanes * 4), q[i]);
+        L::get(word<raw>(words + ring.tile + i * lanes * 4), a[i]);
+      }
+      if (live < S) {                   // past the length: whatever is there
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+          if (i >= live) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) q[i][v] = a[i][v] = 0.f;
+          }
+      }
+    } else {
       raw rx[S], rg[S];
-      rows_of<S>(rx, x + t0 * xl, xl, live);   // past the end zeros: gates of one
-      rows_of<S>(rg, g + t0 * gl, gl, live);
+      rows_of<S>(rx, reinterpret_cast<const raw*>(static_cast<const T*>(p.x) + b * p.xb + c) + t0 * xl, xl, live);
+      rows_of<S>(rg, reinterpret_cast<const raw*>(static_cast<const T*>(p.g) + b * p.gb + c) + t0 * gl, gl, live);
 #pragma unroll
       for (int i = 0; i < S; ++i) {
         L::get(rx[i], q[i]);
         L::get(rg[i], a[i]);
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          top = fmaxf(top, a[i][v]);
-          a[i][v] = expf(at_most_zero(a[i][v]));
-        }
       }
     }
-    const uint32_t resets = resets_of<S>(p, b, t0, live);
+#pragma unroll
+    for (int i = 0; i < S; ++i)
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        top = fmaxf(top, a[i][v]);
+        a[i][v] = expf(at_most_zero(a[i][v]));
+      }
+    const uint32_t resets = resets_of<S>(p, b, t0, alive, lane, lanes);
     Seg mine[V];
     float mine_in[V];
     bool plain = true;
@@ -346,31 +454,45 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 3) gated_fwd_kernel(const __gr
       mine[v] = segment<S, V>(a, v, A, s, resets, plain);
     }
     exchange<V>(sm, round, mine, plain, lanes, rank, p.clusters, enter, mine_in, p.flags);
-    if (on && t0 < p.L) {
+    if (on && seg < segs) {
       if (p.marks) {
 #pragma unroll
         for (int v = 0; v < V; ++v) p.marks[((long long)b * segs + seg) * p.C + c + v] = mine_in[v];
       }
-      raw* ph = h + t0 * hl;
-      if (live == S && !resets) {
+    }
+    const bool whole = live == S && !resets;
+    raw* ph = reinterpret_cast<raw*>(static_cast<T*>(p.h) + (long long)b * p.L * p.C + c) + t0 * hl;
+    const int rows = on ? (int)max(0ll, min((long long)S, p.L - t0)) : 0;
+    auto put = [&](int i, const float* y) {
+      if constexpr (TILE) put_word<raw>(words + i * lanes * 4, L::put(y));
+      else if (i < rows) ph[i * hl] = L::put(y);
+    };
+    if (whole) {
 #pragma unroll
-        for (int i = 0; i < S; ++i) {
+      for (int i = 0; i < S; ++i) {
 #pragma unroll
-          for (int v = 0; v < V; ++v) mine_in[v] = fmaf(a[i][v], mine_in[v], q[i][v]);
-          ph[i * hl] = L::put(mine_in);
+        for (int v = 0; v < V; ++v) mine_in[v] = fmaf(a[i][v], mine_in[v], q[i][v]);
+        put(i, mine_in);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < S; ++i) {
+        float y[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          mine_in[v] = ((resets >> i) & 1u) ? q[i][v] : fmaf(a[i][v], mine_in[v], q[i][v]);
+          y[v] = i < live ? mine_in[v] : 0.f;
         }
-      } else {
-        const int rows = (int)min((long long)S, p.L - t0);
-#pragma unroll
-        for (int i = 0; i < S; ++i) {
-          float y[V];
-#pragma unroll
-          for (int v = 0; v < V; ++v) {
-            mine_in[v] = ((resets >> i) & 1u) ? q[i][v] : fmaf(a[i][v], mine_in[v], q[i][v]);
-            y[v] = i < live ? mine_in[v] : 0.f;
-          }
-          if (i < rows) ph[i * hl] = L::put(y);
-        }
+        put(i, y);
+      }
+    }
+    if constexpr (TILE) {
+      fence_async_smem();
+      __syncthreads();
+      if (threadIdx.x == 0 && tile < count) {
+        for (int i = 0; i < m.boxes; ++i)
+          tile_out(&m.o0, ring.at(slot, 0) + i * (ring.tile / m.boxes), c0, tile * TT + i * (TT / m.boxes), b);
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       }
     }
   }
@@ -379,126 +501,173 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 3) gated_fwd_kernel(const __gr
     for (int v = 0; v < V; ++v) p.last[(long long)b * p.C + c + v] = enter[v];
   }
   if (top > 0.f) p.flags[0] = 1;
+  if (TILE && threadIdx.x == 0) tiles_done(sm);
   if (p.clusters > 1) cg::this_cluster().sync();  // a CTA's shared memory is written until here
 }
 
-template <class T, int V>
-__global__ void __launch_bounds__(32 * kMaxWarps, 2) gated_bwd_kernel(const __grid_constant__ GatedParams p) {
+// The tiles and segments of a sequence in reverse: round 0 has the last ones.
+template <class T, int V, int S, bool TILE>
+__global__ void __launch_bounds__(32 * kMaxWarps, S * V < 12 ? 3 : 2) gated_bwd_kernel(const __grid_constant__ GatedParams p,
+                                                                      const __grid_constant__ Tiles m) {
   using L = Lane<T, V>;
   using raw = typename L::raw;
-  constexpr int S = kValues / V;
-  __shared__ Shared sm;
+  extern __shared__ __align__(128) uint8_t tiles[];
+  __shared__ Shared<V> sm;
   const int lanes = 1 << p.lanes_log2, lane = threadIdx.x & (lanes - 1);
-  const int place = threadIdx.x >> p.lanes_log2, places = blockDim.x >> p.lanes_log2;
+  const int places = blockDim.x >> p.lanes_log2, place = places - 1 - (threadIdx.x >> p.lanes_log2);
   const int rank = blockIdx.x % p.clusters, block = blockIdx.x / p.clusters;
-  const int b = block / p.cols, c = ((block % p.cols) * lanes + lane) * V;
+  const int b = block / p.cols, c0 = (block % p.cols) * lanes * V, c = c0 + lane * V;
   const bool on = c < p.C;
   const int len = length_of(p, b);
-  begin(sm, p.clusters);
-  float enter[V];  // e after the last token of a round, the sequence's last round first
+  const int segs = (p.L + S - 1) / S, count = (segs + places - 1) / places, TT = places * S;  // tiles of TT tokens
+  const Ring ring{sm.full, tiles, (uint32_t)(TT * lanes * 4), 3};
+  begin(sm, p.clusters, TILE);
+  if (TILE && threadIdx.x == 0)
+    for (int s = 0; s < kTileStages && s * p.clusters + rank < count; ++s)
+      stage_in(ring, m, s, c0, (count - 1 - s * p.clusters - rank) * TT, b, TT / m.boxes);
+  float enter[V];  // e after the last token of a round
 #pragma unroll
   for (int v = 0; v < V; ++v) enter[v] = on && p.dlast ? p.dlast[(long long)b * p.C + c + v] : 0.f;
-  const raw* x = reinterpret_cast<const raw*>(static_cast<const T*>(p.x) + b * p.xb + c);
   const raw* g = reinterpret_cast<const raw*>(static_cast<const T*>(p.g) + b * p.gb + c);
   const long long at = (long long)b * p.L * p.C + c, row = p.C / V;
-  const raw* dy = reinterpret_cast<const raw*>(static_cast<const T*>(p.dy) + at);
-  raw* dx = reinterpret_cast<raw*>(static_cast<T*>(p.dx) + at);
-  raw* dg = reinterpret_cast<raw*>(static_cast<T*>(p.dg) + at);
   const long long xl = p.xl / V, gl = p.gl / V;
-  const int segs = (p.L + S - 1) / S, per_round = places * p.clusters;
-  for (int round = 0; round * (long long)per_round < segs; ++round) {
-    const long long seg = segs - 1 - ((long long)round * per_round + rank * places + place);  // below 0: none
-    const long long t0 = seg * S;
-    const int live = on && seg >= 0 ? (int)max(0ll, min((long long)S, len - t0)) : 0;
+  for (int round = 0; round * p.clusters < count; ++round) {
+    const int tile = count - 1 - round * p.clusters - rank, slot = round % kTileStages;  // below 0: none
+    const int seg = tile * places + place;
+    const long long t0 = (long long)seg * S;
+    const int alive = tile < 0 ? 0 : max(0, min(S, (int)min((long long)S, len - t0))), live = on ? alive : 0;
+    const uint32_t words = ring.at(slot, 0) + (place * S * lanes + lane) * 4;
     float a[S][V], h[S][V], d[S][V], top = -1.f;
-    const uint32_t resets = resets_of<S>(p, b, t0, live);
-    {
-      raw rx[S], rg[S], ry[S];
-      rows_of<S>(rx, x + t0 * xl, xl, live);   // past the end zeros: gates of one, nothing added
-      rows_of<S>(rg, g + t0 * gl, gl, live);
-      rows_of<S>(ry, dy + t0 * row, row, live);
-      float s[V];
-#pragma unroll
-      for (int v = 0; v < V; ++v) s[v] = live ? p.marks[((long long)b * segs + seg) * p.C + c + v] : 0.f;
+    if constexpr (TILE) {
+      if (threadIdx.x == 0 && round > 0) {  // the stage of the round before takes the next one
+        tiles_read();
+        const int next = tile - (kTileStages - 1) * p.clusters;
+        if (next >= 0) stage_in(ring, m, (round - 1) % kTileStages, c0, next * TT, b, TT / m.boxes);
+      }
+      if (tile >= 0) tile_wait(sm, slot, (round / kTileStages) & 1, p.flags);
 #pragma unroll
       for (int i = 0; i < S; ++i) {
-        float q[V];
-        L::get(rx[i], q);
+        L::get(word<raw>(words + i * lanes * 4), h[i]);
+        L::get(word<raw>(words + ring.tile + i * lanes * 4), a[i]);
+        L::get(word<raw>(words + 2 * ring.tile + i * lanes * 4), d[i]);
+      }
+      if (live < S) {                   // past the length: whatever is there
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+          if (i >= live) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) h[i][v] = a[i][v] = d[i][v] = 0.f;
+          }
+      }
+    } else {
+      raw rx[S], rg[S], ry[S];
+      rows_of<S>(rx, reinterpret_cast<const raw*>(static_cast<const T*>(p.x) + b * p.xb + c) + t0 * xl, xl, live);
+      rows_of<S>(rg, g + t0 * gl, gl, live);
+      rows_of<S>(ry, reinterpret_cast<const raw*>(static_cast<const T*>(p.dy) + at) + t0 * row, row, live);
+#pragma unroll
+      for (int i = 0; i < S; ++i) {
+        L::get(rx[i], h[i]);
         L::get(rg[i], a[i]);
         L::get(ry[i], d[i]);
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          top = fmaxf(top, a[i][v]);
-          a[i][v] = expf(at_most_zero(a[i][v]));
-          h[i][v] = s[v];  // the state before the token
-          const float next = fmaf(a[i][v], s[v], q[v]);
-          s[v] = resets && ((resets >> i) & 1u) ? q[v] : next;
-        }
       }
     }
+    const uint32_t resets = resets_of<S>(p, b, t0, alive, lane, lanes);
     Seg mine[V];
     float e[V];
     bool plain = true;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      float A = 1.f, s = 0.f;
+      float s = live ? p.marks[((long long)b * segs + seg) * p.C + c + v] : 0.f, A = 1.f, back = 0.f;
+#pragma unroll
+      for (int i = 0; i < S; ++i) {
+        top = fmaxf(top, a[i][v]);
+        a[i][v] = expf(at_most_zero(a[i][v]));
+      }
       if (!resets) {
 #pragma unroll
+        for (int i = 0; i < S; ++i) {
+          const float x = h[i][v];
+          h[i][v] = s;                  // the state before the token
+          s = fmaf(a[i][v], s, x);
+        }
+#pragma unroll
         for (int i = S - 1; i >= 0; --i) {
-          s = a[i][v] * (d[i][v] + s);
+          back = a[i][v] * (d[i][v] + back);
           A *= a[i][v];
         }
       } else {
 #pragma unroll
-        for (int i = S - 1; i >= 0; --i) s = ((resets >> i) & 1u) ? 0.f : a[i][v] * (d[i][v] + s);
+        for (int i = 0; i < S; ++i) {
+          const float x = h[i][v];
+          h[i][v] = s;
+          s = ((resets >> i) & 1u) ? x : fmaf(a[i][v], s, x);
+        }
+#pragma unroll
+        for (int i = S - 1; i >= 0; --i) back = ((resets >> i) & 1u) ? 0.f : a[i][v] * (d[i][v] + back);
       }
-      mine[v] = segment<S, V>(a, v, A, s, resets, plain);
+      mine[v] = segment<S, V>(a, v, A, back, resets, plain);
     }
     exchange<V>(sm, round, mine, plain, lanes, rank, p.clusters, enter, e, p.flags);
-    if (on && seg >= 0) {
-      raw* qx = dx + t0 * row;
-      raw* qg = dg + t0 * row;
-      if (live == S && !resets && !(top > 0.f)) {
+    raw* qx = reinterpret_cast<raw*>(static_cast<T*>(p.dx) + at) + t0 * row;
+    raw* qg = reinterpret_cast<raw*>(static_cast<T*>(p.dg) + at) + t0 * row;
+    const int rows = on && tile >= 0 ? (int)max(0ll, min((long long)S, p.L - t0)) : 0;
+    auto put = [&](int i, const float* ox, const float* og) {
+      if constexpr (TILE) {
+        put_word<raw>(words + i * lanes * 4, L::put(ox));
+        put_word<raw>(words + ring.tile + i * lanes * 4, L::put(og));
+      } else if (i < rows) {
+        qx[i * row] = L::put(ox);
+        qg[i * row] = L::put(og);
+      }
+    };
+    if (live == S && !resets && !(top > 0.f)) {
 #pragma unroll
-        for (int i = S - 1; i >= 0; --i) {
-          float ox[V], og[V];
+      for (int i = S - 1; i >= 0; --i) {
+        float ox[V], og[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          ox[v] = d[i][v] + e[v];
+          e[v] = a[i][v] * ox[v];
+          og[v] = e[v] * h[i][v];
+        }
+        put(i, ox, og);
+      }
+    } else {
+#pragma unroll
+      for (int i = S - 1; i >= 0; --i) {
+        float ox[V] = {}, og[V] = {};
+        if (i < live) {
+          const bool r = (resets >> i) & 1u;
+          float gate[V];
+          L::get(g[(t0 + i) * gl], gate);
 #pragma unroll
           for (int v = 0; v < V; ++v) {
             ox[v] = d[i][v] + e[v];
-            e[v] = a[i][v] * ox[v];
-            og[v] = e[v] * h[i][v];
-          }
-          qx[i * row] = L::put(ox);
-          qg[i * row] = L::put(og);
-        }
-      } else {
-        const int rows = (int)min((long long)S, p.L - t0);
-#pragma unroll
-        for (int i = S - 1; i >= 0; --i) {
-          float ox[V] = {}, og[V] = {};
-          if (i < live) {
-            const bool r = (resets >> i) & 1u;
-            float gate[V];
-            L::get(g[(t0 + i) * gl], gate);
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-              ox[v] = d[i][v] + e[v];
-              e[v] = r ? 0.f : a[i][v] * ox[v];
-              og[v] = r || gate[v] > 0.f ? 0.f : e[v] * h[i][v];
-            }
-          }
-          if (i < rows) {
-            qx[i * row] = L::put(ox);
-            qg[i * row] = L::put(og);
+            e[v] = r ? 0.f : a[i][v] * ox[v];
+            og[v] = r || gate[v] > 0.f ? 0.f : e[v] * h[i][v];
           }
         }
+        put(i, ox, og);
+      }
+    }
+    if constexpr (TILE) {
+      fence_async_smem();
+      __syncthreads();
+      if (threadIdx.x == 0 && tile >= 0) {
+        for (int i = 0; i < m.boxes; ++i) {
+          const uint32_t part = i * (ring.tile / m.boxes);
+          tile_out(&m.o0, ring.at(slot, 0) + part, c0, tile * TT + i * (TT / m.boxes), b);
+          tile_out(&m.o1, ring.at(slot, 1) + part, c0, tile * TT + i * (TT / m.boxes), b);
+        }
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       }
     }
   }
-  if (p.dh0 && on && rank == 0 && place == 0) {
+  if (p.dh0 && on && rank == 0 && place == places - 1) {
 #pragma unroll
     for (int v = 0; v < V; ++v) p.dh0[(long long)b * p.C + c + v] = enter[v];
   }
+  if (TILE && threadIdx.x == 0) tiles_done(sm);
   if (p.clusters > 1) cg::this_cluster().sync();  // a CTA's shared memory is written until here
 }
 
@@ -557,43 +726,95 @@ gdn2_status check_gated(const gdn2_gated_desc* d) {
   return GDN2_OK;
 }
 
-struct GatedPlan {
-  int warps, lanes_log2, clusters, cols;
-};
-
-template <class K>
-cudaError_t launch_gated(K kernel, GatedParams& p, int V, cudaStream_t st) {
-  const int S = kValues / V, segs = (p.L + S - 1) / S;
-  // Enough CTAs for two on every SM: narrower ones first (32-byte rows of 8 channels; their lanes take more
-  // segments), then clusters.  8 x 2048 x 768 fp32, forward + backward: 110 us with 192 CTAs of 32 channels, 92 with
-  // 384 of 16, 99 with 768 of 8, 136 with 384 of 32 in pairs; 1 x 131072 x 256: 794 us with 64 CTAs of 32 channels
-  // in clusters of 8, 459 with 128 of 16, 300 with 256 of 8.
-  const GatedPlan pl = [&] {
-    GatedPlan r{0, 5, 1, 0};
-    auto cols = [&] { return (int)((p.C + (long long)(V << r.lanes_log2) - 1) / (V << r.lanes_log2)); };
-    auto groups = [&] { return 32 >> r.lanes_log2; };
-    while (r.lanes_log2 > 3 && (long long)p.B * cols() < 296 && 2 * groups() <= segs) --r.lanes_log2;
-    r.cols = cols();
-    r.warps = (segs + groups() - 1) / groups();
-    r.warps = r.warps < 1 ? 1 : r.warps > kMaxWarps ? kMaxWarps : r.warps;
-    const int places = r.warps * groups();
-    while (r.clusters < kMaxCluster && (long long)p.B * r.cols * r.clusters * 2 <= 296 && r.clusters * places < segs) r.clusters *= 2;
-    return r;
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+// (B, L, C) with rows `sl` and sequences `sb` elements apart, in boxes of `rows` tokens by `width` channels.  False
+// where tiled copies cannot read it.
+bool tile_map(CUtensorMap* map, const void* p, bool bf16, const GatedParams& q, long long sb, long long sl, int width, int rows) {
+  static const EncodeFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &r) == cudaSuccess &&
+                   r == cudaDriverEntryPointSuccess
+               ? reinterpret_cast<EncodeFn>(f)
+               : nullptr;
   }();
-  p.cols = pl.cols;
-  p.clusters = pl.clusters;
-  p.lanes_log2 = pl.lanes_log2;
+  const long long el = bf16 ? 2 : 4;
+  if (q.L == 1) sl = q.C;
+  if (q.B == 1) sb = sl * q.L;
+  sl = (q.L == 1 ? (sl * el + 15) / 16 * 16 : sl * el);
+  sb = (q.B == 1 ? (sb * el + 15) / 16 * 16 : sb * el);
+  if (!fn || reinterpret_cast<uintptr_t>(p) % 16 || sl % 16 || sb % 16 || sl <= 0 || sb <= 0 || sl >= 1ll << 40 || sb >= 1ll << 40)
+    return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)q.C, (cuuint64_t)q.L, (cuuint64_t)q.B};
+  const cuuint64_t strides[2] = {(cuuint64_t)sl, (cuuint64_t)sb};
+  const cuuint32_t box[3] = {(cuuint32_t)width, (cuuint32_t)rows, 1}, unit[3] = {1, 1, 1};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(p), dims, strides,
+            box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <class T, int V, int S>
+cudaError_t launch_gated_as(bool back, GatedParams& p, cudaStream_t st) {
+  constexpr bool kBf16 = sizeof(T) == 2;
+  const int segs = (p.L + S - 1) / S;
+  // Enough CTAs for two on every SM: narrower ones first (32-byte rows of 8 lanes, which then take more segments), then
+  // clusters (forward + backward of 1 x 131072 x 256: 794 us with 64 CTAs of 32 channels in clusters of 8, 459 with
+  // 128 of 16, 300 with 256 of 8; 8 x 2048 x 768: 110 us with 192 of 32, 92 with 384 of 16, 136 with 384 of 32 in
+  // pairs; all before the tiles).
+  int lanes_log2 = 5, clusters = 1;
+  auto cols = [&] { return (int)((p.C + (long long)(V << lanes_log2) - 1) / (V << lanes_log2)); };
+  auto groups = [&] { return 32 >> lanes_log2; };
+  while (lanes_log2 > 3 && (long long)p.B * cols() < 296 && 2 * groups() <= segs) --lanes_log2;
+  int warps = (segs + groups() - 1) / groups();
+  warps = warps < 1 ? 1 : warps > kMaxWarps ? kMaxWarps : warps;
+  if (warps * groups() * S > 256) warps = (warps + 1) / 2 * 2;  // two boxes of a tile, each on 128 bytes
+  const int places = warps * groups(), TT = places * S;
+  while (clusters < kMaxCluster && (long long)p.B * cols() * clusters * 2 <= 296 && clusters * places < segs) clusters *= 2;
+  p.cols = cols();
+  p.clusters = clusters;
+  p.lanes_log2 = lanes_log2;
+  Tiles m;
+  m.boxes = TT > 256 ? 2 : 1;
+  const int width = V << lanes_log2, rows = TT / m.boxes;
+  const long long cb = (long long)p.L * p.C, cl = p.C;
+  bool tile = sizeof(T) * V == 4 && p.L > 0 && tile_map(&m.x, p.x, kBf16, p, p.xb, p.xl, width, rows) &&
+              tile_map(&m.g, p.g, kBf16, p, p.gb, p.gl, width, rows) &&
+              tile_map(&m.o0, back ? p.dx : p.h, kBf16, p, cb, cl, width, rows);
+  if (tile && back)
+    tile = tile_map(&m.dy, p.dy, kBf16, p, cb, cl, width, rows) && tile_map(&m.o1, p.dg, kBf16, p, cb, cl, width, rows);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.B * pl.cols * pl.clusters));
-  cfg.blockDim = dim3(32u * pl.warps);
+  cfg.gridDim = dim3((unsigned)(p.B * p.cols * clusters));
+  cfg.blockDim = dim3(32u * warps);
+  cfg.dynamicSmemBytes = tile ? (size_t)kTileStages * (back ? 3 : 2) * TT * (4u << lanes_log2) : 0;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = (unsigned)pl.clusters;
+  at[0].val.clusterDim.x = (unsigned)clusters;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, p);
+  auto go = [&](auto kernel, unsigned long long& done) {
+    if (cfg.dynamicSmemBytes > 32768) {
+      const cudaError_t e = smem_attr_once(kernel, kTileStages * 3 * kMaxWarps * tokens(1, false) * 32 * 4, done);
+      if (e != cudaSuccess) return e;
+    }
+    return cudaLaunchKernelEx(&cfg, kernel, p, m);
+  };
+  static unsigned long long done[2] = {};
+  if constexpr (sizeof(T) * V == 4) {
+    if (tile) return back ? go(gated_bwd_kernel<T, V, S, true>, done[1]) : go(gated_fwd_kernel<T, V, S, true>, done[0]);
+  }
+  return back ? go(gated_bwd_kernel<T, V, S, false>, done[1]) : go(gated_fwd_kernel<T, V, S, false>, done[0]);
+}
+
+// Enough channels for more than one CTA of 16 lanes on every SM's two places.
+bool many(long long B, long long C, int V) { return B * ((C + 16 * V - 1) / (16 * V)) >= 296; }
+template <class T, int V>
+cudaError_t launch_gated(bool back, GatedParams& p, cudaStream_t st) {
+  return many(p.B, p.C, V) ? launch_gated_as<T, V, tokens(V, true)>(back, p, st)
+                           : launch_gated_as<T, V, tokens(V, false)>(back, p, st);
 }
 
 GatedParams params_of(const gdn2_gated_desc* d) {
@@ -612,7 +833,8 @@ size_t access(const gdn2_gated_desc* d) { return d->dtype == GDN2_F32 || pairs(d
 extern "C" size_t gdn2_gated_marks_bytes(const gdn2_gated_desc* d) {
   using namespace gdn2;
   if (check_gated(d) != GDN2_OK) return 0;
-  const long long S = kValues / (pairs(d) ? 2 : 1);
+  const int V = pairs(d) ? 2 : 1;
+  const long long S = tokens(V, many(d->B, d->C, V));
   return (size_t)d->B * (size_t)((d->L + S - 1) / S) * (size_t)d->C * sizeof(float);
 }
 
@@ -641,11 +863,11 @@ extern "C" gdn2_status gdn2_gated_fwd(const gdn2_gated_desc* d, const void* x, c
     else gated_step_kernel<__nv_bfloat16, 1><<<grid, 128, 0, st>>>(p);
     e = cudaGetLastError();
   } else if (d->dtype == GDN2_F32) {
-    e = launch_gated(gated_fwd_kernel<float, 1>, p, 1, st);
+    e = launch_gated<float, 1>(false, p, st);
   } else if (pairs(d)) {
-    e = launch_gated(gated_fwd_kernel<__nv_bfloat16, 2>, p, 2, st);
+    e = launch_gated<__nv_bfloat16, 2>(false, p, st);
   } else {
-    e = launch_gated(gated_fwd_kernel<__nv_bfloat16, 1>, p, 1, st);
+    e = launch_gated<__nv_bfloat16, 1>(false, p, st);
   }
   return e == cudaSuccess ? GDN2_OK : GDN2_ERR_CUDA;
 }
@@ -665,8 +887,8 @@ extern "C" gdn2_status gdn2_gated_bwd(const gdn2_gated_desc* d, const void* x, c
   p.x = x; p.g = g; p.lengths = lengths; p.reset = reset; p.marks = const_cast<float*>(marks);
   p.dy = dh; p.dlast = dlast; p.dx = dx; p.dg = dg; p.dh0 = dh0; p.flags = flags;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = d->dtype == GDN2_F32 ? launch_gated(gated_bwd_kernel<float, 1>, p, 1, st)
-                        : pairs(d)           ? launch_gated(gated_bwd_kernel<__nv_bfloat16, 2>, p, 2, st)
-                                             : launch_gated(gated_bwd_kernel<__nv_bfloat16, 1>, p, 1, st);
+  const cudaError_t e = d->dtype == GDN2_F32 ? launch_gated<float, 1>(true, p, st)
+                        : pairs(d)           ? launch_gated<__nv_bfloat16, 2>(true, p, st)
+                                             : launch_gated<__nv_bfloat16, 1>(true, p, st);
   return e == cudaSuccess ? GDN2_OK : GDN2_ERR_CUDA;
 }
