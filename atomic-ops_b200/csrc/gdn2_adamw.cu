@@ -194,15 +194,53 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_prepare_kernel(const __gri
   count_up(t);
 }
 
-// One value's moments, every operation rounded by itself.
-__device__ __forceinline__ void moments(float g, float& m, float& v, const AdamParams& a) {
-  m = __fadd_rn(__fmul_rn(a.fb1, m), __fmul_rn(a.gb1, g));
-  v = __fadd_rn(__fmul_rn(a.fb2, v), __fmul_rn(a.gb2, __fmul_rn(g, g)));
+// Two fp32 values in a register pair: one instruction multiplies both, each rounded to nearest.  Sums of two products
+// are scalar: a packed sum came out joined with its product, rounded once.
+using Two = unsigned long long;
+__device__ __forceinline__ Two two(float a, float b) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
 }
-// Its step from m and the root of v.  The quotient is within 3 ulp: that is 2^-22 of a step, which is itself
-// some 2^-6 of p or less.
-__device__ __forceinline__ float stepped(float p, float m, float r, const Factors& f, const AdamParams& a) {
-  return fmaf(p, f.decay, -f.size * __fdividef(m, fmaf(r, f.root, a.eps)));
+__device__ __forceinline__ Two both(float a) { return two(a, a); }
+__device__ __forceinline__ void apart(Two x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ Two mul(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ Two add(Two a, Two b) {
+  float x[2], y[2];
+  apart(a, x[0], x[1]);
+  apart(b, y[0], y[1]);
+  return two(__fadd_rn(x[0], y[0]), __fadd_rn(x[1], y[1]));
+}
+__device__ __forceinline__ Two fma(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+struct Steps {                          // a tensor's factors and the step's, twice each
+  Two size, root, decay, coef, b1, g1, b2, g2, eps;
+};
+__device__ __forceinline__ Steps steps_of(const Factors& f, const AdamParams& a, float coef) {
+  return {both(-f.size), both(f.root), both(f.decay), both(coef), both(a.fb1), both(a.gb1), both(a.fb2), both(a.gb2), both(a.eps)};
+}
+// Two values' moments, every operation rounded by itself.
+__device__ __forceinline__ void moments(Two g, Two& m, Two& v, const Steps& s) {
+  g = mul(g, s.coef);
+  m = add(mul(s.b1, m), mul(s.g1, g));
+  v = add(mul(s.b2, v), mul(s.g2, mul(g, g)));
+}
+// Their step from m and the roots of v.  The quotient is within 3 ulp: that is 2^-22 of a step, which is itself some
+// 2^-6 of p or less.
+__device__ __forceinline__ Two stepped(Two p, Two m, Two r, const Steps& s) {
+  float a, b;
+  apart(fma(r, s.root, s.eps), a, b);
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(a));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(b));
+  return fma(p, s.decay, mul(s.size, mul(m, two(a, b))));
 }
 __device__ __forceinline__ float root_near(float v) {  // within an ulp
   float r;
@@ -261,61 +299,67 @@ __device__ __forceinline__ void codes4(uint8_t* p, uint32_t c, bool vec, int n) 
   }
 }
 
-__device__ __forceinline__ void decode_m(uint32_t c, float scale, float v[4]) {
+// The values of four codes, in pairs.
+__device__ __forceinline__ void decode_m(uint32_t c, Two scale, Two v[2]) {
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(c >> (16 * j)), __NV_E4M3);
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-    v[2 * j] = __fmul_rn(f.x, scale);
-    v[2 * j + 1] = __fmul_rn(f.y, scale);
+    v[j] = mul(two(f.x, f.y), scale);
   }
 }
-__device__ __forceinline__ void decode_v(uint32_t c, float scale, float v[4]) {
+__device__ __forceinline__ void decode_v(uint32_t c, Two scale, Two v[2]) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    // the code's bits are a float's exponent and mantissa, 2^112 too small
-    const float r = __fmul_rn(__uint_as_float(((c >> (8 * j)) & 255u) << 19) * 0x1p112f, scale);
-    v[j] = __fmul_rn(r, r);
+  for (int j = 0; j < 2; ++j) {
+    // a code's bits are a float's exponent and mantissa, 2^112 too small
+    const uint32_t lo = (j ? c << 3 : c << 19) & 0x07f80000u, hi = (j ? c >> 5 : c << 11) & 0x07f80000u;
+    const Two r = mul(mul(two(__uint_as_float(lo), __uint_as_float(hi)), both(0x1p112f)), scale);
+    v[j] = mul(r, r);
   }
 }
-// The scale of a warp's block from its lanes' largest magnitude, and what values are multiplied by (0: all are stored
-// as zero).  Compared as bits, so that a NaN is the largest.
-__device__ __forceinline__ float scale_of(float largest, float inverse_top, float& up) {
-  const float s = __fmul_rn(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(largest))), inverse_top);
+// The scale of a warp's block from its lanes' largest magnitude, as bits (so that a NaN is the largest), and what values
+// are multiplied by (0: all are stored as zero).
+__device__ __forceinline__ float scale_of(uint32_t largest, float inverse_top, float& up) {
+  const float s = __fmul_rn(__uint_as_float(__reduce_max_sync(0xffffffffu, largest)), inverse_top);
   up = s >= kNormal ? __frcp_rn(s) : 0.f;
   return s;
 }
-__device__ __forceinline__ uint32_t encode_m(const float v[4], float up) {
+__device__ __forceinline__ uint32_t encode_m(const Two v[2], Two up) {
   uint32_t c = 0;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    const float2 f = make_float2(__fmul_rn(v[2 * j], up), __fmul_rn(v[2 * j + 1], up));  // at most 448 and an ulp
+    float2 f;                           // at most 448 and an ulp
+    apart(mul(v[j], up), f.x, f.y);
     c |= (uint32_t)__nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3) << (16 * j);
   }
   return c;
 }
-__device__ __forceinline__ uint32_t encode_r(const float r[4], float up) {
+__device__ __forceinline__ uint32_t encode_r(const Two r[2], Two up) {
   uint32_t c = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float x = __fmul_rn(r[j], up);  // at most 1.9375 and an ulp
-    const uint32_t u = __float_as_uint(x);
-    uint32_t k = x >= 0x1p-14f ? ((u + 0x3ffffu + ((u >> 19) & 1u)) >> 19) - (112u << 4) : (uint32_t)__float2int_rn(x * 0x1p18f);
-    if (r[j] > 0.f && k == 0) k = 1;
+    float x[2], w[2];                   // x: at most 1.9375 and an ulp
+    apart(mul(r[j / 2], up), x[0], x[1]);
+    apart(r[j / 2], w[0], w[1]);
+    const float y = x[j & 1];
+    const uint32_t u = __float_as_uint(y);
+    // to nearest, ties to even: at a normal number's fourth bit, or below 2^-14 to a multiple of 2^-18 (in the low bits
+    // of a sum with 1.5 x 2^23)
+    uint32_t k = y >= 0x1p-14f ? ((u + 0x3ffffu + ((u >> 19) & 1u)) >> 19) - (112u << 4)
+                               : __float_as_uint(__fmaf_rn(y, 0x1p18f, 12582912.f)) & 31u;
+    k = max(k, min(__float_as_uint(w[j & 1]), 1u));   // a root above zero is at least code 1
     c |= (k & 255u) << (8 * j);
   }
   return c;
 }
-__device__ __forceinline__ float magnitude(float a, float b) {  // the larger magnitude; a NaN is the largest
-  return __uint_as_float(max(__float_as_uint(a) & 0x7fffffffu, __float_as_uint(b) & 0x7fffffffu));
-}
 
 // 4 values of a thread, 8 bits: 8 of a lane, a warp to a block.  WHOLE: a full chunk, read 4 values at a time.
 template <class T, bool EIGHT, bool WHOLE>
-__device__ __forceinline__ void chunk_update(const AdamEntry& e, const AdamParams& a, const Factors& f, float coef,
-                                             long long at, int n) {
+__device__ __forceinline__ void chunk_update(const AdamEntry& e, const Steps& st, long long at, int n) {
   T* p = static_cast<T*>(e.p) + at;
   const T* g = static_cast<const T*>(e.g) + at;
+  auto pairs = [](const float v[4], Two q[2]) { q[0] = two(v[0], v[1]); q[1] = two(v[2], v[3]); };
+  auto singles = [](const Two q[2], float v[4]) { apart(q[0], v[0], v[1]); apart(q[1], v[2], v[3]); };
   if constexpr (!EIGHT) {
     float* m = static_cast<float*>(e.m) + at;
     float* v = static_cast<float*>(e.v) + at;
@@ -334,11 +378,21 @@ __device__ __forceinline__ void chunk_update(const AdamEntry& e, const AdamParam
       for (int h = 0; h < 2; ++h) {
         const int i = i0 + h * kAdamThreads * 4;
         const bool vec = WHOLE || (e.vec && i + 4 <= n);
+        Two xs[2], gs[2], ms[2], vs[2];
+        pairs(x[h], xs);
+        pairs(y[h], gs);
+        pairs(mm[h], ms);
+        pairs(vv[h], vs);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          moments(__fmul_rn(y[h][j], coef), mm[h][j], vv[h][j], a);
-          x[h][j] = stepped(x[h][j], mm[h][j], root_near(vv[h][j]), f, a);
+        for (int j = 0; j < 2; ++j) {
+          moments(gs[j], ms[j], vs[j], st);
+          float a, b;
+          apart(vs[j], a, b);
+          xs[j] = stepped(xs[j], ms[j], two(root_near(a), root_near(b)), st);
         }
+        singles(xs, x[h]);
+        singles(ms, mm[h]);
+        singles(vs, vv[h]);
         store4(p + i, x[h], vec, n - i);
         store4(m + i, mm[h], vec, n - i);
         store4(v + i, vv[h], vec, n - i);
@@ -348,34 +402,67 @@ __device__ __forceinline__ void chunk_update(const AdamEntry& e, const AdamParam
     uint8_t* m = static_cast<uint8_t*>(e.m) + at;
     uint8_t* v = static_cast<uint8_t*>(e.v) + at;
     const int lane = threadIdx.x & 31;
-    for (int blk = threadIdx.x >> 5; blk * kBlock < n; blk += kAdamThreads / 32) {
-      const long long s = at / kBlock + blk;
-      const float ms = e.ms[s], vs = e.vs[s];
-      float x[2][4], y[2][4], mm[2][4], vv[2][4], r[2][4], top_m = 0.f, top_r = 0.f;
-      uint32_t cm[2], cv[2];
+    float nx[2][4], ny[2][4], nms, nvs;
+    uint32_t ncm[2], ncv[2];
+    auto load = [&](int blk) {
+      nms = e.ms[at / kBlock + blk];
+      nvs = e.vs[at / kBlock + blk];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int i = blk * kBlock + h * 128 + lane * 4;
         const bool vec = WHOLE || (e.vec && n - i >= 4);
-        load4(p + i, x[h], vec, n - i);
-        load4(g + i, y[h], vec, n - i);
-        cm[h] = codes4(m + i, vec, n - i);
-        cv[h] = codes4(v + i, vec, n - i);
+        load4(p + i, nx[h], vec, n - i);
+        load4(g + i, ny[h], vec, n - i);
+        ncm[h] = codes4(m + i, vec, n - i);
+        ncv[h] = codes4(v + i, vec, n - i);
       }
+    };
+    if (WHOLE) load(threadIdx.x >> 5);
+    for (int blk = threadIdx.x >> 5; blk * kBlock < n; blk += kAdamThreads / 32) {
+      const long long s = at / kBlock + blk;
+      if (!WHOLE) load(blk);
+      const float ms = nms, vs = nvs;
+      float x[2][4], y[2][4];
+      Two mm[2][2], r[2][2];
+      uint32_t cm[2], cv[2], top_m = 0, top_r = 0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        cm[h] = ncm[h];
+        cv[h] = ncv[h];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          x[h][j] = nx[h][j];
+          y[h][j] = ny[h][j];
+        }
+      }
+      if (WHOLE && blk + kAdamThreads / 32 < kChunk / kBlock) load(blk + kAdamThreads / 32);  // before this block's work
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int left = n - (blk * kBlock + h * 128 + lane * 4);
-        decode_m(cm[h], ms, mm[h]);
-        decode_v(cv[h], vs, vv[h]);
+        Two xs[2], gs[2], vv[2];
+        pairs(x[h], xs);
+        pairs(y[h], gs);
+        decode_m(cm[h], both(ms), mm[h]);
+        decode_v(cv[h], both(vs), vv);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          moments(__fmul_rn(y[h][j], coef), mm[h][j], vv[h][j], a);
-          if (!WHOLE && j >= left) mm[h][j] = vv[h][j] = 0.f;  // past the tensor's end
-          r[h][j] = __fsqrt_rn(vv[h][j]);
-          x[h][j] = stepped(x[h][j], mm[h][j], r[h][j], f, a);
-          top_m = magnitude(top_m, mm[h][j]);
-          top_r = magnitude(top_r, r[h][j]);
+        for (int j = 0; j < 2; ++j) {
+          moments(gs[j], mm[h][j], vv[j], st);
+          float a, b, c, d;
+          apart(mm[h][j], a, b);
+          apart(vv[j], c, d);
+          if (!WHOLE) {                 // past the tensor's end
+            if (2 * j >= left) a = c = 0.f;
+            if (2 * j + 1 >= left) b = d = 0.f;
+            mm[h][j] = two(a, b);
+          }
+          c = __fsqrt_rn(c);
+          d = __fsqrt_rn(d);
+          r[h][j] = two(c, d);
+          xs[j] = stepped(xs[j], mm[h][j], r[h][j], st);
+          top_m = max(top_m, max(__float_as_uint(a) & 0x7fffffffu, __float_as_uint(b) & 0x7fffffffu));
+          top_r = max(top_r, max(__float_as_uint(c) & 0x7fffffffu, __float_as_uint(d) & 0x7fffffffu));
         }
+        singles(xs, x[h]);
       }
       float up_m, up_r;
       const float new_ms = scale_of(top_m, 1.f / 448.f, up_m), new_vs = scale_of(top_r, 1.f / 1.9375f, up_r);
@@ -384,8 +471,8 @@ __device__ __forceinline__ void chunk_update(const AdamEntry& e, const AdamParam
         const int i = blk * kBlock + h * 128 + lane * 4;
         const bool vec = WHOLE || (e.vec && n - i >= 4);
         store4(p + i, x[h], vec, n - i);
-        codes4(m + i, encode_m(mm[h], up_m), vec, n - i);
-        codes4(v + i, encode_r(r[h], up_r), vec, n - i);
+        codes4(m + i, encode_m(mm[h], both(up_m)), vec, n - i);
+        codes4(v + i, encode_r(r[h], both(up_r)), vec, n - i);
       }
       if (lane == 0) {
         e.ms[s] = new_ms;
@@ -396,7 +483,7 @@ __device__ __forceinline__ void chunk_update(const AdamEntry& e, const AdamParam
 }
 
 template <int N, bool EIGHT>
-__global__ void __launch_bounds__(kAdamThreads, 4) adamw_update_kernel(const __grid_constant__ AdamTable<N> t,
+__global__ void __launch_bounds__(kAdamThreads, EIGHT ? 3 : 4) adamw_update_kernel(const __grid_constant__ AdamTable<N> t,
                                                                     const __grid_constant__ AdamParams a) {
   pdl_enter();
   if (__ldcg(&a.ctl->ok) == 0.f) return;
@@ -409,11 +496,11 @@ __global__ void __launch_bounds__(kAdamThreads, 4) adamw_update_kernel(const __g
     const long long at = (long long)(chunk - e.first) * kChunk;
     const int n = (int)min((long long)kChunk, e.n - at);
     const bool whole = e.vec && n == kChunk;
+    const Steps s = steps_of(f, a, coef);
     if (e.bf16)
-      whole ? chunk_update<__nv_bfloat16, EIGHT, true>(e, a, f, coef, at, kChunk)
-            : chunk_update<__nv_bfloat16, EIGHT, false>(e, a, f, coef, at, n);
+      whole ? chunk_update<__nv_bfloat16, EIGHT, true>(e, s, at, kChunk) : chunk_update<__nv_bfloat16, EIGHT, false>(e, s, at, n);
     else
-      whole ? chunk_update<float, EIGHT, true>(e, a, f, coef, at, kChunk) : chunk_update<float, EIGHT, false>(e, a, f, coef, at, n);
+      whole ? chunk_update<float, EIGHT, true>(e, s, at, kChunk) : chunk_update<float, EIGHT, false>(e, s, at, n);
   }
 }
 
@@ -443,9 +530,14 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_moments_kernel(const __gri
       for (int h = 0; h < 2; ++h) {
         const int i = blk * kBlock + h * 128 + lane * 4;
         float x[4];
-        decode_m(cm[h], ms, x);
+        Two q[2];
+        decode_m(cm[h], both(ms), q);
+        apart(q[0], x[0], x[1]);
+        apart(q[1], x[2], x[3]);
         store4(om + i, x, e.vec && n - i >= 4, n - i);
-        decode_v(cv[h], vs, x);
+        decode_v(cv[h], both(vs), q);
+        apart(q[0], x[0], x[1]);
+        apart(q[1], x[2], x[3]);
         store4(ov + i, x, e.vec && n - i >= 4, n - i);
       }
     }
@@ -554,9 +646,10 @@ cudaError_t run_adamw(const gdn2_adamw_desc* d, const gdn2_adamw_tensor* ts, int
   for (int i = 0; i < n && e == cudaSuccess;) {
     i = fill(t, d, ts, i, n);
     if (!t.count) break;
-    // codes: a CTA walks several chunks (8 bits, 348 M bf16 weights: 945 us; a CTA for each chunk 1235); 32 bits
-    // move more bytes than they compute and are better off with the scheduler's order (39 M weights: 161, not 174 us)
-    const unsigned grid = (unsigned)(d->state_bits == 8 && t.chunks > 148 * 8 ? 148 * 8 : t.chunks);
+    // codes: as many CTAs as are at work at a time, each walks its chunks (8 bits, 39 M fp32 weights: 125 us; 132 with
+    // 1184 CTAs, 146 with one for each chunk); 32 bits move more bytes than they compute and are better off with the
+    // scheduler's order (39 M weights: 161, not 174 us)
+    const unsigned grid = (unsigned)(d->state_bits == 8 && t.chunks > 148 * 3 ? 148 * 3 : t.chunks);
     e = d->state_bits == 8 ? launch_pdl(adamw_update_kernel<N, true>, grid, kAdamThreads, 0, st, t, a)
                            : launch_pdl(adamw_update_kernel<N, false>, grid, kAdamThreads, 0, st, t, a);
     a.tensor0 += t.count;
