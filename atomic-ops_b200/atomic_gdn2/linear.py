@@ -9,8 +9,8 @@ residual, W stored (din, dout) as in the layers.  x, W and the residual are all 
   go on in rounded fp32 additions: errors are those of a plain fp32 product.  Magnitudes below about 2^-110 lose
   their low bits.
 
-Up to 16 rows of x are multiplied without the tensor cores, W read once per eight rows.  Infinities and NaN come
-out as the plain sums would have them.
+Up to 16 rows of fp32 x (4 of bf16) are multiplied without the tensor cores, W read once per eight rows.  Infinities
+and NaN come out as the plain sums would have them.
 """
 from __future__ import annotations
 

@@ -575,10 +575,24 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const float* parts, in
 }
 
 // ---- operands in the form that the copies need --------------------------------------------------
-// Eight neighbouring values of a row, zeros past its end; `whole`: eight that may be read 16 bytes at a time.
+// Eight neighbouring values of a row, zeros past its end; `whole`: eight that may be read 16 bytes at a time.  bf16 rows
+// that start anywhere are read 4 bytes at a time all the same, and shifted where they start between two words.
 template <class T>
 __device__ __forceinline__ void load8(const T* p, float v[8], bool whole, int left) {
-  if (whole) {
+  if (sizeof(T) == 2 && !whole && left > 8) {
+    const bool off = reinterpret_cast<uintptr_t>(p) & 2u;
+    const uint32_t* q = reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(p) - (off ? 2 : 0));
+    uint32_t w[5];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __ldg(q + i);
+    w[4] = off ? __ldg(q + 4) : 0u;     // up to the ninth value
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t u = off ? __funnelshift_r(w[i], w[i + 1], 16) : w[i];
+      v[2 * i] = __uint_as_float(u << 16);
+      v[2 * i + 1] = __uint_as_float(u & 0xffff0000u);
+    }
+  } else if (whole) {
     if constexpr (sizeof(T) == 4) {
       ld4(p, v);
       ld4(p + 4, v + 4);
@@ -693,9 +707,13 @@ __global__ void __launch_bounds__(256) linear_db_kernel(const float* parts, int 
 }
 
 // ---- few rows -----------------------------------------------------------------------------------
-// Up to 16 rows of x: W is read once, straight into fp32 products.  A CTA takes 32 V columns and a stretch of
-// the sum, its eight warps and the CTAs of a cluster shares of it; their parts meet in shared memory.
-constexpr int kFewRows = 16, kFewStretch = 512;
+// Up to 8 rows of x a launch: W is read once, straight into fp32 products.  A CTA takes 32 V columns and a stretch of
+// the sum, its eight warps and the CTAs of a cluster shares of it; their parts meet in shared memory.  The loads of W
+// bound it: four rows of it (bf16:
+// eight) are on their way while as many are multiplied, and the first ones before x is looked at.
+constexpr int kFewStretch = 256;
+template <class T>
+constexpr int kFewBatch = 16 / (int)sizeof(T);
 
 struct FewParams {
   Epilogue ep;
@@ -703,29 +721,48 @@ struct FewParams {
   long long ldx, ldw;
   int rows, cols, k, clusters;
 };
+// V values of a row of W as they are in memory: 4 of bf16 in two registers.
 template <class T, int V>
-__device__ __forceinline__ void load_w(const T* p, float v[V], bool whole, int left) {
-  if (whole) {
-    if constexpr (V == 4) {
-      ld4(p, v);
-    } else if constexpr (V == 2 && sizeof(T) == 4) {
-      const float2 f = __ldg(reinterpret_cast<const float2*>(p));
-      v[0] = f.x; v[1] = f.y;
-    } else if constexpr (V == 2) {
-      const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p));
-      v[0] = f.x; v[1] = f.y;
+struct Raw {
+  float x[V];
+  __device__ __forceinline__ void load(const T* p, bool whole, int left) {
+    if (whole) {
+      if constexpr (V == 4) ld4(p, x);
+      else x[0] = ld1(p);
     } else {
-      v[0] = ld1(p);
-    }
-  } else {
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = j < left ? ld1(p + j) : 0.f;
+      for (int j = 0; j < V; ++j) x[j] = j < left ? ld1(p + j) : 0.f;
+    }
   }
-}
+  __device__ __forceinline__ void get(float v[V]) const {
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = x[j];
+  }
+};
+template <>
+struct Raw<__nv_bfloat16, 4> {
+  uint2 x;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p, bool whole, int left) {
+    if (whole) {
+      x = __ldg(reinterpret_cast<const uint2*>(p));
+    } else {
+      uint32_t h[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) h[j] = j < left ? __ldg(reinterpret_cast<const unsigned short*>(p) + j) : 0u;
+      x = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+    }
+  }
+  __device__ __forceinline__ void get(float v[4]) const {
+    v[0] = __uint_as_float(x.x << 16);
+    v[1] = __uint_as_float(x.x & 0xffff0000u);
+    v[2] = __uint_as_float(x.y << 16);
+    v[3] = __uint_as_float(x.y & 0xffff0000u);
+  }
+};
 template <class T, int V, int R>
 __global__ void __launch_bounds__(256) linear_few_kernel(const __grid_constant__ FewParams p) {
-  __shared__ float xs[R][kFewStretch];
-  __shared__ float part[8][R][32 * V];
+  __shared__ __align__(16) float xs[kFewStretch][R];
+  __shared__ __align__(16) float part[8][R][32 * V];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rank = blockIdx.x % p.clusters, c = (blockIdx.x / p.clusters * 32 + lane) * V;
   const int share = (p.k + p.clusters - 1) / p.clusters, k0 = rank * share, k1 = min(p.k, k0 + share);
@@ -737,31 +774,53 @@ __global__ void __launch_bounds__(256) linear_few_kernel(const __grid_constant__
 #pragma unroll
   for (int r = 0; r < R; ++r)
 #pragma unroll
-    for (int j = 0; j < V; ++j) acc[r][j] = 0.f;
+    for (int i = 0; i < V; ++i) acc[r][i] = 0.f;
   for (int s = k0; s < k1; s += kFewStretch) {
     const int n = min(kFewStretch, k1 - s);
-    __syncthreads();
+    constexpr int U = kFewBatch<T>;
+    Raw<T, V> now[U], next[U];
+    auto load = [&](int j0, Raw<T, V>* v) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (j0 + 8 * u < n && left > 0) v[u].load(w + (long long)(s + j0 + 8 * u) * p.ldw, whole, left);
+    };
+    load(warp, now);
+    __syncthreads();                    // xs was read
     for (int i = threadIdx.x; i < R * n; i += 256) {
       const int r = i / n, j = i - r * n;
-      xs[r][j] = r < p.rows ? to_f<T>(x[r * p.ldx + s + j]) : 0.f;
+      xs[j][r] = r < p.rows ? to_f<T>(x[r * p.ldx + s + j]) : 0.f;
     }
     __syncthreads();
-    if (left > 0) {
-#pragma unroll 8
-      for (int j = warp; j < n; j += 8) {
-        float v[V];
-        load_w<T, V>(w + (long long)(s + j) * p.ldw, v, whole, left);
+    for (int j0 = warp; j0 < n; j0 += 8 * U) {
+      load(j0 + 8 * U, next);
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+      for (int u = 0; u < U; ++u) {
+        const int j = j0 + 8 * u;
+        if (j < n && left > 0) {
+          float xr[R], v[V];
+          now[u].get(v);
+          if constexpr (R % 4 == 0) {
 #pragma unroll
-          for (int i = 0; i < V; ++i) acc[r][i] = fmaf(xs[r][j], v[i], acc[r][i]);
+            for (int r = 0; r < R; r += 4) *reinterpret_cast<float4*>(xr + r) = *reinterpret_cast<const float4*>(&xs[j][r]);
+          } else {
+#pragma unroll
+            for (int r = 0; r < R; ++r) xr[r] = xs[j][r];
+          }
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int i = 0; i < V; ++i) acc[r][i] = fmaf(xr[r], v[i], acc[r][i]);
+        }
       }
+#pragma unroll
+      for (int u = 0; u < U; ++u) now[u] = next[u];
     }
   }
 #pragma unroll
-  for (int r = 0; r < R; ++r)
-#pragma unroll
-    for (int i = 0; i < V; ++i) part[warp][r][lane * V + i] = acc[r][i];
+  for (int r = 0; r < R; ++r) {
+    if constexpr (V == 4) *reinterpret_cast<float4*>(&part[warp][r][lane * 4]) = make_float4(acc[r][0], acc[r][1], acc[r][2], acc[r][3]);
+    else part[warp][r][lane] = acc[r][0];
+  }
   __syncthreads();
   for (int i = threadIdx.x; i < R * 32 * V; i += 256) {
     const int r = i / (32 * V), j = i % (32 * V);
@@ -777,8 +836,12 @@ __global__ void __launch_bounds__(256) linear_few_kernel(const __grid_constant__
     if (col >= p.cols) continue;
     float s = part[0][r][j];
     if (p.clusters > 1) {
+      float q[8];                       // all on their way at once
+#pragma unroll
+      for (int u = 0; u < 8; ++u) q[u] = u < p.clusters ? cg::this_cluster().map_shared_rank(&part[0][r][j], u)[0] : 0.f;
       s = 0.f;
-      for (int u = 0; u < p.clusters; ++u) s += cg::this_cluster().map_shared_rank(&part[0][r][j], u)[0];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s += q[u];
     }
     finish(p.ep, r, col, s, p.k, p.ep.bias ? load_f(p.ep.bias, col, p.ep.bias_bf16) : 0.f);
   }
@@ -827,8 +890,8 @@ GemmPlan plan_gemm(long long rows, long long cols, long long k, int terms) {
   GemmPlan g{};
   g.kblocks = (int)((k + kBK - 1) / kBK);
   // Single CTAs or pairs, by what the busiest SM has to do: a block of the sum takes a pair 512 cycles and a
-  // single CTA, which reads its operands from shared memory twice as often, about 320; an epilogue of 128 columns
-  // about 3000.  (bf16, 777 x 1001 x 2503: 22.5 us as 40 pairs, XX as 140 CTAs.)
+  // single CTA, whose operands come from L2 and shared memory twice as often, about 320 (measured 500 to 700); an
+  // epilogue of 128 columns about 3000.  (bf16, 777 x 1001 x 2503: 22.5 us as 40 pairs, 15.6 as 140 CTAs.)
   long long best = 0;
   for (int cg = 1; cg <= 2; ++cg) {
     const int t = 128 * cg, workers = kSMs / cg;
@@ -945,13 +1008,17 @@ gdn2_status check_linear(const gdn2_linear_desc* d) {
 bool off(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n != 0; }
 size_t element(const gdn2_linear_desc* d) { return d->dtype == GDN2_BF16 ? 2 : 4; }
 
+// Rows that are multiplied without the tensor cores.  fp32: where W would first be cut into terms (8 x 512 x 4608 10.7 us
+// against 16.3, 16 x 4096 x 4096 43 against about 50); bf16 rows are few where a launch less counts (4 x 512 x 4608 5.8 us
+// against 8.1; of 8 rows 11.2 against 8.1, 8 x 4096 x 4096 21 against 15).
+int few_rows(const gdn2_linear_desc* d) { return d->dtype == GDN2_F32 ? 16 : 4; }
 struct FwdPlan {
   bool few, x_terms, w_terms;
   size_t x_at, w_at, parts_at, total;
 };
 FwdPlan plan_fwd(const gdn2_linear_desc* d, bool x_direct, bool w_direct) {
   FwdPlan f{};
-  f.few = d->M <= kFewRows;
+  f.few = d->M <= few_rows(d);
   if (f.few) return f;
   f.x_terms = !x_direct;
   f.w_terms = !w_direct;
@@ -993,7 +1060,7 @@ template <class T, int V>
 cudaError_t launch_few(FewParams p, cudaStream_t st) {
   const long long blocks = (p.cols + 32 * V - 1) / (32 * V);
   p.clusters = 1;
-  while (p.clusters < 8 && blocks * p.clusters < 2 * kSMs && p.k / p.clusters >= 128) p.clusters *= 2;
+  while (p.clusters < 8 && blocks * p.clusters < 2 * kSMs && p.k / p.clusters >= 64) p.clusters *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(blocks * p.clusters));
   cfg.blockDim = dim3(256);
@@ -1005,8 +1072,14 @@ cudaError_t launch_few(FewParams p, cudaStream_t st) {
   cfg.attrs = at;
   cfg.numAttrs = 1;
   if (p.rows == 1) return cudaLaunchKernelEx(&cfg, linear_few_kernel<T, V, 1>, p);
-  if (p.rows <= 4) return cudaLaunchKernelEx(&cfg, linear_few_kernel<T, V, 4>, p);
-  return cudaLaunchKernelEx(&cfg, linear_few_kernel<T, V, 8>, p);
+  if constexpr (sizeof(T) == 4)
+    if (p.rows > 4) return cudaLaunchKernelEx(&cfg, linear_few_kernel<T, V, 8>, p);
+  return cudaLaunchKernelEx(&cfg, linear_few_kernel<T, V, 4>, p);
+}
+// Four columns to a lane where that leaves a CTA for every SM.
+template <class T>
+cudaError_t launch_few(const FewParams& p, cudaStream_t st) {
+  return (p.cols + 127) / 128 * 8 >= kSMs ? launch_few<T, 4>(p, st) : launch_few<T, 1>(p, st);
 }
 cudaError_t run_few(const gdn2_linear_desc* d, const FewParams& all, cudaStream_t st) {
   for (int r = 0; r < d->M; r += 8) {   // eight rows a launch
@@ -1017,7 +1090,7 @@ cudaError_t run_few(const gdn2_linear_desc* d, const FewParams& all, cudaStream_
     p.ep.y = static_cast<uint8_t*>(p.ep.y) + (size_t)r * p.ep.ldy * el;
     if (p.ep.z) p.ep.z = static_cast<uint8_t*>(p.ep.z) + (size_t)r * p.ep.ldy * el;
     if (p.ep.residual) p.ep.residual = static_cast<const uint8_t*>(p.ep.residual) + (size_t)r * p.ep.ldr * el;
-    const cudaError_t e = d->dtype == GDN2_F32 ? launch_few<float, 1>(p, st) : launch_few<__nv_bfloat16, 2>(p, st);
+    const cudaError_t e = d->dtype == GDN2_F32 ? launch_few<float>(p, st) : launch_few<__nv_bfloat16>(p, st);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
