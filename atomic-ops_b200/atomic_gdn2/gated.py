@@ -129,7 +129,7 @@ def gated_scan(x: torch.Tensor, g: torch.Tensor, h0=None, *, lengths=None, reset
       reset    (B, L) bool: tokens that drop the state before them
       h_index  (B) the row of h0 that each sequence starts from, negative for zeros (beam_select's rows)
       h_out    (B, C) fp32 contiguous, written and returned as `last` (an in-place change to autograd); it may
-               be h0 itself, or without h_index overlap nothing of it
+               be h0 itself where there is no h_index, and overlaps no input otherwise
     Returns h (B, L, C) of x's type and last (B, C) fp32, the state after each sequence's last token.
     Differentiable in x, g and h0, but not with h_index or h_out: those are for answering."""
     global _fast, _last

@@ -21,7 +21,8 @@ scale; the first moment is e4m3, the second is held as its root with four bits o
 they are rounded.  Arithmetic is fp32, the norm's squares are summed in fp64 in a fixed order: the same inputs
 give the same bits.  bf16 parameters are rounded to nearest; there is no fp32 copy of them.
 
-state_dict() has torch.optim.AdamW's keys (and the scales); with state_bits=32 either loads the other's.
+state_dict() has torch.optim.AdamW's keys (and the scales); with state_bits=32 either loads the other's.  It does not
+hold the norms' mean: norm_mean can be read and set.
 A step may be captured into a CUDA graph after one that was not (the first one makes the moments); give lr as a
 tensor of one fp32 value on the device where it changes between replays.
 """
@@ -48,8 +49,15 @@ class AdamW(torch.optim.Optimizer):
         defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay)
         self._check_group(defaults)
         super().__init__(params, defaults)
-        for group in self.param_groups:
-            self._check_group(group)
+
+    def add_param_group(self, param_group):
+        self._check_group({**self.defaults, **param_group})
+        super().add_param_group(param_group)
+
+    def __getstate__(self):
+        """What copies and pickles hold besides torch's: the options and the guard's mean."""
+        keep = ("clip", "spike_factor", "state_bits", "_control")
+        return {**super().__getstate__(), **{k: getattr(self, k) for k in keep}}
 
     @staticmethod
     def _check_group(g):
@@ -132,7 +140,9 @@ class AdamW(torch.optim.Optimizer):
     @property
     def norm_mean(self) -> torch.Tensor:
         """The running mean of the norms that spike_factor goes by; 0 before the first step."""
-        return torch.zeros(()) if self._control is None else self._word(0)
+        if self._control is None:
+            return torch.zeros((), device=self.param_groups[0]["params"][0].device)
+        return self._word(0)
 
     @norm_mean.setter
     def norm_mean(self, value):

@@ -162,6 +162,11 @@ def test_state_dict(bits):
             assert torch.equal(v, other.state[q][k]) and v.dtype == other.state[q][k].dtype
     with pytest.raises(ValueError):
         AdamW(twin, state_bits=40 - bits).load_state_dict(saved)
+    copied = copy.deepcopy(other)                                     # its weights and options with it
+    assert copied.clip == 1.0 and copied.state_bits == bits and float(copied.grad_norm) == float(other.grad_norm)
+    _train(copied, copied.param_groups[0]["params"], gen, 1)
+    with pytest.raises(ValueError):
+        copied.add_param_group(dict(params=[torch.nn.Parameter(torch.zeros(2, device="cuda"))], lr=-1.0))
 
 
 def test_moments():

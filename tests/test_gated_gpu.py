@@ -149,10 +149,11 @@ def test_what_is_masked_does_not_matter(L):
     assert not bool(torch.isfinite(h[:, :t]).all())
 
 
-def test_values_that_are_not_finite():
+@pytest.mark.parametrize("C", [33, 64])
+def test_values_that_are_not_finite(C):
     """An infinite state stays infinite through any number of tokens, a gate of -inf makes NaN of it (0 * inf) and forgets
     a finite one, a NaN stays in its channel."""
-    B, L, C = 1, 3000, 33
+    B, L = 1, 3000
     x, g, _, _, _ = _inputs(B, L, C, torch.float32, 5)
     g[..., :8] = -3.0                                                 # products of gates underflow within a segment
     x[0, 10, 0] = float("inf")
