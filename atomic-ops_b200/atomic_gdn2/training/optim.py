@@ -29,6 +29,7 @@ tensor of one fp32 value on the device where it changes between replays.
 from __future__ import annotations
 
 import torch
+from torch.optim import optimizer as _base
 
 from .. import _lib
 
@@ -95,9 +96,17 @@ class AdamW(torch.optim.Optimizer):
                     st[name + "_scale"] = torch.zeros(-(-p.numel() // BLOCK), device=p.device)
         return st
 
-    @torch.no_grad()
     def step(self, closure=None, *, loss=None):
         """One step; returns closure's loss, or None.  Parameters without a gradient are passed over."""
+        if self._optimizer_step_pre_hooks or self._optimizer_step_post_hooks or _base._global_optimizer_pre_hooks \
+                or _base._global_optimizer_post_hooks:
+            return _hooked_step(self, closure, loss=loss)
+        return self._step(closure, loss=loss)
+
+    # torch wraps a step for its hooks and a profiler's mark, 10 us a call: hooks are looked for above instead
+    step.hooked = True
+
+    def _step(self, closure=None, *, loss=None):
         result = None
         if closure is not None:
             with torch.enable_grad():
@@ -116,7 +125,8 @@ class AdamW(torch.optim.Optimizer):
             for group in self.param_groups:
                 for p in group["params"]:
                     if p.grad is not None:
-                        self._ready(p)
+                        with torch.no_grad():
+                            self._ready(p)
             rc = _lib.binding().adamw_step(self.param_groups, self.state, *args, self._control)
         if rc:
             _lib.check(rc, "gdn2_adamw_step")
@@ -195,3 +205,6 @@ class AdamW(torch.optim.Optimizer):
                     new[name].copy_(x)
                 else:
                     new[name] = x.detach().to(p.device, torch.float32).clone()
+
+
+_hooked_step = torch.optim.Optimizer.profile_hook_step(AdamW._step)

@@ -546,7 +546,8 @@ void check_scale(const at::Tensor& t, const at::Tensor& p, const char* what) {
 
 // A new reference's value in a dict, borrowed, or null without an error.
 PyObject* item(PyObject* dict, PyObject* key) { return PyDict_GetItemWithError(dict, key); }
-at::Tensor tensor_of(PyObject* dict, PyObject* key, const char* what) {
+// The dict's tensor: it lives as long as the dict, whose lock (the interpreter's) the call holds.
+const at::Tensor& tensor_of(PyObject* dict, PyObject* key, const char* what) {
   PyObject* o = item(dict, key);
   if (!o && PyErr_Occurred()) throw python_error();
   TORCH_CHECK_VALUE(o && THPVariable_Check(o), "AdamW: the state of a parameter has no tensor ", what);
@@ -575,9 +576,16 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (PyErr_Occurred()) return nullptr;
   const bool eight = d.state_bits == 8;
   const auto moment_type = eight ? at::kByte : at::kFloat;
-  std::vector<at::Tensor> kept;          // what the call has to hold, and what it changes
-  std::vector<at::Tensor> written;
+  std::vector<at::Tensor> kept;          // gradients
+  std::vector<const at::Tensor*> written;
   std::vector<gdn2_adamw_tensor> table;
+  for (Py_ssize_t gi = 0, k = 0; gi < PyList_GET_SIZE(a[0]); ++gi) {
+    PyObject* params = PyDict_Check(PyList_GET_ITEM(a[0], gi)) ? item(PyList_GET_ITEM(a[0], gi), names.params) : nullptr;
+    if (params && PyList_Check(params)) k += PyList_GET_SIZE(params);
+    kept.reserve(k);
+    table.reserve(k);
+    written.reserve(6 * k);
+  }
   c10::Device dev(c10::kCPU);
   for (Py_ssize_t gi = 0; gi < PyList_GET_SIZE(a[0]); ++gi) {
     PyObject* group = PyList_GET_ITEM(a[0], gi);
@@ -615,12 +623,13 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
                         "AdamW: a gradient must be dense, of its parameter's shape and device");
       if (g.scalar_type() != type || (g.strides() != q.strides() && !(g.is_contiguous() && q.is_contiguous()))) {
         const c10::cuda::CUDAGuard guard(dev);
+        const at::NoGradGuard no_grad;
         at::Tensor c = at::empty_like(q);
         c.copy_(g);
         g = std::move(c);
       }
-      at::Tensor m = tensor_of(st, names.m, "exp_avg"), v = tensor_of(st, names.v, "exp_avg_sq"),
-                 step = tensor_of(st, names.step, "step");
+      const at::Tensor &m = tensor_of(st, names.m, "exp_avg"), &v = tensor_of(st, names.v, "exp_avg_sq"),
+                       &step = tensor_of(st, names.step, "step");
       check_moment(m, q, moment_type, "exp_avg");
       check_moment(v, q, moment_type, "exp_avg_sq");
       TORCH_CHECK_VALUE(step.device() == dev && step.scalar_type() == at::kFloat && step.numel() == 1,
@@ -628,13 +637,13 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
       t.p = q.data_ptr(); t.g = g.data_ptr(); t.m = m.data_ptr(); t.v = v.data_ptr();
       t.step = floats(step);
       if (eight) {
-        at::Tensor ms = tensor_of(st, names.ms, "exp_avg_scale"), vs = tensor_of(st, names.vs, "exp_avg_sq_scale");
+        const at::Tensor &ms = tensor_of(st, names.ms, "exp_avg_scale"), &vs = tensor_of(st, names.vs, "exp_avg_sq_scale");
         check_scale(ms, q, "exp_avg_scale");
         check_scale(vs, q, "exp_avg_sq_scale");
         t.m_scale = floats(ms);
         t.v_scale = floats(vs);
-        written.push_back(std::move(ms));
-        written.push_back(std::move(vs));
+        written.push_back(&ms);
+        written.push_back(&vs);
       }
       if (rate_at.defined()) {
         TORCH_CHECK_VALUE(rate_at.device() == dev && rate_at.scalar_type() == at::kFloat && rate_at.numel() == 1,
@@ -646,10 +655,7 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
       t.n = q.numel();
       t.dtype = dtype_of(type);
       table.push_back(t);
-      written.push_back(q);
-      written.push_back(std::move(m));
-      written.push_back(std::move(v));
-      written.push_back(std::move(step));
+      for (const at::Tensor* t : {&q, &m, &v, &step}) written.push_back(t);
       kept.push_back(std::move(g));
     }
   }
@@ -662,7 +668,8 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     TORCH_CHECK_TYPE(THPVariable_Check(a[8]), "AdamW: loss must be a tensor");
     loss32 = THPVariable_Unpack(a[8]);
     TORCH_CHECK_VALUE(loss32.device() == dev && loss32.numel() == 1, "AdamW: loss must be one value on ", dev);
-    loss32 = loss32.detach().to(at::kFloat);
+    const at::NoGradGuard no_grad;
+    loss32 = loss32.to(at::kFloat);
     loss = floats(loss32);
   }
   TORCH_CHECK_TYPE(THPVariable_Check(a[9]), "AdamW: control must be a tensor");
@@ -674,7 +681,7 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const gdn2_status s = gdn2_adamw_step(&d, table.data(), k, loss, control.data_ptr(), ws.data_ptr(),
                                         c10::cuda::getCurrentCUDAStream(dev.index()).stream());
   if (s == GDN2_OK)
-    for (const at::Tensor& t : written) changed(t);
+    for (const at::Tensor* t : written) changed(*t);
   return PyLong_FromLong(s);
   END_HANDLE_TH_ERRORS
 }

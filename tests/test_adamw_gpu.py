@@ -326,6 +326,21 @@ def test_graph_and_streams(bits):
         assert float(a.grad_norm) == float(b.grad_norm) and float(a.state[params[0]]["step"]) == k + 2
 
 
+def test_hooks_and_schedulers():
+    """torch's hooks around a step, and its learning-rate schedulers, work as on its own optimizers."""
+    params, gen = _model([torch.float32], 12)
+    opt, seen = AdamW(params, lr=1e-2), []
+    sched = torch.optim.lr_scheduler.LambdaLR(opt, lambda k: 0.5 ** k)
+    _train(opt, params, gen, 1)
+    sched.step()
+    assert opt.param_groups[0]["lr"] == 5e-3
+    opt.register_step_pre_hook(lambda o, a, k: seen.append("before"))
+    opt.register_step_post_hook(lambda o, a, k: seen.append("after"))
+    was = params[4].detach().clone()
+    _train(opt, params, gen, 1)
+    assert seen == ["before", "after"] and not torch.equal(was, params[4]) and float(opt.state[params[4]]["step"]) == 2
+
+
 def test_refusals():
     cuda = lambda *s, dtype=torch.float32: torch.nn.Parameter(torch.zeros(*s, device="cuda", dtype=dtype))
     for p in (cuda(4, dtype=torch.float16), cuda(4, dtype=torch.float64), torch.nn.Parameter(torch.zeros(1, device="cuda").expand(5)),
