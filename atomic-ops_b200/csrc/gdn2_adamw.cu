@@ -16,6 +16,10 @@
 // written once.  Two launches: the norm's, whose last CTA also counts the steps and prepares the tensors'
 // factors, and the update's.  The tensors' table travels in the kernels' parameters: nothing is copied to the
 // device, and a captured graph keeps what it needs.
+//
+// Measured, 39 M fp32 weights: norm 39 us (156 MB; the last CTA's turn is some 6 us of it), update 161 us (1095 MB at 6.8
+// TB/s); with 8-bit moments 125 us (626 MB: 64 instructions a value, two thirds of the issue slots).  348 M bf16 weights with
+// 8-bit moments: 940 us (3.5 GB).
 #include <cuda_fp8.h>
 
 #include "gdn2_common.cuh"
