@@ -405,12 +405,14 @@ __device__ __forceinline__ void chunk_update(const AdamEntry& e, const Steps& st
   } else {
     uint8_t* m = static_cast<uint8_t*>(e.m) + at;
     uint8_t* v = static_cast<uint8_t*>(e.v) + at;
+    float* m_scale = e.ms + at / kBlock;
+    float* v_scale = e.vs + at / kBlock;
     const int lane = threadIdx.x & 31;
     float nx[2][4], ny[2][4], nms, nvs;
     uint32_t ncm[2], ncv[2];
     auto load = [&](int blk) {
-      nms = e.ms[at / kBlock + blk];
-      nvs = e.vs[at / kBlock + blk];
+      nms = m_scale[blk];
+      nvs = v_scale[blk];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int i = blk * kBlock + h * 128 + lane * 4;
@@ -423,7 +425,6 @@ __device__ __forceinline__ void chunk_update(const AdamEntry& e, const Steps& st
     };
     if (WHOLE) load(threadIdx.x >> 5);
     for (int blk = threadIdx.x >> 5; blk * kBlock < n; blk += kAdamThreads / 32) {
-      const long long s = at / kBlock + blk;
       if (!WHOLE) load(blk);
       const float ms = nms, vs = nvs;
       float x[2][4], y[2][4];
@@ -479,8 +480,8 @@ __device__ __forceinline__ void chunk_update(const AdamEntry& e, const Steps& st
         codes4(v + i, encode_r(r[h], both(up_r)), vec, n - i);
       }
       if (lane == 0) {
-        e.ms[s] = new_ms;
-        e.vs[s] = new_vs;
+        m_scale[blk] = new_ms;
+        v_scale[blk] = new_vs;
       }
     }
   }

@@ -90,10 +90,11 @@ def _leaves(*ts):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("C", [37, 40])
 @pytest.mark.parametrize("L", [1, 3, 70])
-def test_views_of_one_projection(L, dtype):
+def test_views_of_one_projection(L, C, dtype):
     """x and g side by side in one tensor, odd offsets, transposed and broadcast inputs."""
-    B, C = 3, 37
+    B = 3
     x, g, h0, dy, dl = _inputs(B, L, C, dtype, L)
     both = torch.cat([x, g], 2)
     flat = both.cuda()
