@@ -2,7 +2,8 @@
 //   z = x W + b,  y = act(z) + r;    dz = dy act'(z),  db = sum over rows of dz,  dx = dz W^T,  dW = x^T dz
 // x (M, K), W (K, N), y, z, r (M, N) are bf16 or fp32; sums are fp32.
 //
-// All three products run on the 5th-generation tensor cores from bf16 operands: D (rows, cols) = A B with A and B
+// Small products and few rows have kernels of their own below, in plain fp32.  The others, all three of them, run on the
+// 5th-generation tensor cores from bf16 operands: D (rows, cols) = A B with A and B
 // read in place by tiled copies, either of them contiguous along the summed dimension or across it (W in the
 // forward, x and dz for dW), so that nothing is transposed in memory.  An fp32 operand is first cut into three
 // bf16 terms of 8 bits each (x = t0 + t1 + t2 to 2^-27 of x), and the six products t_i u_j with i + j <= 2 are
@@ -26,6 +27,7 @@
 #include <cooperative_groups.h>
 #include <cuda.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "gdn2_common.cuh"
@@ -857,6 +859,150 @@ __global__ void __launch_bounds__(256) linear_few_kernel(const __grid_constant__
   if (p.clusters > 1) cg::this_cluster().sync();  // a CTA's parts are read until here
 }
 
+// ---- small products -----------------------------------------------------------------------------
+// Where launches cost more than the products: one launch for a forward, one for dx, dW and db together, fp32 products
+// of 32 x 32 tiles from shared memory, dz made as it is read (which sizes, and what both ways take: small_within).
+// Eight groups of 64 threads share a tile's sum, 4 x 4 of its elements a thread, and join at the end in their order.  A
+// step of 64 along the sum takes 1.0 us: the loads' and shared memory's latency, with a tile's 16 warps alone on their SM
+// (four groups, 8 warps: 1.05 us and in bf16 1.3, half of the issue slots empty).
+constexpr int kSmallTile = 32, kSmallK = 64, kSmallRow = kSmallTile + 4, kSmallThreads = 512,
+              kSmallGroups = kSmallThreads / 64, kSmallLoads = kSmallTile * kSmallK / kSmallThreads;
+static_assert(kSmallTile == 32 && kSmallThreads == 512 && kSmallLoads == 4, "SmallOperand");
+struct Product {
+  const void *a, *b;                    // rows x k and k x cols
+  const void* z;                        // not null: a (b where z_of_b) is times the slope of GELU at these
+  long long a_row, a_k, b_k, b_col;     // element strides: of each pair one is 1
+  int rows, cols, k, z_of_b;
+  Epilogue ep;
+  void* sums;                           // sums over k of b's columns, or null
+  int sums_bf16;
+};
+struct Products {
+  Product p[2];
+  int tiles0;                           // of p[0]; the other tiles are p[1]'s
+};
+// One operand's elements of a k-tile: element j of a thread is at i = i0 + di (j % 2), k = kb + dk (j % 2) + 32 (j / 2),
+// so that a warp reads along the stride of one.  In shared memory element (k, i) stands at k rows and i ^ (k / 8 % 4):
+// without bank conflicts along either, and four elements of 16 bytes stay together.
+struct SmallOperand {
+  long long at, step, pitch, pitch2;
+  int kb, dk, left, di, slot;
+  bool along;
+  __device__ __forceinline__ SmallOperand(long long s_i, long long s_k, int i0, int n) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    along = s_k == 1;                   // lanes along k
+    const int i = along ? warp : lane;
+    kb = along ? lane : warp;
+    at = (i0 + i) * s_i + kb * s_k;
+    step = kSmallK * s_k;
+    pitch = 16 * (along ? s_i : s_k);
+    pitch2 = 32 * s_k;
+    dk = along ? 0 : 16;
+    di = along ? 16 : 0;
+    left = n - i0 - i;
+    slot = along ? lane * kSmallRow + (warp ^ (lane >> 3)) : warp * kSmallRow + (lane ^ (warp >> 3));
+  }
+  template <class T>
+  __device__ __forceinline__ void load(T (&v)[kSmallLoads], const void* p, int k) const {
+#pragma unroll
+    for (int j = 0; j < kSmallLoads; ++j)
+      v[j] = left > di * (j & 1) && kb + dk * (j & 1) + 32 * (j >> 1) < k
+                 ? static_cast<const T*>(p)[at + (j & 1) * pitch + (j >> 1) * pitch2] : T(0.f);
+  }
+  __device__ __forceinline__ void keep(const float (&v)[kSmallLoads], float* s) const {
+#pragma unroll
+    for (int j = 0; j < kSmallLoads; ++j)
+      s[(along ? slot + 16 * (j & 1) : (slot ^ 2 * (j & 1)) + 16 * (j & 1) * kSmallRow) + 32 * (j >> 1) * kSmallRow] = v[j];
+  }
+};
+template <class T>
+__global__ void __launch_bounds__(kSmallThreads) linear_small_kernel(const __grid_constant__ Products both) {
+  __shared__ __align__(16) float tiles[2][2][kSmallK * kSmallRow];
+  const bool second = (int)blockIdx.x >= both.tiles0;
+  const Product& p = both.p[second];
+  const int tile = second ? blockIdx.x - both.tiles0 : blockIdx.x, tiles_n = (p.cols + kSmallTile - 1) / kSmallTile;
+  const int row0 = tile / tiles_n * kSmallTile, col0 = tile % tiles_n * kSmallTile;
+  const int group = threadIdx.x >> 6, ty = (threadIdx.x >> 3) & 7, tx = threadIdx.x & 7;
+  SmallOperand oa(p.a_row, p.a_k, row0, p.rows), ob(p.b_col, p.b_k, col0, p.cols);
+  const void *pa = p.a, *pb = p.b, *pz = p.z;
+  const bool z_of_b = p.z_of_b, sums = p.sums && row0 == 0;
+  T ra[kSmallLoads], rb[kSmallLoads], rz[kSmallLoads];
+  auto load = [&](int k) {
+    oa.load(ra, pa, k);
+    ob.load(rb, pb, k);
+    if (pz) {
+      if (z_of_b) ob.load(rz, pz, k);
+      else oa.load(rz, pz, k);
+    }
+    oa.at += oa.step;
+    ob.at += ob.step;
+  };
+  float acc[4][4] = {}, sum[4] = {};
+  load(p.k);
+  int s = 0;
+  for (int k = p.k; k > 0; k -= kSmallK, s ^= 1) {
+    float va[kSmallLoads], vb[kSmallLoads];
+#pragma unroll
+    for (int j = 0; j < kSmallLoads; ++j) {
+      va[j] = to_f<T>(ra[j]);
+      vb[j] = to_f<T>(rb[j]);
+    }
+    if (pz) {
+#pragma unroll
+      for (int j = 0; j < kSmallLoads; ++j) {
+        const float slope = gelu_slope(to_f<T>(rz[j]));
+        if (z_of_b) vb[j] *= slope;
+        else va[j] *= slope;
+      }
+    }
+    oa.keep(va, tiles[s][0]);
+    ob.keep(vb, tiles[s][1]);
+    __syncthreads();                    // the other stage was read before the last one of these
+    if (k > kSmallK) load(k - kSmallK);
+    const float *as = tiles[s][0] + group * kSmallRow + 4 * ty, *bs = tiles[s][1] + group * kSmallRow + 4 * tx;
+#pragma unroll
+    for (int q = 0; q < kSmallK / kSmallGroups; ++q) {      // k = 8 q + group
+      const float4 x4 = *reinterpret_cast<const float4*>(as + kSmallGroups * q * kSmallRow), y4 = *reinterpret_cast<const float4*>(bs + kSmallGroups * q * kSmallRow);
+      const float x[4] = {x4.x, x4.y, x4.z, x4.w}, y[4] = {y4.x, y4.y, y4.z, y4.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(x[i ^ (q & 3)], y[j ^ (q & 3)], acc[i][j]);
+      if (sums)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[j] += y[j ^ (q & 3)];
+    }
+  }
+  __syncthreads();
+  float* join = tiles[0][0];            // 8 groups of 32 x 32 sums, then 8 of 32
+  constexpr int kAll = kSmallTile * kSmallTile;
+  static_assert(sizeof(tiles) >= 4 * kSmallGroups * (kAll + kSmallTile), "join");
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    *reinterpret_cast<float4*>(join + group * kAll + (4 * ty + i) * kSmallTile + 4 * tx) =
+        make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
+  if (sums && ty == 0)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) join[kSmallGroups * kAll + group * kSmallTile + 4 * tx + j] = sum[j];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kAll / kSmallThreads; ++i) {
+    const int e = threadIdx.x + kSmallThreads * i, row = row0 + e / kSmallTile, col = col0 + e % kSmallTile;
+    if (row < p.rows && col < p.cols) {
+      float v = 0.f;
+#pragma unroll
+      for (int g = 0; g < kSmallGroups; ++g) v += join[g * kAll + e];
+      finish(p.ep, row, col, v, p.k, p.ep.bias ? load_f(p.ep.bias, col, p.ep.bias_bf16) : 0.f);
+    }
+  }
+  if (sums && threadIdx.x < kSmallTile && col0 + (int)threadIdx.x < p.cols) {
+    float v = 0.f;
+#pragma unroll
+    for (int g = 0; g < kSmallGroups; ++g) v += join[kSmallGroups * kAll + g * kSmallTile + threadIdx.x];
+    store_f(p.sums, col0 + threadIdx.x, p.sums_bf16, v);
+  }
+}
+
 // ---- host ---------------------------------------------------------------------------------------
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -1021,6 +1167,38 @@ size_t element(const gdn2_linear_desc* d) { return d->dtype == GDN2_BF16 ? 2 : 4
 // against 16.3, 16 x 4096 x 4096 43 against about 50); bf16 rows are few where a launch less counts (4 x 512 x 4608 5.8 us
 // against 8.1; of 8 rows 11.2 against 8.1, 8 x 4096 x 4096 21 against 15).
 int few_rows(const gdn2_linear_desc* d) { return d->dtype == GDN2_F32 ? 16 : 4; }
+// The small kernel takes about 2 + k / 64 us for a sum over k where every tile has an SM of its own, and its tiles' sum shared out where
+// they have not.  It is taken where that is less than the tiled path takes at such sizes: forward 11 to 15 us in fp32 (of
+// which making the terms is 4) and 5 to 8 in bf16; dx with dW 19 to 32 and 12 to 24, one of them alone 10 to 18 and 4 to
+// 5, with GELU's dz to make 6 to 12.  fp32 64 x 128 x 96 forward 10.5 -> 4.6 us, backward 19.8 -> 4.7; 128 x 512 x 256
+// 13.6 -> 10.6 and 24.8 -> 9.0; 256 x 256 x 256 13.1 -> 6.6 and 29.2 -> 7.8; 128 x 1024 x 128 14.2 against 18.7: not taken.
+// bf16 64 x 128 x 96 6.0 -> 4.6 and 13.0 -> 4.8; 128 x 512 x 256 8.1 against 11.2: not taken.
+struct SmallSize { long long tiles, steps; };
+SmallSize small_size(long long rows, long long cols, long long k) {
+  return {(rows + kSmallTile - 1) / kSmallTile * ((cols + kSmallTile - 1) / kSmallTile), (k + kSmallK - 1) / kSmallK + 2};
+}
+bool small_within(SmallSize a, SmallSize b, int us) {
+  const long long sms = kSMs, most = std::max(a.steps, b.steps);
+  if (a.tiles + b.tiles <= sms) return most <= us;
+  return a.tiles <= us * sms && b.tiles <= us * sms && 2 * (a.tiles * a.steps + b.tiles * b.steps) + most * sms <= 2 * us * sms;
+}
+bool small_fwd(const gdn2_linear_desc* d) {
+  return small_within(small_size(d->M, d->N, d->K), {}, d->dtype == GDN2_F32 ? 11 : 6);
+}
+bool small_bwd(const gdn2_linear_desc* d, bool dx, bool dw, bool db) {
+  if ((!dx && !dw) || (db && !dw)) return false;          // a sum of columns alone has no tiles here
+  const bool f32 = d->dtype == GDN2_F32;
+  return small_within(dx ? small_size(d->M, d->K, d->N) : SmallSize{}, dw ? small_size(d->K, d->N, d->M) : SmallSize{},
+                      dx && dw ? (f32 ? 19 : 12) : f32 ? 11 : d->act != GDN2_ACT_NONE ? 7 : 4);
+}
+int small_tiles(const Product& p) { return (int)small_size(p.rows, p.cols, p.k).tiles; }
+cudaError_t run_small(const gdn2_linear_desc* d, const Product& p0, const Product& p1, cudaStream_t st) {
+  Products both{{p0, p1}, small_tiles(p0)};
+  const int tiles = both.tiles0 + small_tiles(p1);
+  if (d->dtype == GDN2_F32) linear_small_kernel<float><<<tiles, kSmallThreads, 0, st>>>(both);
+  else linear_small_kernel<__nv_bfloat16><<<tiles, kSmallThreads, 0, st>>>(both);
+  return cudaGetLastError();
+}
 struct FwdPlan {
   bool few, x_terms, w_terms;
   size_t x_at, w_at, parts_at, total;
@@ -1028,7 +1206,7 @@ struct FwdPlan {
 FwdPlan plan_fwd(const gdn2_linear_desc* d, bool x_direct, bool w_direct) {
   FwdPlan f{};
   f.few = d->M <= few_rows(d);
-  if (f.few) return f;
+  if (f.few || small_fwd(d)) return f;
   f.x_terms = !x_direct;
   f.w_terms = !w_direct;
   f.w_at = f.x_terms ? terms_bytes(d, d->M, d->K) : 0;
@@ -1044,6 +1222,7 @@ struct BwdPlan {
 };
 BwdPlan plan_bwd(const gdn2_linear_desc* d, bool dx, bool dw, bool db, bool x_direct, bool w_direct, bool dy_direct) {
   BwdPlan b{};
+  if (small_bwd(d, dx, dw, db)) return b;
   size_t at = 0;
   auto take = [&](size_t n) { const size_t r = at; at += round256(n); return r; };
   b.dz = (dx || dw) && (!dy_direct || d->act != GDN2_ACT_NONE);
@@ -1140,6 +1319,13 @@ extern "C" gdn2_status gdn2_linear_fwd(const gdn2_linear_desc* d, const void* x,
     p.ep = ep;
     p.x = x; p.w = w; p.ldx = d->x_stride; p.ldw = d->w_stride; p.cols = d->N; p.k = d->K;
     e = run_few(d, p, st);
+  } else if (small_fwd(d)) {
+    Product p{};
+    p.a = x; p.a_row = d->x_stride; p.a_k = 1;
+    p.b = w; p.b_k = d->w_stride; p.b_col = 1;
+    p.rows = d->M; p.cols = d->N; p.k = d->K;
+    p.ep = ep;
+    e = run_small(d, p, Product{}, st);
   } else {
     const int terms = d->dtype == GDN2_F32 ? 3 : 1;
     if (terms == 3) {
@@ -1190,6 +1376,23 @@ extern "C" gdn2_status gdn2_linear_bwd(const gdn2_linear_desc* d, const void* x,
   const int terms = bf16 ? 1 : 3, bands = (d->M + kBand - 1) / kBand;
   const long long ldz = padded(d->N);
   cudaError_t e = cudaSuccess;
+  if (small_bwd(d, dx, dw, db)) {
+    Product px{}, pw{};
+    if (dx) {
+      px.a = dy; px.z = act ? z : nullptr; px.a_row = d->N; px.a_k = 1;
+      px.b = w; px.b_k = 1; px.b_col = d->w_stride;
+      px.rows = d->M; px.cols = d->K; px.k = d->N;
+      px.ep.y = dx; px.ep.ldy = d->K; px.ep.y_bf16 = bf16;
+    }
+    if (dw) {
+      pw.a = x; pw.a_row = 1; pw.a_k = d->x_stride;
+      pw.b = dy; pw.z = act ? z : nullptr; pw.z_of_b = 1; pw.b_k = d->N; pw.b_col = 1;
+      pw.rows = d->K; pw.cols = d->N; pw.k = d->M;
+      pw.ep.y = dw; pw.ep.ldy = d->N; pw.ep.y_bf16 = bf16;
+      pw.sums = db; pw.sums_bf16 = d->bias_dtype == GDN2_BF16;
+    }
+    return run_small(d, px, pw, st) == cudaSuccess ? GDN2_OK : GDN2_ERR_CUDA;
+  }
   if (b.dz || db) {
     const int col_blocks = (d->N + 63) / 64;
     const unsigned grid = (unsigned)(col_blocks * (long long)bands);

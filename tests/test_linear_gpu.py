@@ -269,3 +269,131 @@ def test_large_offsets():
         y = linear(x, w)
     rows = [0, 1, 32767, 65535, 65536, 69887, 69999]
     _close(y[rows], x[rows].double() @ w.double(), x[rows].double().abs() @ w.double().abs(), K, torch.bfloat16)
+
+
+SMALL = [(1, 1, 1), (2, 1, 65), (5, 33, 1), (17, 64, 32), (31, 63, 33), (32, 65, 64), (64, 128, 96), (65, 300, 31), (100, 7, 260),
+         (257, 40, 5), (600, 20, 24), (24, 20, 600), (48, 570, 40), (900, 33, 17)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M,K,N", SMALL)
+def test_small_products(M, K, N, dtype):
+    """Products that are one launch, every element by itself.
+
+    Eight chains of k / 8 rounded additions and eight more: a sum of k products is off by (k / 8 + 8) u of sum |a b|.
+    GELU's slope is off by 16 u, and in bf16 by 0.8 * 2^-8 |z| for the rounded z; dz is not rounded.  A bf16 result is
+    off by 2^-8 of itself.  Where bf16 goes the tiled way instead, its exact products and truncating additions are off by
+    (k / 8 + 16) u and dz by 2^-8 of itself.
+    """
+    x, w, b, r, dy = _data(M, K, N, dtype, M + K + N)
+    bf16 = dtype == torch.bfloat16
+    step = 2.0 ** -8 if bf16 else U
+    views = ((x, w), (torch.cat([x, x[:, :1]], 1)[:, :K], torch.cat([w, w, w], 1)[:, :N]))
+    xd, wd, bd, dyd = (t.double() for t in (x, w, b, dy))
+    for x2, w2 in views:
+        for act in (None, "gelu"):
+            z = xd @ wd + bd
+            t = z.clone().requires_grad_(True)
+            y_r = torch.nn.functional.gelu(t, approximate="tanh") if act else t * 1.0
+            (dz,) = torch.autograd.grad(y_r, t, dyd)
+            d_err = dyd.abs() * (16 * U + (0.8 * 2.0 ** -8 * z.abs() if bf16 else 0.0)) + (2.0 ** -8 * dz.abs() if bf16 else 0.0) if act else 0.0 * dz
+            size = xd.abs() @ wd.abs() + bd.abs()
+            leaves = [t.detach().requires_grad_(True) for t in (x2, w2, b)]
+            y = linear(*leaves, act=act, residual=r)
+            # GELU's slope is at most 1.13; the bias and the residual are one rounded addition each
+            z_err = (K / 8 + 18) * U * size
+            over = (y.detach().double() - (y_r.detach() + r.double())).abs() - 1.13 * z_err - 8 * U * z.abs() - step * (y_r.detach() + r.double()).abs() - U * (
+                y_r.detach().abs() + r.double().abs())
+            assert float(over.max()) <= 0
+            z_in_slope = dyd.abs() * 0.8 * z_err if act else 0.0 * dz
+            want = ((dz @ wd.t(), (N / 8 + 18) * U * (dz.abs() @ wd.abs().t()) + (d_err + z_in_slope) @ wd.abs().t()),
+                    (xd.t() @ dz, (M / 8 + 18) * U * (xd.abs().t() @ dz.abs()) + xd.abs().t() @ (d_err + z_in_slope)),
+                    (dz.sum(0), (M / 8 + 18) * U * dz.abs().sum(0) + (d_err + z_in_slope).sum(0)))
+            for some in ((0, 1, 2), (0,), (1,), (2,), (0, 2), (1, 2), (0, 1)):
+                got = torch.autograd.grad(y, [leaves[i] for i in some], dy, retain_graph=True)
+                for i, g in zip(some, got):
+                    ref, err = want[i]
+                    assert g.shape == leaves[i].shape
+                    assert float(((g.double() - ref).abs() - 1.01 * err - step * ref.abs()).max()) <= 0, (act, some, i)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_tiled_views_and_some_gradients(dtype):
+    """Views in place and views through copies, odd sizes, and each choice of gradients, where products are tiled."""
+    M, K, N = 1291, 150, 1203
+    x, w, b, r, dy = _data(M, K, N, dtype, 3)
+    ref = [t.double().requires_grad_(True) for t in (x, w, b, r)]
+    y_r = linear_ref(*ref[:3], "gelu", ref[3])
+    g_r = torch.autograd.grad(y_r, ref, dy.double())
+    size = x.double().abs() @ w.double().abs()
+    wide = torch.cat([x, x], 1)[:, :K + 2][:, :K]
+    apart = torch.zeros(M, K + 42, dtype=dtype, device="cuda")
+    apart[:, 16:16 + K] = x
+    for i, (x2, w2, r2) in enumerate(((wide, torch.cat([w, w[:, :5]], 1)[:, :N], torch.cat([r, r], 1)[:, N:]),
+                                      (apart[:, 16:16 + K], torch.cat([w, w], 1)[:, :N], r.t().contiguous().t()),
+                                      (x.t().contiguous().t(), w.t().contiguous().t(), r))):
+        for want in range(1, 16) if i == 0 else (15,):
+            ts = [t.detach().requires_grad_(bool(want >> j & 1)) for j, t in enumerate((x2, w2, b, r2))]
+            y = linear(*ts[:3], act="gelu", residual=ts[3])
+            _close(y, y_r, size, K, dtype, 8 * U + 4 * U * (b.double().abs() + r.double().abs()))
+            got = torch.autograd.grad(y, [t for t in ts if t.requires_grad], dy)
+            for a, c, k in zip(got, [g for j, g in enumerate(g_r) if want >> j & 1], [k for j, k in enumerate((N, M, M, 1)) if want >> j & 1]):
+                _norm_close(a, c, (48 + k / 64 + 64) * U if dtype == torch.float32 else 3 * 2.0 ** -8)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M,K,N", [(1291, 150, 1203), (60, 90, 70)])
+def test_graphs_of_tiled_and_small_products(M, K, N, dtype):
+    """Captured forward and backward replay on new inputs, two graphs in turn, beside eager calls on another stream."""
+    atomic_gdn2.set_checks("async")
+    x, w, b, r, dy = _data(M, K, N, dtype, 5)
+    ts = [t.clone().requires_grad_(True) for t in (x, w, b, r)]
+    call = lambda: (lambda y: (y, *torch.autograd.grad(y, ts, dy)))(linear(*ts[:3], act="gelu", residual=ts[3]))
+    graphs = []
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+        graphs.append((graph, out))
+    with torch.no_grad():
+        ts[0].mul_(-0.5)
+        ts[1].add_(0.01)
+    for graph, _ in graphs * 2:
+        graph.replay()
+    want = call()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = call()
+    for graph, out in graphs:
+        graph.replay()
+    torch.cuda.current_stream().wait_stream(side)
+    for _, out in graphs:
+        assert all(torch.equal(a, c) for a, c in zip(want, out))
+    assert all(torch.equal(a, c) for a, c in zip(want, other))
+
+
+@pytest.mark.parametrize("M,K,N", [(1291, 150, 1203), (60, 90, 70)])
+def test_not_finite_gradients_of_tiled_and_small_products(M, K, N):
+    """Infinities and NaN in dy and in the operands reach exactly the gradients that the formulas give them.
+
+    But for elements whose finite products alone, 3.3e38 times some 1.04 among them, can leave fp32's range on the way:
+    infinities of the sum's own meet the operands' there, as in any fp32 sum, and what 64 bits give says nothing.
+    """
+    for dtype in (torch.float32, torch.bfloat16):
+        x, w, b, r, dy = _data(M, K, N, dtype, 8)
+        dy[0, 1], dy[M - 1, N - 1], dy[3, 0] = float("inf"), float("nan"), 3.3e38
+        x[2, 5], w[7, 2] = float("-inf"), 0.0
+        ts = [t.clone().requires_grad_(True) for t in (x, w, b)]
+        d = torch.autograd.grad(linear(*ts), ts, dy)
+        one = torch.ones(1, M, dtype=torch.float64, device="cuda")
+        finite = lambda t: t.nan_to_num(0.0, 0.0, 0.0).abs()
+        for a, p, q in zip(d, (dy.double(), x.double().t(), one), (w.double().t(), dy.double(), dy.double())):
+            c, sure = (p @ q).to(dtype).view(a.shape), (finite(p) @ finite(q) < 3.35e38).view(a.shape)
+            assert bool(sure.any())
+            a, c = a[sure], c[sure]
+            assert torch.equal(torch.isnan(a), torch.isnan(c)) and torch.equal(a[torch.isinf(a)], c[torch.isinf(c)])

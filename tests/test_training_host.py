@@ -95,9 +95,10 @@ def test_entry_points_reject_bad_arguments():
     for kw in (dict(M=2 ** 29), dict(K=2 ** 30, x_stride=2 ** 30), dict(x_stride=2 ** 31), dict(M=2 ** 27, N=2 ** 27, w_stride=2 ** 27)):
         assert lin(**kw)[0] == uns and lin(**kw)[1] == 0, kw
     for kw in (dict(x=0), dict(w=0), dict(y=0), dict(flags=0), dict(x=at + 8), dict(w=at + 4), dict(y=at + 2), dict(bias=at + 2),
-               dict(ws=0), dict(ws=at + 64)):
+               dict(ws=0, K=2048, x_stride=2048), dict(ws=at + 64, K=2048, x_stride=2048)):
         assert lin(**kw)[0] == inv, kw
-    for kw in (dict(x=at + 8), dict(flags=0), dict(act=1), dict(ws=0), dict(y=at + 4)):
+    assert lin(x=0)[1] == 0 and lin(x=0)[3] == 0 and lin(x=0, K=2048, x_stride=2048)[1] > 0     # small products need no workspace
+    for kw in (dict(x=at + 8), dict(flags=0), dict(act=1), dict(ws=0, M=2048), dict(y=at + 4)):
         assert lin(**kw)[2] == inv, kw
     assert lib.gdn2_linear_fwd(0, *[at] * 9) == inv and lib.gdn2_linear_bwd(0, *[at] * 10) == inv
     assert lin(M=0)[0] == _lib.OK and lin(M=0)[2] == inv
