@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_norm_kernel(const __grid_c
     if (a.norm) {
       const float n = (float)sqrt(total), ema = c.ema;
       ok = ok && isfinite(n) && (a.spike <= 0.f || ema <= 0.f || n < a.spike * ema);
-      if (a.clip > 0.f) coef = __fdiv_rn(a.clip, fmaxf(n, a.clip));
+      if (a.clip > 0.f && n > a.clip) coef = __fdiv_rn(a.clip, n);      // clip may be infinite
       if (ok) c.ema = ema > 0.f ? __fadd_rn(__fmul_rn(0.98f, ema), __fmul_rn(0.02f, n)) : n;
       c.norm = n;
       c.ticket = 0;
@@ -701,7 +701,10 @@ extern "C" gdn2_status gdn2_adamw_step(const gdn2_adamw_desc* d, const gdn2_adam
   a.log2_b1 = log2(d->beta1); a.log2_b2 = log2(d->beta2);
   a.fb1 = (float)d->beta1; a.gb1 = (float)(1.0 - d->beta1);
   a.fb2 = (float)d->beta2; a.gb2 = (float)(1.0 - d->beta2);
-  a.eps = (float)d->eps; a.clip = (float)d->clip; a.spike = (float)d->spike;
+  a.eps = (float)d->eps;
+  // above zero they stay so in fp32
+  a.clip = d->clip > 0 ? fmaxf((float)d->clip, kNormal) : 0.f;
+  a.spike = d->spike > 0 ? fmaxf((float)d->spike, kNormal) : 0.f;
   a.norm = d->clip > 0 || d->spike > 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = all.tensors <= kFew ? run_adamw<kFew>(d, tensors, n, a, st) : run_adamw<kMany>(d, tensors, n, a, st);

@@ -270,6 +270,33 @@ def test_guard():
     assert bool(torch.isnan(params[4]).all()) and bool(torch.isfinite(params[0]).all())
 
 
+def test_clips_at_the_ends_of_the_range():
+    """An infinite clip clips nothing (the guard stays), one below fp32's normal numbers leaves next to nothing."""
+    for bits in (32, 8):
+        for clip in (float("inf"), 1e300):
+            params, gen = _model([torch.float32], 11)
+            twin = [torch.nn.Parameter(p.detach().clone()) for p in params]
+            opt, plain = AdamW(params, lr=1e-2, clip=clip, state_bits=bits), AdamW(twin, lr=1e-2, state_bits=bits)
+            for scale in (1.0, 100.0):
+                for p, q, g in zip(params, twin, _grads(params, gen, scale)):
+                    p.grad = g.cuda()
+                    q.grad = p.grad.clone()
+                opt.step()
+                plain.step()
+                assert bool(opt.step_made) and math.isfinite(float(opt.grad_norm))
+            assert all(torch.equal(p, q) for p, q in zip(params, twin))
+            params[4].grad.fill_(float("inf"))
+            opt.step()
+            assert not bool(opt.step_made) and all(torch.equal(p, q) for p, q in zip(params, twin))
+        p = torch.nn.Parameter(torch.ones(300, device="cuda"))
+        p.grad = torch.full_like(p, 3.0)
+        opt = AdamW([p], lr=1e-2, eps=1.0, weight_decay=0.0, clip=1e-60, spike_factor=1e-60, state_bits=bits)
+        opt.step()
+        assert bool((p == 1.0).all()) and bool(opt.step_made)         # steps of 1e-38 or less
+        opt.step()
+        assert not bool(opt.step_made)                                # no norm is below 1e-60 of the mean
+
+
 def test_zero_and_extreme_gradients():
     """A gradient of zeros has norm zero; gradients whose squares fp32 cannot hold are clipped like others."""
     for bits in (32, 8):
