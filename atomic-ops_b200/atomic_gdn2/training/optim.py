@@ -21,8 +21,8 @@ scale; the first moment is e4m3, the second is held as its root with four bits o
 they are rounded.  Arithmetic is fp32, the norm's squares are summed in fp64 in a fixed order: the same inputs
 give the same bits.  bf16 parameters are rounded to nearest; there is no fp32 copy of them.
 
-state_dict() has torch.optim.AdamW's keys (and the scales); with state_bits=32 either loads the other's.  It does not
-hold the norms' mean: norm_mean can be read and set.
+state_dict() has torch.optim.AdamW's keys (and the scales); with state_bits=32 either loads the other's (not amsgrad's or
+maximize's).  It does not hold the norms' mean: norm_mean can be read and set.
 A step may be captured into a CUDA graph after one that was not (the first one makes the moments); give lr as a
 tensor of one fp32 value on the device where it changes between replays.
 """
@@ -70,6 +70,12 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"AdamW: lr={g['lr']} must not be negative")
         if not g["weight_decay"] >= 0.0:
             raise ValueError(f"AdamW: weight_decay={g['weight_decay']} must not be negative")
+        # options of torch's that change the step
+        for name in ("amsgrad", "maximize"):
+            if g.get(name):
+                raise ValueError(f"AdamW: {name} is not supported")
+        if g["weight_decay"] and not g.get("decoupled_weight_decay", True):
+            raise ValueError("AdamW: weight decay that goes through the moments (torch.optim.Adam's) is not supported")
 
     def _check_guard(self):
         for name in ("clip", "spike_factor"):
@@ -186,6 +192,8 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """torch casts a state to its parameter's type: codes, scales and steps are put back as they were saved."""
+        for g in state_dict["param_groups"]:
+            self._check_group(g)
         super().load_state_dict(state_dict)
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         mine = [p for g in self.param_groups for p in g["params"]]

@@ -55,6 +55,29 @@ def test_model_and_step_take_the_operators():
     assert plain.linear_fn is None and isinstance(make_optimizer(plain, 1e-3), torch.optim.AdamW)
 
 
+def test_a_state_of_other_options_is_refused():
+    """What torch's Adam can be told and this optimizer does not do; refused before anything is loaded."""
+    p = torch.nn.Parameter(torch.ones(3, 2))
+    for kind, kw in ((torch.optim.AdamW, dict(amsgrad=True)), (torch.optim.AdamW, dict(maximize=True)), (torch.optim.Adam, dict(weight_decay=0.1))):
+        other = kind([p], lr=0.5, **kw)
+        opt = AdamW([p], lr=0.25)
+        with pytest.raises(ValueError):
+            opt.load_state_dict(other.state_dict())
+        assert opt.param_groups[0]["lr"] == 0.25 and "amsgrad" not in opt.param_groups[0]
+        with pytest.raises(ValueError):
+            AdamW([dict(params=[p], **{k: v for k, v in other.param_groups[0].items() if k != "params"})])
+    opt = AdamW([p], lr=0.25)
+    for kind, kw in ((torch.optim.AdamW, dict(foreach=True)), (torch.optim.Adam, dict(weight_decay=0.0))):
+        opt.load_state_dict(kind([p], lr=0.5, **kw).state_dict())
+        assert opt.param_groups[0]["lr"] == 0.5
+    back = torch.optim.AdamW([p])
+    back.load_state_dict(opt.state_dict())
+    bad = opt.state_dict()
+    bad["param_groups"][0]["betas"] = (0.9, 1.0)
+    with pytest.raises(ValueError):
+        opt.load_state_dict(bad)
+
+
 def test_moment_codes():
     """Half a step: 1/16 of an e4m3 value, 1/32 of a root, each next to the smallest normal numbers of the format;
     zeros stay zeros, and roots above zero stay above zero."""
