@@ -35,6 +35,15 @@ def _readable(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
+def _spans(t: torch.Tensor, out: torch.Tensor) -> bool:
+    """Whether `out`, contiguous, lies within the memory from t's first value to its last."""
+    if not t.numel():
+        return False
+    first, a = t.data_ptr(), out.data_ptr()
+    end = first + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+    return a < end and first < a + out.numel() * out.element_size()
+
+
 def _desc(x, g, n_states):
     B, L, C = x.shape
     key = (x.shape, x.stride(), g.stride(), x.dtype, n_states)
@@ -129,7 +138,7 @@ def gated_scan(x: torch.Tensor, g: torch.Tensor, h0=None, *, lengths=None, reset
       reset    (B, L) bool: tokens that drop the state before them
       h_index  (B) the row of h0 that each sequence starts from, negative for zeros (beam_select's rows)
       h_out    (B, C) fp32 contiguous, written and returned as `last` (an in-place change to autograd); it may
-               be h0 itself where there is no h_index, and overlaps no input otherwise
+               be h0 itself where there is no h_index, and otherwise lies outside the inputs' memory
     Returns h (B, L, C) of x's type and last (B, C) fp32, the state after each sequence's last token.
     Differentiable in x, g and h0, but not with h_index or h_out: those are for answering."""
     global _fast, _last
@@ -184,6 +193,8 @@ def gated_scan(x: torch.Tensor, g: torch.Tensor, h0=None, *, lengths=None, reset
         if h0 is not None and h0.dtype == torch.float32 and _overlap(h0, h_out) and \
                 (h_index is not None or h0.data_ptr() != h_out.data_ptr() or not h0.is_contiguous()):
             raise ValueError("gated_scan: h_out overlaps h0: only h_out = h0 without h_index is possible")
+        if any(_spans(t, h_out) for t in (x, g)):
+            raise ValueError("gated_scan: h_out overlaps an input")
     _, _, h, last, _, fl = _forward(x, g, h0, lengths, reset, h_index, h_out, False)
     if h_out is not None and not h_out.is_inference():         # autograd may have saved it
         torch.autograd.graph.increment_version(h_out)

@@ -213,6 +213,13 @@ def test_refusals():
         gated_scan(x, x, pool[:32].view(2, 16), h_out=pool[16:].view(2, 16))
     with pytest.raises(ValueError):
         gated_scan(x, x, h0, h_index=torch.zeros(2, dtype=torch.int32, device="cuda"), h_out=h0)
+    wide = torch.zeros(2, 3, 64, device="cuda")                       # a state next to its inputs is fine, inside them not
+    own = wide[:1, :, :16]
+    for kw in (dict(x=own, g=own.clone()), dict(x=own.clone(), g=own)):
+        for out in (wide[:1, 0, :16], wide[:1, 2, :16], wide[:1, 1, 8:24]):
+            with pytest.raises(ValueError, match="overlaps"):
+                gated_scan(**kw, h_out=out)
+        gated_scan(**kw, h_out=wide[1:, 0, :16])
     for kw in (dict(h_index=torch.zeros(2, dtype=torch.int32, device="cuda")), dict(h_out=torch.zeros_like(h0))):
         with pytest.raises(RuntimeError, match="no backward"):
             gated_scan(need, x, h0, **kw)
