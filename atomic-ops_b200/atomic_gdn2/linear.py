@@ -8,6 +8,7 @@ residual, W stored (din, dout) as in the layers.  x, W and the residual are all 
 * fp32: the tensor cores multiply three bf16 terms of every value (24 bits), sums leave them every 64 values and
   go on in rounded fp32 additions: errors are those of a plain fp32 product.  Magnitudes below about 2^-110 lose
   their low bits.
+* small products of either type (some 256 x 256 x 256 and below): plain fp32 in one launch, their backward in one.
 
 Up to 16 rows of fp32 x (4 of bf16) are multiplied without the tensor cores, W read once per eight rows.  Infinities
 and NaN come out as the plain sums would have them.

@@ -864,7 +864,7 @@ __global__ void __launch_bounds__(256) linear_few_kernel(const __grid_constant__
 // of 32 x 32 tiles from shared memory, dz made as it is read (which sizes, and what both ways take: small_within).
 // Eight groups of 64 threads share a tile's sum, 4 x 4 of its elements a thread, and join at the end in their order.  A
 // step of 64 along the sum takes 1.0 us: the loads' and shared memory's latency, with a tile's 16 warps alone on their SM
-// (four groups, 8 warps: 1.05 us and in bf16 1.3, half of the issue slots empty).
+// and half of its issue slots empty (four groups, 8 warps: 1.05 us, in bf16 1.3).
 constexpr int kSmallTile = 32, kSmallK = 64, kSmallRow = kSmallTile + 4, kSmallThreads = 512,
               kSmallGroups = kSmallThreads / 64, kSmallLoads = kSmallTile * kSmallK / kSmallThreads;
 static_assert(kSmallTile == 32 && kSmallThreads == 512 && kSmallLoads == 4, "SmallOperand");
@@ -1167,10 +1167,10 @@ size_t element(const gdn2_linear_desc* d) { return d->dtype == GDN2_BF16 ? 2 : 4
 // against 16.3, 16 x 4096 x 4096 43 against about 50); bf16 rows are few where a launch less counts (4 x 512 x 4608 5.8 us
 // against 8.1; of 8 rows 11.2 against 8.1, 8 x 4096 x 4096 21 against 15).
 int few_rows(const gdn2_linear_desc* d) { return d->dtype == GDN2_F32 ? 16 : 4; }
-// The small kernel takes about 2 + k / 64 us for a sum over k where every tile has an SM of its own, and its tiles' sum shared out where
-// they have not.  It is taken where that is less than the tiled path takes at such sizes: forward 11 to 15 us in fp32 (of
-// which making the terms is 4) and 5 to 8 in bf16; dx with dW 19 to 32 and 12 to 24, one of them alone 10 to 18 and 4 to
-// 5, with GELU's dz to make 6 to 12.  fp32 64 x 128 x 96 forward 10.5 -> 4.6 us, backward 19.8 -> 4.7; 128 x 512 x 256
+// The small kernel takes about 2 + k / 64 us for a sum over k where every tile has an SM of its own, and all tiles' work
+// shared out where they have not.  It is taken where that is less than the tiled path takes at such sizes: forward 11 to
+// 15 us in fp32 (of which making the terms is 4) and 5 to 8 in bf16; dx with dW 19 to 32 and 12 to 24, one of them alone
+// 10 to 18 and 4 to 5, with GELU's dz to make 6 to 12.  fp32 64 x 128 x 96 forward 10.5 -> 4.6 us, backward 19.8 -> 4.7; 128 x 512 x 256
 // 13.6 -> 10.6 and 24.8 -> 9.0; 256 x 256 x 256 13.1 -> 6.6 and 29.2 -> 7.8; 128 x 1024 x 128 14.2 against 18.7: not taken.
 // bf16 64 x 128 x 96 6.0 -> 4.6 and 13.0 -> 4.8; 128 x 512 x 256 8.1 against 11.2: not taken.
 struct SmallSize { long long tiles, steps; };
