@@ -98,10 +98,16 @@ class _Linear(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        x, w, z = ctx.saved_tensors
+        x, w, z = ctx.saved_tensors                   # or what their hooks made of them
+        x, w = _rows(x), _rows(w)
+        if z is not None:
+            z = z.contiguous()
         M, K, N, dev = x.shape[0], x.shape[1], w.shape[1], x.device
         want_x, want_w, want_b, want_r, _ = ctx.needs_input_grad
         dr = dy if want_r else None
+        if dy.shape != (M, N) or w.shape[0] != K or (z is not None and z.shape != (M, N)) or \
+                any(t is not None and (t.device != dev or t.dtype != x.dtype) for t in (w, z, dy)):
+            raise RuntimeError("linear: a saved tensor came back on another device, or with another type or size")
         dx = torch.empty((M, K), dtype=x.dtype, device=dev) if want_x else None
         new = torch.empty if M else torch.zeros
         dw = new((K, N), dtype=w.dtype, device=dev) if want_w else None

@@ -286,6 +286,15 @@ variable_list once(variable_list grads, const char* what) {
   return (*node)(std::move(grads));
 }
 
+// What a backward gets of saved tensors is what their hooks gave back (one that keeps them on the host returns copies in an
+// order of its own): their strides are read there, and layouts that the kernels cannot read are copied.
+at::Tensor dense(const at::Tensor& t) { return t.is_contiguous() && on16(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
+at::Tensor matrix(const at::Tensor& t) {
+  if (t.dim() != 2) return dense(t);
+  const bool rows = (t.size(1) == 1 || t.stride(1) == 1) && (t.size(0) == 1 || t.stride(0) >= t.size(1)) && on16(t);
+  return rows ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
 struct LinearCall {
   gdn2_linear_desc d;
   std::vector<int64_t> out;            // y's shape
@@ -311,24 +320,29 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
     ctx->save_for_backward({x, w, z});
     auto& data = ctx->saved_data;
     const gdn2_linear_desc& d = c->d;
-    data["desc"] = std::vector<int64_t>{d.M, d.K, d.N, d.dtype, d.bias_dtype, d.act, d.x_stride, d.w_stride,
-                                        bias.has_value(), res.has_value()};
+    data["desc"] = std::vector<int64_t>{d.M, d.K, d.N, d.dtype, d.bias_dtype, d.act, bias.has_value(), res.has_value()};
     data["flags"] = (int64_t) reinterpret_cast<intptr_t>(flags);
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const at::Tensor &x = saved[0], &w = saved[1], &z = saved[2];
     const auto v = ctx->saved_data["desc"].toIntVector();
-    gdn2_linear_desc d{(int32_t)v[0], (int32_t)v[1], (int32_t)v[2], (int32_t)v[3], (int32_t)v[4], (int32_t)v[5], v[6], v[7], 0};
-    const auto dev = x.device();
+    gdn2_linear_desc d{(int32_t)v[0], (int32_t)v[1], (int32_t)v[2], (int32_t)v[3], (int32_t)v[4], (int32_t)v[5], 0, 0, 0};
+    const auto dev = grads[0].device();
     const c10::cuda::CUDAGuard guard(dev);
+    for (int i = 0; i < (d.act ? 3 : 2); ++i)
+      TORCH_CHECK(saved[i].device() == dev && saved[i].scalar_type() == grads[0].scalar_type() && saved[i].dim() > 1 &&
+                      saved[i].size(-1) == (i ? d.N : d.K) && saved[i].numel() == (int64_t)(i == 1 ? d.K : d.M) * (i ? d.N : d.K),
+                  "linear: a saved tensor came back on another device, or with another type or size");
+    const at::Tensor x = matrix(saved[0]), w = matrix(saved[1]), z = d.act ? dense(saved[2]) : at::Tensor();
+    d.x_stride = x.dim() == 2 && d.M > 1 ? x.stride(0) : d.K;
+    d.w_stride = d.K > 1 ? w.stride(0) : d.N;
     at::Tensor dy = grads[0].contiguous(), dx, dw, db;
     if (!on16(dy)) dy = dy.clone();
     if (ctx->needs_input_grad(0)) dx = fresh(x.sizes(), x.scalar_type(), dev);
     if (ctx->needs_input_grad(1)) dw = fresh(w.sizes(), w.scalar_type(), dev);
     const int64_t n[1] = {d.N};
-    const bool has_b = v[8], has_r = v[9];
+    const bool has_b = v[6], has_r = v[7];
     if (has_b && ctx->needs_input_grad(2)) db = fresh(n, d.bias_dtype == GDN2_BF16 ? at::kBFloat16 : at::kFloat, dev);
     const int32_t want = (dx.defined() ? 1 : 0) + (dw.defined() ? 2 : 0) + (db.defined() ? 4 : 0);
     if (want) {
@@ -407,6 +421,18 @@ gdn2_gated_desc gated_desc(const at::Tensor& x, const at::Tensor& g) {
 struct GatedMasks {
   at::Tensor lengths, reset;
 };
+// Unit stride along C, on 4 bytes.
+at::Tensor rows(const at::Tensor& t) {
+  const bool as_is = (t.size(2) == 1 || t.stride(2) == 1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 4 == 0;
+  return as_is ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+// A copy whose rows are an odd number of values apart.
+at::Tensor odd_rows(const at::Tensor& t) {
+  const int64_t C = t.size(2) | 1, size[3] = {t.size(0), t.size(1), C};
+  at::Tensor r = fresh(size, t.scalar_type(), t.device()).narrow(2, 0, t.size(2));
+  r.copy_(t);
+  return r;
+}
 struct GatedFn : torch::autograd::Function<GatedFn> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& g, const std::optional<at::Tensor>& first,
                                const GatedMasks* masks, uint32_t* flags) {
@@ -429,10 +455,38 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const at::Tensor &x = saved[0], &g = saved[1], &marks = saved[2], &lengths = saved[3], &reset = saved[4];
-    const auto dev = x.device();
+    const auto dev = saved[0].device();
+    TORCH_CHECK(dev.is_cuda(), "gated_scan: a saved tensor came back on another device");
     const c10::cuda::CUDAGuard guard(dev);
+    for (const auto& t : saved)
+      TORCH_CHECK(!t.defined() || t.device() == dev, "gated_scan: a saved tensor came back on another device");
+    for (const auto& t : grads)
+      TORCH_CHECK(!t.defined() || t.device() == dev, "gated_scan: a saved tensor came back on another device");
+    const auto size = saved[0].sizes();
+    const auto type = saved[0].scalar_type();
+    TORCH_CHECK(size.size() == 3 && saved[1].sizes() == size && saved[1].scalar_type() == type &&
+                    saved[2].scalar_type() == at::kByte &&
+                    (!saved[3].defined() || (saved[3].numel() == size[0] && saved[3].scalar_type() == at::kInt)) &&
+                    (!saved[4].defined() || (saved[4].numel() == size[0] * size[1] && saved[4].scalar_type() == at::kBool)) &&
+                    (!grads[0].defined() || (grads[0].sizes() == size && grads[0].scalar_type() == type)) &&
+                    (!grads[1].defined() || (grads[1].size(0) == size[0] && grads[1].size(1) == size[2])),
+                "gated_scan: a saved tensor came back with another type or size");
+    at::Tensor x = rows(saved[0]), g = rows(saved[1]);
+    const at::Tensor marks = dense(saved[2]), lengths = saved[3].defined() ? dense(saved[3]) : saved[3],
+                     reset = saved[4].defined() ? dense(saved[4]) : saved[4];
     gdn2_gated_desc d = gated_desc(x, g);
+    // The marks lie as x's and g's rows were in the forward, one or two channels to a lane.
+    const auto other = [&] { return (int64_t)gdn2_gated_marks_bytes(&d) != marks.numel(); };
+    if (other()) {
+      x = x.clone(at::MemoryFormat::Contiguous);
+      g = g.clone(at::MemoryFormat::Contiguous);
+      d = gated_desc(x, g);
+    }
+    if (other()) {
+      x = odd_rows(x);
+      d = gated_desc(x, g);
+    }
+    TORCH_CHECK(!other(), "gated_scan: a saved tensor came back with another type or size");
     at::Tensor dh = grads[0], dlast = grads[1], dx = fresh(x.sizes(), x.scalar_type(), dev), dg = fresh(x.sizes(), x.scalar_type(), dev), d0;
     if (dh.defined()) {
       dh = dh.contiguous();

@@ -339,6 +339,37 @@ def test_other_stream_and_graph():
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,L,C", [(2, 100, 64), (3, 1, 64), (1, 37, 40), (40, 200, 256)])
+def test_saved_tensors_that_come_back_in_another_order(B, L, C, dtype):
+    """Saved on the host they come back contiguous, whatever the strides they had; other hooks may turn them.  The marks
+    of a forward whose rows had an odd number of values are not those of an even one."""
+    gen = torch.Generator(device="cuda").manual_seed(L)
+    n = lambda *s: torch.randn(*s, generator=gen, device="cuda")
+    x, g, dh, h0, dlast = n(B, L, C).to(dtype), -n(B, L, C).abs().to(dtype), n(B, L, C).to(dtype), n(B, C), n(B, C)
+    lengths = torch.randint(0, L + 1, (B,), generator=gen, device="cuda", dtype=torch.int32)
+    reset = torch.rand(B, L, generator=gen, device="cuda") < 0.05
+    views = ((x, g), (torch.cat([x, x], 2)[..., :C], torch.cat([g, g], 2)[..., :C]),
+             (torch.cat([x, x[..., :1]], 2)[..., :C], g), (x, torch.cat([g, g[..., :3]], 2)[..., :C]))
+    hooks = (None, torch.autograd.graph.save_on_cpu(), torch.autograd.graph.saved_tensors_hooks(
+        lambda t: t, lambda t: torch.cat([t, t[..., :1]], 2)[..., :C] if t.ndim == 3 else t),
+        torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.mT.contiguous().mT if t.ndim == 3 else t))
+    for x2, g2 in views:
+        want = None
+        for hook in hooks:
+            ts = [t.detach().requires_grad_(True) for t in (x2, g2, h0)]
+            with hook or torch.enable_grad():
+                out = gated_scan(*ts, lengths=lengths, reset=reset)
+            got = torch.autograd.grad(out, ts, (dh, dlast))
+            want = want or got
+            assert all(torch.equal(a, c) for a, c in zip(got, want))
+    for back, match in ((lambda t: t.cpu(), "another device"), (lambda t: t[:, :0] if t.ndim == 3 else t, "size")):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, back):
+            h, _ = gated_scan(*ts)
+        with pytest.raises(RuntimeError, match=match):
+            h.sum().backward()
+
+
 def test_same_bits_every_time():
     for B, L, C in ((1, 20000, 40), (3, 1111, 700)):
         x, g, h0, dy, dl = _inputs(B, L, C, torch.float32, 17)

@@ -259,6 +259,34 @@ def test_other_stream_and_graph(dtype):
         assert all(torch.equal(a, c) for a, c in zip(want, out)) and torch.equal(few, want_few)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M,K,N", [(70, 96, 40), (1300, 100, 1160)])
+def test_saved_tensors_that_come_back_in_another_order(M, K, N, dtype):
+    """Saved on the host they come back contiguous, whatever the strides they had; other hooks may turn them."""
+    x, w, b, r, dy = _data(M, K, N, dtype, 12)
+    want = None
+    hooks = (None, torch.autograd.graph.save_on_cpu(), torch.autograd.graph.saved_tensors_hooks(
+        lambda t: t, lambda t: t.mT.contiguous().mT if t.ndim == 2 else t))
+    for x2, w2 in ((x, w), (torch.cat([x, x, x], 1)[:, 8:8 + K], torch.cat([w, w], 1)[:, :N])):
+        if x2 is not x:
+            x2.copy_(x)
+        for hook in hooks:
+            ts = [t.detach().requires_grad_(True) for t in (x2, w2, b)]
+            with hook or torch.enable_grad():
+                y = linear(*ts, act="gelu", residual=r)
+            got = torch.autograd.grad(y, ts, dy)
+            want = want or got
+            assert all(torch.equal(a, c) for a, c in zip(got, want))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.cpu()):
+        y = linear(*ts)
+    with pytest.raises(RuntimeError, match="another device"):
+        y.sum().backward()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t[:-1]):
+        y = linear(*ts)
+    with pytest.raises(RuntimeError, match="size"):
+        y.sum().backward()
+
+
 def test_large_offsets():
     """Outputs of more than 2^31 values."""
     M, K, N = 70000, 16, 32768
