@@ -111,13 +111,7 @@ class _Gated(torch.autograd.Function):
         if any(t is not None and t.device != dev for t in (g, marks, lengths, reset, dh, dlast)):
             raise RuntimeError("gated_scan: a saved tensor came back on another device")
         for t, shape in ((g, x.shape), (lengths, (B,)), (reset, (B, L)), (dh, x.shape), (dlast, (B, C))):
-            if t is not None and t.shape != shape or g.dtype != x.dtype:
-                raise RuntimeError("gated_scan: a saved tensor came back with another type or size")
-        if _desc(x, g, 0)[2] != marks.numel():              # they lie as the rows were in the forward, see _readable
-            x, g = x.contiguous(), g.contiguous()
-            if _desc(x, g, 0)[2] != marks.numel():
-                x = torch.nn.functional.pad(x, (0, 1 - C % 2))[..., :C]
-            if _desc(x, g, 0)[2] != marks.numel():
+            if t is not None and t.shape != shape or g.dtype != x.dtype or marks.numel() != _desc(x, g, 0)[2]:
                 raise RuntimeError("gated_scan: a saved tensor came back with another type or size")
         tx, tg, th = ctx.types
         if dlast is not None:

@@ -5,7 +5,7 @@
 // Past a sequence's length the state stands still and outputs and gradients are zero.
 //
 // The bytes bound it: x and g are read and h is written once, backward x, g and dy are read and dx and dg
-// written once.  A thread walks S tokens of V channels in registers: once from zero, for what the segment
+// written once.  A thread walks S tokens of a channel in registers: once from zero, for what the segment
 // does to a state (h -> A h + q), and, when the state that enters is known, once more as the recurrence
 // itself, so that an output carries the rounding of its own steps and of the few joined segments before.
 // Segments are joined over a warp's lanes by shuffles, over a CTA's warps in shared memory and over the CTAs of
@@ -18,7 +18,8 @@
 //
 // Measured (forward + backward kernels): 8 x 2048 x 768 fp32 31 + 46 us, 403 MB at 5.2 TB/s; 1 x 131072 x 256
 // fp32 101 + 141 us, 34 dependent rounds of 3 and 4 us; 5 x 3001 x 1001 bf16 (ragged) 46 + 75 us, rows that start
-// on odd places are read two bytes at a time and the longest sequence's rounds follow one another.
+// on odd places are read two bytes at a time and the longest sequence's rounds follow one another; 16 x 3001 x 1000 bf16
+// 130 + 184 us, 769 MB at 2.4 TB/s: issue slots, a value takes as many instructions as in fp32.
 #include <cooperative_groups.h>
 #include <cuda.h>
 
@@ -35,11 +36,12 @@ constexpr float kReset = -1.f;        // a segment's factor when a reset is in i
 constexpr float kTiny = 1.17549435e-38f;
 constexpr int kMaxWarps = 8, kMaxCluster = 8;
 constexpr int kTileStages = 2;
-// Tokens of a thread's segment of V channels.  Odd: where the lanes of a warp hold several segments, their rows in a
-// tile in shared memory start in different banks.  Three CTAs of the backward pass fit an SM with 11 (5 of pairs), two
-// with 15 (7): where there are many sequences and channels the former count (8 x 2048 x 768: 60 -> 45 us), where few
-// long ones are walked in clusters the fewer rounds (1 x 131072 x 256: 174 -> 141 us).
-constexpr int tokens(int V, bool many) { return V == 1 ? (many ? 11 : 15) : many ? 5 : 7; }
+// Tokens of a thread's segment.  Odd: where the lanes of a warp hold several segments, their rows in a tile in shared
+// memory start in different banks.  Three CTAs of the backward pass fit an SM with 11, two with 15: where there are many
+// sequences and channels the former count (8 x 2048 x 768: 60 -> 45 us), where few long ones are walked in clusters the
+// fewer rounds (1 x 131072 x 256: 174 -> 141 us).  (bf16 channels in pairs, 5 or 7 tokens: half the loads, but the
+// joins of two channels for fewer tokens: 16 x 3001 x 1000 161 + 219 us against 130 + 184.)
+constexpr int tokens(bool many) { return many ? 11 : 15; }
 
 struct GatedParams {
   const void *x, *g, *dy;
@@ -59,7 +61,14 @@ struct GatedParams {
   int cols, clusters, lanes_log2;     // column blocks, CTAs of a cluster, lanes along C
 };
 
-// ---- values of V neighbouring channels ----------------------------------------------------------
+__device__ __forceinline__ float value(float r) { return r; }
+__device__ __forceinline__ float value(__nv_bfloat16 r) { return __bfloat162float(r); }
+template <class T>
+__device__ __forceinline__ T rounded(float v) {
+  if constexpr (sizeof(T) == 2) return __float2bfloat16_rn(v);
+  else return v;
+}
+// V neighbouring channels of a step
 template <class T, int V>
 struct Lane;
 template <>
@@ -134,23 +143,22 @@ __device__ __forceinline__ uint32_t resets_of(const GatedParams& p, int b, long 
 }
 
 // The first `live` of S rows: all at once where there are S.
-template <int S, class raw>
-__device__ __forceinline__ void rows_of(raw r[S], const raw* p, long long ld, int live) {
+template <int S, class T>
+__device__ __forceinline__ void rows_of(T r[S], const T* p, long long ld, int live) {
   if (live == S) {
 #pragma unroll
     for (int i = 0; i < S; ++i) r[i] = __ldg(p + i * ld);
   } else {
-    for (int i = 0; i < S; ++i) r[i] = raw{};
+    for (int i = 0; i < S; ++i) r[i] = T{};
 #pragma unroll
     for (int i = 0; i < S; ++i)
       if (i < live) r[i] = __ldg(p + i * ld);
   }
 }
 
-template <int V>
 struct Shared {
-  Seg part[2][kMaxWarps][32 * V];       // a warp's segments together, by channel of a row of lanes, for two rounds
-  Seg inbox[2][kMaxCluster][32 * V];    // the CTAs' of the cluster, for two rounds
+  Seg part[2][kMaxWarps][32];       // a warp's segments together, by channel of a row of lanes, for two rounds
+  Seg inbox[2][kMaxCluster][32];    // the CTAs' of the cluster, for two rounds
   uint64_t bar[2];                      // that they are there
   uint64_t full[kTileStages];           // that a stage's tiles are
   volatile int dead;                    // a wait ran out
@@ -160,8 +168,7 @@ struct Shared {
 // receiver's barrier.  (A barrier over the cluster would order all of the CTA's memory accesses, the outputs' of the
 // round before among them: 5.0 us a round of 8 CTAs.)  A CTA sends round r + 2 after it has seen every CTA's
 // round r + 1, which these send after they have read round r: two boxes are enough.
-template <int V>
-__device__ __forceinline__ void send(Shared<V>& sm, int box, int from, int to, int at, Seg s) {
+__device__ __forceinline__ void send(Shared& sm, int box, int from, int to, int at, Seg s) {
   uint32_t dst, bar;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(dst) : "r"(smem_u32(&sm.inbox[box][from][at])), "r"(to));
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_u32(&sm.bar[box])), "r"(to));
@@ -185,8 +192,7 @@ __device__ __forceinline__ bool cluster_wait(uint64_t* bar, uint32_t parity) {
   }
 }
 
-template <int V>
-__device__ __forceinline__ void begin(Shared<V>& sm, int n, bool tiles) {
+__device__ __forceinline__ void begin(Shared& sm, int n, bool tiles) {
   if (n == 1 && !tiles) return;
   if (threadIdx.x == 0) {
     mbar_init(&sm.bar[0], 1);
@@ -198,15 +204,13 @@ __device__ __forceinline__ void begin(Shared<V>& sm, int n, bool tiles) {
   if (n > 1) cg::this_cluster().sync();
   else __syncthreads();
 }
-template <int V>
-__device__ __forceinline__ void tile_wait(Shared<V>& sm, int stage, uint32_t parity, uint32_t* flags) {
+__device__ __forceinline__ void tile_wait(Shared& sm, int stage, uint32_t parity, uint32_t* flags) {
   if (sm.dead || cluster_wait(&sm.full[stage], parity)) return;
   sm.dead = 1;
   if (flags) flags[2] = 1;
 }
 // Before the CTA ends: its copies out of shared memory are over, and had a wait run out, those into it are given time.
-template <int V>
-__device__ __forceinline__ void tiles_done(const Shared<V>& sm) {
+__device__ __forceinline__ void tiles_done(const Shared& sm) {
   asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   if (sm.dead) {
     const long long t0 = clock64();
@@ -225,77 +229,67 @@ __device__ __forceinline__ float step_as(Seg s, float h) {
   if constexpr (PLAIN) return fmaf(s.A, h, s.q);
   else return step(s, h);
 }
-template <bool PLAIN, int V>
-__device__ __forceinline__ void join_warp(Seg (*part)[32 * V], const Seg mine[V], int lanes, Seg before[V]) {
+template <bool PLAIN>
+__device__ __forceinline__ void join_warp(Seg (*part)[32], Seg all, int lanes, Seg& before) {
   const int at = threadIdx.x & 31, lane = at & (lanes - 1), warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    Seg all = mine[v];
-    for (int d = lanes; d < 32; d <<= 1) {
-      const Seg left = {__shfl_up_sync(0xffffffffu, all.A, d), __shfl_up_sync(0xffffffffu, all.q, d)};
-      if (at >= d) all = join_as<PLAIN>(left, all);
-    }
-    if (at >= 32 - lanes) part[warp][lane * V + v] = all;
-    before[v] = {1.f, 0.f};
-    if (lanes < 32) {
-      before[v] = {__shfl_up_sync(0xffffffffu, all.A, lanes), __shfl_up_sync(0xffffffffu, all.q, lanes)};
-      if (at < lanes) before[v] = {1.f, 0.f};
-    }
+  for (int d = lanes; d < 32; d <<= 1) {
+    const Seg left = {__shfl_up_sync(0xffffffffu, all.A, d), __shfl_up_sync(0xffffffffu, all.q, d)};
+    if (at >= d) all = join_as<PLAIN>(left, all);
+  }
+  if (at >= 32 - lanes) part[warp][lane] = all;
+  before = {1.f, 0.f};
+  if (lanes < 32) {
+    before = {__shfl_up_sync(0xffffffffu, all.A, lanes), __shfl_up_sync(0xffffffffu, all.q, lanes)};
+    if (at < lanes) before = {1.f, 0.f};
   }
 }
-template <bool PLAIN, int V>
-__device__ __forceinline__ void join_cta(Shared<V>& sm, int round, int lanes, int rank, int n, Seg before[V], float enter[V], float mine_in[V]) {
+template <bool PLAIN>
+__device__ __forceinline__ void join_cta(Shared& sm, int round, int lanes, int rank, int n, Seg& before, float& enter, float& mine_in) {
   const int at = threadIdx.x & 31, lane = at & (lanes - 1), warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    if (n > 1) {
-      Seg pre = {1.f, 0.f};
-      for (int i = 0; i < warp; ++i) pre = join_as<PLAIN>(pre, sm.part[round & 1][i][lane * V + v]);
-      if (warp == warps - 1 && at < lanes) {
-        const Seg all = join_as<PLAIN>(pre, sm.part[round & 1][warp][lane * V + v]);
-        for (int r = 0; r < n; ++r) send(sm, round & 1, rank, r, lane * V + v, all);
-      }
-      before[v] = join_as<PLAIN>(pre, before[v]);
-    } else {                            // the state itself goes from warp to warp
-      float h = enter[v], in = h;
-      for (int i = 0; i < warps; ++i) {
-        if (i == warp) in = h;
-        h = step_as<PLAIN>(sm.part[round & 1][i][lane * V + v], h);
-      }
-      mine_in[v] = step_as<PLAIN>(before[v], in);
-      enter[v] = h;
+  if (n > 1) {
+    Seg pre = {1.f, 0.f};
+    for (int i = 0; i < warp; ++i) pre = join_as<PLAIN>(pre, sm.part[round & 1][i][lane]);
+    if (warp == warps - 1 && at < lanes) {
+      const Seg all = join_as<PLAIN>(pre, sm.part[round & 1][warp][lane]);
+      for (int r = 0; r < n; ++r) send(sm, round & 1, rank, r, lane, all);
     }
+    before = join_as<PLAIN>(pre, before);
+  } else {                              // the state itself goes from warp to warp
+    float h = enter, in = h;
+    for (int i = 0; i < warps; ++i) {
+      if (i == warp) in = h;
+      h = step_as<PLAIN>(sm.part[round & 1][i][lane], h);
+    }
+    mine_in = step_as<PLAIN>(before, in);
+    enter = h;
   }
 }
 
 // Joins the segments of all threads.  The lanes of a warp hold 32 / lanes neighbouring segments of the same
-// channels, the warps of a CTA and the CTAs of a cluster follow one another.  enter[] is the state that the
-// cluster's first segment enters with; on return mine_in[] is what this thread's enters with, and enter[] what the
+// channels, the warps of a CTA and the CTAs of a cluster follow one another.  `enter` is the state that the
+// cluster's first segment enters with; on return `mine_in` is what this thread's enters with, and `enter` what the
 // next round's first one does.  `plain`: no reset and no gate of zero in this thread's segment.
-template <int V>
-__device__ __forceinline__ void exchange(Shared<V>& sm, int round, const Seg mine[V], bool plain, int lanes, int rank, int n,
-                                         float enter[V], float mine_in[V], uint32_t* flags) {
+__device__ __forceinline__ void exchange(Shared& sm, int round, Seg mine, bool plain, int lanes, int rank, int n,
+                                         float& enter, float& mine_in, uint32_t* flags) {
   const int lane = threadIdx.x & (lanes - 1);
-  Seg before[V];                        // of this warp's segments before this thread's
-  if (__all_sync(0xffffffffu, plain)) join_warp<true, V>(sm.part[round & 1], mine, lanes, before);
-  else join_warp<false, V>(sm.part[round & 1], mine, lanes, before);
-  if (__syncthreads_and(plain)) join_cta<true, V>(sm, round, lanes, rank, n, before, enter, mine_in);
-  else join_cta<false, V>(sm, round, lanes, rank, n, before, enter, mine_in);
+  Seg before;                           // of this warp's segments before this thread's
+  if (__all_sync(0xffffffffu, plain)) join_warp<true>(sm.part[round & 1], mine, lanes, before);
+  else join_warp<false>(sm.part[round & 1], mine, lanes, before);
+  if (__syncthreads_and(plain)) join_cta<true>(sm, round, lanes, rank, n, before, enter, mine_in);
+  else join_cta<false>(sm, round, lanes, rank, n, before, enter, mine_in);
   if (n > 1) {
-    Seg(*inbox)[32 * V] = sm.inbox[round & 1];
-    if (threadIdx.x == 0) mbar_arrive_expect_tx(&sm.bar[round & 1], (uint32_t)(n * lanes * V * sizeof(Seg)));
+    Seg(*inbox)[32] = sm.inbox[round & 1];
+    if (threadIdx.x == 0) mbar_arrive_expect_tx(&sm.bar[round & 1], (uint32_t)(n * lanes * sizeof(Seg)));
     if (!sm.dead && !cluster_wait(&sm.bar[round & 1], (round >> 1) & 1)) {
       sm.dead = 1;
       if (flags) flags[2] = 1;
     }
 #pragma unroll
     for (int r = 0; r < kMaxCluster; ++r)
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-        if (r < n) {
-          if (r == rank) mine_in[v] = step(before[v], enter[v]);
-          enter[v] = step(inbox[r][lane * V + v], enter[v]);
-        }
+      if (r < n) {
+        if (r == rank) mine_in = step(before, enter);
+        enter = step(inbox[r][lane], enter);
+      }
   }
 }
 
@@ -305,13 +299,13 @@ __device__ __forceinline__ float at_most_zero(float g) {  // a NaN stays one
   return r;
 }
 // What S tokens do to a state, from the product of their gates and the state that they make of zero.
-template <int S, int V>
-__device__ __forceinline__ Seg segment(const float (*a)[V], int v, float A, float q, uint32_t resets, bool& plain) {
+template <int S>
+__device__ __forceinline__ Seg segment(const float a[S], float A, float q, uint32_t resets, bool& plain) {
   if (resets) A = kReset;
   else if (!(A >= kTiny)) {             // underflow, or a gate that is zero (or a NaN)
     bool zero = false;
 #pragma unroll
-    for (int i = 0; i < S; ++i) zero |= a[i][v] == 0.f;
+    for (int i = 0; i < S; ++i) zero |= a[i] == 0.f;
     A = A != A ? A : zero ? 0.f : kTiny;
   }
   plain = plain && A > 0.f;
@@ -324,12 +318,14 @@ struct Tiles {
   CUtensorMap x, g, dy, o0, o1;         // o0: h or dx, o1: dg
   int boxes;                            // copies of a tile: their boxes have up to 256 rows
 };
+__host__ __device__ __forceinline__ uint32_t tile_pitch(uint32_t bytes) { return (bytes + 127) / 128 * 128; }
 struct Ring {
   uint64_t* bar;
   uint8_t* base;
-  uint32_t tile;                        // bytes
+  uint32_t bytes;                       // of a tile
   int arrays;                           // tiles of a stage
-  __device__ __forceinline__ uint32_t at(int stage, int array) const { return smem_u32(base) + (stage * arrays + array) * tile; }
+  __device__ __forceinline__ uint32_t tile() const { return tile_pitch(bytes); }
+  __device__ __forceinline__ uint32_t at(int stage, int array) const { return smem_u32(base) + (stage * arrays + array) * tile(); }
 };
 __device__ __forceinline__ void tile_in(uint32_t dst, const CUtensorMap* m, int c, int t, int b, uint32_t bar) {
   asm volatile(
@@ -346,75 +342,80 @@ __device__ __forceinline__ void tiles_read() {  // what was sent away has been r
   asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
 }
 __device__ __forceinline__ void stage_in(const Ring& r, const Tiles& m, int stage, int c, int t, int b, int rows) {
-  mbar_arrive_expect_tx(&r.bar[stage], r.tile * r.arrays);
-  const uint32_t bar = smem_u32(&r.bar[stage]), part = r.tile / m.boxes;
+  mbar_arrive_expect_tx(&r.bar[stage], r.bytes * r.arrays);
+  const uint32_t bar = smem_u32(&r.bar[stage]), part = r.bytes / m.boxes;
   for (int i = 0; i < m.boxes; ++i) {
     tile_in(r.at(stage, 0) + i * part, &m.x, c, t + i * rows, b, bar);
     tile_in(r.at(stage, 1) + i * part, &m.g, c, t + i * rows, b, bar);
     if (r.arrays == 3) tile_in(r.at(stage, 2) + i * part, &m.dy, c, t + i * rows, b, bar);
   }
 }
-template <class raw>
-__device__ __forceinline__ raw word(uint32_t at) {
-  uint32_t u;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(u) : "r"(at));
-  raw r;
-  memcpy(&r, &u, sizeof(raw));
+template <class T>
+__device__ __forceinline__ T word(uint32_t at) {
+  T r;
+  if constexpr (sizeof(T) == 4) {
+    uint32_t u;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(u) : "r"(at));
+    memcpy(&r, &u, 4);
+  } else {
+    uint16_t u;
+    asm volatile("ld.shared.b16 %0, [%1];" : "=h"(u) : "r"(at));
+    memcpy(&r, &u, 2);
+  }
   return r;
 }
-template <class raw>
-__device__ __forceinline__ void put_word(uint32_t at, raw r) {
-  uint32_t u = 0;
-  memcpy(&u, &r, sizeof(raw));
-  asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(u) : "memory");
+template <class T>
+__device__ __forceinline__ void put_word(uint32_t at, T r) {
+  if constexpr (sizeof(T) == 4) {
+    uint32_t u;
+    memcpy(&u, &r, 4);
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(u) : "memory");
+  } else {
+    uint16_t u;
+    memcpy(&u, &r, 2);
+    asm volatile("st.shared.b16 [%0], %1;" ::"r"(at), "h"(u) : "memory");
+  }
 }
 
 // Tiles past a sequence's length: zeros, and nothing else to do.
-template <class T, int V, int S>
+template <class T, int S>
 __device__ __forceinline__ void zero_rows(void* out, const GatedParams& p, int b, int c, int TT, int count, int rank, int place) {
-  using raw = typename Lane<T, V>::raw;
-  const float none[V] = {};
   for (long long tile = count + (rank - count % p.clusters + p.clusters) % p.clusters; tile * TT < p.L; tile += p.clusters) {
     const long long t0 = tile * TT + place * S;
-    raw* to = reinterpret_cast<raw*>(static_cast<T*>(out) + ((long long)b * p.L + t0) * p.C + c);
-    for (int i = 0; i < S && t0 + i < p.L; ++i) to[i * (long long)(p.C / V)] = Lane<T, V>::put(none);
+    T* to = static_cast<T*>(out) + ((long long)b * p.L + t0) * p.C + c;
+    for (int i = 0; i < S && t0 + i < p.L; ++i) to[i * (long long)p.C] = rounded<T>(0.f);
   }
 }
 
 // TILE: the rows come and go by tiled copies, a stage ahead of the work; else each thread reads and writes its own.
 // (8 x 2048 x 768 fp32: 46 instructions a value without tiles, 41 with them, and 92 against 76 us both ways: the
 // exponential is 8 of them, the segments' joins about 10.)
-template <class T, int V, int S, bool TILE>
+template <class T, int S, bool TILE>
 __global__ void __launch_bounds__(32 * kMaxWarps, 3) gated_fwd_kernel(const __grid_constant__ GatedParams p,
                                                                       const __grid_constant__ Tiles m) {
-  using L = Lane<T, V>;
-  using raw = typename L::raw;
   extern __shared__ __align__(128) uint8_t tiles[];
-  __shared__ Shared<V> sm;
+  __shared__ Shared sm;
   const int lanes = 1 << p.lanes_log2, lane = threadIdx.x & (lanes - 1);
   const int place = threadIdx.x >> p.lanes_log2, places = blockDim.x >> p.lanes_log2;
   const int rank = blockIdx.x % p.clusters, block = blockIdx.x / p.clusters;
-  const int b = block / p.cols, c0 = (block % p.cols) * lanes * V, c = c0 + lane * V;
+  const int b = block / p.cols, c0 = (block % p.cols) * lanes, c = c0 + lane;
   const bool on = c < p.C;
   const int len = length_of(p, b);
   const long long row = state_row(p, b);
   const int segs = (p.L + S - 1) / S, TT = places * S, count = (len + TT - 1) / TT;  // tiles of TT tokens with work
-  const Ring ring{sm.full, tiles, (uint32_t)(TT * lanes * 4), 2};
+  const Ring ring{sm.full, tiles, (uint32_t)(TT * lanes * sizeof(T)), 2};
   begin(sm, p.clusters, TILE);
   if (TILE && threadIdx.x == 0)
     for (int s = 0; s < kTileStages && s * p.clusters + rank < count; ++s)
       stage_in(ring, m, s, c0, (s * p.clusters + rank) * TT, b, TT / m.boxes);
-  float enter[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) enter[v] = on && row >= 0 ? p.h0[row * p.C + c + v] : 0.f;
-  const long long xl = p.xl / V, gl = p.gl / V, hl = p.C / V;
+  float enter = on && row >= 0 ? p.h0[row * p.C + c] : 0.f;
   float top = -1.f;                     // the largest gate
   for (int round = 0; round * p.clusters < count; ++round) {
     const int tile = round * p.clusters + rank, seg = tile * places + place, slot = round % kTileStages;
     const long long t0 = (long long)seg * S;
     const int alive = max(0, min(S, (int)min((long long)S, len - t0))), live = on ? alive : 0;
-    const uint32_t words = ring.at(slot, 0) + (place * S * lanes + lane) * 4;
-    float a[S][V], q[S][V];
+    const uint32_t words = ring.at(slot, 0) + (place * S * lanes + lane) * (int)sizeof(T);
+    float a[S], q[S];
     if constexpr (TILE) {
       if (threadIdx.x == 0 && round > 0) {  // the stage of the round before takes the next one
         tiles_read();
@@ -424,82 +425,63 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 3) gated_fwd_kernel(const __gr
       if (tile < count) tile_wait(sm, slot, (round / kTileStages) & 1, p.flags);
 #pragma unroll
       for (int i = 0; i < S; ++i) {
-        L::get(word<raw>(words + i * lanes * 4), q[i]);
-        L::get(word<raw>(words + ring.tile + i * lanes * 4), a[i]);
+        q[i] = value(word<T>(words + i * lanes * (int)sizeof(T)));
+        a[i] = value(word<T>(words + ring.tile() + i * lanes * (int)sizeof(T)));
       }
       if (live < S) {                   // past the length: whatever is there
 #pragma unroll
         for (int i = 0; i < S; ++i)
-          if (i >= live) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) q[i][v] = a[i][v] = 0.f;
-          }
+          if (i >= live) q[i] = a[i] = 0.f;
       }
     } else {
-      raw rx[S], rg[S];
-      rows_of<S>(rx, reinterpret_cast<const raw*>(static_cast<const T*>(p.x) + b * p.xb + c) + t0 * xl, xl, live);
-      rows_of<S>(rg, reinterpret_cast<const raw*>(static_cast<const T*>(p.g) + b * p.gb + c) + t0 * gl, gl, live);
+      T rx[S], rg[S];
+      rows_of<S>(rx, static_cast<const T*>(p.x) + b * p.xb + c + t0 * p.xl, p.xl, live);
+      rows_of<S>(rg, static_cast<const T*>(p.g) + b * p.gb + c + t0 * p.gl, p.gl, live);
 #pragma unroll
       for (int i = 0; i < S; ++i) {
-        L::get(rx[i], q[i]);
-        L::get(rg[i], a[i]);
+        q[i] = value(rx[i]);
+        a[i] = value(rg[i]);
       }
     }
 #pragma unroll
-    for (int i = 0; i < S; ++i)
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        top = fmaxf(top, a[i][v]);
-        a[i][v] = expf(at_most_zero(a[i][v]));
-      }
+    for (int i = 0; i < S; ++i) {
+      top = fmaxf(top, a[i]);
+      a[i] = expf(at_most_zero(a[i]));
+    }
     const uint32_t resets = resets_of<S>(p, b, t0, alive, lane, lanes);
-    Seg mine[V];
-    float mine_in[V];
+    float A = 1.f, s = 0.f, mine_in;
     bool plain = true;
+    if (!resets) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      float A = 1.f, s = 0.f;
-      if (!resets) {
-#pragma unroll
-        for (int i = 0; i < S; ++i) {
-          s = fmaf(a[i][v], s, q[i][v]);
-          A *= a[i][v];
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < S; ++i) s = ((resets >> i) & 1u) ? q[i][v] : fmaf(a[i][v], s, q[i][v]);
+      for (int i = 0; i < S; ++i) {
+        s = fmaf(a[i], s, q[i]);
+        A *= a[i];
       }
-      mine[v] = segment<S, V>(a, v, A, s, resets, plain);
-    }
-    exchange<V>(sm, round, mine, plain, lanes, rank, p.clusters, enter, mine_in, p.flags);
-    if (p.marks && live) {
+    } else {
 #pragma unroll
-      for (int v = 0; v < V; ++v) p.marks[((long long)b * segs + seg) * p.C + c + v] = mine_in[v];
+      for (int i = 0; i < S; ++i) s = ((resets >> i) & 1u) ? q[i] : fmaf(a[i], s, q[i]);
     }
+    const Seg mine = segment<S>(a, A, s, resets, plain);
+    exchange(sm, round, mine, plain, lanes, rank, p.clusters, enter, mine_in, p.flags);
+    if (p.marks && live) p.marks[((long long)b * segs + seg) * p.C + c] = mine_in;
     const bool whole = live == S && !resets;
-    raw* ph = reinterpret_cast<raw*>(static_cast<T*>(p.h) + (long long)b * p.L * p.C + c) + t0 * hl;
+    T* ph = static_cast<T*>(p.h) + ((long long)b * p.L + t0) * p.C + c;
     const int rows = on && tile < count ? (int)max(0ll, min((long long)S, p.L - t0)) : 0;
-    auto put = [&](int i, const float* y) {
-      if constexpr (TILE) put_word<raw>(words + i * lanes * 4, L::put(y));
-      else if (i < rows) ph[i * hl] = L::put(y);
+    auto put = [&](int i, float y) {
+      if constexpr (TILE) put_word(words + i * lanes * (int)sizeof(T), rounded<T>(y));
+      else if (i < rows) ph[i * (long long)p.C] = rounded<T>(y);
     };
     if (whole) {
 #pragma unroll
       for (int i = 0; i < S; ++i) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) mine_in[v] = fmaf(a[i][v], mine_in[v], q[i][v]);
+        mine_in = fmaf(a[i], mine_in, q[i]);
         put(i, mine_in);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < S; ++i) {
-        float y[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          mine_in[v] = ((resets >> i) & 1u) ? q[i][v] : fmaf(a[i][v], mine_in[v], q[i][v]);
-          y[v] = i < live ? mine_in[v] : 0.f;
-        }
-        put(i, y);
+        mine_in = ((resets >> i) & 1u) ? q[i] : fmaf(a[i], mine_in, q[i]);
+        put(i, i < live ? mine_in : 0.f);
       }
     }
     if constexpr (TILE) {
@@ -507,54 +489,46 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 3) gated_fwd_kernel(const __gr
       __syncthreads();
       if (threadIdx.x == 0 && tile < count) {
         for (int i = 0; i < m.boxes; ++i)
-          tile_out(&m.o0, ring.at(slot, 0) + i * (ring.tile / m.boxes), c0, tile * TT + i * (TT / m.boxes), b);
+          tile_out(&m.o0, ring.at(slot, 0) + i * (ring.bytes / m.boxes), c0, tile * TT + i * (TT / m.boxes), b);
         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       }
     }
   }
-  if (on) zero_rows<T, V, S>(p.h, p, b, c, TT, count, rank, place);
-  if (on && rank == 0 && place == 0) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) p.last[(long long)b * p.C + c + v] = enter[v];
-  }
+  if (on) zero_rows<T, S>(p.h, p, b, c, TT, count, rank, place);
+  if (on && rank == 0 && place == 0) p.last[(long long)b * p.C + c] = enter;
   if (top > 0.f) p.flags[0] = 1;
   if (TILE && threadIdx.x == 0) tiles_done(sm);
   if (p.clusters > 1) cg::this_cluster().sync();  // a CTA's shared memory is written until here
 }
 
 // The tiles and segments of a sequence in reverse: round 0 has the last ones.
-template <class T, int V, int S, bool TILE>
-__global__ void __launch_bounds__(32 * kMaxWarps, S * V < 12 ? 3 : 2) gated_bwd_kernel(const __grid_constant__ GatedParams p,
+template <class T, int S, bool TILE>
+__global__ void __launch_bounds__(32 * kMaxWarps, S < 12 ? 3 : 2) gated_bwd_kernel(const __grid_constant__ GatedParams p,
                                                                       const __grid_constant__ Tiles m) {
-  using L = Lane<T, V>;
-  using raw = typename L::raw;
   extern __shared__ __align__(128) uint8_t tiles[];
-  __shared__ Shared<V> sm;
+  __shared__ Shared sm;
   const int lanes = 1 << p.lanes_log2, lane = threadIdx.x & (lanes - 1);
   const int places = blockDim.x >> p.lanes_log2, place = places - 1 - (threadIdx.x >> p.lanes_log2);
   const int rank = blockIdx.x % p.clusters, block = blockIdx.x / p.clusters;
-  const int b = block / p.cols, c0 = (block % p.cols) * lanes * V, c = c0 + lane * V;
+  const int b = block / p.cols, c0 = (block % p.cols) * lanes, c = c0 + lane;
   const bool on = c < p.C;
   const int len = length_of(p, b);
   const int segs = (p.L + S - 1) / S, TT = places * S, count = (len + TT - 1) / TT;  // tiles of TT tokens with work
-  const Ring ring{sm.full, tiles, (uint32_t)(TT * lanes * 4), 3};
+  const Ring ring{sm.full, tiles, (uint32_t)(TT * lanes * sizeof(T)), 3};
   begin(sm, p.clusters, TILE);
   if (TILE && threadIdx.x == 0)
     for (int s = 0; s < kTileStages && s * p.clusters + rank < count; ++s)
       stage_in(ring, m, s, c0, (count - 1 - s * p.clusters - rank) * TT, b, TT / m.boxes);
-  float enter[V];  // e after the last token of a round
-#pragma unroll
-  for (int v = 0; v < V; ++v) enter[v] = on && p.dlast ? p.dlast[(long long)b * p.C + c + v] : 0.f;
-  const raw* g = reinterpret_cast<const raw*>(static_cast<const T*>(p.g) + b * p.gb + c);
-  const long long at = (long long)b * p.L * p.C + c, row = p.C / V;
-  const long long xl = p.xl / V, gl = p.gl / V;
+  float enter = on && p.dlast ? p.dlast[(long long)b * p.C + c] : 0.f;  // e after the last token of a round
+  const T* g = static_cast<const T*>(p.g) + b * p.gb + c;
+  const long long at = (long long)b * p.L * p.C + c, row = p.C;
   for (int round = 0; round * p.clusters < count; ++round) {
     const int tile = count - 1 - round * p.clusters - rank, slot = round % kTileStages;  // below 0: none
     const int seg = tile * places + place;
     const long long t0 = (long long)seg * S;
     const int alive = tile < 0 ? 0 : max(0, min(S, (int)min((long long)S, len - t0))), live = on ? alive : 0;
-    const uint32_t words = ring.at(slot, 0) + (place * S * lanes + lane) * 4;
-    float a[S][V], h[S][V], d[S][V], top = -1.f;
+    const uint32_t words = ring.at(slot, 0) + (place * S * lanes + lane) * (int)sizeof(T);
+    float a[S], h[S], d[S], top = -1.f;
     if constexpr (TILE) {
       if (threadIdx.x == 0 && round > 0) {  // the stage of the round before takes the next one
         tiles_read();
@@ -564,105 +538,87 @@ __global__ void __launch_bounds__(32 * kMaxWarps, S * V < 12 ? 3 : 2) gated_bwd_
       if (tile >= 0) tile_wait(sm, slot, (round / kTileStages) & 1, p.flags);
 #pragma unroll
       for (int i = 0; i < S; ++i) {
-        L::get(word<raw>(words + i * lanes * 4), h[i]);
-        L::get(word<raw>(words + ring.tile + i * lanes * 4), a[i]);
-        L::get(word<raw>(words + 2 * ring.tile + i * lanes * 4), d[i]);
+        h[i] = value(word<T>(words + i * lanes * (int)sizeof(T)));
+        a[i] = value(word<T>(words + ring.tile() + i * lanes * (int)sizeof(T)));
+        d[i] = value(word<T>(words + 2 * ring.tile() + i * lanes * (int)sizeof(T)));
       }
       if (live < S) {                   // past the length: whatever is there
 #pragma unroll
         for (int i = 0; i < S; ++i)
-          if (i >= live) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) h[i][v] = a[i][v] = d[i][v] = 0.f;
-          }
+          if (i >= live) h[i] = a[i] = d[i] = 0.f;
       }
     } else {
-      raw rx[S], rg[S], ry[S];
-      rows_of<S>(rx, reinterpret_cast<const raw*>(static_cast<const T*>(p.x) + b * p.xb + c) + t0 * xl, xl, live);
-      rows_of<S>(rg, g + t0 * gl, gl, live);
-      rows_of<S>(ry, reinterpret_cast<const raw*>(static_cast<const T*>(p.dy) + at) + t0 * row, row, live);
+      T rx[S], rg[S], ry[S];
+      rows_of<S>(rx, static_cast<const T*>(p.x) + b * p.xb + c + t0 * p.xl, p.xl, live);
+      rows_of<S>(rg, g + t0 * p.gl, p.gl, live);
+      rows_of<S>(ry, static_cast<const T*>(p.dy) + at + t0 * row, row, live);
 #pragma unroll
       for (int i = 0; i < S; ++i) {
-        L::get(rx[i], h[i]);
-        L::get(rg[i], a[i]);
-        L::get(ry[i], d[i]);
+        h[i] = value(rx[i]);
+        a[i] = value(rg[i]);
+        d[i] = value(ry[i]);
       }
     }
     const uint32_t resets = resets_of<S>(p, b, t0, alive, lane, lanes);
-    Seg mine[V];
-    float e[V];
     bool plain = true;
+    float s = live ? p.marks[((long long)b * segs + seg) * p.C + c] : 0.f, A = 1.f, back = 0.f, e;
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      float s = live ? p.marks[((long long)b * segs + seg) * p.C + c + v] : 0.f, A = 1.f, back = 0.f;
+    for (int i = 0; i < S; ++i) {
+      top = fmaxf(top, a[i]);
+      a[i] = expf(at_most_zero(a[i]));
+    }
+    if (!resets) {
 #pragma unroll
       for (int i = 0; i < S; ++i) {
-        top = fmaxf(top, a[i][v]);
-        a[i][v] = expf(at_most_zero(a[i][v]));
+        const float x = h[i];
+        h[i] = s;                       // the state before the token
+        s = fmaf(a[i], s, x);
       }
-      if (!resets) {
 #pragma unroll
-        for (int i = 0; i < S; ++i) {
-          const float x = h[i][v];
-          h[i][v] = s;                  // the state before the token
-          s = fmaf(a[i][v], s, x);
-        }
-#pragma unroll
-        for (int i = S - 1; i >= 0; --i) {
-          back = a[i][v] * (d[i][v] + back);
-          A *= a[i][v];
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < S; ++i) {
-          const float x = h[i][v];
-          h[i][v] = s;
-          s = ((resets >> i) & 1u) ? x : fmaf(a[i][v], s, x);
-        }
-#pragma unroll
-        for (int i = S - 1; i >= 0; --i) back = ((resets >> i) & 1u) ? 0.f : a[i][v] * (d[i][v] + back);
+      for (int i = S - 1; i >= 0; --i) {
+        back = a[i] * (d[i] + back);
+        A *= a[i];
       }
-      mine[v] = segment<S, V>(a, v, A, back, resets, plain);
+    } else {
+#pragma unroll
+      for (int i = 0; i < S; ++i) {
+        const float x = h[i];
+        h[i] = s;
+        s = ((resets >> i) & 1u) ? x : fmaf(a[i], s, x);
+      }
+#pragma unroll
+      for (int i = S - 1; i >= 0; --i) back = ((resets >> i) & 1u) ? 0.f : a[i] * (d[i] + back);
     }
-    exchange<V>(sm, round, mine, plain, lanes, rank, p.clusters, enter, e, p.flags);
-    raw* qx = reinterpret_cast<raw*>(static_cast<T*>(p.dx) + at) + t0 * row;
-    raw* qg = reinterpret_cast<raw*>(static_cast<T*>(p.dg) + at) + t0 * row;
+    const Seg mine = segment<S>(a, A, back, resets, plain);
+    exchange(sm, round, mine, plain, lanes, rank, p.clusters, enter, e, p.flags);
+    T* qx = static_cast<T*>(p.dx) + at + t0 * row;
+    T* qg = static_cast<T*>(p.dg) + at + t0 * row;
     const int rows = on && tile >= 0 ? (int)max(0ll, min((long long)S, p.L - t0)) : 0;
-    auto put = [&](int i, const float* ox, const float* og) {
+    auto put = [&](int i, float ox, float og) {
       if constexpr (TILE) {
-        put_word<raw>(words + i * lanes * 4, L::put(ox));
-        put_word<raw>(words + ring.tile + i * lanes * 4, L::put(og));
+        put_word(words + i * lanes * (int)sizeof(T), rounded<T>(ox));
+        put_word(words + ring.tile() + i * lanes * (int)sizeof(T), rounded<T>(og));
       } else if (i < rows) {
-        qx[i * row] = L::put(ox);
-        qg[i * row] = L::put(og);
+        qx[i * row] = rounded<T>(ox);
+        qg[i * row] = rounded<T>(og);
       }
     };
     if (live == S && !resets && !(top > 0.f)) {
 #pragma unroll
       for (int i = S - 1; i >= 0; --i) {
-        float ox[V], og[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          ox[v] = d[i][v] + e[v];
-          e[v] = a[i][v] * ox[v];
-          og[v] = e[v] * h[i][v];
-        }
-        put(i, ox, og);
+        const float ox = d[i] + e;
+        e = a[i] * ox;
+        put(i, ox, e * h[i]);
       }
     } else {
 #pragma unroll
       for (int i = S - 1; i >= 0; --i) {
-        float ox[V] = {}, og[V] = {};
+        float ox = 0.f, og = 0.f;
         if (i < live) {
           const bool r = (resets >> i) & 1u;
-          float gate[V];
-          L::get(g[(t0 + i) * gl], gate);
-#pragma unroll
-          for (int v = 0; v < V; ++v) {
-            ox[v] = d[i][v] + e[v];
-            e[v] = r ? 0.f : a[i][v] * ox[v];
-            og[v] = r || gate[v] > 0.f ? 0.f : e[v] * h[i][v];
-          }
+          ox = d[i] + e;
+          e = r ? 0.f : a[i] * ox;
+          og = r || value(g[(t0 + i) * p.gl]) > 0.f ? 0.f : e * h[i];
         }
         put(i, ox, og);
       }
@@ -672,7 +628,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, S * V < 12 ? 3 : 2) gated_bwd_
       __syncthreads();
       if (threadIdx.x == 0 && tile >= 0) {
         for (int i = 0; i < m.boxes; ++i) {
-          const uint32_t part = i * (ring.tile / m.boxes);
+          const uint32_t part = i * (ring.bytes / m.boxes);
           tile_out(&m.o0, ring.at(slot, 0) + part, c0, tile * TT + i * (TT / m.boxes), b);
           tile_out(&m.o1, ring.at(slot, 1) + part, c0, tile * TT + i * (TT / m.boxes), b);
         }
@@ -681,13 +637,10 @@ __global__ void __launch_bounds__(32 * kMaxWarps, S * V < 12 ? 3 : 2) gated_bwd_
     }
   }
   if (on) {
-    zero_rows<T, V, S>(p.dx, p, b, c, TT, count, rank, place);
-    zero_rows<T, V, S>(p.dg, p, b, c, TT, count, rank, place);
+    zero_rows<T, S>(p.dx, p, b, c, TT, count, rank, place);
+    zero_rows<T, S>(p.dg, p, b, c, TT, count, rank, place);
   }
-  if (p.dh0 && on && rank == 0 && place == places - 1) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) p.dh0[(long long)b * p.C + c + v] = enter[v];
-  }
+  if (p.dh0 && on && rank == 0 && place == places - 1) p.dh0[(long long)b * p.C + c] = enter;
   if (TILE && threadIdx.x == 0) tiles_done(sm);
   if (p.clusters > 1) cg::this_cluster().sync();  // a CTA's shared memory is written until here
 }
@@ -777,7 +730,7 @@ bool tile_map(CUtensorMap* map, const void* p, bool bf16, const GatedParams& q, 
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <class T, int V, int S>
+template <class T, int S>
 cudaError_t launch_gated_as(bool back, GatedParams& p, cudaStream_t st) {
   constexpr bool kBf16 = sizeof(T) == 2;
   const int segs = (p.L + S - 1) / S;
@@ -786,12 +739,13 @@ cudaError_t launch_gated_as(bool back, GatedParams& p, cudaStream_t st) {
   // 128 of 16, 300 with 256 of 8; 8 x 2048 x 768: 110 us with 192 of 32, 92 with 384 of 16, 136 with 384 of 32 in
   // pairs; all before the tiles).
   int lanes_log2 = 5, clusters = 1;
-  auto cols = [&] { return (int)((p.C + (long long)(V << lanes_log2) - 1) / (V << lanes_log2)); };
+  auto cols = [&] { return (int)((p.C + (1ll << lanes_log2) - 1) >> lanes_log2); };
   auto groups = [&] { return 32 >> lanes_log2; };
   while (lanes_log2 > 3 && (long long)p.B * cols() < 296 && 2 * groups() <= segs) --lanes_log2;
   int warps = (segs + groups() - 1) / groups();
   warps = warps < 1 ? 1 : warps > kMaxWarps ? kMaxWarps : warps;
-  if (warps * groups() * S > 256) warps = (warps + 1) / 2 * 2;  // two boxes of a tile, each on 128 bytes
+  constexpr int kEven = 8 / sizeof(T);
+  if (warps * groups() * S > 256) warps = (warps + kEven - 1) / kEven * kEven;  // two boxes of a tile, each on 128 bytes
   const int places = warps * groups(), TT = places * S;
   // with lengths half of the tiles or so are empty (5 x 3001 x 1001 bf16: 129 us with single CTAs, 120 in pairs, 129 in
   // fours)
@@ -801,9 +755,9 @@ cudaError_t launch_gated_as(bool back, GatedParams& p, cudaStream_t st) {
   p.lanes_log2 = lanes_log2;
   Tiles m;
   m.boxes = TT > 256 ? 2 : 1;
-  const int width = V << lanes_log2, rows = TT / m.boxes;
+  const int width = 1 << lanes_log2, rows = TT / m.boxes;
   const long long cb = (long long)p.L * p.C, cl = p.C;
-  bool tile = sizeof(T) * V == 4 && p.L > 0 && tile_map(&m.x, p.x, kBf16, p, p.xb, p.xl, width, rows) &&
+  bool tile = p.L > 0 && tile_map(&m.x, p.x, kBf16, p, p.xb, p.xl, width, rows) &&
               tile_map(&m.g, p.g, kBf16, p, p.gb, p.gl, width, rows) &&
               tile_map(&m.o0, back ? p.dx : p.h, kBf16, p, cb, cl, width, rows);
   if (tile && back)
@@ -811,7 +765,7 @@ cudaError_t launch_gated_as(bool back, GatedParams& p, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(p.B * p.cols * clusters));
   cfg.blockDim = dim3(32u * warps);
-  cfg.dynamicSmemBytes = tile ? (size_t)kTileStages * (back ? 3 : 2) * TT * (4u << lanes_log2) : 0;
+  cfg.dynamicSmemBytes = tile ? (size_t)kTileStages * (back ? 3 : 2) * tile_pitch(TT * (uint32_t)sizeof(T) * width) : 0;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -821,24 +775,21 @@ cudaError_t launch_gated_as(bool back, GatedParams& p, cudaStream_t st) {
   cfg.numAttrs = 1;
   auto go = [&](auto kernel, unsigned long long& done) {
     if (cfg.dynamicSmemBytes > 32768) {
-      const cudaError_t e = smem_attr_once(kernel, kTileStages * 3 * kMaxWarps * tokens(1, false) * 32 * 4, done);
+      const cudaError_t e = smem_attr_once(kernel, kTileStages * 3 * kMaxWarps * tokens(false) * 32 * 4, done);
       if (e != cudaSuccess) return e;
     }
     return cudaLaunchKernelEx(&cfg, kernel, p, m);
   };
   static unsigned long long done[2] = {};
-  if constexpr (sizeof(T) * V == 4) {
-    if (tile) return back ? go(gated_bwd_kernel<T, V, S, true>, done[1]) : go(gated_fwd_kernel<T, V, S, true>, done[0]);
-  }
-  return back ? go(gated_bwd_kernel<T, V, S, false>, done[1]) : go(gated_fwd_kernel<T, V, S, false>, done[0]);
+  if (tile) return back ? go(gated_bwd_kernel<T, S, true>, done[1]) : go(gated_fwd_kernel<T, S, true>, done[0]);
+  return back ? go(gated_bwd_kernel<T, S, false>, done[1]) : go(gated_fwd_kernel<T, S, false>, done[0]);
 }
 
 // Enough channels for more than one CTA of 16 lanes on every SM's two places.
-bool many(long long B, long long C, int V) { return B * ((C + 16 * V - 1) / (16 * V)) >= 296; }
-template <class T, int V>
+bool many(long long B, long long C) { return B * ((C + 15) / 16) >= 296; }
+template <class T>
 cudaError_t launch_gated(bool back, GatedParams& p, cudaStream_t st) {
-  return many(p.B, p.C, V) ? launch_gated_as<T, V, tokens(V, true)>(back, p, st)
-                           : launch_gated_as<T, V, tokens(V, false)>(back, p, st);
+  return many(p.B, p.C) ? launch_gated_as<T, tokens(true)>(back, p, st) : launch_gated_as<T, tokens(false)>(back, p, st);
 }
 
 GatedParams params_of(const gdn2_gated_desc* d) {
@@ -857,8 +808,7 @@ size_t access(const gdn2_gated_desc* d) { return d->dtype == GDN2_F32 || pairs(d
 extern "C" size_t gdn2_gated_marks_bytes(const gdn2_gated_desc* d) {
   using namespace gdn2;
   if (check_gated(d) != GDN2_OK) return 0;
-  const int V = pairs(d) ? 2 : 1;
-  const long long S = tokens(V, many(d->B, d->C, V));
+  const long long S = tokens(many(d->B, d->C));
   return (size_t)d->B * (size_t)((d->L + S - 1) / S) * (size_t)d->C * sizeof(float);
 }
 
@@ -887,11 +837,9 @@ extern "C" gdn2_status gdn2_gated_fwd(const gdn2_gated_desc* d, const void* x, c
     else gated_step_kernel<__nv_bfloat16, 1><<<grid, 128, 0, st>>>(p);
     e = cudaGetLastError();
   } else if (d->dtype == GDN2_F32) {
-    e = launch_gated<float, 1>(false, p, st);
-  } else if (pairs(d)) {
-    e = launch_gated<__nv_bfloat16, 2>(false, p, st);
+    e = launch_gated<float>(false, p, st);
   } else {
-    e = launch_gated<__nv_bfloat16, 1>(false, p, st);
+    e = launch_gated<__nv_bfloat16>(false, p, st);
   }
   return e == cudaSuccess ? GDN2_OK : GDN2_ERR_CUDA;
 }
@@ -911,8 +859,7 @@ extern "C" gdn2_status gdn2_gated_bwd(const gdn2_gated_desc* d, const void* x, c
   p.x = x; p.g = g; p.lengths = lengths; p.reset = reset; p.marks = const_cast<float*>(marks);
   p.dy = dh; p.dlast = dlast; p.dx = dx; p.dg = dg; p.dh0 = dh0; p.flags = flags;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = d->dtype == GDN2_F32 ? launch_gated<float, 1>(true, p, st)
-                        : pairs(d)           ? launch_gated<__nv_bfloat16, 2>(true, p, st)
-                                             : launch_gated<__nv_bfloat16, 1>(true, p, st);
+  const cudaError_t e = d->dtype == GDN2_F32 ? launch_gated<float>(true, p, st)
+                                             : launch_gated<__nv_bfloat16>(true, p, st);
   return e == cudaSuccess ? GDN2_OK : GDN2_ERR_CUDA;
 }

@@ -426,13 +426,6 @@ at::Tensor rows(const at::Tensor& t) {
   const bool as_is = (t.size(2) == 1 || t.stride(2) == 1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 4 == 0;
   return as_is ? t : t.clone(at::MemoryFormat::Contiguous);
 }
-// A copy whose rows are an odd number of values apart.
-at::Tensor odd_rows(const at::Tensor& t) {
-  const int64_t C = t.size(2) | 1, size[3] = {t.size(0), t.size(1), C};
-  at::Tensor r = fresh(size, t.scalar_type(), t.device()).narrow(2, 0, t.size(2));
-  r.copy_(t);
-  return r;
-}
 struct GatedFn : torch::autograd::Function<GatedFn> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& g, const std::optional<at::Tensor>& first,
                                const GatedMasks* masks, uint32_t* flags) {
@@ -471,22 +464,10 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
                     (!grads[0].defined() || (grads[0].sizes() == size && grads[0].scalar_type() == type)) &&
                     (!grads[1].defined() || (grads[1].size(0) == size[0] && grads[1].size(1) == size[2])),
                 "gated_scan: a saved tensor came back with another type or size");
-    at::Tensor x = rows(saved[0]), g = rows(saved[1]);
-    const at::Tensor marks = dense(saved[2]), lengths = saved[3].defined() ? dense(saved[3]) : saved[3],
+    const at::Tensor x = rows(saved[0]), g = rows(saved[1]), marks = dense(saved[2]), lengths = saved[3].defined() ? dense(saved[3]) : saved[3],
                      reset = saved[4].defined() ? dense(saved[4]) : saved[4];
     gdn2_gated_desc d = gated_desc(x, g);
-    // The marks lie as x's and g's rows were in the forward, one or two channels to a lane.
-    const auto other = [&] { return (int64_t)gdn2_gated_marks_bytes(&d) != marks.numel(); };
-    if (other()) {
-      x = x.clone(at::MemoryFormat::Contiguous);
-      g = g.clone(at::MemoryFormat::Contiguous);
-      d = gated_desc(x, g);
-    }
-    if (other()) {
-      x = odd_rows(x);
-      d = gated_desc(x, g);
-    }
-    TORCH_CHECK(!other(), "gated_scan: a saved tensor came back with another type or size");
+    TORCH_CHECK((int64_t)gdn2_gated_marks_bytes(&d) == marks.numel(), "gated_scan: a saved tensor came back with another type or size");
     at::Tensor dh = grads[0], dlast = grads[1], dx = fresh(x.sizes(), x.scalar_type(), dev), dg = fresh(x.sizes(), x.scalar_type(), dev), d0;
     if (dh.defined()) {
       dh = dh.contiguous();

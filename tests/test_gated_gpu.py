@@ -342,8 +342,8 @@ def test_other_stream_and_graph():
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("B,L,C", [(2, 100, 64), (3, 1, 64), (1, 37, 40), (40, 200, 256)])
 def test_saved_tensors_that_come_back_in_another_order(B, L, C, dtype):
-    """Saved on the host they come back contiguous, whatever the strides they had; other hooks may turn them.  The marks
-    of a forward whose rows had an odd number of values are not those of an even one."""
+    """Saved on the host they come back contiguous, whatever the strides they had; other hooks may turn them, rows of
+    an odd number of values to rows of an even one and back."""
     gen = torch.Generator(device="cuda").manual_seed(L)
     n = lambda *s: torch.randn(*s, generator=gen, device="cuda")
     x, g, dh, h0, dlast = n(B, L, C).to(dtype), -n(B, L, C).abs().to(dtype), n(B, L, C).to(dtype), n(B, C), n(B, C)
