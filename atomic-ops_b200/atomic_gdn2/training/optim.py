@@ -22,7 +22,9 @@ they are rounded.  Arithmetic is fp32, the norm's squares are summed in fp64 in 
 give the same bits.  bf16 parameters are rounded to nearest; there is no fp32 copy of them.
 
 state_dict() has torch.optim.AdamW's keys (and the scales); with state_bits=32 either loads the other's (not amsgrad's or
-maximize's).  It does not hold the norms' mean: norm_mean can be read and set.
+maximize's).  It does not hold the norms' mean: norm_mean can be read and set.  An 8-bit state whose parameter had another
+order in memory (transposed, channels last) is encoded anew when it is loaded: its scales go by the saved codes' strides, so
+keep these.
 A step may be captured into a CUDA graph after one that was not (the first one makes the moments); give lr as a
 tensor of one fp32 value on the device where it changes between replays.
 """
@@ -34,6 +36,57 @@ from torch.optim import optimizer as _base
 from .. import _lib
 
 BLOCK = 256
+
+
+def _order(t: torch.Tensor):
+    """The dimensions by their place in t's memory, the slowest first; None where its values do not fill it."""
+    dims = sorted((i for i in range(t.ndim) if t.shape[i] > 1 and t.numel()), key=lambda i: -t.stride(i))
+    step = 1
+    for i in reversed(dims):
+        if t.stride(i) != step:
+            return None
+        step *= t.shape[i]
+    return dims
+
+
+def _flat(t: torch.Tensor) -> torch.Tensor:
+    """t's values in the order of its memory, which they fill."""
+    return t.as_strided((t.numel(),), (1,))
+
+
+def _code_values(square: bool, dev) -> torch.Tensor:
+    """What the 256 codes stand for, of the first moment or of the second one's root."""
+    c = torch.arange(256, dtype=torch.int32)
+    if not square:
+        return c.to(torch.uint8).view(torch.float8_e4m3fn).float().to(dev)
+    return (torch.where(c < 16, c, 16 + c % 16) * torch.exp2(torch.clamp(c // 16 - 1, min=0).double()) * 2.0 ** -18).float().to(dev)
+
+
+def _recoded(codes: torch.Tensor, scale: torch.Tensor, p: torch.Tensor, square: bool):
+    """8-bit codes and scales of a tensor of p's shape whose memory has another order than p's, for p's order: decoded there
+    and encoded here, as a step does (the second moment's by its root)."""
+    values = _code_values(square, codes.device)
+    new = torch.empty_like(p, dtype=torch.uint8, device=codes.device, requires_grad=False)
+    n, blocks = codes.numel(), scale.numel()
+    if blocks == 1:                                          # the block's values are the same
+        return new.copy_(codes), scale
+    wide = torch.empty_like(codes, dtype=torch.float32)
+    _flat(wide).copy_(values[_flat(codes).int()] * scale.repeat_interleave(BLOCK)[:n])
+    x = torch.zeros(blocks * BLOCK, device=codes.device)
+    x[:n] = _flat(torch.empty_like(new, dtype=torch.float32).copy_(wide))
+    x = x.view(blocks, BLOCK)
+    top = 1.9375 if square else 448.0
+    scale = x.abs().amax(1) * (1.0 / top)
+    y = torch.clamp(x * torch.where(scale >= 2.0 ** -126, 1.0 / scale, 0.0)[:, None], -top, top)
+    if square:
+        ties = (values[:-1] + values[1:]) / 2                # exact; a tie goes to the even code
+        k = torch.searchsorted(ties, y)
+        k += (k % 2 == 1) & (y == ties[torch.clamp(k, max=254)])
+        k = torch.where((x > 0) & (k == 0), 1, k).to(torch.uint8)
+    else:
+        k = y.to(torch.float8_e4m3fn).view(torch.uint8)
+    _flat(new).copy_(k.view(-1)[:n])
+    return new, scale
 
 
 class AdamW(torch.optim.Optimizer):
@@ -204,8 +257,16 @@ class AdamW(torch.optim.Optimizer):
             have = "exp_avg_scale" in st
             if have != (self.state_bits == 8):
                 raise ValueError(f"AdamW: the saved moments have {8 if have else 32} bits, this optimizer {self.state_bits}")
-            new = self.state[p]
+            new, moved = self.state[p], {}
             for name, x in st.items():
+                if not isinstance(x, torch.Tensor):
+                    x = torch.tensor(float(x))
+                if have and name in ("exp_avg", "exp_avg_sq"):      # a scale belongs to 256 values of memory's order
+                    if _order(x) is None:
+                        raise ValueError(f"AdamW: the saved {name} does not fill its memory: in which order its scales go is not known")
+                    if _order(x) != _order(torch.empty_like(p)):
+                        moved[name], moved[name + "_scale"] = _recoded(x.detach(), st[name + "_scale"].detach().float(), p, name == "exp_avg_sq")
+            for name, x in {**st, **moved}.items():
                 if not isinstance(x, torch.Tensor):
                     x = torch.tensor(float(x))
                 if name in ("exp_avg", "exp_avg_sq"):

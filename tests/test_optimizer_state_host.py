@@ -1,0 +1,101 @@
+"""AdamW's saved states, loaded on the CPU: memory orders, torch's load hooks, refused loads."""
+import copy
+import pathlib
+import sys
+
+import pytest
+import torch
+
+sys.path.insert(0, str(pathlib.Path(__file__).resolve().parent))
+from atomic_gdn2.training import AdamW  # noqa: E402
+from training_ref import BLOCK, code_m, code_r, decode, encode, root  # noqa: E402
+
+
+def _order(t):
+    """t's values, flat, in the order of its memory."""
+    dims = sorted(range(t.ndim), key=lambda i: -t.stride(i))
+    return t.permute(dims).reshape(-1)
+
+
+def _as(flat, like):
+    """Flat values, in memory's order, as a tensor of `like`'s shape and strides."""
+    out = torch.empty_like(like, dtype=flat.dtype, requires_grad=False)
+    out.as_strided((flat.numel(),), (1,)).copy_(flat)
+    return out
+
+
+def _weights(shape, order, dtype=torch.float32):
+    """A parameter of `shape` whose memory has its dimensions in `order`, the slowest first."""
+    back = [order.index(i) for i in range(len(shape))]
+    return torch.nn.Parameter(torch.zeros([shape[i] for i in order], dtype=dtype).permute(back))
+
+
+def _stepped(p, bits, seed=0):
+    """An optimizer of p whose state stands for moments drawn here: magnitudes of neighbours in memory differ by orders."""
+    gen = torch.Generator().manual_seed(seed)
+    n = p.numel()
+    size = torch.exp(torch.linspace(-6.0, 6.0, n))
+    m, v = torch.randn(n, generator=gen) * size, (torch.randn(n, generator=gen) * size) ** 2
+    opt = AdamW([p], lr=1e-2, state_bits=bits)
+    st = opt.state[p]
+    st["step"] = torch.tensor(3.0)
+    if bits == 32:
+        st["exp_avg"], st["exp_avg_sq"] = _as(m, p), _as(v, p)
+    else:
+        (m8, ms), (v8, vs) = encode(m, 448.0, code_m), encode(root(v), 1.9375, code_r)
+        st["exp_avg"], st["exp_avg_scale"], st["exp_avg_sq"], st["exp_avg_sq_scale"] = _as(m8, p), ms, _as(v8, p), vs
+    return opt
+
+
+def _moments(opt, p):
+    """What the state stands for: m and v in the parameter's shape."""
+    st = opt.state[p]
+    if opt.state_bits == 32:
+        return st["exp_avg"], st["exp_avg_sq"]
+    m, v = decode(_order(st["exp_avg"]), st["exp_avg_scale"], _order(st["exp_avg_sq"]), st["exp_avg_sq_scale"])
+    return _as(m, p), _as(v, p)
+
+
+ORDERS = [((90, 100), (0, 1), (1, 0)), ((90, 100), (1, 0), (0, 1)), ((4, 6, 10, 7), (0, 1, 2, 3), (0, 2, 3, 1)),
+          ((4, 6, 10, 7), (3, 0, 2, 1), (0, 1, 2, 3)), ((1, 300), (0, 1), (1, 0)), ((3, 5), (0, 1), (1, 0)), ((4, 0, 3), (0, 1, 2), (2, 1, 0)), ((90, 100), (1, 0), (1, 0))]
+
+
+@pytest.mark.parametrize("shape,saved,new", ORDERS)
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_state_loads_into_another_order(shape, saved, new, bits, dtype):
+    """The moments of every value, whatever order the parameters' memory has.  8 bits: where the order is the same, or one
+    block holds all, bit by bit; else rounded once more into the new blocks: half a step of a code, 1/16 of m and 1/32 of
+    sqrt v, or half of the new scale's smallest step (2^-10 and 2^-19), and a root above zero stays above zero, at one such
+    step at most."""
+    p, q = _weights(shape, saved, dtype), _weights(shape, new, dtype)
+    opt, other = _stepped(p, bits), AdamW([q], state_bits=bits)
+    was = _moments(opt, p)
+    other.load_state_dict(copy.deepcopy(opt.state_dict()))
+    st = other.state[q]
+    assert float(st["step"]) == 3.0 and st["exp_avg"].stride() == q.stride() == st["exp_avg_sq"].stride()
+    now = _moments(other, q)
+    if bits == 32 or saved == new or 1 in shape or q.numel() <= BLOCK:
+        assert all(torch.equal(a, b) for a, b in zip(was, now))
+        return
+    far_m = _as(st["exp_avg_scale"].repeat_interleave(BLOCK)[:q.numel()], q)
+    far_r = _as(st["exp_avg_sq_scale"].repeat_interleave(BLOCK)[:q.numel()], q)
+    assert bool(((now[0] - was[0]).abs() <= (was[0].abs() / 16 + far_m * 2.0 ** -10) * 1.0001).all())
+    r, r2 = was[1].sqrt(), now[1].sqrt()
+    assert bool(((r2 - r).abs() <= (r / 32 + far_r * 2.0 ** -18) * 1.0001).all())
+    assert bool(((now[1] > 0) == (was[1] > 0)).all())
+    again = torch.empty_like(q, dtype=torch.float32, requires_grad=False).copy_(was[0])
+    m8, ms = encode(_order(again), 448.0, code_m)
+    assert torch.equal(_order(st["exp_avg"]), m8) and torch.equal(st["exp_avg_scale"], ms)
+
+
+def test_codes_whose_blocks_are_unknown_are_refused():
+    """Codes that do not fill their memory have no order that scales could belong to."""
+    p = _weights((20, 30), (0, 1))
+    opt, other = _stepped(p, 8), AdamW([_weights((20, 30), (0, 1))], state_bits=8)
+    saved = copy.deepcopy(opt.state_dict())
+    wide = torch.zeros(20, 60, dtype=torch.uint8)
+    wide[:, ::2] = saved["state"][0]["exp_avg"]
+    saved["state"][0]["exp_avg"] = wide[:, ::2]
+    with pytest.raises(ValueError, match="order"):
+        other.load_state_dict(saved)
