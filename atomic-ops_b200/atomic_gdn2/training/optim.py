@@ -244,10 +244,24 @@ class AdamW(torch.optim.Optimizer):
         return out
 
     def load_state_dict(self, state_dict):
-        """torch casts a state to its parameter's type: codes, scales and steps are put back as they were saved."""
-        for g in state_dict["param_groups"]:
-            self._check_group(g)
-        super().load_state_dict(state_dict)
+        """torch casts a state to its parameter's type: codes, scales and steps are put back as they were saved, or as the
+        hooks before a load returned them, before the hooks after it run."""
+        taken = {}
+
+        def check(_, d):
+            for g in d["param_groups"]:
+                self._check_group(g)
+            taken.update(d)
+
+        last = self.register_load_state_dict_pre_hook(check)
+        first = self.register_load_state_dict_post_hook(lambda _: self._put_back(taken), prepend=True)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            last.remove()
+            first.remove()
+
+    def _put_back(self, state_dict):
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         mine = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(saved, mine):

@@ -99,3 +99,35 @@ def test_codes_whose_blocks_are_unknown_are_refused():
     saved["state"][0]["exp_avg"] = wide[:, ::2]
     with pytest.raises(ValueError, match="order"):
         other.load_state_dict(saved)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_load_hooks(bits):
+    """What a pre hook returns is what is loaded, and what a post hook writes stays, as in torch's optimizers."""
+    p, q = _weights((20, 30), (0, 1)), _weights((20, 30), (0, 1))
+    opt, other = _stepped(p, bits), AdamW([q], state_bits=bits)
+    name = "exp_avg" if bits == 32 else "exp_avg_scale"
+
+    def before(o, d):
+        assert o is other
+        d = copy.deepcopy(d)
+        d["state"][0][name] *= 4.0
+        d["state"][0]["step"] += 2.0
+        return d
+
+    def after(o):
+        st = o.state[q]
+        assert torch.equal(_moments(o, q)[0], 4.0 * _moments(opt, p)[0])    # all of it is there by now
+        st["exp_avg_sq"].zero_()
+
+    handles = [other.register_load_state_dict_pre_hook(before), other.register_load_state_dict_post_hook(after)]
+    saved = opt.state_dict()
+    for _ in range(2):
+        other.load_state_dict(saved)
+        m, v = _moments(other, q)
+        assert torch.equal(m, 4.0 * _moments(opt, p)[0]) and not bool(v.any()) and float(other.state[q]["step"]) == 5.0
+    for h in handles:
+        h.remove()
+    other.load_state_dict(saved)
+    assert all(torch.equal(a, b) for a, b in zip(_moments(other, q), _moments(opt, p))) and float(other.state[q]["step"]) == 3.0
+    assert not other._optimizer_load_state_dict_pre_hooks and not other._optimizer_load_state_dict_post_hooks
