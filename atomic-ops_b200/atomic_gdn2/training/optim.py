@@ -245,12 +245,15 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """torch casts a state to its parameter's type: codes, scales and steps are put back as they were saved, or as the
-        hooks before a load returned them, before the hooks after it run."""
+        hooks before a load returned them, before the hooks after it run.  What cannot be taken is refused before anything
+        changes."""
         taken = {}
 
         def check(_, d):
             for g in d["param_groups"]:
                 self._check_group(g)
+            for p, st in self._saved(d):
+                self._check_state(p, st)
             taken.update(d)
 
         last = self.register_load_state_dict_pre_hook(check)
@@ -261,33 +264,48 @@ class AdamW(torch.optim.Optimizer):
             last.remove()
             first.remove()
 
-    def _put_back(self, state_dict):
-        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+    def _saved(self, state_dict):
+        """The parameters and their saved states that are not empty."""
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         mine = [p for g in self.param_groups for p in g["params"]]
-        for i, p in zip(saved, mine):
-            st = state_dict["state"].get(i)
-            if not st:
+        return [(p, state_dict["state"][i]) for i, p in zip(ids, mine) if state_dict["state"].get(i)]
+
+    def _check_state(self, p, st):
+        have = "exp_avg_scale" in st or "exp_avg_sq_scale" in st or getattr(st.get("exp_avg"), "dtype", None) == torch.uint8
+        if have != (self.state_bits == 8):
+            raise ValueError(f"AdamW: the saved moments have {8 if have else 32} bits, this optimizer {self.state_bits}")
+        step = st.get("step")
+        if step is None or (isinstance(step, torch.Tensor) and step.numel() != 1):
+            raise ValueError(f"AdamW: the saved state of a {tuple(p.shape)} parameter needs one step count")
+        for name in ("exp_avg", "exp_avg_sq"):
+            x = st.get(name)
+            if not isinstance(x, torch.Tensor) or x.shape != p.shape or not (x.dtype == torch.uint8 if have else x.is_floating_point()):
+                raise ValueError(f"AdamW: the saved {name} of a {tuple(p.shape)} parameter must be a tensor of its shape, "
+                                 + ("uint8" if have else "floating"))
+            if not have:
                 continue
-            have = "exp_avg_scale" in st
-            if have != (self.state_bits == 8):
-                raise ValueError(f"AdamW: the saved moments have {8 if have else 32} bits, this optimizer {self.state_bits}")
+            scale, n = st.get(name + "_scale"), -(-p.numel() // BLOCK)
+            if not isinstance(scale, torch.Tensor) or scale.numel() != n or not scale.is_floating_point():
+                raise ValueError(f"AdamW: the saved {name} of a {tuple(p.shape)} parameter needs {n} scales")
+            if _order(x) is None:
+                raise ValueError(f"AdamW: the saved {name} does not fill its memory: in which order its scales go is not known")
+
+    def _put_back(self, state_dict):
+        for p, st in self._saved(state_dict):
             new, moved = self.state[p], {}
-            for name, x in st.items():
-                if not isinstance(x, torch.Tensor):
-                    x = torch.tensor(float(x))
-                if have and name in ("exp_avg", "exp_avg_sq"):      # a scale belongs to 256 values of memory's order
-                    if _order(x) is None:
-                        raise ValueError(f"AdamW: the saved {name} does not fill its memory: in which order its scales go is not known")
-                    if _order(x) != _order(torch.empty_like(p)):
-                        moved[name], moved[name + "_scale"] = _recoded(x.detach(), st[name + "_scale"].detach().float(), p, name == "exp_avg_sq")
+            if self.state_bits == 8:                         # a scale belongs to 256 values of memory's order
+                for name in ("exp_avg", "exp_avg_sq"):
+                    if _order(st[name]) != _order(torch.empty_like(p)):
+                        moved[name], moved[name + "_scale"] = _recoded(st[name].detach(), st[name + "_scale"].detach().float().flatten(),
+                                                                       p, name == "exp_avg_sq")
             for name, x in {**st, **moved}.items():
-                if not isinstance(x, torch.Tensor):
-                    x = torch.tensor(float(x))
                 if name in ("exp_avg", "exp_avg_sq"):
-                    new[name] = torch.empty_like(p, dtype=torch.uint8 if have else torch.float32, requires_grad=False)
+                    new[name] = torch.empty_like(p, dtype=torch.uint8 if self.state_bits == 8 else torch.float32, requires_grad=False)
                     new[name].copy_(x)
-                else:
-                    new[name] = x.detach().to(p.device, torch.float32).clone()
+                elif isinstance(x, torch.Tensor):
+                    new[name] = x.detach().to(p.device, torch.float32).clone(memory_format=torch.contiguous_format)
+            if not isinstance(st["step"], torch.Tensor):
+                new["step"] = torch.tensor(float(st["step"]), device=p.device)
 
 
 _hooked_step = torch.optim.Optimizer.profile_hook_step(AdamW._step)

@@ -131,3 +131,74 @@ def test_load_hooks(bits):
     other.load_state_dict(saved)
     assert all(torch.equal(a, b) for a, b in zip(_moments(other, q), _moments(opt, p))) and float(other.state[q]["step"]) == 3.0
     assert not other._optimizer_load_state_dict_pre_hooks and not other._optimizer_load_state_dict_post_hooks
+
+
+def _everything(opt):
+    return copy.deepcopy([(k, v.stride(), v) if isinstance(v, torch.Tensor) else (k, v) for p in opt.param_groups[0]["params"]
+                          for k, v in sorted(opt.state[p].items())]), {k: v for k, v in opt.param_groups[0].items() if k != "params"}
+
+
+def _without(d, *names):
+    return {k: v for k, v in d.items() if k not in names}
+
+
+BAD = {
+    "width": lambda st, bits: None,                                  # the other width's state
+    "no scale": lambda st, bits: _without(st, "exp_avg_sq_scale"),
+    "no scales": lambda st, bits: _without(st, "exp_avg_scale", "exp_avg_sq_scale"),
+    "one scale too many": lambda st, bits: {**st, "exp_avg_scale": torch.ones(1)},
+    "no moment": lambda st, bits: _without(st, "exp_avg_sq"),
+    "no step": lambda st, bits: _without(st, "step"),
+    "two steps": lambda st, bits: {**st, "step": torch.ones(2)},
+    "shape": lambda st, bits: {**st, "exp_avg": st["exp_avg"].t()},
+    "one row": lambda st, bits: {**st, "exp_avg_sq": st["exp_avg_sq"][:1]},
+    "type": lambda st, bits: {**st, "exp_avg": st["exp_avg"].to(torch.int32)},
+    "not a tensor": lambda st, bits: {**st, "exp_avg": 0.0},
+    "another optimizer's": lambda st, bits: {"momentum_buffer": torch.zeros(20, 30)},
+}
+
+
+@pytest.mark.parametrize("bad", sorted(BAD))
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_refused_load_changes_nothing(bad, bits):
+    """Weights, moments, scales, step counts, rates: all as before, and the optimizer goes on from there."""
+    if bits == 32 and bad in ("no scale", "no scales"):
+        pytest.skip("32 bits have none")
+    good, p = _weights((20, 30), (0, 1)), _weights((20, 30), (0, 1))
+    q = torch.nn.Parameter(torch.ones(4))
+    opt = _stepped(p, bits, seed=5)
+    opt.add_param_group(dict(params=[q]))
+    opt.state[q] = {}
+    saved = copy.deepcopy(_stepped(good, 40 - bits if bad == "width" else bits, seed=6).state_dict())
+    saved["param_groups"][0]["lr"] = 0.5
+    saved["param_groups"].append({**saved["param_groups"][0], "params": [1]})
+    st = BAD[bad](saved["state"][0], bits)
+    if st is not None:
+        saved["state"][0] = st
+    was = _everything(opt)
+    with pytest.raises(ValueError, match="AdamW"):
+        opt.load_state_dict(saved)
+    now = _everything(opt)
+    assert now[1] == was[1] and opt.param_groups[1]["lr"] == 1e-2
+    assert [x[:2] for x in now[0]] == [x[:2] for x in was[0]] and all(torch.equal(a[2], b[2]) for a, b in zip(now[0], was[0]))
+    assert not opt._optimizer_load_state_dict_pre_hooks and not opt._optimizer_load_state_dict_post_hooks
+
+
+def test_what_still_loads():
+    """torch's own states, of either type; a parameter that was not stepped; a step that is a number."""
+    p = torch.nn.Parameter(torch.ones(3, 4, dtype=torch.bfloat16))
+    theirs = torch.optim.AdamW([p])
+    p.grad = torch.ones_like(p)
+    theirs.step()
+    p.grad = None
+    opt = AdamW([p, torch.nn.Parameter(torch.zeros(2))])
+    d = theirs.state_dict()
+    d["param_groups"][0]["params"].append(1)
+    opt.load_state_dict(d)
+    st = opt.state[p]
+    assert st["exp_avg"].dtype == torch.float32 and torch.equal(st["exp_avg"], theirs.state[p]["exp_avg"].float()) and float(st["step"]) == 1.0
+    d["state"][0]["step"], d["state"][1] = 7, {}
+    opt.load_state_dict(d)
+    assert float(opt.state[p]["step"]) == 7.0 and opt.state[p]["step"].dtype == torch.float32
+    with pytest.raises(ValueError):                                   # torch's own refusal
+        opt.load_state_dict(torch.optim.AdamW([p]).state_dict())
