@@ -76,7 +76,7 @@ def _forward(x, w, bias, residual, act, keep):
     z = torch.empty_like(y) if keep else None
     fl = pipeline._host_flags(dev)
     if x.shape[0]:
-        _, at, ws_bytes, _ = _desc(x, w, None if bias is None else bias.dtype, act,
+        d, at, ws_bytes, _ = _desc(x, w, None if bias is None else bias.dtype, act,
                                    0 if residual is None else residual.stride(0))
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
         with _guard(dev):
@@ -116,7 +116,7 @@ class _Linear(torch.autograd.Function):
             dy = dy.contiguous()
             if dy.data_ptr() % 16:
                 dy = dy.clone()
-            _, at, _, sizes = _desc(x, w, ctx.bias_dtype, ctx.act, 0)
+            d, at, _, sizes = _desc(x, w, ctx.bias_dtype, ctx.act, 0)
             ws_bytes = sizes[want_x + 2 * want_w + 4 * want_b]
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
             fl = pipeline._host_flags(dev)

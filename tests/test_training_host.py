@@ -172,3 +172,40 @@ def test_entry_points_reject_bad_arguments():
     t = (_lib.AdamwTensor * 1)()
     t[0].n = 5
     assert lib.gdn2_adamw_moments(ctypes.addressof(t), 1, 0) == inv and lib.gdn2_adamw_step(0, 0, 0, 0, at, at, 0) == inv
+
+
+def test_a_descriptor_lives_as_long_as_its_call(monkeypatch):
+    """Other threads may empty the descriptors' cache while a call, which has let go of the interpreter, reads its own."""
+    import gc
+    import importlib
+    import types
+    import weakref
+
+    L = importlib.import_module("atomic_gdn2.linear")      # the package's name is the function's
+    made, calls = [], []
+
+    class Desc(_lib.LinearDesc):
+        def __init__(self):
+            super().__init__()
+            made.append(weakref.ref(self))
+
+    def call(at, *_):
+        L._descs.clear()
+        gc.collect()
+        calls.append(any(r() is not None and ctypes.addressof(r()) == at for r in made))
+        return 0
+
+    lib = types.SimpleNamespace(gdn2_linear_fwd=call, gdn2_linear_bwd=call, gdn2_linear_fwd_workspace_bytes=lambda at: 0,
+                                gdn2_linear_bwd_workspace_bytes=lambda at, want: 0)
+    monkeypatch.setattr(L._lib, "load", lambda: lib)
+    monkeypatch.setattr(L._lib, "LinearDesc", Desc)
+    monkeypatch.setattr(L, "_guard", lambda dev: L.pipeline._NULL)
+    monkeypatch.setattr(L, "_raw_stream", lambda i: 0)
+    monkeypatch.setattr(L, "_check_flags", lambda *a: None)
+    monkeypatch.setattr(L.pipeline, "_host_flags", lambda dev: types.SimpleNamespace(ptr=0))
+    L._descs.clear()
+    x, w = torch.zeros(5, 3), torch.zeros(3, 4)
+    x, w, y, _ = L._forward(x, w, None, None, 0, False)
+    ctx = types.SimpleNamespace(saved_tensors=(x, w, None), needs_input_grad=(True, True, False, False, False), act=0, bias_dtype=None)
+    L._Linear.backward(ctx, torch.zeros(5, 4))
+    assert calls == [True, True]
