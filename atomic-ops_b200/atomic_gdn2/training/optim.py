@@ -11,9 +11,9 @@ One step is two launches, whatever the number of tensors: the gradients' global 
 
 `clip` bounds the gradients' global norm (as optax.clip_by_global_norm), `spike_factor` skips steps whose norm is
 not below that many times the running mean of the norms of the steps that were made (0.98 / 0.02; as the
-reference's training step, training/train.py:47-53).  With either of them a step whose norm, or whose `loss` where
-it is given, is not finite is skipped as well: weights, moments and step counts stay as they are.  Nothing of
-that comes to the host: grad_norm and step_made are device values.
+reference's training step, training/train.py:47-53).  With either of them a step whose norm is not finite, or the one
+value that its closure returns, is skipped as well, and a step whose `loss` is given and not finite always is: weights,
+moments and step counts stay as they are.  Nothing of that comes to the host: grad_norm and step_made are device values.
 
 Moments take 8 bytes a parameter, or 2 with state_bits=8: 256 values that follow one another in memory share a
 scale; the first moment is e4m3, the second is held as its root with four bits of exponent and four of mantissa
@@ -156,7 +156,7 @@ class AdamW(torch.optim.Optimizer):
         return st
 
     def step(self, closure=None, *, loss=None):
-        """One step; returns closure's loss, or None.  Parameters without a gradient are passed over."""
+        """One step; returns what closure returns, or None.  Parameters without a gradient are passed over."""
         if self._optimizer_step_pre_hooks or self._optimizer_step_post_hooks or _base._global_optimizer_pre_hooks \
                 or _base._global_optimizer_post_hooks:
             return _hooked_step(self, closure, loss=loss)
@@ -170,8 +170,9 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 result = closure()
-            if loss is None and isinstance(result, torch.Tensor):
-                loss = result
+            if loss is None and (self.clip or self.spike_factor) and isinstance(result, torch.Tensor) and result.numel() == 1 \
+                    and not result.is_complex():
+                loss = next((result.detach().to(p.device) for g in self.param_groups for p in g["params"]), None)
         self._check_guard()
         first = self.param_groups[0]
         for group in self.param_groups[1:]:

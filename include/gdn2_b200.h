@@ -369,8 +369,9 @@ size_t gdn2_linear_bwd_workspace_bytes(const gdn2_linear_desc* desc, int32_t wan
 /* One AdamW step over many tensors, with their gradients' global norm n, clipping and a guard:
  *   g' = g clip / max(n, clip),  m = b1 m + (1 - b1) g',  v = b2 v + (1 - b2) g'^2,
  *   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps).
- * With clip or spike > 0 the norm is taken, and a step whose loss or norm is not finite, or whose norm is not below
- * spike times the mean of earlier norms (ema > 0), changes nothing but the control's norm and ok. */
+ * With clip or spike > 0 the norm is taken.  A step whose loss is given and not finite, whose norm is taken and not finite,
+ * or whose norm is not below spike times the mean of earlier norms (ema > 0), changes nothing but the control's norm, ok and
+ * factor. */
 typedef struct gdn2_adamw_desc {
   int32_t state_bits;     /* 32: m and v are fp32.  8: codes with a scale per 256 values */
   int32_t reserved;

@@ -209,3 +209,21 @@ def test_a_descriptor_lives_as_long_as_its_call(monkeypatch):
     ctx = types.SimpleNamespace(saved_tensors=(x, w, None), needs_input_grad=(True, True, False, False, False), act=0, bias_dtype=None)
     L._Linear.backward(ctx, torch.zeros(5, 4))
     assert calls == [True, True]
+
+
+@pytest.mark.parametrize("clip", [None, 1.0])
+def test_a_closures_loss(clip, monkeypatch):
+    """What a closure returns guards the step only where there is a guard, and may be anything: torch's optimizers take no
+    notice of it.  A loss that is given always counts."""
+    import types
+    seen = []
+    monkeypatch.setattr(_lib, "binding", lambda: types.SimpleNamespace(adamw_step=lambda *a: seen.append(a[8]) or 0))
+    p = torch.nn.Parameter(torch.zeros(3))
+    p.grad = torch.zeros(3)
+    opt = AdamW([p], clip=clip)
+    losses = [torch.tensor(float("nan")), torch.zeros(2), torch.zeros(0), torch.zeros((), dtype=torch.complex64), 1.5, None, (torch.zeros(()), 2)]
+    for x in losses:
+        assert opt.step(lambda: x) is x
+    assert opt.step(lambda: losses[1], loss=losses[0]) is losses[1]
+    assert all(s is None for s in seen[1:-1]) and seen[-1] is losses[0]
+    assert seen[0] is None if clip is None else bool(torch.isnan(seen[0])) and seen[0].device == p.device
