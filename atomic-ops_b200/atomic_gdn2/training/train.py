@@ -57,19 +57,43 @@ def make_optimizer(model: torch.nn.Module, lr: float, wd: float = 0.1, state_bit
 
 class TrainStep:
     """One optimisation step (train.py:47-56).  `model` may be wrapped in DistributedDataParallel;
-    the gradient all-reduce then happens inside backward()."""
+    the gradient all-reduce then happens inside backward().  "default": what the optimizer of .optim was given, else a
+    clip of 1 and a spike_factor of 5; that optimizer holds both, and they may be changed there or here."""
 
-    def __init__(self, model, opt, lr=3e-4, warmup=200, total=2000, clip=1.0, spike_factor=5.0):
+    def __init__(self, model, opt, lr=3e-4, warmup=200, total=2000, clip="default", spike_factor="default"):
         self.model, self.opt = model, opt
-        self.lr, self.warmup, self.total, self.clip, self.spike = lr, warmup, total, clip, spike_factor
+        self.lr, self.warmup, self.total = lr, warmup, total
         dev = next(model.parameters()).device
         self.params = [p for p in model.parameters()]
         self.own = isinstance(opt, AdamW)     # clips and guards by itself
-        if self.own:
-            opt.clip, opt.spike_factor = clip, spike_factor
-        else:
+        given = (opt.clip, opt.spike_factor) if self.own else (None, None)
+        self.clip, self.spike = ((had or usual) if x == "default" else x
+                                 for x, had, usual in zip((clip, spike_factor), given, (1.0, 5.0)))
+        if not self.own:
             self.gn_ema = torch.zeros((), device=dev)
         self.i = 0
+
+    @property
+    def clip(self):
+        return self.opt.clip if self.own else self._clip
+
+    @clip.setter
+    def clip(self, value):
+        if self.own:
+            self.opt.clip = value
+        else:
+            self._clip = value
+
+    @property
+    def spike(self):
+        return self.opt.spike_factor if self.own else self._spike
+
+    @spike.setter
+    def spike(self, value):
+        if self.own:
+            self.opt.spike_factor = value
+        else:
+            self._spike = value
 
     @property
     def gn_ema(self) -> torch.Tensor:

@@ -227,3 +227,23 @@ def test_a_closures_loss(clip, monkeypatch):
     assert opt.step(lambda: losses[1], loss=losses[0]) is losses[1]
     assert all(s is None for s in seen[1:-1]) and seen[-1] is losses[0]
     assert seen[0] is None if clip is None else bool(torch.isnan(seen[0])) and seen[0].device == p.device
+
+
+def test_a_steps_clip_and_spike_are_the_optimizers():
+    """TrainStep's limits hold from when they are set, with either optimizer, and an optimizer keeps those that it was given."""
+    m = GDN2LM(make_cfg(), d_model=32, n_heads=1, d_head=16, n_layers=1, blr_fn=lambda *a: None)
+    opt = make_optimizer(m, 1e-3, state_bits=32)
+    step = TrainStep(m, opt)
+    assert (step.clip, step.spike, opt.clip, opt.spike_factor) == (1.0, 5.0, 1.0, 5.0)
+    step.clip, step.spike = 0.25, 7.0
+    assert (step.clip, step.spike, opt.clip, opt.spike_factor) == (0.25, 7.0, 0.25, 7.0)
+    opt.clip, opt.spike_factor = 0.5, None
+    assert (step.clip, step.spike) == (0.5, None)
+    opt = AdamW(m.parameters(), clip=0.3, spike_factor=9.0)
+    step = TrainStep(m, opt)
+    assert (step.clip, step.spike, opt.clip, opt.spike_factor) == (0.3, 9.0, 0.3, 9.0)
+    step = TrainStep(m, opt, clip=None, spike_factor=2.0)
+    assert (step.clip, step.spike, opt.clip, opt.spike_factor) == (None, 2.0, None, 2.0)
+    step = TrainStep(m, make_optimizer(m, 1e-3))
+    step.clip = 0.75
+    assert (step.clip, step.spike) == (0.75, 5.0)
