@@ -12,6 +12,9 @@ still, h and the gradients are zero, and what the inputs hold there does not mat
 after the other in a sequence: `reset` marks the tokens that start from nothing (h_t = x_t, whatever the
 state before it holds).
 
+Gates that multiply up to less than fp32's smallest number within a stretch of tokens count as that number, 2^-149:
+next to nothing, but of a state of 1e38 it is 1e-7.
+
 Device status as with make_blr_recurrent: a positive gate, an index or a length out of range are reported in
 mapped host memory, by default at a later call.
 """

@@ -33,7 +33,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr float kReset = -1.f;        // a segment's factor when a reset is in it: what entered is dropped
-constexpr float kTiny = 1.17549435e-38f;
+constexpr float kLeast = 1.40129846e-45f;  // the smallest number above zero
 constexpr int kMaxWarps = 8, kMaxCluster = 8;
 constexpr int kTileStages = 2;
 // Tokens of a thread's segment.  Odd: where the lanes of a warp hold several segments, their rows in a tile in shared
@@ -95,8 +95,8 @@ struct Lane<__nv_bfloat16, 2> {
 };
 
 // What a stretch of tokens does to the state that enters it: h -> A h + q, or q where A is kReset.  A is
-// held at the smallest normal number or above as long as no gate in the stretch is zero: an infinite state
-// stays infinite through any number of them, as it does token by token.
+// held above zero as long as no gate in the stretch is zero: an infinite state stays infinite through any number of
+// them, as it does token by token.  Of a finite one at most 2^-149 is left that should not be.
 struct Seg {
   float A, q;
 };
@@ -104,7 +104,7 @@ __device__ __forceinline__ float step(Seg s, float h) { return s.A < 0.f ? s.q :
 __device__ __forceinline__ Seg join(Seg a, Seg b) {  // a first
   Seg r;
   r.q = step(b, a.q);
-  r.A = (a.A < 0.f || b.A < 0.f) ? kReset : (a.A == 0.f || b.A == 0.f) ? 0.f : fmaxf(a.A * b.A, kTiny);
+  r.A = (a.A < 0.f || b.A < 0.f) ? kReset : (a.A == 0.f || b.A == 0.f) ? 0.f : fmaxf(a.A * b.A, kLeast);
   return r;
 }
 
@@ -221,7 +221,7 @@ __device__ __forceinline__ void tiles_done(const Shared& sm) {
 // join() and step() where no reset and no gate of zero is about (plain), or with them.
 template <bool PLAIN>
 __device__ __forceinline__ Seg join_as(Seg a, Seg b) {
-  if constexpr (PLAIN) return {fmaxf(a.A * b.A, kTiny), fmaf(b.A, a.q, b.q)};
+  if constexpr (PLAIN) return {fmaxf(a.A * b.A, kLeast), fmaf(b.A, a.q, b.q)};
   else return join(a, b);
 }
 template <bool PLAIN>
@@ -302,11 +302,11 @@ __device__ __forceinline__ float at_most_zero(float g) {  // a NaN stays one
 template <int S>
 __device__ __forceinline__ Seg segment(const float a[S], float A, float q, uint32_t resets, bool& plain) {
   if (resets) A = kReset;
-  else if (!(A >= kTiny)) {             // underflow, or a gate that is zero (or a NaN)
+  else if (!(A > 0.f)) {                // underflow, or a gate that is zero (or a NaN)
     bool zero = false;
 #pragma unroll
     for (int i = 0; i < S; ++i) zero |= a[i] == 0.f;
-    A = A != A ? A : zero ? 0.f : kTiny;
+    A = A != A ? A : zero ? 0.f : kLeast;
   }
   plain = plain && A > 0.f;
   return {A, q};
