@@ -276,6 +276,13 @@ __device__ __forceinline__ void tmem_st32(uint32_t tbase, uint32_t col, const fl
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
+// The current device's context for a driver call of this thread.  A thread that has made no runtime call yet that needs one
+// (autograd's, whose tensors all came from the allocator's cache) has none, and cuTensorMapEncodeTiled then fails.
+inline void bind_context() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaSetDevice(dev);
+}
+
 // Raise a kernel's dynamic shared-memory limit once per device (the attribute persists), so that
 // launches made while a stream is being captured into a CUDA graph issue no attribute calls.
 // `done` is a per-kernel bit mask of devices already set up.

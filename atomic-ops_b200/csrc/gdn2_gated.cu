@@ -725,9 +725,12 @@ bool tile_map(CUtensorMap* map, const void* p, bool bf16, const GatedParams& q, 
   const cuuint64_t dims[3] = {(cuuint64_t)q.C, (cuuint64_t)q.L, (cuuint64_t)q.B};
   const cuuint64_t strides[2] = {(cuuint64_t)sl, (cuuint64_t)sb};
   const cuuint32_t box[3] = {(cuuint32_t)width, (cuuint32_t)rows, 1}, unit[3] = {1, 1, 1};
-  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(p), dims, strides,
-            box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  auto encode = [&] {
+    return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(p), dims,
+              strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  return encode() || (bind_context(), encode());
 }
 
 template <class T, int S>

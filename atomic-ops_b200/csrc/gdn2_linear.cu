@@ -1031,9 +1031,12 @@ bool make_map(CUtensorMap* m, const Operand& o, int terms) {
   const cuuint64_t dims[3] = {(cuuint64_t)o.inner, (cuuint64_t)o.outer, (cuuint64_t)terms};
   const cuuint64_t strides[2] = {(cuuint64_t)o.ld * 2, (cuuint64_t)(terms > 1 ? o.term : o.ld * o.outer) * 2};
   const cuuint32_t box[3] = {64, o.mn ? 64u : 128u, (cuuint32_t)terms}, unit[3] = {1, 1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(o.p), dims, strides, box, unit,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  auto encode = [&] {
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(o.p), dims, strides, box, unit,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  return encode() || (bind_context(), encode());
 }
 
 constexpr int kSMs = 148;
