@@ -3,8 +3,9 @@
 The full-precision sibling of w4_linear, for training and for prompts: differentiable in x, W, b and the
 residual, W stored (din, dout) as in the layers.  x, W and the residual are all fp32 or all bf16; sums are fp32.
 
-* bf16: products are exact, y is rounded once.  The backward rounds dz = dy act'(z) to bf16 before its two
-  products, and z is kept in bf16 between the passes (half a step of each, 2^-8).
+* bf16: products are exact; the tensor cores add up to 1024 of them, truncating (some 4e-6 of their sum), and these
+  sums meet in rounded fp32 additions, whatever the length; y is rounded once.  The backward rounds dz = dy act'(z) to
+  bf16 before its two products (not in small products), and z is kept in bf16 between the passes (half a step of each, 2^-8).
 * fp32: the tensor cores multiply three bf16 terms of every value (24 bits), sums leave them every 64 values and
   go on in rounded fp32 additions: errors are those of a plain fp32 product.  Magnitudes below about 2^-110 lose
   their low bits.

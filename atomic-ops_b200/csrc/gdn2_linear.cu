@@ -11,7 +11,10 @@
 // is kept, which two fp16 terms with a scale (half the products) would not.
 // The tensor cores' additions truncate: fp32 sums leave them every 64 values of the summed dimension and go on in
 // registers with rounded additions (2048 x 512 x 2048: 1e-7 of the result off; every 128 values 6e-7, 256 1.5e-6, for
-// 4 to 20 % of the time; a plain fp32 product 4e-7).
+// 4 to 20 % of the time; a plain fp32 product 4e-7).  bf16 sums leave them every 1024 values, so
+// that what truncation takes, some 4e-6 of a sum, does not grow with its length: 2048 x K x 2048 random values are rounded to
+// another bf16 value than the exact sum in 7 places of 10000 at any K (7e-5 of the result's norm); without it in 47 at K = 8192
+// (2.2e-4) and in 1000 at K = 262144 (1.3e-3).  8192 x 4096 x 4096 takes 206 us for 199, with 2048 values 203 us (1e-4).
 // An infinite or huge fp32 value makes infinities of opposite signs in its terms: a result that is NaN is summed
 // again by itself from the fp32 operands, and so is what the plain sum makes of them.
 //
@@ -194,6 +197,7 @@ struct Gemm {
   static constexpr int kStages = P == 1 ? 5 : 2;
   static constexpr int kTmem = 2 * kTileN;                          // two accumulators' columns
   static constexpr int kCols = P == 1 ? 32 : 16;                    // columns that a warp turns around at a time
+  static constexpr int kTurn = P == 1 ? 16 : 1;                     // blocks of the sum in an accumulator's turn
   static constexpr size_t kStaging = kEpiWarps * 32 * kCols * sizeof(float);
   static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + kStaging + 256;
 };
@@ -278,10 +282,61 @@ __device__ __forceinline__ Work work_of(const GemmParams& p, int i) {
   return w;
 }
 
-template <int CG, int P>
-__global__ void __launch_bounds__(kGemmThreads) linear_gemm_kernel(const __grid_constant__ CUtensorMap map_a,
-                                                                   const __grid_constant__ CUtensorMap map_b,
-                                                                   const __grid_constant__ GemmParams p) {
+// What an epilogue warp does with the accumulators' turns: `acc` is the one whose turn it is, `phase` the turn's parity.
+struct Turns {
+  uint64_t *full, *empty;
+  volatile int* dead;
+  uint32_t* flags;
+  uint32_t tmem, col0;                  // the warp's first column
+  __device__ __forceinline__ void wait(uint32_t acc, uint32_t phase) const {
+    bounded_wait(&full[acc], phase, dead, flags);
+    __syncwarp();
+    tc_fence_after();
+  }
+  template <int CG>
+  __device__ __forceinline__ void release(uint32_t& acc, uint32_t& phase) const {
+    tc_fence_before();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) {
+      if constexpr (CG == 2)
+        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_addr(&empty[acc])) : "memory");
+      else
+        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&empty[acc])) : "memory");
+    }
+    acc ^= 1u;
+    if (!acc) phase ^= 1u;
+  }
+  // A sum's turns added up, in the last one's accumulator: the epilogue needs the registers.
+  template <int CG, int P>
+  __device__ __forceinline__ void add(int blocks, uint32_t& acc, uint32_t& phase) const {
+    using G = Gemm<CG, P>;
+    constexpr int kQuarter = G::kTileN / 4;
+    float sum[kQuarter];
+#pragma unroll
+    for (int j = 0; j < kQuarter; ++j) sum[j] = 0.f;
+    for (int k = G::kTurn;; k += G::kTurn) {
+      wait(acc, phase);
+#pragma unroll
+      for (int c = 0; c < kQuarter; c += 16) {
+        float v[16];
+        tmem_ld16(tmem + acc * G::kTileN, col0 + c, v);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sum[c + j] += v[j];
+      }
+      if (k >= blocks) break;
+      release<CG>(acc, phase);
+    }
+#pragma unroll
+    for (int c = 0; c < kQuarter; c += 16) tmem_st16(tmem + acc * G::kTileN, col0 + c, sum + c);
+  }
+};
+
+// LONG: sums of several turns.  A kernel of its own, so that sums of one turn keep their registers: 8192 x 4096 x 4096 in one
+// turn 193 us, 195.5 where the code for several stood beside it.  (One CTA a SM: for two the compiler leaves it 56 registers.)
+template <int CG, int P, bool LONG>
+__global__ void __launch_bounds__(kGemmThreads, LONG && P == 1 ? 1 : 0)
+    linear_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                       const __grid_constant__ GemmParams p) {
   using G = Gemm<CG, P>;
   extern __shared__ uint8_t raw[];
   uint8_t* stages = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
@@ -383,7 +438,8 @@ __global__ void __launch_bounds__(kGemmThreads) linear_gemm_kernel(const __grid_
       for (int it = blockIdx.x / CG; it < items && fine; it += stride) {
         const Work w = work_of(p, it);
         for (int kb = w.kb0; kb < w.kb1 && fine; ++kb) {
-          const bool first = P == 3 || kb == w.kb0;      // of an accumulator's turn
+          const int turn = (kb - w.kb0) % G::kTurn;
+          const bool first = turn == 0;                  // of an accumulator's turn
           if (first && !(fine = bounded_wait(&acc_empty[acc], acc_phase ^ 1u, dead, p.flags))) break;
           if (!(fine = bounded_wait(&full[stage], phase, dead, p.flags))) break;
           tc_fence_after();
@@ -412,7 +468,7 @@ __global__ void __launch_bounds__(kGemmThreads) linear_gemm_kernel(const __grid_
             stage = 0;
             phase ^= 1u;
           }
-          if (P == 3 || kb == w.kb1 - 1) {
+          if (turn == G::kTurn - 1 || kb == w.kb1 - 1) {
             commit<CG>(&acc_full[acc]);
             acc ^= 1u;
             if (!acc) acc_phase ^= 1u;
@@ -426,19 +482,6 @@ __global__ void __launch_bounds__(kGemmThreads) linear_gemm_kernel(const __grid_
     const uint32_t col0 = (warp >> 2) * kQuarter;
     const int half = lane >> 4, in = lane & 15;
     uint32_t acc = 0, acc_phase = 0;
-    auto release = [&] {
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if constexpr (CG == 2)
-          asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_addr(&acc_empty[acc]))
-                       : "memory");
-        else
-          asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&acc_empty[acc])) : "memory");
-      }
-      acc ^= 1u;
-      if (!acc) acc_phase ^= 1u;
-    };
     for (int it = blockIdx.x / CG; it < items; it += stride) {
       const Work w = work_of(p, it);
       const long long row0 = (long long)w.tm * G::kTileM + rank * 128 + (warp & 3) * 32;
@@ -507,43 +550,23 @@ __global__ void __launch_bounds__(kGemmThreads) linear_gemm_kernel(const __grid_
         }
         __syncwarp();
       };
+      const Turns turns{acc_full, acc_empty, dead, p.flags, tmem, col0};
+      if constexpr (LONG) turns.template add<CG, P>(w.kb1 - w.kb0, acc, acc_phase);
+      else turns.wait(acc, acc_phase);
       if constexpr (P == 3) {
-        float sum[kQuarter];
-#pragma unroll
-        for (int j = 0; j < kQuarter; ++j) sum[j] = 0.f;
-        for (int kb = w.kb0;; ++kb) {
-          bounded_wait(&acc_full[acc], acc_phase, dead, p.flags);
-          __syncwarp();
-          tc_fence_after();
-#pragma unroll
-          for (int c = 0; c < kQuarter; c += 16) {
-            float v[16];
-            tmem_ld16(tmem + acc * G::kTileN, col0 + c, v);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) sum[c + j] += v[j];
-          }
-          if (kb + 1 >= w.kb1) break;
-          release();
-        }
-        // the sums go back to the accumulator that they came from last: the epilogue needs the registers
-#pragma unroll
-        for (int c = 0; c < kQuarter; c += 16) tmem_st16(tmem + acc * G::kTileN, col0 + c, sum + c);
 #pragma unroll 1
         for (int c = 0; c < kQuarter; c += 16) {
           float v[16];
           tmem_ld16(tmem + acc * G::kTileN, col0 + c, v);
-          if (c + 16 == kQuarter) release();
+          if (c + 16 == kQuarter) turns.template release<CG>(acc, acc_phase);
           put(v, c);
         }
       } else {
-        bounded_wait(&acc_full[acc], acc_phase, dead, p.flags);
-        __syncwarp();
-        tc_fence_after();
 #pragma unroll
         for (int c = 0; c < kQuarter; c += 32) {
           float v[32];
           tmem_ld32(tmem + acc * G::kTileN, col0 + c, v);
-          if (c + 32 == kQuarter) release();
+          if (c + 32 == kQuarter) turns.template release<CG>(acc, acc_phase);
           put(v, c);
         }
       }
@@ -1080,11 +1103,11 @@ size_t parts_of(const GemmPlan& g, long long rows, long long cols) {
   return g.splits > 1 ? round256((size_t)g.splits * rows * cols * sizeof(float)) : 0;
 }
 
-template <int CG, int P>
+template <int CG, int P, bool LONG>
 cudaError_t launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p, cudaStream_t st) {
   using G = Gemm<CG, P>;
   static unsigned long long done = 0;
-  cudaError_t e = smem_attr_once(linear_gemm_kernel<CG, P>, (int)G::kSmem, done);
+  cudaError_t e = smem_attr_once(linear_gemm_kernel<CG, P, LONG>, (int)G::kSmem, done);
   if (e != cudaSuccess) return e;
   const int items = p.tiles_m * p.tiles_n * p.splits, workers = kSMs / CG;
   cudaLaunchConfig_t cfg = {};
@@ -1100,7 +1123,7 @@ cudaError_t launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmPa
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, linear_gemm_kernel<CG, P>, a, b, p);
+  return cudaLaunchKernelEx(&cfg, linear_gemm_kernel<CG, P, LONG>, a, b, p);
 }
 
 // One product; `parts` has parts_of() bytes.
@@ -1118,8 +1141,11 @@ cudaError_t gemm(const Operand& a, const Operand& b, int terms, Epilogue ep, lon
   p.pairs = cols % 2 == 0 && even(ep.y, ep.ldy) && even(ep.z, ep.ldy) && even(ep.residual, ep.ldr);
   p.flags = flags;
   p.ep.parts = g.splits > 1 ? parts : nullptr;
-  cudaError_t e = g.cg == 2 ? (terms == 3 ? launch_gemm<2, 3>(ma, mb, p, st) : launch_gemm<2, 1>(ma, mb, p, st))
-                            : (terms == 3 ? launch_gemm<1, 3>(ma, mb, p, st) : launch_gemm<1, 1>(ma, mb, p, st));
+  const bool turns = g.per_split > Gemm<1, 1>::kTurn;
+  auto launch = terms == 3 ? (g.cg == 2 ? launch_gemm<2, 3, true> : launch_gemm<1, 3, true>)
+                : turns    ? (g.cg == 2 ? launch_gemm<2, 1, true> : launch_gemm<1, 1, true>)
+                           : (g.cg == 2 ? launch_gemm<2, 1, false> : launch_gemm<1, 1, false>);
+  cudaError_t e = launch(ma, mb, p, st);
   if (e != cudaSuccess || g.splits == 1) return e;
   const int col_blocks = (int)((cols + 31) / 32);
   const unsigned grid = (unsigned)(col_blocks * ((rows + 63) / 64));

@@ -1,0 +1,45 @@
+"""linear on the B200: long sums, the size of bf16 gradients' errors.  u = 2^-24."""
+import pathlib
+import sys
+
+import pytest
+import torch
+
+sys.path.insert(0, str(pathlib.Path(__file__).resolve().parent))
+from atomic_gdn2 import last_status, linear  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+@pytest.fixture(autouse=True)
+def _status():
+    yield
+    assert last_status() == 0
+
+
+def _product(a, b):
+    """a b in 64 bits."""
+    y = torch.zeros(a.shape[0], b.shape[1], dtype=torch.float64, device="cuda")
+    for k in range(0, a.shape[1], 16384):
+        y += a[:, k:k + 16384].double() @ b[k:k + 16384].double()
+    return y
+
+
+@pytest.mark.parametrize("what", ["forward", "dW"])
+def test_long_bf16_sums(what):
+    """262144 positive products, so that every error of the additions goes one way, in so many results that no sum is split:
+    1024 products meet in truncating additions of 16 (144 u of the sum, as in the tests beside this one), these sums in
+    at most 256 rounded additions (u each), and the result is rounded once: 400 u and half a step, 2^-8."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    make = lambda *s: (1.0 + torch.rand(*s, generator=gen, device="cuda")).bfloat16()
+    n, long = 2048, 1 << 18
+    if what == "forward":
+        x, w = make(n, long), make(long, n)
+        y, ref = linear(x, w), _product(x, w)
+    else:
+        x, dy, w = make(long, n), make(long, n), torch.zeros(n, n, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+        y = torch.autograd.grad(linear(x, w), w, dy)[0]
+        ref = _product(x.t(), dy)
+    off = ((y.double() - ref) / ref).abs().max()
+    assert float(off) <= 1.001 * (400 * U + 2.0 ** -8)
