@@ -5,7 +5,8 @@
 The elementwise sibling of make_blr_trainable and make_blr_recurrent in one operator: any L >= 0, long
 sequences by a scan over their segments, single tokens while a model answers, differentiable.  Gates are
 logarithms as there (domain I-1: g <= 0, -inf forgets everything); states are fp32, inputs and outputs fp32 or
-bf16, rounded once.
+bf16, rounded once.  x and g of two types, or of others, are copied to fp32; h and the gradients come back in the types of
+their inputs.
 
 Sequences of different lengths in one padded batch: `lengths`; past a sequence's length the state stands
 still, h and the gradients are zero, and what the inputs hold there does not matter.  Several documents one
@@ -94,6 +95,10 @@ def _forward(x, g, h0, lengths, reset, h_index, last, keep):
     return x, g, h, last, marks, fl
 
 
+def _as_input(h: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    return h.to(dtype) if dtype.is_floating_point else h
+
+
 class _Gated(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, g, h0, lengths, reset):
@@ -102,7 +107,7 @@ class _Gated(torch.autograd.Function):
         ctx.save_for_backward(x, g, marks, lengths, reset)
         ctx.set_materialize_grads(False)
         _check_flags(fl, "gdn2_gated_fwd")
-        return h, last
+        return _as_input(h, ctx.types[0]), last
 
     @staticmethod
     def backward(ctx, dh, dlast):
@@ -142,14 +147,15 @@ class _Gated(torch.autograd.Function):
 
 
 def gated_scan(x: torch.Tensor, g: torch.Tensor, h0=None, *, lengths=None, reset=None, h_index=None, h_out=None):
-    """x, g (B, L, C) on the GPU, fp32 or bf16 (mixed or other types are taken as fp32), rows of any strides.
+    """x, g (B, L, C) on the GPU, both fp32 or both bf16 (copied to fp32 where they are not), rows of any strides.
       h0       (B, C), or None for zeros; with h_index any number of rows: (n, C)
       lengths  (B) int32 or int64, tokens of each sequence, 0..L
       reset    (B, L) bool: tokens that drop the state before them
       h_index  (B) the row of h0 that each sequence starts from, negative for zeros (beam_select's rows)
       h_out    (B, C) fp32 contiguous, written and returned as `last` (an in-place change to autograd); it may
                be h0 itself where there is no h_index, and otherwise lies outside the inputs' memory
-    Returns h (B, L, C) of x's type and last (B, C) fp32, the state after each sequence's last token.
+    Returns h (B, L, C) of x's type (fp32 where x is of whole numbers) and last (B, C) fp32, the state after each
+    sequence's last token.
     Differentiable in x, g and h0, but not with h_index or h_out: those are for answering."""
     global _fast, _last
     if isinstance(x, torch.Tensor) and x.is_cuda and pipeline._check_mode != "sync":
@@ -209,4 +215,4 @@ def gated_scan(x: torch.Tensor, g: torch.Tensor, h0=None, *, lengths=None, reset
     if h_out is not None and not h_out.is_inference():         # autograd may have saved it
         torch.autograd.graph.increment_version(h_out)
     _check_flags(fl, "gdn2_gated_fwd")
-    return h, last
+    return _as_input(h, x.dtype), last

@@ -47,3 +47,43 @@ def test_a_large_state_decays_to_nothing(L, C, gate):
     near(last, l_r)
     near(got[0], want[0])
     near(got[2], want[2])
+
+
+HALF = {torch.float32: 0.0, torch.float64: 0.0, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+@pytest.mark.parametrize("L,C", [(1, 7), (130, 40), (1000, 33)])
+@pytest.mark.parametrize("tx,tg", [(a, b) for a in HALF for b in HALF])
+def test_types(tx, tg, L, C):
+    """Any two floating types: taken as they are where both are fp32 or both bf16, else as fp32, and h and the gradients come
+    back in their inputs' types, rounded once (half a step; fp64 inputs here are fp32's values).  fp32's own part of the
+    error as in the tests beside this one: 48 u of the norm, twice that for gradients."""
+    gen = torch.Generator().manual_seed(L)
+    x, h0, dy = (torch.randn(2, L, C, generator=gen).to(tx) for _ in range(3))
+    g, h0, dl = (-torch.rand(2, L, C, generator=gen) - 0.02).to(tg), h0[:, 0].float(), torch.randn(2, C, generator=gen)
+    ref = [t.double().requires_grad_(True) for t in (x, g, h0)]
+    h_r, l_r = gated_ref(*ref)
+    want = torch.autograd.grad((h_r, l_r), ref, (dy.double(), dl.double()))
+    dev = [t.cuda().requires_grad_(True) for t in (x, g, h0)]
+    h, last = gated_scan(*dev)
+    assert h.dtype == tx and last.dtype == torch.float32
+    got = torch.autograd.grad((h, last), dev, (dy.cuda(), dl.cuda()))
+    with torch.no_grad():
+        h2, l2 = gated_scan(*dev)
+    assert h2.dtype == tx and torch.equal(h, h2) and torch.equal(last, l2)
+
+    def near(a, b, tol):
+        assert float((a.detach().double().cpu() - b.detach()).norm()) <= tol * float(b.detach().norm())
+
+    near(h, h_r, 48 * U + HALF[tx])
+    near(last, l_r, 48 * U)
+    for a, b, t in zip(got, want, (x, g, h0)):
+        assert a.dtype == t.dtype
+        near(a, b, 96 * U + HALF[t.dtype])
+
+
+def test_whole_numbers():
+    """Whole numbers are taken as fp32, and h comes back as that."""
+    x, g = torch.tensor([[[2], [3], [4]]], device="cuda"), torch.zeros(1, 3, 1, device="cuda")
+    h, last = gated_scan(x, g)
+    assert h.dtype == torch.float32 and h.flatten().tolist() == [2.0, 5.0, 9.0] and float(last) == 9.0
