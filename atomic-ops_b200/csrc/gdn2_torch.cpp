@@ -289,9 +289,11 @@ variable_list once(variable_list grads, const char* what) {
 // What a backward gets of saved tensors is what their hooks gave back (one that keeps them on the host returns copies in an
 // order of its own): their strides are read there, and layouts that the kernels cannot read are copied.
 at::Tensor dense(const at::Tensor& t) { return t.is_contiguous() && on16(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
+// n rows of `width` elements that do not overlap and are not further apart than the products take.
+bool near_rows(int64_t n, int64_t width, int64_t ld) { return ld >= width && ld <= (1 << 28) && n * ld <= (int64_t{1} << 36); }
 at::Tensor matrix(const at::Tensor& t) {
   if (t.dim() != 2) return dense(t);
-  const bool rows = (t.size(1) == 1 || t.stride(1) == 1) && (t.size(0) == 1 || t.stride(0) >= t.size(1)) && on16(t);
+  const bool rows = (t.size(1) == 1 || t.stride(1) == 1) && (t.size(0) == 1 || near_rows(t.size(0), t.size(1), t.stride(0))) && on16(t);
   return rows ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
@@ -379,7 +381,7 @@ PyObject* linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   c.d.act = (int32_t)PyLong_AsLong(a[4]);
   c.d.x_stride = M > 1 && x->dim() == 2 ? x->stride(0) : K;
   c.d.w_stride = K > 1 ? w->stride(0) : N;
-  if (c.d.x_stride < K || c.d.w_stride < N) Py_RETURN_NONE;
+  if (!near_rows(M, K, c.d.x_stride) || !near_rows(K, N, c.d.w_stride) || M * N > (int64_t{1} << 36)) Py_RETURN_NONE;
   c.out = x->sizes().vec();
   c.out[last] = N;
   std::optional<at::Tensor> bias, res;

@@ -43,3 +43,23 @@ def test_long_bf16_sums(what):
         ref = _product(x.t(), dy)
     off = ((y.double() - ref) / ref).abs().max()
     assert float(off) <= 1.001 * (400 * U + 2.0 ** -8)
+
+
+@pytest.mark.parametrize("M", [2, 40])
+def test_rows_far_apart(M):
+    """Rows 2^28 + 8 elements apart, of x and of W: copied, forward and backward."""
+    ld = (1 << 28) + 8
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    store = torch.empty((M - 1) * ld + 64 if M < 3 else ld + 64, dtype=torch.bfloat16, device="cuda")
+    x = store.as_strided((M, 64), (ld, 1)) if M < 3 else torch.empty(M, 64, dtype=torch.bfloat16, device="cuda")
+    w = torch.empty(64, 48, dtype=torch.bfloat16, device="cuda") if M < 3 else store.as_strided((2, 48), (ld, 1))
+    x = x if M < 3 else x[:, :2]
+    for t in (x, w):
+        t.copy_(torch.randint(-4, 5, t.shape, generator=gen, device="cuda"))      # sums that are exact
+    dy = torch.randint(-2, 3, (M, 48), generator=gen, device="cuda").bfloat16()
+    want = x.double() @ w.double(), dy.double() @ w.double().t(), x.double().t() @ dy.double()
+    assert torch.equal(linear(x, w).double(), want[0].bfloat16().double())
+    x.requires_grad_(True), w.requires_grad_(True)
+    y = linear(x, w)
+    for a, b in zip((y, *torch.autograd.grad(y, (x, w), dy)), want):
+        assert torch.equal(a.double(), b.bfloat16().double())

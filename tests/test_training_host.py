@@ -247,3 +247,16 @@ def test_a_steps_clip_and_spike_are_the_optimizers():
     step = TrainStep(m, make_optimizer(m, 1e-3))
     step.clip = 0.75
     assert (step.clip, step.spike) == (0.75, 5.0)
+
+
+def test_rows_too_far_apart_are_copied():
+    """linear reads rows of any strides; those beyond what the kernels take (2^28 elements, or 2^36 in all) are copied first."""
+    import importlib
+    rows = importlib.import_module("atomic_gdn2.linear")._rows
+    wide = lambda n, ld: torch.empty((n - 1) * ld + 64, device="meta", dtype=torch.bfloat16).as_strided((n, 64), (ld, 1))
+    for n, ld in ((2, 2 ** 28 + 8), (2, 2 ** 31), (2 ** 12 + 1, 2 ** 24)):
+        t = rows(wide(n, ld))
+        assert t.is_contiguous() and t.shape == (n, 64)
+    for n, ld in ((2, 2 ** 28), (2 ** 12, 2 ** 24), (1, 2 ** 40), (3, 64)):
+        t = wide(n, ld)
+        assert rows(t) is t
