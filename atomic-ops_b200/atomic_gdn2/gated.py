@@ -34,7 +34,7 @@ _fast, _last = None, (None, None)
 
 def _readable(t: torch.Tensor) -> torch.Tensor:
     """t, or a copy of it that the kernels can read: unit stride along C, bf16 pairs on 4 bytes."""
-    if (t.shape[2] != 1 and t.stride(2) != 1) or (t.dtype == torch.bfloat16 and t.data_ptr() % 4):
+    if (t.shape[2] != 1 and t.stride(2) != 1) or (t.dtype == torch.bfloat16 and t.data_ptr() % 4) or t.is_neg():
         return t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -81,7 +81,7 @@ def _forward(x, g, h0, lengths, reset, h_index, last, keep):
         x, g = x.float(), g.float()
     x, g = _readable(x), _readable(g)
     if h0 is not None:
-        h0 = h0.to(torch.float32).contiguous()
+        h0 = h0.to(torch.float32).resolve_neg().contiguous()
     d, at, mark_bytes = _desc(x, g, 0 if h0 is None else h0.shape[0])
     h = torch.empty(x.shape, dtype=x.dtype, device=dev)
     if last is None:
@@ -123,14 +123,14 @@ class _Gated(torch.autograd.Function):
                 raise RuntimeError("gated_scan: a saved tensor came back with another type or size")
         tx, tg, th = ctx.types
         if dlast is not None:
-            dlast = dlast.to(torch.float32).contiguous()
+            dlast = dlast.to(torch.float32).resolve_neg().contiguous()
         if L == 0:
             d0 = None
             if th is not None:
                 d0 = (torch.zeros(B, C, device=dev) if dlast is None else dlast).to(th)
             empty = [torch.empty(B, L, C, dtype=t, device=dev) for t in (tx, tg)]
             return *pipeline._once("gated_scan", (*empty, d0)), None, None
-        dh = torch.zeros(x.shape, dtype=x.dtype, device=dev) if dh is None else dh.to(x.dtype).contiguous()
+        dh = torch.zeros(x.shape, dtype=x.dtype, device=dev) if dh is None else dh.to(x.dtype).resolve_neg().contiguous()
         if dh.data_ptr() % 4:
             dh = dh.clone()
         dx, dg = torch.empty_like(dh), torch.empty_like(dh)
@@ -204,7 +204,8 @@ def gated_scan(x: torch.Tensor, g: torch.Tensor, h0=None, *, lengths=None, reset
         return _Gated.apply(x, g, h0, lengths, reset)
     pipeline._refuse_gradients("gated_scan", (x, g, h0, h_out))
     if h_out is not None:
-        if h_out.shape != (B, C) or h_out.dtype != torch.float32 or not h_out.is_contiguous() or h_out.device != dev:
+        if h_out.shape != (B, C) or h_out.dtype != torch.float32 or not h_out.is_contiguous() or h_out.device != dev \
+                or h_out.is_neg():
             raise ValueError(f"gated_scan: h_out must be a contiguous fp32 tensor of shape {(B, C)} on {dev}")
         if h0 is not None and h0.dtype == torch.float32 and _overlap(h0, h_out) and \
                 (h_index is not None or h0.data_ptr() != h_out.data_ptr() or not h0.is_contiguous()):

@@ -32,7 +32,8 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     """A matrix, or a copy of it, whose rows the kernels can read: unit stride, not overlapping, 16-byte aligned, less than
     2^28 elements apart and 2^36 in all."""
     n, ld = t.shape[0], t.stride(0)
-    if (t.shape[1] > 1 and t.stride(1) != 1) or (n > 1 and not (t.shape[1] <= ld <= 1 << 28 and n * ld <= 1 << 36)) or t.data_ptr() % 16:
+    if (t.shape[1] > 1 and t.stride(1) != 1) or (n > 1 and not (t.shape[1] <= ld <= 1 << 28 and n * ld <= 1 << 36)) or t.data_ptr() % 16 \
+            or t.is_neg():
         return t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -71,10 +72,12 @@ def _forward(x, w, bias, residual, act, keep):
     """x (M, K), w (K, N), bias (N), residual (M, N) -> x and w as they were read, y, z (None unless `keep`)."""
     dev = x.device
     x, w = _rows(x), _rows(w)
-    if bias is not None and not bias.is_contiguous():
-        bias = bias.contiguous()
-    if residual is not None and residual.shape[1] > 1 and residual.stride(1) != 1:
-        residual = residual.contiguous()
+    if bias is not None:
+        bias = bias.resolve_neg().contiguous()
+    if residual is not None:
+        residual = residual.resolve_neg()
+        if residual.shape[1] > 1 and residual.stride(1) != 1:
+            residual = residual.contiguous()
     y = torch.empty((x.shape[0], w.shape[1]), dtype=x.dtype, device=dev)
     z = torch.empty_like(y) if keep else None
     fl = pipeline._host_flags(dev)
@@ -104,7 +107,7 @@ class _Linear(torch.autograd.Function):
         x, w, z = ctx.saved_tensors                   # or what their hooks made of them
         x, w = _rows(x), _rows(w)
         if z is not None:
-            z = z.contiguous()
+            z = z.resolve_neg().contiguous()
         M, K, N, dev = x.shape[0], x.shape[1], w.shape[1], x.device
         want_x, want_w, want_b, want_r, _ = ctx.needs_input_grad
         dr = dy if want_r else None
@@ -116,7 +119,7 @@ class _Linear(torch.autograd.Function):
         dw = new((K, N), dtype=w.dtype, device=dev) if want_w else None
         db = new((N,), dtype=ctx.bias_dtype, device=dev) if want_b else None
         if M and (want_x or want_w or want_b):
-            dy = dy.contiguous()
+            dy = dy.resolve_neg().contiguous()
             if dy.data_ptr() % 16:
                 dy = dy.clone()
             d, at, _, sizes = _desc(x, w, ctx.bias_dtype, ctx.act, 0)

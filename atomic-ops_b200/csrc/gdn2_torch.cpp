@@ -264,7 +264,7 @@ using torch::autograd::variable_list;
 const at::Tensor* input(PyObject* o, bool& grad) {
   if (!THPVariable_CheckExact(o)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(o);
-  if (!t.is_cuda() || t.layout() != at::kStrided || t._fw_grad(0).defined()) return nullptr;
+  if (!t.is_cuda() || t.layout() != at::kStrided || t.is_neg() || t._fw_grad(0).defined()) return nullptr;
   grad = grad || (t.requires_grad() && c10::GradMode::is_enabled());
   return &t;
 }
@@ -288,12 +288,15 @@ variable_list once(variable_list grads, const char* what) {
 
 // What a backward gets of saved tensors is what their hooks gave back (one that keeps them on the host returns copies in an
 // order of its own): their strides are read there, and layouts that the kernels cannot read are copied.
-at::Tensor dense(const at::Tensor& t) { return t.is_contiguous() && on16(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
+// A view whose values are its memory's negated (the imaginary part of a conjugate is one) is copied too.
+at::Tensor dense(const at::Tensor& t) {
+  return t.is_contiguous() && on16(t) && !t.is_neg() ? t : t.clone(at::MemoryFormat::Contiguous);
+}
 // n rows of `width` elements that do not overlap and are not further apart than the products take.
 bool near_rows(int64_t n, int64_t width, int64_t ld) { return ld >= width && ld <= (1 << 28) && n * ld <= (int64_t{1} << 36); }
 at::Tensor matrix(const at::Tensor& t) {
   if (t.dim() != 2) return dense(t);
-  const bool rows = (t.size(1) == 1 || t.stride(1) == 1) && (t.size(0) == 1 || near_rows(t.size(0), t.size(1), t.stride(0))) && on16(t);
+  const bool rows = (t.size(1) == 1 || t.stride(1) == 1) && (t.size(0) == 1 || near_rows(t.size(0), t.size(1), t.stride(0))) && on16(t) && !t.is_neg();
   return rows ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
@@ -339,8 +342,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
     const at::Tensor x = matrix(saved[0]), w = matrix(saved[1]), z = d.act ? dense(saved[2]) : at::Tensor();
     d.x_stride = x.dim() == 2 && d.M > 1 ? x.stride(0) : d.K;
     d.w_stride = d.K > 1 ? w.stride(0) : d.N;
-    at::Tensor dy = grads[0].contiguous(), dx, dw, db;
-    if (!on16(dy)) dy = dy.clone();
+    at::Tensor dy = dense(grads[0]), dx, dw, db;
     if (ctx->needs_input_grad(0)) dx = fresh(x.sizes(), x.scalar_type(), dev);
     if (ctx->needs_input_grad(1)) dw = fresh(w.sizes(), w.scalar_type(), dev);
     const int64_t n[1] = {d.N};
@@ -425,7 +427,7 @@ struct GatedMasks {
 };
 // Unit stride along C, on 4 bytes.
 at::Tensor rows(const at::Tensor& t) {
-  const bool as_is = (t.size(2) == 1 || t.stride(2) == 1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 4 == 0;
+  const bool as_is = (t.size(2) == 1 || t.stride(2) == 1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 4 == 0 && !t.is_neg();
   return as_is ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 struct GatedFn : torch::autograd::Function<GatedFn> {
@@ -472,12 +474,12 @@ struct GatedFn : torch::autograd::Function<GatedFn> {
     TORCH_CHECK((int64_t)gdn2_gated_marks_bytes(&d) == marks.numel(), "gated_scan: a saved tensor came back with another type or size");
     at::Tensor dh = grads[0], dlast = grads[1], dx = fresh(x.sizes(), x.scalar_type(), dev), dg = fresh(x.sizes(), x.scalar_type(), dev), d0;
     if (dh.defined()) {
-      dh = dh.contiguous();
+      dh = dh.resolve_neg().contiguous();
       if (reinterpret_cast<uintptr_t>(dh.data_ptr()) % 4) dh = dh.clone();
     } else {
       dh = at::zeros_like(dx);
     }
-    if (dlast.defined()) dlast = dlast.contiguous();
+    if (dlast.defined()) dlast = dlast.resolve_neg().contiguous();
     const int64_t state[2] = {d.B, d.C};
     if (ctx->saved_data["h0"].toBool() && ctx->needs_input_grad(2)) d0 = fresh(state, at::kFloat, dev);
     const gdn2_status s = gdn2_gated_bwd(&d, x.data_ptr(), g.data_ptr(), static_cast<const int32_t*>(ptr(lengths)),
@@ -654,11 +656,11 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
       TORCH_CHECK(q.is_cuda(), "AdamW: the parameters must be on a CUDA device (the step runs only on the B200 kernels)");
       TORCH_CHECK_VALUE(q.device() == dev, "AdamW: parameters on ", q.device(), " and on ", dev, ": one optimizer steps one device's");
       TORCH_CHECK_VALUE(type == at::kFloat || type == at::kBFloat16, "AdamW: parameters must be float32 or bfloat16, not ", type);
-      TORCH_CHECK_VALUE(q.layout() == at::kStrided && q.is_non_overlapping_and_dense(),
+      TORCH_CHECK_VALUE(q.layout() == at::kStrided && q.is_non_overlapping_and_dense() && !q.is_neg(),
                         "AdamW: a parameter's values must fill their memory, each at one place");
       TORCH_CHECK_VALUE(g.layout() == at::kStrided && g.device() == dev && g.sizes() == q.sizes() && !g.is_complex(),
                         "AdamW: a gradient must be dense, of its parameter's shape and device");
-      if (g.scalar_type() != type || (g.strides() != q.strides() && !(g.is_contiguous() && q.is_contiguous()))) {
+      if (g.scalar_type() != type || g.is_neg() || (g.strides() != q.strides() && !(g.is_contiguous() && q.is_contiguous()))) {
         const c10::cuda::CUDAGuard guard(dev);
         const at::NoGradGuard no_grad;
         at::Tensor c = at::empty_like(q);
