@@ -237,8 +237,8 @@ __device__ __forceinline__ void moments(Two g, Two& m, Two& v, const Steps& s) {
   m = add(mul(s.b1, m), mul(s.g1, g));
   v = add(mul(s.b2, v), mul(s.g2, mul(g, g)));
 }
-// Their step from m and the roots of v.  The quotient is within 3 ulp: that is 2^-22 of a step, which is itself some
-// 2^-6 of p or less.
+// Their step from m and the roots of v.  The approximate root and reciprocal and the products leave the step within some 4 ulp
+// of itself, 2^-21: two roundings more than an exact division would, whatever the size of p.
 __device__ __forceinline__ Two stepped(Two p, Two m, Two r, const Steps& s) {
   float a, b;
   apart(fma(r, s.root, s.eps), a, b);

@@ -72,8 +72,9 @@ struct GemmParams {
 
 // ---- activation ---------------------------------------------------------------------------------
 constexpr float kGeluC = 0.7978845608028654f, kGeluA = 0.044715f;
-// 0.5 z (1 + tanh u) = z / (1 + exp(-2 u)),  u = C (z + A z^3); the approximate exponential and reciprocal leave
-// about 2^-22 of the gate
+// 0.5 z (1 + tanh u) = z / (1 + exp(-2 u)),  u = C (z + A z^3).  The approximate exponential and reciprocal leave about
+// 2^-22 of the gate, and so does the rounding of the exponent above z = -1; below, it leaves 2^-20.3 at -3, 2^-18.6 at -5 and
+// 2^-16.2 at -10, of gates that are 2^-10, 2^-24 and 2^-126 by then.  GELU itself is within 2^-25 and 2^-22 of its value.
 __device__ __forceinline__ float gelu_gate(float z) {
   constexpr float kA = -2.f * kGeluC * 1.4426950408889634f, kB = kA * kGeluA;
   float e, r;
