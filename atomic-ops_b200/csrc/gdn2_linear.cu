@@ -85,7 +85,8 @@ __device__ __forceinline__ float gelu_gate(float z) {
 __device__ __forceinline__ float gelu(float z) { return z * gelu_gate(z); }
 __device__ __forceinline__ float gelu_slope(float z) {
   const float s = gelu_gate(z);
-  return s + z * s * (1.f - s) * (2.f * kGeluC) * (1.f + 3.f * kGeluA * z * z);
+  // s is 0 or 1 long before z^2 overflows, and the second term nothing
+  return s + z * s * (1.f - s) * (2.f * kGeluC) * (1.f + 3.f * kGeluA * fminf(z * z, 1e38f));
 }
 
 __device__ __forceinline__ float load_f(const void* p, long long i, int bf16) {

@@ -63,3 +63,22 @@ def test_rows_far_apart(M):
     y = linear(x, w)
     for a, b in zip((y, *torch.autograd.grad(y, (x, w), dy)), want):
         assert torch.equal(a.double(), b.bfloat16().double())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M,K,N", [(3, 8, 40), (256, 1024, 512), (2048, 128, 1024)])
+def test_gelu_of_huge_values(M, K, N, dtype):
+    """Where z is so large that its square overflows GELU's slope is 1, or 0 to the left: finite gradients of finite inputs.
+    One value of x and of W in each sum and powers of two, so that y and the gradients are exact."""
+    x, w = torch.zeros(M, K, device="cuda", dtype=dtype), torch.zeros(K, N, device="cuda", dtype=dtype)
+    x[:, 0] = 2.0 ** (50.0 + torch.arange(M, device="cuda") % 8)
+    w[0] = 2.0 ** (30.0 + torch.arange(N, device="cuda") % 8) * (1 - 2.0 * (torch.arange(N, device="cuda") % 3 == 0))
+    dy = torch.zeros(M, N, device="cuda", dtype=dtype)
+    dy[:, N // 2:N // 2 + 3] = 1.0
+    x.requires_grad_(True), w.requires_grad_(True)
+    y = linear(x, w, act="gelu")
+    z = x.detach().double() @ w.detach().double()
+    assert torch.equal(y.double(), torch.clamp(z, min=0.0))
+    dz = dy.double() * (z > 0)
+    for a, b in zip(torch.autograd.grad(y, (x, w), dy), (dz @ w.detach().double().t(), x.detach().double().t() @ dz)):
+        assert torch.equal(a.double(), b.to(dtype).double())
