@@ -14,7 +14,9 @@
 // 4 to 20 % of the time; a plain fp32 product 4e-7).  bf16 sums leave them every 1024 values, so
 // that what truncation takes, some 4e-6 of a sum, does not grow with its length: 2048 x K x 2048 random values are rounded to
 // another bf16 value than the exact sum in 7 places of 10000 at any K (7e-5 of the result's norm); without it in 47 at K = 8192
-// (2.2e-4) and in 1000 at K = 262144 (1.3e-3).  8192 x 4096 x 4096 takes 206 us for 199, with 2048 values 203 us (1e-4).
+// (2.2e-4) and in 1000 at K = 262144 (1.3e-3).  8192 x 4096 x 4096 takes 202 us for 198, with a residual 229 for 211: an
+// epilogue that reads is still at work when the next turn is there to be taken out.  Every 2048 values 200 and 224 us (1e-4),
+// every 4096 198 and 212 (1.5e-4 at any K above).
 // An infinite or huge fp32 value makes infinities of opposite signs in its terms: a result that is NaN is summed
 // again by itself from the fp32 operands, and so is what the plain sum makes of them.
 //
