@@ -82,3 +82,38 @@ def test_gelu_of_huge_values(M, K, N, dtype):
     dz = dy.double() * (z > 0)
     for a, b in zip(torch.autograd.grad(y, (x, w), dy), (dz @ w.detach().double().t(), x.detach().double().t() @ dz)):
         assert torch.equal(a.double(), b.to(dtype).double())
+
+
+def test_bf16_gradients_through_gelu():
+    """A value's rounding to bf16 is off by up to 2^-8 / m, m its mantissa: r = 2^-8 / sqrt(3) sqrt(mean of 1 / m^2), 0.425 2^-8,
+    in the root of the mean square where mantissas are spread evenly over the logarithm.  A gradient has dz's rounding
+    (r: its errors are independent), z's (|gelu''(z) z| <= 0.29 where gelu' has a mean square of 0.4: below r / 2) and its
+    own (r): 1.5 r of its norm, 5 % for the spread.  The same of y, which is rounded once: r."""
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    M, K, N, r = 2048, 512, 2048, 0.425 * 2.0 ** -8
+    x = torch.randn(M, K, generator=gen, device="cuda").bfloat16().requires_grad_(True)
+    w = (torch.randn(K, N, generator=gen, device="cuda") / K ** 0.5).bfloat16().requires_grad_(True)
+    dy = torch.randn(M, N, generator=gen, device="cuda").bfloat16()
+    y = linear(x, w, act="gelu")
+    ref = [t.detach().double().requires_grad_(True) for t in (x, w)]
+    y_r = torch.nn.functional.gelu(ref[0] @ ref[1], approximate="tanh")
+    off = lambda a, b: float((a.double() - b).norm() / b.norm())
+    assert off(y.detach(), y_r.detach()) <= 1.05 * r
+    for a, b in zip(torch.autograd.grad(y, (x, w), dy), torch.autograd.grad(y_r, ref, dy.double())):
+        assert off(a, b) <= 1.05 * 1.5 * r
+
+
+@pytest.mark.parametrize("M,K,N", [(300, 1025, 200), (300, 2048, 201), (1000, 3000, 1000), (2048, 1088, 2560), (2500, 4160, 2049),
+                                   (130, 65536, 260), (257, 70001, 129), (2048, 1024, 2048)])
+def test_bf16_sums_of_several_turns(M, K, N):
+    """Whole numbers whose sums are exact in fp32, so that results are the exact ones, rounded once: sums of one and several
+    turns, the last of them short, split and whole, in single CTAs and pairs, cut tiles, rows on odd places."""
+    gen = torch.Generator(device="cuda").manual_seed(K)
+    whole = lambda *s: torch.randint(-4, 5, s, generator=gen, device="cuda").bfloat16()
+    x, w, b, r, dy = whole(M, K), whole(K, N), whole(N), whole(M, N), whole(M, N)
+    leaves = [t.requires_grad_(True) for t in (x, w, b, r)]
+    y = linear(x, w, b, residual=r)
+    want = [_product(x.detach(), w.detach()) + b.detach().double() + r.detach().double(), _product(dy, w.detach().t()),
+            _product(x.detach().t(), dy), dy.double().sum(0), dy.double()]
+    for a, e in zip((y, *torch.autograd.grad(y, leaves, dy)), want):
+        assert torch.equal(a.detach(), e.bfloat16())
