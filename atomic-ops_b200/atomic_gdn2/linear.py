@@ -13,6 +13,10 @@ residual, W stored (din, dout) as in the layers.  x, W and the residual are all 
 
 Up to 16 rows of fp32 x (4 of bf16) are multiplied without the tensor cores, W read once per eight rows.  Infinities
 and NaN come out as the plain sums would have them.
+
+Workspace, for the time of a call: fp32 6 bytes a value of x and W, in the backward of x, W and dz; bf16 2 bytes a value of
+dz behind an activation and of operands whose rows are not on 16 bytes; up to 16 times 4 bytes a result where few results
+have long sums.
 """
 from __future__ import annotations
 

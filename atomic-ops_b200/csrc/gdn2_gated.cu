@@ -17,7 +17,7 @@
 // for bf16, half a step of h in dg.
 //
 // Measured (forward + backward kernels): 8 x 2048 x 768 fp32 31 + 46 us, 403 MB at 5.2 TB/s; 1 x 131072 x 256
-// fp32 101 + 141 us, 34 dependent rounds of 3 and 4 us; 5 x 3001 x 1001 bf16 (ragged) 46 + 75 us, rows that start
+// fp32 101 + 141 us, 34 dependent rounds of 3 and 4 us; 5 x 3001 x 1001 bf16 (ragged) 48 + 80 us, rows that start
 // on odd places are read two bytes at a time and the longest sequence's rounds follow one another; 16 x 3001 x 1000 bf16
 // 130 + 184 us, 769 MB at 2.4 TB/s: issue slots, a value takes as many instructions as in fp32.
 #include <cooperative_groups.h>
@@ -752,8 +752,8 @@ cudaError_t launch_gated_as(bool back, GatedParams& p, cudaStream_t st) {
   const int places = warps * groups(), TT = places * S;
   // The same with lengths, whatever part of the tiles may be empty: over 156 shapes (2 to 24 sequences of 1500 to 8192 tokens,
   // 256 to 1536 channels, both types) a doubling beyond this takes 1 to 37 % longer in all but a few, full sequences and
-  // such of any length alike (up to 700 CTAs: 8 % longer on average; 5 x 3001 x 1001 bf16 of any lengths 104 -> 85 us, but
-  // 4 x 4096 x 512 fp32 57 -> 66 and 8 x 2048 x 256 35 -> 45).
+  // such of any length alike (up to 700 CTAs: 8 % longer on average; 5 x 3001 x 1001 bf16 104 -> 85 us with some lengths, 112
+  // -> 126 with others, 4 x 4096 x 512 fp32 57 -> 66, 8 x 2048 x 256 35 -> 45).
   while (clusters < kMaxCluster && (long long)p.B * cols() * clusters * 2 <= 296 && clusters * places < segs) clusters *= 2;
   p.cols = cols();
   p.clusters = clusters;

@@ -25,8 +25,8 @@
 // memory, sixteen warps empty the other one through the epilogue.  Few tiles with a long sum are split along it,
 // and a second launch adds the parts in a fixed order.
 //
-// Measured.  bf16, 8192 x 4096 x 4096: 192 to 205 us a product (1.35 to 1.43 PFLOP/s; the products alone, without
-// copies, 163, the copies alone 122: what is left is their overlap under the power limit).  fp32, 16384 x 512 x 2048:
+// Measured.  bf16, 8192 x 4096 x 4096: 202 to 206 us a product, 218 with 8192 values to a sum (1.26 to 1.36 PFLOP/s; the
+// products alone, without copies, 163, the copies alone 122: what is left is their overlap under the power limit).  fp32, 16384 x 512 x 2048:
 // 151 to 162 us (1.3 PFLOP/s of bf16 products); the forward's epilogue writes y and z, 268 MB, and is a fifth of it:
 // the warps that empty the accumulators every 64 values are the ones that write.
 #include <cooperative_groups.h>
