@@ -36,8 +36,8 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     """A matrix, or a copy of it, whose rows the kernels can read: unit stride, not overlapping, 16-byte aligned, less than
     2^28 elements apart and 2^36 in all."""
     n, ld = t.shape[0], t.stride(0)
-    if (t.shape[1] > 1 and t.stride(1) != 1) or (n > 1 and not (t.shape[1] <= ld <= 1 << 28 and n * ld <= 1 << 36)) or t.data_ptr() % 16 \
-            or t.is_neg():
+    if (t.shape[1] > 1 and t.stride(1) != 1) or (n > 1 and not (t.shape[1] <= ld <= 1 << 28 and n * ld <= 1 << 36)) \
+            or t.data_ptr() % 16 or t.is_neg():
         return t.clone(memory_format=torch.contiguous_format)
     return t
 

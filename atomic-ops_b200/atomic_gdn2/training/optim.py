@@ -62,31 +62,39 @@ def _code_values(square: bool, dev) -> torch.Tensor:
     return (torch.where(c < 16, c, 16 + c % 16) * torch.exp2(torch.clamp(c // 16 - 1, min=0).double()) * 2.0 ** -18).float().to(dev)
 
 
+def _encoded(x: torch.Tensor, values: torch.Tensor, square: bool):
+    """Codes and scales of blocks (n, 256) of fp32 values, the first moment's or the second one's roots, as a step makes them."""
+    top = 1.9375 if square else 448.0
+    scale = x.abs().amax(1) * (1.0 / top)
+    y = torch.clamp(x * torch.where(scale >= 2.0 ** -126, 1.0 / scale, 0.0)[:, None], -top, top)
+    if not square:
+        return y.to(torch.float8_e4m3fn).view(torch.uint8), scale
+    ties = (values[:-1] + values[1:]) / 2                    # exact; a tie goes to the even code
+    k = torch.searchsorted(ties, y, out_int32=True)
+    k += (k % 2 == 1) & (y == ties[torch.clamp(k, max=254)])
+    return torch.where((x > 0) & (k == 0), 1, k).to(torch.uint8), scale
+
+
 def _recoded(codes: torch.Tensor, scale: torch.Tensor, p: torch.Tensor, square: bool):
     """8-bit codes and scales of a tensor of p's shape whose memory has another order than p's, for p's order: decoded there
-    and encoded here, as a step does (the second moment's by its root)."""
+    and encoded here, a part at a time."""
     values = _code_values(square, codes.device)
     new = torch.empty_like(p, dtype=torch.uint8, device=codes.device, requires_grad=False)
     n, blocks = codes.numel(), scale.numel()
     if blocks == 1:                                          # the block's values are the same
         return new.copy_(codes), scale
-    wide = torch.empty_like(codes, dtype=torch.float32)
-    _flat(wide).copy_(values[_flat(codes).int()] * scale.repeat_interleave(BLOCK)[:n])
-    x = torch.zeros(blocks * BLOCK, device=codes.device)
-    x[:n] = _flat(torch.empty_like(new, dtype=torch.float32).copy_(wide))
-    x = x.view(blocks, BLOCK)
-    top = 1.9375 if square else 448.0
-    scale = x.abs().amax(1) * (1.0 / top)
-    y = torch.clamp(x * torch.where(scale >= 2.0 ** -126, 1.0 / scale, 0.0)[:, None], -top, top)
-    if square:
-        ties = (values[:-1] + values[1:]) / 2                # exact; a tie goes to the even code
-        k = torch.searchsorted(ties, y)
-        k += (k % 2 == 1) & (y == ties[torch.clamp(k, max=254)])
-        k = torch.where((x > 0) & (k == 0), 1, k).to(torch.uint8)
-    else:
-        k = y.to(torch.float8_e4m3fn).view(torch.uint8)
-    _flat(new).copy_(k.view(-1)[:n])
-    return new, scale
+    wide, x = torch.empty_like(codes, dtype=torch.float32), torch.empty_like(new, dtype=torch.float32)
+    part, scales = BLOCK << 14, []
+    for a in range(0, n, part):
+        c = _flat(codes)[a:a + part]
+        _flat(wide)[a:a + part] = values[c.int()] * scale[a // BLOCK:(a + part) // BLOCK].repeat_interleave(BLOCK)[:c.numel()]
+    x.copy_(wide)
+    for a in range(0, n, part):
+        y = _flat(x)[a:a + part]
+        k, s = _encoded(torch.nn.functional.pad(y, (0, -y.numel() % BLOCK)).view(-1, BLOCK), values, square)
+        _flat(new)[a:a + part] = k.view(-1)[:y.numel()]
+        scales.append(s)
+    return new, torch.cat(scales)
 
 
 class AdamW(torch.optim.Optimizer):
@@ -289,7 +297,8 @@ class AdamW(torch.optim.Optimizer):
             if not isinstance(scale, torch.Tensor) or scale.numel() != n or not scale.is_floating_point():
                 raise ValueError(f"AdamW: the saved {name} of a {tuple(p.shape)} parameter needs {n} scales")
             if _order(x) is None:
-                raise ValueError(f"AdamW: the saved {name} does not fill its memory: in which order its scales go is not known")
+                raise ValueError(f"AdamW: the saved {name} does not fill its memory: in which order its scales go is not "
+                                 "known")
 
     def _put_back(self, state_dict):
         for p, st in self._saved(state_dict):
@@ -297,12 +306,12 @@ class AdamW(torch.optim.Optimizer):
             if self.state_bits == 8:                         # a scale belongs to 256 values of memory's order
                 for name in ("exp_avg", "exp_avg_sq"):
                     if _order(st[name]) != _order(torch.empty_like(p)):
-                        moved[name], moved[name + "_scale"] = _recoded(st[name].detach(), st[name + "_scale"].detach().float().flatten(),
-                                                                       p, name == "exp_avg_sq")
+                        scale = st[name + "_scale"].detach().float().flatten().to(st[name].device)
+                        moved[name], moved[name + "_scale"] = _recoded(st[name].detach(), scale, p, name == "exp_avg_sq")
             for name, x in {**st, **moved}.items():
                 if name in ("exp_avg", "exp_avg_sq"):
-                    new[name] = torch.empty_like(p, dtype=torch.uint8 if self.state_bits == 8 else torch.float32, requires_grad=False)
-                    new[name].copy_(x)
+                    kind = torch.uint8 if self.state_bits == 8 else torch.float32
+                    new[name] = torch.empty_like(p, dtype=kind, requires_grad=False).copy_(x)
                 elif isinstance(x, torch.Tensor):
                     new[name] = x.detach().to(p.device, torch.float32).clone(memory_format=torch.contiguous_format)
             if not isinstance(st["step"], torch.Tensor):

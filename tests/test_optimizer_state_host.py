@@ -202,3 +202,18 @@ def test_what_still_loads():
     assert float(opt.state[p]["step"]) == 7.0 and opt.state[p]["step"].dtype == torch.float32
     with pytest.raises(ValueError):                                   # torch's own refusal
         opt.load_state_dict(torch.optim.AdamW([p]).state_dict())
+
+
+def test_a_large_state_is_encoded_in_parts():
+    """More values than are encoded at a time, the last block and the last part short: as if all were encoded at once."""
+    p, q = _weights((2049, 2051), (0, 1)), _weights((2049, 2051), (1, 0))
+    opt, other = _stepped(p, 8), AdamW([q], state_bits=8)
+    m, v = _moments(opt, p)
+    other.load_state_dict(opt.state_dict())
+    st, new = other.state[q], lambda t: _order(torch.empty_like(q, dtype=torch.float32, requires_grad=False).copy_(t))
+    r = decode(torch.zeros(p.numel(), dtype=torch.uint8), opt.state[p]["exp_avg_scale"], _order(opt.state[p]["exp_avg_sq"]),
+               opt.state[p]["exp_avg_sq_scale"])[1]
+    assert torch.equal(_as(r, p), v)
+    for name, x, top, code in (("exp_avg", new(m), 448.0, code_m), ("exp_avg_sq", root(new(v)), 1.9375, code_r)):
+        codes, scale = encode(x, top, code)
+        assert torch.equal(_order(st[name]), codes) and torch.equal(st[name + "_scale"], scale), name
